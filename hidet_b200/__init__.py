@@ -8,6 +8,7 @@ nor the library.
 from . import ffi
 from . import quant
 from . import graph
+from . import serving
 from .cuda_graph import CudaGraph
 from .quant import (
     symmetric_quantize,
@@ -16,6 +17,15 @@ from .quant import (
     symmetric_quant_matmul,
     symmetric_quant_matmul_f16_i8,
     symmetric_quant_matmul_atomic_f16_i8,
+)
+from .serving import (
+    rotary_table,
+    rotary_embedding,
+    quantized_cache,
+    quantized_cache_append,
+    quantized_cache_read,
+    quantized_cache_attention,
+    token_log_probs,
 )
 
 __version__ = '0.1.0'

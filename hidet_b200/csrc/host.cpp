@@ -20,6 +20,8 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
+#include <type_traits>
 #include <unordered_map>
 #include <utility>
 
@@ -36,6 +38,12 @@ struct Library {
     decltype(&b200q_qlinear_f16_i8_fused) linear_fused = nullptr;
     decltype(&b200q_qlinear_f16_u4_workspace_bytes) w4_workspace_bytes = nullptr;
     decltype(&b200q_qlinear_f16_u4) w4 = nullptr;
+    decltype(&b200q_rotary_embedding) rotary = nullptr;
+    decltype(&b200q_quantized_cache_append) append = nullptr;
+    decltype(&b200q_quantized_cache_read) read = nullptr;
+    decltype(&b200q_quantized_cache_attention_workspace_bytes) attention_workspace_bytes = nullptr;
+    decltype(&b200q_quantized_cache_attention) attention = nullptr;
+    decltype(&b200q_token_log_probs) log_probs = nullptr;
 } lib;
 
 // Scratch buffers that the Python side owns and has told us about, by stream and device.
@@ -283,18 +291,229 @@ PyObject *w4(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
-// bind(quantize, dequantize, take, workspace_bytes, linear, linear_fused, w4_workspace_bytes, w4): addresses
+// Like plain_tensor for the heads of tokens, [tokens, heads, dim]: strides between tokens and heads are the kernels' to follow.
+inline const at::Tensor *heads_tensor(PyObject *o) {
+    if (!THPVariable_Check(o)) return nullptr;
+    const at::Tensor &t = THPVariable_Unpack(o);
+    return t.is_cuda() && t.layout() == at::kStrided && t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch() && !t.is_neg() && t.dim() == 3 &&
+                   t.stride(2) == 1 && t.numel() > 0
+               ? &t
+               : nullptr;
+}
+inline b200q_heads heads_of(const at::Tensor &t) { return {const_cast<void *>(t.const_data_ptr()), t.stride(0), t.stride(1)}; }
+inline int layout_code(PyObject *o) { return is_text(o, "half") ? B200Q_ROTARY_HALF : is_text(o, "interleaved") ? B200Q_ROTARY_INTERLEAVED : -1; }
+inline bool is_index(const at::Tensor *t) { return t && (t->scalar_type() == at::kLong || t->scalar_type() == at::kInt); }
+inline bool is_table(const at::Tensor *t, int64_t dim) { return t && t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(1) % 2 == 0 && t->size(1) >= 2 && t->size(1) <= dim; }
+// head_dim of a cache, or 0
+inline int64_t cache_dim(const at::Tensor *t) {
+    if (!t || t->scalar_type() != at::kByte || t->dim() != 4 || t->numel() == 0) return 0;
+    const int64_t d = (t->size(3) - 128) / 32;
+    return t->size(3) == 32 * d + 128 && (d == 64 || d == 96 || d == 128 || d == 192 || d == 256) ? d : 0;
+}
+// The new references of `first` and `second` as a pair, or what went wrong.
+inline PyObject *pair_of(PyObject *first, PyObject *second) {
+    PyObject *pair = first && second ? PyTuple_Pack(2, first, second) : nullptr;
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    return pair;
+}
+
+// rotary(q, k or None, positions, table, layout) -> (q', k')
+PyObject *rotary(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    PLAIN_OR_NONE(n_args == 5 && lib.rotary != nullptr && !watched());
+    const at::Tensor *q = heads_tensor(args[0]), *k = args[1] != Py_None ? heads_tensor(args[1]) : nullptr;
+    const at::Tensor *positions = plain_tensor(args[2]), *table = plain_tensor(args[3]);
+    PLAIN_OR_NONE(q && (k || args[1] == Py_None) && is_index(positions) && layout_code(args[4]) >= 0);
+    const int64_t tokens = q->size(0), heads = q->size(1), dim = q->size(2), kv_heads = k ? k->size(1) : 0;
+    const int type = float_code(q->scalar_type());
+    Where w;
+    PLAIN_OR_NONE(type >= 0 && is_table(table, dim) && positions->dim() == 1 && positions->size(0) == tokens && where_is(*q, w) && positions->get_device() == w.device &&
+                  table->get_device() == w.device);
+    PLAIN_OR_NONE(!k || (k->size(0) == tokens && k->size(2) == dim && k->scalar_type() == q->scalar_type() && k->get_device() == w.device));
+    at::Tensor q_out = empty(q->sizes(), q->scalar_type(), w.device), k_out;
+    if (k) k_out = empty(k->sizes(), q->scalar_type(), w.device);
+    const b200q_heads qs = heads_of(*q), qo = heads_of(q_out), ks = k ? heads_of(*k) : b200q_heads{}, ko = k ? heads_of(k_out) : b200q_heads{};
+    const void *at = positions->const_data_ptr();
+    const float *angles = static_cast<const float *>(table->const_data_ptr());
+    int status;
+    WITHOUT_GIL(status, lib.rotary(&qs, k ? &ks : nullptr, &qo, k ? &ko : nullptr, at, angles, tokens, heads, kv_heads, dim, table->size(1), table->size(0), layout_code(args[4]), type,
+                                   (int)positions->element_size(), w.stream));
+    PLAIN_OR_NONE(status == B200Q_OK);
+    PyObject *first = THPVariable_Wrap(std::move(q_out));
+    return pair_of(first, k ? THPVariable_Wrap(std::move(k_out)) : Py_NewRef(Py_None));
+    END_HANDLE_TH_ERRORS
+}
+
+// append(cache, k, v, slots, q or None, positions or None, table or None, layout) -> q', or True without q
+PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    PLAIN_OR_NONE(n_args == 8 && lib.append != nullptr && !watched());
+    const at::Tensor *cache = plain_tensor(args[0]), *k = heads_tensor(args[1]), *v = heads_tensor(args[2]), *slots = plain_tensor(args[3]);
+    const int64_t dim = cache_dim(cache);
+    PLAIN_OR_NONE(dim > 0 && k && v && is_index(slots) && layout_code(args[7]) >= 0);
+    const int64_t tokens = k->size(0), kv_heads = cache->size(1);
+    const int type = float_code(k->scalar_type());
+    Where w;
+    PLAIN_OR_NONE(type >= 0 && v->scalar_type() == k->scalar_type() && k->size(1) == kv_heads && k->size(2) == dim && v->sizes() == k->sizes() && slots->dim() == 1 &&
+                  slots->size(0) == tokens && where_is(*k, w) && v->get_device() == w.device && cache->get_device() == w.device && slots->get_device() == w.device);
+    const at::Tensor *q = nullptr, *positions = nullptr, *table = nullptr;
+    PLAIN_OR_NONE((args[5] == Py_None) == (args[6] == Py_None) && (args[4] == Py_None || args[5] != Py_None));
+    if (args[5] != Py_None) {
+        positions = plain_tensor(args[5]);
+        table = plain_tensor(args[6]);
+        PLAIN_OR_NONE(is_index(positions) && is_table(table, dim) && table->size(1) % 16 == 0 && positions->dim() == 1 && positions->size(0) == tokens &&
+                      positions->get_device() == w.device && table->get_device() == w.device);
+    }
+    at::Tensor q_out;
+    b200q_heads qs = {}, qo = {};
+    if (args[4] != Py_None) {
+        q = heads_tensor(args[4]);
+        PLAIN_OR_NONE(q && q->scalar_type() == k->scalar_type() && q->size(0) == tokens && q->size(2) == dim && q->get_device() == w.device);
+        q_out = empty(q->sizes(), q->scalar_type(), w.device);
+        qs = heads_of(*q);
+        qo = heads_of(q_out);
+    }
+    const b200q_heads ks = heads_of(*k), vs = heads_of(*v);
+    void *bytes = cache->data_ptr();
+    const void *where = slots->const_data_ptr(), *at = positions ? positions->const_data_ptr() : nullptr;
+    const float *angles = table ? static_cast<const float *>(table->const_data_ptr()) : nullptr;
+    int status;
+    WITHOUT_GIL(status, lib.append(bytes, cache->size(0), cache->size(2) * 16, &ks, &vs, q ? &qs : nullptr, q ? &qo : nullptr, where, at, angles, tokens, q ? q->size(1) : 0, kv_heads, dim,
+                                   table ? table->size(1) : 0, table ? table->size(0) : 0, layout_code(args[7]), type, (int)slots->element_size(),
+                                   positions ? (int)positions->element_size() : 0, w.stream));
+    PLAIN_OR_NONE(status == B200Q_OK);
+    if (!q) Py_RETURN_TRUE;
+    return THPVariable_Wrap(std::move(q_out));
+    END_HANDLE_TH_ERRORS
+}
+
+// read(cache, slots, dtype) -> (k, v)
+PyObject *read(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    PLAIN_OR_NONE(n_args == 3 && lib.read != nullptr && !watched() && THPDtype_Check(args[2]));
+    const at::Tensor *cache = plain_tensor(args[0]), *slots = plain_tensor(args[1]);
+    const at::ScalarType dtype = reinterpret_cast<THPDtype *>(args[2])->scalar_type;
+    const int64_t dim = cache_dim(cache);
+    Where w;
+    PLAIN_OR_NONE(dim > 0 && is_index(slots) && slots->numel() > 0 && float_code(dtype) >= 0 && where_is(*cache, w) && slots->get_device() == w.device);
+    at::DimVector shape(slots->sizes());
+    shape.push_back(cache->size(1));
+    shape.push_back(dim);
+    at::Tensor k = empty(shape, dtype, w.device), v = empty(shape, dtype, w.device);
+    const void *bytes = cache->const_data_ptr(), *where = slots->const_data_ptr();
+    void *kp = k.data_ptr(), *vp = v.data_ptr();
+    int status;
+    WITHOUT_GIL(status, lib.read(bytes, cache->size(0), cache->size(2) * 16, where, kp, vp, slots->numel(), cache->size(1), dim, float_code(dtype), (int)slots->element_size(), w.stream));
+    PLAIN_OR_NONE(status == B200Q_OK);
+    PyObject *first = THPVariable_Wrap(std::move(k));
+    return pair_of(first, THPVariable_Wrap(std::move(v)));
+    END_HANDLE_TH_ERRORS
+}
+
+// attention(q, cache, page_table, lengths, starts or None, mask or None, scale or None, return_lse) -> out or (out, lse)
+PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    PLAIN_OR_NONE(n_args == 8 && lib.attention != nullptr && !watched());
+    const at::Tensor *q = plain_tensor(args[0]), *cache = plain_tensor(args[1]), *pages = plain_tensor(args[2]), *lengths = plain_tensor(args[3]);
+    const int64_t dim = cache_dim(cache);
+    PLAIN_OR_NONE(q && dim > 0 && pages && lengths && (q->dim() == 3 || q->dim() == 4) && q->numel() > 0 && q->size(-1) == dim);
+    PLAIN_OR_NONE(q->scalar_type() == at::kHalf || q->scalar_type() == at::kBFloat16);
+    PLAIN_OR_NONE(lengths->scalar_type() == at::kInt && lengths->dim() == 1 && pages->scalar_type() == at::kInt && pages->dim() == 2);
+    const int64_t batch = lengths->size(0), heads = q->size(-2), kv_heads = cache->size(1), tokens = q->dim() == 3 ? q->size(0) : q->size(0) * q->size(1);
+    Where w;
+    PLAIN_OR_NONE(batch > 0 && pages->size(0) == batch && pages->size(1) > 0 && heads % kv_heads == 0 && where_is(*q, w) && cache->get_device() == w.device &&
+                  pages->get_device() == w.device && lengths->get_device() == w.device && (reinterpret_cast<uintptr_t>(q->const_data_ptr()) & 7u) == 0);
+    const at::Tensor *starts = nullptr, *mask = nullptr;
+    if (args[4] != Py_None) {
+        starts = plain_tensor(args[4]);
+        PLAIN_OR_NONE(starts && q->dim() == 3 && starts->scalar_type() == at::kInt && starts->dim() == 1 && starts->size(0) == batch + 1 && starts->get_device() == w.device);
+    } else {
+        PLAIN_OR_NONE(q->size(0) == batch);
+    }
+    if (args[5] != Py_None) {
+        mask = plain_tensor(args[5]);
+        PLAIN_OR_NONE(mask && (mask->scalar_type() == at::kBool || mask->scalar_type() == at::kByte) && mask->dim() == 2 && mask->size(0) == tokens && mask->get_device() == w.device &&
+                      (starts || mask->size(1) >= tokens / batch));
+    }
+    double scale = 1.0 / std::sqrt((double)dim);
+    if (args[6] != Py_None) {
+        PLAIN_OR_NONE(PyFloat_CheckExact(args[6]));
+        scale = PyFloat_AS_DOUBLE(args[6]);
+    }
+    PLAIN_OR_NONE(PyBool_Check(args[7]));
+    const bool with_lse = args[7] == Py_True;
+    void *ws;
+    size_t ws_bytes;
+    PLAIN_OR_NONE(find_scratch(w, lib.attention_workspace_bytes(dim), ws, ws_bytes));
+    at::Tensor out = empty(q->sizes(), q->scalar_type(), w.device), lse;
+    if (with_lse) lse = empty(q->sizes().slice(0, q->dim() - 1), at::kFloat, w.device);
+    const b200q_heads rows = {const_cast<void *>(q->const_data_ptr()), heads * dim, dim};
+    void *dst = out.data_ptr();
+    float *lse_dst = with_lse ? static_cast<float *>(lse.data_ptr()) : nullptr;
+    const void *bytes = cache->const_data_ptr(), *seen = mask ? mask->const_data_ptr() : nullptr;
+    const int32_t *table = static_cast<const int32_t *>(pages->const_data_ptr()), *n = static_cast<const int32_t *>(lengths->const_data_ptr());
+    const int32_t *first_rows = starts ? static_cast<const int32_t *>(starts->const_data_ptr()) : nullptr;
+    int status;
+    WITHOUT_GIL(status, lib.attention(&rows, dst, lse_dst, bytes, cache->size(0), cache->size(2) * 16, table, pages->size(1), pages->size(1), n, first_rows, seen, mask ? mask->size(1) : 0,
+                                      mask ? mask->size(1) : 0, batch, tokens, heads, kv_heads, dim, (float)scale, float_code(q->scalar_type()), ws, ws_bytes, w.stream));
+    PLAIN_OR_NONE(status == B200Q_OK);
+    PyObject *first = THPVariable_Wrap(std::move(out));
+    if (!with_lse) return first;
+    return pair_of(first, THPVariable_Wrap(std::move(lse)));
+    END_HANDLE_TH_ERRORS
+}
+
+// log_probs(logits, tokens, top) -> (log_probs, entropy, top_log_probs, top_indices)
+PyObject *log_probs(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    PLAIN_OR_NONE(n_args == 3 && lib.log_probs != nullptr && !watched() && PyLong_CheckExact(args[2]));
+    const at::Tensor *logits = plain_tensor(args[0]), *tokens = plain_tensor(args[1]);
+    PLAIN_OR_NONE(logits && is_index(tokens) && logits->dim() >= 1 && logits->numel() > 0 && tokens->numel() > 0);
+    const int64_t lead = logits->dim() - 1, vocab = logits->size(-1), top = PyLong_AsLongLong(args[2]);
+    PLAIN_OR_NONE(float_code(logits->scalar_type()) >= 0 && top >= 0 && top <= 32 && top <= vocab && (tokens->dim() == lead || tokens->dim() == lead + 1));
+    for (int64_t d = 0; d < lead; ++d) PLAIN_OR_NONE(tokens->size(d) == logits->size(d));
+    const int64_t rows = logits->numel() / vocab, given = tokens->dim() > lead ? tokens->size(-1) : 1;
+    Where w;
+    PLAIN_OR_NONE(where_is(*logits, w) && tokens->get_device() == w.device);
+    const at::IntArrayRef shape = logits->sizes().slice(0, lead);
+    at::DimVector top_shape(shape);
+    top_shape.push_back(top);
+    at::Tensor result[4] = {empty(tokens->sizes(), at::kFloat, w.device), empty(shape, at::kFloat, w.device), empty(top_shape, at::kFloat, w.device),
+                            empty(top_shape, at::kLong, w.device)};
+    float *lp = static_cast<float *>(result[0].data_ptr()), *entropy = static_cast<float *>(result[1].data_ptr()), *values = static_cast<float *>(result[2].data_ptr());
+    int64_t *indices = static_cast<int64_t *>(result[3].data_ptr());
+    const void *x = logits->const_data_ptr(), *which = tokens->const_data_ptr();
+    int status;
+    WITHOUT_GIL(status, lib.log_probs(x, vocab, which, lp, entropy, values, indices, rows, vocab, given, top, float_code(logits->scalar_type()), (int)tokens->element_size(), w.stream));
+    PLAIN_OR_NONE(status == B200Q_OK);
+    PyObject *all = PyTuple_New(4);
+    for (int i = 0; all && i < 4; ++i) {
+        PyObject *one = THPVariable_Wrap(std::move(result[i]));
+        if (!one) {
+            Py_CLEAR(all);
+            break;
+        }
+        PyTuple_SET_ITEM(all, i, one);
+    }
+    return all;
+    END_HANDLE_TH_ERRORS
+}
+
+// bind(an address for each member of Library, in their order)
 PyObject *bind(PyObject *, PyObject *args) {
-    unsigned long long p[8];
-    if (!PyArg_ParseTuple(args, "KKKKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7])) return nullptr;
-    lib.quantize = reinterpret_cast<decltype(lib.quantize)>(p[0]);
-    lib.dequantize = reinterpret_cast<decltype(lib.dequantize)>(p[1]);
-    lib.take = reinterpret_cast<decltype(lib.take)>(p[2]);
-    lib.workspace_bytes = reinterpret_cast<decltype(lib.workspace_bytes)>(p[3]);
-    lib.linear = reinterpret_cast<decltype(lib.linear)>(p[4]);
-    lib.linear_fused = reinterpret_cast<decltype(lib.linear_fused)>(p[5]);
-    lib.w4_workspace_bytes = reinterpret_cast<decltype(lib.w4_workspace_bytes)>(p[6]);
-    lib.w4 = reinterpret_cast<decltype(lib.w4)>(p[7]);
+    static_assert(sizeof(Library) % sizeof(void *) == 0, "");
+    constexpr Py_ssize_t N = sizeof(Library) / sizeof(void *);
+    if (PyTuple_GET_SIZE(args) != N) return PyErr_Format(PyExc_TypeError, "bind takes %zd addresses", N);
+    unsigned long long p[N];
+    for (Py_ssize_t i = 0; i < N; ++i) {
+        p[i] = PyLong_AsUnsignedLongLong(PyTuple_GET_ITEM(args, i));
+        if (PyErr_Occurred()) return nullptr;
+    }
+    int i = 0;
+    auto set = [&](auto &member) { member = reinterpret_cast<std::remove_reference_t<decltype(member)>>(p[i++]); };
+    set(lib.quantize), set(lib.dequantize), set(lib.take), set(lib.workspace_bytes), set(lib.linear), set(lib.linear_fused), set(lib.w4_workspace_bytes), set(lib.w4);
+    set(lib.rotary), set(lib.append), set(lib.read), set(lib.attention_workspace_bytes), set(lib.attention), set(lib.log_probs);
     Py_RETURN_NONE;
 }
 
@@ -322,6 +541,11 @@ PyMethodDef methods[] = {FAST(linear),
                          FAST(dequantize),
                          FAST(take),
                          FAST(w4),
+                         FAST(rotary),
+                         FAST(append),
+                         FAST(read),
+                         FAST(attention),
+                         FAST(log_probs),
                          {"bind", bind, METH_VARARGS, nullptr},
                          {"set_scratch", set_scratch, METH_VARARGS, nullptr},
                          {"clear_scratch", clear_scratch, METH_NOARGS, nullptr},

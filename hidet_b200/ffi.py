@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 from typing import Callable, Dict, List, Optional
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -39,12 +39,20 @@ F16, BF16, F32 = 0, 1, 2
 I8, I16 = 0, 1
 LAYOUT_KN, LAYOUT_NK = 0, 1
 ACT_NONE, ACT_SILU_MUL = 0, 1
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 
 
 class Epilogue(ctypes.Structure):
     """b200q_epilogue of include/hidet_b200q.h."""
 
     _fields_ = [('bias', c_void_p), ('residual', c_void_p), ('ldr', c_int64), ('activation', c_int)]
+
+
+class Heads(ctypes.Structure):
+    """b200q_heads of include/hidet_b200q.h."""
+
+    _fields_ = [('data', c_void_p), ('token_stride', c_int64), ('head_stride', c_int64)]
+
 
 _lib: Optional[ctypes.CDLL] = None
 _funcs: Dict[str, Callable] = {}
@@ -164,6 +172,21 @@ SIGNATURES = {
     'b200q_qlinear_static_scratch_bytes': ([], c_size_t, False),
     'b200q_qlinear_f16_i8_static': ([c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p], c_int, True),
     'b200q_qlinear_f16_i8_parts': ([c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p], c_int, True),
+    'b200q_rotary_embedding': ([POINTER(Heads)] * 4 + [c_void_p] * 2 + [c_int64] * 6 + [c_int] * 3 + [c_void_p], c_int, True),
+    'b200q_quantized_cache_append': (
+        [c_void_p, c_int64, c_int64] + [POINTER(Heads)] * 4 + [c_void_p] * 3 + [c_int64] * 6 + [c_int] * 4 + [c_void_p],
+        c_int,
+        True,
+    ),
+    'b200q_quantized_cache_read': ([c_void_p, c_int64, c_int64] + [c_void_p] * 3 + [c_int64] * 3 + [c_int] * 2 + [c_void_p], c_int, True),
+    'b200q_quantized_cache_attention_workspace_bytes': ([c_int64], c_size_t, False),
+    'b200q_quantized_cache_attention': (
+        [POINTER(Heads), c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]
+        + [c_int64] * 7 + [c_float, c_int, c_void_p, c_size_t, c_void_p],
+        c_int,
+        True,
+    ),
+    'b200q_token_log_probs': ([c_void_p, c_int64] + [c_void_p] * 5 + [c_int64] * 4 + [c_int] * 2 + [c_void_p], c_int, True),
 }
 
 

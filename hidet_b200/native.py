@@ -25,8 +25,10 @@ LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'lib')
 
 # what csrc/host.cpp calls, in the order of its bind()
 _BOUND = ('b200q_symmetric_quantize', 'b200q_symmetric_dequantize', 'b200q_embedding_dequantize', 'b200q_qlinear_workspace_bytes',
-          'b200q_qlinear_f16_i8', 'b200q_qlinear_f16_i8_fused', 'b200q_qlinear_f16_u4_workspace_bytes', 'b200q_qlinear_f16_u4')
-_FUNCTIONS = ('linear', 'quantize', 'dequantize', 'take', 'w4')
+          'b200q_qlinear_f16_i8', 'b200q_qlinear_f16_i8_fused', 'b200q_qlinear_f16_u4_workspace_bytes', 'b200q_qlinear_f16_u4',
+          'b200q_rotary_embedding', 'b200q_quantized_cache_append', 'b200q_quantized_cache_read', 'b200q_quantized_cache_attention_workspace_bytes',
+          'b200q_quantized_cache_attention', 'b200q_token_log_probs')
+_FUNCTIONS = ('linear', 'quantize', 'dequantize', 'take', 'w4', 'rotary', 'append', 'read', 'attention', 'log_probs')
 _module = None
 
 
@@ -82,4 +84,4 @@ def _stand_in(name):
     return first_call
 
 
-linear, quantize, dequantize, take, w4 = (_stand_in(name) for name in _FUNCTIONS)
+linear, quantize, dequantize, take, w4, rotary, append, read, attention, log_probs = (_stand_in(name) for name in _FUNCTIONS)

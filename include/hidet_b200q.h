@@ -27,8 +27,8 @@
  *     not want to rely on which it is takes the exception to hold for every M <= 64.  (It waits with its codes too at 17 to
  *     24 rows on weights of 6 Mi codes and more.)
  *     Kernels that do not themselves execute griddepcontrol.launch_dependents (b200q_symmetric_quantize, the packing
- *     kernels and every other kernel of this library but the quantized linears, memcpy / memset nodes, ordinary
- *     kernels) let dependents start only when they have finished, so producing a weight with
+ *     kernels and every other kernel of this library but the quantized linears and the operators around them (rotary, cache,
+ *     attention, log probabilities), memcpy / memset nodes, ordinary kernels) let dependents start only when they have finished, so producing a weight with
  *     b200q_symmetric_quantize and using it in the next call on the same stream is safe.  Not safe: writing the codes of
  *     an int8 weight from a kernel that triggers its dependents early when nothing but kernels of that kind lie between
  *     it and the quantized linear that reads them on the same stream (the quantized linears are themselves of that
@@ -289,6 +289,85 @@ B200Q_API size_t b200q_qlinear_static_scratch_bytes(void);
  */
 B200Q_API int b200q_qlinear_f16_i8_static(const void *a, const void *wq, const void *scale, void *c, int64_t M, int64_t N,
                                           int64_t K, int w_layout, void *stream);
+
+/*
+ * ---- the operators around the linears of a decoder ----
+ *
+ * Launched as programmatic dependents of the kernel in front; they read and write nothing before the dependency on it is honoured, and
+ * let the kernel behind them start early.  They write no weight codes, so a quantized linear may follow any of them.
+ * Indexes on the device (positions, slots, pages, lengths, tokens) are checked there: one outside its range is never followed, the entry
+ * point says what stands in the place of its result, and b200q_check_status reports it.
+ */
+
+/* heads of tokens: element (token, head, i) is data[token * token_stride + head * head_stride + i], strides in elements */
+typedef struct b200q_heads {
+    void *data;
+    int64_t token_stride, head_stride;
+} b200q_heads;
+/* which elements of a head are a pair: (i, i + rotary_dim / 2), or (2 i, 2 i + 1) */
+typedef enum b200q_rotary_layout { B200Q_ROTARY_HALF = 0, B200Q_ROTARY_INTERLEAVED = 1 } b200q_rotary_layout;
+
+/*
+ * Rotary positions.  The pairs (a, b) of the first rotary_dim elements of every head become (a cos - b sin, b cos + a sin), with
+ * cosine and sine i of the token's position at table[position * rotary_dim + i] and [.. + rotary_dim / 2 + i] (float); the other elements
+ * are copied.  In float, each product and sum rounded by itself, then one rounding to `type` (b200q_float_type).  q and k have `heads` and
+ * `kv_heads` heads (either may be 0 with a NULL).  q_out may be q, k_out may be k (same pointer and strides); otherwise they do not overlap.
+ * positions: int32 or int64 [tokens] (position_bytes 4 or 8).  A position outside the table gives zeros in the place of the rotated elements.
+ */
+B200Q_API int b200q_rotary_embedding(const b200q_heads *q, const b200q_heads *k, const b200q_heads *q_out, const b200q_heads *k_out,
+                                     const void *positions, const float *table, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                     int64_t head_dim, int64_t rotary_dim, int64_t table_rows, int layout, int type, int position_bytes,
+                                     void *stream);
+
+/*
+ * The quantized key/value cache: uint8 [pages][kv_heads][page_size / 16][32 head_dim + 128], page_size a multiple of 16, head_dim 64, 96,
+ * 128, 192 or 256.  A record of 16 positions of one head holds 16 rows of K codes and 16 rows of V codes (head_dim bytes each, a byte is
+ * code + 128), then the 16 float scales of K and the 16 of V.  Inside row r the 16-byte chunks stand in the order c ^ s(r): s(r) is
+ * the upper log2(gcd(head_dim / 16, 8)) bits of the three bits (r3, r2, r0) of r for K and (r2, r1, r0) for V.
+ * code = rint(x * (127 / amax)) (ties to even), scale = amax / 127, amax the largest magnitude of the row's head_dim elements; a row whose amax is
+ * below 2^-100 is stored as zeros, a row with a NaN or an infinity with a scale of NaN and zeros.  Zeroed memory is an empty cache.
+ * A position of a sequence lives in slot page * page_size + offset.
+ *
+ * append: row t of k and v into slot slots[t] (int32 or int64 by slot_bytes); a negative slot is passed over (padding), one beyond the cache
+ * is passed over and reported.  Slots of one call differ.  With rotary_dim > 0, k is rotated first as by b200q_rotary_embedding but quantized from float without a
+ * rounding between (rotary_dim a multiple of 16), and `heads` heads of q (0: none) are rotated into q_out.
+ * read: k[t], v[t] (dense [tokens, kv_heads, head_dim], 16-byte aligned) = code * scale rounded to `type`; zeros for a slot outside the cache.
+ */
+B200Q_API int b200q_quantized_cache_append(void *cache, int64_t pages, int64_t page_size, const b200q_heads *k, const b200q_heads *v,
+                                           const b200q_heads *q, const b200q_heads *q_out, const void *slots, const void *positions,
+                                           const float *table, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                           int64_t rotary_dim, int64_t table_rows, int layout, int type, int slot_bytes, int position_bytes,
+                                           void *stream);
+B200Q_API int b200q_quantized_cache_read(const void *cache, int64_t pages, int64_t page_size, const void *slots, void *k, void *v, int64_t tokens,
+                                         int64_t kv_heads, int64_t head_dim, int type, int slot_bytes, void *stream);
+
+/*
+ * Attention of the newest tokens of `batch` sequences over that cache, which already holds them.  lengths[b] positions of sequence b are
+ * cached, in the pages page_table[b * table_stride + i] (a length is cut to table_width pages; a page outside the cache gives that tile of
+ * positions another page's contents; both are reported).  Its tokens are rows starts[b] .. starts[b + 1] - 1 of q and out, or
+ * tokens / batch rows each where starts is NULL, and stand at its last positions.  A token sees every position in front of them, and of
+ * them those up to itself, or, with a mask, those with mask[row * mask_stride + j] != 0 (a byte for the j-th of its sequence's new tokens, j < mask_width).
+ * A row that sees nothing has zeros, and -inf in lse.  head h reads key/value head h / (heads / kv_heads).
+ *   out[row, h] = sum_j softmax_j(scale q . k_j) v_j, dense [tokens, heads, head_dim] in q's type (f16 or bf16); lse (float [tokens, heads], may be
+ * NULL) the natural logarithm of the softmax's denominator.  q: 8-byte aligned, strides multiples of 4 elements.
+ * The workspace is one of b200q_qlinear_f16_i8's kind: zero-filled once, its counters are zero again after every call.
+ */
+B200Q_API size_t b200q_quantized_cache_attention_workspace_bytes(int64_t head_dim);
+B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, float *lse, const void *cache, int64_t pages, int64_t page_size,
+                                              const int32_t *page_table, int64_t table_width, int64_t table_stride, const int32_t *lengths,
+                                              const int32_t *starts, const void *mask, int64_t mask_width, int64_t mask_stride, int64_t batch,
+                                              int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, int type,
+                                              void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Log probabilities under softmax(logits[row, :]): log_probs[row, j] of tokens[row, j] (int32 or int64 [rows, given]), the entropy of the row
+ * (in nats), and the `top` (at most 32) largest log probabilities, descending, equal logits by index, with their tokens.  All float sums and
+ * results; logits f16, bf16 or f32, rows row_stride elements apart.  A token outside the vocabulary has -inf and is reported.  -inf logits are
+ * tokens without probability; a row with a NaN or +inf, or of nothing but -inf, has NaN.
+ */
+B200Q_API int b200q_token_log_probs(const void *logits, int64_t row_stride, const void *tokens, float *log_probs, float *entropy,
+                                    float *top_log_probs, int64_t *top_indices, int64_t rows, int64_t vocab, int64_t given, int64_t top, int type,
+                                    int token_bytes, void *stream);
 
 /*
  * Device-side status word of the calling thread's current device: 0 if no bounded wait of any
