@@ -8,15 +8,15 @@
 // they cannot leave f16's range whatever the values' size), are rounded to f16 for the second product, an error of 2^-12 of each, at random; the sums
 // that divide are float.
 //
-// A unit of work is a tile of positions for one (sequence, key/value head, 16 * MT query rows).  The tiles of all sequences stand in
-// one line, which is cut into equal pieces, one a CTA, whatever the sequences' lengths are (the host does not know them: they
+// The work is in tiles of positions for one (sequence, key/value head, 8 * NT query rows).  The tiles of all sequences stand in
+// one line, with a gap in front of every item for what that costs besides where pieces are long, and the line is cut into equal pieces, one a CTA, whatever the sequences' lengths are (the host does not know them: they
 // are on the device, so that a captured step can be replayed as they grow).  A CTA's piece may end one item and begin others; items in
 // several pieces leave partial sums in the workspace, and the CTA that arrives last adds them in the order of the pieces.
 //
 // One warp copies whole records (codes and scales, one bulk copy per run of a page) into a ring of shared memory; each of
-// the other warps takes one record of 16 positions of a tile: it loads K fragments with plain and V fragments with transposing matrix loads, converts
-// two codes an instruction and multiplies.  With the positions (and not the rows) shared out among the warps, each code is converted
-// once per CTA.
+// the other warps takes one record of 16 positions of a tile: it loads K with plain and V with transposing matrix loads, converts two codes an
+// instruction and multiplies, with the codes as the 16-row operand (positions of K, elements of V) and eight query rows as columns.  With the positions
+// (and not the rows) shared out among the warps, each code is converted once per CTA.
 #include <atomic>
 #include <type_traits>
 
@@ -27,8 +27,8 @@ namespace b200q {
 namespace {
 
 constexpr unsigned int kKernelCacheAttention = 7;
-constexpr int kMaxCtas = 2 * 148;         // of a launch; the workspace is made for them
-constexpr int kCounterBytes = 65536 * 4;  // arrival counters in front of the workspace, zero between calls
+constexpr int kMaxCtas = 3 * 148;         // of a launch; the workspace is made for them
+constexpr int kCounterBytes = 65536 * 4;  // arrival counters in front of the workspace, zero between calls: kMaxCtas a level
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are kept 2^6 times as large, and a row's maximum is raised when a score passes it by 2^8 (rarely, behind its first
@@ -61,16 +61,16 @@ struct AttentionArgs {
     unsigned int *status;
 };
 
-// What a consumer has to know of a tile.
-struct Step {
-    int head, row0, rows;  // key/value head; first query row (token * group + head in group) and rows of this item
-    int key0, length, fresh;  // first position of the tile; cached positions; of them those of the new tokens
-    int token0;
-    int flags;
-    int first_cta, last_cta, slot;  // of an item in several pieces: who holds them, and where this CTA's goes
-    int first_slot;
+// A key/value head of a sequence with some of its query rows, and the pieces that it is in.
+struct Item {
+    int head, row0, rows, token0;       // key/value head; first query row (token * group + head in group) and how many, -1: no more items; the sequence's first row of q
+    int length, fresh;                  // cached positions; of them those of the new tokens
+    int first_cta, last_cta, slot;      // who holds the pieces; the place of this CTA's
 };
-constexpr int kFirst = 1, kLast = 2, kEnd = 4;
+struct Tile {
+    int key0;  // first position
+    int last;  // of the item, in this CTA
+};
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -88,33 +88,49 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
     return v;
+}
+__device__ __forceinline__ float lds32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+// 8 x 8 elements of 16 bits: from lane (g, t) holding (row g, columns 2t, 2t + 1) to it holding (rows 2t, 2t + 1, column g).
+__device__ __forceinline__ uint32_t transpose(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
 constexpr int MOST_STAGES = 6;
+constexpr int kItemUnits = 2;           // what an item costs besides its tiles, in tiles
+constexpr int FAN = 8;                  // pieces of an item that are added at once
+constexpr int WARPS = 4;                // that multiply
+constexpr int CONSUMERS = 32 * WARPS;
+constexpr int THREADS = CONSUMERS + 32;
+constexpr int TILE = 16 * WARPS;        // positions
 
-template <int D, int MT, int WARPS>
+template <int D, int NT>
 struct Layout {
-    static constexpr int TILE = 16 * WARPS;  // positions
-    static constexpr int ROWS = 16 * MT;
+    static constexpr int ROWS = 8 * NT;
     static constexpr int RECORD = record_bytes(D);
     static constexpr int STAGE = WARPS * RECORD;
-    static constexpr int PITCH = D + 8;  // floats between rows of a merge buffer: eight rows of float2 in different banks
+    static constexpr int PITCH = D + 4;  // floats between rows of a merge buffer: what a warp stores at once lies in 32 banks
     static constexpr int MERGE = ROWS * PITCH * 4;
     static constexpr int BUFFERS = WARPS / 2;
-    static constexpr int THREADS = 32 * WARPS + 32;
-    static constexpr int PER_SM = WARPS == 4 ? 2 : 1;
+    static constexpr int PER_SM = NT * D <= 128 ? 3 : NT * D <= 256 ? 2 : 1;
     static constexpr int Q = ROWS * D * 2;
     static constexpr int FIXED = Q + BUFFERS * MERGE;
-    static constexpr int ROOM = (PER_SM == 2 ? 113 : 226) * 1024 - 4096 - FIXED;  // 4096: Control, and what an SM keeps for itself
+    static constexpr int ROOM = (PER_SM == 3 ? 75 : PER_SM == 2 ? 113 : 226) * 1024 - 3072 - FIXED;  // 3072: Control, and what an SM keeps for itself
     static constexpr int STAGES = ROOM / STAGE > MOST_STAGES ? MOST_STAGES : ROOM / STAGE;
     static constexpr int SMEM = FIXED + STAGES * STAGE;
+    static constexpr bool Q_IN_REGISTERS = NT * D <= 128;
     static_assert(STAGES >= 2, "");
 };
 
@@ -136,16 +152,15 @@ __device__ __forceinline__ bool all_of(bool ok) {
     return all != 0;
 }
 
+constexpr int ITEMS = 2;  // of which the consumers may know
 struct Control {
-    uint64_t full[MOST_STAGES], empty[MOST_STAGES];
-    Step steps[MOST_STAGES];
-    float m[8][32], l[8][32], vref[8];  // at most 8 warps, 32 rows
-    float q_scale[32];
-    int64_t scan[16];
-    int64_t begin_offset;
-    int begin_sequence, abort, last;
+    uint64_t full[MOST_STAGES], empty[MOST_STAGES], item_full[ITEMS], item_empty[ITEMS];
+    Tile tiles[MOST_STAGES];
+    Item items[ITEMS];
+    float m[WARPS][16], l[WARPS][16], q_scale[16];
+    int abort, last;
 };
-static_assert(sizeof(Control) <= 3072, "");
+static_assert(sizeof(Control) <= 2048, "");
 
 template <typename T>
 __device__ __forceinline__ void load_q4(const T *p, float (&f)[4]) {
@@ -160,7 +175,7 @@ struct Sequence {
     int tiles;     // of one item
     int row_tiles; // items of a key/value head
 };
-template <int TILE, int ROWS>
+template <int ROWS>
 __device__ __forceinline__ Sequence sequence_of(const AttentionArgs &p, int b) {
     Sequence s;
     int64_t n = p.lengths[b];
@@ -178,14 +193,125 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionArgs &p, int b) {
         s.fresh = p.per_sequence;
     }
     s.tiles = max(1, (s.length + TILE - 1) / TILE);  // an empty sequence has a tile too: its rows are written
-    s.row_tiles = (int)(((int64_t)s.fresh * p.group + ROWS - 1) / ROWS);
+    s.row_tiles = (s.fresh * p.group + ROWS - 1) / ROWS;
     return s;
 }
 
-template <int D, int MT, int WARPS, typename T>
-__global__ void __launch_bounds__(32 * WARPS + 32, WARPS == 4 ? 2 : 1) cache_attention_kernel(const AttentionArgs p) {
-    using L = Layout<D, MT, WARPS>;
-    constexpr int TILE = L::TILE, ROWS = L::ROWS, CONSUMERS = 32 * WARPS, STAGES = L::STAGES;
+// The largest of the warps' maxima of a row.
+__device__ __forceinline__ float row_top(const Control &ctl, int r) {
+    float n = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) n = fmaxf(n, ctl.m[w][r]);
+    return n;
+}
+
+// What becomes of an item whose sums stand in the merge buffers: the result, or a piece of it.  All consumers.  
+template <int D, int NT, typename T>
+__device__ __forceinline__ void finish_item(const AttentionArgs &p, Control &ctl, float *merge, const Item &item) {
+    using L = Layout<D, NT>;
+    constexpr int ROWS = L::ROWS;
+    const bool whole = item.first_cta == item.last_cta;
+    float *part = p.partial + (int64_t)item.slot * ROWS * (D + 2);
+    constexpr int VECS = ROWS * D / 4;
+    auto write_out = [&](int r, int d, float4 v, float total_l, float top_log2) {
+        const int row = item.row0 + r, token = row / p.group, head = item.head * p.group + row - token * p.group;
+        const int64_t at = (int64_t)(item.token0 + token) * p.kv_heads * p.group + head;
+        const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
+        T y[4] = {Elems<T>::round(v.x * inv), Elems<T>::round(v.y * inv), Elems<T>::round(v.z * inv), Elems<T>::round(v.w * inv)};
+        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at * D + d) = *reinterpret_cast<const uint2 *>(y);
+        if (d == 0 && p.lse != nullptr) p.lse[at] = total_l == 0.0f ? -INFINITY : (top_log2 - kBias + __log2f(total_l)) * kLn2;
+    };
+    for (int i = threadIdx.x; i < VECS; i += CONSUMERS) {
+        const int r = i / (D / 4), d = 4 * (i % (D / 4));
+        if (r >= item.rows) break;
+        const float top = row_top(ctl, r), scale = ctl.q_scale[r];
+        float sum_l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) sum_l += ctl.m[w][r] == -INFINITY ? ctl.l[w][r] : ctl.l[w][r] * ex2((ctl.m[w][r] - top) * scale);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < L::BUFFERS; ++k) {
+            const float4 x = *reinterpret_cast<const float4 *>(merge + k * (L::MERGE / 4) + r * L::PITCH + d);
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        }
+        const float top_log2 = top * scale;
+        if (whole) {
+            write_out(r, d, v, sum_l, top_log2);
+        } else {
+            __stcg(reinterpret_cast<float4 *>(part + r * D + d), v);
+            if (d == 0) {
+                __stcg(part + ROWS * D + r, top_log2);
+                __stcg(part + ROWS * (D + 1) + r, sum_l);
+            }
+        }
+    }
+    // ---- the pieces of an item meet: FAN neighbours at a time, in the CTA that arrives last of them, then FAN of those ----
+    if (!whole) {
+        int k = blockIdx.x - item.first_cta, n = item.last_cta - item.first_cta + 1, stride = 1;
+        auto part_of = [&](int i) { return p.partial + (int64_t)(2 * (item.first_cta + i) + (i == 0 ? 1 : 0)) * ROWS * (D + 2); };
+        float (*part_m)[16] = reinterpret_cast<float (*)[16]>(merge), (*part_l)[16] = part_m + FAN;  // the merge buffers are free behind the next barrier
+        static_assert(L::BUFFERS * L::MERGE >= 2 * FAN * 16 * 4, "");
+        for (unsigned int *counters = p.counters;; counters += kMaxCtas, k /= FAN, n = (n + FAN - 1) / FAN, stride *= FAN) {
+            const int first = k / FAN * FAN, some = min(FAN, n - first);
+            // The last piece by itself is its own sum.  (It has no counter either: where it starts another item may have its first.)
+            if (some == 1) continue;
+            asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
+            if (threadIdx.x == 0) {
+                unsigned int *counter = counters + item.first_cta + first * stride;
+                unsigned int before;  // releases what the barrier put in front, the stores of all threads of the CTA
+                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+                ctl.last = before == (unsigned int)(some - 1);
+                if (ctl.last) *counter = 0;
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
+            if (!ctl.last) break;
+            for (int i = threadIdx.x; i < some * ROWS; i += CONSUMERS) {
+                const float *from = part_of((first + i / ROWS) * stride) + ROWS * D + i % ROWS;
+                const bool there = i % ROWS < item.rows;
+                part_m[i / ROWS][i % ROWS] = there ? __ldcg(from) : -INFINITY;
+                part_l[i / ROWS][i % ROWS] = there ? __ldcg(from + ROWS) : 0.0f;
+            }
+            const bool done = n <= FAN;
+            for (int i0 = 0; i0 < item.rows * (D / 4); i0 += CONSUMERS) {
+                const int i = i0 + threadIdx.x, r = i / (D / 4), d = 4 * (i % (D / 4));
+                float4 x[FAN];
+#pragma unroll
+                for (int j = 0; j < FAN; ++j)
+                    if (j < some && r < item.rows) x[j] = __ldcg(reinterpret_cast<const float4 *>(part_of((first + j) * stride) + r * D + d));
+                if (i0 == 0) asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
+                if (r >= item.rows) continue;
+                float top = -INFINITY, sum_l = 0.0f;
+#pragma unroll
+                for (int j = 0; j < FAN; ++j)
+                    if (j < some) top = fmaxf(top, part_m[j][r]);
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int j = 0; j < FAN; ++j)
+                    if (j < some) {
+                        const float by = part_m[j][r] == -INFINITY ? 1.0f : ex2(part_m[j][r] - top);
+                        sum_l = fmaf(part_l[j][r], by, sum_l);
+                        v.x = fmaf(x[j].x, by, v.x), v.y = fmaf(x[j].y, by, v.y), v.z = fmaf(x[j].z, by, v.z), v.w = fmaf(x[j].w, by, v.w);
+                    }
+                if (done) {
+                    write_out(r, d, v, sum_l, top);
+                } else {  // into the place of the first of them, whose statistics are in shared memory by now
+                    float *to = part_of(first * stride);
+                    __stcg(reinterpret_cast<float4 *>(to + r * D + d), v);
+                    if (d == 0) {
+                        __stcg(to + ROWS * D + r, top);
+                        __stcg(to + ROWS * (D + 1) + r, sum_l);
+                    }
+                }
+            }
+            if (done) break;
+        }
+    }
+}
+
+template <int D, int NT, typename T>
+__global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attention_kernel(const __grid_constant__ AttentionArgs p) {
+    using L = Layout<D, NT>;
+    constexpr int ROWS = L::ROWS, STAGES = L::STAGES;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Control ctl;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -197,154 +323,146 @@ __global__ void __launch_bounds__(32 * WARPS + 32, WARPS == 4 ? 2 : 1) cache_att
             mbar_init(smem_u32(&ctl.full[s]), 1);
             mbar_init(smem_u32(&ctl.empty[s]), WARPS);
         }
+        for (int s = 0; s < ITEMS; ++s) {
+            mbar_init(smem_u32(&ctl.item_full[s]), 1);
+            mbar_init(smem_u32(&ctl.item_empty[s]), WARPS);
+        }
         ctl.abort = 0;
         mbar_fence_init();
     }
+    __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
 
-    // ---- this CTA's piece of the line of tiles ----
-    int64_t sum = 0;
-    for (int b = threadIdx.x; b < p.batch; b += L::THREADS) {
-        const Sequence s = sequence_of<TILE, ROWS>(p, b);
-        sum += (int64_t)s.tiles * s.row_tiles;
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) ctl.scan[warp] = sum;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS + 1; ++w) total += ctl.scan[w];
-    total *= p.kv_heads;
-    const int64_t ctas = min((int64_t)gridDim.x, total);
-    if (blockIdx.x >= ctas) return;
-    const int64_t begin = blockIdx.x * total / ctas, end = (blockIdx.x + 1) * total / ctas;
-    // the sequence that `begin` lies in
-    int64_t base = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += L::THREADS) {
-        const int b = b0 + threadIdx.x;
-        int64_t own = 0;
-        if (b < p.batch) {
-            const Sequence s = sequence_of<TILE, ROWS>(p, b);
-            own = (int64_t)s.tiles * s.row_tiles * p.kv_heads;
-        }
-        int64_t incl = own;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const int64_t below = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += below;
-        }
-        __syncthreads();
-        if (lane == 31) ctl.scan[warp] = incl;
-        __syncthreads();
-        int64_t before = base, all = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS + 1; ++w) {
-            if (w < warp) before += ctl.scan[w];
-            all += ctl.scan[w];
-        }
-        const int64_t from = before + incl - own;
-        if (from <= begin && begin < from + own) {
-            ctl.begin_sequence = b;
-            ctl.begin_offset = begin - from;
-        }
-        base += all;
-        if (base > begin) break;
-    }
-    __syncthreads();
-
     if (warp == WARPS) {
         // ---------------- producer ----------------
-        int b = ctl.begin_sequence;
-        int64_t offset = ctl.begin_offset, cur = begin;
-        const int records_per_page = p.page_size >> 4;
+        bool dead = false;
+        auto wait_for = [&](uint64_t &barrier, uint32_t parity) {
+            const uint32_t bar = smem_u32(&barrier);
+            bool ok = false;
+            for (uint32_t i = 0; i < umma::kFastPolls && !ok; ++i) ok = mbar_try_wait(bar, parity);
+            if (!ok) ok = umma::wait_or_abort<kKernelCacheAttention>(bar, parity, 1, &ctl.abort, p.status);
+            dead = !__all_sync(0xffffffffu, ok);
+        };
+        int n_items = 0;
+        auto publish = [&](const Item &item) {
+            const int slot = n_items % ITEMS;
+            if (n_items >= ITEMS) wait_for(ctl.item_empty[slot], (n_items / ITEMS - 1) & 1);
+            if (!dead && lane == 0) {
+                ctl.items[slot] = item;
+                mbar_arrive(smem_u32(&ctl.item_full[slot]));
+            }
+            ++n_items;
+        };
+
+        // ---- this CTA's piece of the line ----
+        int items = 0, tiles = 0;
+        for (int b = lane; b < p.batch; b += 32) {
+            const Sequence s = sequence_of<ROWS>(p, b);
+            items += s.row_tiles;
+            tiles += s.row_tiles * s.tiles;
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) {
+            items += __shfl_xor_sync(0xffffffffu, items, d);
+            tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
+        }
+        items *= p.kv_heads;
+        tiles *= p.kv_heads;
+        // No more pieces of an item than are added at once, as long as the wait for another round of additions, about two tiles, would be longer
+        // than what shorter pieces save.
+        int ctas = min((int)gridDim.x, tiles);
+        if (ctas > FAN * items && tiles / (FAN * max(1, items)) - tiles / ctas <= 2) ctas = FAN * items;
+        // Where pieces are long, a gap in front of every item stands for what it costs besides its tiles.
+        const int gap = tiles >= 8 * ctas ? kItemUnits : 0, units = tiles + items * gap;
+        const int each = units / max(1, ctas), more = units - each * ctas;  // the first `more` pieces have one unit more
+        auto piece = [&](int c) { return c * each + min(c, more); };
+        auto cta_of = [&](int unit) { return unit < more * (each + 1) ? unit / (each + 1) : more + (unit - more * (each + 1)) / each; };
+        int cur = 0, end = 0, b = 0, offset = 0;  // units; the sequence that cur lies in, and where in its items
+        if ((int)blockIdx.x < ctas && items > 0) {
+            cur = piece(blockIdx.x);
+            end = piece(blockIdx.x + 1);
+            for (int base = 0, b0 = 0;; b0 += 32) {
+                int own = 0;
+                if (b0 + lane < p.batch) {
+                    const Sequence s = sequence_of<ROWS>(p, b0 + lane);
+                    own = (s.tiles + gap) * s.row_tiles * p.kv_heads;
+                }
+                int until = own;
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const int below = __shfl_up_sync(0xffffffffu, until, d);
+                    if (lane >= d) until += below;
+                }
+                const uint32_t behind = __ballot_sync(0xffffffffu, base + until > cur);
+                if (behind != 0) {
+                    const int l = __ffs(behind) - 1;
+                    b = b0 + l;
+                    offset = cur - base - __shfl_sync(0xffffffffu, until - own, l);
+                    break;
+                }
+                base += __shfl_sync(0xffffffffu, until, 31);
+            }
+        }
+        const int begin = cur, records_per_page = p.page_size >> 4;
         int slot = 0, it = 0;
         uint32_t parity = 0;
-        bool dead = false;
-        auto next_stage = [&]() {
-            if (it >= STAGES) {
-                const uint32_t bar = smem_u32(&ctl.empty[slot]);
-                bool ok = false;
-                for (uint32_t i = 0; i < umma::kFastPolls && !ok; ++i) ok = mbar_try_wait(bar, parity ^ 1u);
-                if (!ok) ok = umma::wait_or_abort<kKernelCacheAttention>(bar, parity ^ 1u, 1, &ctl.abort, p.status);
-                dead = !__all_sync(0xffffffffu, ok);
-            }
-        };
         while (cur < end && !dead) {
-            const Sequence s = sequence_of<TILE, ROWS>(p, b);
+            const Sequence s = sequence_of<ROWS>(p, b);
+            const int per = s.tiles + gap;
             if (s.row_tiles == 0) {
                 ++b;
                 continue;
             }
-            const int64_t item = offset / s.tiles;
-            const int tile0 = (int)(offset - item * s.tiles);
-            const int head = (int)(item / s.row_tiles), rt = (int)(item - (int64_t)head * s.row_tiles);
-            const int n = (int)min((int64_t)(s.tiles - tile0), end - cur);
-            const int64_t item_begin = cur - tile0, item_end = item_begin + s.tiles;
-            const int first_cta = (int)(((item_begin + 1) * ctas - 1) / total), last_cta = (int)((item_end * ctas - 1) / total);
-            const int first_slot = first_cta * total / ctas == item_begin ? 0 : 1;
+            const int index = offset / per, head = index / s.row_tiles, rt = index - head * s.row_tiles;
+            const int item_begin = cur - (offset - index * per), tiles_begin = item_begin + gap, item_end = item_begin + per;
+            const int to = min(end, item_end), tile0 = max(cur, tiles_begin) - tiles_begin, n = to - tiles_begin - tile0;
             const int32_t *pages = p.table + (int64_t)b * p.table_stride;
-            // lane i < 8 brings the i-th page that the tile touches; its number is asked for one tile ahead
+            offset += to - cur;
+            cur = to;
+            if (offset == per * s.row_tiles * p.kv_heads) ++b, offset = 0;
+            if (n <= 0) continue;  // its tiles are another CTA's
+            // lane i brings the i-th page that the tile touches; its number is asked for one tile ahead
             auto page_of = [&](int tile) {
                 const int page = tile * TILE / p.page_size + lane;
                 return tile < tile0 + n && lane <= WARPS && (int64_t)page * p.page_size < s.length ? pages[page] : 0;
             };
             int page = page_of(tile0);
+            publish({head, rt * ROWS, min(ROWS, s.fresh * p.group - rt * ROWS), s.token0, s.length, s.fresh, cta_of(tiles_begin), cta_of(item_end - 1),
+                     2 * (int)blockIdx.x + (tiles_begin >= begin ? 1 : 0)});
             for (int i = 0; i < n && !dead; ++i) {
                 const int tile = tile0 + i, key0 = tile * TILE;
                 const int next = page_of(tile + 1);
-                next_stage();
+                if (it >= STAGES) wait_for(ctl.empty[slot], parity ^ 1u);
                 if (dead) break;
                 const int keys = min(TILE, (s.length - key0 + 15) & ~15);  // 0 where the sequence is empty
                 const uint32_t bar = smem_u32(&ctl.full[slot]);
                 if (lane == 0) {
-                    Step &st = ctl.steps[slot];
-                    st.head = head;
-                    st.row0 = rt * ROWS;
-                    st.rows = min(ROWS, s.fresh * p.group - rt * ROWS);
-                    st.key0 = key0;
-                    st.length = s.length;
-                    st.fresh = s.fresh;
-                    st.token0 = s.token0;
-                    st.flags = (i == 0 ? kFirst : 0) | (i == n - 1 ? kLast : 0);
-                    st.first_cta = first_cta;
-                    st.last_cta = last_cta;
-                    st.first_slot = first_slot;
-                    st.slot = 2 * blockIdx.x + (cur == begin ? 0 : 1);
+                    ctl.tiles[slot] = {key0, i == n - 1};
                     if (keys > 0) mbar_expect_tx(bar, (uint32_t)(keys >> 4) * L::RECORD);
                     else mbar_arrive(bar);
                 }
                 __syncwarp();
                 const int at = (key0 / p.page_size + lane) * p.page_size;  // first position of this lane's page
-                const int from = max(at, key0), to = min(at + p.page_size, key0 + keys);
-                if (lane <= WARPS && from < to) {
+                const int from = max(at, key0), until = min(at + p.page_size, key0 + keys);
+                if (lane <= WARPS && from < until) {
                     if (page < 0 || page >= p.pages) {
                         page = 0;
                         if (p.status != nullptr) atomicOr(p.status, kBadPage);
                     }
                     const uint8_t *src = p.cache + (((int64_t)page * p.kv_heads + head) * records_per_page + ((from - at) >> 4)) * L::RECORD;
-                    bulk_load(stages + slot * L::STAGE + ((from - key0) >> 4) * L::RECORD, src, (uint32_t)((to - from) >> 4) * L::RECORD, bar);
+                    bulk_load(stages + slot * L::STAGE + ((from - key0) >> 4) * L::RECORD, src, (uint32_t)((until - from) >> 4) * L::RECORD, bar);
                 }
                 page = next;
                 ++it;
                 if (++slot == STAGES) slot = 0, parity ^= 1u;
             }
-            cur += n;
-            offset += n;
-            if (offset == (int64_t)s.tiles * s.row_tiles * p.kv_heads) ++b, offset = 0;
         }
-        if (!dead) {
-            next_stage();
-            if (!dead && lane == 0) {
-                ctl.steps[slot].flags = kEnd;
-                mbar_arrive(smem_u32(&ctl.full[slot]));
-            }
-        }
+        if (!dead) publish({0, 0, -1, 0, 0, 0, 0, 0, 0});
         if (dead) {  // nothing may be on its way when the CTA ends
             for (int back = 1; back <= STAGES && back <= it; ++back) {
-                const int s = (it - back) % STAGES;
-                mbar_wait(smem_u32(&ctl.full[s]), ((it - back) / STAGES) & 1, 1u << 16);
+                const int at = it - back;
+                mbar_wait(smem_u32(&ctl.full[at % STAGES]), (at / STAGES) & 1, 1u << 16);
             }
         }
         return;
@@ -352,32 +470,40 @@ __global__ void __launch_bounds__(32 * WARPS + 32, WARPS == 4 ? 2 : 1) cache_att
 
     // ---------------- consumers ----------------
     const int g = lane >> 2, t = lane & 3;
-    // K: lane l addresses row 4 (c / 2) + c % 2 + 2 (l / 16) of its record, c = l % 8, and of a pair of chunks the (l / 8 % 2)-th.  So MMA
-    // columns 2t, 2t + 1 of the first matrix are positions 4t, 4t + 1 and of the second 4t + 2, 4t + 3: the four whose codes a transposing
-    // load of V leaves in one register of this lane.  Inside a chunk a lane holds elements 4t .. 4t + 3; the query's fragments follow that.
-    const uint32_t k_row = 4 * ((lane & 7) >> 1) + (lane & 1) + 2 * (lane >> 4);
-    const uint32_t k_off = k_row * D, k_sw = k_order(k_row, D), k_chunk = (lane >> 3) & 1;
+    // K: lane l addresses row 4 (c / 2) + c % 2 + 2 (l / 8 % 2) of its record, c = l % 8, and of a pair of chunks the (l / 16)-th.  So MMA
+    // row g is position 4 (g / 2) + g % 2 and row g + 8 the one two further on: after the transposition of the probabilities
+    // lane (g, t) has positions 4t .. 4t + 3 of query row g, the four whose codes a transposing load of V leaves in one register.  Inside a
+    // chunk a lane holds elements 4t .. 4t + 3; the query's fragments follow that.
+    const uint32_t k_row = 4 * ((lane & 7) >> 1) + (lane & 1) + 2 * ((lane >> 3) & 1);
+    const uint32_t k_off = k_row * D, k_sw = k_order(k_row, D), k_chunk = lane >> 4;
     const uint32_t v_row = lane & 15;
     const uint32_t v_off = 16 * D + v_row * D, v_sw = v_order(v_row, D), v_chunk = lane >> 4;
-    float o[MT][D / 8][4];
-    float m[MT][2], l[MT][2], shift[MT][2], qs[MT][2], rise[MT][2];  // shift: m, or 0 as long as nothing was seen
-    float vref = 0.0f, v_inv = 0.0f, v_limit = kLeastNormal;  // a power of two, its reciprocal, and the first scale that is too large for it
+    const int key_of_lane = 4 * (g >> 1) + (g & 1);  // of the scores in [0] and [1]; those in [2] and [3] are two positions further on
     // A warp whose wait runs out brings `false` to the next barrier of all consumers, where all of them leave: one by one, it would
     // leave the others waiting there.  `met`: this warp has been at that barrier.
     bool alive = true, met = false;
-    for (int slot = 0, parity = 0;;) {
-        {
-            const uint32_t bar = smem_u32(&ctl.full[slot]);
-            bool ok = false;
-            for (uint32_t i = 0; i < umma::kFastPolls && !ok; ++i) ok = mbar_try_wait(bar, parity);
-            if (!ok) ok = umma::wait_or_abort<kKernelCacheAttention>(bar, parity, 2, &ctl.abort, p.status);
-            alive = __all_sync(0xffffffffu, ok);
-        }
+    int slot = 0, parity = 0;
+    auto wait_for = [&](uint64_t &barrier, uint32_t phase) {
+        const uint32_t bar = smem_u32(&barrier);
+        bool ok = false;
+        for (uint32_t i = 0; i < umma::kFastPolls && !ok; ++i) ok = mbar_try_wait(bar, phase);
+        if (!ok) ok = umma::wait_or_abort<kKernelCacheAttention>(bar, phase, 2, &ctl.abort, p.status);
+        alive = __all_sync(0xffffffffu, ok);
+    };
+    for (int n_item = 0;; ++n_item) {
+        wait_for(ctl.item_full[n_item % ITEMS], (n_item / ITEMS) & 1);
         if (!alive) break;
-        const Step st = ctl.steps[slot];
-        if (st.flags & kEnd) break;
-        if (st.flags & kFirst) {
-            // the queries, as MMA fragments: for chunk c and rows g, g + 8 lane (g, t) has elements 16 c + 4t .. + 3 of both
+        const Item item = ctl.items[n_item % ITEMS];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[n_item % ITEMS]));
+        if (item.rows < 0) break;
+        const int length = item.length, fresh = item.fresh;
+        float o[NT][D / 16][4];  // elements 16 i + g (0, 1) and + 8 (2, 3) of query rows 2t (0, 2) and 2t + 1 (1, 3)
+        float m[NT][2], l[NT][2], shift[NT][2], qs[NT][2], rise[NT][2];  // shift: m, or 0 as long as nothing was seen
+        float vref = 0.0f, v_inv = 0.0f, v_limit = kLeastNormal;  // a power of two, its reciprocal, and the first scale that is too large for it
+        uint2 q_reg[L::Q_IN_REGISTERS ? NT * D / 16 : 1];
+        {
+            // the queries, as MMA fragments: for chunk c and row g lane (g, t) has elements 16 c + 4t .. + 3
             if (!all_of<CONSUMERS>(true)) {
                 met = true;
                 break;
@@ -385,8 +511,8 @@ __global__ void __launch_bounds__(32 * WARPS + 32, WARPS == 4 ? 2 : 1) cache_att
 #pragma unroll
             for (int r0 = 0; r0 < ROWS; r0 += WARPS) {
                 const int r = r0 + warp;
-                const int row = st.row0 + r, token = row / p.group;
-                const T *src = static_cast<const T *>(p.q) + (int64_t)(st.token0 + token) * p.q_token + (int64_t)(st.head * p.group + row - token * p.group) * p.q_head;
+                const int row = item.row0 + r, token = row / p.group;
+                const T *src = static_cast<const T *>(p.q) + (int64_t)(item.token0 + token) * p.q_token + (int64_t)(item.head * p.group + row - token * p.group) * p.q_head;
                 float f[(D + 127) / 128][4];
                 float top = 0.0f;
 #pragma unroll
@@ -394,7 +520,7 @@ __global__ void __launch_bounds__(32 * WARPS + 32, WARPS == 4 ? 2 : 1) cache_att
                     const int d = 4 * lane + 128 * j;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) f[j][e] = 0.0f;
-                    if (r < st.rows && d < D) load_q4(src + d, f[j]);
+                    if (r < item.rows && d < D) load_q4(src + d, f[j]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(f[j][e]));
                 }
@@ -410,315 +536,237 @@ __global__ void __launch_bounds__(32 * WARPS + 32, WARPS == 4 ? 2 : 1) cache_att
                 for (int j = 0; j < (D + 127) / 128; ++j) {
                     const int d = 4 * lane + 128 * j;
                     if (d < D) {
-                        const uint32_t at = (((r >> 4) * (D / 16) + (d >> 4)) * 32 + ((r & 7) << 2) + ((d >> 2) & 3)) * 16 + ((r >> 3) & 1) * 4;
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(q_frag + at), "r"(pack_f16(f[j][0] * down, f[j][1] * down)) : "memory");
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(q_frag + at + 8), "r"(pack_f16(f[j][2] * down, f[j][3] * down)) : "memory");
+                        const uint32_t at = (((r >> 3) * (D / 16) + (d >> 4)) * 32 + ((r & 7) << 2) + ((d >> 2) & 3)) * 8;
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(q_frag + at), "r"(pack_f16(f[j][0] * down, f[j][1] * down)), "r"(pack_f16(f[j][2] * down, f[j][3] * down)) : "memory");
                     }
                 }
             }
             asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                for (int n = 0; n < D / 8; ++n)
+                for (int n = 0; n < D / 16; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.0f;
+                    for (int e = 0; e < 4; ++e) o[nt][n][e] = 0.0f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    m[mt][h] = -INFINITY;
-                    l[mt][h] = shift[mt][h] = 0.0f;
-                    qs[mt][h] = ctl.q_scale[16 * mt + 8 * h + g];
-                    rise[mt][h] = fminf(kRise / qs[mt][h], 1e38f);
+                    m[nt][h] = -INFINITY;
+                    l[nt][h] = shift[nt][h] = 0.0f;
+                    qs[nt][h] = ctl.q_scale[8 * nt + 2 * t + h];
+                    rise[nt][h] = fminf(kRise / qs[nt][h], 1e38f);
                 }
             }
-            vref = v_inv = 0.0f;
-            v_limit = kLeastNormal;
+            if (L::Q_IN_REGISTERS) {
+#pragma unroll
+                for (int i = 0; i < NT * D / 16; ++i) q_reg[L::Q_IN_REGISTERS ? i : 0] = lds64(q_frag + (i * 32 + lane) * 8);
+            }
         }
-        const int key0 = st.key0 + 16 * warp;
-        if (key0 < st.length) {
-            const uint32_t rec = stages + slot * L::STAGE + warp * L::RECORD;
-            const uint4 ks4 = lds128(rec + 32 * D + 16 * t), vs4 = lds128(rec + 32 * D + 64 + 16 * t);
-            const float ks[4] = {__uint_as_float(ks4.x), __uint_as_float(ks4.y), __uint_as_float(ks4.z), __uint_as_float(ks4.w)};
-            float vs[4] = {__uint_as_float(vs4.x), __uint_as_float(vs4.y), __uint_as_float(vs4.z), __uint_as_float(vs4.w)};
-            float c[MT][2][4];
+        for (;;) {
+            wait_for(ctl.full[slot], parity);
+            if (!alive) break;
+            const Tile tile = ctl.tiles[slot];
+            const int key0 = tile.key0 + 16 * warp;
+            if (key0 < length) {
+                const uint32_t rec = stages + slot * L::STAGE + warp * L::RECORD;
+                const uint32_t scales = rec + 32 * D + 4 * key_of_lane;
+                const float ks[2] = {lds32(scales), lds32(scales + 8)};
+                float vs[2] = {lds32(scales + 64), lds32(scales + 72)};
+                float s[NT][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                    for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) c[mt][j][e] = 0.0f;
-#pragma unroll
-            for (int kk = 0; kk < D / 32; ++kk) {
-                uint32_t r[4];
-                umma::ldmatrix_x4(r, rec + k_off + (((2 * kk + k_chunk) ^ k_sw) << 4));
-                uint32_t b[4][2];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) codes_to_f16(r[i], b[i][0], b[i][1]);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int kk = 0; kk < D / 32; ++kk) {
+                    uint32_t r[4];
+                    umma::ldmatrix_x4(r, rec + k_off + (((2 * kk + k_chunk) ^ k_sw) << 4));
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint4 a = lds128(q_frag + ((mt * (D / 16) + 2 * kk + i) * 32 + lane) * 16);
-                        mma_m16n8k16(c[mt][0], a.x, a.y, a.z, a.w, b[i][0], b[i][1]);
-                        mma_m16n8k16(c[mt][1], a.x, a.y, a.z, a.w, b[2 + i][0], b[2 + i][1]);
-                    }
-            }
-            // scores, four positions of each of the lane's rows
-            float s[MT][2][4];
+                        uint32_t a[4];
+                        codes_to_f16(r[2 * i], a[0], a[2]);
+                        codes_to_f16(r[2 * i + 1], a[1], a[3]);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[mt][h][e] = c[mt][e >> 1][2 * h + (e & 1)] * ks[e];
-            const int old = st.length - st.fresh;  // positions in front of the new tokens
-            const bool partly = key0 + 16 > (p.mask != nullptr ? old : min(old + 1, st.length));
-            if (partly) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (key0 + 4 * t + e >= st.length) vs[e] = 0.0f;
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int r = 16 * mt + 8 * h + g, token = (st.row0 + r) / p.group;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int pos = key0 + 4 * t + e, drafted = pos - old;
-                            bool seen = pos < st.length && r < st.rows;
-                            if (seen && drafted >= 0) {
-                                seen = p.mask == nullptr ? drafted <= token : drafted < p.mask_width && p.mask[(int64_t)(st.token0 + token) * p.mask_stride + drafted] != 0;
-                            }
-                            if (!seen) s[mt][h][e] = -INFINITY;
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const int at = nt * (D / 16) + 2 * kk + i;
+                            const uint2 b = L::Q_IN_REGISTERS ? q_reg[L::Q_IN_REGISTERS ? at : 0] : lds64(q_frag + (at * 32 + lane) * 8);
+                            mma_m16n8k16(s[nt], a[0], a[1], a[2], a[3], b.x, b.y);
                         }
                     }
-            }
-            bool up = false;
-            const float v_top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-            up = v_top >= v_limit;
-            float top[MT][2];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    top[mt][h] = fmaxf(fmaxf(s[mt][h][0], s[mt][h][1]), fmaxf(s[mt][h][2], s[mt][h][3]));
-                    up |= top[mt][h] > m[mt][h] + rise[mt][h];
                 }
-            if (__any_sync(0xffffffffu, up)) {
-                float v_new = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, 1));
-                v_new = fmaxf(fmaxf(v_new, __shfl_xor_sync(0xffffffffu, v_new, 2)), vref);
-                const uint32_t power = __float_as_uint(v_new) & 0x7f800000u;
-                const float beta = power != 0 ? vref * __uint_as_float(0x7f000000u - power) : 1.0f;
-                vref = __uint_as_float(power);
-                v_inv = power != 0 ? __uint_as_float(0x7f000000u - power) : 0.0f;
-                v_limit = power != 0 ? 2.0f * vref : kLeastNormal;
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    float by[2];
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[nt][e] *= ks[e >> 1];
+                const int old = length - fresh;  // positions in front of the new tokens
+                const bool partly = key0 + 16 > (p.mask != nullptr ? old : min(old + 1, length));
+                if (partly) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        float n = fmaxf(top[mt][h], __shfl_xor_sync(0xffffffffu, top[mt][h], 1));
-                        n = fmaxf(fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 2)), m[mt][h]);
-                        const float alpha = n == -INFINITY ? 1.0f : ex2((m[mt][h] - n) * qs[mt][h]);
-                        m[mt][h] = n;
-                        shift[mt][h] = n == -INFINITY ? 0.0f : n;
-                        l[mt][h] *= alpha;
-                        by[h] = alpha * beta;
-                    }
+                        const int pos = key0 + key_of_lane + 2 * h, drafted = pos - old;
+                        if (pos >= length) vs[h] = 0.0f;
 #pragma unroll
-                    for (int n = 0; n < D / 8; ++n) {
-                        o[mt][n][0] *= by[0];
-                        o[mt][n][1] *= by[0];
-                        o[mt][n][2] *= by[1];
-                        o[mt][n][3] *= by[1];
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int r = 8 * nt + 2 * t + e, token = (item.row0 + r) / p.group;
+                                bool seen = pos < length && r < item.rows;
+                                if (seen && drafted >= 0) {
+                                    seen = p.mask == nullptr ? drafted <= token : drafted < p.mask_width && p.mask[(int64_t)(item.token0 + token) * p.mask_stride + drafted] != 0;
+                                }
+                                if (!seen) s[nt][2 * h + e] = -INFINITY;
+                            }
                     }
                 }
-            }
-            uint32_t a[MT][4];
+                const float v_top = fmaxf(vs[0], vs[1]);
+                bool up = v_top >= v_limit;
+                float top[NT][2];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float w[4];
+                    for (int h = 0; h < 2; ++h) {
+                        top[nt][h] = fmaxf(s[nt][h], s[nt][2 + h]);
+                        up |= top[nt][h] > m[nt][h] + rise[nt][h];
+                    }
+                if (__any_sync(0xffffffffu, up)) {
+                    float v_new = v_top;
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) v_new = fmaxf(v_new, __shfl_xor_sync(0xffffffffu, v_new, d));
+                    v_new = fmaxf(v_new, vref);
+                    const uint32_t power = __float_as_uint(v_new) & 0x7f800000u;
+                    const float beta = power != 0 ? vref * __uint_as_float(0x7f000000u - power) : 1.0f;
+                    vref = __uint_as_float(power);
+                    v_inv = power != 0 ? __uint_as_float(0x7f000000u - power) : 0.0f;
+                    v_limit = power != 0 ? 2.0f * vref : kLeastNormal;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float by[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float n = top[nt][h];
+#pragma unroll
+                            for (int d = 4; d < 32; d *= 2) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, d));
+                            n = fmaxf(n, m[nt][h]);
+                            const float alpha = n == -INFINITY ? 1.0f : ex2((m[nt][h] - n) * qs[nt][h]);
+                            m[nt][h] = n;
+                            shift[nt][h] = n == -INFINITY ? 0.0f : n;
+                            l[nt][h] *= alpha;
+                            by[h] = alpha * beta;
+                        }
+#pragma unroll
+                        for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[nt][n][e] *= by[e & 1];
+                    }
+                }
+                const float w[2] = {vs[0] * v_inv, vs[1] * v_inv};
+                uint32_t b[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float x[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float x = ex2(fmaf(s[mt][h][e] - shift[mt][h], qs[mt][h], kBias));
-                        l[mt][h] += x;
-                        w[e] = x * (vs[e] * v_inv);
-                        if (partly && s[mt][h][e] == -INFINITY) w[e] = 0.0f;  // whatever the scale of a position that is not seen
+                        x[e] = ex2(fmaf(s[nt][e] - shift[nt][e & 1], qs[nt][e & 1], kBias));
+                        l[nt][e & 1] += x[e];
+                        x[e] *= w[e >> 1];
+                        if (partly && s[nt][e] == -INFINITY) x[e] = 0.0f;  // whatever the scale of a position that is not seen
                     }
-                    a[mt][h] = pack_f16(w[0], w[1]);
-                    a[mt][2 + h] = pack_f16(w[2], w[3]);
+                    b[nt][0] = transpose(pack_f16(x[0], x[1]));
+                    b[nt][1] = transpose(pack_f16(x[2], x[3]));
                 }
 #pragma unroll
-            for (int dd = 0; dd < D / 32; ++dd) {
-                uint32_t r[4];
-                umma::ldmatrix_x2_trans_b8(r, rec + v_off + (((2 * dd + v_chunk) ^ v_sw) << 4));
+                for (int dd = 0; dd < D / 32; ++dd) {
+                    uint32_t r[4];
+                    umma::ldmatrix_x2_trans_b8(r, rec + v_off + (((2 * dd + v_chunk) ^ v_sw) << 4));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t b0, b1;
-                    codes_to_f16(r[i], b0, b1);
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t a[4];
+                        codes_to_f16(r[2 * i], a[0], a[2]);
+                        codes_to_f16(r[2 * i + 1], a[1], a[3]);
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) mma_m16n8k16(o[mt][4 * dd + i], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b0, b1);
+                        for (int nt = 0; nt < NT; ++nt) mma_m16n8k16(o[nt][2 * dd + i], a[0], a[1], a[2], a[3], b[nt][0], b[nt][1]);
+                    }
                 }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&ctl.empty[slot]));
+            if (++slot == STAGES) slot = 0, parity ^= 1;
+            if (tile.last) break;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&ctl.empty[slot]));
-        if (++slot == STAGES) slot = 0, parity ^= 1;
-        if (!(st.flags & kLast)) continue;
+        if (!alive) break;
 
         // ---- the warps' sums meet ----
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 1);
-                l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 2);
-                if (t == 0) {
-                    ctl.m[warp][16 * mt + 8 * h + g] = m[mt][h];
-                    ctl.l[warp][16 * mt + 8 * h + g] = l[mt][h];
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], d);
+                if (g == 0) {
+                    ctl.m[warp][8 * nt + 2 * t + h] = m[nt][h];
+                    ctl.l[warp][8 * nt + 2 * t + h] = l[nt][h];
                 }
             }
         if (!all_of<CONSUMERS>(true)) {
             met = true;
             break;
         }
-        auto row_top = [&](int r) {
-            float n = -INFINITY;
+        float factor[NT][2];
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) n = fmaxf(n, ctl.m[w][r]);
-            return n;
-        };
-        float factor[MT][2];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) factor[mt][h] = m[mt][h] == -INFINITY ? vref : ex2((m[mt][h] - row_top(16 * mt + 8 * h + g)) * qs[mt][h]) * vref;
-        float *mine = merge + (warp % L::BUFFERS) * (L::MERGE / 4) + g * L::PITCH + 2 * t;
+            for (int h = 0; h < 2; ++h) factor[nt][h] = m[nt][h] == -INFINITY ? vref : ex2((m[nt][h] - row_top(ctl, 8 * nt + 2 * t + h)) * qs[nt][h]) * vref;
+        float *mine = merge + (warp % L::BUFFERS) * (L::MERGE / 4) + 2 * t * L::PITCH + g;
         if (warp >= L::BUFFERS) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int n = 0; n < D / 8; ++n)
+                for (int n = 0; n < D / 16; ++n)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        *reinterpret_cast<float2 *>(mine + (16 * mt + 8 * h) * L::PITCH + 8 * n) = make_float2(o[mt][n][2 * h] * factor[mt][h], o[mt][n][2 * h + 1] * factor[mt][h]);
+                    for (int e = 0; e < 4; ++e) mine[(8 * nt + (e & 1)) * L::PITCH + 16 * n + 8 * (e >> 1)] = o[nt][n][e] * factor[nt][e & 1];
         }
         asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
         if (warp < L::BUFFERS) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int n = 0; n < D / 8; ++n)
+                for (int n = 0; n < D / 16; ++n)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float2 *at = reinterpret_cast<float2 *>(mine + (16 * mt + 8 * h) * L::PITCH + 8 * n);
-                        const float2 other = *at;
-                        *at = make_float2(fmaf(o[mt][n][2 * h], factor[mt][h], other.x), fmaf(o[mt][n][2 * h + 1], factor[mt][h], other.y));
+                    for (int e = 0; e < 4; ++e) {
+                        float *at = mine + (8 * nt + (e & 1)) * L::PITCH + 16 * n + 8 * (e >> 1);
+                        *at = fmaf(o[nt][n][e], factor[nt][e & 1], *at);
                     }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
-        const bool whole = st.first_cta == st.last_cta;
-        float *part = p.partial + (int64_t)st.slot * ROWS * (D + 2);
-        constexpr int VECS = ROWS * D / 4;
-        auto write_out = [&](int r, int d, float4 v, float total_l, float top_log2) {
-            const int row = st.row0 + r, token = row / p.group, head = st.head * p.group + row - token * p.group;
-            const int64_t at = (int64_t)(st.token0 + token) * p.kv_heads * p.group + head;
-            const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
-            T y[4] = {Elems<T>::round(v.x * inv), Elems<T>::round(v.y * inv), Elems<T>::round(v.z * inv), Elems<T>::round(v.w * inv)};
-            *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at * D + d) = *reinterpret_cast<const uint2 *>(y);
-            if (d == 0 && p.lse != nullptr) p.lse[at] = total_l == 0.0f ? -INFINITY : (top_log2 - kBias + __log2f(total_l)) * kLn2;
-        };
-        for (int i = threadIdx.x; i < VECS; i += CONSUMERS) {
-            const int r = i / (D / 4), d = 4 * (i % (D / 4));
-            if (r >= st.rows) break;
-            const float top = row_top(r), scale = ctl.q_scale[r];
-            float sum_l = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) sum_l += ctl.m[w][r] == -INFINITY ? ctl.l[w][r] : ctl.l[w][r] * ex2((ctl.m[w][r] - top) * scale);
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int k = 0; k < L::BUFFERS; ++k) {
-                const float4 x = *reinterpret_cast<const float4 *>(merge + k * (L::MERGE / 4) + r * L::PITCH + d);
-                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-            }
-            const float top_log2 = top * scale;
-            if (whole) {
-                write_out(r, d, v, sum_l, top_log2);
-            } else {
-                __stcg(reinterpret_cast<float4 *>(part + r * D + d), v);
-                if (d == 0) {
-                    __stcg(part + ROWS * D + r, top_log2);
-                    __stcg(part + ROWS * (D + 1) + r, sum_l);
-                }
-            }
-        }
-        if (!whole) {
-            __threadfence();
-            asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
-            const int parts = st.last_cta - st.first_cta + 1;
-            if (threadIdx.x == 0) {
-                const unsigned int before = atomicAdd(p.counters + st.first_cta, 1u);
-                ctl.last = before == (unsigned int)(parts - 1);
-                if (ctl.last) p.counters[st.first_cta] = 0;
-                __threadfence();
-            }
-            asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
-            if (ctl.last) {
-                __threadfence();
-                auto part_of = [&](int k) { return p.partial + (int64_t)(2 * (st.first_cta + k) + (k == 0 ? st.first_slot : 0)) * ROWS * (D + 2); };
-                for (int i = threadIdx.x; i < VECS; i += CONSUMERS) {
-                    const int r = i / (D / 4), d = 4 * (i % (D / 4));
-                    if (r >= st.rows) break;
-                    float top = -INFINITY, sum_l = 0.0f;
-#pragma unroll 8
-                    for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(part_of(k) + ROWS * D + r));
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                    for (int k = 0; k < parts; ++k) {
-                        const float *from = part_of(k);
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(from + r * D + d));
-                        const float own = __ldcg(from + ROWS * D + r), part_l = __ldcg(from + ROWS * (D + 1) + r);
-                        const float by = own == -INFINITY ? 1.0f : ex2(own - top);
-                        sum_l = fmaf(part_l, by, sum_l);
-                        v.x = fmaf(x.x, by, v.x), v.y = fmaf(x.y, by, v.y), v.z = fmaf(x.z, by, v.z), v.w = fmaf(x.w, by, v.w);
-                    }
-                    write_out(r, d, v, sum_l, top);
-                }
-            }
-        }
+        finish_item<D, NT, T>(p, ctl, merge, item);
         // the merge buffers and statistics are written again only behind the barrier in front of the next item's queries
     }
     if (!met) all_of<CONSUMERS>(alive);
 }
 
-template <int D, int MT, int WARPS, typename T>
-int launch_sized(AttentionArgs p, int64_t most_tiles, cudaStream_t stream) {
-    using L = Layout<D, MT, WARPS>;
-    auto kernel = cache_attention_kernel<D, MT, WARPS, T>;
-    static std::atomic<bool> attr_set[64];  // per device; a repeated set by a racing thread is harmless
+template <int D, int NT, typename T>
+int launch_sized(AttentionArgs p, cudaStream_t stream) {
+    using L = Layout<D, NT>;
+    auto kernel = cache_attention_kernel<D, NT, T>;
+    static std::atomic<bool> attr_set[64];
     const int rc = allow_smem(attr_set, kernel, L::SMEM);
     if (rc != B200Q_OK) return rc;
-    const int64_t at_once = L::PER_SM * (int64_t)sm_count();
-    int64_t grid = most_tiles < at_once ? most_tiles : at_once;
+    const int64_t tiles = p.kv_heads * (p.tokens * p.group / L::ROWS + p.batch) * (p.capacity / TILE + 1), at_once = L::PER_SM * (int64_t)sm_count();
+    if (tiles > (1ll << 29)) return set_error(B200Q_UNSUPPORTED, "quantized_cache_attention: up to %lld tiles of %d rows and %d positions", (long long)tiles, L::ROWS, TILE);
+    int64_t grid = tiles < at_once ? tiles : at_once;
     if (grid > kMaxCtas) grid = kMaxCtas;
-    return launch_after("cache_attention_kernel", kernel, dim3((unsigned)grid), L::THREADS, L::SMEM, 1, stream, p);
+    return launch_after("cache_attention_kernel", kernel, dim3((unsigned)grid), THREADS, L::SMEM, 1, stream, p);
 }
 
-// Rows of the query that share a key/value head, on average: up to 16 in 16-row items, two CTAs an SM; more in 32-row items, each code
-// converted for twice as many products, one CTA of eight warps an SM (its sums need the registers).
+// Rows of the query that share a key/value head, on average: up to 8 in 8-row items, more in 16-row items.
 template <typename T>
 int launch_typed(const AttentionArgs &p, int dim, cudaStream_t stream) {
-    const bool wide = dim <= 128 && p.tokens * p.group > 16 * (int64_t)p.batch;
-    const int rows = wide ? 32 : 16, tile = wide ? 128 : 64;
-    const int64_t tiles = p.kv_heads * (p.tokens * p.group / rows + p.batch) * (p.capacity / tile + 1);
+    const bool wide = p.tokens * p.group > 8 * (int64_t)p.batch;
     switch (dim) {
-        case 64: return wide ? launch_sized<64, 2, 8, T>(p, tiles, stream) : launch_sized<64, 1, 4, T>(p, tiles, stream);
-        case 96: return wide ? launch_sized<96, 2, 8, T>(p, tiles, stream) : launch_sized<96, 1, 4, T>(p, tiles, stream);
-        case 128: return wide ? launch_sized<128, 2, 8, T>(p, tiles, stream) : launch_sized<128, 1, 4, T>(p, tiles, stream);
-        case 192: return launch_sized<192, 1, 4, T>(p, tiles, stream);
-        default: return launch_sized<256, 1, 4, T>(p, tiles, stream);
+        case 64: return wide ? launch_sized<64, 2, T>(p, stream) : launch_sized<64, 1, T>(p, stream);
+        case 96: return wide ? launch_sized<96, 2, T>(p, stream) : launch_sized<96, 1, T>(p, stream);
+        case 128: return wide ? launch_sized<128, 2, T>(p, stream) : launch_sized<128, 1, T>(p, stream);
+        case 192: return wide ? launch_sized<192, 2, T>(p, stream) : launch_sized<192, 1, T>(p, stream);
+        default: return wide ? launch_sized<256, 2, T>(p, stream) : launch_sized<256, 1, T>(p, stream);
     }
 }
 
@@ -730,8 +778,7 @@ extern "C" {
 B200Q_API size_t b200q_quantized_cache_attention_workspace_bytes(int64_t head_dim) {
     using namespace b200q;
     if (!cache_dim(head_dim)) return 0;
-    const int64_t rows = head_dim <= 128 ? 32 : 16;
-    return (size_t)(kCounterBytes + (int64_t)2 * kMaxCtas * rows * (head_dim + 2) * 4);
+    return (size_t)(kCounterBytes + (int64_t)2 * kMaxCtas * 16 * (head_dim + 2) * 4);
 }
 
 B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, float *lse, const void *cache, int64_t pages, int64_t page_size, const int32_t *page_table,
