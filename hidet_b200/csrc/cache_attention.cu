@@ -20,74 +20,19 @@
 #include <atomic>
 #include <type_traits>
 
-#include "serving.cuh"
-#include "umma.cuh"
+#include "cache_attention.cuh"
 
 namespace b200q {
+namespace cache_attention {
 namespace {
 
 constexpr unsigned int kKernelCacheAttention = 7;
-constexpr int kMaxCtas = 3 * 148;         // of a launch; the workspace is made for them
-constexpr int kCounterBytes = 65536 * 4;  // arrival counters in front of the workspace, zero between calls: kMaxCtas a level
-constexpr float kLn2 = 0.69314718055994531f;
-constexpr float kLog2e = 1.4426950408889634f;
-// Probabilities are kept 2^6 times as large, and a row's maximum is raised when a score passes it by 2^8 (rarely, behind its first
-// positions): with a value's scale below 2 that is at most 2^15 of f16's 2^16, and a probability of 2^-31 is still there, so that a long tail of
-// small ones is not lost.
-constexpr float kBias = 6.0f, kRise = 8.0f;
-constexpr float kLeastNormal = 1.1754943508222875e-38f;
 
-struct AttentionArgs {
-    const void *q;
-    int64_t q_token, q_head;
-    void *out;
-    float *lse;
-    const uint8_t *cache;
-    int64_t pages;
-    int page_size;
-    const int32_t *table;
-    int64_t table_stride;
-    int64_t capacity;  // positions that a row of the table covers
-    const int32_t *lengths, *starts;
-    int64_t tokens;    // all rows of q
-    int per_sequence;  // tokens of every sequence where starts is null
-    const uint8_t *mask;
-    int64_t mask_stride;
-    int mask_width;
-    int batch, kv_heads, group;
-    float scale_log2;
-    float *partial;
-    unsigned int *counters;
-    unsigned int *status;
-};
-
-// A key/value head of a sequence with some of its query rows, and the pieces that it is in.
-struct Item {
-    int head, row0, rows, token0;       // key/value head; first query row (token * group + head in group) and how many, -1: no more items; the sequence's first row of q
-    int length, fresh;                  // cached positions; of them those of the new tokens
-    int first_cta, last_cta, slot;      // who holds the pieces; the place of this CTA's
-};
 struct Tile {
     int key0;  // first position
     int last;  // of the item, in this CTA
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// Four bytes of code + 128 -> f16 pairs of codes (0x6400 | u is 1024 + u).
-__device__ __forceinline__ void codes_to_f16(uint32_t u, uint32_t &p01, uint32_t &p23) {
-    const uint32_t bias = 0x64806480u;
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(p01) : "r"(__byte_perm(u, 0x64646464u, 0x4140)), "r"(bias));
-    asm("sub.f16x2 %0, %1, %2;" : "=r"(p23) : "r"(__byte_perm(u, 0x64646464u, 0x4342)), "r"(bias));
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
     uint2 v;
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
@@ -104,17 +49,11 @@ __device__ __forceinline__ uint32_t transpose(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-
 constexpr int MOST_STAGES = 6;
-constexpr int kItemUnits = 2;           // what an item costs besides its tiles, in tiles
-constexpr int FAN = 8;                  // pieces of an item that are added at once
 constexpr int WARPS = 4;                // that multiply
 constexpr int CONSUMERS = 32 * WARPS;
 constexpr int THREADS = CONSUMERS + 32;
-constexpr int TILE = 16 * WARPS;        // positions
+static_assert(WARPS == RECORDS, "");
 
 template <int D, int NT>
 struct Layout {
@@ -134,24 +73,6 @@ struct Layout {
     static_assert(STAGES >= 2, "");
 };
 
-// One answer for the N threads that meet at named barrier 1: true where all of them bring true.
-template <int N>
-__device__ __forceinline__ bool all_of(bool ok) {
-    uint32_t all;
-    __syncwarp();
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p, q;\n\t"
-        "setp.ne.u32 p, %2, 0;\n\t"
-        "bar.red.and.pred q, 1, %1, p;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t"
-        "}\n"
-        : "=r"(all)
-        : "n"(N), "r"((uint32_t)ok)
-        : "memory");
-    return all != 0;
-}
-
 constexpr int ITEMS = 2;  // of which the consumers may know
 struct Control {
     uint64_t full[MOST_STAGES], empty[MOST_STAGES], item_full[ITEMS], item_empty[ITEMS];
@@ -170,33 +91,6 @@ __device__ __forceinline__ void load_q4(const T *p, float (&f)[4]) {
     for (int i = 0; i < 4; ++i) f[i] = Elems<T>::one(v[i]);
 }
 
-struct Sequence {
-    int length, fresh, token0;
-    int tiles;     // of one item
-    int row_tiles; // items of a key/value head
-};
-template <int ROWS>
-__device__ __forceinline__ Sequence sequence_of(const AttentionArgs &p, int b) {
-    Sequence s;
-    int64_t n = p.lengths[b];
-    if (n > p.capacity) {
-        n = p.capacity;
-        if (p.status != nullptr) atomicOr(p.status, kBadPage);
-    }
-    s.length = n < 0 ? 0 : (int)n;
-    if (p.starts != nullptr) {
-        const int64_t first = min(max((int64_t)p.starts[b], (int64_t)0), p.tokens), end = min(max((int64_t)p.starts[b + 1], first), p.tokens);
-        s.token0 = (int)first;
-        s.fresh = (int)(end - first);
-    } else {
-        s.token0 = b * p.per_sequence;
-        s.fresh = p.per_sequence;
-    }
-    s.tiles = max(1, (s.length + TILE - 1) / TILE);  // an empty sequence has a tile too: its rows are written
-    s.row_tiles = (s.fresh * p.group + ROWS - 1) / ROWS;
-    return s;
-}
-
 // The largest of the warps' maxima of a row.
 __device__ __forceinline__ float row_top(const Control &ctl, int r) {
     float n = -INFINITY;
@@ -205,107 +99,30 @@ __device__ __forceinline__ float row_top(const Control &ctl, int r) {
     return n;
 }
 
-// What becomes of an item whose sums stand in the merge buffers: the result, or a piece of it.  All consumers.  
+// What becomes of an item whose sums stand in the merge buffers: the result, or a piece of it.  All consumers.
 template <int D, int NT, typename T>
 __device__ __forceinline__ void finish_item(const AttentionArgs &p, Control &ctl, float *merge, const Item &item) {
     using L = Layout<D, NT>;
     constexpr int ROWS = L::ROWS;
     const bool whole = item.first_cta == item.last_cta;
-    float *part = p.partial + (int64_t)item.slot * ROWS * (D + 2);
-    constexpr int VECS = ROWS * D / 4;
-    auto write_out = [&](int r, int d, float4 v, float total_l, float top_log2) {
-        const int row = item.row0 + r, token = row / p.group, head = item.head * p.group + row - token * p.group;
-        const int64_t at = (int64_t)(item.token0 + token) * p.kv_heads * p.group + head;
-        const float inv = total_l == 0.0f ? 0.0f : 1.0f / total_l;
-        T y[4] = {Elems<T>::round(v.x * inv), Elems<T>::round(v.y * inv), Elems<T>::round(v.z * inv), Elems<T>::round(v.w * inv)};
-        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at * D + d) = *reinterpret_cast<const uint2 *>(y);
-        if (d == 0 && p.lse != nullptr) p.lse[at] = total_l == 0.0f ? -INFINITY : (top_log2 - kBias + __log2f(total_l)) * kLn2;
-    };
-    for (int i = threadIdx.x; i < VECS; i += CONSUMERS) {
+    float *piece = p.partial + (int64_t)item.slot * kPieceFloats<D, ROWS>;
+    for (int i = threadIdx.x; i < item.rows * (D / 4); i += CONSUMERS) {
         const int r = i / (D / 4), d = 4 * (i % (D / 4));
-        if (r >= item.rows) break;
         const float top = row_top(ctl, r), scale = ctl.q_scale[r];
-        float sum_l = 0.0f;
+        float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) sum_l += ctl.m[w][r] == -INFINITY ? ctl.l[w][r] : ctl.l[w][r] * ex2((ctl.m[w][r] - top) * scale);
+        for (int w = 0; w < WARPS; ++w) sum += ctl.m[w][r] == -INFINITY ? ctl.l[w][r] : ctl.l[w][r] * ex2((ctl.m[w][r] - top) * scale);
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int k = 0; k < L::BUFFERS; ++k) {
             const float4 x = *reinterpret_cast<const float4 *>(merge + k * (L::MERGE / 4) + r * L::PITCH + d);
             v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
         }
-        const float top_log2 = top * scale;
-        if (whole) {
-            write_out(r, d, v, sum_l, top_log2);
-        } else {
-            __stcg(reinterpret_cast<float4 *>(part + r * D + d), v);
-            if (d == 0) {
-                __stcg(part + ROWS * D + r, top_log2);
-                __stcg(part + ROWS * (D + 1) + r, sum_l);
-            }
-        }
+        if (whole) write_out<D, T>(p, item, r, d, v, sum, top * scale);
+        else write_piece<D, ROWS>(piece, r, d, v, sum, top * scale);
     }
-    // ---- the pieces of an item meet: FAN neighbours at a time, in the CTA that arrives last of them, then FAN of those ----
-    if (!whole) {
-        int k = blockIdx.x - item.first_cta, n = item.last_cta - item.first_cta + 1, stride = 1;
-        auto part_of = [&](int i) { return p.partial + (int64_t)(2 * (item.first_cta + i) + (i == 0 ? 1 : 0)) * ROWS * (D + 2); };
-        float (*part_m)[16] = reinterpret_cast<float (*)[16]>(merge), (*part_l)[16] = part_m + FAN;  // the merge buffers are free behind the next barrier
-        static_assert(L::BUFFERS * L::MERGE >= 2 * FAN * 16 * 4, "");
-        for (unsigned int *counters = p.counters;; counters += kMaxCtas, k /= FAN, n = (n + FAN - 1) / FAN, stride *= FAN) {
-            const int first = k / FAN * FAN, some = min(FAN, n - first);
-            // The last piece by itself is its own sum.  (It has no counter either: where it starts another item may have its first.)
-            if (some == 1) continue;
-            asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
-            if (threadIdx.x == 0) {
-                unsigned int *counter = counters + item.first_cta + first * stride;
-                unsigned int before;  // releases what the barrier put in front, the stores of all threads of the CTA
-                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
-                ctl.last = before == (unsigned int)(some - 1);
-                if (ctl.last) *counter = 0;
-            }
-            asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
-            if (!ctl.last) break;
-            for (int i = threadIdx.x; i < some * ROWS; i += CONSUMERS) {
-                const float *from = part_of((first + i / ROWS) * stride) + ROWS * D + i % ROWS;
-                const bool there = i % ROWS < item.rows;
-                part_m[i / ROWS][i % ROWS] = there ? __ldcg(from) : -INFINITY;
-                part_l[i / ROWS][i % ROWS] = there ? __ldcg(from + ROWS) : 0.0f;
-            }
-            const bool done = n <= FAN;
-            for (int i0 = 0; i0 < item.rows * (D / 4); i0 += CONSUMERS) {
-                const int i = i0 + threadIdx.x, r = i / (D / 4), d = 4 * (i % (D / 4));
-                float4 x[FAN];
-#pragma unroll
-                for (int j = 0; j < FAN; ++j)
-                    if (j < some && r < item.rows) x[j] = __ldcg(reinterpret_cast<const float4 *>(part_of((first + j) * stride) + r * D + d));
-                if (i0 == 0) asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
-                if (r >= item.rows) continue;
-                float top = -INFINITY, sum_l = 0.0f;
-#pragma unroll
-                for (int j = 0; j < FAN; ++j)
-                    if (j < some) top = fmaxf(top, part_m[j][r]);
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int j = 0; j < FAN; ++j)
-                    if (j < some) {
-                        const float by = part_m[j][r] == -INFINITY ? 1.0f : ex2(part_m[j][r] - top);
-                        sum_l = fmaf(part_l[j][r], by, sum_l);
-                        v.x = fmaf(x[j].x, by, v.x), v.y = fmaf(x[j].y, by, v.y), v.z = fmaf(x[j].z, by, v.z), v.w = fmaf(x[j].w, by, v.w);
-                    }
-                if (done) {
-                    write_out(r, d, v, sum_l, top);
-                } else {  // into the place of the first of them, whose statistics are in shared memory by now
-                    float *to = part_of(first * stride);
-                    __stcg(reinterpret_cast<float4 *>(to + r * D + d), v);
-                    if (d == 0) {
-                        __stcg(to + ROWS * D + r, top);
-                        __stcg(to + ROWS * (D + 1) + r, sum_l);
-                    }
-                }
-            }
-            if (done) break;
-        }
-    }
+    static_assert(L::BUFFERS * L::MERGE >= 2 * FAN * ROWS * 4, "");
+    if (!whole) meet<D, ROWS, CONSUMERS, 1, T>(p, item, threadIdx.x, merge, &ctl.last);  // whose first barrier frees the merge buffers
 }
 
 template <int D, int NT, typename T>
@@ -355,110 +172,33 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
             ++n_items;
         };
 
-        // ---- this CTA's piece of the line ----
-        int items = 0, tiles = 0;
-        for (int b = lane; b < p.batch; b += 32) {
-            const Sequence s = sequence_of<ROWS>(p, b);
-            items += s.row_tiles;
-            tiles += s.row_tiles * s.tiles;
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) {
-            items += __shfl_xor_sync(0xffffffffu, items, d);
-            tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
-        }
-        items *= p.kv_heads;
-        tiles *= p.kv_heads;
-        // No more pieces of an item than are added at once, as long as the wait for another round of additions, about two tiles, would be longer
-        // than what shorter pieces save.
-        int ctas = min((int)gridDim.x, tiles);
-        if (ctas > FAN * items && tiles / (FAN * max(1, items)) - tiles / ctas <= 2) ctas = FAN * items;
-        // Where pieces are long, a gap in front of every item stands for what it costs besides its tiles.
-        const int gap = tiles >= 8 * ctas ? kItemUnits : 0, units = tiles + items * gap;
-        const int each = units / max(1, ctas), more = units - each * ctas;  // the first `more` pieces have one unit more
-        auto piece = [&](int c) { return c * each + min(c, more); };
-        auto cta_of = [&](int unit) { return unit < more * (each + 1) ? unit / (each + 1) : more + (unit - more * (each + 1)) / each; };
-        int cur = 0, end = 0, b = 0, offset = 0;  // units; the sequence that cur lies in, and where in its items
-        if ((int)blockIdx.x < ctas && items > 0) {
-            cur = piece(blockIdx.x);
-            end = piece(blockIdx.x + 1);
-            for (int base = 0, b0 = 0;; b0 += 32) {
-                int own = 0;
-                if (b0 + lane < p.batch) {
-                    const Sequence s = sequence_of<ROWS>(p, b0 + lane);
-                    own = (s.tiles + gap) * s.row_tiles * p.kv_heads;
-                }
-                int until = own;
-#pragma unroll
-                for (int d = 1; d < 32; d *= 2) {
-                    const int below = __shfl_up_sync(0xffffffffu, until, d);
-                    if (lane >= d) until += below;
-                }
-                const uint32_t behind = __ballot_sync(0xffffffffu, base + until > cur);
-                if (behind != 0) {
-                    const int l = __ffs(behind) - 1;
-                    b = b0 + l;
-                    offset = cur - base - __shfl_sync(0xffffffffu, until - own, l);
-                    break;
-                }
-                base += __shfl_sync(0xffffffffu, until, 31);
-            }
-        }
-        const int begin = cur, records_per_page = p.page_size >> 4;
+        Line<ROWS> line(p, lane);
+        Item item;
+        const int32_t *table;
         int slot = 0, it = 0;
         uint32_t parity = 0;
-        while (cur < end && !dead) {
-            const Sequence s = sequence_of<ROWS>(p, b);
-            const int per = s.tiles + gap;
-            if (s.row_tiles == 0) {
-                ++b;
-                continue;
-            }
-            const int index = offset / per, head = index / s.row_tiles, rt = index - head * s.row_tiles;
-            const int item_begin = cur - (offset - index * per), tiles_begin = item_begin + gap, item_end = item_begin + per;
-            const int to = min(end, item_end), tile0 = max(cur, tiles_begin) - tiles_begin, n = to - tiles_begin - tile0;
-            const int32_t *pages = p.table + (int64_t)b * p.table_stride;
-            offset += to - cur;
-            cur = to;
-            if (offset == per * s.row_tiles * p.kv_heads) ++b, offset = 0;
-            if (n <= 0) continue;  // its tiles are another CTA's
-            // lane i brings the i-th page that the tile touches; its number is asked for one tile ahead
-            auto page_of = [&](int tile) {
-                const int page = tile * TILE / p.page_size + lane;
-                return tile < tile0 + n && lane <= WARPS && (int64_t)page * p.page_size < s.length ? pages[page] : 0;
-            };
-            int page = page_of(tile0);
-            publish({head, rt * ROWS, min(ROWS, s.fresh * p.group - rt * ROWS), s.token0, s.length, s.fresh, cta_of(tiles_begin), cta_of(item_end - 1),
-                     2 * (int)blockIdx.x + (tiles_begin >= begin ? 1 : 0)});
-            for (int i = 0; i < n && !dead; ++i) {
-                const int tile = tile0 + i, key0 = tile * TILE;
-                const int next = page_of(tile + 1);
+        while (!dead && line.next(item, table)) {
+            Pages pages(p, item, lane, table);
+            publish(item);
+            for (int i = 0; i < item.tiles && !dead; ++i) {
+                const int key0 = (item.tile0 + i) * TILE;
                 if (it >= STAGES) wait_for(ctl.empty[slot], parity ^ 1u);
                 if (dead) break;
-                const int keys = min(TILE, (s.length - key0 + 15) & ~15);  // 0 where the sequence is empty
                 const uint32_t bar = smem_u32(&ctl.full[slot]);
                 if (lane == 0) {
-                    ctl.tiles[slot] = {key0, i == n - 1};
+                    const int keys = copied_keys(item, key0);
+                    ctl.tiles[slot] = {key0, i == item.tiles - 1};
                     if (keys > 0) mbar_expect_tx(bar, (uint32_t)(keys >> 4) * L::RECORD);
                     else mbar_arrive(bar);
                 }
                 __syncwarp();
-                const int at = (key0 / p.page_size + lane) * p.page_size;  // first position of this lane's page
-                const int from = max(at, key0), until = min(at + p.page_size, key0 + keys);
-                if (lane <= WARPS && from < until) {
-                    if (page < 0 || page >= p.pages) {
-                        page = 0;
-                        if (p.status != nullptr) atomicOr(p.status, kBadPage);
-                    }
-                    const uint8_t *src = p.cache + (((int64_t)page * p.kv_heads + head) * records_per_page + ((from - at) >> 4)) * L::RECORD;
-                    bulk_load(stages + slot * L::STAGE + ((from - key0) >> 4) * L::RECORD, src, (uint32_t)((until - from) >> 4) * L::RECORD, bar);
-                }
-                page = next;
+                copy_tile<D>(p, item, pages, lane, key0, stages + slot * L::STAGE, bar);
                 ++it;
                 if (++slot == STAGES) slot = 0, parity ^= 1u;
             }
         }
-        if (!dead) publish({0, 0, -1, 0, 0, 0, 0, 0, 0});
+        item.rows = -1;
+        if (!dead) publish(item);
         if (dead) {  // nothing may be on its way when the CTA ends
             for (int back = 1; back <= STAGES && back <= it; ++back) {
                 const int at = it - back;
@@ -497,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[n_item % ITEMS]));
         if (item.rows < 0) break;
-        const int length = item.length, fresh = item.fresh;
+        const int length = item.length, hidden = first_hidden(p, item);
         float o[NT][D / 16][4];  // elements 16 i + g (0, 1) and + 8 (2, 3) of query rows 2t (0, 2) and 2t + 1 (1, 3)
         float m[NT][2], l[NT][2], shift[NT][2], qs[NT][2], rise[NT][2];  // shift: m, or 0 as long as nothing was seen
         float vref = 0.0f, v_inv = 0.0f, v_limit = kLeastNormal;  // a power of two, its reciprocal, and the first scale that is too large for it
@@ -541,7 +281,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
                     }
                 }
             }
-            asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
+            sync_of<CONSUMERS>();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -597,23 +337,18 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[nt][e] *= ks[e >> 1];
-                const int old = length - fresh;  // positions in front of the new tokens
-                const bool partly = key0 + 16 > (p.mask != nullptr ? old : min(old + 1, length));
+                const bool partly = key0 + 16 > hidden;
                 if (partly) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int pos = key0 + key_of_lane + 2 * h, drafted = pos - old;
+                        const int pos = key0 + key_of_lane + 2 * h;
                         if (pos >= length) vs[h] = 0.0f;
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                const int r = 8 * nt + 2 * t + e, token = (item.row0 + r) / p.group;
-                                bool seen = pos < length && r < item.rows;
-                                if (seen && drafted >= 0) {
-                                    seen = p.mask == nullptr ? drafted <= token : drafted < p.mask_width && p.mask[(int64_t)(item.token0 + token) * p.mask_stride + drafted] != 0;
-                                }
-                                if (!seen) s[nt][2 * h + e] = -INFINITY;
+                                const int r = 8 * nt + 2 * t + e;
+                                if (!may_see(p, item, r, (item.row0 + r) / p.group, pos)) s[nt][2 * h + e] = -INFINITY;
                             }
                     }
                 }
@@ -724,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
 #pragma unroll
                     for (int e = 0; e < 4; ++e) mine[(8 * nt + (e & 1)) * L::PITCH + 16 * n + 8 * (e >> 1)] = o[nt][n][e] * factor[nt][e & 1];
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
+        sync_of<CONSUMERS>();
         if (warp < L::BUFFERS) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -736,7 +471,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
                         *at = fmaf(o[nt][n][e], factor[nt][e & 1], *at);
                     }
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(CONSUMERS) : "memory");
+        sync_of<CONSUMERS>();
         finish_item<D, NT, T>(p, ctl, merge, item);
         // the merge buffers and statistics are written again only behind the barrier in front of the next item's queries
     }
@@ -750,7 +485,7 @@ int launch_sized(AttentionArgs p, cudaStream_t stream) {
     static std::atomic<bool> attr_set[64];
     const int rc = allow_smem(attr_set, kernel, L::SMEM);
     if (rc != B200Q_OK) return rc;
-    const int64_t tiles = p.kv_heads * (p.tokens * p.group / L::ROWS + p.batch) * (p.capacity / TILE + 1), at_once = L::PER_SM * (int64_t)sm_count();
+    const int64_t tiles = most_tiles(p, L::ROWS), at_once = L::PER_SM * (int64_t)sm_count();
     if (tiles > (1ll << 29)) return set_error(B200Q_UNSUPPORTED, "quantized_cache_attention: up to %lld tiles of %d rows and %d positions", (long long)tiles, L::ROWS, TILE);
     int64_t grid = tiles < at_once ? tiles : at_once;
     if (grid > kMaxCtas) grid = kMaxCtas;
@@ -771,12 +506,14 @@ int launch_typed(const AttentionArgs &p, int dim, cudaStream_t stream) {
 }
 
 }  // namespace
+}  // namespace cache_attention
 }  // namespace b200q
 
 extern "C" {
 
 B200Q_API size_t b200q_quantized_cache_attention_workspace_bytes(int64_t head_dim) {
     using namespace b200q;
+    using namespace b200q::cache_attention;
     if (!cache_dim(head_dim)) return 0;
     return (size_t)(kCounterBytes + (int64_t)2 * kMaxCtas * 16 * (head_dim + 2) * 4);
 }
@@ -786,6 +523,7 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
                                               int64_t mask_stride, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, int type,
                                               void *workspace, size_t workspace_bytes, void *stream) {
     using namespace b200q;
+    using namespace b200q::cache_attention;
     const char *op = "quantized_cache_attention";
     if (batch < 0 || tokens < 0 || table_width < 0 || mask_width < 0) return set_error(B200Q_INVALID_ARGUMENT, "%s: negative size", op);
     if (type != B200Q_F16 && type != B200Q_BF16) return set_error(B200Q_UNSUPPORTED, "%s: float type %d: float16 and bfloat16 are supported", op, type);

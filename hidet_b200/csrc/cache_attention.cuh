@@ -1,0 +1,368 @@
+// What the two kernels of attention over the quantized cache share: their arguments, the line of tiles and its pieces, the copies of a tile's
+// records, and the sum of an item's pieces.
+#pragma once
+
+#include "serving.cuh"
+#include "umma.cuh"
+
+namespace b200q {
+namespace cache_attention {
+
+constexpr int kMaxCtas = 3 * 148;         // of a launch; the workspace is made for them
+constexpr int kCounterBytes = 65536 * 4;  // arrival counters in front of the workspace, zero between calls: kMaxCtas a round of additions
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr float kLog2e = 1.4426950408889634f;
+// Probabilities are kept 2^6 times as large, and a row's maximum is raised when a score passes it by 2^8 (rarely, behind its first
+// positions): with a value's scale below 2 that is at most 2^15 of f16's 2^16, and a probability of 2^-31 is still there, so that a long tail of
+// small ones is not lost.
+constexpr float kBias = 6.0f, kRise = 8.0f;
+constexpr float kLeastNormal = 1.1754943508222875e-38f;
+
+constexpr int TILE = 64;       // positions: four records
+constexpr int RECORDS = 4;
+constexpr int kItemUnits = 2;  // what an item costs besides its tiles, in tiles
+constexpr int FAN = 8;         // pieces of an item that are added at once
+
+struct AttentionArgs {
+    const void *q;
+    int64_t q_token, q_head;
+    void *out;
+    float *lse;
+    const uint8_t *cache;
+    int64_t pages;
+    int page_size;
+    const int32_t *table;
+    int64_t table_stride;
+    int64_t capacity;  // positions that a row of the table covers
+    const int32_t *lengths, *starts;
+    int64_t tokens;    // all rows of q
+    int per_sequence;  // tokens of every sequence where starts is null
+    const uint8_t *mask;
+    int64_t mask_stride;
+    int mask_width;
+    int batch, kv_heads, group;
+    float scale_log2;
+    float *partial;
+    unsigned int *counters;
+    unsigned int *status;
+};
+
+// At most this many tiles of `rows` query rows.
+inline int64_t most_tiles(const AttentionArgs &p, int rows) { return p.kv_heads * (p.tokens * p.group / rows + p.batch) * (p.capacity / TILE + 1); }
+// More than 16 query rows a key/value head, on average, of 64 or 128 elements: tiles of 128 rows on tcgen05 (cache_attention_wide.cu).
+inline bool wide_rows(int64_t tokens, int64_t group, int64_t batch, int64_t dim) { return (dim == 64 || dim == 128) && tokens * group > 16 * batch; }
+int launch_wide(const AttentionArgs &p, int dim, bool bf16, cudaStream_t stream);
+
+#ifdef __CUDACC__
+
+// A key/value head of a sequence with some of its query rows, and the pieces that it is in.
+struct Item {
+    int head, row0, rows, token0;   // key/value head; first query row (token * group + head in group) and how many, -1: no more items; the sequence's first row of q
+    int length, fresh;              // cached positions; of them those of the new tokens
+    int first_cta, last_cta, slot;  // who holds the pieces; the place of this CTA's
+    int tile0, tiles;               // of this piece
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Four bytes of code + 128 -> f16 pairs of codes (0x6400 | u is 1024 + u).
+__device__ __forceinline__ void codes_to_f16(uint32_t u, uint32_t &p01, uint32_t &p23) {
+    const uint32_t bias = 0x64806480u;
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(p01) : "r"(__byte_perm(u, 0x64646464u, 0x4140)), "r"(bias));
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(p23) : "r"(__byte_perm(u, 0x64646464u, 0x4342)), "r"(bias));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void sync_of() {
+    asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
+}
+// One answer for the N threads that meet at named barrier 1: true where all of them bring true.
+template <int N>
+__device__ __forceinline__ bool all_of(bool ok) {
+    uint32_t all;
+    __syncwarp();
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %2, 0;\n\t"
+        "bar.red.and.pred q, 1, %1, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t"
+        "}\n"
+        : "=r"(all)
+        : "n"(N), "r"((uint32_t)ok)
+        : "memory");
+    return all != 0;
+}
+
+struct Sequence {
+    int length, fresh, token0;
+    int tiles;      // of one item
+    int row_tiles;  // items of a key/value head
+};
+template <int ROWS>
+__device__ __forceinline__ Sequence sequence_of(const AttentionArgs &p, int b) {
+    Sequence s;
+    int64_t n = p.lengths[b];
+    if (n > p.capacity) {
+        n = p.capacity;
+        if (p.status != nullptr) atomicOr(p.status, kBadPage);
+    }
+    s.length = n < 0 ? 0 : (int)n;
+    if (p.starts != nullptr) {
+        const int64_t first = min(max((int64_t)p.starts[b], (int64_t)0), p.tokens), end = min(max((int64_t)p.starts[b + 1], first), p.tokens);
+        s.token0 = (int)first;
+        s.fresh = (int)(end - first);
+    } else {
+        s.token0 = b * p.per_sequence;
+        s.fresh = p.per_sequence;
+    }
+    s.tiles = max(1, (s.length + TILE - 1) / TILE);  // an empty sequence has a tile too: its rows are written
+    s.row_tiles = (s.fresh * p.group + ROWS - 1) / ROWS;
+    return s;
+}
+
+// This CTA's piece of the line of tiles: a sequence's items one behind the other, head by head, and the sequences behind one another.  One warp.
+template <int ROWS>
+struct Line {
+    const AttentionArgs &p;
+    const int lane;
+    int each = 0, more = 0, gap = 0;            // units of a piece; the first `more` pieces have one more; units in front of an item's tiles
+    int begin = 0, cur = 0, end = 0;            // units
+    int b = 0, offset = 0;                      // the sequence that cur lies in, and where in its items
+
+    __device__ __forceinline__ int piece(int c) const { return c * each + min(c, more); }
+    __device__ __forceinline__ int cta_of(int unit) const { return unit < more * (each + 1) ? unit / (each + 1) : more + (unit - more * (each + 1)) / each; }
+
+    __device__ __forceinline__ Line(const AttentionArgs &args, int lane_) : p(args), lane(lane_) {
+        int items = 0, tiles = 0;
+        for (int s0 = lane; s0 < p.batch; s0 += 32) {
+            const Sequence s = sequence_of<ROWS>(p, s0);
+            items += s.row_tiles;
+            tiles += s.row_tiles * s.tiles;
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) {
+            items += __shfl_xor_sync(0xffffffffu, items, d);
+            tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
+        }
+        items *= p.kv_heads;
+        tiles *= p.kv_heads;
+        // No more pieces of an item than are added at once, as long as the wait for another round of additions, about two tiles, would be longer
+        // than what shorter pieces save.
+        int ctas = min((int)gridDim.x, tiles);
+        if (ctas > FAN * items && tiles / (FAN * max(1, items)) - tiles / ctas <= 2) ctas = FAN * items;
+        if ((int)blockIdx.x >= ctas) return;
+        // Where pieces are long, a gap in front of every item stands for what it costs besides its tiles.
+        gap = tiles >= 8 * ctas ? kItemUnits : 0;
+        const int units = tiles + items * gap;
+        each = units / ctas;
+        more = units - each * ctas;
+        begin = cur = piece(blockIdx.x);
+        end = piece(blockIdx.x + 1);
+        for (int base = 0, b0 = 0;; b0 += 32) {
+            int own = 0;
+            if (b0 + lane < p.batch) {
+                const Sequence s = sequence_of<ROWS>(p, b0 + lane);
+                own = (s.tiles + gap) * s.row_tiles * p.kv_heads;
+            }
+            int until = own;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int below = __shfl_up_sync(0xffffffffu, until, d);
+                if (lane >= d) until += below;
+            }
+            const uint32_t behind = __ballot_sync(0xffffffffu, base + until > cur);
+            if (behind != 0) {
+                const int l = __ffs(behind) - 1;
+                b = b0 + l;
+                offset = cur - base - __shfl_sync(0xffffffffu, until - own, l);
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, until, 31);
+        }
+    }
+
+    // The next item with tiles in this piece, and its sequence's pages; false behind the last.
+    __device__ __forceinline__ bool next(Item &item, const int32_t *&pages) {
+        while (cur < end) {
+            const Sequence s = sequence_of<ROWS>(p, b);
+            if (s.row_tiles == 0) {
+                ++b;
+                continue;
+            }
+            const int per = s.tiles + gap, index = offset / per;
+            const int item_begin = cur - (offset - index * per), tiles_begin = item_begin + gap, item_end = item_begin + per, to = min(end, item_end);
+            item.head = index / s.row_tiles;
+            item.row0 = (index - item.head * s.row_tiles) * ROWS;
+            item.rows = min(ROWS, s.fresh * p.group - item.row0);
+            item.token0 = s.token0;
+            item.length = s.length;
+            item.fresh = s.fresh;
+            item.first_cta = cta_of(tiles_begin);
+            item.last_cta = cta_of(item_end - 1);
+            item.slot = 2 * (int)blockIdx.x + (tiles_begin >= begin ? 1 : 0);  // only its first piece can begin in this CTA, and only the first item here have begun before
+            item.tile0 = max(cur, tiles_begin) - tiles_begin;
+            item.tiles = to - tiles_begin - item.tile0;
+            pages = p.table + (int64_t)b * p.table_stride;
+            offset += to - cur;
+            cur = to;
+            if (offset == per * s.row_tiles * p.kv_heads) ++b, offset = 0;
+            if (item.tiles > 0) return true;  // else they are another CTA's
+        }
+        item.rows = -1;
+        return false;
+    }
+};
+
+// The pages of an item's tiles: lane i < 5 has the number of the i-th page that a tile touches, asked for one tile ahead.
+struct Pages {
+    const int32_t *pages;
+    int end, page;  // behind the item's last tile here; of the next tile
+    __device__ __forceinline__ int of(const AttentionArgs &p, const Item &item, int lane, int tile) const {
+        const int i = tile * TILE / p.page_size + lane;
+        return tile < end && lane <= RECORDS && (int64_t)i * p.page_size < item.length ? pages[i] : 0;
+    }
+    __device__ __forceinline__ Pages(const AttentionArgs &p, const Item &item, int lane, const int32_t *table) : pages(table), end(item.tile0 + item.tiles) { page = of(p, item, lane, item.tile0); }
+};
+// Positions of a tile that are copied, whole records; 0 where the sequence is empty.
+__device__ __forceinline__ int copied_keys(const Item &item, int key0) { return min(TILE, (item.length - key0 + 15) & ~15); }
+// Brings a tile's records, one bulk copy for each page.
+template <int D>
+__device__ __forceinline__ void copy_tile(const AttentionArgs &p, const Item &item, Pages &pages, int lane, int key0, uint32_t dst, uint32_t bar) {
+    int page = pages.page;
+    pages.page = pages.of(p, item, lane, key0 / TILE + 1);
+    const int at = (key0 / p.page_size + lane) * p.page_size;  // first position of this lane's page
+    const int from = max(at, key0), until = min(at + p.page_size, key0 + copied_keys(item, key0));
+    if (lane <= RECORDS && from < until) {
+        if (page < 0 || page >= p.pages) {
+            page = 0;
+            if (p.status != nullptr) atomicOr(p.status, kBadPage);
+        }
+        const uint8_t *src = p.cache + (((int64_t)page * p.kv_heads + item.head) * (p.page_size >> 4) + ((from - at) >> 4)) * record_bytes(D);
+        bulk_load(dst + ((from - key0) >> 4) * record_bytes(D), src, (uint32_t)((until - from) >> 4) * record_bytes(D), bar);
+    }
+}
+
+// Whether query row r of the item may see a position.
+__device__ __forceinline__ bool may_see(const AttentionArgs &p, const Item &item, int r, int token, int pos) {
+    const int drafted = pos - (item.length - item.fresh);
+    if (pos >= item.length || r >= item.rows) return false;
+    if (drafted < 0) return true;
+    if (p.mask == nullptr) return drafted <= token;
+    return drafted < p.mask_width && p.mask[(int64_t)(item.token0 + token) * p.mask_stride + drafted] != 0;
+}
+// Positions from here on may be hidden from a row.
+__device__ __forceinline__ int first_hidden(const AttentionArgs &p, const Item &item) {
+    const int old = item.length - item.fresh;
+    return p.mask != nullptr ? old : min(old + 1, item.length);
+}
+
+// Four elements of a query row's result, from the sum of its values and of its probabilities, both in units of 2^top.
+template <int D, typename T>
+__device__ __forceinline__ void write_out(const AttentionArgs &p, const Item &item, int r, int d, float4 v, float sum, float top) {
+    const int row = item.row0 + r, token = row / p.group, head = item.head * p.group + row - token * p.group;
+    const int64_t at = (int64_t)(item.token0 + token) * p.kv_heads * p.group + head;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T y[4] = {Elems<T>::round(v.x * inv), Elems<T>::round(v.y * inv), Elems<T>::round(v.z * inv), Elems<T>::round(v.w * inv)};
+    *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at * D + d) = *reinterpret_cast<const uint2 *>(y);
+    if (d == 0 && p.lse != nullptr) p.lse[at] = sum == 0.0f ? -INFINITY : (top - kBias + __log2f(sum)) * kLn2;
+}
+
+// A piece in the workspace: [ROWS][D] sums of values, then the rows' units (log2) and sums of probabilities.
+template <int D, int ROWS>
+constexpr int kPieceFloats = ROWS * (D + 2);
+template <int D, int ROWS>
+__device__ __forceinline__ void write_piece(float *piece, int r, int d, float4 v, float sum, float top) {
+    __stcg(reinterpret_cast<float4 *>(piece + r * D + d), v);
+    if (d == 0) {
+        __stcg(piece + ROWS * D + r, top);
+        __stcg(piece + ROWS * (D + 1) + r, sum);
+    }
+}
+
+// The sum of `some` pieces for this thread's groups of four elements, GROUPS of them with their loads in flight together.  tops, sums: of the
+// pieces' rows, [FAN][ROWS], filled by all threads in front of the barrier behind the first loads.
+template <int D, int ROWS, int N, int GROUPS, typename T, typename PieceOf>
+__device__ __forceinline__ void add_pieces(const AttentionArgs &p, const Item &item, const float *tops, const float *sums, int tid, int some, bool done, PieceOf piece_of) {
+    bool waited = false;
+    for (int i0 = tid; i0 < item.rows * (D / 4) || !waited; i0 += GROUPS * N) {
+        float4 x[GROUPS][FAN];
+#pragma unroll
+        for (int u = 0; u < GROUPS; ++u) {
+            const int i = i0 + u * N, r = i / (D / 4), d = 4 * (i % (D / 4));
+#pragma unroll
+            for (int j = 0; j < FAN; ++j)
+                if (j < some && r < item.rows) x[u][j] = __ldcg(reinterpret_cast<const float4 *>(p.partial + (piece_of(j) + r * D + d)));
+        }
+        if (!waited) sync_of<N>();
+        waited = true;
+#pragma unroll
+        for (int u = 0; u < GROUPS; ++u) {
+            const int i = i0 + u * N, r = i / (D / 4), d = 4 * (i % (D / 4));
+            if (r >= item.rows) continue;
+            float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < FAN; ++j)
+                if (j < some) top = fmaxf(top, tops[j * ROWS + r]);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < FAN; ++j)
+                if (j < some) {
+                    const float own = tops[j * ROWS + r], by = own == -INFINITY ? 1.0f : ex2(own - top);
+                    sum = fmaf(sums[j * ROWS + r], by, sum);
+                    v.x = fmaf(x[u][j].x, by, v.x), v.y = fmaf(x[u][j].y, by, v.y), v.z = fmaf(x[u][j].z, by, v.z), v.w = fmaf(x[u][j].w, by, v.w);
+                }
+            if (done) write_out<D, T>(p, item, r, d, v, sum, top);
+            else write_piece<D, ROWS>(p.partial + piece_of(0), r, d, v, sum, top);  // into the place of the first of them, whose rows' units and sums are in shared memory by now
+        }
+    }
+}
+
+// The pieces of an item meet: FAN neighbours at a time, in the CTA that arrives last of them, then FAN of those.  N threads, which have written this
+// CTA's piece; scratch: 2 * FAN * ROWS floats.
+template <int D, int ROWS, int N, int GROUPS, typename T>
+__device__ __forceinline__ void meet(const AttentionArgs &p, const Item &item, int tid, float *scratch, int *last) {
+    int k = blockIdx.x - item.first_cta, n = item.last_cta - item.first_cta + 1, stride = 1;
+    auto place = [&](int i) { return (2 * (item.first_cta + i) + (i == 0 ? 1 : 0)) * kPieceFloats<D, ROWS>; };  // 32 bits are enough for the workspace
+    float *tops = scratch, *sums = scratch + FAN * ROWS;
+    for (unsigned int *counters = p.counters;; counters += kMaxCtas, k /= FAN, n = (n + FAN - 1) / FAN, stride *= FAN) {
+        const int first = k / FAN * FAN, some = min(FAN, n - first);
+        // The last piece by itself is its own sum.  (It has no counter either: where it starts another item may have its first.)
+        if (some == 1) continue;
+        sync_of<N>();
+        if (tid == 0) {
+            unsigned int *counter = counters + item.first_cta + first * stride;
+            unsigned int before;  // releases what the barrier put in front, the stores of all threads of the CTA
+            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+            *last = before == (unsigned int)(some - 1);
+            if (*last) *counter = 0;
+        }
+        sync_of<N>();
+        if (!*last) break;
+        auto piece_of = [&](int j) { return place((first + j) * stride); };
+        for (int i = tid; i < some * ROWS; i += N) {
+            const int j = i / ROWS, r = i % ROWS;
+            const float *from = p.partial + piece_of(j) + ROWS * D + r;
+            tops[i] = r < item.rows ? __ldcg(from) : -INFINITY;
+            sums[i] = r < item.rows ? __ldcg(from + ROWS) : 0.0f;
+        }
+        const bool done = n <= FAN;
+        add_pieces<D, ROWS, N, GROUPS, T>(p, item, tops, sums, tid, some, done, piece_of);
+        if (done) break;
+    }
+}
+
+#endif  // __CUDACC__
+
+}  // namespace cache_attention
+}  // namespace b200q
