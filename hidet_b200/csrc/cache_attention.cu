@@ -1,4 +1,5 @@
-// Attention of new tokens (one a sequence, several, or a tree of drafted ones) over the quantized, paged key/value cache.
+// Attention of new tokens (one a sequence, several, or a tree of drafted ones) over the quantized, paged key/value cache: the entry point, and the kernel
+// for few query rows a key/value head, decoding above all.  (cache_attention_wide.cu: for many.)
 //
 // For query row i (a token and one of the `group` heads that share a key/value head) and position j:
 //     s_ij = scale * (q_i . kcode_j) * kscale_j,     o_i = sum_j exp(s_ij - m_i) * vscale_j * vcode_j / sum_j exp(s_ij - m_i)
@@ -18,7 +19,6 @@
 // instruction and multiplies, with the codes as the 16-row operand (positions of K, elements of V) and eight query rows as columns.  With the positions
 // (and not the rows) shared out among the warps, each code is converted once per CTA.
 #include <atomic>
-#include <type_traits>
 
 #include "cache_attention.cuh"
 
@@ -511,11 +511,13 @@ int launch_typed(const AttentionArgs &p, int dim, cudaStream_t stream) {
 
 extern "C" {
 
-B200Q_API size_t b200q_quantized_cache_attention_workspace_bytes(int64_t head_dim) {
+B200Q_API size_t b200q_quantized_cache_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
     using namespace b200q;
     using namespace b200q::cache_attention;
-    if (!cache_dim(head_dim)) return 0;
-    return (size_t)(kCounterBytes + (int64_t)2 * kMaxCtas * 16 * (head_dim + 2) * 4);
+    if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || !cache_dim(head_dim)) return 0;
+    const bool wide = wide_rows(tokens, heads / kv_heads, batch, head_dim);
+    const int64_t pieces = 2 * (wide ? kMostWideCtas : kMaxCtas), rows = wide ? 128 : 16;
+    return (size_t)(kCounterBytes + pieces * rows * (head_dim + 2) * 4);
 }
 
 B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, float *lse, const void *cache, int64_t pages, int64_t page_size, const int32_t *page_table,
@@ -545,7 +547,7 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
     if (!aligned_to(cache, 16) || !aligned_to(q->data, 8) || !aligned_to(out, 8) || q->token_stride % 4 != 0 || q->head_stride % 4 != 0) {
         return set_error(B200Q_INVALID_ARGUMENT, "%s: a 16-byte aligned cache, 8-byte aligned q and out and strides of 4 elements are wanted", op);
     }
-    const size_t need = b200q_quantized_cache_attention_workspace_bytes(head_dim);
+    const size_t need = b200q_quantized_cache_attention_workspace_bytes(batch, tokens, heads, kv_heads, head_dim);
     if (workspace == nullptr || workspace_bytes < need) return set_error(B200Q_WORKSPACE_TOO_SMALL, "%s: a workspace of %zu bytes is needed, got %zu", op, need, workspace_bytes);
     if (!aligned_to(workspace, 16)) return set_error(B200Q_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", op);
     AttentionArgs p = {};
@@ -576,6 +578,7 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
     p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kCounterBytes);
     p.status = device_status_word();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (wide_rows(tokens, heads / kv_heads, batch, head_dim)) return launch_wide(p, (int)head_dim, type == B200Q_BF16, s);
     return type == B200Q_F16 ? launch_typed<__half>(p, (int)head_dim, s) : launch_typed<__nv_bfloat16>(p, (int)head_dim, s);
 }
 

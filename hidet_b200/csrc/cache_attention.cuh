@@ -2,6 +2,8 @@
 // records, and the sum of an item's pieces.
 #pragma once
 
+#include <type_traits>
+
 #include "serving.cuh"
 #include "umma.cuh"
 
@@ -9,6 +11,7 @@ namespace b200q {
 namespace cache_attention {
 
 constexpr int kMaxCtas = 3 * 148;         // of a launch; the workspace is made for them
+constexpr int kMostWideCtas = 148;        // of the kernel for many rows
 constexpr int kCounterBytes = 65536 * 4;  // arrival counters in front of the workspace, zero between calls: kMaxCtas a round of additions
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -318,9 +321,10 @@ __device__ __forceinline__ void add_pieces(const AttentionArgs &p, const Item &i
 #pragma unroll
             for (int j = 0; j < FAN; ++j)
                 if (j < some) {
-                    const float own = tops[j * ROWS + r], by = own == -INFINITY ? 1.0f : ex2(own - top);
-                    sum = fmaf(sums[j * ROWS + r], by, sum);
-                    v.x = fmaf(x[u][j].x, by, v.x), v.y = fmaf(x[u][j].y, by, v.y), v.z = fmaf(x[u][j].z, by, v.z), v.w = fmaf(x[u][j].w, by, v.w);
+                    // in two steps: units may lie so far apart that the whole factor leaves float's range where the products do not
+                    const float own = tops[j * ROWS + r], by = own == -INFINITY ? 1.0f : ex2(0.5f * (own - top));
+                    sum = fmaf(sums[j * ROWS + r] * by, by, sum);
+                    v.x = fmaf(x[u][j].x * by, by, v.x), v.y = fmaf(x[u][j].y * by, by, v.y), v.z = fmaf(x[u][j].z * by, by, v.z), v.w = fmaf(x[u][j].w * by, by, v.w);
                 }
             if (done) write_out<D, T>(p, item, r, d, v, sum, top);
             else write_piece<D, ROWS>(p.partial + piece_of(0), r, d, v, sum, top);  // into the place of the first of them, whose rows' units and sums are in shared memory by now

@@ -1,0 +1,556 @@
+// Attention over the quantized cache where many query rows share a key/value head (trees of drafted tokens, grouped heads, short prompts): the products
+// on tcgen05, 128 rows at a time.
+//
+// As in cache_attention.cu the tiles of all items stand in one line that is cut into equal pieces, one a CTA, one CTA an SM.  Inside a CTA:
+//   one warp plans and copies records (codes and scales) into a ring;
+//   four warps convert a tile's codes to f16, each one record: K as it lies, [position][element], V through transposing matrix loads as
+//       [element][position], both in the 128-byte swizzle, so that both are K-major operands;
+//   one thread issues S = Q K^T (128 x 64) and O += P V (128 x D), sums in tensor memory;
+//   two groups of four warps turn scores into probabilities, a thread a row, alternate tiles: each group has its own S, P, O, maxima and sums, which
+//       meet at the end of the item.
+// The probabilities go back into tensor memory as the first operand of the second product.  A thread has a whole row of 64 scores, so maximum and sum
+// need no exchange.  A row's unit is 2^u: u is its running maximum (in log2) plus the exponent of the largest value scale so far, so that the products with
+// value scales fit f16 and sums of probabilities and of values are in the same unit.
+//
+// Bound by instructions: per tile and row about 470 of them for 64 scores, and 700 a warp for the conversion of a tile's 16 K codes.
+#include "cache_attention.cuh"
+
+namespace b200q {
+namespace cache_attention {
+namespace {
+
+constexpr unsigned int kKernelCacheAttentionWide = 9;
+
+constexpr int ROWS = 128;
+constexpr int GROUP_WARPS = 4;                  // of a group that turns scores into probabilities
+constexpr int SOFTMAX_THREADS = 2 * 32 * GROUP_WARPS;
+constexpr int CONVERT_WARP0 = 8, PRODUCER_WARP = 12, MMA_WARP = 13;
+constexpr int THREADS = 32 * 16;                // four groups of four warps, for the split of the registers
+// Registers a thread of the groups: softmax (two groups), conversion, the rest.  Together what the block is launched with.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 192, kConvertRegs = 72, kOtherRegs = 56;
+static_assert(2 * kSoftmaxRegs + kConvertRegs + kOtherRegs <= 4 * kLaunchRegs, "");
+template <int N>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+constexpr int ITEMS = 2;                        // that the other roles may know of
+constexpr int RAW_STAGES = 4, KV_STAGES = 3;
+constexpr uint32_t TMEM_COLS = 512;
+// columns of a group's scores, probabilities and sums
+__device__ __forceinline__ constexpr uint32_t s_col(int group) { return 64 * group; }
+__device__ __forceinline__ constexpr uint32_t p_col(int group) { return 128 + 32 * group; }
+__device__ __forceinline__ constexpr uint32_t o_col(int group) { return 192 + 128 * group; }
+constexpr float kLeastUnit = -90.0f;            // exponents of value scales below are not followed: sums in that unit stay in float's range
+
+template <int D>
+struct Layout {
+    static constexpr int Q = ROWS * D * 2;
+    static constexpr int K = TILE * D * 2, V = D * TILE * 2, KV = K + V;
+    static constexpr int RAW = RECORDS * record_bytes(D);
+    static constexpr int KV_AT = Q, RAW_AT = Q + KV_STAGES * KV;
+    static constexpr int SMEM = RAW_AT + RAW_STAGES * RAW + 1024;  // 1024: the operands begin at a multiple of it
+    static_assert(2 * FAN * ROWS * 4 <= Q, "");
+};
+
+// Four scales, read where this stands: ahead of their use they would take as many registers as the scores.
+__device__ __forceinline__ float4 scales_at(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
+}
+
+struct Control {
+    uint64_t raw_full[RAW_STAGES], raw_empty[RAW_STAGES], kv_full[KV_STAGES], kv_empty[KV_STAGES], item_full[ITEMS], item_empty[ITEMS];
+    uint64_t q_full, s_full[2], s_empty[2], p_full[2], pv_done[2], drained;
+    float k_scale[KV_STAGES][TILE], v_scale[KV_STAGES][TILE], v_top[KV_STAGES][RECORDS];
+    int key0[RAW_STAGES], length[RAW_STAGES];  // length -1: no more tiles
+    Item items[ITEMS];
+    float top[2][ROWS], unit[2][ROWS], sum[2][ROWS];
+    int abort, last;
+    uint32_t tmem;
+};
+
+template <int D, typename T>
+__global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const __grid_constant__ AttentionArgs p) {
+    using L = Layout<D>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Control ctl;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem_gen = smem_raw + (smem - smem_u32(smem_raw));
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < RAW_STAGES; ++i) mbar_init(smem_u32(&ctl.raw_full[i]), 1), mbar_init(smem_u32(&ctl.raw_empty[i]), RECORDS);
+        for (int i = 0; i < KV_STAGES; ++i) mbar_init(smem_u32(&ctl.kv_full[i]), RECORDS), mbar_init(smem_u32(&ctl.kv_empty[i]), 1);
+        for (int i = 0; i < ITEMS; ++i) mbar_init(smem_u32(&ctl.item_full[i]), 1), mbar_init(smem_u32(&ctl.item_empty[i]), 2 * GROUP_WARPS + 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&ctl.s_full[i]), 1), mbar_init(smem_u32(&ctl.s_empty[i]), GROUP_WARPS);
+            mbar_init(smem_u32(&ctl.p_full[i]), GROUP_WARPS), mbar_init(smem_u32(&ctl.pv_done[i]), 1);
+        }
+        mbar_init(smem_u32(&ctl.q_full), 2 * GROUP_WARPS);
+        mbar_init(smem_u32(&ctl.drained), 1);
+        ctl.abort = 0;
+        mbar_fence_init();
+    }
+    // Tensor memory is taken when the kernel in front is over (its CTAs that have yet to begin may need it) and before any kernel behind may begin.
+    pdl_wait();
+    if (warp == MMA_WARP) {
+        umma::alloc(smem_u32(&ctl.tmem), TMEM_COLS);
+        umma::relinquish();
+        umma::fence_before_sync();
+    }
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = ctl.tmem;
+
+    auto wait_one = [&](uint64_t &barrier, uint32_t parity, unsigned int site) -> bool {  // one thread's
+        // inline, unlike the other kernels' (a call in a kernel whose groups have registers of their own is not compiled)
+        const uint32_t bar = smem_u32(&barrier);
+        if (mbar_wait(bar, parity, umma::kFastPolls)) return true;
+#pragma unroll 1
+        for (uint32_t round = 0; round < kSpinLimit / 1024u; ++round) {
+            if (mbar_wait(bar, parity, 1024u)) return true;
+            if (*reinterpret_cast<volatile int *>(&ctl.abort) != 0) return false;
+        }
+        report_timeout(p.status, kKernelCacheAttentionWide, site);
+        atomicExch(&ctl.abort, 1);
+        return false;
+    };
+    auto wait = [&](uint64_t &barrier, uint32_t parity, unsigned int site) -> bool { return __all_sync(0xffffffffu, wait_one(barrier, parity, site)); };
+
+    if (warp >= PRODUCER_WARP) {
+        fewer_registers<kOtherRegs>();
+        if (warp == PRODUCER_WARP) {
+            // ---------------- plan and copies ----------------
+            pdl_launch_dependents();
+            Line<ROWS> line(p, lane);
+            Item item;
+            const int32_t *table;
+            int n_items = 0, it = 0, slot = 0;
+            uint32_t parity = 0;
+            bool ok = true;
+            auto publish = [&]() {
+                const int at = n_items % ITEMS;
+                if (n_items >= ITEMS) ok = wait(ctl.item_empty[at], (n_items / ITEMS - 1) & 1, 1);
+                if (ok && lane == 0) {
+                    ctl.items[at] = item;
+                    mbar_arrive(smem_u32(&ctl.item_full[at]));
+                }
+                ++n_items;
+            };
+            while (ok && line.next(item, table)) {
+                Pages pages(p, item, lane, table);
+                publish();
+                for (int i = 0; ok && i < item.tiles; ++i) {
+                    const int key0 = (item.tile0 + i) * TILE;
+                    if (it >= RAW_STAGES) ok = wait(ctl.raw_empty[slot], parity ^ 1u, 2);
+                    if (!ok) break;
+                    const uint32_t bar = smem_u32(&ctl.raw_full[slot]);
+                    if (lane == 0) {
+                        const int keys = copied_keys(item, key0);
+                        ctl.key0[slot] = key0;
+                        ctl.length[slot] = item.length;
+                        if (keys > 0) mbar_expect_tx(bar, (uint32_t)(keys >> 4) * record_bytes(D));
+                        else mbar_arrive(bar);
+                    }
+                    __syncwarp();
+                    copy_tile<D>(p, item, pages, lane, key0, smem + L::RAW_AT + slot * L::RAW, bar);
+                    ++it;
+                    if (++slot == RAW_STAGES) slot = 0, parity ^= 1u;
+                }
+            }
+            item.rows = -1;
+            if (ok) publish();
+            if (ok && it >= RAW_STAGES) ok = wait(ctl.raw_empty[slot], parity ^ 1u, 3);
+            if (ok && lane == 0) {
+                ctl.length[slot] = -1;
+                mbar_arrive(smem_u32(&ctl.raw_full[slot]));
+            }
+            if (!ok) {  // nothing may be on its way when the CTA ends
+                for (int back = 1; back <= RAW_STAGES && back <= it; ++back) {
+                    const int at = it - back;
+                    mbar_wait(smem_u32(&ctl.raw_full[at % RAW_STAGES]), (at / RAW_STAGES) & 1, 1u << 16);
+                }
+            }
+        } else if (warp == MMA_WARP) {  // the two others are only there for the split of the registers
+            // ---------------- products ----------------
+            if (elect_one()) {
+                const uint32_t qk_desc = umma::instr_desc_f16(ROWS, TILE), pv_desc = umma::instr_desc_f16(ROWS, D);
+                uint32_t n_s[2] = {0, 0}, n_p[2] = {0, 0};  // products issued, by group
+                int kv = 0;                                 // tiles
+                bool ok = true;
+                for (int n_items = 0; ok; ++n_items) {
+                    ok = wait_one(ctl.item_full[n_items % ITEMS], (n_items / ITEMS) & 1, 4);
+                    if (!ok) break;
+                    const int rows = ctl.items[n_items % ITEMS].rows, tiles = ctl.items[n_items % ITEMS].tiles;
+                    mbar_arrive(smem_u32(&ctl.item_empty[n_items % ITEMS]));
+                    if (rows < 0) break;
+                    ok = wait_one(ctl.q_full, n_items & 1, 5);
+                    for (int i = 0; ok && i <= tiles; ++i) {
+                        if (i < tiles) {
+                            const int s = i & 1, buf = (kv + i) % KV_STAGES;
+                            ok = wait_one(ctl.kv_full[buf], ((kv + i) / KV_STAGES) & 1, 6) && (n_s[s] == 0 || wait_one(ctl.s_empty[s], (n_s[s] - 1) & 1, 7));
+                            if (!ok) break;
+                            umma::fence_after_sync();
+                            const uint64_t a = umma::smem_desc_sw128(smem), b = umma::smem_desc_sw128(smem + L::KV_AT + buf * L::KV);
+#pragma unroll
+                            for (int k = 0; k < D / 16; ++k) {
+                                const int half = k / 4, at = 2 * (k % 4);  // 16-byte units
+                                umma::mma_ss(tmem + s_col(s), a + half * (ROWS * 128 / 16) + at, b + half * (TILE * 128 / 16) + at, qk_desc, k > 0);
+                            }
+                            umma::commit(smem_u32(&ctl.s_full[s]));
+                            ++n_s[s];
+                        }
+                        if (i > 0) {
+                            const int s = (i - 1) & 1, buf = (kv + i - 1) % KV_STAGES;
+                            ok = wait_one(ctl.p_full[s], n_p[s] & 1, 8);
+                            if (!ok) break;
+                            umma::fence_after_sync();
+                            const uint64_t b = umma::smem_desc_sw128(smem + L::KV_AT + buf * L::KV + L::K);
+#pragma unroll
+                            for (int k = 0; k < TILE / 16; ++k) umma::mma_ts(tmem + o_col(s), tmem + p_col(s) + 8 * k, b + 2 * k, pv_desc, i > 2 || k > 0);
+                            umma::commit(smem_u32(&ctl.pv_done[s]));
+                            umma::commit(smem_u32(&ctl.kv_empty[buf]));
+                            ++n_p[s];
+                        }
+                    }
+                    kv += tiles;
+                }
+                umma::commit(smem_u32(&ctl.drained));  // tensor memory is given back when nothing is on its way
+                if (!mbar_wait(smem_u32(&ctl.drained), 0)) report_timeout(p.status, kKernelCacheAttentionWide, 9);
+            }
+            __syncwarp();
+        }
+    } else if (warp >= CONVERT_WARP0) {
+        // ---------------- codes to f16 ----------------
+        fewer_registers<kConvertRegs>();
+        const int w = warp - CONVERT_WARP0, g = lane >> 2, t = lane & 3;
+        // K: this lane's row of the record, in the order whose ranks give eight lanes eight places
+        const uint32_t row = 4 * ((lane & 7) >> 1) + (lane & 1) + 2 * ((lane >> 3) & 1), sw = k_order(row, D), key = 16 * w + row;
+        const uint32_t v_row = lane & 15, v_sw = v_order(v_row, D);
+        for (int it = 0;; ++it) {
+            const int slot = it % RAW_STAGES, buf = it % KV_STAGES;
+            if (!wait(ctl.raw_full[slot], (it / RAW_STAGES) & 1, 10)) break;
+            const int key0 = ctl.key0[slot] + 16 * w, length = ctl.length[slot];
+            if (length < 0) break;
+            if (it >= KV_STAGES && !wait(ctl.kv_empty[buf], (it / KV_STAGES - 1) & 1, 11)) break;
+            const uint32_t rec = smem + L::RAW_AT + slot * L::RAW + w * record_bytes(D);
+            const uint32_t k_dst = smem + L::KV_AT + buf * L::KV + (key >> 3) * 1024 + (key & 7) * 128, v_dst = smem + L::KV_AT + buf * L::KV + L::K;
+            if (lane < 16) {
+                const float *scales = reinterpret_cast<const float *>(smem_gen + L::RAW_AT + slot * L::RAW + w * record_bytes(D) + 32 * D);
+                const bool there = key0 + lane < length;  // behind the end, and in records that were not copied, is anything
+                const float ks = there ? scales[lane] : 0.0f, vs = there ? scales[16 + lane] : 0.0f;
+                ctl.k_scale[buf][16 * w + lane] = ks;
+                ctl.v_scale[buf][16 * w + lane] = vs;
+                float top = vs;
+#pragma unroll
+                for (int d = 8; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffu, top, d));
+                if (lane == 0) ctl.v_top[buf][w] = top;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {  // two chunks of 16 codes of every row
+                const uint32_t c = 2 * i + (lane >> 4);
+                uint32_t x[4], y[8];
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(rec + row * D + ((c ^ sw) << 4)));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) codes_to_f16(x[e], y[2 * e], y[2 * e + 1]);
+                const uint32_t half = c >> 2, at = (c & 3) * 2;  // 16-byte places of a 128-byte row
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(k_dst + half * (TILE * 128) + (((at + e) ^ (key & 7)) << 4)), "r"(y[4 * e]), "r"(y[4 * e + 1]),
+                                 "r"(y[4 * e + 2]), "r"(y[4 * e + 3])
+                                 : "memory");
+            }
+#pragma unroll
+            for (int dd = 0; dd < D / 32; ++dd) {
+                uint32_t r[4];
+                umma::ldmatrix_x2_trans_b8(r, rec + 16 * D + v_row * D + (((2 * dd + (lane >> 4)) ^ v_sw) << 4));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // element 32 dd + 8 i + g, positions 16 w + 4 t .. + 3
+                    uint32_t lo, hi;
+                    codes_to_f16(r[i], lo, hi);
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(v_dst + (4 * dd + i) * 1024 + g * 128 + (((2 * w + (t >> 1)) ^ g) << 4) + 8 * (t & 1)), "r"(lo), "r"(hi) : "memory");
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&ctl.kv_full[buf]));
+                mbar_arrive(smem_u32(&ctl.raw_empty[slot]));
+            }
+        }
+    } else {
+        // ---------------- scores to probabilities ----------------
+        more_registers<kSoftmaxRegs>();
+        const int grp = warp / GROUP_WARPS, quarter = warp % GROUP_WARPS, r = 32 * quarter + lane;  // this thread's row
+        const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
+        const uint32_t s_addr = tmem + lanes + s_col(grp), p_addr = tmem + lanes + p_col(grp), o_addr = tmem + lanes + o_col(grp);
+        uint32_t n = 0;  // tiles of this group
+        int kv = 0;      // of both
+        bool alive = true, met = false;  // as in the other kernel
+        for (int n_items = 0;; ++n_items) {
+            alive = wait(ctl.item_full[n_items % ITEMS], (n_items / ITEMS) & 1, 12);
+            if (!alive) break;
+            const Item item = ctl.items[n_items % ITEMS];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[n_items % ITEMS]));
+            if (item.rows < 0) break;
+            const int token = (item.row0 + r) / p.group, hidden = first_hidden(p, item);
+            const bool busy = 32 * quarter < item.rows;  // this warp has rows
+
+            // ---- the queries: group 0 brings the first half of a row, group 1 the second ----
+            float qs = p.scale_log2;
+            {
+                constexpr int N = D / 2;
+                uint4 x[N / 8];
+                const T *src = static_cast<const T *>(p.q) + (int64_t)(item.token0 + token) * p.q_token + (int64_t)(item.head * p.group + item.row0 + r - token * p.group) * p.q_head + grp * N;
+#pragma unroll
+                for (int i = 0; i < N / 8; ++i) {
+                    uint2 a = make_uint2(0, 0), b = a;
+                    if (r < item.rows) a = reinterpret_cast<const uint2 *>(src)[2 * i], b = reinterpret_cast<const uint2 *>(src)[2 * i + 1];
+                    x[i] = make_uint4(a.x, a.y, b.x, b.y);
+                }
+                float down = 1.0f;
+                if (std::is_same<T, __nv_bfloat16>::value) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < N / 8; ++i) {
+                        const T *v = reinterpret_cast<const T *>(&x[i]);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(Elems<T>::one(v[e])));
+                    }
+                    ctl.top[grp][r] = top;
+                }
+                if (!all_of<SOFTMAX_THREADS>(true)) {  // behind it no thread reads or writes anything of the item in front
+                    met = true;
+                    break;
+                }
+                if (std::is_same<T, __nv_bfloat16>::value) {
+                    const float top = fmaxf(ctl.top[0][r], ctl.top[1][r]);
+                    const uint32_t e = min(max(__float_as_uint(top) >> 23, 64u), 253u);
+                    if (top > 0.0f) down = __uint_as_float((254u - e) << 23), qs *= __uint_as_float(e << 23);
+                }
+#pragma unroll
+                for (int i = 0; i < N / 8; ++i) {
+                    if (std::is_same<T, __nv_bfloat16>::value) {
+                        const T *v = reinterpret_cast<const T *>(&x[i]);
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = pack_f16(Elems<T>::one(v[2 * e]) * down, Elems<T>::one(v[2 * e + 1]) * down);
+                        x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    const int c = grp * (N / 8) + i;  // 16-byte chunk of the row
+                    *reinterpret_cast<uint4 *>(smem_gen + (c >> 3) * (ROWS * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[i];
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl.q_full));
+            }
+            const float rise = fminf(kRise / qs, 1e38f);
+            float m = -INFINITY, shift = 0.0f, sum = 0.0f;  // shift: m, or 0 as long as nothing was seen
+            float exponent = 0.0f, v_limit = kLeastNormal;  // of the value scales, and the first scale that is too large for it
+
+            for (int i = grp; i < item.tiles; i += 2) {
+                const int buf = (kv + i) % KV_STAGES, key0 = (item.tile0 + i) * TILE;
+                alive = wait(ctl.s_full[grp], n & 1, 13) && wait(ctl.kv_full[buf], ((kv + i) / KV_STAGES) & 1, 14);  // the latter for the scales
+                if (!alive) break;
+                umma::fence_after_sync();
+                float s[TILE];
+                if (busy) {
+                    umma::ld_32x32b_x32(s_addr, *reinterpret_cast<uint32_t (*)[32]>(&s[0]));
+                    umma::ld_32x32b_x32(s_addr + 32, *reinterpret_cast<uint32_t (*)[32]>(&s[32]));
+                    umma::ld_wait();
+                }
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl.s_empty[grp]));
+                bool raise = false;
+                float top = -INFINITY, v_top = 0.0f;
+                const bool partly = key0 + TILE > hidden;
+                if (busy) {
+                    const uint32_t ks = smem_u32(ctl.k_scale[buf]);
+#pragma unroll
+                    for (int j = 0; j < TILE / 4; ++j) {
+                        const float4 k = scales_at(ks + 16 * j);
+                        s[4 * j] *= k.x, s[4 * j + 1] *= k.y, s[4 * j + 2] *= k.z, s[4 * j + 3] *= k.w;
+                    }
+                    if (partly) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t seen = 0;
+#pragma unroll 4
+                            for (int j = 0; j < 32; ++j) seen |= (uint32_t)may_see(p, item, r, token, key0 + 32 * h + j) << j;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (!(seen >> j & 1u)) s[32 * h + j] = -INFINITY;
+                        }
+                    }
+                    float tops[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int j = 4; j < TILE; ++j) tops[j & 3] = fmaxf(tops[j & 3], s[j]);
+                    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                    v_top = fmaxf(fmaxf(ctl.v_top[buf][0], ctl.v_top[buf][1]), fmaxf(ctl.v_top[buf][2], ctl.v_top[buf][3]));
+                    raise = top > m + rise || v_top >= v_limit;
+                }
+                raise = __any_sync(0xffffffffu, raise);
+                if (n > 0) {  // P and O are this thread's again
+                    alive = wait(ctl.pv_done[grp], (n - 1) & 1, 15);
+                    if (!alive) break;
+                    umma::fence_after_sync();
+                }
+                if (raise) {
+                    const float was = exponent;
+                    if (v_top >= v_limit) {
+                        exponent = fmaxf((float)((int)(__float_as_uint(v_top) >> 23) - 127), kLeastUnit);
+                        v_limit = __uint_as_float((uint32_t)((int)exponent + 128) << 23);
+                    }
+                    const float higher = fmaxf(m, top);
+                    // in two steps: with value scales of very unlike sizes the whole may leave float's range where its product with the sum does not
+                    const float by = higher == -INFINITY ? 1.0f : ex2(0.5f * ((m - higher) * qs + (was - exponent)));
+                    m = higher;
+                    shift = higher == -INFINITY ? 0.0f : higher;
+                    sum = sum * by * by;
+                    if (i > grp) {
+#pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            umma::ld_32x32b_x32(o_addr + c, o);
+                            umma::ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by * by);
+                            umma::st_32x32b_x32(o_addr + c, o);
+                        }
+                    }
+                }
+                if (busy) {
+                    const uint32_t vs = smem_u32(ctl.v_scale[buf]);
+                    const float bias = kBias - exponent;
+                    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    uint32_t packed[32];
+#pragma unroll
+                    for (int j = 0; j < TILE / 4; ++j) {
+                        const float4 v4 = scales_at(vs + 16 * j);
+                        const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+                        float x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            x[e] = ex2(fmaf(s[4 * j + e] - shift, qs, bias));
+                            sums[e] += x[e];
+                            x[e] *= v[e];
+                        }
+                        packed[2 * j] = pack_f16(x[0], x[1]);
+                        packed[2 * j + 1] = pack_f16(x[2], x[3]);
+                    }
+                    if (partly) {  // nothing, whatever the scale of a position that is not seen
+#pragma unroll
+                        for (int j = 0; j < TILE / 2; ++j) {
+                            if (s[2 * j] == -INFINITY) packed[j] &= 0xffff0000u;
+                            if (s[2 * j + 1] == -INFINITY) packed[j] &= 0x0000ffffu;
+                        }
+                    }
+                    sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                    umma::st_32x32b_x32(p_addr, packed);
+                }
+                umma::st_wait();
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&ctl.p_full[grp]));
+                ++n;
+            }
+            if (!alive) break;
+            kv += item.tiles;
+
+            // ---- the two groups' sums meet ----
+            if (item.tiles > grp) {
+                alive = wait(ctl.pv_done[grp], (n - 1) & 1, 16);
+                if (!alive) break;
+            }
+            ctl.unit[grp][r] = m == -INFINITY ? -INFINITY : m * qs + exponent;
+            ctl.sum[grp][r] = sum;
+            umma::fence_before_sync();
+            if (!all_of<SOFTMAX_THREADS>(true)) {
+                met = true;
+                break;
+            }
+            umma::fence_after_sync();
+            const bool whole = item.first_cta == item.last_cta;
+            if (busy) {
+                const float u0 = ctl.unit[0][r], u1 = ctl.unit[1][r], unit = fmaxf(u0, u1);
+                const float f0 = u0 == -INFINITY ? 1.0f : ex2(0.5f * (u0 - unit)), f1 = u1 == -INFINITY ? 1.0f : ex2(0.5f * (u1 - unit));
+                const float total = ctl.sum[0][r] * f0 * f0 + ctl.sum[1][r] * f1 * f1;
+                float *piece = p.partial + (int64_t)item.slot * kPieceFloats<D, ROWS>;
+#pragma unroll
+                for (int c0 = 0; c0 < D / 2; c0 += 32) {  // group 0 takes the first half of the elements, group 1 the second
+                    const int c = grp * (D / 2) + c0;
+                    uint32_t a[32], b[32];
+                    umma::ld_32x32b_x32(tmem + lanes + o_col(0) + c, a);
+                    umma::ld_32x32b_x32(tmem + lanes + o_col(1) + c, b);
+                    umma::ld_wait();
+                    if (r < item.rows) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            float v[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {  // the second sum begins with the item's second tile
+                                v[e] = __uint_as_float(a[j + e]) * f0 * f0;
+                                if (item.tiles > 1) v[e] = fmaf(__uint_as_float(b[j + e]) * f1, f1, v[e]);
+                            }
+                            const float4 v4 = make_float4(v[0], v[1], v[2], v[3]);
+                            if (whole) write_out<D, T>(p, item, r, c + j, v4, total, unit);
+                            else write_piece<D, ROWS>(piece, r, c + j, v4, total, unit);
+                        }
+                    }
+                }
+                umma::fence_before_sync();
+            }
+            // The first operand's place serves for the pieces' units and sums: all products with it are over.
+            if (!whole) meet<D, ROWS, SOFTMAX_THREADS, 1, T>(p, item, threadIdx.x, reinterpret_cast<float *>(smem_gen), &ctl.last);
+        }
+        if (!met) all_of<SOFTMAX_THREADS>(alive);
+    }
+    __syncwarp();
+    __syncthreads();
+    if (warp == MMA_WARP) {
+        umma::fence_after_sync();
+        umma::dealloc(tmem, TMEM_COLS);
+    }
+}
+
+template <int D, typename T>
+int launch_sized(const AttentionArgs &p, cudaStream_t stream) {
+    using L = Layout<D>;
+    auto kernel = cache_attention_wide_kernel<D, T>;
+    static std::atomic<bool> attr_set[64];
+    const int rc = allow_smem(attr_set, kernel, L::SMEM);
+    if (rc != B200Q_OK) return rc;
+    // The registers that the groups take and give have to be there, or their first would wait for good.
+    static std::atomic<int> regs{0};
+    if (regs.load(std::memory_order_relaxed) == 0) {
+        cudaFuncAttributes attributes;
+        B200Q_CUDA_TRY(cudaFuncGetAttributes(&attributes, kernel));
+        regs.store(attributes.numRegs, std::memory_order_relaxed);
+    }
+    if (regs.load(std::memory_order_relaxed) < kLaunchRegs) {
+        return set_error(B200Q_UNSUPPORTED, "quantized_cache_attention: the kernel was built for %d registers a thread, %d are wanted", regs.load(), kLaunchRegs);
+    }
+    const int64_t tiles = most_tiles(p, ROWS), at_once = sm_count();
+    if (tiles > (1ll << 29)) return set_error(B200Q_UNSUPPORTED, "quantized_cache_attention: up to %lld tiles of %d rows and %d positions", (long long)tiles, ROWS, TILE);
+    int64_t grid = tiles < at_once ? tiles : at_once;
+    if (grid > kMostWideCtas) grid = kMostWideCtas;
+    return launch_after("cache_attention_wide_kernel", kernel, dim3((unsigned)grid), THREADS, L::SMEM, 1, stream, p);
+}
+
+}  // namespace
+
+int launch_wide(const AttentionArgs &p, int dim, bool bf16, cudaStream_t stream) {
+    if (dim == 64) return bf16 ? launch_sized<64, __nv_bfloat16>(p, stream) : launch_sized<64, __half>(p, stream);
+    return bf16 ? launch_sized<128, __nv_bfloat16>(p, stream) : launch_sized<128, __half>(p, stream);
+}
+
+}  // namespace cache_attention
+}  // namespace b200q

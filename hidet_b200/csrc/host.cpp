@@ -445,7 +445,7 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     const bool with_lse = args[7] == Py_True;
     void *ws;
     size_t ws_bytes;
-    PLAIN_OR_NONE(find_scratch(w, lib.attention_workspace_bytes(dim), ws, ws_bytes));
+    PLAIN_OR_NONE(find_scratch(w, lib.attention_workspace_bytes(batch, tokens, heads, kv_heads, dim), ws, ws_bytes));
     at::Tensor out = empty(q->sizes(), q->scalar_type(), w.device), lse;
     if (with_lse) lse = empty(q->sizes().slice(0, q->dim() - 1), at::kFloat, w.device);
     const b200q_heads rows = {const_cast<void *>(q->const_data_ptr()), heads * dim, dim};

@@ -179,7 +179,7 @@ SIGNATURES = {
         True,
     ),
     'b200q_quantized_cache_read': ([c_void_p, c_int64, c_int64] + [c_void_p] * 3 + [c_int64] * 3 + [c_int] * 2 + [c_void_p], c_int, True),
-    'b200q_quantized_cache_attention_workspace_bytes': ([c_int64], c_size_t, False),
+    'b200q_quantized_cache_attention_workspace_bytes': ([c_int64] * 5, c_size_t, False),
     'b200q_quantized_cache_attention': (
         [POINTER(Heads), c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]
         + [c_int64] * 7 + [c_float, c_int, c_void_p, c_size_t, c_void_p],

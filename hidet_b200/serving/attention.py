@@ -73,7 +73,7 @@ def quantized_cache_attention(q: torch.Tensor, cache: torch.Tensor, page_table: 
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
     with torch.cuda.device(q.device):
-        ws_ptr, ws_size = workspaces.get(q.device, ffi.func('b200q_quantized_cache_attention_workspace_bytes')(dim))
+        ws_ptr, ws_size = workspaces.get(q.device, ffi.func('b200q_quantized_cache_attention_workspace_bytes')(batch, tokens, heads, kv_heads, dim))
         ffi.func('b200q_quantized_cache_attention')(
             heads_struct(rows), out.data_ptr(), lse.data_ptr() if return_lse else None, cache.data_ptr(), pages, page_size, page_table.data_ptr(), page_table.shape[1],
             page_table.stride(0), lengths.data_ptr(), starts.data_ptr() if starts is not None else None, mask.data_ptr() if mask is not None else None,

@@ -352,7 +352,8 @@ B200Q_API int b200q_quantized_cache_read(const void *cache, int64_t pages, int64
  * NULL) the natural logarithm of the softmax's denominator.  q: 8-byte aligned, strides multiples of 4 elements.
  * The workspace is one of b200q_qlinear_f16_i8's kind: zero-filled once, its counters are zero again after every call.
  */
-B200Q_API size_t b200q_quantized_cache_attention_workspace_bytes(int64_t head_dim);
+B200Q_API size_t b200q_quantized_cache_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                                                 int64_t head_dim);
 B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, float *lse, const void *cache, int64_t pages, int64_t page_size,
                                               const int32_t *page_table, int64_t table_width, int64_t table_stride, const int32_t *lengths,
                                               const int32_t *starts, const void *mask, int64_t mask_width, int64_t mask_stride, int64_t batch,
