@@ -121,8 +121,8 @@ __device__ __forceinline__ void finish_item(const AttentionArgs &p, Control &ctl
         if (whole) write_out<D, T>(p, item, r, d, v, sum, top * scale);
         else write_piece<D, ROWS>(piece, r, d, v, sum, top * scale);
     }
-    static_assert(L::BUFFERS * L::MERGE >= 2 * FAN * ROWS * 4, "");
-    if (!whole) meet<D, ROWS, CONSUMERS, 1, T>(p, item, threadIdx.x, merge, &ctl.last);  // whose first barrier frees the merge buffers
+    static_assert(L::BUFFERS * L::MERGE >= 2 * FEW_FAN * ROWS * 4, "");
+    if (!whole) meet<D, ROWS, CONSUMERS, FEW_FAN, 1, T>(p, item, threadIdx.x, merge, &ctl.last);  // whose first barrier frees the merge buffers
 }
 
 template <int D, int NT, typename T>
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
             ++n_items;
         };
 
-        Line<ROWS> line(p, lane);
+        Line<ROWS, FEW_FAN> line(p, lane);
         Item item;
         const int32_t *table;
         int slot = 0, it = 0;

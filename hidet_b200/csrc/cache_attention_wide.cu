@@ -8,11 +8,13 @@
 //   one thread issues S = Q K^T (128 x 64) and O += P V (128 x D), sums in tensor memory;
 //   two groups of four warps turn scores into probabilities, a thread a row, alternate tiles: each group has its own S, P, O, maxima and sums, which
 //       meet at the end of the item.
-// The probabilities go back into tensor memory as the first operand of the second product.  A thread has a whole row of 64 scores, so maximum and sum
+// The probabilities go back into tensor memory, in the place of their scores, as the first operand of the second product.  A thread has a whole row of 64 scores, so maximum and sum
 // need no exchange.  A row's unit is 2^u: u is its running maximum (in log2) plus the exponent of the largest value scale so far, so that the products with
 // value scales fit f16 and sums of probabilities and of values are in the same unit.
 //
 // Bound by instructions: per tile and row about 470 of them for 64 scores, and 700 a warp for the conversion of a tile's 16 K codes.
+#include <stddef.h>
+
 #include "cache_attention.cuh"
 
 namespace b200q {
@@ -27,7 +29,7 @@ constexpr int SOFTMAX_THREADS = 2 * 32 * GROUP_WARPS;
 constexpr int CONVERT_WARP0 = 8, PRODUCER_WARP = 12, MMA_WARP = 13;
 constexpr int THREADS = 32 * 16;                // four groups of four warps, for the split of the registers
 // Registers a thread of the groups: softmax (two groups), conversion, the rest.  Together what the block is launched with.
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 192, kConvertRegs = 72, kOtherRegs = 56;
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 192, kConvertRegs = 64, kOtherRegs = 64;
 static_assert(2 * kSoftmaxRegs + kConvertRegs + kOtherRegs <= 4 * kLaunchRegs, "");
 template <int N>
 __device__ __forceinline__ void more_registers() {
@@ -38,12 +40,12 @@ __device__ __forceinline__ void fewer_registers() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 constexpr int ITEMS = 2;                        // that the other roles may know of
-constexpr int RAW_STAGES = 4, KV_STAGES = 3;
+constexpr int RAW_STAGES = 3, KV_STAGES = 4;
+constexpr int AHEAD = 2;                        // tiles whose scores are asked for in front of the probabilities of another
 constexpr uint32_t TMEM_COLS = 512;
-// columns of a group's scores, probabilities and sums
-__device__ __forceinline__ constexpr uint32_t s_col(int group) { return 64 * group; }
-__device__ __forceinline__ constexpr uint32_t p_col(int group) { return 128 + 32 * group; }
-__device__ __forceinline__ constexpr uint32_t o_col(int group) { return 192 + 128 * group; }
+// Columns of a group's scores, two tiles of them (the probabilities take the place of their scores), and of its sums.
+__device__ __forceinline__ constexpr uint32_t s_col(int group, int buffer) { return 64 * (2 * group + buffer); }
+__device__ __forceinline__ constexpr uint32_t o_col(int group) { return 256 + 128 * group; }
 constexpr float kLeastUnit = -90.0f;            // exponents of value scales below are not followed: sums in that unit stay in float's range
 
 template <int D>
@@ -53,26 +55,54 @@ struct Layout {
     static constexpr int RAW = RECORDS * record_bytes(D);
     static constexpr int KV_AT = Q, RAW_AT = Q + KV_STAGES * KV;
     static constexpr int SMEM = RAW_AT + RAW_STAGES * RAW + 1024;  // 1024: the operands begin at a multiple of it
-    static_assert(2 * FAN * ROWS * 4 <= Q, "");
+    static_assert(2 * WIDE_FAN * ROWS * 4 <= Q, "");
 };
 
-// Four scales, read where this stands: ahead of their use they would take as many registers as the scores.
-__device__ __forceinline__ float4 scales_at(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-    return v;
+// Two floats in a register pair, for the instructions that take two at once.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
 }
+__device__ __forceinline__ f32x2 pair_of(uint32_t lo, uint32_t hi) { return pair_of(__uint_as_float(lo), __uint_as_float(hi)); }
+__device__ __forceinline__ void halves(f32x2 x, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// Four scales, read where this stands: ahead of their use they would take as many registers as the scores.
+__device__ __forceinline__ void scales_at(uint32_t addr, f32x2 &a, f32x2 &b) { asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr)); }
 
 struct Control {
     uint64_t raw_full[RAW_STAGES], raw_empty[RAW_STAGES], kv_full[KV_STAGES], kv_empty[KV_STAGES], item_full[ITEMS], item_empty[ITEMS];
-    uint64_t q_full, s_full[2], s_empty[2], p_full[2], pv_done[2], drained;
-    float k_scale[KV_STAGES][TILE], v_scale[KV_STAGES][TILE], v_top[KV_STAGES][RECORDS];
+    uint64_t q_full, s_full[2][2], p_full[2][2], pv_done[2], item_done, drained;  // [group][buffer]
+    alignas(16) float k_scale[KV_STAGES][TILE];  // read four at a time
+    alignas(16) float v_scale[KV_STAGES][TILE];
+    float v_top[KV_STAGES][RECORDS];
     int key0[RAW_STAGES], length[RAW_STAGES];  // length -1: no more tiles
     Item items[ITEMS];
     float top[2][ROWS], unit[2][ROWS], sum[2][ROWS];
     int abort, last;
     uint32_t tmem;
 };
+static_assert(offsetof(Control, k_scale) % 16 == 0 && offsetof(Control, v_scale) % 16 == 0 && alignof(Control) % 16 == 0, "");
 
 template <int D, typename T>
 __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const __grid_constant__ AttentionArgs p) {
@@ -88,10 +118,11 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
         for (int i = 0; i < KV_STAGES; ++i) mbar_init(smem_u32(&ctl.kv_full[i]), RECORDS), mbar_init(smem_u32(&ctl.kv_empty[i]), 1);
         for (int i = 0; i < ITEMS; ++i) mbar_init(smem_u32(&ctl.item_full[i]), 1), mbar_init(smem_u32(&ctl.item_empty[i]), 2 * GROUP_WARPS + 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&ctl.s_full[i]), 1), mbar_init(smem_u32(&ctl.s_empty[i]), GROUP_WARPS);
-            mbar_init(smem_u32(&ctl.p_full[i]), GROUP_WARPS), mbar_init(smem_u32(&ctl.pv_done[i]), 1);
+            for (int j = 0; j < 2; ++j) mbar_init(smem_u32(&ctl.s_full[i][j]), 1), mbar_init(smem_u32(&ctl.p_full[i][j]), GROUP_WARPS);
+            mbar_init(smem_u32(&ctl.pv_done[i]), 1);
         }
         mbar_init(smem_u32(&ctl.q_full), 2 * GROUP_WARPS);
+        mbar_init(smem_u32(&ctl.item_done), 1);
         mbar_init(smem_u32(&ctl.drained), 1);
         ctl.abort = 0;
         mbar_fence_init();
@@ -127,7 +158,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
         if (warp == PRODUCER_WARP) {
             // ---------------- plan and copies ----------------
             pdl_launch_dependents();
-            Line<ROWS> line(p, lane);
+            Line<ROWS, WIDE_FAN> line(p, lane);
             Item item;
             const int32_t *table;
             int n_items = 0, it = 0, slot = 0;
@@ -180,8 +211,10 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
             // ---------------- products ----------------
             if (elect_one()) {
                 const uint32_t qk_desc = umma::instr_desc_f16(ROWS, TILE), pv_desc = umma::instr_desc_f16(ROWS, D);
-                uint32_t n_s[2] = {0, 0}, n_p[2] = {0, 0};  // products issued, by group
-                int kv = 0;                                 // tiles
+                // Products are carried out in the order they are issued, so the second product of a tile frees the place of its scores for a later
+                // tile's without a wait.
+                uint32_t n[2] = {0, 0};  // tiles of the groups, of the items in front
+                int kv = 0;              // of both
                 bool ok = true;
                 for (int n_items = 0; ok; ++n_items) {
                     ok = wait_one(ctl.item_full[n_items % ITEMS], (n_items / ITEMS) & 1, 4);
@@ -190,35 +223,38 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                     mbar_arrive(smem_u32(&ctl.item_empty[n_items % ITEMS]));
                     if (rows < 0) break;
                     ok = wait_one(ctl.q_full, n_items & 1, 5);
-                    for (int i = 0; ok && i <= tiles; ++i) {
-                        if (i < tiles) {
-                            const int s = i & 1, buf = (kv + i) % KV_STAGES;
-                            ok = wait_one(ctl.kv_full[buf], ((kv + i) / KV_STAGES) & 1, 6) && (n_s[s] == 0 || wait_one(ctl.s_empty[s], (n_s[s] - 1) & 1, 7));
+                    for (int i = 0, asked = 0; ok && i < tiles; ++i) {
+                        for (; ok && asked < min(tiles, i + AHEAD + 1); ++asked) {
+                            const int g = asked & 1, buf = (kv + asked) % KV_STAGES;
+                            const uint32_t at = n[g] + (asked >> 1);
+                            ok = wait_one(ctl.kv_full[buf], ((kv + asked) / KV_STAGES) & 1, 6);
                             if (!ok) break;
                             umma::fence_after_sync();
                             const uint64_t a = umma::smem_desc_sw128(smem), b = umma::smem_desc_sw128(smem + L::KV_AT + buf * L::KV);
 #pragma unroll
                             for (int k = 0; k < D / 16; ++k) {
-                                const int half = k / 4, at = 2 * (k % 4);  // 16-byte units
-                                umma::mma_ss(tmem + s_col(s), a + half * (ROWS * 128 / 16) + at, b + half * (TILE * 128 / 16) + at, qk_desc, k > 0);
+                                const int half = k / 4, to = 2 * (k % 4);  // 16-byte units
+                                umma::mma_ss(tmem + s_col(g, at & 1), a + half * (ROWS * 128 / 16) + to, b + half * (TILE * 128 / 16) + to, qk_desc, k > 0);
                             }
-                            umma::commit(smem_u32(&ctl.s_full[s]));
-                            ++n_s[s];
+                            umma::commit(smem_u32(&ctl.s_full[g][at & 1]));
                         }
-                        if (i > 0) {
-                            const int s = (i - 1) & 1, buf = (kv + i - 1) % KV_STAGES;
-                            ok = wait_one(ctl.p_full[s], n_p[s] & 1, 8);
-                            if (!ok) break;
-                            umma::fence_after_sync();
-                            const uint64_t b = umma::smem_desc_sw128(smem + L::KV_AT + buf * L::KV + L::K);
+                        if (!ok) break;
+                        const int g = i & 1, buf = (kv + i) % KV_STAGES;
+                        const uint32_t at = n[g] + (i >> 1);
+                        ok = wait_one(ctl.p_full[g][at & 1], (at >> 1) & 1, 8);
+                        if (!ok) break;
+                        umma::fence_after_sync();
+                        const uint64_t b = umma::smem_desc_sw128(smem + L::KV_AT + buf * L::KV + L::K);
 #pragma unroll
-                            for (int k = 0; k < TILE / 16; ++k) umma::mma_ts(tmem + o_col(s), tmem + p_col(s) + 8 * k, b + 2 * k, pv_desc, i > 2 || k > 0);
-                            umma::commit(smem_u32(&ctl.pv_done[s]));
-                            umma::commit(smem_u32(&ctl.kv_empty[buf]));
-                            ++n_p[s];
-                        }
+                        for (int k = 0; k < TILE / 16; ++k) umma::mma_ts(tmem + o_col(g), tmem + s_col(g, at & 1) + 8 * k, b + 2 * k, pv_desc, i > 1 || k > 0);
+                        umma::commit(smem_u32(&ctl.pv_done[g]));
+                        umma::commit(smem_u32(&ctl.kv_empty[buf]));
                     }
+                    if (!ok) break;
+                    umma::commit(smem_u32(&ctl.item_done));
                     kv += tiles;
+                    n[0] += (tiles + 1) >> 1;
+                    n[1] += tiles >> 1;
                 }
                 umma::commit(smem_u32(&ctl.drained));  // tensor memory is given back when nothing is on its way
                 if (!mbar_wait(smem_u32(&ctl.drained), 0)) report_timeout(p.status, kKernelCacheAttentionWide, 9);
@@ -289,7 +325,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
         more_registers<kSoftmaxRegs>();
         const int grp = warp / GROUP_WARPS, quarter = warp % GROUP_WARPS, r = 32 * quarter + lane;  // this thread's row
         const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
-        const uint32_t s_addr = tmem + lanes + s_col(grp), p_addr = tmem + lanes + p_col(grp), o_addr = tmem + lanes + o_col(grp);
+        const uint32_t o_addr = tmem + lanes + o_col(grp);
         uint32_t n = 0;  // tiles of this group
         int kv = 0;      // of both
         bool alive = true, met = false;  // as in the other kernel
@@ -357,27 +393,24 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
 
             for (int i = grp; i < item.tiles; i += 2) {
                 const int buf = (kv + i) % KV_STAGES, key0 = (item.tile0 + i) * TILE;
-                alive = wait(ctl.s_full[grp], n & 1, 13) && wait(ctl.kv_full[buf], ((kv + i) / KV_STAGES) & 1, 14);  // the latter for the scales
+                const uint32_t s_addr = tmem + lanes + s_col(grp, n & 1);
+                alive = wait(ctl.s_full[grp][n & 1], (n >> 1) & 1, 13) && wait(ctl.kv_full[buf], ((kv + i) / KV_STAGES) & 1, 14);  // the latter for the scales
                 if (!alive) break;
                 umma::fence_after_sync();
-                float s[TILE];
                 if (busy) {
-                    umma::ld_32x32b_x32(s_addr, *reinterpret_cast<uint32_t (*)[32]>(&s[0]));
-                    umma::ld_32x32b_x32(s_addr + 32, *reinterpret_cast<uint32_t (*)[32]>(&s[32]));
+                    uint32_t raw[TILE];
+                    umma::ld_32x32b_x32(s_addr, *reinterpret_cast<uint32_t (*)[32]>(&raw[0]));
+                    umma::ld_32x32b_x32(s_addr + 32, *reinterpret_cast<uint32_t (*)[32]>(&raw[32]));
                     umma::ld_wait();
-                }
-                umma::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&ctl.s_empty[grp]));
-                bool raise = false;
-                float top = -INFINITY, v_top = 0.0f;
-                const bool partly = key0 + TILE > hidden;
-                if (busy) {
-                    const uint32_t ks = smem_u32(ctl.k_scale[buf]);
+                    const bool partly = key0 + TILE > hidden;
+                    f32x2 s[TILE / 2];
+                    const uint32_t ks = smem_u32(ctl.k_scale[buf]), vs = smem_u32(ctl.v_scale[buf]);
 #pragma unroll
                     for (int j = 0; j < TILE / 4; ++j) {
-                        const float4 k = scales_at(ks + 16 * j);
-                        s[4 * j] *= k.x, s[4 * j + 1] *= k.y, s[4 * j + 2] *= k.z, s[4 * j + 3] *= k.w;
+                        f32x2 k0, k1;
+                        scales_at(ks + 16 * j, k0, k1);
+                        s[2 * j] = mul2(pair_of(raw[4 * j], raw[4 * j + 1]), k0);
+                        s[2 * j + 1] = mul2(pair_of(raw[4 * j + 2], raw[4 * j + 3]), k1);
                     }
                     if (partly) {
 #pragma unroll
@@ -386,90 +419,96 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
 #pragma unroll 4
                             for (int j = 0; j < 32; ++j) seen |= (uint32_t)may_see(p, item, r, token, key0 + 32 * h + j) << j;
 #pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (!(seen >> j & 1u)) s[32 * h + j] = -INFINITY;
+                            for (int j = 0; j < 16; ++j) {
+                                float lo, hi;
+                                halves(s[16 * h + j], lo, hi);
+                                s[16 * h + j] = pair_of(seen >> (2 * j) & 1u ? lo : -INFINITY, seen >> (2 * j + 1) & 1u ? hi : -INFINITY);
+                            }
                         }
                     }
-                    float tops[4] = {s[0], s[1], s[2], s[3]};
+                    float top = -INFINITY, other = -INFINITY;
 #pragma unroll
-                    for (int j = 4; j < TILE; ++j) tops[j & 3] = fmaxf(tops[j & 3], s[j]);
-                    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-                    v_top = fmaxf(fmaxf(ctl.v_top[buf][0], ctl.v_top[buf][1]), fmaxf(ctl.v_top[buf][2], ctl.v_top[buf][3]));
-                    raise = top > m + rise || v_top >= v_limit;
-                }
-                raise = __any_sync(0xffffffffu, raise);
-                if (n > 0) {  // P and O are this thread's again
-                    alive = wait(ctl.pv_done[grp], (n - 1) & 1, 15);
-                    if (!alive) break;
-                    umma::fence_after_sync();
-                }
-                if (raise) {
-                    const float was = exponent;
-                    if (v_top >= v_limit) {
-                        exponent = fmaxf((float)((int)(__float_as_uint(v_top) >> 23) - 127), kLeastUnit);
-                        v_limit = __uint_as_float((uint32_t)((int)exponent + 128) << 23);
+                    for (int j = 0; j < TILE / 2; j += 2) {
+                        float lo, hi;
+                        halves(s[j], lo, hi);
+                        top = max3(top, lo, hi);
+                        halves(s[j + 1], lo, hi);
+                        other = max3(other, lo, hi);
                     }
-                    const float higher = fmaxf(m, top);
-                    // in two steps: with value scales of very unlike sizes the whole may leave float's range where its product with the sum does not
-                    const float by = higher == -INFINITY ? 1.0f : ex2(0.5f * ((m - higher) * qs + (was - exponent)));
-                    m = higher;
-                    shift = higher == -INFINITY ? 0.0f : higher;
-                    sum = sum * by * by;
-                    if (i > grp) {
+                    top = fmaxf(top, other);
+                    const float v_top = fmaxf(fmaxf(ctl.v_top[buf][0], ctl.v_top[buf][1]), fmaxf(ctl.v_top[buf][2], ctl.v_top[buf][3]));
+                    if (__any_sync(0xffffffffu, top > m + rise || v_top >= v_limit)) {
+                        const float was = exponent;
+                        if (v_top >= v_limit) {
+                            exponent = fmaxf((float)((int)(__float_as_uint(v_top) >> 23) - 127), kLeastUnit);
+                            v_limit = __uint_as_float((uint32_t)((int)exponent + 128) << 23);
+                        }
+                        const float higher = fmaxf(m, top);
+                        // in two steps: with value scales of very unlike sizes the whole may leave float's range where its product with the sum does not
+                        const float by = higher == -INFINITY ? 1.0f : ex2(0.5f * ((m - higher) * qs + (was - exponent)));
+                        m = higher;
+                        shift = higher == -INFINITY ? 0.0f : higher;
+                        sum = sum * by * by;
+                        if (i > grp) {
+                            // O is this thread's when the group's product in front is over.  (The one in front of that is: this tile's scores were issued behind it.)
+                            alive = wait(ctl.pv_done[grp], (n - 1) & 1, 15);
+                            if (!alive) break;
+                            umma::fence_after_sync();
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 32) {
+                                uint32_t o[32];
+                                umma::ld_32x32b_x32(o_addr + c, o);
+                                umma::ld_wait();
 #pragma unroll
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            umma::ld_32x32b_x32(o_addr + c, o);
-                            umma::ld_wait();
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by * by);
-                            umma::st_32x32b_x32(o_addr + c, o);
+                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by * by);
+                                umma::st_32x32b_x32(o_addr + c, o);
+                            }
                         }
                     }
-                }
-                if (busy) {
-                    const uint32_t vs = smem_u32(ctl.v_scale[buf]);
-                    const float bias = kBias - exponent;
-                    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    uint32_t packed[32];
+                    const f32x2 minus = pair_of(-shift, -shift), scale2 = pair_of(qs, qs), bias = pair_of(kBias - exponent, kBias - exponent);
+                    f32x2 sums[2] = {0, 0};
+                    uint32_t packed[TILE / 2];
 #pragma unroll
                     for (int j = 0; j < TILE / 4; ++j) {
-                        const float4 v4 = scales_at(vs + 16 * j);
-                        const float v[4] = {v4.x, v4.y, v4.z, v4.w};
-                        float x[4];
+                        f32x2 v[2];
+                        scales_at(vs + 16 * j, v[0], v[1]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            x[e] = ex2(fmaf(s[4 * j + e] - shift, qs, bias));
-                            sums[e] += x[e];
-                            x[e] *= v[e];
+                        for (int e = 0; e < 2; ++e) {
+                            float lo, hi;
+                            halves(fma2(add2(s[2 * j + e], minus), scale2, bias), lo, hi);
+                            const f32x2 x = pair_of(ex2(lo), ex2(hi));
+                            sums[e] = add2(sums[e], x);
+                            halves(mul2(x, v[e]), lo, hi);
+                            packed[2 * j + e] = pack_f16(lo, hi);
                         }
-                        packed[2 * j] = pack_f16(x[0], x[1]);
-                        packed[2 * j + 1] = pack_f16(x[2], x[3]);
                     }
                     if (partly) {  // nothing, whatever the scale of a position that is not seen
 #pragma unroll
                         for (int j = 0; j < TILE / 2; ++j) {
-                            if (s[2 * j] == -INFINITY) packed[j] &= 0xffff0000u;
-                            if (s[2 * j + 1] == -INFINITY) packed[j] &= 0x0000ffffu;
+                            float lo, hi;
+                            halves(s[j], lo, hi);
+                            if (lo == -INFINITY) packed[j] &= 0xffff0000u;
+                            if (hi == -INFINITY) packed[j] &= 0x0000ffffu;
                         }
                     }
-                    sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
-                    umma::st_32x32b_x32(p_addr, packed);
+                    float lo, hi;
+                    halves(add2(sums[0], sums[1]), lo, hi);
+                    sum += lo + hi;
+                    umma::st_32x32b_x32(s_addr, packed);
+                    umma::st_wait();
                 }
-                umma::st_wait();
                 umma::fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&ctl.p_full[grp]));
+                if (lane == 0) mbar_arrive(smem_u32(&ctl.p_full[grp][n & 1]));
                 ++n;
             }
             if (!alive) break;
             kv += item.tiles;
 
             // ---- the two groups' sums meet ----
-            if (item.tiles > grp) {
-                alive = wait(ctl.pv_done[grp], (n - 1) & 1, 16);
-                if (!alive) break;
-            }
+            // (Not by pv_done: two of its phases may be under way, and a wait tells a phase only from its neighbours.)
+            alive = wait(ctl.item_done, n_items & 1, 16);
+            if (!alive) break;
             ctl.unit[grp][r] = m == -INFINITY ? -INFINITY : m * qs + exponent;
             ctl.sum[grp][r] = sum;
             umma::fence_before_sync();
@@ -509,7 +548,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                 umma::fence_before_sync();
             }
             // The first operand's place serves for the pieces' units and sums: all products with it are over.
-            if (!whole) meet<D, ROWS, SOFTMAX_THREADS, 1, T>(p, item, threadIdx.x, reinterpret_cast<float *>(smem_gen), &ctl.last);
+            if (!whole) meet<D, ROWS, SOFTMAX_THREADS, WIDE_FAN, 4, T>(p, item, threadIdx.x, reinterpret_cast<float *>(smem_gen), &ctl.last);
         }
         if (!met) all_of<SOFTMAX_THREADS>(alive);
     }
