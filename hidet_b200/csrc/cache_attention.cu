@@ -121,8 +121,8 @@ __device__ __forceinline__ void finish_item(const AttentionArgs &p, Control &ctl
         if (whole) write_out<D, T>(p, item, r, d, v, sum, top * scale);
         else write_piece<D, ROWS>(piece, r, d, v, sum, top * scale);
     }
-    static_assert(L::BUFFERS * L::MERGE >= 2 * FEW_FAN * ROWS * 4, "");
-    if (!whole) meet<D, ROWS, CONSUMERS, FEW_FAN, 1, T>(p, item, threadIdx.x, merge, &ctl.last);  // whose first barrier frees the merge buffers
+    static_assert(L::BUFFERS * L::MERGE >= 2 * FAN * ROWS * 4, "");
+    if (!whole) meet<D, ROWS, CONSUMERS, 1, T>(p, item, threadIdx.x, merge, &ctl.last);  // whose first barrier frees the merge buffers
 }
 
 template <int D, int NT, typename T>
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
             ++n_items;
         };
 
-        Line<ROWS, FEW_FAN> line(p, lane);
+        Line<ROWS, FAN> line(p, lane);
         Item item;
         const int32_t *table;
         int slot = 0, it = 0;
@@ -517,7 +517,7 @@ B200Q_API size_t b200q_quantized_cache_attention_workspace_bytes(int64_t batch, 
     if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || !cache_dim(head_dim)) return 0;
     const bool wide = wide_rows(tokens, heads / kv_heads, batch, head_dim);
     const int64_t pieces = 2 * (wide ? kMostWideCtas : kMaxCtas), rows = wide ? 128 : 16;
-    return (size_t)(kCounterBytes + pieces * rows * (head_dim + 2) * 4);
+    return (size_t)(kCounterBytes + pieces * rows * (head_dim + 2) * 4 + (wide ? kMostWideCtas * 64 : 0));  // 64: an item's description
 }
 
 B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, float *lse, const void *cache, int64_t pages, int64_t page_size, const int32_t *page_table,
@@ -576,6 +576,7 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
     p.scale_log2 = scale * kLog2e;
     p.counters = static_cast<unsigned int *>(workspace);
     p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kCounterBytes);
+    p.partial_floats = wide_rows(tokens, heads / kv_heads, batch, head_dim) ? 2 * kMostWideCtas * 128 * (head_dim + 2) : 0;
     p.status = device_status_word();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (wide_rows(tokens, heads / kv_heads, batch, head_dim)) return launch_wide(p, (int)head_dim, type == B200Q_BF16, s);

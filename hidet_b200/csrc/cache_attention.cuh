@@ -24,8 +24,7 @@ constexpr float kLeastNormal = 1.1754943508222875e-38f;
 constexpr int TILE = 64;       // positions: four records
 constexpr int RECORDS = 4;
 constexpr int kItemUnits = 2;  // what an item costs besides its tiles, in tiles
-constexpr int FEW_FAN = 8;     // pieces of an item that are added at once: of few rows
-constexpr int WIDE_FAN = 4;    // and of many
+constexpr int FAN = 8;         // pieces of an item that are added at once
 
 struct AttentionArgs {
     const void *q;
@@ -47,6 +46,7 @@ struct AttentionArgs {
     int batch, kv_heads, group;
     float scale_log2;
     float *partial;
+    int64_t partial_floats;  // of all pieces
     unsigned int *counters;
     unsigned int *status;
 };
@@ -136,7 +136,7 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionArgs &p, int b) {
 }
 
 // This CTA's piece of the line of tiles: a sequence's items one behind the other, head by head, and the sequences behind one another.  One warp.
-template <int ROWS, int FAN>
+template <int ROWS, int ROUND>  // ROUND: pieces of an item that are added at once
 struct Line {
     const AttentionArgs &p;
     const int lane;
@@ -164,7 +164,7 @@ struct Line {
         // No more pieces of an item than are added at once, as long as the wait for another round of additions, about two tiles, would be longer
         // than what shorter pieces save.
         int ctas = min((int)gridDim.x, tiles);
-        if (ctas > FAN * items && tiles / (FAN * max(1, items)) - tiles / ctas <= 2) ctas = FAN * items;
+        if (ctas > ROUND * items && tiles / (ROUND * max(1, items)) - tiles / ctas <= 2) ctas = ROUND * items;
         if ((int)blockIdx.x >= ctas) return;
         // Where pieces are long, a gap in front of every item stands for what it costs besides its tiles.
         gap = tiles >= 8 * ctas ? kItemUnits : 0;
@@ -296,7 +296,7 @@ __device__ __forceinline__ void write_piece(float *piece, int r, int d, float4 v
 
 // The sum of `some` pieces for this thread's groups of four elements, GROUPS of them with their loads in flight together.  tops, sums: of the
 // pieces' rows, [FAN][ROWS], filled by all threads in front of the barrier behind the first loads.
-template <int D, int ROWS, int N, int FAN, int GROUPS, typename T, typename PieceOf>
+template <int D, int ROWS, int N, int GROUPS, typename T, typename PieceOf>
 __device__ __forceinline__ void add_pieces(const AttentionArgs &p, const Item &item, const float *tops, const float *sums, int tid, int some, bool done, PieceOf piece_of) {
     bool waited = false;
     for (int i0 = tid; i0 < item.rows * (D / 4) || !waited; i0 += GROUPS * N) {
@@ -335,7 +335,7 @@ __device__ __forceinline__ void add_pieces(const AttentionArgs &p, const Item &i
 
 // The pieces of an item meet: FAN neighbours at a time, in the CTA that arrives last of them, then FAN of those.  N threads, which have written this
 // CTA's piece; scratch: 2 * FAN * ROWS floats.
-template <int D, int ROWS, int N, int FAN, int GROUPS, typename T>
+template <int D, int ROWS, int N, int GROUPS, typename T>
 __device__ __forceinline__ void meet(const AttentionArgs &p, const Item &item, int tid, float *scratch, int *last) {
     int k = blockIdx.x - item.first_cta, n = item.last_cta - item.first_cta + 1, stride = 1;
     auto place = [&](int i) { return (2 * (item.first_cta + i) + (i == 0 ? 1 : 0)) * kPieceFloats<D, ROWS>; };  // 32 bits are enough for the workspace
@@ -362,7 +362,7 @@ __device__ __forceinline__ void meet(const AttentionArgs &p, const Item &item, i
             sums[i] = r < item.rows ? __ldcg(from + ROWS) : 0.0f;
         }
         const bool done = n <= FAN;
-        add_pieces<D, ROWS, N, FAN, GROUPS, T>(p, item, tops, sums, tid, some, done, piece_of);
+        add_pieces<D, ROWS, N, GROUPS, T>(p, item, tops, sums, tid, some, done, piece_of);
         if (done) break;
     }
 }

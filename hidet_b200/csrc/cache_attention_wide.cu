@@ -27,21 +27,13 @@ constexpr int ROWS = 128;
 constexpr int GROUP_WARPS = 4;                  // of a group that turns scores into probabilities
 constexpr int SOFTMAX_THREADS = 2 * 32 * GROUP_WARPS;
 constexpr int CONVERT_WARP0 = 8, PRODUCER_WARP = 12, MMA_WARP = 13;
-constexpr int THREADS = 32 * 16;                // four groups of four warps, for the split of the registers
-// Registers a thread of the groups: softmax (two groups), conversion, the rest.  Together what the block is launched with.
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 192, kConvertRegs = 64, kOtherRegs = 64;
-static_assert(2 * kSoftmaxRegs + kConvertRegs + kOtherRegs <= 4 * kLaunchRegs, "");
-template <int N>
-__device__ __forceinline__ void more_registers() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewer_registers() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
+constexpr int THREADS = 32 * 14;
 constexpr int ITEMS = 2;                        // that the other roles may know of
 constexpr int RAW_STAGES = 3, KV_STAGES = 4;
 constexpr int AHEAD = 2;                        // tiles whose scores are asked for in front of the probabilities of another
+// Items of which the first of several pieces is a CTA's, behind the pieces in the workspace.
+__device__ __forceinline__ Item *split_items(const AttentionArgs &p) { return reinterpret_cast<Item *>(p.partial + p.partial_floats); }
+static_assert(sizeof(Item) <= 64, "");
 constexpr uint32_t TMEM_COLS = 512;
 // Columns of a group's scores, two tiles of them (the probabilities take the place of their scores), and of its sums.
 __device__ __forceinline__ constexpr uint32_t s_col(int group, int buffer) { return 64 * (2 * group + buffer); }
@@ -55,8 +47,10 @@ struct Layout {
     static constexpr int RAW = RECORDS * record_bytes(D);
     static constexpr int KV_AT = Q, RAW_AT = Q + KV_STAGES * KV;
     static constexpr int SMEM = RAW_AT + RAW_STAGES * RAW + 1024;  // 1024: the operands begin at a multiple of it
-    static_assert(2 * WIDE_FAN * ROWS * 4 <= Q, "");
 };
+
+// The position of a record that stands in place j of it (below eight: the first two of every four, above: the others).
+__device__ __forceinline__ uint32_t position_of(uint32_t j) { return 4 * ((j & 7) >> 1) + (j & 1) + 2 * (j >> 3); }
 
 // Two floats in a register pair, for the instructions that take two at once.
 typedef unsigned long long f32x2;
@@ -139,178 +133,164 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
     const uint32_t tmem = ctl.tmem;
 
     auto wait_one = [&](uint64_t &barrier, uint32_t parity, unsigned int site) -> bool {  // one thread's
-        // inline, unlike the other kernels' (a call in a kernel whose groups have registers of their own is not compiled)
         const uint32_t bar = smem_u32(&barrier);
-        if (mbar_wait(bar, parity, umma::kFastPolls)) return true;
-#pragma unroll 1
-        for (uint32_t round = 0; round < kSpinLimit / 1024u; ++round) {
-            if (mbar_wait(bar, parity, 1024u)) return true;
-            if (*reinterpret_cast<volatile int *>(&ctl.abort) != 0) return false;
-        }
-        report_timeout(p.status, kKernelCacheAttentionWide, site);
-        atomicExch(&ctl.abort, 1);
-        return false;
+        return mbar_wait(bar, parity, umma::kFastPolls) || umma::wait_or_abort<kKernelCacheAttentionWide>(bar, parity, site, &ctl.abort, p.status);
     };
     auto wait = [&](uint64_t &barrier, uint32_t parity, unsigned int site) -> bool { return __all_sync(0xffffffffu, wait_one(barrier, parity, site)); };
 
-    if (warp >= PRODUCER_WARP) {
-        fewer_registers<kOtherRegs>();
-        if (warp == PRODUCER_WARP) {
-            // ---------------- plan and copies ----------------
-            pdl_launch_dependents();
-            Line<ROWS, WIDE_FAN> line(p, lane);
-            Item item;
-            const int32_t *table;
-            int n_items = 0, it = 0, slot = 0;
-            uint32_t parity = 0;
-            bool ok = true;
-            auto publish = [&]() {
-                const int at = n_items % ITEMS;
-                if (n_items >= ITEMS) ok = wait(ctl.item_empty[at], (n_items / ITEMS - 1) & 1, 1);
-                if (ok && lane == 0) {
-                    ctl.items[at] = item;
-                    mbar_arrive(smem_u32(&ctl.item_full[at]));
-                }
-                ++n_items;
-            };
-            while (ok && line.next(item, table)) {
-                Pages pages(p, item, lane, table);
-                publish();
-                for (int i = 0; ok && i < item.tiles; ++i) {
-                    const int key0 = (item.tile0 + i) * TILE;
-                    if (it >= RAW_STAGES) ok = wait(ctl.raw_empty[slot], parity ^ 1u, 2);
-                    if (!ok) break;
-                    const uint32_t bar = smem_u32(&ctl.raw_full[slot]);
-                    if (lane == 0) {
-                        const int keys = copied_keys(item, key0);
-                        ctl.key0[slot] = key0;
-                        ctl.length[slot] = item.length;
-                        if (keys > 0) mbar_expect_tx(bar, (uint32_t)(keys >> 4) * record_bytes(D));
-                        else mbar_arrive(bar);
-                    }
-                    __syncwarp();
-                    copy_tile<D>(p, item, pages, lane, key0, smem + L::RAW_AT + slot * L::RAW, bar);
-                    ++it;
-                    if (++slot == RAW_STAGES) slot = 0, parity ^= 1u;
-                }
-            }
-            item.rows = -1;
-            if (ok) publish();
-            if (ok && it >= RAW_STAGES) ok = wait(ctl.raw_empty[slot], parity ^ 1u, 3);
+    if (warp == PRODUCER_WARP) {
+        // ---------------- plan and copies ----------------
+        pdl_launch_dependents();
+        Line<ROWS, 4> line(p, lane);
+        Item item;
+        const int32_t *table;
+        int n_items = 0, it = 0, slot = 0;
+        uint32_t parity = 0;
+        bool ok = true;
+        auto publish = [&]() {
+            const int at = n_items % ITEMS;
+            if (n_items >= ITEMS) ok = wait(ctl.item_empty[at], (n_items / ITEMS - 1) & 1, 1);
             if (ok && lane == 0) {
-                ctl.length[slot] = -1;
-                mbar_arrive(smem_u32(&ctl.raw_full[slot]));
+                ctl.items[at] = item;
+                mbar_arrive(smem_u32(&ctl.item_full[at]));
             }
-            if (!ok) {  // nothing may be on its way when the CTA ends
-                for (int back = 1; back <= RAW_STAGES && back <= it; ++back) {
-                    const int at = it - back;
-                    mbar_wait(smem_u32(&ctl.raw_full[at % RAW_STAGES]), (at / RAW_STAGES) & 1, 1u << 16);
+            ++n_items;
+        };
+        Item *split = split_items(p) + blockIdx.x;  // the item whose first piece of several is here, for the kernel behind
+        if (lane == 0) split->rows = -1;
+        while (ok && line.next(item, table)) {
+            if (lane == 0 && item.first_cta == (int)blockIdx.x && item.last_cta > (int)blockIdx.x) *split = item;
+            Pages pages(p, item, lane, table);
+            publish();
+            for (int i = 0; ok && i < item.tiles; ++i) {
+                const int key0 = (item.tile0 + i) * TILE;
+                if (it >= RAW_STAGES) ok = wait(ctl.raw_empty[slot], parity ^ 1u, 2);
+                if (!ok) break;
+                const uint32_t bar = smem_u32(&ctl.raw_full[slot]);
+                if (lane == 0) {
+                    const int keys = copied_keys(item, key0);
+                    ctl.key0[slot] = key0;
+                    ctl.length[slot] = item.length;
+                    if (keys > 0) mbar_expect_tx(bar, (uint32_t)(keys >> 4) * record_bytes(D));
+                    else mbar_arrive(bar);
                 }
+                __syncwarp();
+                copy_tile<D>(p, item, pages, lane, key0, smem + L::RAW_AT + slot * L::RAW, bar);
+                ++it;
+                if (++slot == RAW_STAGES) slot = 0, parity ^= 1u;
             }
-        } else if (warp == MMA_WARP) {  // the two others are only there for the split of the registers
-            // ---------------- products ----------------
-            if (elect_one()) {
-                const uint32_t qk_desc = umma::instr_desc_f16(ROWS, TILE), pv_desc = umma::instr_desc_f16(ROWS, D);
-                // Products are carried out in the order they are issued, so the second product of a tile frees the place of its scores for a later
-                // tile's without a wait.
-                uint32_t n[2] = {0, 0};  // tiles of the groups, of the items in front
-                int kv = 0;              // of both
-                bool ok = true;
-                for (int n_items = 0; ok; ++n_items) {
-                    ok = wait_one(ctl.item_full[n_items % ITEMS], (n_items / ITEMS) & 1, 4);
-                    if (!ok) break;
-                    const int rows = ctl.items[n_items % ITEMS].rows, tiles = ctl.items[n_items % ITEMS].tiles;
-                    mbar_arrive(smem_u32(&ctl.item_empty[n_items % ITEMS]));
-                    if (rows < 0) break;
-                    ok = wait_one(ctl.q_full, n_items & 1, 5);
-                    for (int i = 0, asked = 0; ok && i < tiles; ++i) {
-                        for (; ok && asked < min(tiles, i + AHEAD + 1); ++asked) {
-                            const int g = asked & 1, buf = (kv + asked) % KV_STAGES;
-                            const uint32_t at = n[g] + (asked >> 1);
-                            ok = wait_one(ctl.kv_full[buf], ((kv + asked) / KV_STAGES) & 1, 6);
-                            if (!ok) break;
-                            umma::fence_after_sync();
-                            const uint64_t a = umma::smem_desc_sw128(smem), b = umma::smem_desc_sw128(smem + L::KV_AT + buf * L::KV);
-#pragma unroll
-                            for (int k = 0; k < D / 16; ++k) {
-                                const int half = k / 4, to = 2 * (k % 4);  // 16-byte units
-                                umma::mma_ss(tmem + s_col(g, at & 1), a + half * (ROWS * 128 / 16) + to, b + half * (TILE * 128 / 16) + to, qk_desc, k > 0);
-                            }
-                            umma::commit(smem_u32(&ctl.s_full[g][at & 1]));
-                        }
-                        if (!ok) break;
-                        const int g = i & 1, buf = (kv + i) % KV_STAGES;
-                        const uint32_t at = n[g] + (i >> 1);
-                        ok = wait_one(ctl.p_full[g][at & 1], (at >> 1) & 1, 8);
+        }
+        item.rows = -1;
+        if (ok) publish();
+        if (ok && it >= RAW_STAGES) ok = wait(ctl.raw_empty[slot], parity ^ 1u, 3);
+        if (ok && lane == 0) {
+            ctl.length[slot] = -1;
+            mbar_arrive(smem_u32(&ctl.raw_full[slot]));
+        }
+        if (!ok) {  // nothing may be on its way when the CTA ends
+            for (int back = 1; back <= RAW_STAGES && back <= it; ++back) {
+                const int at = it - back;
+                mbar_wait(smem_u32(&ctl.raw_full[at % RAW_STAGES]), (at / RAW_STAGES) & 1, 1u << 16);
+            }
+        }
+    } else if (warp == MMA_WARP) {
+        // ---------------- products ----------------
+        if (elect_one()) {
+            const uint32_t qk_desc = umma::instr_desc_f16(ROWS, TILE), pv_desc = umma::instr_desc_f16(ROWS, D);
+            // Products are carried out in the order they are issued, so the second product of a tile frees the place of its scores for a later
+            // tile's without a wait.
+            uint32_t n[2] = {0, 0};  // tiles of the groups, of the items in front
+            int kv = 0;              // of both
+            bool ok = true;
+            for (int n_items = 0; ok; ++n_items) {
+                ok = wait_one(ctl.item_full[n_items % ITEMS], (n_items / ITEMS) & 1, 4);
+                if (!ok) break;
+                const int rows = ctl.items[n_items % ITEMS].rows, tiles = ctl.items[n_items % ITEMS].tiles;
+                mbar_arrive(smem_u32(&ctl.item_empty[n_items % ITEMS]));
+                if (rows < 0) break;
+                ok = wait_one(ctl.q_full, n_items & 1, 5);
+                for (int i = 0, asked = 0; ok && i < tiles; ++i) {
+                    for (; ok && asked < min(tiles, i + AHEAD + 1); ++asked) {
+                        const int g = asked & 1, buf = (kv + asked) % KV_STAGES;
+                        const uint32_t at = n[g] + (asked >> 1);
+                        ok = wait_one(ctl.kv_full[buf], ((kv + asked) / KV_STAGES) & 1, 6);
                         if (!ok) break;
                         umma::fence_after_sync();
-                        const uint64_t b = umma::smem_desc_sw128(smem + L::KV_AT + buf * L::KV + L::K);
+                        const uint64_t a = umma::smem_desc_sw128(smem), b = umma::smem_desc_sw128(smem + L::KV_AT + buf * L::KV);
 #pragma unroll
-                        for (int k = 0; k < TILE / 16; ++k) umma::mma_ts(tmem + o_col(g), tmem + s_col(g, at & 1) + 8 * k, b + 2 * k, pv_desc, i > 1 || k > 0);
-                        umma::commit(smem_u32(&ctl.pv_done[g]));
-                        umma::commit(smem_u32(&ctl.kv_empty[buf]));
+                        for (int k = 0; k < D / 16; ++k) {
+                            const int half = k / 4, to = 2 * (k % 4);  // 16-byte units
+                            umma::mma_ss(tmem + s_col(g, at & 1), a + half * (ROWS * 128 / 16) + to, b + half * (TILE * 128 / 16) + to, qk_desc, k > 0);
+                        }
+                        umma::commit(smem_u32(&ctl.s_full[g][at & 1]));
                     }
                     if (!ok) break;
-                    umma::commit(smem_u32(&ctl.item_done));
-                    kv += tiles;
-                    n[0] += (tiles + 1) >> 1;
-                    n[1] += tiles >> 1;
+                    const int g = i & 1, buf = (kv + i) % KV_STAGES;
+                    const uint32_t at = n[g] + (i >> 1);
+                    ok = wait_one(ctl.p_full[g][at & 1], (at >> 1) & 1, 8);
+                    if (!ok) break;
+                    umma::fence_after_sync();
+                    const uint64_t b = umma::smem_desc_sw128(smem + L::KV_AT + buf * L::KV + L::K);
+#pragma unroll
+                    for (int k = 0; k < TILE / 16; ++k) umma::mma_ts(tmem + o_col(g), tmem + s_col(g, at & 1) + 8 * k, b + 2 * k, pv_desc, i > 1 || k > 0);
+                    umma::commit(smem_u32(&ctl.pv_done[g]));
+                    umma::commit(smem_u32(&ctl.kv_empty[buf]));
                 }
-                umma::commit(smem_u32(&ctl.drained));  // tensor memory is given back when nothing is on its way
-                if (!mbar_wait(smem_u32(&ctl.drained), 0)) report_timeout(p.status, kKernelCacheAttentionWide, 9);
+                if (!ok) break;
+                umma::commit(smem_u32(&ctl.item_done));
+                kv += tiles;
+                n[0] += (tiles + 1) >> 1;
+                n[1] += tiles >> 1;
             }
-            __syncwarp();
+            umma::commit(smem_u32(&ctl.drained));  // tensor memory is given back when nothing is on its way
+            if (!mbar_wait(smem_u32(&ctl.drained), 0)) report_timeout(p.status, kKernelCacheAttentionWide, 9);
         }
+        __syncwarp();
     } else if (warp >= CONVERT_WARP0) {
         // ---------------- codes to f16 ----------------
-        fewer_registers<kConvertRegs>();
-        const int w = warp - CONVERT_WARP0, g = lane >> 2, t = lane & 3;
-        // K: this lane's row of the record, in the order whose ranks give eight lanes eight places
-        const uint32_t row = 4 * ((lane & 7) >> 1) + (lane & 1) + 2 * ((lane >> 3) & 1), sw = k_order(row, D), key = 16 * w + row;
-        const uint32_t v_row = lane & 15, v_sw = v_order(v_row, D);
+        const int w = warp - CONVERT_WARP0;
+        // Matrix stores take the halves of what a transposing load of V leaves in a register (positions 4t .. 4t + 3) apart, so place j of a
+        // record holds position position_of(j), in K, V and the scales alike.  The same order gives eight lanes' rows of K different banks.
+        const uint32_t place = lane & 15, row = position_of(place), sw = k_order(row, D), v_sw = v_order(place, D);
+        const uint32_t k_at = (2 * w + (place >> 3)) * 1024 + (place & 7) * 128;                    // of this lane's row of K
+        const uint32_t v_at = (lane >> 4) * 1024 + (lane & 7) * 128 + (((2 * w + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);  // of its row of a matrix store
         for (int it = 0;; ++it) {
             const int slot = it % RAW_STAGES, buf = it % KV_STAGES;
             if (!wait(ctl.raw_full[slot], (it / RAW_STAGES) & 1, 10)) break;
             const int key0 = ctl.key0[slot] + 16 * w, length = ctl.length[slot];
             if (length < 0) break;
-            if (it >= KV_STAGES && !wait(ctl.kv_empty[buf], (it / KV_STAGES - 1) & 1, 11)) break;
             const uint32_t rec = smem + L::RAW_AT + slot * L::RAW + w * record_bytes(D);
-            const uint32_t k_dst = smem + L::KV_AT + buf * L::KV + (key >> 3) * 1024 + (key & 7) * 128, v_dst = smem + L::KV_AT + buf * L::KV + L::K;
-            if (lane < 16) {
-                const float *scales = reinterpret_cast<const float *>(smem_gen + L::RAW_AT + slot * L::RAW + w * record_bytes(D) + 32 * D);
-                const bool there = key0 + lane < length;  // behind the end, and in records that were not copied, is anything
-                const float ks = there ? scales[lane] : 0.0f, vs = there ? scales[16 + lane] : 0.0f;
-                ctl.k_scale[buf][16 * w + lane] = ks;
-                ctl.v_scale[buf][16 * w + lane] = vs;
-                float top = vs;
+            if (it >= KV_STAGES && !wait(ctl.kv_empty[buf], (it / KV_STAGES - 1) & 1, 11)) break;
+            const uint32_t k_dst = smem + L::KV_AT + buf * L::KV + k_at, v_dst = smem + L::KV_AT + buf * L::KV + L::K + v_at;
+            const float *scales = reinterpret_cast<const float *>(smem_gen + L::RAW_AT + slot * L::RAW + w * record_bytes(D) + 32 * D);
+            const bool there = key0 + (int)row < length;  // behind the end, and in records that were not copied, is anything
+            const float ks = there ? scales[row] : 0.0f, vs = there ? scales[16 + row] : 0.0f;
+            float top = vs;
 #pragma unroll
-                for (int d = 8; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffu, top, d));
-                if (lane == 0) ctl.v_top[buf][w] = top;
-            }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) {  // two chunks of 16 codes of every row
-                const uint32_t c = 2 * i + (lane >> 4);
-                uint32_t x[4], y[8];
+            for (int d = 8; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            if (lane < 16) ctl.k_scale[buf][16 * w + lane] = ks, ctl.v_scale[buf][16 * w + lane] = vs;
+            if (lane == 0) ctl.v_top[buf][w] = top;
+            // Loops that stay loops, here and in the softmax: the roles' code together has to stay in the instruction caches nearest to the
+            // schedulers.  Unrolled, warps waited for instructions more than for anything else (2.8 of 13 clocks an instruction).
+#pragma unroll 1
+            for (int i = 0; i < D / 32; ++i) {
+                const uint32_t c = 2 * i + (lane >> 4), at = (c & 3) * 2;  // chunk of 16 codes of K, and its 16-byte places in a row of 128
+                uint32_t x[4], v[4], y[8];
                 asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(rec + row * D + ((c ^ sw) << 4)));
+                umma::ldmatrix_x2_trans_b8(v, rec + 16 * D + place * D + ((c ^ v_sw) << 4));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) codes_to_f16(x[e], y[2 * e], y[2 * e + 1]);
-                const uint32_t half = c >> 2, at = (c & 3) * 2;  // 16-byte places of a 128-byte row
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(k_dst + half * (TILE * 128) + (((at + e) ^ (key & 7)) << 4)), "r"(y[4 * e]), "r"(y[4 * e + 1]),
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(k_dst + (c >> 2) * (TILE * 128) + (((at + e) ^ (place & 7)) << 4)), "r"(y[4 * e]), "r"(y[4 * e + 1]),
                                  "r"(y[4 * e + 2]), "r"(y[4 * e + 3])
                                  : "memory");
-            }
 #pragma unroll
-            for (int dd = 0; dd < D / 32; ++dd) {
-                uint32_t r[4];
-                umma::ldmatrix_x2_trans_b8(r, rec + 16 * D + v_row * D + (((2 * dd + (lane >> 4)) ^ v_sw) << 4));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {  // element 32 dd + 8 i + g, positions 16 w + 4 t .. + 3
-                    uint32_t lo, hi;
-                    codes_to_f16(r[i], lo, hi);
-                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(v_dst + (4 * dd + i) * 1024 + g * 128 + (((2 * w + (t >> 1)) ^ g) << 4) + 8 * (t & 1)), "r"(lo), "r"(hi) : "memory");
+                for (int h = 0; h < 2; ++h) {  // elements 32 i + 16 h .. + 15 of V: two blocks of eight, two halves of the record's positions each
+                    uint32_t z[4];
+                    codes_to_f16(v[2 * h], z[0], z[1]);
+                    codes_to_f16(v[2 * h + 1], z[2], z[3]);
+                    umma::stmatrix_x4(v_dst + (4 * i + 2 * h) * 1024, z);
                 }
             }
             fence_proxy_async_smem();
@@ -322,7 +302,6 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
         }
     } else {
         // ---------------- scores to probabilities ----------------
-        more_registers<kSoftmaxRegs>();
         const int grp = warp / GROUP_WARPS, quarter = warp % GROUP_WARPS, r = 32 * quarter + lane;  // this thread's row
         const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
         const uint32_t o_addr = tmem + lanes + o_col(grp);
@@ -398,42 +377,52 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                 if (!alive) break;
                 umma::fence_after_sync();
                 if (busy) {
-                    uint32_t raw[TILE];
-                    umma::ld_32x32b_x32(s_addr, *reinterpret_cast<uint32_t (*)[32]>(&raw[0]));
-                    umma::ld_32x32b_x32(s_addr + 32, *reinterpret_cast<uint32_t (*)[32]>(&raw[32]));
-                    umma::ld_wait();
+                    // Two passes over the scores, 32 at a time, rather than one with all in registers.
                     const bool partly = key0 + TILE > hidden;
-                    f32x2 s[TILE / 2];
                     const uint32_t ks = smem_u32(ctl.k_scale[buf]), vs = smem_u32(ctl.v_scale[buf]);
-#pragma unroll
-                    for (int j = 0; j < TILE / 4; ++j) {
-                        f32x2 k0, k1;
-                        scales_at(ks + 16 * j, k0, k1);
-                        s[2 * j] = mul2(pair_of(raw[4 * j], raw[4 * j + 1]), k0);
-                        s[2 * j + 1] = mul2(pair_of(raw[4 * j + 2], raw[4 * j + 3]), k1);
-                    }
+                    uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
                     if (partly) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            uint32_t seen = 0;
+                            seen[h] = 0;
 #pragma unroll 4
-                            for (int j = 0; j < 32; ++j) seen |= (uint32_t)may_see(p, item, r, token, key0 + 32 * h + j) << j;
+                            for (int j = 0; j < 32; ++j) seen[h] |= (uint32_t)may_see(p, item, r, token, key0 + 32 * h + (j & 16) + (int)position_of(j & 15)) << j;
+                        }
+                    }
+                    auto scores = [&](int h, f32x2 (&s)[16]) {
+                        uint32_t raw[32];
+                        umma::ld_32x32b_x32(s_addr + 32 * h, raw);
+                        umma::ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            f32x2 k0, k1;
+                            scales_at(ks + 128 * h + 16 * j, k0, k1);
+                            s[2 * j] = mul2(pair_of(raw[4 * j], raw[4 * j + 1]), k0);
+                            s[2 * j + 1] = mul2(pair_of(raw[4 * j + 2], raw[4 * j + 3]), k1);
+                        }
+                        if (partly) {
+                            const uint32_t bits = h == 0 ? seen[0] : seen[1];
 #pragma unroll
                             for (int j = 0; j < 16; ++j) {
                                 float lo, hi;
-                                halves(s[16 * h + j], lo, hi);
-                                s[16 * h + j] = pair_of(seen >> (2 * j) & 1u ? lo : -INFINITY, seen >> (2 * j + 1) & 1u ? hi : -INFINITY);
+                                halves(s[j], lo, hi);
+                                s[j] = pair_of(bits >> (2 * j) & 1u ? lo : -INFINITY, bits >> (2 * j + 1) & 1u ? hi : -INFINITY);
                             }
                         }
-                    }
+                    };
                     float top = -INFINITY, other = -INFINITY;
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        f32x2 s[16];
+                        scores(h, s);
 #pragma unroll
-                    for (int j = 0; j < TILE / 2; j += 2) {
-                        float lo, hi;
-                        halves(s[j], lo, hi);
-                        top = max3(top, lo, hi);
-                        halves(s[j + 1], lo, hi);
-                        other = max3(other, lo, hi);
+                        for (int j = 0; j < 16; j += 2) {
+                            float lo, hi;
+                            halves(s[j], lo, hi);
+                            top = max3(top, lo, hi);
+                            halves(s[j + 1], lo, hi);
+                            other = max3(other, lo, hi);
+                        }
                     }
                     top = fmaxf(top, other);
                     const float v_top = fmaxf(fmaxf(ctl.v_top[buf][0], ctl.v_top[buf][1]), fmaxf(ctl.v_top[buf][2], ctl.v_top[buf][3]));
@@ -467,34 +456,38 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                     }
                     const f32x2 minus = pair_of(-shift, -shift), scale2 = pair_of(qs, qs), bias = pair_of(kBias - exponent, kBias - exponent);
                     f32x2 sums[2] = {0, 0};
-                    uint32_t packed[TILE / 2];
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        f32x2 s[16];
+                        scores(h, s);
+                        uint32_t packed[16];
 #pragma unroll
-                    for (int j = 0; j < TILE / 4; ++j) {
-                        f32x2 v[2];
-                        scales_at(vs + 16 * j, v[0], v[1]);
+                        for (int j = 0; j < 8; ++j) {
+                            f32x2 v[2];
+                            scales_at(vs + 128 * h + 16 * j, v[0], v[1]);
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float lo, hi;
-                            halves(fma2(add2(s[2 * j + e], minus), scale2, bias), lo, hi);
-                            const f32x2 x = pair_of(ex2(lo), ex2(hi));
-                            sums[e] = add2(sums[e], x);
-                            halves(mul2(x, v[e]), lo, hi);
-                            packed[2 * j + e] = pack_f16(lo, hi);
+                            for (int e = 0; e < 2; ++e) {
+                                float lo, hi;
+                                halves(fma2(add2(s[2 * j + e], minus), scale2, bias), lo, hi);
+                                const f32x2 x = pair_of(ex2(lo), ex2(hi));
+                                sums[e] = add2(sums[e], x);
+                                halves(mul2(x, v[e]), lo, hi);
+                                packed[2 * j + e] = pack_f16(lo, hi);
+                            }
                         }
-                    }
-                    if (partly) {  // nothing, whatever the scale of a position that is not seen
+                        if (partly) {  // nothing, whatever the scale of a position that is not seen
+                            const uint32_t bits = h == 0 ? seen[0] : seen[1];
 #pragma unroll
-                        for (int j = 0; j < TILE / 2; ++j) {
-                            float lo, hi;
-                            halves(s[j], lo, hi);
-                            if (lo == -INFINITY) packed[j] &= 0xffff0000u;
-                            if (hi == -INFINITY) packed[j] &= 0x0000ffffu;
+                            for (int j = 0; j < 16; ++j) {
+                                if (!(bits >> (2 * j) & 1u)) packed[j] &= 0xffff0000u;
+                                if (!(bits >> (2 * j + 1) & 1u)) packed[j] &= 0x0000ffffu;
+                            }
                         }
+                        umma::st_32x32b_x16(s_addr + 16 * h, packed);
                     }
                     float lo, hi;
                     halves(add2(sums[0], sums[1]), lo, hi);
                     sum += lo + hi;
-                    umma::st_32x32b_x32(s_addr, packed);
                     umma::st_wait();
                 }
                 umma::fence_before_sync();
@@ -547,8 +540,6 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                 }
                 umma::fence_before_sync();
             }
-            // The first operand's place serves for the pieces' units and sums: all products with it are over.
-            if (!whole) meet<D, ROWS, SOFTMAX_THREADS, WIDE_FAN, 4, T>(p, item, threadIdx.x, reinterpret_cast<float *>(smem_gen), &ctl.last);
         }
         if (!met) all_of<SOFTMAX_THREADS>(alive);
     }
@@ -560,6 +551,40 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
     }
 }
 
+// Adds the pieces of the items that are in several: a CTA takes ADD_ROWS rows of one, a thread four elements of a row at a time.  (In the CTA that is
+// last with its piece, as the kernel for few rows does it, 128 rows would take 13 us; here they are spread over the device.)
+constexpr int ADD_ROWS = 16, ADD_THREADS = 256;
+template <int D, typename T>
+__global__ void __launch_bounds__(ADD_THREADS) add_pieces_kernel(const __grid_constant__ AttentionArgs p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const Item item = split_items(p)[blockIdx.x];
+    const int row0 = blockIdx.y * ADD_ROWS;
+    if (row0 >= item.rows) return;
+    const int parts = item.last_cta - item.first_cta + 1;
+    for (int i = threadIdx.x; i < ADD_ROWS * D / 4; i += ADD_THREADS) {
+        const int r = row0 + i / (D / 4), d = 4 * (i % (D / 4));
+        if (r >= item.rows) break;
+        const float *first = p.partial + (2 * item.first_cta + 1) * kPieceFloats<D, ROWS>, *others = p.partial + 2 * (item.first_cta + 1) * kPieceFloats<D, ROWS>;
+        auto piece = [&](int j) { return j == 0 ? first : others + (j - 1) * 2 * kPieceFloats<D, ROWS>; };
+        float top = -INFINITY;
+#pragma unroll 8
+        for (int j = 0; j < parts; ++j) top = fmaxf(top, __ldcg(piece(j) + ROWS * D + r));
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int j = 0; j < parts; ++j) {
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(piece(j) + r * D + d));
+            const float own = __ldcg(piece(j) + ROWS * D + r), s = __ldcg(piece(j) + ROWS * (D + 1) + r);
+            // in two steps: units may lie so far apart that the whole factor leaves float's range where the products do not
+            const float by = own == -INFINITY ? 1.0f : ex2(0.5f * (own - top));
+            sum = fmaf(s * by, by, sum);
+            v.x = fmaf(x.x * by, by, v.x), v.y = fmaf(x.y * by, by, v.y), v.z = fmaf(x.z * by, by, v.z), v.w = fmaf(x.w * by, by, v.w);
+        }
+        write_out<D, T>(p, item, r, d, v, sum, top);
+    }
+}
+
 template <int D, typename T>
 int launch_sized(const AttentionArgs &p, cudaStream_t stream) {
     using L = Layout<D>;
@@ -567,21 +592,13 @@ int launch_sized(const AttentionArgs &p, cudaStream_t stream) {
     static std::atomic<bool> attr_set[64];
     const int rc = allow_smem(attr_set, kernel, L::SMEM);
     if (rc != B200Q_OK) return rc;
-    // The registers that the groups take and give have to be there, or their first would wait for good.
-    static std::atomic<int> regs{0};
-    if (regs.load(std::memory_order_relaxed) == 0) {
-        cudaFuncAttributes attributes;
-        B200Q_CUDA_TRY(cudaFuncGetAttributes(&attributes, kernel));
-        regs.store(attributes.numRegs, std::memory_order_relaxed);
-    }
-    if (regs.load(std::memory_order_relaxed) < kLaunchRegs) {
-        return set_error(B200Q_UNSUPPORTED, "quantized_cache_attention: the kernel was built for %d registers a thread, %d are wanted", regs.load(), kLaunchRegs);
-    }
     const int64_t tiles = most_tiles(p, ROWS), at_once = sm_count();
     if (tiles > (1ll << 29)) return set_error(B200Q_UNSUPPORTED, "quantized_cache_attention: up to %lld tiles of %d rows and %d positions", (long long)tiles, ROWS, TILE);
     int64_t grid = tiles < at_once ? tiles : at_once;
     if (grid > kMostWideCtas) grid = kMostWideCtas;
-    return launch_after("cache_attention_wide_kernel", kernel, dim3((unsigned)grid), THREADS, L::SMEM, 1, stream, p);
+    const int status = launch_after("cache_attention_wide_kernel", kernel, dim3((unsigned)grid), THREADS, L::SMEM, 1, stream, p);
+    if (status != B200Q_OK || grid == 1) return status;
+    return launch_after("add_pieces_kernel", add_pieces_kernel<D, T>, dim3((unsigned)grid, ROWS / ADD_ROWS), ADD_THREADS, 0, 1, stream, p);
 }
 
 }  // namespace
