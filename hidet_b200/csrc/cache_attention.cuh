@@ -265,6 +265,26 @@ __device__ __forceinline__ bool may_see(const AttentionArgs &p, const Item &item
     if (p.mask == nullptr) return drafted <= token;
     return drafted < p.mask_width && p.mask[(int64_t)(item.token0 + token) * p.mask_stride + drafted] != 0;
 }
+// The same for the 64 positions from key0 on, as bits.
+__device__ __forceinline__ uint64_t seen_of_64(const AttentionArgs &p, const Item &item, int r, int token, int key0) {
+    if (r >= item.rows) return 0;
+    const int old = item.length - item.fresh;
+    const int sure = p.mask == nullptr ? min(item.length, old + token + 1) - key0 : old - key0;  // positions in front of this one
+    uint64_t seen = sure >= 64 ? ~0ull : sure > 0 ? (1ull << sure) - 1 : 0;
+    if (p.mask != nullptr) {
+        const uint8_t *row = p.mask + (int64_t)(item.token0 + token) * p.mask_stride + (key0 - old);
+        const int from = old - key0, until = min(item.length, old + p.mask_width) - key0;
+#pragma unroll 1
+        for (int h = 0; h < 64; h += 32) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)  // all loads on their way together
+                if (h + j >= from && h + j < until && row[h + j] != 0) bits |= 1u << j;
+            seen |= (uint64_t)bits << h;
+        }
+    }
+    return seen;
+}
 // Positions from here on may be hidden from a row.
 __device__ __forceinline__ int first_hidden(const AttentionArgs &p, const Item &item) {
     const int old = item.length - item.fresh;

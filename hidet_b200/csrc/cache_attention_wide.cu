@@ -50,7 +50,8 @@ struct Layout {
 };
 
 // The position of a record that stands in place j of it (below eight: the first two of every four, above: the others).
-__device__ __forceinline__ uint32_t position_of(uint32_t j) { return 4 * ((j & 7) >> 1) + (j & 1) + 2 * (j >> 3); }
+__device__ __forceinline__ constexpr uint32_t position_of(uint32_t j) { return 4 * ((j & 7) >> 1) + (j & 1) + 2 * (j >> 3); }
+__device__ __forceinline__ constexpr uint32_t position_of32(uint32_t j) { return (j & 16) + position_of(j & 15); }  // of two records
 
 // Two floats in a register pair, for the instructions that take two at once.
 typedef unsigned long long f32x2;
@@ -89,7 +90,8 @@ struct Control {
     uint64_t q_full, s_full[2][2], p_full[2][2], pv_done[2], item_done, drained;  // [group][buffer]
     alignas(16) float k_scale[KV_STAGES][TILE];  // read four at a time
     alignas(16) float v_scale[KV_STAGES][TILE];
-    float v_top[KV_STAGES][RECORDS];
+    alignas(16) float k_top[KV_STAGES][RECORDS];
+    alignas(16) float v_top[KV_STAGES][RECORDS];
     int key0[RAW_STAGES], length[RAW_STAGES];  // length -1: no more tiles
     Item items[ITEMS];
     float top[2][ROWS], unit[2][ROWS], sum[2][ROWS];
@@ -260,26 +262,33 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
             const int key0 = ctl.key0[slot] + 16 * w, length = ctl.length[slot];
             if (length < 0) break;
             const uint32_t rec = smem + L::RAW_AT + slot * L::RAW + w * record_bytes(D);
-            if (it >= KV_STAGES && !wait(ctl.kv_empty[buf], (it / KV_STAGES - 1) & 1, 11)) break;
-            const uint32_t k_dst = smem + L::KV_AT + buf * L::KV + k_at, v_dst = smem + L::KV_AT + buf * L::KV + L::K + v_at;
+            uint32_t x[4], v[4];
+            auto load = [&](int i) {  // a chunk of 16 codes of a row of K, and two 16 x 16 blocks of V
+                const uint32_t c = 2 * i + (lane >> 4);
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(rec + row * D + ((c ^ sw) << 4)));
+                umma::ldmatrix_x2_trans_b8(v, rec + 16 * D + place * D + ((c ^ v_sw) << 4));
+            };
+            load(0);
             const float *scales = reinterpret_cast<const float *>(smem_gen + L::RAW_AT + slot * L::RAW + w * record_bytes(D) + 32 * D);
             const bool there = key0 + (int)row < length;  // behind the end, and in records that were not copied, is anything
             const float ks = there ? scales[row] : 0.0f, vs = there ? scales[16 + row] : 0.0f;
-            float top = vs;
-#pragma unroll
-            for (int d = 8; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            // the largest of each (they are not negative)
+            const uint32_t k_top = __reduce_max_sync(0xffffffffu, ks == ks ? __float_as_uint(ks) : 0u), v_top = __reduce_max_sync(0xffffffffu, vs == vs ? __float_as_uint(vs) : 0u);
+            if (it >= KV_STAGES && !wait(ctl.kv_empty[buf], (it / KV_STAGES - 1) & 1, 11)) break;
+            const uint32_t k_dst = smem + L::KV_AT + buf * L::KV + k_at, v_dst = smem + L::KV_AT + buf * L::KV + L::K + v_at;
             if (lane < 16) ctl.k_scale[buf][16 * w + lane] = ks, ctl.v_scale[buf][16 * w + lane] = vs;
-            if (lane == 0) ctl.v_top[buf][w] = top;
-            // Loops that stay loops, here and in the softmax: the roles' code together has to stay in the instruction caches nearest to the
-            // schedulers.  Unrolled, warps waited for instructions more than for anything else (2.8 of 13 clocks an instruction).
+            if (lane == 0) ctl.k_top[buf][w] = __uint_as_float(k_top), ctl.v_top[buf][w] = __uint_as_float(v_top);
+            // A loop that stays a loop: the roles' code together has to stay in the instruction caches nearest to the schedulers.  Where all was unrolled,
+            // warps waited for instructions more than for anything else (2.8 of 13 clocks an instruction).
 #pragma unroll 1
             for (int i = 0; i < D / 32; ++i) {
-                const uint32_t c = 2 * i + (lane >> 4), at = (c & 3) * 2;  // chunk of 16 codes of K, and its 16-byte places in a row of 128
-                uint32_t x[4], v[4], y[8];
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(rec + row * D + ((c ^ sw) << 4)));
-                umma::ldmatrix_x2_trans_b8(v, rec + 16 * D + place * D + ((c ^ v_sw) << 4));
+                const uint32_t c = 2 * i + (lane >> 4), at = (c & 3) * 2;  // the chunk's 16-byte places in a row of 128
+                uint32_t y[8], z[8];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) codes_to_f16(x[e], y[2 * e], y[2 * e + 1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) codes_to_f16(v[e], z[2 * e], z[2 * e + 1]);
+                if (i + 1 < D / 32) load(i + 1);
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(k_dst + (c >> 2) * (TILE * 128) + (((at + e) ^ (place & 7)) << 4)), "r"(y[4 * e]), "r"(y[4 * e + 1]),
@@ -287,10 +296,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                                  : "memory");
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {  // elements 32 i + 16 h .. + 15 of V: two blocks of eight, two halves of the record's positions each
-                    uint32_t z[4];
-                    codes_to_f16(v[2 * h], z[0], z[1]);
-                    codes_to_f16(v[2 * h + 1], z[2], z[3]);
-                    umma::stmatrix_x4(v_dst + (4 * i + 2 * h) * 1024, z);
+                    const uint32_t block[4] = {z[4 * h], z[4 * h + 1], z[4 * h + 2], z[4 * h + 3]};
+                    umma::stmatrix_x4(v_dst + (4 * i + 2 * h) * 1024, block);
                 }
             }
             fence_proxy_async_smem();
@@ -380,15 +387,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                     // Two passes over the scores, 32 at a time, rather than one with all in registers.
                     const bool partly = key0 + TILE > hidden;
                     const uint32_t ks = smem_u32(ctl.k_scale[buf]), vs = smem_u32(ctl.v_scale[buf]);
-                    uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-                    if (partly) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            seen[h] = 0;
-#pragma unroll 4
-                            for (int j = 0; j < 32; ++j) seen[h] |= (uint32_t)may_see(p, item, r, token, key0 + 32 * h + (j & 16) + (int)position_of(j & 15)) << j;
-                        }
-                    }
+                    uint64_t seen = ~0ull;
+                    if (partly) seen = seen_of_64(p, item, r, token, key0);
                     auto scores = [&](int h, f32x2 (&s)[16]) {
                         uint32_t raw[32];
                         umma::ld_32x32b_x32(s_addr + 32 * h, raw);
@@ -401,32 +401,53 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                             s[2 * j + 1] = mul2(pair_of(raw[4 * j + 2], raw[4 * j + 3]), k1);
                         }
                         if (partly) {
-                            const uint32_t bits = h == 0 ? seen[0] : seen[1];
+                            const uint32_t bits = (uint32_t)(seen >> (32 * h));
 #pragma unroll
                             for (int j = 0; j < 16; ++j) {
                                 float lo, hi;
                                 halves(s[j], lo, hi);
-                                s[j] = pair_of(bits >> (2 * j) & 1u ? lo : -INFINITY, bits >> (2 * j + 1) & 1u ? hi : -INFINITY);
+                                s[j] = pair_of(bits >> position_of32(2 * j) & 1u ? lo : -INFINITY, bits >> position_of32(2 * j + 1) & 1u ? hi : -INFINITY);
                             }
                         }
                     };
-                    float top = -INFINITY, other = -INFINITY;
+                    // Whether a score can pass the maximum so far by too much: first by the largest product and the largest scale.  (Scales are read from
+                    // shared memory by all lanes at once, four bytes a clock; most tiles need those of K once so.)
+                    float top = 0.0f, other = 0.0f;
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
-                        f32x2 s[16];
-                        scores(h, s);
+                        uint32_t raw[32];
+                        umma::ld_32x32b_x32(s_addr + 32 * h, raw);
+                        umma::ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            float lo, hi;
-                            halves(s[j], lo, hi);
-                            top = max3(top, lo, hi);
-                            halves(s[j + 1], lo, hi);
-                            other = max3(other, lo, hi);
+                        for (int j = 0; j < 32; j += 4) {
+                            top = max3(top, __uint_as_float(raw[j]), __uint_as_float(raw[j + 1]));
+                            other = max3(other, __uint_as_float(raw[j + 2]), __uint_as_float(raw[j + 3]));
                         }
                     }
-                    top = fmaxf(top, other);
-                    const float v_top = fmaxf(fmaxf(ctl.v_top[buf][0], ctl.v_top[buf][1]), fmaxf(ctl.v_top[buf][2], ctl.v_top[buf][3]));
-                    if (__any_sync(0xffffffffu, top > m + rise || v_top >= v_limit)) {
+                    const float4 k_tops = *reinterpret_cast<const float4 *>(ctl.k_top[buf]), v_tops = *reinterpret_cast<const float4 *>(ctl.v_top[buf]);
+                    const float k_top = max3(fmaxf(k_tops.x, k_tops.y), k_tops.z, k_tops.w), v_top = max3(fmaxf(v_tops.x, v_tops.y), v_tops.z, v_tops.w);
+                    bool raise = v_top >= v_limit;
+                    if (__any_sync(0xffffffffu, fmaxf(top, other) * k_top > m + rise)) {
+                        top = other = -INFINITY;
+#pragma unroll 1
+                        for (int h = 0; h < 2; ++h) {
+                            f32x2 s[16];
+                            scores(h, s);
+#pragma unroll
+                            for (int j = 0; j < 16; j += 2) {
+                                float lo, hi;
+                                halves(s[j], lo, hi);
+                                top = max3(top, lo, hi);
+                                halves(s[j + 1], lo, hi);
+                                other = max3(other, lo, hi);
+                            }
+                        }
+                        top = fmaxf(top, other);
+                        raise |= top > m + rise;
+                    } else {
+                        top = m;
+                    }
+                    if (__any_sync(0xffffffffu, raise)) {
                         const float was = exponent;
                         if (v_top >= v_limit) {
                             exponent = fmaxf((float)((int)(__float_as_uint(v_top) >> 23) - 127), kLeastUnit);
@@ -476,11 +497,11 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                             }
                         }
                         if (partly) {  // nothing, whatever the scale of a position that is not seen
-                            const uint32_t bits = h == 0 ? seen[0] : seen[1];
+                            const uint32_t bits = (uint32_t)(seen >> (32 * h));
 #pragma unroll
                             for (int j = 0; j < 16; ++j) {
-                                if (!(bits >> (2 * j) & 1u)) packed[j] &= 0xffff0000u;
-                                if (!(bits >> (2 * j + 1) & 1u)) packed[j] &= 0x0000ffffu;
+                                if (!(bits >> position_of32(2 * j) & 1u)) packed[j] &= 0xffff0000u;
+                                if (!(bits >> position_of32(2 * j + 1) & 1u)) packed[j] &= 0x0000ffffu;
                             }
                         }
                         umma::st_32x32b_x16(s_addr + 16 * h, packed);
