@@ -50,6 +50,7 @@ __device__ __forceinline__ uint32_t transpose(uint32_t x) {
     return y;
 }
 constexpr int MOST_STAGES = 6;
+constexpr int kItemUnits = 2;           // what an item costs besides its tiles, in tiles
 constexpr int WARPS = 4;                // that multiply
 constexpr int CONSUMERS = 32 * WARPS;
 constexpr int THREADS = CONSUMERS + 32;
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
             ++n_items;
         };
 
-        Line<ROWS, FAN> line(p, lane);
+        Line<ROWS, FAN, kItemUnits> line(p, lane);
         Item item;
         const int32_t *table;
         int slot = 0, it = 0;
@@ -544,8 +545,8 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
         return set_error(B200Q_INVALID_ARGUMENT, "%s: null pointer argument", op);
     }
     if (pages <= 0 && table_width > 0) return set_error(B200Q_INVALID_ARGUMENT, "%s: a cache of %lld pages", op, (long long)pages);
-    if (!aligned_to(cache, 16) || !aligned_to(q->data, 8) || !aligned_to(out, 8) || q->token_stride % 4 != 0 || q->head_stride % 4 != 0) {
-        return set_error(B200Q_INVALID_ARGUMENT, "%s: a 16-byte aligned cache, 8-byte aligned q and out and strides of 4 elements are wanted", op);
+    if (!aligned_to(cache, 16) || !aligned_to(q->data, 16) || !aligned_to(out, 16) || q->token_stride % 8 != 0 || q->head_stride % 8 != 0) {
+        return set_error(B200Q_INVALID_ARGUMENT, "%s: 16-byte aligned cache, q and out and strides of 8 elements are wanted", op);
     }
     const size_t need = b200q_quantized_cache_attention_workspace_bytes(batch, tokens, heads, kv_heads, head_dim);
     if (workspace == nullptr || workspace_bytes < need) return set_error(B200Q_WORKSPACE_TOO_SMALL, "%s: a workspace of %zu bytes is needed, got %zu", op, need, workspace_bytes);

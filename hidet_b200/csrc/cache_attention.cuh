@@ -23,7 +23,6 @@ constexpr float kLeastNormal = 1.1754943508222875e-38f;
 
 constexpr int TILE = 64;       // positions: four records
 constexpr int RECORDS = 4;
-constexpr int kItemUnits = 2;  // what an item costs besides its tiles, in tiles
 constexpr int FAN = 8;         // pieces of an item that are added at once
 
 struct AttentionArgs {
@@ -136,7 +135,7 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionArgs &p, int b) {
 }
 
 // This CTA's piece of the line of tiles: a sequence's items one behind the other, head by head, and the sequences behind one another.  One warp.
-template <int ROWS, int ROUND>  // ROUND: pieces of an item that are added at once
+template <int ROWS, int ROUND, int UNITS>  // ROUND: pieces of an item that are added at once; UNITS: what an item costs besides its tiles, in tiles
 struct Line {
     const AttentionArgs &p;
     const int lane;
@@ -167,7 +166,7 @@ struct Line {
         if (ctas > ROUND * items && tiles / (ROUND * max(1, items)) - tiles / ctas <= 2) ctas = ROUND * items;
         if ((int)blockIdx.x >= ctas) return;
         // Where pieces are long, a gap in front of every item stands for what it costs besides its tiles.
-        gap = tiles >= 8 * ctas ? kItemUnits : 0;
+        gap = tiles >= 8 * ctas ? UNITS : 0;
         const int units = tiles + items * gap;
         each = units / ctas;
         more = units - each * ctas;
@@ -291,6 +290,9 @@ __device__ __forceinline__ int first_hidden(const AttentionArgs &p, const Item &
     return p.mask != nullptr ? old : min(old + 1, item.length);
 }
 
+__device__ __forceinline__ void write_lse(const AttentionArgs &p, int64_t at, float sum, float top) {
+    if (p.lse != nullptr) p.lse[at] = sum == 0.0f ? -INFINITY : (top - kBias + __log2f(sum)) * kLn2;
+}
 // Four elements of a query row's result, from the sum of its values and of its probabilities, both in units of 2^top.
 template <int D, typename T>
 __device__ __forceinline__ void write_out(const AttentionArgs &p, const Item &item, int r, int d, float4 v, float sum, float top) {
@@ -299,7 +301,7 @@ __device__ __forceinline__ void write_out(const AttentionArgs &p, const Item &it
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     T y[4] = {Elems<T>::round(v.x * inv), Elems<T>::round(v.y * inv), Elems<T>::round(v.z * inv), Elems<T>::round(v.w * inv)};
     *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at * D + d) = *reinterpret_cast<const uint2 *>(y);
-    if (d == 0 && p.lse != nullptr) p.lse[at] = sum == 0.0f ? -INFINITY : (top - kBias + __log2f(sum)) * kLn2;
+    if (d == 0) write_lse(p, at, sum, top);
 }
 
 // A piece in the workspace: [ROWS][D] sums of values, then the rows' units (log2) and sums of probabilities.

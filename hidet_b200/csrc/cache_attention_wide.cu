@@ -28,6 +28,7 @@ constexpr int GROUP_WARPS = 4;                  // of a group that turns scores 
 constexpr int SOFTMAX_THREADS = 2 * 32 * GROUP_WARPS;
 constexpr int CONVERT_WARP0 = 8, PRODUCER_WARP = 12, MMA_WARP = 13;
 constexpr int THREADS = 32 * 14;
+constexpr int kItemUnits = 8;                   // what an item costs besides its tiles, in tiles
 constexpr int ITEMS = 2;                        // that the other roles may know of
 constexpr int RAW_STAGES = 3, KV_STAGES = 4;
 constexpr int AHEAD = 2;                        // tiles whose scores are asked for in front of the probabilities of another
@@ -42,6 +43,7 @@ constexpr float kLeastUnit = -90.0f;            // exponents of value scales bel
 
 template <int D>
 struct Layout {
+    // Pieces in the workspace: four elements of all rows, the next four, ..., then the rows' units (log2) and sums of probabilities.
     static constexpr int Q = ROWS * D * 2;
     static constexpr int K = TILE * D * 2, V = D * TILE * 2, KV = K + V;
     static constexpr int RAW = RECORDS * record_bytes(D);
@@ -143,7 +145,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
     if (warp == PRODUCER_WARP) {
         // ---------------- plan and copies ----------------
         pdl_launch_dependents();
-        Line<ROWS, 4> line(p, lane);
+        Line<ROWS, 4, kItemUnits> line(p, lane);
         Item item;
         const int32_t *table;
         int n_items = 0, it = 0, slot = 0;
@@ -328,46 +330,47 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
             // ---- the queries: group 0 brings the first half of a row, group 1 the second ----
             float qs = p.scale_log2;
             {
-                constexpr int N = D / 2;
-                uint4 x[N / 8];
-                const T *src = static_cast<const T *>(p.q) + (int64_t)(item.token0 + token) * p.q_token + (int64_t)(item.head * p.group + item.row0 + r - token * p.group) * p.q_head + grp * N;
+                // Of the warp's 32 rows, D / 2 elements each: LANES lanes take a row, 16 bytes each, so that what a load brings lies together.
+                constexpr int LANES = D / 16, STEP = 32 / LANES;
+                uint4 x[LANES];
 #pragma unroll
-                for (int i = 0; i < N / 8; ++i) {
-                    uint2 a = make_uint2(0, 0), b = a;
-                    if (r < item.rows) a = reinterpret_cast<const uint2 *>(src)[2 * i], b = reinterpret_cast<const uint2 *>(src)[2 * i + 1];
-                    x[i] = make_uint4(a.x, a.y, b.x, b.y);
+                for (int i = 0; i < LANES; ++i) {
+                    const int own = 32 * quarter + STEP * i + lane / LANES, row = item.row0 + own, tok = row / p.group;
+                    const T *src = static_cast<const T *>(p.q) + (int64_t)(item.token0 + tok) * p.q_token + (int64_t)(item.head * p.group + row - tok * p.group) * p.q_head;
+                    x[i] = own < item.rows ? *reinterpret_cast<const uint4 *>(src + grp * (D / 2) + 8 * (lane % LANES)) : make_uint4(0, 0, 0, 0);
                 }
-                float down = 1.0f;
-                if (std::is_same<T, __nv_bfloat16>::value) {
-                    float top = 0.0f;
+                constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;
+                if (kScaled) {
 #pragma unroll
-                    for (int i = 0; i < N / 8; ++i) {
+                    for (int i = 0; i < LANES; ++i) {
                         const T *v = reinterpret_cast<const T *>(&x[i]);
+                        float top = 0.0f;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(Elems<T>::one(v[e])));
+#pragma unroll
+                        for (int d = 1; d < LANES; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        if (lane % LANES == 0) ctl.top[grp][32 * quarter + STEP * i + lane / LANES] = top;
                     }
-                    ctl.top[grp][r] = top;
                 }
                 if (!all_of<SOFTMAX_THREADS>(true)) {  // behind it no thread reads or writes anything of the item in front
                     met = true;
                     break;
                 }
-                if (std::is_same<T, __nv_bfloat16>::value) {
-                    const float top = fmaxf(ctl.top[0][r], ctl.top[1][r]);
-                    const uint32_t e = min(max(__float_as_uint(top) >> 23, 64u), 253u);
-                    if (top > 0.0f) down = __uint_as_float((254u - e) << 23), qs *= __uint_as_float(e << 23);
-                }
+                auto exponent_of = [&](int row) { return min(max(__float_as_uint(fmaxf(ctl.top[0][row], ctl.top[1][row])) >> 23, 64u), 253u); };
+                if (kScaled) qs *= __uint_as_float(exponent_of(r) << 23);
 #pragma unroll
-                for (int i = 0; i < N / 8; ++i) {
-                    if (std::is_same<T, __nv_bfloat16>::value) {
+                for (int i = 0; i < LANES; ++i) {
+                    const int own = 32 * quarter + STEP * i + lane / LANES;
+                    if (kScaled) {
+                        const float down = __uint_as_float((254u - exponent_of(own)) << 23);
                         const T *v = reinterpret_cast<const T *>(&x[i]);
                         uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) w[e] = pack_f16(Elems<T>::one(v[2 * e]) * down, Elems<T>::one(v[2 * e + 1]) * down);
                         x[i] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    const int c = grp * (N / 8) + i;  // 16-byte chunk of the row
-                    *reinterpret_cast<uint4 *>(smem_gen + (c >> 3) * (ROWS * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[i];
+                    const int c = grp * LANES + lane % LANES;  // 16-byte chunk of the row
+                    *reinterpret_cast<uint4 *>(smem_gen + (c >> 3) * (ROWS * 128) + (own >> 3) * 1024 + (own & 7) * 128 + (((c & 7) ^ (own & 7)) << 4)) = x[i];
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -545,17 +548,26 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                     umma::ld_32x32b_x32(tmem + lanes + o_col(1) + c, b);
                     umma::ld_wait();
                     if (r < item.rows) {
+                        float v[32];
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            float v[4];
+                        for (int j = 0; j < 32; ++j) {  // the second sum begins with the item's second tile
+                            v[j] = __uint_as_float(a[j]) * f0 * f0;
+                            if (item.tiles > 1) v[j] = fmaf(__uint_as_float(b[j]) * f1, f1, v[j]);
+                        }
+                        if (whole) {
+                            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+                            const int row = item.row0 + r, head = item.head * p.group + row - token * p.group;
+                            const int64_t at = (int64_t)(item.token0 + token) * p.kv_heads * p.group + head;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {  // the second sum begins with the item's second tile
-                                v[e] = __uint_as_float(a[j + e]) * f0 * f0;
-                                if (item.tiles > 1) v[e] = fmaf(__uint_as_float(b[j + e]) * f1, f1, v[e]);
+                            for (int j = 0; j < 32; j += 8) {
+                                const float y[8] = {v[j] * inv, v[j + 1] * inv, v[j + 2] * inv, v[j + 3] * inv, v[j + 4] * inv, v[j + 5] * inv, v[j + 6] * inv, v[j + 7] * inv};
+                                store8<T, true>(static_cast<T *>(p.out) + at * D + c + j, narrow<T>(y));
                             }
-                            const float4 v4 = make_float4(v[0], v[1], v[2], v[3]);
-                            if (whole) write_out<D, T>(p, item, r, c + j, v4, total, unit);
-                            else write_piece<D, ROWS>(piece, r, c + j, v4, total, unit);
+                            if (c == 0) write_lse(p, at, total, unit);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) __stcg(reinterpret_cast<float4 *>(piece) + (c + j) / 4 * ROWS + r, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
+                            if (c == 0) __stcg(piece + ROWS * D + r, unit), __stcg(piece + ROWS * (D + 1) + r, total);
                         }
                     }
                 }
@@ -584,8 +596,8 @@ __global__ void __launch_bounds__(ADD_THREADS) add_pieces_kernel(const __grid_co
     if (row0 >= item.rows) return;
     const int parts = item.last_cta - item.first_cta + 1;
     for (int i = threadIdx.x; i < ADD_ROWS * D / 4; i += ADD_THREADS) {
-        const int r = row0 + i / (D / 4), d = 4 * (i % (D / 4));
-        if (r >= item.rows) break;
+        const int r = row0 + i % ADD_ROWS, d = 4 * (i / ADD_ROWS);
+        if (r >= item.rows) continue;
         const float *first = p.partial + (2 * item.first_cta + 1) * kPieceFloats<D, ROWS>, *others = p.partial + 2 * (item.first_cta + 1) * kPieceFloats<D, ROWS>;
         auto piece = [&](int j) { return j == 0 ? first : others + (j - 1) * 2 * kPieceFloats<D, ROWS>; };
         float top = -INFINITY;
@@ -595,7 +607,7 @@ __global__ void __launch_bounds__(ADD_THREADS) add_pieces_kernel(const __grid_co
         float sum = 0.0f;
 #pragma unroll 4
         for (int j = 0; j < parts; ++j) {
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(piece(j) + r * D + d));
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(piece(j)) + d / 4 * ROWS + r);
             const float own = __ldcg(piece(j) + ROWS * D + r), s = __ldcg(piece(j) + ROWS * (D + 1) + r);
             // in two steps: units may lie so far apart that the whole factor leaves float's range where the products do not
             const float by = own == -INFINITY ? 1.0f : ex2(0.5f * (own - top));

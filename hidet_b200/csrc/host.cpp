@@ -423,7 +423,7 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     const int64_t batch = lengths->size(0), heads = q->size(-2), kv_heads = cache->size(1), tokens = q->dim() == 3 ? q->size(0) : q->size(0) * q->size(1);
     Where w;
     PLAIN_OR_NONE(batch > 0 && pages->size(0) == batch && pages->size(1) > 0 && heads % kv_heads == 0 && where_is(*q, w) && cache->get_device() == w.device &&
-                  pages->get_device() == w.device && lengths->get_device() == w.device && (reinterpret_cast<uintptr_t>(q->const_data_ptr()) & 7u) == 0);
+                  pages->get_device() == w.device && lengths->get_device() == w.device && (reinterpret_cast<uintptr_t>(q->const_data_ptr()) & 15u) == 0);
     const at::Tensor *starts = nullptr, *mask = nullptr;
     if (args[4] != Py_None) {
         starts = plain_tensor(args[4]);

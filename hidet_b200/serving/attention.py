@@ -55,8 +55,8 @@ def quantized_cache_attention(q: torch.Tensor, cache: torch.Tensor, page_table: 
     elif q.shape[0] != batch:
         raise ValueError('{} sequences have lengths, {} have rows of q'.format(batch, q.shape[0]))
     rows, _ = heads_of(q, 'q', list(q.shape[:-2]), dim)
-    if rows.data_ptr() % 8 != 0 or rows.stride(0) % 4 != 0 or rows.stride(1) % 4 != 0:
-        rows = rows.clone(memory_format=torch.contiguous_format)  # loads of four elements
+    if rows.data_ptr() % 16 != 0 or rows.stride(0) % 8 != 0 or rows.stride(1) % 8 != 0:
+        rows = rows.clone(memory_format=torch.contiguous_format)  # loads of eight elements
     tokens = rows.shape[0]
     if mask is not None:
         if mask.dtype not in (torch.bool, torch.uint8) or mask.dim() != 2 or mask.shape[0] != tokens:

@@ -349,7 +349,8 @@ B200Q_API int b200q_quantized_cache_read(const void *cache, int64_t pages, int64
  * them those up to itself, or, with a mask, those with mask[row * mask_stride + j] != 0 (a byte for the j-th of its sequence's new tokens, j < mask_width).
  * A row that sees nothing has zeros, and -inf in lse.  head h reads key/value head h / (heads / kv_heads).
  *   out[row, h] = sum_j softmax_j(scale q . k_j) v_j, dense [tokens, heads, head_dim] in q's type (f16 or bf16); lse (float [tokens, heads], may be
- * NULL) the natural logarithm of the softmax's denominator.  q: 8-byte aligned, strides multiples of 4 elements.
+ * NULL) the natural logarithm of the softmax's denominator.  q and out: 16-byte aligned,
+ * strides multiples of 8 elements.
  * The workspace is one of b200q_qlinear_f16_i8's kind: zero-filled once, its counters are zero again after every call.
  */
 B200Q_API size_t b200q_quantized_cache_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
