@@ -516,9 +516,9 @@ B200Q_API size_t b200q_quantized_cache_attention_workspace_bytes(int64_t batch, 
     using namespace b200q;
     using namespace b200q::cache_attention;
     if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || !cache_dim(head_dim)) return 0;
-    const bool wide = wide_rows(tokens, heads / kv_heads, batch, head_dim);
-    const int64_t pieces = 2 * (wide ? kMostWideCtas : kMaxCtas), rows = wide ? 128 : 16;
-    return (size_t)(kCounterBytes + pieces * rows * (head_dim + 2) * 4 + (wide ? kMostWideCtas * 64 : 0));  // 64: an item's description
+    const int64_t few = (int64_t)2 * kMaxCtas * 16 * (head_dim + 2) * 4;
+    const int64_t many = may_be_wide(tokens, heads / kv_heads, batch, head_dim) ? (int64_t)2 * kMostWideCtas * 128 * (head_dim + 2) * 4 + kMostWideCtas * 64 : 0;  // 64: an item's description
+    return (size_t)(kCounterBytes + (few > many ? few : many));
 }
 
 B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, float *lse, const void *cache, int64_t pages, int64_t page_size, const int32_t *page_table,
@@ -577,10 +577,10 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
     p.scale_log2 = scale * kLog2e;
     p.counters = static_cast<unsigned int *>(workspace);
     p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kCounterBytes);
-    p.partial_floats = wide_rows(tokens, heads / kv_heads, batch, head_dim) ? 2 * kMostWideCtas * 128 * (head_dim + 2) : 0;
+    p.partial_floats = (int64_t)2 * kMostWideCtas * 128 * (head_dim + 2);  // of the kernel for many rows
     p.status = device_status_word();
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (wide_rows(tokens, heads / kv_heads, batch, head_dim)) return launch_wide(p, (int)head_dim, type == B200Q_BF16, s);
+    if (is_wide(p, head_dim)) return launch_wide(p, (int)head_dim, type == B200Q_BF16, s);
     return type == B200Q_F16 ? launch_typed<__half>(p, (int)head_dim, s) : launch_typed<__nv_bfloat16>(p, (int)head_dim, s);
 }
 
