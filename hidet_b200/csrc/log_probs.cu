@@ -21,7 +21,7 @@ namespace b200q {
 namespace {
 
 constexpr unsigned int kKernelLogProbs = 8;
-constexpr int THREADS = 512;
+constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int GROUPS = 64;               // thread i belongs to group i % 64
 constexpr int MOST_TOP = 32;
@@ -49,13 +49,18 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// 16 bytes of logits.
+// 16 bytes of logits.  pairs: as floats, none below a number whose probability is zero beside any other, so that this times it is zero as well.
 template <typename T>
 struct Vec16;
 template <>
 struct Vec16<float> {
     static constexpr int N = 4;
     static __device__ __forceinline__ void widen(uint4 v, float (&f)[4]) { f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w); }
+    static __device__ __forceinline__ void pairs(uint4 v, f32x2 (&p)[2]) {
+        float f[4];
+        widen(v, f);
+        p[0] = pair_of(fmaxf(f[0], -1e30f), fmaxf(f[1], -1e30f)), p[1] = pair_of(fmaxf(f[2], -1e30f), fmaxf(f[3], -1e30f));
+    }
     static __device__ __forceinline__ float top(uint4 v) {
         float f[4];
         widen(v, f);
@@ -74,6 +79,14 @@ struct Vec16<__half> {
             f[2 * i] = p.x, f[2 * i + 1] = p.y;
         }
     }
+    static __device__ __forceinline__ void pairs(uint4 v, f32x2 (&p)[4]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(__hmax2(h2(w[i]), __float2half2_rn(-65504.0f)));
+            p[i] = pair_of(f.x, f.y);
+        }
+    }
     static __device__ __forceinline__ float top(uint4 v) {
         const __half2 m = __hmax2_nan(__hmax2_nan(h2(v.x), h2(v.y)), __hmax2_nan(h2(v.z), h2(v.w)));
         return max_nan(__low2float(m), __high2float(m));
@@ -87,6 +100,15 @@ struct Vec16<__nv_bfloat16> {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+    static __device__ __forceinline__ void pairs(uint4 v, f32x2 (&p)[4]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 b = __hmax2(b2(w[i]), __float2bfloat162_rn(-1e30f));
+            const uint32_t u = *reinterpret_cast<const uint32_t *>(&b);
+            p[i] = pair_of(u << 16, u & 0xffff0000u);
+        }
     }
     static __device__ __forceinline__ float top(uint4 v) {
         const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(b2(v.x), b2(v.y)), __hmax2_nan(b2(v.z), b2(v.w)));
@@ -236,19 +258,31 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
 
     // ---- the sums ----
     const float shift = fabsf(m) < INFINITY ? m : 0.0f;
-    float sum = 0.0f, weighted = 0.0f;
+    float sum, weighted;
+    {
+        const f32x2 minus = pair_of(-shift, -shift), log2e = pair_of(kLog2e, kLog2e);
+        f32x2 sums = 0, products = 0;
 #pragma unroll 2
-    for (int v = threadIdx.x; v < vecs; v += THREADS) {
-        float f[N];
-        Vec16<T>::widen(x[v], f);
+        for (int v = threadIdx.x; v < vecs; v += THREADS) {
+            f32x2 f[N / 2];
+            Vec16<T>::pairs(x[v], f);
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float y = fmaxf((f[e] - shift) * kLog2e, -200.0f);  // a probability of zero adds 0 * -200
-            float z;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z) : "f"(y));
-            sum += z;
-            weighted = fmaf(z, y, weighted);
+            for (int e = 0; e < N / 2; ++e) {
+                const f32x2 y = mul2(add2(f[e], minus), log2e);  // zero for the largest
+                float lo, hi;
+                halves(y, lo, hi);
+                asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(lo));
+                asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(hi));
+                const f32x2 z = pair_of(lo, hi);
+                sums = add2(sums, z);
+                products = fma2(z, y, products);
+            }
         }
+        float lo, hi;
+        halves(sums, lo, hi);
+        sum = lo + hi;
+        halves(products, lo, hi);
+        weighted = lo + hi;
     }
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) {
