@@ -9,10 +9,10 @@
 // behind its last 16-byte boundary by loads) and read from there twice: for the maximum of every thread, and for the sums.  Bound by the
 // copy where rows are many.  CTAs of a row are a cluster and meet in the shared memory of the first.
 //
-// The maxima of 64 groups of threads bound the alternatives: at least `top` elements are no smaller than the top-th largest of them,
-// so only threads whose own maximum passes that bound hold candidates (some 1.2 * top on random rows); their elements are looked at again by all
-// threads, and the candidates put in order by counting.  Rows made to defeat this (thousands of candidates in few threads) take a slower
-// way: one search for each alternative.
+// The maxima of 64 groups of threads bound the alternatives: at least `top` elements are no smaller than the top-th largest of them.  So what the second
+// reading passes over is compared with that bound, eight elements at once, and the few that reach it (some 1.2 * top on random rows) are put
+// in order by counting.  Where there are too many (rows made so, or vocabularies of fewer elements than the groups need) there is a search for each
+// alternative.
 #include <atomic>
 
 #include "serving.cuh"
@@ -23,7 +23,7 @@ namespace {
 constexpr unsigned int kKernelLogProbs = 8;
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
-constexpr int GROUPS = 64;               // thread i belongs to group i % 64
+constexpr int GROUPS = 64;               // four lanes of a warp each
 constexpr int MOST_TOP = 32;
 constexpr int MOST_CLUSTER = 8;
 constexpr int CANDIDATES = 512;
@@ -142,14 +142,15 @@ struct Block {
     uint64_t bar;
     float m[WARPS], sum[WARPS], weighted[WARPS];
     uint64_t group_key[GROUPS];
-    uint64_t bound, found;
+    uint64_t bound;
     uint64_t warp_key[WARPS];
-    int n_threads, n_candidates;
-    uint16_t threads[THREADS];
-    uint64_t candidates[CANDIDATES];  // first the keys of all threads
+    uint64_t best[MOST_TOP];
+    int n_candidates, n_vectors;
+    uint16_t vectors[CANDIDATES];  // that hold candidates
+    uint64_t candidates[CANDIDATES];
     Share shares[MOST_CLUSTER];
 };
-static_assert(sizeof(Block) <= 8704 && CANDIDATES >= THREADS && CANDIDATES >= MOST_CLUSTER * MOST_TOP, "");
+static_assert(sizeof(Block) <= 8704 && CANDIDATES >= MOST_CLUSTER * MOST_TOP && THREADS == 4 * GROUPS, "");
 
 // Puts the n keys of `keys` in descending order; the first `top` go to `best` (0 where there are fewer).  All threads.
 __device__ __forceinline__ void order_keys(const uint64_t *keys, int n, int top, uint64_t *best) {
@@ -175,7 +176,8 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
     if (threadIdx.x == 0) {
         mbar_init(bar, 1);
         mbar_fence_init();
-        blk.n_threads = blk.n_candidates = 0;
+        blk.n_candidates = blk.n_vectors = 0;
+        blk.bound = 0;
     }
     if (ranks > 1) cluster_arrive_release();
     __syncthreads();
@@ -209,9 +211,11 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
     }
     // the given tokens' logits, by the first CTA
     float own_logit = 0.0f;
+    bool inside = true;
     if (rank == 0 && threadIdx.x < p.given) {
         const int64_t token = index_at(p.tokens, p.token_bytes, row * p.given + threadIdx.x);
-        own_logit = token >= 0 && token < p.vocab ? Elems<T>::one(static_cast<const T *>(p.logits)[row * p.row_stride + token]) : -INFINITY;
+        inside = token >= 0 && token < p.vocab;
+        own_logit = inside ? Elems<T>::one(static_cast<const T *>(p.logits)[row * p.row_stride + token]) : -INFINITY;
     }
     __syncthreads();
     if (!mbar_wait(bar, 0)) {
@@ -223,7 +227,7 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
     // ---- the maximum of every thread, and the first vector that it stands in ----
     float most = -INFINITY;
     int at = threadIdx.x;
-#pragma unroll 4
+#pragma unroll 8
     for (int v = threadIdx.x; v < vecs; v += THREADS) {
         const float y = Vec16<T>::top(x[v]);
         if (!(y <= most) && most == most) {  // a NaN stays
@@ -231,30 +235,43 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
             at = v;
         }
     }
-    const uint64_t own_key = (int)threadIdx.x < vecs ? key_of(most, at) : 0;
+    uint64_t key = (int)threadIdx.x < vecs ? key_of(most, at) : 0;
     float m = most;
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
     if (lane == 0) blk.m[warp] = m;
-    if (p.top > 0) blk.candidates[threadIdx.x] = own_key;
+    if (p.top > 0) {
+#pragma unroll
+        for (int d = 8; d < 32; d *= 2) {
+            const uint64_t other = __shfl_xor_sync(0xffffffffu, key, d);
+            key = other > key ? other : key;
+        }
+        if (lane < 8) blk.group_key[8 * warp + lane] = key;
+    }
     __syncthreads();
     m = blk.m[0];
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) m = max_nan(m, blk.m[w]);
-    if (p.top > 0 && threadIdx.x < GROUPS) {  // the top-th largest of the groups' keys
-        uint64_t own = 0;
+    uint64_t bound = 0;
+    if (p.top > 0) {  // the top-th largest of the groups' keys: four threads compare one with all
+        const int g = threadIdx.x / 4;
+        const uint64_t own = blk.group_key[g];
+        int before = 0;
 #pragma unroll
-        for (int i = 0; i < THREADS / GROUPS; ++i) {
-            const uint64_t k = blk.candidates[threadIdx.x + i * GROUPS];
-            own = k > own ? k : own;
+        for (int i = 0; i < GROUPS / 4; ++i) {
+            const int j = 4 * i + threadIdx.x % 4;
+            const uint64_t k = blk.group_key[j];
+            before += k > own || (k == own && j < g);
         }
-        blk.group_key[threadIdx.x] = own;
-        asm volatile("bar.sync 1, %0;" ::"n"(GROUPS) : "memory");
-        int r = 0;
-#pragma unroll 16
-        for (int j = 0; j < GROUPS; ++j) r += blk.group_key[j] > own || (blk.group_key[j] == own && j < (int)threadIdx.x);
-        if (r == p.top - 1) blk.bound = own;
+        before += __shfl_xor_sync(0xffffffffu, before, 1);
+        before += __shfl_xor_sync(0xffffffffu, before, 2);
+        if (before == p.top - 1 && threadIdx.x % 4 == 0) blk.bound = own;
+        __syncthreads();
+        bound = blk.bound;
     }
+    // With fewer groups than alternatives there is no bound, and nothing is collected.
+    const bool collect = bound != 0;
+    const float least = collect ? value_of(bound) : INFINITY;
 
     // ---- the sums ----
     const float shift = fabsf(m) < INFINITY ? m : 0.0f;
@@ -262,10 +279,15 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
     {
         const f32x2 minus = pair_of(-shift, -shift), log2e = pair_of(kLog2e, kLog2e);
         f32x2 sums = 0, products = 0;
-#pragma unroll 2
+#pragma unroll 4
         for (int v = threadIdx.x; v < vecs; v += THREADS) {
             f32x2 f[N / 2];
-            Vec16<T>::pairs(x[v], f);
+            const uint4 raw = x[v];
+            if (!(Vec16<T>::top(raw) < least)) {  // rarely; NaN too
+                const int k = atomicAdd(&blk.n_vectors, 1);
+                if (k < CANDIDATES) blk.vectors[k] = (uint16_t)v;
+            }
+            Vec16<T>::pairs(raw, f);
 #pragma unroll
             for (int e = 0; e < N / 2; ++e) {
                 const f32x2 y = mul2(add2(f[e], minus), log2e);  // zero for the largest
@@ -293,28 +315,25 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
 
     // ---- this part's best ----
     Share &mine = blk.shares[0];
+    __syncthreads();
     if (p.top > 0) {
-        __syncthreads();
-        const uint64_t bound = blk.bound;
-        if (own_key != 0 && own_key >= bound) blk.threads[atomicAdd(&blk.n_threads, 1)] = (uint16_t)threadIdx.x;
-        __syncthreads();
-        const int each = (vecs + THREADS - 1) / THREADS, looks = blk.n_threads * each;
-        for (int i = threadIdx.x; i < looks; i += THREADS) {
-            const int v = blk.threads[i / each] + (i % each) * THREADS;
-            if (v >= vecs) continue;
-            float f[N];
-            Vec16<T>::widen(x[v], f);
+        if (collect && blk.n_vectors <= CANDIDATES) {
+            for (int i = threadIdx.x; i < blk.n_vectors; i += THREADS) {
+                const int v = blk.vectors[i];
+                float f[N];
+                Vec16<T>::widen(x[v], f);
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const int index = v * N + e - lead;
-                if (index >= 0 && index < n && key_of(f[e], v) >= bound) {
-                    const int k = atomicAdd(&blk.n_candidates, 1);
-                    if (k < CANDIDATES) blk.candidates[k] = key_of(f[e], (uint32_t)(from + index));
+                for (int e = 0; e < N; ++e) {
+                    const int index = v * N + e - lead;
+                    if (!(f[e] < least) && index >= 0 && index < n && key_of(f[e], (uint32_t)v) >= bound) {
+                        const int k = atomicAdd(&blk.n_candidates, 1);
+                        if (k < CANDIDATES) blk.candidates[k] = key_of(f[e], (uint32_t)(from + index));
+                    }
                 }
             }
+            __syncthreads();
         }
-        __syncthreads();
-        if (blk.n_candidates <= CANDIDATES) {
+        if (collect && blk.n_vectors <= CANDIDATES && blk.n_candidates <= CANDIDATES) {
             order_keys(blk.candidates, blk.n_candidates, p.top, mine.best);
         } else {
             uint64_t last = ~0ull;
@@ -345,13 +364,13 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
             }
         }
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        float s = 0.0f, w = 0.0f;
-        for (int i = 0; i < WARPS; ++i) s += blk.sum[i], w += blk.weighted[i];
+    float part_sum = 0.0f, part_weighted = 0.0f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) part_sum += blk.sum[i], part_weighted += blk.weighted[i];
+    if (ranks > 1 && threadIdx.x == 0) {
         mine.m = m;
-        mine.sum = s;
-        mine.weighted = w;
+        mine.sum = part_sum;
+        mine.weighted = part_weighted;
     }
     __syncthreads();
 
@@ -369,23 +388,27 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
         cluster_wait_acquire();
         if (rank > 0) return;
     }
-    float all_m = blk.shares[0].m;
-    for (uint32_t r = 1; r < ranks; ++r) all_m = max_nan(all_m, blk.shares[r].m);
-    float all_sum = 0.0f, all_weighted = 0.0f;  // the latter of (x - all_m) log2(e)
-    for (uint32_t r = 0; r < ranks; ++r) {
-        const Share &s = blk.shares[r];
-        if (!(fabsf(s.m) < INFINITY)) continue;  // nothing above -inf in it; +inf and NaN are told by all_m
-        const float down = (s.m - all_m) * kLog2e, by = exp2f(down);
-        all_sum = fmaf(s.sum, by, all_sum);
-        all_weighted = fmaf(fmaf(s.sum, fmaxf(down, -200.0f), s.weighted), by, all_weighted);
+    float all_m = m, all_sum = part_sum, all_weighted = part_weighted;  // the latter of (x - all_m) log2(e)
+    if (ranks > 1) {
+        for (uint32_t r = 1; r < ranks; ++r) all_m = max_nan(all_m, blk.shares[r].m);
+        all_sum = all_weighted = 0.0f;
+        for (uint32_t r = 0; r < ranks; ++r) {
+            const Share &s = blk.shares[r];
+            if (!(fabsf(s.m) < INFINITY)) continue;  // nothing above -inf in it; +inf and NaN are told by all_m
+            const float down = (s.m - all_m) * kLog2e, by = exp2f(down);
+            all_sum = fmaf(s.sum, by, all_sum);
+            all_weighted = fmaf(fmaf(s.sum, fmaxf(down, -200.0f), s.weighted), by, all_weighted);
+        }
     }
     if (!(fabsf(all_m) < INFINITY)) all_sum = __uint_as_float(0x7fc00000u);
     const float log_sum = logf(all_sum), lse = all_m + log_sum;
     if (threadIdx.x == 0) p.entropy[row] = log_sum - all_weighted / all_sum * kLn2;
     for (int64_t i = threadIdx.x; i < p.given; i += THREADS) {
-        const int64_t token = index_at(p.tokens, p.token_bytes, row * p.given + i);
-        const bool inside = token >= 0 && token < p.vocab;
-        if (i >= THREADS) own_logit = inside ? Elems<T>::one(static_cast<const T *>(p.logits)[row * p.row_stride + token]) : -INFINITY;
+        if (i >= THREADS) {
+            const int64_t token = index_at(p.tokens, p.token_bytes, row * p.given + i);
+            inside = token >= 0 && token < p.vocab;
+            own_logit = inside ? Elems<T>::one(static_cast<const T *>(p.logits)[row * p.row_stride + token]) : -INFINITY;
+        }
         if (!inside && p.status != nullptr) atomicOr(p.status, kBadToken);
         p.log_probs[row * p.given + i] = own_logit - lse;
     }
@@ -395,9 +418,9 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
             uint64_t *keys = blk.candidates;
             for (int i = threadIdx.x; i < (int)ranks * p.top; i += THREADS) keys[i] = blk.shares[i / p.top].best[i % p.top];
             __syncthreads();
-            order_keys(keys, (int)ranks * p.top, p.top, blk.group_key);
+            order_keys(keys, (int)ranks * p.top, p.top, blk.best);
             __syncthreads();
-            best = blk.group_key;
+            best = blk.best;
         }
         if (threadIdx.x < p.top) {
             const uint64_t key = best[threadIdx.x];
