@@ -16,7 +16,7 @@
 namespace b200q {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;      // of a block, at most
 constexpr float kTinyRow = 7.8886090522101180541e-31f;  // 2^-100
 
 struct HeadRows {
@@ -56,78 +56,121 @@ __device__ __forceinline__ void load_floats(const float *p, float (&f)[N]) {
     }
 }
 
-// Two chunks of eight elements of one head, whose pairs are (half) across them, from angle i on, or (interleaved) inside them.
+// The two chunks of eight elements of a head that lane j of its dim / 16 lanes holds, so that neighbouring lanes have neighbouring chunks: partners of a
+// rotation (half), or half a head apart.
+__device__ __forceinline__ void chunks_of(int j, int dim, const RotaryArgs &r, int &a, int &b) {
+    const int pairs = r.interleaved ? 0 : r.rotary_dim >> 4, rest = (dim >> 4) - pairs;
+    a = j < pairs ? j : pairs + j;
+    b = j < pairs ? j + pairs : pairs + j + rest;
+}
+
+// Cosines and sines for a lane's two chunks: of eight pairs of elements, or (interleaved) of four of each chunk.
+struct Angles {
+    f32x2 c[4], s[4];
+};
 template <bool VEC>
-__device__ __forceinline__ void rotate_chunks(float (&a)[8], float (&b)[8], const float *angles, int half_dim, int i, bool interleaved) {
-    alignas(16) float c[8], s[8];
-    load_floats<VEC>(angles + i, c);
-    load_floats<VEC>(angles + half_dim + i, s);
+__device__ __forceinline__ void load_pairs(const float *p, f32x2 &a, f32x2 &b) {
+    alignas(16) float x[4];
+    load_floats<VEC>(p, x);
+    a = pair_of(x[0], x[1]), b = pair_of(x[2], x[3]);
+}
+template <bool VEC>
+__device__ __forceinline__ Angles angles_for(const float *row, const RotaryArgs &r, int ca, int cb) {
+    Angles g;
+    const int half = r.rotary_dim >> 1;
+    const int i = r.interleaved ? min(4 * ca, half - 4) : 8 * ca, j = r.interleaved ? min(4 * cb, half - 4) : 8 * ca + 4;  // a chunk that is not rotated takes any
+    load_pairs<VEC>(row + i, g.c[0], g.c[1]);
+    load_pairs<VEC>(row + j, g.c[2], g.c[3]);
+    load_pairs<VEC>(row + half + i, g.s[0], g.s[1]);
+    load_pairs<VEC>(row + half + j, g.s[2], g.s[3]);
+    return g;
+}
+// Whether the chunks are rotated: both of a pair, or (interleaved) each by itself.
+struct Turned {
+    bool a, b;
+};
+__device__ __forceinline__ Turned turned(const RotaryArgs &r, int ca, int cb) { return {8 * ca < r.rotary_dim, 8 * cb < r.rotary_dim}; }
+
+// a cos - b sin and b cos + a sin, every product and sum rounded by itself.
+__device__ __forceinline__ void rotate_chunks(f32x2 (&a)[4], f32x2 (&b)[4], const Angles &g, bool interleaved, Turned t) {
     if (interleaved) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            rotate(a[2 * e], a[2 * e + 1], c[e], s[e]);
-            rotate(b[2 * e], b[2 * e + 1], c[e + 4], s[e + 4]);
-        }
-    } else {
+            float c[2], s[2], x, y;
+            halves(g.c[e], c[0], c[1]);
+            halves(g.s[e], s[0], s[1]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) rotate(a[e], b[e], c[e], s[e]);
+            for (int h = 0; h < 2; ++h) {  // the two pairs of elements that these angles turn
+                f32x2 &pair = e < 2 ? a[2 * e + h] : b[2 * (e - 2) + h];
+                if (!(e < 2 ? t.a : t.b)) continue;
+                halves(pair, x, y);
+                rotate(x, y, c[h], s[h]);
+                pair = pair_of(x, y);
+            }
+        }
+    } else if (t.a) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // one by one: a product and a sum of packed pairs become one instruction with one rounding
+            float a0, a1, b0, b1, c0, c1, s0, s1;
+            halves(a[e], a0, a1), halves(b[e], b0, b1), halves(g.c[e], c0, c1), halves(g.s[e], s0, s1);
+            rotate(a0, b0, c0, s0);
+            rotate(a1, b1, c1, s1);
+            a[e] = pair_of(a0, a1), b[e] = pair_of(b0, b1);
+        }
     }
 }
 
-// The two chunks of a head that lane j of its dim / 16 lanes holds: partners of a rotation as long as there are such.
-__device__ __forceinline__ void chunks_of(int j, int rotary_dim, bool interleaved, int &a, int &b) {
-    const int pairs = rotary_dim >> 4;
-    const bool across = !interleaved && j < pairs;
-    a = across ? j : 2 * j;
-    b = across ? j + pairs : 2 * j + 1;
+__device__ __forceinline__ void zero_turned(f32x2 (&a)[4], f32x2 (&b)[4], Turned t) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (t.a) a[e] = 0;
+        if (t.b) b[e] = 0;
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
 // rotary_embedding
 // ---------------------------------------------------------------------------------------------
 
-// A thread takes two chunks of eight elements of a head (dim / 16 threads a head).  One or a few CTAs a token where tokens are few, and several
-// tokens a CTA where they are many, so that a thread has about four such units: (2048 tokens, 64 + 8 heads of 128, bf16).
+// A thread takes two chunks of eight elements of one head of one token (dim / 16 threads a head, threadIdx.x), with everything on its way at once but the angles, which
+// wait for the position.  Few registers and many threads: with four heads a thread, which would save the other three's angles, (2048 tokens, 64 + 8 heads
+// of 128) took 28.7 us for 21.2 with indexes divided out of one number.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(HeadRows q, HeadRows k, HeadRows q_out, HeadRows k_out, RotaryArgs r, int64_t tokens, int heads, int all_heads,
-                                                          int dim, int tokens_per_cta) {
+__global__ void __launch_bounds__(kThreads, 6) rotary_kernel(const __grid_constant__ HeadRows q, const __grid_constant__ HeadRows k, const __grid_constant__ HeadRows q_out,
+                                                              const __grid_constant__ HeadRows k_out, const __grid_constant__ RotaryArgs r, int64_t tokens, int heads, int all_heads,
+                                                              int dim) {
     pdl_wait();
     pdl_launch_dependents();
-    const int lanes = dim >> 4, units = all_heads * lanes;
-    const int64_t first = (int64_t)blockIdx.x * tokens_per_cta;
-    const int n = (int)min((int64_t)tokens_per_cta, tokens - first) * units;
-#pragma unroll 2
-    for (int u = blockIdx.y * kThreads + threadIdx.x; u < n; u += gridDim.y * kThreads) {
-        const int t = u / units, in_token = u - t * units;
-        const int head = in_token / lanes, j = in_token - head * lanes;
-        const int64_t token = first + t;
-        const bool is_q = head < heads;
-        const HeadRows &src = is_q ? q : k, &dst = is_q ? q_out : k_out;
-        const int h = is_q ? head : head - heads;
-        int ca, cb;
-        chunks_of(j, r.rotary_dim, r.interleaved, ca, cb);
-        const T *x = static_cast<const T *>(src.data) + token * src.token_stride + h * src.head_stride;
-        T *y = static_cast<T *>(dst.data) + token * dst.token_stride + h * dst.head_stride;
-        const Pack8<T> xa = load8<T, VEC>(x + 8 * ca), xb = load8<T, VEC>(x + 8 * cb);
-        if (16 * j < r.rotary_dim) {
-            const float *angles = angles_of(r, token);
-            float a[8], b[8];
-            if (angles != nullptr) {
-                widen(xa, a);
-                widen(xb, b);
-                rotate_chunks<VEC>(a, b, angles, r.rotary_dim >> 1, 8 * j, r.interleaved);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) a[e] = b[e] = 0.0f;
-                if (in_token == 0 && r.status != nullptr) atomicOr(r.status, kBadPosition);
-            }
-            store8<T, VEC>(y + 8 * ca, narrow<T>(a));
-            store8<T, VEC>(y + 8 * cb, narrow<T>(b));
-        } else if (x != y) {
-            store8<T, VEC>(y + 8 * ca, xa);
-            store8<T, VEC>(y + 8 * cb, xb);
+    const int j = threadIdx.x, head = blockIdx.y * blockDim.y + threadIdx.y;
+    const int64_t token = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
+    if (token >= tokens || head >= all_heads) return;
+    const bool is_q = head < heads;
+    const HeadRows &src = is_q ? q : k, &dst = is_q ? q_out : k_out;
+    const int h = is_q ? head : head - heads;
+    int ca, cb;
+    chunks_of(j, dim, r, ca, cb);
+    const T *x = static_cast<const T *>(src.data) + token * src.token_stride + h * src.head_stride;
+    T *y = static_cast<T *>(dst.data) + token * dst.token_stride + h * dst.head_stride;
+    const Turned t = turned(r, ca, cb);
+    if (!t.a && !t.b && x == y) return;
+    Pack8<T> xa = load8<T, VEC>(x + 8 * ca), xb = load8<T, VEC>(x + 8 * cb);
+    if (t.a || t.b) {
+        const float *row = angles_of(r, token);
+        f32x2 a[4], b[4];
+        Pairs<T>::widen(xa, a);
+        Pairs<T>::widen(xb, b);
+        if (row != nullptr) {
+            const Angles g = angles_for<VEC>(row, r, ca, cb);
+            rotate_chunks(a, b, g, r.interleaved, t);
+        } else {
+            zero_turned(a, b, t);
+            if (j == 0 && head == 0 && r.status != nullptr) atomicOr(r.status, kBadPosition);
         }
+        xa = Pairs<T>::narrow(a);
+        xb = Pairs<T>::narrow(b);
     }
+    store8<T, VEC>(y + 8 * ca, xa);
+    store8<T, VEC>(y + 8 * cb, xb);
 }
 
 // Any sizes: a thread per pair, and per element that is only copied.
@@ -170,97 +213,100 @@ __global__ void __launch_bounds__(kThreads) rotary_generic_kernel(HeadRows q, He
 // ---------------------------------------------------------------------------------------------
 
 // Codes of eight elements, plus 128, as bytes: adding 1.5 * 2^23 + 128 rounds to the nearest even integer and leaves it in the low byte.
-__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float inv) {
-    uint32_t m[8];
+__device__ __forceinline__ uint2 codes_of(const f32x2 (&x)[4], float inv) {
+    uint32_t u[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.0f + 128.0f));
-    uint2 r;
-    r.x = __byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410);
-    r.y = __byte_perm(__byte_perm(m[4], m[5], 0x0040), __byte_perm(m[6], m[7], 0x0040), 0x5410);
+    for (int i = 0; i < 4; ++i) {
+        float lo, hi;
+        halves(x[i], lo, hi);
+        u[2 * i] = __float_as_uint(__fadd_rn(__fmul_rn(lo, inv), 12582912.0f + 128.0f));
+        u[2 * i + 1] = __float_as_uint(__fadd_rn(__fmul_rn(hi, inv), 12582912.0f + 128.0f));
+    }
+    return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
+}
+// The largest magnitude of both; NaN stays.
+__device__ __forceinline__ float larger(float top, float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(x)));
     return r;
 }
 
-// GROUP lanes (dim / 16 of them active) hold a row: a head of q (rotated and written), of k (rotated and quantized) or of v (quantized).
+// GROUP lanes (threadIdx.x, dim / 16 of them active) hold a row: a head of q (rotated and written), of k (rotated and quantized) or of v (quantized).
 template <typename T, bool VEC, int GROUP>
-__global__ void __launch_bounds__(kThreads) append_kernel(HeadRows q, HeadRows q_out, HeadRows k, HeadRows v, uint8_t *cache, CacheShape c, const void *slots, int slot_bytes,
-                                                          RotaryArgs r, int64_t tokens, int heads, int tokens_per_cta) {
+__global__ void __launch_bounds__(kThreads, 6) append_kernel(const __grid_constant__ HeadRows q, const __grid_constant__ HeadRows q_out, const __grid_constant__ HeadRows k,
+                                                              const __grid_constant__ HeadRows v, uint8_t *cache, const __grid_constant__ CacheShape c, const void *slots, int slot_bytes,
+                                                              const __grid_constant__ RotaryArgs r, int64_t tokens, int heads) {
     pdl_wait();
     pdl_launch_dependents();
-    const int j = threadIdx.x % GROUP, rows = heads + 2 * c.kv_heads;
-    const bool active = 16 * j < c.dim;
-    const int64_t first = (int64_t)blockIdx.x * tokens_per_cta;
-    const int n = (int)min((int64_t)tokens_per_cta, tokens - first) * rows;
-    constexpr int PER_CTA = kThreads / GROUP;
-    const bool across = r.rotary_dim > 0;  // 0: nothing is rotated
-    // every lane of a warp makes the same number of rounds, for the shuffles
-    const int rounds = (n - (int)blockIdx.y * PER_CTA + (int)gridDim.y * PER_CTA - 1) / ((int)gridDim.y * PER_CTA);
-    for (int round = 0; round < rounds; ++round) {
-        const int u = (round * gridDim.y + blockIdx.y) * PER_CTA + threadIdx.x / GROUP;
-        const bool there = u < n;
-        const int t = there ? u / rows : 0, in_token = there ? u - t * rows : 0;
-        const int64_t token = first + t;
-        const bool is_q = in_token < heads, is_v = in_token >= heads + c.kv_heads;
-        const int h = is_q ? in_token : is_v ? in_token - heads - c.kv_heads : in_token - heads;
-        const HeadRows &src = is_q ? q : is_v ? v : k;
-        const bool rotated = across && !is_v && 16 * j < r.rotary_dim;
-        int ca = 2 * j, cb = 2 * j + 1;
-        if (across && !is_v) chunks_of(j, r.rotary_dim, r.interleaved, ca, cb);
-        float a[8], b[8];
+    const int j = threadIdx.x, row = blockIdx.y * blockDim.y + threadIdx.y, rows = heads + 2 * c.kv_heads;
+    const int64_t token = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
+    const bool active = token < tokens && row < rows && 16 * j < c.dim;
+    const bool is_q = row < heads, is_v = row >= heads + c.kv_heads;
+    const int h = is_q ? row : is_v ? row - heads - c.kv_heads : row - heads;
+    const HeadRows &src = is_q ? q : is_v ? v : k;
+    int ca, cb;
+    chunks_of(j, c.dim, r, ca, cb);
+    f32x2 a[4], b[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] = b[e] = 0.0f;
-        if (there && active) {
-            const T *x = static_cast<const T *>(src.data) + token * src.token_stride + h * src.head_stride;
-            const Pack8<T> xa = load8<T, VEC>(x + 8 * ca), xb = load8<T, VEC>(x + 8 * cb);
-            const float *angles = rotated ? angles_of(r, token) : nullptr;
-            if (rotated && angles == nullptr) {
-                if (in_token == 0 && j == 0 && r.status != nullptr) atomicOr(r.status, kBadPosition);
-            } else {
-                widen(xa, a);
-                widen(xb, b);
-            }
-            if (angles != nullptr) rotate_chunks<VEC>(a, b, angles, r.rotary_dim >> 1, 8 * j, r.interleaved);
+    for (int e = 0; e < 4; ++e) a[e] = b[e] = 0;
+    int64_t slot = -1;
+    if (active) {
+        const T *x = static_cast<const T *>(src.data) + token * src.token_stride + h * src.head_stride;
+        const Pack8<T> xa = load8<T, VEC>(x + 8 * ca), xb = load8<T, VEC>(x + 8 * cb);
+        if (!is_q) slot = index_at(slots, slot_bytes, token);
+        const Turned t = turned(r, ca, cb);
+        const bool turns = r.rotary_dim > 0 && !is_v && (t.a || t.b);
+        const float *angles = turns ? angles_of(r, token) : nullptr;
+        Angles g;
+        if (angles != nullptr) g = angles_for<VEC>(angles, r, ca, cb);
+        Pairs<T>::widen(xa, a);
+        Pairs<T>::widen(xb, b);
+        if (angles != nullptr) {
+            rotate_chunks(a, b, g, r.interleaved, t);
+        } else if (turns) {
+            zero_turned(a, b, t);
+            if (row == 0 && j == 0 && r.status != nullptr) atomicOr(r.status, kBadPosition);
         }
-        // max |x| as bits: NaNs and infinities are larger than every finite value
-        uint32_t top = 0;
+    }
+    if (active && is_q) {
+        T *y = static_cast<T *>(q_out.data) + token * q_out.token_stride + h * q_out.head_stride;
+        store8<T, VEC>(y + 8 * ca, Pairs<T>::narrow(a));
+        store8<T, VEC>(y + 8 * cb, Pairs<T>::narrow(b));
+    }
+    if (!__any_sync(0xffffffffu, active && !is_q)) return;  // nothing to quantize in this warp
+    float top = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(b[e]) & 0x7fffffffu));
+    for (int e = 0; e < 4; ++e) {
+        float lo, hi;
+        halves(a[e], lo, hi);
+        top = larger(larger(top, lo), hi);
+        halves(b[e], lo, hi);
+        top = larger(larger(top, lo), hi);
+    }
 #pragma unroll
-        for (int d = GROUP / 2; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-        if (!there || !active) continue;
-        if (is_q) {
-            T *y = static_cast<T *>(q_out.data) + token * q_out.token_stride + h * q_out.head_stride;
-            store8<T, VEC>(y + 8 * ca, narrow<T>(a));
-            store8<T, VEC>(y + 8 * cb, narrow<T>(b));
-            continue;
-        }
-        const int64_t slot = index_at(slots, slot_bytes, token);
-        if (slot < 0) continue;  // padding
-        if (slot >= c.slots) {
-            if (in_token == heads && j == 0 && r.status != nullptr) atomicOr(r.status, kBadSlot);
-            continue;
-        }
-        const float amax = __uint_as_float(top);
-        const bool fine = top < 0x7f800000u && amax >= kTinyRow;
-        const float inv = fine ? __fdiv_rn(127.0f, amax) : 0.0f;
-        if (!fine) {  // 0 * inf is no zero
+    for (int d = GROUP / 2; d > 0; d /= 2) top = larger(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (!active || is_q) return;
+    if (slot < 0) return;  // padding
+    if (slot >= c.slots) {
+        if (row == heads && j == 0 && r.status != nullptr) atomicOr(r.status, kBadSlot);
+        return;
+    }
+    const bool fine = top < INFINITY && top >= kTinyRow;
+    const float inv = fine ? __fdiv_rn(127.0f, top) : 0.0f;
+    if (!fine) {  // 0 * inf is no zero
 #pragma unroll
-            for (int e = 0; e < 8; ++e) a[e] = b[e] = 0.0f;
-        }
-        uint32_t row;
-        uint8_t *record = record_of(cache, c, slot, h, row);
-        const uint32_t order = is_v ? v_order(row, c.dim) : k_order(row, c.dim);
-        uint8_t *codes = record + (is_v ? 16 * c.dim : 0) + row * c.dim;
-        const uint2 xa = codes_of(a, inv), xb = codes_of(b, inv);
-        if (cb == ca + 1 && (ca & 1) == 0) {
-            *reinterpret_cast<uint4 *>(codes + 16 * (((uint32_t)ca >> 1) ^ order)) = make_uint4(xa.x, xa.y, xb.x, xb.y);
-        } else {
-            *reinterpret_cast<uint2 *>(codes + 16 * (((uint32_t)ca >> 1) ^ order) + 8 * (ca & 1)) = xa;
-            *reinterpret_cast<uint2 *>(codes + 16 * (((uint32_t)cb >> 1) ^ order) + 8 * (cb & 1)) = xb;
-        }
-        if (j == 0) {
-            const float scale = fine ? __fdiv_rn(amax, 127.0f) : top < 0x7f800000u ? 0.0f : __uint_as_float(0x7fc00000u);
-            reinterpret_cast<float *>(record + 32 * c.dim)[(is_v ? 16 : 0) + row] = scale;
-        }
+        for (int e = 0; e < 4; ++e) a[e] = b[e] = 0;
+    }
+    uint32_t in_record;
+    uint8_t *record = record_of(cache, c, slot, h, in_record);
+    const uint32_t order = is_v ? v_order(in_record, c.dim) : k_order(in_record, c.dim);
+    uint8_t *codes = record + (is_v ? 16 * c.dim : 0) + in_record * c.dim;
+    *reinterpret_cast<uint2 *>(codes + 16 * (((uint32_t)ca >> 1) ^ order) + 8 * (ca & 1)) = codes_of(a, inv);
+    *reinterpret_cast<uint2 *>(codes + 16 * (((uint32_t)cb >> 1) ^ order) + 8 * (cb & 1)) = codes_of(b, inv);
+    if (j == 0) {
+        const float scale = fine ? __fdiv_rn(top, 127.0f) : top < INFINITY ? 0.0f : __uint_as_float(0x7fc00000u);
+        reinterpret_cast<float *>(record + 32 * c.dim)[(is_v ? 16 : 0) + in_record] = scale;
     }
 }
 
@@ -268,57 +314,52 @@ __global__ void __launch_bounds__(kThreads) append_kernel(HeadRows q, HeadRows q
 // quantized_cache_read
 // ---------------------------------------------------------------------------------------------
 
-// A thread restores one 16-byte chunk of a row; the rows of k and of v of a token are taken by the same CTA.
+// A thread restores eight elements of a row of K and the same of V.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) read_kernel(const uint8_t *cache, CacheShape c, const void *slots, int slot_bytes, T *k, T *v, int64_t tokens,
-                                                        int tokens_per_cta, unsigned int *status) {
+__global__ void __launch_bounds__(kThreads) read_kernel(const uint8_t *cache, const __grid_constant__ CacheShape c, const void *slots, int slot_bytes, T *k, T *v, int64_t tokens,
+                                                            unsigned int *status) {
     pdl_wait();
     pdl_launch_dependents();
-    const int chunks = c.dim >> 4, units = 2 * c.kv_heads * chunks;
-    const int64_t first = (int64_t)blockIdx.x * tokens_per_cta;
-    const int n = (int)min((int64_t)tokens_per_cta, tokens - first) * units;
-#pragma unroll 2
-    for (int u = blockIdx.y * kThreads + threadIdx.x; u < n; u += gridDim.y * kThreads) {
-        const int t = u / units, in_token = u - t * units;
-        const int unit_row = in_token / chunks, chunk = in_token - unit_row * chunks;
-        const bool is_v = unit_row >= c.kv_heads;
-        const int h = is_v ? unit_row - c.kv_heads : unit_row;
-        const int64_t token = first + t, slot = index_at(slots, slot_bytes, token);
-        float lo[8], hi[8];
-        if (slot < 0 || slot >= c.slots) {
-            if (slot >= c.slots && in_token == 0 && status != nullptr) atomicOr(status, kBadSlot);
+    const int j = threadIdx.x, h = blockIdx.y * blockDim.y + threadIdx.y;
+    const int64_t token = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
+    if (token >= tokens || h >= c.kv_heads) return;
+    const int64_t slot = index_at(slots, slot_bytes, token);
+    uint2 x[2] = {make_uint2(0x80808080u, 0x80808080u), make_uint2(0x80808080u, 0x80808080u)};
+    float scale[2] = {0.0f, 0.0f};
+    if (slot >= 0 && slot < c.slots) {
+        uint32_t in_record;
+        const uint8_t *record = record_of(const_cast<uint8_t *>(cache), c, slot, h, in_record), *codes = record + in_record * c.dim + 8 * (j & 1);
+        x[0] = *reinterpret_cast<const uint2 *>(codes + 16 * (((uint32_t)j >> 1) ^ k_order(in_record, c.dim)));
+        x[1] = *reinterpret_cast<const uint2 *>(codes + 16 * c.dim + 16 * (((uint32_t)j >> 1) ^ v_order(in_record, c.dim)));
+        scale[0] = reinterpret_cast<const float *>(record + 32 * c.dim)[in_record];
+        scale[1] = reinterpret_cast<const float *>(record + 32 * c.dim)[16 + in_record];
+    } else if (slot >= c.slots && j == 0 && h == 0 && status != nullptr) {
+        atomicOr(status, kBadSlot);
+    }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) lo[e] = hi[e] = 0.0f;
-        } else {
-            uint32_t row;
-            const uint8_t *record = record_of(const_cast<uint8_t *>(cache), c, slot, h, row);
-            const uint32_t order = is_v ? v_order(row, c.dim) : k_order(row, c.dim);
-            const uint4 x = *reinterpret_cast<const uint4 *>(record + (is_v ? 16 * c.dim : 0) + row * c.dim + 16 * ((uint32_t)chunk ^ order));
-            const float scale = reinterpret_cast<const float *>(record + 32 * c.dim)[(is_v ? 16 : 0) + row];
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    for (int i = 0; i < 2; ++i) {
+        f32x2 y[4];
+        const f32x2 minus = pair_of(-(8388608.0f + 128.0f), -(8388608.0f + 128.0f)), by = pair_of(scale[i], scale[i]);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {  // 2^23 + byte, exactly
-                const float code = __uint_as_float(__byte_perm(w[e >> 2], 0x4b000000u, 0x7540u | (e & 3))) - (8388608.0f + 128.0f);
-                (e < 8 ? lo[e & 7] : hi[e & 7]) = __fmul_rn(code, scale);
-            }
+        for (int e = 0; e < 4; ++e) {  // 2^23 + byte, exactly
+            const uint32_t w = e < 2 ? x[i].x : x[i].y;
+            y[e] = mul2(add2(pair_of(__byte_perm(w, 0x4b000000u, 0x7540u | (2 * e & 3)), __byte_perm(w, 0x4b000000u, 0x7540u | (2 * e + 1 & 3))), minus), by);
         }
-        T *y = (is_v ? v : k) + (token * c.kv_heads + h) * c.dim + 16 * chunk;
-        store8<T, true>(y, narrow<T>(lo));
-        store8<T, true>(y + 8, narrow<T>(hi));
+        store8<T, true>((i == 0 ? k : v) + (token * c.kv_heads + h) * c.dim + 8 * j, Pairs<T>::narrow(y));
     }
 }
 
-// Tokens a CTA takes, and CTAs a token, for `units` threads' work per token: one sweep of a CTA while the whole is less than what
-// runs at once, about four beyond.
-void spread(int64_t tokens, int64_t units, int &tokens_per_cta, dim3 &grid) {
-    const int64_t at_once = (int64_t)sm_count() * 4 * kThreads;
-    if (tokens * units <= at_once || units >= 4 * kThreads) {
-        tokens_per_cta = 1;
-        grid = dim3((unsigned)tokens, (unsigned)ceil_div(units, tokens * units <= at_once ? kThreads : 4 * kThreads), 1);
-        return;
-    }
-    tokens_per_cta = (int)max((int64_t)1, 4 * kThreads / units);
-    grid = dim3((unsigned)ceil_div(tokens, tokens_per_cta), 1, 1);
+// Blocks of lanes x rows x tokens threads, about kThreads of them: the rows of a token in as many equal blocks as they need, or several tokens a block.  `unit`: rows
+// come in multiples of it.
+void shape(int64_t tokens, int rows, int lanes, int unit, dim3 &block, dim3 &grid) {
+    const int room = kThreads / lanes > unit ? kThreads / lanes / unit * unit : unit, parts = (rows + room - 1) / room;
+    const int each = ((rows + parts - 1) / parts + unit - 1) / unit * unit;
+    int together = parts == 1 && room > each ? room / each : 1;
+    const int64_t spread_out = ceil_div(tokens, (int64_t)2 * sm_count());  // a block for every SM, and another, before tokens share one
+    if (together > spread_out) together = spread_out > 1 ? (int)spread_out : 1;
+    if (together > 64) together = 64;
+    block = dim3((unsigned)lanes, (unsigned)each, (unsigned)together);
+    grid = dim3((unsigned)ceil_div(tokens, together), (unsigned)((rows + each - 1) / each), 1);
 }
 
 bool rows_aligned(const HeadRows &r, size_t item) {
@@ -353,14 +394,13 @@ template <typename T>
 int rotary_typed(const HeadRows &q, const HeadRows &k, const HeadRows &q_out, const HeadRows &k_out, const RotaryArgs &r, int64_t tokens, int heads, int kv_heads, int dim,
                  cudaStream_t stream) {
     const int all = heads + kv_heads;
-    if (dim % 16 == 0 && r.rotary_dim % 16 == 0 && (int64_t)all * dim < (1 << 24)) {
+    if (dim % 16 == 0 && dim <= 16 * 32 && r.rotary_dim % 16 == 0) {
         const size_t s = sizeof(T);
         const bool vec = rows_aligned(q, s) && rows_aligned(q_out, s) && rows_aligned(k, s) && rows_aligned(k_out, s) && aligned_to(r.table, 16);
-        int per_cta;
-        dim3 grid;
-        spread(tokens, (int64_t)all * (dim / 16), per_cta, grid);
+        dim3 block, grid;
+        shape(tokens, all, dim / 16, 1, block, grid);
         auto kernel = vec ? rotary_kernel<T, true> : rotary_kernel<T, false>;
-        return launch_after("rotary_kernel", kernel, grid, kThreads, 0, 1, stream, q, k, q_out, k_out, r, tokens, heads, all, dim, per_cta);
+        return launch_after("rotary_kernel", kernel, grid, block, 0, 1, stream, q, k, q_out, k_out, r, tokens, heads, all, dim);
     }
     const int64_t ctas = ceil_div(tokens * all * (dim - r.rotary_dim / 2), kThreads);
     return launch_after("rotary_generic_kernel", rotary_generic_kernel<T>, dim3((unsigned)(ctas < 65536 ? ctas : 65536)), kThreads, 0, 1, stream, q, k, q_out, k_out, r, tokens, heads,
@@ -371,11 +411,10 @@ template <typename T, bool VEC>
 int append_sized(const HeadRows &q, const HeadRows &q_out, const HeadRows &k, const HeadRows &v, uint8_t *cache, const CacheShape &c, const void *slots, int slot_bytes,
                  const RotaryArgs &r, int64_t tokens, int heads, cudaStream_t stream) {
     const int group = c.dim <= 64 ? 4 : c.dim <= 128 ? 8 : 16;
-    int per_cta;
-    dim3 grid;
-    spread(tokens, (int64_t)(heads + 2 * c.kv_heads) * group, per_cta, grid);
+    dim3 block, grid;
+    shape(tokens, heads + 2 * c.kv_heads, group, 32 / group, block, grid);  // whole warps, for the shuffles
     auto kernel = group == 4 ? append_kernel<T, VEC, 4> : group == 8 ? append_kernel<T, VEC, 8> : append_kernel<T, VEC, 16>;
-    return launch_after("append_kernel", kernel, grid, kThreads, 0, 1, stream, q, q_out, k, v, cache, c, slots, slot_bytes, r, tokens, heads, per_cta);
+    return launch_after("append_kernel", kernel, grid, block, 0, 1, stream, q, q_out, k, v, cache, c, slots, slot_bytes, r, tokens, heads);
 }
 
 template <typename T>
@@ -389,11 +428,9 @@ int append_typed(const HeadRows &q, const HeadRows &q_out, const HeadRows &k, co
 
 template <typename T>
 int read_typed(const uint8_t *cache, const CacheShape &c, const void *slots, int slot_bytes, void *k, void *v, int64_t tokens, cudaStream_t stream) {
-    int per_cta;
-    dim3 grid;
-    spread(tokens, (int64_t)2 * c.kv_heads * (c.dim / 16), per_cta, grid);
-    return launch_after("read_kernel", read_kernel<T>, grid, kThreads, 0, 1, stream, cache, c, slots, slot_bytes, static_cast<T *>(k), static_cast<T *>(v), tokens, per_cta,
-                        device_status_word());
+    dim3 block, grid;
+    shape(tokens, c.kv_heads, c.dim / 8, 1, block, grid);
+    return launch_after("read_kernel", read_kernel<T>, grid, block, 0, 1, stream, cache, c, slots, slot_bytes, static_cast<T *>(k), static_cast<T *>(v), tokens, device_status_word());
 }
 
 constexpr int64_t kMostTokens = 2147483647;  // of the grid's first dimension

@@ -40,8 +40,16 @@ struct CacheShape {
 
 // A slot's place: the record, and the row in it.
 __device__ __forceinline__ uint8_t *record_of(uint8_t *cache, const CacheShape &c, int64_t slot, int head, uint32_t &row) {
-    const int64_t page = slot / c.page_size;
-    const uint32_t in_page = (uint32_t)(slot - page * c.page_size);
+    int64_t page;
+    uint32_t in_page;
+    if (c.slots <= 0xffffffffll) {  // a division of 32 bits takes a fifth of one of 64
+        const uint32_t p = (uint32_t)slot / (uint32_t)c.page_size;
+        page = p;
+        in_page = (uint32_t)slot - p * (uint32_t)c.page_size;
+    } else {
+        page = slot / c.page_size;
+        in_page = (uint32_t)(slot - page * c.page_size);
+    }
     row = in_page & 15u;
     return cache + ((page * c.kv_heads + head) * (c.page_size >> 4) + (in_page >> 4)) * record_bytes(c.dim);
 }
@@ -93,19 +101,6 @@ __device__ __forceinline__ void store8(T *p, const Pack8<T> &x) {
         for (int i = 0; i < 8; ++i) p[i] = x.v[i];
     }
 }
-template <typename T>
-__device__ __forceinline__ void widen(const Pack8<T> &x, float (&f)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = Elems<T>::one(x.v[i]);
-}
-template <typename T>
-__device__ __forceinline__ Pack8<T> narrow(const float (&f)[8]) {
-    Pack8<T> x;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x.v[i] = Elems<T>::round(f[i]);
-    return x;
-}
-
 // Two floats in a register pair, for the instructions that take two at once.
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
@@ -131,16 +126,78 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
     return r;
 }
 
+// Eight elements as four pairs of floats, and back.
+template <typename T>
+struct Pairs;
+template <>
+struct Pairs<__half> {
+    static __device__ __forceinline__ void widen(const Pack8<__half> &x, f32x2 (&f)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&x.v[2 * i]));
+            f[i] = pair_of(p.x, p.y);
+        }
+    }
+    static __device__ __forceinline__ Pack8<__half> narrow(const f32x2 (&f)[4]) {
+        Pack8<__half> x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float lo, hi;
+            halves(f[i], lo, hi);
+            *reinterpret_cast<__half2 *>(&x.v[2 * i]) = __floats2half2_rn(lo, hi);
+        }
+        return x;
+    }
+};
+template <>
+struct Pairs<__nv_bfloat16> {
+    static __device__ __forceinline__ void widen(const Pack8<__nv_bfloat16> &x, f32x2 (&f)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = *reinterpret_cast<const uint32_t *>(&x.v[2 * i]);
+            f[i] = pair_of(u << 16, u & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ Pack8<__nv_bfloat16> narrow(const f32x2 (&f)[4]) {
+        Pack8<__nv_bfloat16> x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float lo, hi;
+            halves(f[i], lo, hi);
+            *reinterpret_cast<__nv_bfloat162 *>(&x.v[2 * i]) = __floats2bfloat162_rn(lo, hi);
+        }
+        return x;
+    }
+};
+template <>
+struct Pairs<float> {
+    static __device__ __forceinline__ void widen(const Pack8<float> &x, f32x2 (&f)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = pair_of(x.v[2 * i], x.v[2 * i + 1]);
+    }
+    static __device__ __forceinline__ Pack8<float> narrow(const f32x2 (&f)[4]) {
+        Pack8<float> x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) halves(f[i], x.v[2 * i], x.v[2 * i + 1]);
+        return x;
+    }
+};
+template <typename T>
+__device__ __forceinline__ Pack8<T> narrow(const float (&f)[8]) {
+    const f32x2 p[4] = {pair_of(f[0], f[1]), pair_of(f[2], f[3]), pair_of(f[4], f[5]), pair_of(f[6], f[7])};
+    return Pairs<T>::narrow(p);
+}
+
 __device__ __forceinline__ int64_t index_at(const void *p, int bytes, int64_t i) {
     return bytes == 8 ? static_cast<const int64_t *>(p)[i] : (int64_t) static_cast<const int32_t *>(p)[i];
 }
 
 // A launch as a programmatic dependent of the kernel in front, in clusters of `cluster` CTAs along x.
 template <typename... Params, typename... Args>
-inline int launch_after(const char *name, void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, Args... args) {
+inline int launch_after(const char *name, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3((unsigned)threads, 1, 1);
+    cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attrs[2];
