@@ -11,8 +11,8 @@
 //
 // The maxima of 64 groups of threads bound the alternatives: at least `top` elements are no smaller than the top-th largest of them.  So what the second
 // reading passes over is compared with that bound, eight elements at once, and the few that reach it (some 1.2 * top on random rows) are put
-// in order by counting.  Where there are too many (rows made so, or vocabularies of fewer elements than the groups need) there is a search for each
-// alternative.
+// in order by counting.  Where that is too many, mostly equals of the bound, only the first of those are taken; what is left (rows made so, and vocabularies of fewer
+// elements than the groups need) has a search for each alternative.
 #include <atomic>
 
 #include "serving.cuh"
@@ -31,11 +31,14 @@ constexpr int kMostPart = 200 * 1024;    // bytes of a row in one CTA
 constexpr int kGoodPart = 66 * 1024;     // three CTAs an SM
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
-// A value and the place it stands at as one number: larger values first, then smaller places.  NaN is the largest; -0 is 0.
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t place) {
+// A value as a whole number in its order: NaN is the largest, -0 is 0; none is 0.
+__device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);
-    const uint32_t o = x != x ? 0xffffffffu : b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
-    return ((uint64_t)o << 32) | (0xffffffffu - place);
+    return x != x ? 0xffffffffu : b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+// A value and the place it stands at as one number: larger values first, then smaller places.
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t place) {
+    return ((uint64_t)ordered(x) << 32) | (0xffffffffu - place);
 }
 __device__ __forceinline__ float value_of(uint64_t key) {
     const uint32_t o = (uint32_t)(key >> 32);
@@ -61,11 +64,16 @@ struct Vec16<float> {
         widen(v, f);
         p[0] = pair_of(fmaxf(f[0], -1e30f), fmaxf(f[1], -1e30f)), p[1] = pair_of(fmaxf(f[2], -1e30f), fmaxf(f[3], -1e30f));
     }
-    static __device__ __forceinline__ float top(uint4 v) {
+    typedef float Top;
+    static __device__ __forceinline__ Top all(float x) { return x; }
+    static __device__ __forceinline__ Top top(uint4 v) {
         float f[4];
         widen(v, f);
         return max_nan(max_nan(f[0], f[1]), max_nan(f[2], f[3]));
     }
+    static __device__ __forceinline__ Top larger(Top a, Top b) { return max_nan(a, b); }
+    static __device__ __forceinline__ float value(Top t) { return t; }
+    static __device__ __forceinline__ bool below(Top t, Top bound) { return t < bound; }
 };
 template <>
 struct Vec16<__half> {
@@ -87,10 +95,12 @@ struct Vec16<__half> {
             p[i] = pair_of(f.x, f.y);
         }
     }
-    static __device__ __forceinline__ float top(uint4 v) {
-        const __half2 m = __hmax2_nan(__hmax2_nan(h2(v.x), h2(v.y)), __hmax2_nan(h2(v.z), h2(v.w)));
-        return max_nan(__low2float(m), __high2float(m));
-    }
+    typedef __half2 Top;  // of the elements at even and at odd places
+    static __device__ __forceinline__ Top all(float x) { return __float2half2_rn(x); }
+    static __device__ __forceinline__ Top top(uint4 v) { return __hmax2_nan(__hmax2_nan(h2(v.x), h2(v.y)), __hmax2_nan(h2(v.z), h2(v.w))); }
+    static __device__ __forceinline__ Top larger(Top a, Top b) { return __hmax2_nan(a, b); }
+    static __device__ __forceinline__ float value(Top t) { return max_nan(__low2float(t), __high2float(t)); }
+    static __device__ __forceinline__ bool below(Top t, Top bound) { return __hblt2(t, bound); }  // both
 };
 template <>
 struct Vec16<__nv_bfloat16> {
@@ -110,10 +120,12 @@ struct Vec16<__nv_bfloat16> {
             p[i] = pair_of(u << 16, u & 0xffff0000u);
         }
     }
-    static __device__ __forceinline__ float top(uint4 v) {
-        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(b2(v.x), b2(v.y)), __hmax2_nan(b2(v.z), b2(v.w)));
-        return max_nan(__low2float(m), __high2float(m));
-    }
+    typedef __nv_bfloat162 Top;  // of the elements at even and at odd places
+    static __device__ __forceinline__ Top all(float x) { return __float2bfloat162_rn(x); }
+    static __device__ __forceinline__ Top top(uint4 v) { return __hmax2_nan(__hmax2_nan(b2(v.x), b2(v.y)), __hmax2_nan(b2(v.z), b2(v.w))); }
+    static __device__ __forceinline__ Top larger(Top a, Top b) { return __hmax2_nan(a, b); }
+    static __device__ __forceinline__ float value(Top t) { return max_nan(__low2float(t), __high2float(t)); }
+    static __device__ __forceinline__ bool below(Top t, Top bound) { return __hblt2(t, bound); }  // both
 };
 template <typename T>
 __device__ __forceinline__ T minus_infinity() { return Elems<T>::round(-INFINITY); }
@@ -141,8 +153,8 @@ struct Share {
 struct Block {
     uint64_t bar;
     float m[WARPS], sum[WARPS], weighted[WARPS];
-    uint64_t group_key[GROUPS];
-    uint64_t bound;
+    uint32_t group_top[GROUPS], bound;
+    int equals[WARPS];
     uint64_t warp_key[WARPS];
     uint64_t best[MOST_TOP];
     int n_candidates, n_vectors;
@@ -159,6 +171,7 @@ __device__ __forceinline__ void order_keys(const uint64_t *keys, int n, int top,
     for (int i = threadIdx.x; i < n; i += THREADS) {
         const uint64_t own = keys[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < n; ++j) rank += keys[j] > own || (keys[j] == own && j < i);
         if (rank < top) best[rank] = own;
     }
@@ -224,43 +237,34 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
     }
     const uint4 *x = reinterpret_cast<const uint4 *>(smem);
 
-    // ---- the maximum of every thread, and the first vector that it stands in ----
-    float most = -INFINITY;
-    int at = threadIdx.x;
+    // ---- the maximum of every thread ----
+    using V = Vec16<T>;
+    typename V::Top tops = V::all(-INFINITY);
 #pragma unroll 8
-    for (int v = threadIdx.x; v < vecs; v += THREADS) {
-        const float y = Vec16<T>::top(x[v]);
-        if (!(y <= most) && most == most) {  // a NaN stays
-            most = y;
-            at = v;
-        }
-    }
-    uint64_t key = (int)threadIdx.x < vecs ? key_of(most, at) : 0;
-    float m = most;
+    for (int v = threadIdx.x; v < vecs; v += THREADS) tops = V::larger(tops, V::top(x[v]));
+    float m = V::value(tops);
+    uint32_t group = (int)threadIdx.x < vecs ? ordered(m) : 0;
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
     if (lane == 0) blk.m[warp] = m;
     if (p.top > 0) {
 #pragma unroll
-        for (int d = 8; d < 32; d *= 2) {
-            const uint64_t other = __shfl_xor_sync(0xffffffffu, key, d);
-            key = other > key ? other : key;
-        }
-        if (lane < 8) blk.group_key[8 * warp + lane] = key;
+        for (int d = 8; d < 32; d *= 2) group = max(group, __shfl_xor_sync(0xffffffffu, group, d));
+        if (lane < 8) blk.group_top[8 * warp + lane] = group;
     }
     __syncthreads();
     m = blk.m[0];
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) m = max_nan(m, blk.m[w]);
-    uint64_t bound = 0;
-    if (p.top > 0) {  // the top-th largest of the groups' keys: four threads compare one with all
+    uint32_t bound = 0;
+    if (p.top > 0) {  // the top-th largest of the groups': four threads compare one with all
         const int g = threadIdx.x / 4;
-        const uint64_t own = blk.group_key[g];
+        const uint32_t own = blk.group_top[g];
         int before = 0;
 #pragma unroll
         for (int i = 0; i < GROUPS / 4; ++i) {
             const int j = 4 * i + threadIdx.x % 4;
-            const uint64_t k = blk.group_key[j];
+            const uint32_t k = blk.group_top[j];
             before += k > own || (k == own && j < g);
         }
         before += __shfl_xor_sync(0xffffffffu, before, 1);
@@ -271,7 +275,8 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
     }
     // With fewer groups than alternatives there is no bound, and nothing is collected.
     const bool collect = bound != 0;
-    const float least = collect ? value_of(bound) : INFINITY;
+    const float least = collect ? value_of((uint64_t)bound << 32) : INFINITY;
+    const typename V::Top least_of_all = V::all(least);
 
     // ---- the sums ----
     const float shift = fabsf(m) < INFINITY ? m : 0.0f;
@@ -283,7 +288,7 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
         for (int v = threadIdx.x; v < vecs; v += THREADS) {
             f32x2 f[N / 2];
             const uint4 raw = x[v];
-            if (!(Vec16<T>::top(raw) < least)) {  // rarely; NaN too
+            if (collect && !V::below(V::top(raw), least_of_all)) {  // rarely; NaN too
                 const int k = atomicAdd(&blk.n_vectors, 1);
                 if (k < CANDIDATES) blk.vectors[k] = (uint16_t)v;
             }
@@ -317,23 +322,64 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
     Share &mine = blk.shares[0];
     __syncthreads();
     if (p.top > 0) {
-        if (collect && blk.n_vectors <= CANDIDATES) {
-            for (int i = threadIdx.x; i < blk.n_vectors; i += THREADS) {
-                const int v = blk.vectors[i];
-                float f[N];
-                Vec16<T>::widen(x[v], f);
+        // Elements of a vector that pass the bound, or (ties) that are equal to it.
+        auto offer = [&](int v, bool ties) {
+            float f[N];
+            V::widen(x[v], f);
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const int index = v * N + e - lead;
-                    if (!(f[e] < least) && index >= 0 && index < n && key_of(f[e], (uint32_t)v) >= bound) {
-                        const int k = atomicAdd(&blk.n_candidates, 1);
-                        if (k < CANDIDATES) blk.candidates[k] = key_of(f[e], (uint32_t)(from + index));
-                    }
-                }
+            for (int e = 0; e < N; ++e) {
+                const int index = v * N + e - lead;
+                if (index < 0 || index >= n || (ties ? ordered(f[e]) != bound : ordered(f[e]) <= bound)) continue;
+                const int k = atomicAdd(&blk.n_candidates, 1);
+                if (k < CANDIDATES) blk.candidates[k] = key_of(f[e], (uint32_t)(from + index));
+            }
+        };
+        bool listed = collect;
+        if (collect && blk.n_vectors <= CANDIDATES) {
+            for (int i = threadIdx.x; i < blk.n_vectors * N; i += THREADS) {  // a thread an element
+                const int at = blk.vectors[i / N] * N + i % N, index = at - lead;
+                const float one = Elems<T>::one(buf[at]);
+                if (index < 0 || index >= n || ordered(one) < bound) continue;
+                const int k = atomicAdd(&blk.n_candidates, 1);
+                if (k < CANDIDATES) blk.candidates[k] = key_of(one, (uint32_t)(from + index));
             }
             __syncthreads();
+        } else if (collect) {
+            // Too many: mostly equals of the bound (a row of one value, or whose allowed tokens are fewer than the alternatives).  Those above it, and
+            // then the first of its equals, as many as are wanted.
+            for (int v = threadIdx.x; v < vecs; v += THREADS) offer(v, false);
+            __syncthreads();
+            const int above = blk.n_candidates;
+            for (int base = 0, equals = 0; base < vecs && above < p.top && equals < p.top - above; base += THREADS) {
+                const int v = base + threadIdx.x;
+                int own = 0;
+                if (v < vecs) {
+                    float f[N];
+                    V::widen(x[v], f);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) own += v * N + e >= lead && v * N + e - lead < n && ordered(f[e]) == bound;
+                }
+                int until = own;
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const int below = __shfl_up_sync(0xffffffffu, until, d);
+                    if (lane >= d) until += below;
+                }
+                if (lane == 31) blk.equals[warp] = until;
+                __syncthreads();
+                int in_front = equals + until - own, all = 0;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) {
+                    if (w < warp) in_front += blk.equals[w];
+                    all += blk.equals[w];
+                }
+                if (own > 0 && in_front < p.top - above) offer(v, true);
+                equals += all;
+                __syncthreads();
+            }
         }
-        if (collect && blk.n_vectors <= CANDIDATES && blk.n_candidates <= CANDIDATES) {
+        listed = listed && blk.n_candidates <= CANDIDATES;
+        if (listed) {
             order_keys(blk.candidates, blk.n_candidates, p.top, mine.best);
         } else {
             uint64_t last = ~0ull;
