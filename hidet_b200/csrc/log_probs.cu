@@ -52,12 +52,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// 16 bytes of logits.  pairs: as floats, none below a number whose probability is zero beside any other, so that this times it is zero as well.
+// 16 bytes of logits.  pairs: as floats, none below a finite number, whose probability is zero beside a maximum of at least kLeast, so that this times it is zero
+// as well.
 template <typename T>
 struct Vec16;
 template <>
 struct Vec16<float> {
     static constexpr int N = 4;
+    static constexpr float kLeast = -1e29f;
     static __device__ __forceinline__ void widen(uint4 v, float (&f)[4]) { f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w); }
     static __device__ __forceinline__ void pairs(uint4 v, f32x2 (&p)[2]) {
         float f[4];
@@ -78,6 +80,7 @@ struct Vec16<float> {
 template <>
 struct Vec16<__half> {
     static constexpr int N = 8;
+    static constexpr float kLeast = -65504.0f + 256.0f;
     static __device__ __forceinline__ __half2 h2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
     static __device__ __forceinline__ void widen(uint4 v, float (&f)[8]) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -105,6 +108,7 @@ struct Vec16<__half> {
 template <>
 struct Vec16<__nv_bfloat16> {
     static constexpr int N = 8;
+    static constexpr float kLeast = -1e29f;
     static __device__ __forceinline__ __nv_bfloat162 b2(uint32_t u) { return *reinterpret_cast<__nv_bfloat162 *>(&u); }
     static __device__ __forceinline__ void widen(uint4 v, float (&f)[8]) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -280,8 +284,8 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
 
     // ---- the sums ----
     const float shift = fabsf(m) < INFINITY ? m : 0.0f;
-    float sum, weighted;
-    {
+    float sum = 0.0f, weighted = 0.0f;
+    if (m >= V::kLeast || !(fabsf(m) < INFINITY)) {
         const f32x2 minus = pair_of(-shift, -shift), log2e = pair_of(kLog2e, kLog2e);
         f32x2 sums = 0, products = 0;
 #pragma unroll 4
@@ -310,6 +314,23 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
         sum = lo + hi;
         halves(products, lo, hi);
         weighted = lo + hi;
+    } else {
+        // Nothing but numbers around the type's lowest, which stand for what is not allowed, and -inf: the two differ here.
+        for (int v = threadIdx.x; v < vecs; v += THREADS) {
+            float f[N];
+            const uint4 raw = x[v];
+            if (collect && !V::below(V::top(raw), least_of_all)) {
+                const int k = atomicAdd(&blk.n_vectors, 1);
+                if (k < CANDIDATES) blk.vectors[k] = (uint16_t)v;
+            }
+            V::widen(raw, f);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float y = (f[e] - shift) * kLog2e, z = exp2f(y);
+                sum += z;
+                weighted += z > 0.0f ? z * y : 0.0f;
+            }
+        }
     }
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) {
@@ -480,17 +501,17 @@ template <typename T>
 int launch_typed(LogProbsArgs p, int64_t rows, cudaStream_t stream) {
     // The fewest CTAs a row whose parts let three of them share an SM; with few rows more, as long as parts have 8 KB and SMs are idle.
     const int64_t bytes = p.vocab * (int64_t)sizeof(T);
-    int64_t ranks = 1;
-    while (ranks < MOST_CLUSTER && (bytes > ranks * kGoodPart || (rows * ranks * 2 <= sm_count() && bytes > ranks * 8192))) ranks *= 2;
+    int64_t ranks = ceil_div(bytes, kGoodPart) < MOST_CLUSTER ? ceil_div(bytes, kGoodPart) : MOST_CLUSTER;
+    while (2 * ranks <= MOST_CLUSTER && rows * ranks * 2 <= sm_count() && bytes > ranks * 8192) ranks *= 2;
     p.part = round_up(ceil_div(p.vocab, ranks), 64);
     if (p.part * (int64_t)sizeof(T) > kMostPart) {
         return set_error(B200Q_UNSUPPORTED, "token_log_probs: rows of %lld bytes: up to %d are supported", (long long)bytes, MOST_CLUSTER * kMostPart);
     }
+    if (rows > 2147483647LL / ranks) return set_error(B200Q_UNSUPPORTED, "token_log_probs: %lld rows", (long long)rows);
     const int smem = (int)(p.part * sizeof(T)) + 32;
     static std::atomic<bool> attr_set[64];
     const int rc = allow_smem(attr_set, log_probs_kernel<T>, kMostPart + 32);
     if (rc != B200Q_OK) return rc;
-    if (rows > 2147483647LL / ranks) return set_error(B200Q_UNSUPPORTED, "token_log_probs: %lld rows", (long long)rows);
     return launch_after("log_probs_kernel", log_probs_kernel<T>, dim3((unsigned)(rows * ranks)), THREADS, smem, (int)ranks, stream, p);
 }
 
