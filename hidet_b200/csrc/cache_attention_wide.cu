@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                     }
                     const float4 k_tops = *reinterpret_cast<const float4 *>(ctl.k_top[buf]), v_tops = *reinterpret_cast<const float4 *>(ctl.v_top[buf]);
                     const float k_top = max3(fmaxf(k_tops.x, k_tops.y), k_tops.z, k_tops.w), v_top = max3(fmaxf(v_tops.x, v_tops.y), v_tops.z, v_tops.w);
-                    bool raise = v_top >= v_limit;
+                    bool raised = false;
                     if (__any_sync(0xffffffffu, fmaxf(top, other) * k_top > m + rise)) {
                         top = other = -INFINITY;
 #pragma unroll 1
@@ -422,11 +422,12 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                             }
                         }
                         top = fmaxf(top, other);
-                        raise |= top > m + rise;
-                    } else {
-                        top = m;
+                        raised = top > m + rise;
                     }
-                    if (__any_sync(0xffffffffu, raise)) {
+                    // The bound counts what lies behind the end too, in records that were not copied whatever the ring held.  So a maximum is taken
+                    // over only where one of the warp's rows passes its own by too much: results do not depend on what ran before.
+                    if (!__any_sync(0xffffffffu, raised)) top = m;
+                    if (__any_sync(0xffffffffu, raised || v_top >= v_limit)) {
                         const float was = exponent;
                         if (v_top >= v_limit) {
                             exponent = fmaxf((float)((int)(__float_as_uint(v_top) >> 23) - 127), kLeastUnit);
