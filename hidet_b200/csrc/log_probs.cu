@@ -285,6 +285,9 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
     // ---- the sums ----
     const float shift = fabsf(m) < INFINITY ? m : 0.0f;
     float sum = 0.0f, weighted = 0.0f;
+    // Which of this thread's vectors reach the bound, the last in bit 0: with a branch for each, which few take, the loop's loads and arithmetic could not overlap.
+    uint64_t hits = 0;
+    static_assert(kMostPart / 16 / THREADS < 63, "");
     if (m >= V::kLeast || !(fabsf(m) < INFINITY)) {
         const f32x2 minus = pair_of(-shift, -shift), log2e = pair_of(kLog2e, kLog2e);
         f32x2 sums = 0, products = 0;
@@ -292,10 +295,7 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
         for (int v = threadIdx.x; v < vecs; v += THREADS) {
             f32x2 f[N / 2];
             const uint4 raw = x[v];
-            if (collect && !V::below(V::top(raw), least_of_all)) {  // rarely; NaN too
-                const int k = atomicAdd(&blk.n_vectors, 1);
-                if (k < CANDIDATES) blk.vectors[k] = (uint16_t)v;
-            }
+            hits = hits << 1 | (V::below(V::top(raw), least_of_all) ? 0 : 1);  // NaN is a hit too
             Vec16<T>::pairs(raw, f);
 #pragma unroll
             for (int e = 0; e < N / 2; ++e) {
@@ -319,10 +319,7 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
         for (int v = threadIdx.x; v < vecs; v += THREADS) {
             float f[N];
             const uint4 raw = x[v];
-            if (collect && !V::below(V::top(raw), least_of_all)) {
-                const int k = atomicAdd(&blk.n_vectors, 1);
-                if (k < CANDIDATES) blk.vectors[k] = (uint16_t)v;
-            }
+            hits = hits << 1 | (V::below(V::top(raw), least_of_all) ? 0 : 1);
             V::widen(raw, f);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
@@ -330,6 +327,13 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
                 sum += z;
                 weighted += z > 0.0f ? z * y : 0.0f;
             }
+        }
+    }
+    if (collect) {
+        const int last = (int)threadIdx.x + (vecs - 1 - (int)threadIdx.x) / THREADS * THREADS;  // this thread's, if it has any
+        for (; hits != 0; hits &= hits - 1) {
+            const int k = atomicAdd(&blk.n_vectors, 1);
+            if (k < CANDIDATES) blk.vectors[k] = (uint16_t)(last - (__ffsll((long long)hits) - 1) * THREADS);
         }
     }
 #pragma unroll
