@@ -18,6 +18,10 @@
 // the other warps takes one record of 16 positions of a tile: it loads K with plain and V with transposing matrix loads, converts two codes an
 // instruction and multiplies, with the codes as the 16-row operand (positions of K, elements of V) and eight query rows as columns.  With the positions
 // (and not the rows) shared out among the warps, each code is converted once per CTA.
+//
+// Bound by the cache's bytes where sequences are long: pieces stream at 5.9 TB/s, and 8 us are the launch, the plan, the first tile and the additions.  Measured with
+// 128 elements a head, 64 heads over 8: 32 sequences of 90 to 8000 positions 58 us, one of 131071 58 us, 4.7 TB/s each.  Where they are short it is
+// latency: 5.4 us for one tile, 7.5 for two pieces and their sum, 11.1 for 577 positions of 32 heads.
 #include <atomic>
 
 #include "cache_attention.cuh"
@@ -123,7 +127,7 @@ __device__ __forceinline__ void finish_item(const AttentionArgs &p, Control &ctl
         else write_piece<D, ROWS>(piece, r, d, v, sum, top * scale);
     }
     static_assert(L::BUFFERS * L::MERGE >= 2 * FAN * ROWS * 4, "");
-    if (!whole) meet<D, ROWS, CONSUMERS, 1, T>(p, item, threadIdx.x, merge, &ctl.last);  // whose first barrier frees the merge buffers
+    if (!whole) meet<D, ROWS, CONSUMERS, T>(p, item, threadIdx.x, merge, &ctl.last);  // whose first barrier frees the merge buffers
 }
 
 template <int D, int NT, typename T>

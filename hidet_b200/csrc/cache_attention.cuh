@@ -324,48 +324,41 @@ __device__ __forceinline__ void write_piece(float *piece, int r, int d, float4 v
     }
 }
 
-// The sum of `some` pieces for this thread's groups of four elements, GROUPS of them with their loads in flight together.  tops, sums: of the
-// pieces' rows, [FAN][ROWS], filled by all threads in front of the barrier behind the first loads.
-template <int D, int ROWS, int N, int GROUPS, typename T, typename PieceOf>
+// The sum of `some` pieces, four elements of a row a thread at a time.  tops, sums: of the pieces' rows, [FAN][ROWS], filled by all threads in front of
+// the barrier behind the first loads.
+template <int D, int ROWS, int N, typename T, typename PieceOf>
 __device__ __forceinline__ void add_pieces(const AttentionArgs &p, const Item &item, const float *tops, const float *sums, int tid, int some, bool done, PieceOf piece_of) {
     bool waited = false;
-    for (int i0 = tid; i0 < item.rows * (D / 4) || !waited; i0 += GROUPS * N) {
-        float4 x[GROUPS][FAN];
+    for (int i = tid; i < item.rows * (D / 4) || !waited; i += N) {
+        const int r = i / (D / 4), d = 4 * (i % (D / 4));
+        float4 x[FAN];
 #pragma unroll
-        for (int u = 0; u < GROUPS; ++u) {
-            const int i = i0 + u * N, r = i / (D / 4), d = 4 * (i % (D / 4));
-#pragma unroll
-            for (int j = 0; j < FAN; ++j)
-                if (j < some && r < item.rows) x[u][j] = __ldcg(reinterpret_cast<const float4 *>(p.partial + (piece_of(j) + r * D + d)));
-        }
+        for (int j = 0; j < FAN; ++j)
+            if (j < some && r < item.rows) x[j] = __ldcg(reinterpret_cast<const float4 *>(p.partial + (piece_of(j) + r * D + d)));
         if (!waited) sync_of<N>();
         waited = true;
+        if (r >= item.rows) continue;
+        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int u = 0; u < GROUPS; ++u) {
-            const int i = i0 + u * N, r = i / (D / 4), d = 4 * (i % (D / 4));
-            if (r >= item.rows) continue;
-            float top = -INFINITY, sum = 0.0f;
+        for (int j = 0; j < FAN; ++j)
+            if (j < some) top = fmaxf(top, tops[j * ROWS + r]);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int j = 0; j < FAN; ++j)
-                if (j < some) top = fmaxf(top, tops[j * ROWS + r]);
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int j = 0; j < FAN; ++j)
-                if (j < some) {
-                    // in two steps: units may lie so far apart that the whole factor leaves float's range where the products do not
-                    const float own = tops[j * ROWS + r], by = own == -INFINITY ? 1.0f : ex2(0.5f * (own - top));
-                    sum = fmaf(sums[j * ROWS + r] * by, by, sum);
-                    v.x = fmaf(x[u][j].x * by, by, v.x), v.y = fmaf(x[u][j].y * by, by, v.y), v.z = fmaf(x[u][j].z * by, by, v.z), v.w = fmaf(x[u][j].w * by, by, v.w);
-                }
-            if (done) write_out<D, T>(p, item, r, d, v, sum, top);
-            else write_piece<D, ROWS>(p.partial + piece_of(0), r, d, v, sum, top);  // into the place of the first of them, whose rows' units and sums are in shared memory by now
-        }
+        for (int j = 0; j < FAN; ++j)
+            if (j < some) {
+                // in two steps: units may lie so far apart that the whole factor leaves float's range where the products do not
+                const float own = tops[j * ROWS + r], by = own == -INFINITY ? 1.0f : ex2(0.5f * (own - top));
+                sum = fmaf(sums[j * ROWS + r] * by, by, sum);
+                v.x = fmaf(x[j].x * by, by, v.x), v.y = fmaf(x[j].y * by, by, v.y), v.z = fmaf(x[j].z * by, by, v.z), v.w = fmaf(x[j].w * by, by, v.w);
+            }
+        if (done) write_out<D, T>(p, item, r, d, v, sum, top);
+        else write_piece<D, ROWS>(p.partial + piece_of(0), r, d, v, sum, top);  // into the place of the first of them, whose rows' units and sums are in shared memory by now
     }
 }
 
 // The pieces of an item meet: FAN neighbours at a time, in the CTA that arrives last of them, then FAN of those.  N threads, which have written this
 // CTA's piece; scratch: 2 * FAN * ROWS floats.
-template <int D, int ROWS, int N, int GROUPS, typename T>
+template <int D, int ROWS, int N, typename T>
 __device__ __forceinline__ void meet(const AttentionArgs &p, const Item &item, int tid, float *scratch, int *last) {
     int k = blockIdx.x - item.first_cta, n = item.last_cta - item.first_cta + 1, stride = 1;
     auto place = [&](int i) { return (2 * (item.first_cta + i) + (i == 0 ? 1 : 0)) * kPieceFloats<D, ROWS>; };  // 32 bits are enough for the workspace
@@ -392,7 +385,7 @@ __device__ __forceinline__ void meet(const AttentionArgs &p, const Item &item, i
             sums[i] = r < item.rows ? __ldcg(from + ROWS) : 0.0f;
         }
         const bool done = n <= FAN;
-        add_pieces<D, ROWS, N, GROUPS, T>(p, item, tops, sums, tid, some, done, piece_of);
+        add_pieces<D, ROWS, N, T>(p, item, tops, sums, tid, some, done, piece_of);
         if (done) break;
     }
 }

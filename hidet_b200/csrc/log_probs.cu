@@ -9,6 +9,11 @@
 // behind its last 16-byte boundary by loads) and read from there twice: for the maximum of every thread, and for the sums.  Bound by the
 // copy where rows are many.  CTAs of a row are a cluster and meet in the shared memory of the first.
 //
+// Measured: 2047 rows of 32002 bf16 logits with 20 alternatives 41.2 us, 3.2 TB/s; one row 6.1 us.  A copy at memory's rate would take 20 us, and the instructions, 12 an element,
+// 22: what is above that is that a row's steps (copy, maxima, bound, sums, alternatives) wait for one another, and with three rows an SM, all that fits its
+// shared memory, half of the issue slots stay empty.  More threads a row, parts of half the size (two CTAs a row: 83 us) and candidates sought outside
+// the sums' loop (43 to 50 us) are slower.
+//
 // The maxima of 64 groups of threads bound the alternatives: at least `top` elements are no smaller than the top-th largest of them.  So what the second
 // reading passes over is compared with that bound, eight elements at once, and the few that reach it (some 1.2 * top on random rows) are put
 // in order by counting.  Where that is too many, mostly equals of the bound, only the first of those are taken; what is left (rows made so, and vocabularies of fewer
