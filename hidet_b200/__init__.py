@@ -1,4 +1,5 @@
-"""hidet_b200: Hidet's weight-only int8 quantized linear path on B200 (sm_100a).
+"""hidet_b200: Hidet's weight-only int8 quantized linear path on B200 (sm_100a), and the operators that decoding with such
+linears needs around them (hidet_b200.serving).
 
 The public names follow the reference (hidet.ops.symmetric_quantize, hidet.ops.symmetric_dequantize,
 hidet.ops.quant.*); tensors are CUDA torch tensors and every computation runs in the hand-written
