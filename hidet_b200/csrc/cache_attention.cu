@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
 #pragma unroll
             for (int r0 = 0; r0 < ROWS; r0 += WARPS) {
                 const int r = r0 + warp;
-                const int row = item.row0 + r, token = row / p.group;
+                const int row = item.row0 + r, token = token_of(p, row);
                 const T *src = static_cast<const T *>(p.q) + (int64_t)(item.token0 + token) * p.q_token + (int64_t)(item.head * p.group + row - token * p.group) * p.q_head;
                 float f[(D + 127) / 128][4];
                 float top = 0.0f;
@@ -345,17 +345,21 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
                 const bool partly = key0 + 16 > hidden;
                 if (partly) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int pos = key0 + key_of_lane + 2 * h;
-                        if (pos >= length) vs[h] = 0.0f;
+                    for (int nt = 0; nt < NT; ++nt) {
+                        bool seen[4];
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
+                        for (int e = 0; e < 2; ++e) {
+                            const int r = 8 * nt + 2 * t + e, token = token_of(p, item.row0 + r);
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int r = 8 * nt + 2 * t + e;
-                                if (!may_see(p, item, r, (item.row0 + r) / p.group, pos)) s[nt][2 * h + e] = -INFINITY;
-                            }
+                            for (int h = 0; h < 2; ++h) seen[2 * h + e] = may_see(p, item, r, token, key0 + key_of_lane + 2 * h);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (!seen[e]) s[nt][e] = -INFINITY;
                     }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (key0 + key_of_lane + 2 * h >= length) vs[h] = 0.0f;
                 }
                 const float v_top = fmaxf(vs[0], vs[1]);
                 bool up = v_top >= v_limit;
@@ -578,6 +582,10 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
     p.batch = (int)batch;
     p.kv_heads = (int)kv_heads;
     p.group = (int)(heads / kv_heads);
+    int power = 0;
+    while ((1ll << power) < p.group) ++power;
+    p.by_group = (uint32_t)(((1ull << (31 + power)) + p.group - 1) / p.group);
+    p.by_group_shift = 31 + power;
     p.scale_log2 = scale * kLog2e;
     p.counters = static_cast<unsigned int *>(workspace);
     p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kCounterBytes);

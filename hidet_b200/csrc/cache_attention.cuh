@@ -43,6 +43,7 @@ struct AttentionArgs {
     int64_t mask_stride;
     int mask_width;
     int batch, kv_heads, group;
+    uint32_t by_group, by_group_shift;  // row / group = row * by_group >> by_group_shift for rows below 2^31 (token_of)
     float scale_log2;
     float *partial;
     int64_t partial_floats;  // of all pieces of the kernel for many rows
@@ -65,6 +66,9 @@ inline bool is_wide(const AttentionArgs &p, int64_t dim) {
 int launch_wide(const AttentionArgs &p, int dim, bool bf16, cudaStream_t stream);
 
 #ifdef __CUDACC__
+
+// Of a query row (token * group + head in group): 2^31+s / group rounded up, 2^s the power of two from group on, is off by less than one part in 2^31.
+__device__ __forceinline__ int token_of(const AttentionArgs &p, int row) { return (int)((uint64_t)(uint32_t)row * p.by_group >> p.by_group_shift); }
 
 // A key/value head of a sequence with some of its query rows, and the pieces that it is in.
 struct Item {
@@ -152,22 +156,23 @@ struct Line {
     int b = 0, offset = 0;                      // the sequence that cur lies in, and where in its items
 
     __device__ __forceinline__ int piece(int c) const { return c * each + min(c, more); }
-    __device__ __forceinline__ int cta_of(int unit) const { return unit < more * (each + 1) ? unit / (each + 1) : more + (unit - more * (each + 1)) / each; }
+    __device__ __forceinline__ int cta_of(int unit) const {
+        const int longer = more * (each + 1);
+        return unit < longer ? (int)((uint32_t)unit / (uint32_t)(each + 1)) : more + (int)((uint32_t)(unit - longer) / (uint32_t)each);
+    }
 
     __device__ __forceinline__ Line(const AttentionArgs &args, int lane_) : p(args), lane(lane_) {
-        int items = 0, tiles = 0;
-        for (int s0 = lane; s0 < p.batch; s0 += 32) {
+        // The plan is in front of everything else, alone: few sums and divisions, and no sequence looked up twice that need not be.
+        Sequence mine = {};
+        if (lane < p.batch) mine = sequence_of<ROWS>(p, lane);
+        int items = mine.row_tiles, tiles = mine.row_tiles * mine.tiles;
+        for (int s0 = lane + 32; s0 < p.batch; s0 += 32) {
             const Sequence s = sequence_of<ROWS>(p, s0);
             items += s.row_tiles;
             tiles += s.row_tiles * s.tiles;
         }
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) {
-            items += __shfl_xor_sync(0xffffffffu, items, d);
-            tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
-        }
-        items *= p.kv_heads;
-        tiles *= p.kv_heads;
+        items = __reduce_add_sync(0xffffffffu, items) * p.kv_heads;
+        tiles = __reduce_add_sync(0xffffffffu, tiles) * p.kv_heads;
         // No more pieces of an item than are added at once, as long as the wait for another round of additions, about two tiles, would be longer
         // than what shorter pieces save.
         int ctas = min((int)gridDim.x, tiles);
@@ -176,16 +181,13 @@ struct Line {
         // Where pieces are long, a gap in front of every item stands for what it costs besides its tiles.
         gap = tiles >= 8 * ctas ? UNITS : 0;
         const int units = tiles + items * gap;
-        each = units / ctas;
+        each = (int)((uint32_t)units / (uint32_t)ctas);
         more = units - each * ctas;
         begin = cur = piece(blockIdx.x);
         end = piece(blockIdx.x + 1);
         for (int base = 0, b0 = 0;; b0 += 32) {
-            int own = 0;
-            if (b0 + lane < p.batch) {
-                const Sequence s = sequence_of<ROWS>(p, b0 + lane);
-                own = (s.tiles + gap) * s.row_tiles * p.kv_heads;
-            }
+            if (b0 > 0) mine = b0 + lane < p.batch ? sequence_of<ROWS>(p, b0 + lane) : Sequence{};
+            const int own = (mine.tiles + gap) * mine.row_tiles * p.kv_heads;
             int until = own;
 #pragma unroll
             for (int d = 1; d < 32; d *= 2) {
@@ -211,16 +213,16 @@ struct Line {
                 ++b;
                 continue;
             }
-            const int per = s.tiles + gap, index = offset / per;
+            const int per = s.tiles + gap, index = (int)((uint32_t)offset / (uint32_t)per);
             const int item_begin = cur - (offset - index * per), tiles_begin = item_begin + gap, item_end = item_begin + per, to = min(end, item_end);
-            item.head = index / s.row_tiles;
+            item.head = s.row_tiles == 1 ? index : (int)((uint32_t)index / (uint32_t)s.row_tiles);
             item.row0 = (index - item.head * s.row_tiles) * ROWS;
             item.rows = min(ROWS, s.fresh * p.group - item.row0);
             item.token0 = s.token0;
             item.length = s.length;
             item.fresh = s.fresh;
-            item.first_cta = cta_of(tiles_begin);
-            item.last_cta = cta_of(item_end - 1);
+            item.first_cta = tiles_begin >= begin ? blockIdx.x : cta_of(tiles_begin);
+            item.last_cta = item_end <= end ? blockIdx.x : cta_of(item_end - 1);
             item.slot = 2 * (int)blockIdx.x + (tiles_begin >= begin ? 1 : 0);  // only its first piece can begin in this CTA, and only the first item here have begun before
             item.tile0 = max(cur, tiles_begin) - tiles_begin;
             item.tiles = to - tiles_begin - item.tile0;
@@ -264,13 +266,13 @@ __device__ __forceinline__ void copy_tile(const AttentionArgs &p, const Item &it
     }
 }
 
-// Whether query row r of the item may see a position.
+// Whether query row r of the item may see a position.  (Without a return in between: several of these have their loads on their way together.)
 __device__ __forceinline__ bool may_see(const AttentionArgs &p, const Item &item, int r, int token, int pos) {
     const int drafted = pos - (item.length - item.fresh);
-    if (pos >= item.length || r >= item.rows) return false;
-    if (drafted < 0) return true;
-    if (p.mask == nullptr) return drafted <= token;
-    return drafted < p.mask_width && p.mask[(int64_t)(item.token0 + token) * p.mask_stride + drafted] != 0;
+    const bool there = pos < item.length && r < item.rows;
+    uint8_t seen = drafted < 0 || (p.mask == nullptr && drafted <= token);
+    if (there && drafted >= 0 && drafted < p.mask_width) seen = p.mask[(int64_t)(item.token0 + token) * p.mask_stride + drafted];
+    return there && seen != 0;
 }
 // The same for the 64 positions from key0 on, as bits.
 __device__ __forceinline__ uint64_t seen_of_64(const AttentionArgs &p, const Item &item, int r, int token, int key0) {
@@ -304,7 +306,7 @@ __device__ __forceinline__ void write_lse(const AttentionArgs &p, int64_t at, fl
 // Four elements of a query row's result, from the sum of its values and of its probabilities, both in units of 2^top.
 template <int D, typename T>
 __device__ __forceinline__ void write_out(const AttentionArgs &p, const Item &item, int r, int d, float4 v, float sum, float top) {
-    const int row = item.row0 + r, token = row / p.group, head = item.head * p.group + row - token * p.group;
+    const int row = item.row0 + r, token = token_of(p, row), head = item.head * p.group + row - token * p.group;
     const int64_t at = (int64_t)(item.token0 + token) * p.kv_heads * p.group + head;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     T y[4] = {Elems<T>::round(v.x * inv), Elems<T>::round(v.y * inv), Elems<T>::round(v.z * inv), Elems<T>::round(v.w * inv)};

@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&ctl.item_empty[n_items % ITEMS]));
             if (item.rows < 0) break;
-            const int token = (item.row0 + r) / p.group, hidden = first_hidden(p, item);
+            const int token = token_of(p, item.row0 + r), hidden = first_hidden(p, item);
             const bool busy = 32 * quarter < item.rows;  // this warp has rows
 
             // ---- the queries: group 0 brings the first half of a row, group 1 the second ----
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                 uint4 x[LANES];
 #pragma unroll
                 for (int i = 0; i < LANES; ++i) {
-                    const int own = 32 * quarter + STEP * i + lane / LANES, row = item.row0 + own, tok = row / p.group;
+                    const int own = 32 * quarter + STEP * i + lane / LANES, row = item.row0 + own, tok = token_of(p, row);
                     const T *src = static_cast<const T *>(p.q) + (int64_t)(item.token0 + tok) * p.q_token + (int64_t)(item.head * p.group + row - tok * p.group) * p.q_head;
                     x[i] = own < item.rows ? *reinterpret_cast<const uint4 *>(src + grp * (D / 2) + 8 * (lane % LANES)) : make_uint4(0, 0, 0, 0);
                 }
