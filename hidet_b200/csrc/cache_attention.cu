@@ -582,10 +582,7 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
     p.batch = (int)batch;
     p.kv_heads = (int)kv_heads;
     p.group = (int)(heads / kv_heads);
-    int power = 0;
-    while ((1ll << power) < p.group) ++power;
-    p.by_group = (uint32_t)(((1ull << (31 + power)) + p.group - 1) / p.group);
-    p.by_group_shift = 31 + power;
+    p.by_group = divisor_of((uint32_t)p.group);
     p.scale_log2 = scale * kLog2e;
     p.counters = static_cast<unsigned int *>(workspace);
     p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kCounterBytes);

@@ -43,7 +43,7 @@ struct AttentionArgs {
     int64_t mask_stride;
     int mask_width;
     int batch, kv_heads, group;
-    uint32_t by_group, by_group_shift;  // row / group = row * by_group >> by_group_shift for rows below 2^31 (token_of)
+    Divisor by_group;
     float scale_log2;
     float *partial;
     int64_t partial_floats;  // of all pieces of the kernel for many rows
@@ -67,8 +67,8 @@ int launch_wide(const AttentionArgs &p, int dim, bool bf16, cudaStream_t stream)
 
 #ifdef __CUDACC__
 
-// Of a query row (token * group + head in group): 2^31+s / group rounded up, 2^s the power of two from group on, is off by less than one part in 2^31.
-__device__ __forceinline__ int token_of(const AttentionArgs &p, int row) { return (int)((uint64_t)(uint32_t)row * p.by_group >> p.by_group_shift); }
+// Of a query row, token * group + head in group.
+__device__ __forceinline__ int token_of(const AttentionArgs &p, int row) { return (int)quotient((uint32_t)row, p.by_group); }
 
 // A key/value head of a sequence with some of its query rows, and the pieces that it is in.
 struct Item {

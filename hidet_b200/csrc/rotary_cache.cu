@@ -37,7 +37,7 @@ struct RotaryArgs {
 };
 
 // The table row of a token's position, or nullptr where the position lies outside the table.
-__device__ __forceinline__ const float *angles_of(const RotaryArgs &r, int64_t token) {
+__device__ __forceinline__ const float *angles_of(const RotaryArgs &r, uint32_t token) {
     const int64_t p = index_at(r.positions, r.position_bytes, token);
     return p < 0 || p >= r.table_rows ? nullptr : r.table + p * r.rotary_dim;
 }
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 6) rotary_kernel(const __grid_consta
     pdl_wait();
     pdl_launch_dependents();
     const int j = threadIdx.x, head = blockIdx.y * blockDim.y + threadIdx.y;
-    const int64_t token = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
+    const uint32_t token = blockIdx.x * blockDim.z + threadIdx.z;  // 32 bits are enough for what the host lets through, rounded up to blocks
     if (token >= tokens || head >= all_heads) return;
     const bool is_q = head < heads;
     const HeadRows &src = is_q ? q : k, &dst = is_q ? q_out : k_out;
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kThreads) rotary_generic_kernel(HeadRows q, He
             continue;
         }
         const int ia = r.interleaved ? 2 * i : i, ib = r.interleaved ? 2 * i + 1 : i + half;
-        const float *angles = angles_of(r, token);
+        const float *angles = angles_of(r, (uint32_t)token);
         float a = 0.0f, b = 0.0f;
         if (angles != nullptr) {
             a = Elems<T>::one(x[ia]);
@@ -237,13 +237,13 @@ __device__ __forceinline__ float larger(float top, float x) {
 
 // GROUP lanes (threadIdx.x, dim / 16 of them active) hold a row: a head of q (rotated and written), of k (rotated and quantized) or of v (quantized).
 template <typename T, bool VEC, int GROUP>
-__global__ void __launch_bounds__(kThreads, 6) append_kernel(const __grid_constant__ HeadRows q, const __grid_constant__ HeadRows q_out, const __grid_constant__ HeadRows k,
+__global__ void __launch_bounds__(kThreads, 5) append_kernel(const __grid_constant__ HeadRows q, const __grid_constant__ HeadRows q_out, const __grid_constant__ HeadRows k,
                                                               const __grid_constant__ HeadRows v, uint8_t *cache, const __grid_constant__ CacheShape c, const void *slots, int slot_bytes,
                                                               const __grid_constant__ RotaryArgs r, int64_t tokens, int heads) {
     pdl_wait();
     pdl_launch_dependents();
     const int j = threadIdx.x, row = blockIdx.y * blockDim.y + threadIdx.y, rows = heads + 2 * c.kv_heads;
-    const int64_t token = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
+    const uint32_t token = blockIdx.x * blockDim.z + threadIdx.z;  // 32 bits are enough for what the host lets through, rounded up to blocks
     const bool active = token < tokens && row < rows && 16 * j < c.dim;
     const bool is_q = row < heads, is_v = row >= heads + c.kv_heads;
     const int h = is_q ? row : is_v ? row - heads - c.kv_heads : row - heads;
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 6) append_kernel(const __grid_consta
     }
     uint32_t in_record;
     uint8_t *record = record_of(cache, c, slot, h, in_record);
-    const uint32_t order = is_v ? v_order(in_record, c.dim) : k_order(in_record, c.dim);
+    const uint32_t order = (is_v ? v_rank(in_record) : k_rank(in_record)) >> c.order;
     uint8_t *codes = record + (is_v ? 16 * c.dim : 0) + in_record * c.dim;
     *reinterpret_cast<uint2 *>(codes + 16 * (((uint32_t)ca >> 1) ^ order) + 8 * (ca & 1)) = codes_of(a, inv);
     *reinterpret_cast<uint2 *>(codes + 16 * (((uint32_t)cb >> 1) ^ order) + 8 * (cb & 1)) = codes_of(b, inv);
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const uint8_t *cache, co
     pdl_wait();
     pdl_launch_dependents();
     const int j = threadIdx.x, h = blockIdx.y * blockDim.y + threadIdx.y;
-    const int64_t token = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
+    const uint32_t token = blockIdx.x * blockDim.z + threadIdx.z;  // 32 bits are enough for what the host lets through, rounded up to blocks
     if (token >= tokens || h >= c.kv_heads) return;
     const int64_t slot = index_at(slots, slot_bytes, token);
     uint2 x[2] = {make_uint2(0x80808080u, 0x80808080u), make_uint2(0x80808080u, 0x80808080u)};
@@ -332,8 +332,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const uint8_t *cache, co
     if (slot >= 0 && slot < c.slots) {
         uint32_t in_record;
         const uint8_t *record = record_of(const_cast<uint8_t *>(cache), c, slot, h, in_record), *codes = record + in_record * c.dim + 8 * (j & 1);
-        x[0] = *reinterpret_cast<const uint2 *>(codes + 16 * (((uint32_t)j >> 1) ^ k_order(in_record, c.dim)));
-        x[1] = *reinterpret_cast<const uint2 *>(codes + 16 * c.dim + 16 * (((uint32_t)j >> 1) ^ v_order(in_record, c.dim)));
+        x[0] = *reinterpret_cast<const uint2 *>(codes + 16 * (((uint32_t)j >> 1) ^ k_rank(in_record) >> c.order));
+        x[1] = *reinterpret_cast<const uint2 *>(codes + 16 * c.dim + 16 * (((uint32_t)j >> 1) ^ v_rank(in_record) >> c.order));
         scale[0] = reinterpret_cast<const float *>(record + 32 * c.dim)[in_record];
         scale[1] = reinterpret_cast<const float *>(record + 32 * c.dim)[16 + in_record];
     } else if (slot >= c.slots && j == 0 && h == 0 && status != nullptr) {
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const uint8_t *cache, co
             const uint32_t w = e < 2 ? x[i].x : x[i].y;
             y[e] = mul2(add2(pair_of(__byte_perm(w, 0x4b000000u, 0x7540u | (2 * e & 3)), __byte_perm(w, 0x4b000000u, 0x7540u | (2 * e + 1 & 3))), minus), by);
         }
-        store8<T, true>((i == 0 ? k : v) + (token * c.kv_heads + h) * c.dim + 8 * j, Pairs<T>::narrow(y));
+        store8<T, true>((i == 0 ? k : v) + ((int64_t)token * c.kv_heads + h) * c.dim + 8 * j, Pairs<T>::narrow(y));
     }
 }
 
@@ -389,6 +389,7 @@ int check_cache(const char *op, const void *cache, int64_t pages, int64_t page_s
     }
     if (!cache_dim(head_dim)) return set_error(B200Q_UNSUPPORTED, "%s: heads of %lld elements: 64, 96, 128, 192 and 256 are supported", op, (long long)head_dim);
     if (kv_heads > 65536) return set_error(B200Q_UNSUPPORTED, "%s: %lld heads", op, (long long)kv_heads);
+    if (pages > 1ll << 40) return set_error(B200Q_UNSUPPORTED, "%s: %lld pages", op, (long long)pages);
     if (pages > 0 && (cache == nullptr || !aligned_to(cache, 16))) return set_error(B200Q_INVALID_ARGUMENT, "%s: the cache must be 16-byte aligned, got %p", op, cache);
     return B200Q_OK;
 }
@@ -491,7 +492,7 @@ B200Q_API int b200q_quantized_cache_append(void *cache, int64_t pages, int64_t p
         (heads > 0 && (q == nullptr || q_out == nullptr || q->data == nullptr || q_out->data == nullptr))) {
         return set_error(B200Q_INVALID_ARGUMENT, "%s: null pointer argument", op);
     }
-    const CacheShape c = {pages, pages * page_size, (int)page_size, (int)kv_heads, (int)head_dim};
+    const CacheShape c = cache_shape(pages, page_size, kv_heads, head_dim);
     const RotaryArgs r = {positions, table, table_rows, position_bytes, (int)rotary_dim, layout == B200Q_ROTARY_INTERLEAVED, device_status_word()};
     const HeadRows none = {nullptr, 0, 0};
     const HeadRows a = heads > 0 ? rows_of(q) : none, ao = heads > 0 ? rows_of(q_out) : none, kr = rows_of(k), vr = rows_of(v);
@@ -517,7 +518,7 @@ B200Q_API int b200q_quantized_cache_read(const void *cache, int64_t pages, int64
     if (tokens > kMostTokens) return set_error(B200Q_UNSUPPORTED, "%s: %lld tokens", op, (long long)tokens);
     if (slots == nullptr || k == nullptr || v == nullptr) return set_error(B200Q_INVALID_ARGUMENT, "%s: null pointer argument", op);
     if (!aligned_to(k, 16) || !aligned_to(v, 16)) return set_error(B200Q_INVALID_ARGUMENT, "%s: k and v must be 16-byte aligned", op);
-    const CacheShape c = {pages, pages * page_size, (int)page_size, (int)kv_heads, (int)head_dim};
+    const CacheShape c = cache_shape(pages, page_size, kv_heads, head_dim);
     const uint8_t *bytes = static_cast<const uint8_t *>(cache);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (type) {

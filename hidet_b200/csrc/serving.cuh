@@ -26,32 +26,55 @@ constexpr unsigned int kBadToken = 1u << 26;     // a token outside the vocabula
 // different banks by themselves; rows of 96 bytes keep conflicts of degree two.
 __host__ __device__ constexpr int record_bytes(int dim) { return 32 * dim + 128; }
 __host__ __device__ constexpr int order_shift(int dim) { return dim % 128 == 0 ? 0 : dim % 64 == 0 ? 1 : 2; }
-__host__ __device__ constexpr uint32_t k_order(uint32_t row, int dim) { return (((row >> 1) & 6u) | (row & 1u)) >> order_shift(dim); }
-__host__ __device__ constexpr uint32_t v_order(uint32_t row, int dim) { return (row & 7u) >> order_shift(dim); }
+__host__ __device__ constexpr uint32_t k_rank(uint32_t row) { return ((row >> 1) & 6u) | (row & 1u); }
+__host__ __device__ constexpr uint32_t v_rank(uint32_t row) { return row & 7u; }
+__host__ __device__ constexpr uint32_t k_order(uint32_t row, int dim) { return k_rank(row) >> order_shift(dim); }
+__host__ __device__ constexpr uint32_t v_order(uint32_t row, int dim) { return v_rank(row) >> order_shift(dim); }
 inline bool cache_dim(int64_t dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256; }
 
+// n / d for n below 2^31 as n * by >> shift: by is 2^31+s / d rounded up, 2^s the power of two from d on, off by less than one part in 2^31.  Three instructions for
+// the two dozen of a division.
+struct Divisor {
+    uint32_t by, shift;
+};
+inline Divisor divisor_of(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return {(uint32_t)(((1ull << (31 + s)) + d - 1) / d), 31 + s};
+}
+
 struct CacheShape {
-    int64_t pages;
     int64_t slots;  // pages * page_size
     int page_size, kv_heads, dim;
+    Divisor by_page;
+    int records;      // of a page and head
+    int page_records;  // of a page
+    int order;        // order_shift(dim)
 };
+inline CacheShape cache_shape(int64_t pages, int64_t page_size, int64_t kv_heads, int64_t dim) {
+    const int records = (int)page_size >> 4;
+    return {pages * page_size, (int)page_size, (int)kv_heads, (int)dim, divisor_of((uint32_t)page_size), records, records * (int)kv_heads, order_shift((int)dim)};
+}
 
 #ifdef __CUDACC__
 
+__device__ __forceinline__ uint32_t quotient(uint32_t n, Divisor d) { return (uint32_t)((uint64_t)n * d.by >> d.shift); }
+
 // A slot's place: the record, and the row in it.
 __device__ __forceinline__ uint8_t *record_of(uint8_t *cache, const CacheShape &c, int64_t slot, int head, uint32_t &row) {
-    int64_t page;
+    int64_t record;
     uint32_t in_page;
-    if (c.slots <= 0xffffffffll) {  // a division of 32 bits takes a fifth of one of 64
-        const uint32_t p = (uint32_t)slot / (uint32_t)c.page_size;
-        page = p;
-        in_page = (uint32_t)slot - p * (uint32_t)c.page_size;
+    if (c.slots <= 0x80000000ll) {
+        const uint32_t page = quotient((uint32_t)slot, c.by_page);
+        record = (uint64_t)page * (uint32_t)c.page_records;
+        in_page = (uint32_t)slot - page * (uint32_t)c.page_size;
     } else {
-        page = slot / c.page_size;
+        const int64_t page = slot / c.page_size;
+        record = page * c.page_records;
         in_page = (uint32_t)(slot - page * c.page_size);
     }
     row = in_page & 15u;
-    return cache + ((page * c.kv_heads + head) * (c.page_size >> 4) + (in_page >> 4)) * record_bytes(c.dim);
+    return cache + (record + ((uint32_t)(head * c.records) + (in_page >> 4))) * record_bytes(c.dim);
 }
 
 // ---- eight elements <-> float ----
