@@ -21,7 +21,8 @@
 //
 // Bound by the cache's bytes where sequences are long: pieces stream at 5.9 TB/s, and 8 us are the launch, the plan, the first tile and the additions.  Measured with
 // 128 elements a head, 64 heads over 8: 32 sequences of 90 to 8000 positions 58 us, one of 131071 58 us, 4.7 TB/s each.  Where they are short it is
-// latency: 5.4 us for one tile, 7.5 for two pieces and their sum, 11.1 for 577 positions of 32 heads.
+// latency: 5.25 us for one tile, 7.6 for two pieces and their sum, 10.6 for 577 positions of 32 heads.  (Code that the instruction caches hold already, by an
+// item without rows in front, and all of the queries' loads on their way at once change nothing there.)
 #include <atomic>
 
 #include "cache_attention.cuh"

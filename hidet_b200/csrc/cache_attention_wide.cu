@@ -17,11 +17,11 @@
 // memory, for scales (four bytes a clock, whoever asks for them) and for instructions.  The codes' conversion, 900 clocks a tile, keeps out of the way.
 // An item has about 8000 clocks that no tile hides: its queries, its first scores, the last product and the result.
 //
-// Measured with 128 elements a head, f16 (and in the kernel for few rows), us: 8 sequences of 4096 positions, 64 rows, 64 heads over 8: 140.7 (523), 488 TFLOP/s counting
-// all positions; 8 of 820 to 4096, 64 rows, 32 over 8: 58 (197); 16 of 600, 48 rows, 32 over 8: 41 (96); 50 of 90, 11 rows, 128 over 32, where it is the
-// items' cost above all: 82 (146).
+// Measured with 128 elements a head, f16 (and in the kernel for few rows), us: 8 sequences of 4096 positions, 64 rows, 64 heads over 8: 142 (523), 483 TFLOP/s counting
+// all positions; 8 of 820 to 4096, 64 rows, 32 over 8: 59 (197); 16 of 600, 48 rows, 32 over 8: 41 (96); 50 of 90, 11 rows, 128 over 32, where it is the
+// items' cost above all: 77 (146).
 // Slower: one reading of the scores with all 64 in registers (spills, and code beyond the instruction caches), two groups that convert, the
-// next item's queries loaded in front of the last product (registers spill: 88 us for the 82).
+// next item's queries loaded in front of the last product (registers spill: 88 us where it was 82 then).
 #include <stddef.h>
 
 #include "cache_attention.cuh"

@@ -6,13 +6,13 @@
 // distribution: its values are NaN.
 //
 // A row, or with few or long rows a part of one, is brought into a CTA's shared memory by one bulk copy (the bytes in front of its first and
-// behind its last 16-byte boundary by loads) and read from there twice: for the maximum of every thread, and for the sums.  Bound by the
-// copy where rows are many.  CTAs of a row are a cluster and meet in the shared memory of the first.
+// behind its last 16-byte boundary by loads) and read from there twice: for the maximum of every thread, and for the sums.  CTAs of a row are a cluster and meet in the shared memory of the first.
 //
-// Measured: 2047 rows of 32002 bf16 logits with 20 alternatives 41.2 us, 3.2 TB/s; one row 6.1 us.  A copy at memory's rate would take 20 us, and the instructions, 12 an element,
-// 22: what is above that is that a row's steps (copy, maxima, bound, sums, alternatives) wait for one another, and with three rows an SM, all that fits its
+// Measured: 2047 rows of 32002 bf16 logits with 20 alternatives 41 us, 3.2 TB/s (without alternatives 30); 2476 of 6842 with 5: 21.8; one row 6.1.  A copy at
+// memory's rate would take 20 us, and the instructions, 12 an element, 22: what is above that is that a row's steps (copy, maxima, bound, sums, alternatives) wait for one another, and with three rows an SM, all that fits its
 // shared memory, half of the issue slots stay empty.  More threads a row, parts of half the size (two CTAs a row: 83 us) and candidates sought outside
-// the sums' loop (43 to 50 us) are slower.
+// the sums' loop (43 to 50 us) are slower.  Five CTAs an SM, where shared memory lets them, want 48 registers, for which loops are unrolled by two and four: with three
+// and 78 registers rows of 6842 took 28.5 us and long rows as long as now; with six and 40, 20.4, and long rows 1 to 2 % more.
 //
 // The maxima of 64 groups of threads bound the alternatives: at least `top` elements are no smaller than the top-th largest of them.  So what the second
 // reading passes over is compared with that bound, eight elements at once, and the few that reach it (some 1.2 * top on random rows) are put
@@ -180,14 +180,14 @@ __device__ __forceinline__ void order_keys(const uint64_t *keys, int n, int top,
     for (int i = threadIdx.x; i < n; i += THREADS) {
         const uint64_t own = keys[i];
         int rank = 0;
-#pragma unroll 8
+#pragma unroll 4
         for (int j = 0; j < n; ++j) rank += keys[j] > own || (keys[j] == own && j < i);
         if (rank < top) best[rank] = own;
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArgs p) {
+__global__ void __launch_bounds__(THREADS, 5) log_probs_kernel(const LogProbsArgs p) {
     constexpr int N = Vec16<T>::N;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Block blk;
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
     // ---- the maximum of every thread ----
     using V = Vec16<T>;
     typename V::Top tops = V::all(-INFINITY);
-#pragma unroll 8
+#pragma unroll 4
     for (int v = threadIdx.x; v < vecs; v += THREADS) tops = V::larger(tops, V::top(x[v]));
     float m = V::value(tops);
     uint32_t group = (int)threadIdx.x < vecs ? ordered(m) : 0;
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(THREADS, 3) log_probs_kernel(const LogProbsArg
     if (m >= V::kLeast || !(fabsf(m) < INFINITY)) {
         const f32x2 minus = pair_of(-shift, -shift), log2e = pair_of(kLog2e, kLog2e);
         f32x2 sums = 0, products = 0;
-#pragma unroll 4
+#pragma unroll 2
         for (int v = threadIdx.x; v < vecs; v += THREADS) {
             f32x2 f[N / 2];
             const uint4 raw = x[v];
