@@ -72,7 +72,7 @@ struct Layout {
     static constexpr int PER_SM = NT * D <= 128 ? 3 : NT * D <= 256 ? 2 : 1;
     static constexpr int Q = ROWS * D * 2;
     static constexpr int FIXED = Q + BUFFERS * MERGE;
-    static constexpr int ROOM = (PER_SM == 3 ? 75 : PER_SM == 2 ? 113 : 226) * 1024 - 3072 - FIXED;  // 3072: Control, and what an SM keeps for itself
+    static constexpr int ROOM = (PER_SM == 3 ? 75 : PER_SM == 2 ? 113 : 226) * 1024 - 3 * 1024 - FIXED;  // 3 KB: Control, and what an SM keeps for itself
     static constexpr int STAGES = ROOM / STAGE > MOST_STAGES ? MOST_STAGES : ROOM / STAGE;
     static constexpr int SMEM = FIXED + STAGES * STAGE;
     static constexpr bool Q_IN_REGISTERS = NT * D <= 128;
