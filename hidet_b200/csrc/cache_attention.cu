@@ -502,16 +502,19 @@ int launch_sized(AttentionArgs p, cudaStream_t stream) {
     return launch_after("cache_attention_kernel", kernel, dim3((unsigned)grid), THREADS, L::SMEM, 1, stream, p);
 }
 
-// Rows of the query that share a key/value head, on average: up to 8 in 8-row items, more in 16-row items.
+// Items of 8 query rows, and of 16 where more than 8 share a key/value head and there is much work: these read the cache once for twice the rows, but a tile, an item's ends
+// and the additions take them half as long again, and fewer fit an SM.  Measured (8 / 16 rows, us; tiles as in is_wide): 1 sequence of 512 positions, 8 heads of
+// 128, 16 rows (72 tiles) 9.2 / 13.0; of 16384 (2056) 21.9 / 30.0; 16 of 4096 (8320) 50.1 / 53.5; 24 of 4000 (12192) 68.1 / 69.2, with 64 elements 48.9 / 41.9, 96: 61.8 / 55.5,
+// 192: 99.4 / 85.8, 256: 138 / 122; 1 of 131071 (16392) 92 / 86.
 template <typename T>
 int launch_typed(const AttentionArgs &p, int dim, cudaStream_t stream) {
-    const bool wide = p.tokens * p.group > 8 * (int64_t)p.batch;
+    const bool sixteen = p.tokens * p.group > 8 * (int64_t)p.batch && tiles_of_16(p) > 10000;
     switch (dim) {
-        case 64: return wide ? launch_sized<64, 2, T>(p, stream) : launch_sized<64, 1, T>(p, stream);
-        case 96: return wide ? launch_sized<96, 2, T>(p, stream) : launch_sized<96, 1, T>(p, stream);
-        case 128: return wide ? launch_sized<128, 2, T>(p, stream) : launch_sized<128, 1, T>(p, stream);
-        case 192: return wide ? launch_sized<192, 2, T>(p, stream) : launch_sized<192, 1, T>(p, stream);
-        default: return wide ? launch_sized<256, 2, T>(p, stream) : launch_sized<256, 1, T>(p, stream);
+        case 64: return sixteen ? launch_sized<64, 2, T>(p, stream) : launch_sized<64, 1, T>(p, stream);
+        case 96: return sixteen ? launch_sized<96, 2, T>(p, stream) : launch_sized<96, 1, T>(p, stream);
+        case 128: return sixteen ? launch_sized<128, 2, T>(p, stream) : launch_sized<128, 1, T>(p, stream);
+        case 192: return sixteen ? launch_sized<192, 2, T>(p, stream) : launch_sized<192, 1, T>(p, stream);
+        default: return sixteen ? launch_sized<256, 2, T>(p, stream) : launch_sized<256, 1, T>(p, stream);
     }
 }
 

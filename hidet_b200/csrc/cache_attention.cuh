@@ -55,14 +55,12 @@ struct AttentionArgs {
 inline int64_t most_tiles(const AttentionArgs &p, int rows) { return p.kv_heads * (p.tokens * p.group / rows + p.batch) * (p.capacity / TILE + 1); }
 // The kernel for many rows (cache_attention_wide.cu) takes heads of 64 and 128 elements; its workspace is asked for from 17 query rows a key/value head on.
 inline bool may_be_wide(int64_t tokens, int64_t group, int64_t batch, int64_t dim) { return (dim == 64 || dim == 128) && tokens * group > 16 * batch; }
-// It takes the calls with more work than 3500 tiles of 64 positions and 16 rows, by what the page table could hold; its fixed costs are 6 us higher.  Measured
-// (few / many rows, us): 1 sequence of 4096 positions, 8 key/value heads: 32 rows 27.2 / 33.1, 96 rows (3120 tiles) 27.8 / 35.0; 16 of 600, 48 rows (3840)
-// 32.4 / 26.4; 4 of 4096, 32 rows (4160) 32.1 / 32.4, 64 rows 46.1 / 33.2; 16 of 4096, 64 rows 147 / 79.
-inline bool is_wide(const AttentionArgs &p, int64_t dim) {
-    if (!may_be_wide(p.tokens, p.group, p.batch, dim)) return false;
-    const int64_t rows = p.tokens * p.group / p.batch;
-    return p.batch * (int64_t)p.kv_heads * (p.capacity / TILE + 1) * ((rows + 15) / 16) > 3500;
-}
+// Tiles of 64 positions and 16 rows, by what the page table could hold.
+inline int64_t tiles_of_16(const AttentionArgs &p) { return p.batch * (int64_t)p.kv_heads * (p.capacity / TILE + 1) * ((p.tokens * p.group / p.batch + 15) / 16); }
+// It takes the calls with more than 4200 of them; its fixed costs are 6 us higher, its tiles of 128 rows cost as much as three of the other kernel's of 8.  Measured
+// (few / many rows, us) with 8 key/value heads of 128 elements: 1 sequence of 4096 positions, 96 rows (3120 tiles) 24.8 / 39.3; 4 of 4096, 32 rows (4160) 29.5 / 34.3;
+// 16 of 600, 48 rows (4224) 31.5 / 26.5; 16 of 300, 96 rows (4608) 35.6 / 24.6; 4 of 4096, 64 rows (8320) 48 / 35; 8 of 8000, 48 rows (24192) 128 / 78.
+inline bool is_wide(const AttentionArgs &p, int64_t dim) { return may_be_wide(p.tokens, p.group, p.batch, dim) && tiles_of_16(p) > 4200; }
 int launch_wide(const AttentionArgs &p, int dim, bool bf16, cudaStream_t stream);
 
 #ifdef __CUDACC__

@@ -32,6 +32,17 @@ def test_ragged_batches(dtype, heads, kv_heads, dim, page_size):
 
 
 @pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('heads,kv_heads,dim,page_size', [(12, 3, 64, 16), (20, 4, 96, 48), (8, 2, 128, 64), (12, 3, 192, 16), (4, 1, 256, 256)])
+def test_items_of_sixteen_rows(dtype, heads, kv_heads, dim, page_size):
+    """Nine to sixteen rows a key/value head on average, much work by the page table."""
+    lengths, tokens = [700, 64, 1, 333, 0, 2049, 16], [3, 4, 1, 9, 2, 3, 2]
+    cache = wide(a_cache(lengths, kv_heads, dim, page_size))
+    check_attention(lengths, tokens, heads, kv_heads, dim, page_size, dtype, cache=cache)
+    mask = torch.rand((sum(tokens), 9), device='cuda', generator=torch.Generator('cuda').manual_seed(44)) < 0.5
+    check_attention(lengths, tokens, heads, kv_heads, dim, page_size, dtype, cache=cache, mask=mask)
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize('heads,kv_heads,dim,most', [(16, 2, 128, 40), (8, 1, 64, 33), (32, 8, 128, 64), (4, 2, 128, 150)])
 def test_trees(dtype, heads, kv_heads, dim, most):
     tokens = [most, 1, most // 2, 3, most]
