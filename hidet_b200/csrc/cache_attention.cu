@@ -205,6 +205,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
         }
         item.rows = -1;
         if (!dead) publish(item);
+        write_unowned<D>(p, lane);
         if (dead) {  // nothing may be on its way when the CTA ends
             for (int back = 1; back <= STAGES && back <= it; ++back) {
                 const int at = it - back;
@@ -499,6 +500,7 @@ int launch_sized(AttentionArgs p, cudaStream_t stream) {
     if (tiles > (1ll << 29)) return set_error(B200Q_UNSUPPORTED, "quantized_cache_attention: up to %lld tiles of %d rows and %d positions", (long long)tiles, L::ROWS, TILE);
     int64_t grid = tiles < at_once ? tiles : at_once;
     if (grid > kMaxCtas) grid = kMaxCtas;
+    if (grid < 1) grid = 1;  // no sequences, whose rows are written all the same
     return launch_after("cache_attention_kernel", kernel, dim3((unsigned)grid), THREADS, L::SMEM, 1, stream, p);
 }
 
@@ -508,7 +510,7 @@ int launch_sized(AttentionArgs p, cudaStream_t stream) {
 // 192: 99.4 / 85.8, 256: 138 / 122; 1 of 131071 (16392) 92 / 86.
 template <typename T>
 int launch_typed(const AttentionArgs &p, int dim, cudaStream_t stream) {
-    const bool sixteen = p.tokens * p.group > 8 * (int64_t)p.batch && tiles_of_16(p) > 10000;
+    const bool sixteen = p.batch > 0 && p.tokens * p.group > 8 * (int64_t)p.batch && tiles_of_16(p) > 10000;
     switch (dim) {
         case 64: return sixteen ? launch_sized<64, 2, T>(p, stream) : launch_sized<64, 1, T>(p, stream);
         case 96: return sixteen ? launch_sized<96, 2, T>(p, stream) : launch_sized<96, 1, T>(p, stream);
@@ -550,18 +552,18 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
     }
     if (!cache_dim(head_dim)) return set_error(B200Q_UNSUPPORTED, "%s: heads of %lld elements: 64, 96, 128, 192 and 256 are supported", op, (long long)head_dim);
     if (!(scale > 0.0f) || scale > 1e30f || scale < 1e-20f) return set_error(B200Q_INVALID_ARGUMENT, "%s: the scale must be a positive number, got %g", op, (double)scale);
-    if (batch == 0 || tokens == 0) return B200Q_OK;
-    if (starts == nullptr && tokens % batch != 0) return set_error(B200Q_INVALID_ARGUMENT, "%s: %lld tokens of %lld sequences need starts", op, (long long)tokens, (long long)batch);
+    if (tokens == 0) return B200Q_OK;
+    if (starts == nullptr && batch > 0 && tokens % batch != 0) return set_error(B200Q_INVALID_ARGUMENT, "%s: %lld tokens of %lld sequences need starts", op, (long long)tokens, (long long)batch);
     if (batch > 1 << 20 || kv_heads > 65536 || tokens > (1ll << 31) / 4 / heads) return set_error(B200Q_UNSUPPORTED, "%s: %lld sequences, %lld tokens of %lld heads", op, (long long)batch, (long long)tokens, (long long)heads);
-    if (q == nullptr || q->data == nullptr || out == nullptr || lengths == nullptr || (table_width > 0 && page_table == nullptr) || (pages > 0 && cache == nullptr)) {
+    if (q == nullptr || q->data == nullptr || out == nullptr || (batch > 0 && (lengths == nullptr || (table_width > 0 && page_table == nullptr))) || (pages > 0 && cache == nullptr)) {
         return set_error(B200Q_INVALID_ARGUMENT, "%s: null pointer argument", op);
     }
-    if (pages <= 0 && table_width > 0) return set_error(B200Q_INVALID_ARGUMENT, "%s: a cache of %lld pages", op, (long long)pages);
+    if (batch > 0 && pages <= 0 && table_width > 0) return set_error(B200Q_INVALID_ARGUMENT, "%s: a cache of %lld pages", op, (long long)pages);
     if (!aligned_to(cache, 16) || !aligned_to(q->data, 16) || !aligned_to(out, 16) || q->token_stride % 8 != 0 || q->head_stride % 8 != 0) {
         return set_error(B200Q_INVALID_ARGUMENT, "%s: 16-byte aligned cache, q and out and strides of 8 elements are wanted", op);
     }
     const size_t need = b200q_quantized_cache_attention_workspace_bytes(batch, tokens, heads, kv_heads, head_dim);
-    if (workspace == nullptr || workspace_bytes < need) return set_error(B200Q_WORKSPACE_TOO_SMALL, "%s: a workspace of %zu bytes is needed, got %zu", op, need, workspace_bytes);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return set_error(B200Q_WORKSPACE_TOO_SMALL, "%s: a workspace of %zu bytes is needed, got %zu", op, need, workspace_bytes);
     if (!aligned_to(workspace, 16)) return set_error(B200Q_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", op);
     AttentionArgs p = {};
     p.q = q->data;
@@ -579,7 +581,7 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
     p.lengths = lengths;
     p.starts = starts;
     p.tokens = tokens;
-    p.per_sequence = starts == nullptr ? (int)(tokens / batch) : 0;
+    p.per_sequence = starts == nullptr && batch > 0 ? (int)(tokens / batch) : 0;
     p.mask = static_cast<const uint8_t *>(mask);
     p.mask_stride = mask_stride;
     p.mask_width = (int)(mask_width < (1 << 30) ? mask_width : 1 << 30);

@@ -56,11 +56,11 @@ inline int64_t most_tiles(const AttentionArgs &p, int rows) { return p.kv_heads 
 // The kernel for many rows (cache_attention_wide.cu) takes heads of 64 and 128 elements; its workspace is asked for from 17 query rows a key/value head on.
 inline bool may_be_wide(int64_t tokens, int64_t group, int64_t batch, int64_t dim) { return (dim == 64 || dim == 128) && tokens * group > 16 * batch; }
 // Tiles of 64 positions and 16 rows, by what the page table could hold.
-inline int64_t tiles_of_16(const AttentionArgs &p) { return p.batch * (int64_t)p.kv_heads * (p.capacity / TILE + 1) * ((p.tokens * p.group / p.batch + 15) / 16); }
+inline int64_t tiles_of_16(const AttentionArgs &p) { return p.batch * (int64_t)p.kv_heads * (p.capacity / TILE + 1) * ((p.tokens * p.group / p.batch + 15) / 16); }  // batch > 0
 // It takes the calls with more than 4200 of them; its fixed costs are 6 us higher.  Measured
 // (few / many rows, us) with 8 key/value heads of 128 elements: 1 sequence of 4096 positions, 96 rows (3120 tiles) 24.8 / 39.3; 4 of 4096, 32 rows (4160) 29.5 / 34.3;
 // 16 of 600, 48 rows (4224) 31.5 / 26.5; 16 of 300, 96 rows (4608) 35.6 / 24.6; 4 of 4096, 64 rows (8320) 48 / 35; 8 of 8000, 48 rows (24192) 128 / 78.
-inline bool is_wide(const AttentionArgs &p, int64_t dim) { return may_be_wide(p.tokens, p.group, p.batch, dim) && tiles_of_16(p) > 4200; }
+inline bool is_wide(const AttentionArgs &p, int64_t dim) { return p.batch > 0 && may_be_wide(p.tokens, p.group, p.batch, dim) && tiles_of_16(p) > 4200; }
 int launch_wide(const AttentionArgs &p, int dim, bool bf16, cudaStream_t stream);
 
 #ifdef __CUDACC__
@@ -300,6 +300,22 @@ __device__ __forceinline__ int first_hidden(const AttentionArgs &p, const Item &
 
 __device__ __forceinline__ void write_lse(const AttentionArgs &p, int64_t at, float sum, float top) {
     if (p.lse != nullptr) p.lse[at] = sum == 0.0f ? -INFINITY : (top - kBias + __log2f(sum)) * kLn2;
+}
+// Zeros, and -inf for their softmax's denominators, in the place of the results of rows of q that no sequence has: those in front of the first one's and behind the
+// last one's (a captured step has a fixed number of rows, often with fewer in use).  One warp of every CTA, with nothing waiting for it.
+template <int D>
+__device__ __forceinline__ void write_unowned(const AttentionArgs &p, int lane) {
+    if (p.starts == nullptr && p.batch > 0) return;  // tokens / batch each: all rows
+    const int64_t from = p.starts != nullptr ? min(max((int64_t)p.starts[0], (int64_t)0), p.tokens) : 0;
+    const int64_t to = p.starts != nullptr ? min(max((int64_t)p.starts[p.batch], from), p.tokens) : 0;
+    const int heads = p.kv_heads * p.group;
+    for (int64_t i = blockIdx.x; i < p.tokens - (to - from); i += gridDim.x) {
+        const int64_t row = (i < from ? i : i + (to - from)) * heads;
+        uint4 *out = reinterpret_cast<uint4 *>(p.out) + row * (D / 8);
+        for (int j = lane; j < heads * (D / 8); j += 32) out[j] = make_uint4(0, 0, 0, 0);
+        if (p.lse != nullptr)
+            for (int j = lane; j < heads; j += 32) p.lse[row + j] = -INFINITY;
+    }
 }
 // Four elements of a query row's result, from the sum of its values and of its probabilities, both in units of 2^top.
 template <int D, typename T>

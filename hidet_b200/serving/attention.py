@@ -17,7 +17,8 @@ def quantized_cache_attention(q: torch.Tensor, cache: torch.Tensor, page_table: 
     """softmax(scale * q k^T) v over the cached positions of every sequence, its newest tokens (the rows of q) among them.
 
     q           float16 or bfloat16: [batch, heads, dim], one token a sequence; [batch, t, heads, dim], t tokens each; or, with starts, [tokens, heads, dim],
-                those of sequence b in rows starts[b] .. starts[b + 1] - 1 (int32 [batch + 1]).  heads is a multiple of the cache's.
+                those of sequence b in rows starts[b] .. starts[b + 1] - 1 (int32 [batch + 1]).  heads is a multiple of the cache's.  Rows in front of
+                starts[0] and from starts[batch] on, such as a captured step's unused ones, are zeros, with -inf for their denominators.
     page_table  int32 [batch, n]: the pages of every sequence, in order; lengths int32 [batch]: its cached positions, new tokens included.
     mask        None: a token sees every position up to its own.  Or bool / uint8 [tokens, w] with a row for every row of q: of the positions in front of its
                 sequence's new tokens it sees all, and the j-th of these where mask[row, j] (w at least the most of a sequence).  Trees of drafted

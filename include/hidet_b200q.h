@@ -347,7 +347,7 @@ B200Q_API int b200q_quantized_cache_read(const void *cache, int64_t pages, int64
  * positions another page's contents; both are reported).  Its tokens are rows starts[b] .. starts[b + 1] - 1 of q and out, or
  * tokens / batch rows each where starts is NULL, and stand at its last positions.  A token sees every position in front of them, and of
  * them those up to itself, or, with a mask, those with mask[row * mask_stride + j] != 0 (a byte for the j-th of its sequence's new tokens, j < mask_width).
- * A row that sees nothing has zeros, and -inf in lse.  head h reads key/value head h / (heads / kv_heads).
+ * A row that sees nothing has zeros, and -inf in lse, and so has a row that no sequence has (in front of starts[0], from starts[batch] on).  head h reads key/value head h / (heads / kv_heads).
  *   out[row, h] = sum_j softmax_j(scale q . k_j) v_j, dense [tokens, heads, head_dim] in q's type (f16 or bf16); lse (float [tokens, heads], may be
  * NULL) the natural logarithm of the softmax's denominator.  q and out: 16-byte aligned,
  * strides multiples of 8 elements.

@@ -1,0 +1,65 @@
+"""The decoding operators where a call's data is at an end of its range: rows that no sequence has, and what their neighbours hold."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import hidet_b200
+from hidet_b200 import ffi
+from test_serving_gpu import a_cache, clean_status, normal  # noqa: F401
+from test_serving_paths_gpu import wide
+
+pytestmark = pytest.mark.gpu
+
+
+def attention_into(out, lse, q, cache, table, lengths, starts=None, mask=None, mask_width=None):
+    """The entry point's result in tensors of the caller's, contiguous q [tokens, heads, dim].  Returns them."""
+    tokens, heads, dim = q.shape
+    batch, kv_heads = len(lengths), cache.shape[1]
+    need = ffi.func('b200q_quantized_cache_attention_workspace_bytes')(batch, tokens, heads, kv_heads, dim)
+    workspace = torch.zeros(max(16, need), dtype=torch.uint8, device='cuda')
+    ffi.func('b200q_quantized_cache_attention')(
+        ctypes.byref(ffi.Heads(q.data_ptr(), heads * dim, dim)), out.data_ptr(), lse.data_ptr(), cache.data_ptr(), cache.shape[0], cache.shape[2] * 16, table.data_ptr(), table.shape[1],
+        table.stride(0), lengths.data_ptr(), starts.data_ptr() if starts is not None else None, mask.data_ptr() if mask is not None else None,
+        mask_width if mask_width is not None else mask.shape[1] if mask is not None else 0, mask.stride(0) if mask is not None else 0, batch, tokens, heads, kv_heads, dim, 1 / math.sqrt(dim),
+        {torch.float16: ffi.F16, torch.bfloat16: ffi.BF16}[q.dtype], workspace.data_ptr(), workspace.numel(), torch.cuda.current_stream().cuda_stream)
+    return out, lse
+
+
+def ints(*x):
+    return torch.tensor(x, dtype=torch.int32, device='cuda')
+
+
+# heads, kv_heads, dim and tokens of two sequences, the page table made for long ones: one or two of 8 rows, of 16, and the kernel for many
+FORMS = [(4, 2, 64, (1, 1), False), (4, 1, 128, (3, 5), False), (8, 1, 96, (2, 1), True), (8, 2, 128, (40, 23), True), (16, 2, 64, (9, 30), True)]
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('heads,kv_heads,dim,tokens,long', FORMS)
+@pytest.mark.parametrize('front,behind', [(0, 3), (2, 0), (1, 700)])
+def test_rows_that_no_sequence_has_are_zeros(dtype, heads, kv_heads, dim, tokens, long, front, behind):
+    lengths = [700, 90]
+    cache, table = a_cache(lengths, kv_heads, dim, 16)
+    if long:
+        cache, table = wide((cache, table))
+    q = normal(front + sum(tokens) + behind, heads, dim, seed=61, dtype=dtype)
+    starts, n = ints(front, front + tokens[0], front + sum(tokens)), ints(*lengths)
+    out, lse = attention_into(torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device='cuda'), q, cache, table, n, starts)
+    own = slice(front, front + sum(tokens))
+    want = hidet_b200.quantized_cache_attention(q[own], cache, table, n, starts=starts - front, return_lse=True)
+    if not behind == 700:  # so many rows may choose another kernel
+        assert torch.equal(out[own], want[0]) and torch.equal(lse[own], want[1])
+    for rest in (slice(0, front), slice(front + sum(tokens), None)):
+        assert not out[rest].any() and (lse[rest] == -math.inf).all()
+
+
+def test_rows_without_sequences():
+    cache = hidet_b200.quantized_cache(2, 2, 64, 16)
+    q = normal(5, 4, 64, seed=62)
+    out, lse = hidet_b200.quantized_cache_attention(q, cache, ints().reshape(0, 3), ints(), starts=ints(0), return_lse=True)
+    assert not out.any() and (lse == -math.inf).all()
+    out, lse = attention_into(torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device='cuda'), q, cache, ints().reshape(0, 3), ints())
+    assert not out.any() and (lse == -math.inf).all()
+    out, lse = hidet_b200.quantized_cache_attention(q, cache, ints(0, 1)[:, None], ints(9, 4), starts=ints(2, 2, 2), return_lse=True)
+    assert not out.any() and (lse == -math.inf).all()
