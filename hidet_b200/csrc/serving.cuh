@@ -5,14 +5,9 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "status_bits.h"
 
 namespace b200q {
-
-// ---- bits of the status word for indexes that a kernel met outside their range (bit 30: the embedding lookup) ----
-constexpr unsigned int kBadPosition = 1u << 29;  // a rotary position outside the table
-constexpr unsigned int kBadSlot = 1u << 28;      // a slot outside the cache
-constexpr unsigned int kBadPage = 1u << 27;      // a page outside the cache, or a length beyond its row of the page table
-constexpr unsigned int kBadToken = 1u << 26;     // a token outside the vocabulary
 
 // ---- the cache ----
 // uint8 [pages][kv_heads][page_size / 16][32 D + 128]: a record per 16 positions of a head.  A record holds 16 rows of K
