@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
         }
         item.rows = -1;
         if (!dead) publish(item);
-        write_unowned<D>(p, lane);
+        write_unowned<D>(p, line.placed, lane);
         if (dead) {  // nothing may be on its way when the CTA ends
             for (int back = 1; back <= STAGES && back <= it; ++back) {
                 const int at = it - back;

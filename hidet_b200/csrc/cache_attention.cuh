@@ -168,12 +168,13 @@ __device__ __forceinline__ void write_lse(const AttentionArgs &p, int64_t at, fl
     if (p.lse != nullptr) p.lse[at] = sum == 0.0f ? -INFINITY : (top - kBias + __log2f(sum)) * kLn2;
 }
 // Zeros, and -inf for their softmax's denominators, in the place of the results of rows of q that no sequence has: those in front of the first one's and behind the
-// last one's (a captured step has a fixed number of rows, often with fewer in use).  One warp of every CTA, with nothing waiting for it.
+// last one's (a captured step has a fixed number of rows, often with fewer in use); all where the sequences' rows are not `placed`.  One warp of every
+// CTA, with nothing waiting for it.
 template <int D>
-__device__ __forceinline__ void write_unowned(const AttentionArgs &p, int lane) {
+__device__ __forceinline__ void write_unowned(const AttentionArgs &p, bool placed, int lane) {
     if (p.starts == nullptr && p.batch > 0) return;  // tokens / batch each: all rows
-    const int64_t from = p.starts != nullptr ? min(max((int64_t)p.starts[0], (int64_t)0), p.tokens) : 0;
-    const int64_t to = p.starts != nullptr ? min(max((int64_t)p.starts[p.batch], from), p.tokens) : 0;
+    const bool any = p.batch > 0 && placed;
+    const int64_t from = any ? min(max((int64_t)p.starts[0], (int64_t)0), p.tokens) : 0, to = any ? min(max((int64_t)p.starts[p.batch], from), p.tokens) : 0;
     const int heads = p.kv_heads * p.group;
     for (int64_t i = blockIdx.x; i < p.tokens - (to - from); i += gridDim.x) {
         const int64_t row = (i < from ? i : i + (to - from)) * heads;

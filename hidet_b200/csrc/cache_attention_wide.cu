@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
             mbar_arrive(smem_u32(&ctl.raw_full[slot]));
         }
         __syncwarp();
-        write_unowned<D>(p, lane);
+        write_unowned<D>(p, line.placed, lane);
         if (!ok) {  // nothing may be on its way when the CTA ends
             for (int back = 1; back <= RAW_STAGES && back <= it; ++back) {
                 const int at = it - back;

@@ -33,6 +33,7 @@ struct Item {
 
 struct Sequence {
     int length, fresh, token0;
+    bool placed;    // its rows lie inside, and do not end in front of where they begin
     int tiles;      // of one item
     int row_tiles;  // items of a key/value head
 };
@@ -46,10 +47,12 @@ __device__ __forceinline__ Sequence sequence_of(const PlanArgs &p, int b) {
     }
     s.length = n < 0 ? 0 : (int)n;
     if (p.starts != nullptr) {
-        const int64_t first = min(max((int64_t)p.starts[b], (int64_t)0), p.tokens), end = min(max((int64_t)p.starts[b + 1], first), p.tokens);
-        s.token0 = (int)first;
-        s.fresh = (int)(end - first);
+        const int first = p.starts[b], end = p.starts[b + 1];
+        s.placed = first >= 0 && end >= first && end <= p.tokens;
+        s.token0 = s.placed ? first : 0;
+        s.fresh = s.placed ? end - first : 0;
     } else {
+        s.placed = true;
         s.token0 = b * p.per_sequence;
         s.fresh = p.per_sequence;
     }
@@ -66,6 +69,7 @@ struct Line {
     int each = 0, more = 0, gap = 0;            // units of a piece; the first `more` pieces have one more; units in front of an item's tiles
     int begin = 0, cur = 0, end = 0;            // units
     int b = 0, offset = 0;                      // the sequence that cur lies in, and where in its items
+    bool placed = true;                         // all sequences are: no row is in two of them, so that the tiles of all are as few as the host allows
 
     __device__ __forceinline__ int piece(int c) const { return c * each + min(c, more); }
     __device__ __forceinline__ int cta_of(int unit) const {
@@ -76,12 +80,18 @@ struct Line {
     __device__ __forceinline__ Line(const PlanArgs &args, int lane_) : p(args), lane(lane_) {
         // The plan is in front of everything else, alone: few sums and divisions, and no sequence looked up twice that need not be.
         Sequence mine = {};
-        if (lane < p.batch) mine = sequence_of<ROWS>(p, lane);
+        if (lane < p.batch) mine = sequence_of<ROWS>(p, lane), placed = mine.placed;
         int items = mine.row_tiles, tiles = mine.row_tiles * mine.tiles;
         for (int s0 = lane + 32; s0 < p.batch; s0 += 32) {
             const Sequence s = sequence_of<ROWS>(p, s0);
             items += s.row_tiles;
             tiles += s.row_tiles * s.tiles;
+            placed &= s.placed;
+        }
+        if (p.starts != nullptr && !__all_sync(0xffffffffu, placed)) {  // then these are sums of anything, beyond 32 bits too
+            placed = false;
+            if (lane == 0 && p.status != nullptr) atomicOr(p.status, kBadStarts);
+            return;
         }
         items = __reduce_add_sync(0xffffffffu, items) * p.kv_heads;
         tiles = __reduce_add_sync(0xffffffffu, tiles) * p.kv_heads;
@@ -97,7 +107,7 @@ struct Line {
         more = units - each * ctas;
         begin = cur = piece(blockIdx.x);
         end = piece(blockIdx.x + 1);
-        for (int base = 0, b0 = 0;; b0 += 32) {
+        for (int base = 0, b0 = 0; b0 < p.batch; b0 += 32) {
             if (b0 > 0) mine = b0 + lane < p.batch ? sequence_of<ROWS>(p, b0 + lane) : Sequence{};
             const int own = (mine.tiles + gap) * mine.row_tiles * p.kv_heads;
             int until = own;
@@ -111,15 +121,16 @@ struct Line {
                 const int l = __ffs(behind) - 1;
                 b = b0 + l;
                 offset = cur - base - __shfl_sync(0xffffffffu, until - own, l);
-                break;
+                return;
             }
             base += __shfl_sync(0xffffffffu, until, 31);
         }
+        end = cur;  // lengths that have become less since they were counted
     }
 
     // The next item with tiles in this piece, and its sequence's pages; false behind the last.
     __device__ __forceinline__ bool next(Item &item, const int32_t *&pages) {
-        while (cur < end) {
+        while (cur < end && b < p.batch) {
             const Sequence s = sequence_of<ROWS>(p, b);
             if (s.row_tiles == 0) {
                 ++b;

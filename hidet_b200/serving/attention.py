@@ -27,7 +27,8 @@ def quantized_cache_attention(q: torch.Tensor, cache: torch.Tensor, page_table: 
     Returns the result in q's shape and type, and with return_lse also the natural logarithm of the softmax's denominators, float32 of q's shape without dim.
 
     Everything that changes from step to step is on the device: a captured step can be replayed while the sequences grow.  Lengths beyond the page
-    table are cut, and they and pages outside the cache are reported by b200q_check_status."""
+    table are cut, and they and pages outside the cache are reported by b200q_check_status.  So are starts that fall or lie outside the rows; all rows are
+    zeros then."""
     result = native.attention(q, cache, page_table, lengths, starts, mask, scale, return_lse)
     if result is not None:
         return result

@@ -86,3 +86,18 @@ def test_lengths_beyond_the_page_table(program):
     pieces, status = plan(program, 8, 5, [10 ** 9, -3, 100], 3, None, 1, 1, capacity=640)
     check(pieces, 8, [640, -3, 100], [0, 1, 2, 3], 1, 1)
     assert status == 1 << 27
+
+
+@pytest.mark.parametrize('rows,grid', [(8, 444), (16, 296), (128, 148)])
+@pytest.mark.parametrize('starts', [[0, 4096] * 32 + [0], [4096] * 64 + [0], [0] * 64 + [4097], [-1] + [4096] * 64, [0, 5] + [3] * 62 + [9], [2 ** 31 - 1] * 65, [-2 ** 31] * 65,
+                                    [0] * 40 + [4096, 4095] + [4096] * 23, list(range(4096, 4096 - 65, -1))], ids=lambda s: '{}_{}_{}'.format(s[0], s[1], s[-1]))
+def test_starts_out_of_order_or_range(program, rows, grid, starts):
+    """Nothing is planned, and the status word tells.  (The first of these claims every row 32 times over, more tiles than 32 bits count.)"""
+    pieces, status = plan(program, rows, grid, [131072] * 64, 4096, starts, 8, 8)
+    assert not pieces and status == 1 << 25
+
+
+@pytest.mark.parametrize('rows,grid', [(8, 444), (128, 148)])
+def test_rows_without_a_sequence(program, rows, grid):
+    for starts in ([0, 0, 0], [9, 9, 9]):
+        assert plan(program, rows, grid, [100, 200], 9, starts) == ([], 0)

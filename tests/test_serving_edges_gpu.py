@@ -63,3 +63,33 @@ def test_rows_without_sequences():
     assert not out.any() and (lse == -math.inf).all()
     out, lse = hidet_b200.quantized_cache_attention(q, cache, ints(0, 1)[:, None], ints(9, 4), starts=ints(2, 2, 2), return_lse=True)
     assert not out.any() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize('heads,kv_heads,dim,tokens,long', FORMS)
+@pytest.mark.parametrize('starts', [(3, 1, 4), (0, 5, 4), (-1, 1, 2), (0, 1, 10 ** 6), (2 ** 31 - 1, 0, 2 ** 31 - 1), (0, 0, -2 ** 31)])
+def test_starts_out_of_order_or_range_are_reported_and_harmless(heads, kv_heads, dim, tokens, long, starts):
+    lengths = [700, 90]
+    cache, table = a_cache(lengths, kv_heads, dim, 16)
+    if long:
+        cache, table = wide((cache, table))
+    q, n = normal(sum(tokens) + 2, heads, dim, seed=63), ints(*lengths)
+    out, lse = hidet_b200.quantized_cache_attention(q, cache, table, n, starts=ints(*starts), return_lse=True)
+    with pytest.raises(ffi.BackendException, match='sequences whose rows are out of order or outside'):
+        ffi.func('b200q_check_status')()
+    assert not out.any() and (lse == -math.inf).all()
+    fine = ints(0, tokens[0], sum(tokens))
+    assert hidet_b200.quantized_cache_attention(q, cache, table, n, starts=fine)[:sum(tokens)].any()  # the workspace is as it was
+    assert ffi.func('b200q_check_status')() == ffi.OK
+
+
+@pytest.mark.parametrize('dim', [96, 128])
+def test_sequences_that_all_claim_all_rows(dim):
+    """More tiles together than 32 bits count."""
+    cache = hidet_b200.quantized_cache(4, 8, dim, 64)
+    q = normal(4096, 8, dim, seed=64)
+    table = torch.zeros((64, 2048), dtype=torch.int32, device='cuda')
+    n = torch.full((64,), 131072, dtype=torch.int32, device='cuda')
+    out, lse = hidet_b200.quantized_cache_attention(q, cache, table, n, starts=ints(*[0, 4096] * 32, 0), return_lse=True)
+    with pytest.raises(ffi.BackendException, match='sequences whose rows are out of order or outside'):
+        ffi.func('b200q_check_status')()
+    assert not out.any() and (lse == -math.inf).all()
