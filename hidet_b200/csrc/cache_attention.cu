@@ -584,7 +584,7 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
     p.per_sequence = starts == nullptr && batch > 0 ? (int)(tokens / batch) : 0;
     p.mask = static_cast<const uint8_t *>(mask);
     p.mask_stride = mask_stride;
-    p.mask_width = (int)(mask_width < (1 << 30) ? mask_width : 1 << 30);
+    p.mask_width = mask == nullptr ? 0 : (int)(mask_width < (1 << 30) ? mask_width : 1 << 30);  // what lies inside the width is read
     p.batch = (int)batch;
     p.kv_heads = (int)kv_heads;
     p.group = (int)(heads / kv_heads);

@@ -346,7 +346,8 @@ B200Q_API int b200q_quantized_cache_read(const void *cache, int64_t pages, int64
  * cached, in the pages page_table[b * table_stride + i] (a length is cut to table_width pages; a page outside the cache gives that tile of
  * positions another page's contents; both are reported).  Its tokens are rows starts[b] .. starts[b + 1] - 1 of q and out (starts that fall, or
  * lie outside 0 .. tokens, are reported, and no row is anyone's then), or tokens / batch rows each where starts is NULL, and stand at its last positions.  A token sees every position in front of them, and of
- * them those up to itself, or, with a mask, those with mask[row * mask_stride + j] != 0 (a byte for the j-th of its sequence's new tokens, j < mask_width).
+ * them those up to itself, or, with a mask, those with mask[row * mask_stride + j] != 0 (a byte for the j-th of its sequence's new tokens, j < mask_width; without a
+ * mask, NULL, the width counts as 0).
  * A row that sees nothing has zeros, and -inf in lse, and so has a row that no sequence has (in front of starts[0], from starts[batch] on).  head h reads key/value head h / (heads / kv_heads).
  *   out[row, h] = sum_j softmax_j(scale q . k_j) v_j, dense [tokens, heads, head_dim] in q's type (f16 or bf16); lse (float [tokens, heads], may be
  * NULL) the natural logarithm of the softmax's denominator.  q and out: 16-byte aligned,

@@ -93,3 +93,17 @@ def test_sequences_that_all_claim_all_rows(dim):
     with pytest.raises(ffi.BackendException, match='sequences whose rows are out of order or outside'):
         ffi.func('b200q_check_status')()
     assert not out.any() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize('heads,kv_heads,dim,tokens,long', FORMS)
+def test_a_width_without_a_mask_is_none(heads, kv_heads, dim, tokens, long):
+    lengths = [700, 90]
+    cache, table = a_cache(lengths, kv_heads, dim, 16)
+    if long:
+        cache, table = wide((cache, table))
+    q = normal(sum(tokens), heads, dim, seed=65)
+    starts, n = ints(0, tokens[0], sum(tokens)), ints(*lengths)
+    want = hidet_b200.quantized_cache_attention(q, cache, table, n, starts=starts, return_lse=True)
+    for width in (1, 64, 1 << 40):
+        got = attention_into(torch.empty_like(q), torch.empty(q.shape[:2], device='cuda'), q, cache, table, n, starts, mask_width=width)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
