@@ -146,7 +146,7 @@ __device__ __forceinline__ uint64_t seen_of_64(const AttentionArgs &p, const Ite
     uint64_t seen = sure >= 64 ? ~0ull : sure > 0 ? (1ull << sure) - 1 : 0;
     if (p.mask != nullptr) {
         const uint8_t *row = p.mask + (int64_t)(item.token0 + token) * p.mask_stride + (key0 - old);
-        const int from = old - key0, until = min(item.length, old + p.mask_width) - key0;
+        const int from = old - key0, until = from + min(item.fresh, p.mask_width);
 #pragma unroll 1
         for (int h = 0; h < 64; h += 32) {
             uint32_t bits = 0;

@@ -107,3 +107,23 @@ def test_a_width_without_a_mask_is_none(heads, kv_heads, dim, tokens, long):
     for width in (1, 64, 1 << 40):
         got = attention_into(torch.empty_like(q), torch.empty(q.shape[:2], device='cuda'), q, cache, table, n, starts, mask_width=width)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_a_wide_mask_of_a_very_long_sequence():
+    """Positions and the mask's width together pass 31 bits.  All pages but the last are one."""
+    length, page, heads, dim = 1_200_000_017, 65536, 16, 64
+    cache, table = a_cache([2 * page], 1, dim, page, spare=0)
+    table = table[:, :1].repeat(1, -(-length // page))
+    table[:, -1] = 1 - table[0, 0]
+    q, mask = normal(3, heads, dim, seed=66), torch.tensor([[1, 0, 0], [0, 1, 0], [1, 0, 1]], dtype=torch.uint8, device='cuda')
+    own = table[0, -1].long() * page + torch.arange(length - 3, length, device='cuda') % page
+    loud = torch.zeros((3, 1, dim), device='cuda')
+    loud[:, 0, 0] = 400.0
+    hidet_b200.quantized_cache_append(cache, loud, normal(3, 1, dim, seed=67, dtype=torch.float32), own)  # the drafted positions decide a row's result
+    q[:, :, 0] = 8.0
+    starts, n = ints(0, 3), ints(length)
+    got = [attention_into(torch.empty_like(q), torch.empty(q.shape[:2], device='cuda'), q, cache, table, n, starts, mask, width) for width in (3, 1 << 30)]
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    v = hidet_b200.quantized_cache_read(cache, own, torch.float32)[1][:, 0]
+    want = torch.stack([v[0], v[1], (v[0] + v[2]) / 2])[:, None].expand(3, heads, dim)
+    assert (got[1][0].float() - want).abs().max() < 1e-2  # every other score is 300 below theirs
