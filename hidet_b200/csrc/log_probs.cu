@@ -58,13 +58,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // 16 bytes of logits.  pairs: as floats, none below a finite number, whose probability is zero beside a maximum of at least kLeast, so that this times it is zero
-// as well.
+// as well; for a maximum of at most kMost its distance, in log2, is finite too.
 template <typename T>
 struct Vec16;
 template <>
 struct Vec16<float> {
     static constexpr int N = 4;
-    static constexpr float kLeast = -1e29f;
+    static constexpr float kLeast = -1e29f, kMost = 1e38f;
     static __device__ __forceinline__ void widen(uint4 v, float (&f)[4]) { f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w); }
     static __device__ __forceinline__ void pairs(uint4 v, f32x2 (&p)[2]) {
         float f[4];
@@ -85,7 +85,7 @@ struct Vec16<float> {
 template <>
 struct Vec16<__half> {
     static constexpr int N = 8;
-    static constexpr float kLeast = -65504.0f + 256.0f;
+    static constexpr float kLeast = -65504.0f + 256.0f, kMost = 65504.0f;
     static __device__ __forceinline__ __half2 h2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
     static __device__ __forceinline__ void widen(uint4 v, float (&f)[8]) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -113,7 +113,7 @@ struct Vec16<__half> {
 template <>
 struct Vec16<__nv_bfloat16> {
     static constexpr int N = 8;
-    static constexpr float kLeast = -1e29f;
+    static constexpr float kLeast = -1e29f, kMost = 1e38f;
     static __device__ __forceinline__ __nv_bfloat162 b2(uint32_t u) { return *reinterpret_cast<__nv_bfloat162 *>(&u); }
     static __device__ __forceinline__ void widen(uint4 v, float (&f)[8]) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(THREADS, 5) log_probs_kernel(const LogProbsArg
     // Which of this thread's vectors reach the bound, the last in bit 0: with a branch for each, which few take, the loop's loads and arithmetic could not overlap.
     uint64_t hits = 0;
     static_assert(kMostPart / 16 / THREADS < 63, "");
-    if (m >= V::kLeast || !(fabsf(m) < INFINITY)) {
+    if ((m >= V::kLeast && m <= V::kMost) || !(fabsf(m) < INFINITY)) {
         const f32x2 minus = pair_of(-shift, -shift), log2e = pair_of(kLog2e, kLog2e);
         f32x2 sums = 0, products = 0;
 #pragma unroll 2
@@ -320,7 +320,8 @@ __global__ void __launch_bounds__(THREADS, 5) log_probs_kernel(const LogProbsArg
         halves(products, lo, hi);
         weighted = lo + hi;
     } else {
-        // Nothing but numbers around the type's lowest, which stand for what is not allowed, and -inf: the two differ here.
+        // Nothing but numbers around the type's lowest, which stand for what is not allowed, and -inf: the two differ here.  Or a maximum so large that a distance from
+        // it may be -inf.
         for (int v = threadIdx.x; v < vecs; v += THREADS) {
             float f[N];
             const uint4 raw = x[v];

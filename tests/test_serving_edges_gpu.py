@@ -7,7 +7,7 @@ import torch
 
 import hidet_b200
 from hidet_b200 import ffi
-from test_serving_gpu import a_cache, clean_status, normal  # noqa: F401
+from test_serving_gpu import TYPES, a_cache, check_log_probs, clean_status, normal  # noqa: F401
 from test_serving_paths_gpu import wide
 
 pytestmark = pytest.mark.gpu
@@ -127,3 +127,29 @@ def test_a_wide_mask_of_a_very_long_sequence():
     v = hidet_b200.quantized_cache_read(cache, own, torch.float32)[1][:, 0]
     want = torch.stack([v[0], v[1], (v[0] + v[2]) / 2])[:, None].expand(3, heads, dim)
     assert (got[1][0].float() - want).abs().max() < 1e-2  # every other score is 300 below theirs
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [700, 32002, 200000])
+@pytest.mark.parametrize('repeat', [1, 70])
+def test_log_probs_of_rows_up_to_the_largest_number(dtype, vocab, repeat):
+    """A token that is forced by the type's largest number has all the probability, and the entropy is zero; with two of them it is log 2."""
+    most = torch.finfo(dtype).max
+    x = normal(6, vocab, seed=68, dtype=torch.float32, std=3.0).to(dtype)
+    x[0, vocab // 2] = most
+    x[1, [3, vocab - 1]] = most
+    x[2, 5] = most
+    x[2, 6:9] = torch.tensor([0.72, 0.5, 0.3], dtype=torch.float64, device='cuda').mul(most).to(dtype)
+    x[3] = -math.inf
+    x[3, [0, vocab - 2]] = most
+    x[4] = most
+    x[5, 1] = 0.6 * most
+    tokens = torch.full((6, 2), vocab - 1, device='cuda')
+    tokens[:, 1] = 5
+    for top in (0, 3, 32):
+        got = check_log_probs(x.repeat(repeat, 1), tokens.repeat(repeat, 1), top)
+        for at in range(0, 6 * repeat, 6):
+            entropy = got[1][at:at + 6].tolist()
+            # what is not at the largest number adds nothing: 16 bits hold it 16 apart from its neighbour
+            assert entropy[0] == entropy[2] == entropy[5] == 0.0 and entropy[1] == pytest.approx(math.log(2.0), abs=1e-6) and entropy[3] == pytest.approx(math.log(2.0), abs=1e-6)
+            assert entropy[4] == pytest.approx(math.log(vocab), abs=1e-5)
