@@ -5,8 +5,8 @@
 //     s_ij = scale * (q_i . kcode_j) * kscale_j,     o_i = sum_j exp(s_ij - m_i) * vscale_j * vcode_j / sum_j exp(s_ij - m_i)
 // over the positions that the row may see, with the running maximum m_i and sum of one pass over the cache.  Codes are exact in f16, so
 // the products q . kcode run on f16 tensor-core instructions with float sums; bf16 queries go through f16 too, scaled row by row by a power of
-// two (their eight bits fit; what is 2^-24 of the row's largest element is lost).  Probabilities, times vscale_j over the power of two below the largest vscale so far (so that
-// they cannot leave f16's range whatever the values' size), are rounded to f16 for the second product, an error of 2^-12 of each, at random; the sums
+// two (their eight bits fit; what is 2^-24 of the row's largest element is lost).  Probabilities, times vscale_j over the power of two below the largest vscale that the row has seen so far (so
+// that they cannot leave f16's range whatever the values' size), are rounded to f16 for the second product, an error of 2^-12 of each, at random; the sums
 // that divide are float.
 //
 // The work is in tiles of positions for one (sequence, key/value head, 8 * NT query rows).  The tiles of all sequences stand in
@@ -97,9 +97,15 @@ __device__ __forceinline__ void load_q4(const T *p, float (&f)[4]) {
     for (int i = 0; i < 4; ++i) f[i] = Elems<T>::one(v[i]);
 }
 
+// The reciprocal of a power of two.
+__device__ __forceinline__ float power_over(float power) { return __uint_as_float(0x7f000000u - __float_as_uint(power)); }
+
+// A row's maximum as long as it has seen nothing: finite, so that differences from it are numbers.  Hidden positions have -inf.
+constexpr float kNothing = -3.4028234663852886e38f;
+
 // The largest of the warps' maxima of a row.
 __device__ __forceinline__ float row_top(const Control &ctl, int r) {
-    float n = -INFINITY;
+    float n = kNothing;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) n = fmaxf(n, ctl.m[w][r]);
     return n;
@@ -117,7 +123,7 @@ __device__ __forceinline__ void finish_item(const AttentionArgs &p, Control &ctl
         const float top = row_top(ctl, r), scale = ctl.q_scale[r];
         float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) sum += ctl.m[w][r] == -INFINITY ? ctl.l[w][r] : ctl.l[w][r] * ex2((ctl.m[w][r] - top) * scale);
+        for (int w = 0; w < WARPS; ++w) sum += ctl.l[w][r] * ex2((ctl.m[w][r] - top) * scale);
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int k = 0; k < L::BUFFERS; ++k) {
@@ -246,8 +252,10 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
         if (item.rows < 0) break;
         const int length = item.length, hidden = first_hidden(p, item);
         float o[NT][D / 16][4];  // elements 16 i + g (0, 1) and + 8 (2, 3) of query rows 2t (0, 2) and 2t + 1 (1, 3)
-        float m[NT][2], l[NT][2], shift[NT][2], qs[NT][2], rise[NT][2];  // shift: m, or 0 as long as nothing was seen
-        float vref = 0.0f, v_inv = 0.0f, v_limit = kLeastNormal;  // a power of two, its reciprocal, and the first scale that is too large for it
+        float m[NT][2], l[NT][2], qs[NT][2], limit[NT][2];  // limit: a score beyond it is too large for m
+        // A row's values are counted in a power of two: its reciprocal, and the first scale that is too large for one of this thread's rows.  Each row has its own,
+        // since what one row sees may be larger by any factor than what another does.
+        float v_inv[NT][2], v_limit = 2.0f * kLeastNormal;
         uint2 q_reg[L::Q_IN_REGISTERS ? NT * D / 16 : 1];
         {
             // the queries, as MMA fragments: for chunk c and row g lane (g, t) has elements 16 c + 4t .. + 3
@@ -297,10 +305,11 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
                     for (int e = 0; e < 4; ++e) o[nt][n][e] = 0.0f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    m[nt][h] = -INFINITY;
-                    l[nt][h] = shift[nt][h] = 0.0f;
+                    m[nt][h] = kNothing;
+                    limit[nt][h] = -INFINITY;
+                    l[nt][h] = 0.0f;
                     qs[nt][h] = ctl.q_scale[8 * nt + 2 * t + h];
-                    rise[nt][h] = fminf(kRise / qs[nt][h], 1e38f);
+                    v_inv[nt][h] = power_over(kLeastNormal);
                 }
             }
             if (L::Q_IN_REGISTERS) {
@@ -363,38 +372,41 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
                     for (int h = 0; h < 2; ++h)
                         if (key0 + key_of_lane + 2 * h >= length) vs[h] = 0.0f;
                 }
-                const float v_top = fmaxf(vs[0], vs[1]);
-                bool up = v_top >= v_limit;
-                float top[NT][2];
+                bool up = false, v_up = fmaxf(vs[0], vs[1]) >= v_limit;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        top[nt][h] = fmaxf(s[nt][h], s[nt][2 + h]);
-                        up |= top[nt][h] > m[nt][h] + rise[nt][h];
-                    }
-                if (__any_sync(0xffffffffu, up)) {
-                    float v_new = v_top;
+                    for (int h = 0; h < 2; ++h) up |= fmaxf(s[nt][h], s[nt][2 + h]) > limit[nt][h];
+                // The largest scale that a row sees.
+                auto v_top = [&](int nt, int h) { return fmaxf(partly && s[nt][h] == -INFINITY ? 0.0f : vs[0], partly && s[nt][2 + h] == -INFINITY ? 0.0f : vs[1]); };
+                if (partly && v_up) {
+                    v_up = false;
 #pragma unroll
-                    for (int d = 4; d < 32; d *= 2) v_new = fmaxf(v_new, __shfl_xor_sync(0xffffffffu, v_new, d));
-                    v_new = fmaxf(v_new, vref);
-                    const uint32_t power = __float_as_uint(v_new) & 0x7f800000u;
-                    const float beta = power != 0 ? vref * __uint_as_float(0x7f000000u - power) : 1.0f;
-                    vref = __uint_as_float(power);
-                    v_inv = power != 0 ? __uint_as_float(0x7f000000u - power) : 0.0f;
-                    v_limit = power != 0 ? 2.0f * vref : kLeastNormal;
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) v_up |= v_top(nt, h) * v_inv[nt][h] >= 2.0f;
+                }
+                if (__any_sync(0xffffffffu, up || v_up)) {
+                    const bool higher = __any_sync(0xffffffffu, up);  // else a row's maximum stays, whoever's values are large
+                    v_limit = INFINITY;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float by[2];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            float n = top[nt][h];
+                            float n = higher ? fmaxf(s[nt][h], s[nt][2 + h]) : kNothing, v = v_top(nt, h);
 #pragma unroll
-                            for (int d = 4; d < 32; d *= 2) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, d));
+                            for (int d = 4; d < 32; d *= 2) {
+                                n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, d));
+                                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+                            }
                             n = fmaxf(n, m[nt][h]);
-                            const float alpha = n == -INFINITY ? 1.0f : ex2((m[nt][h] - n) * qs[nt][h]);
+                            const float v_ref = power_over(v_inv[nt][h]), v_new = __uint_as_float(__float_as_uint(fmaxf(v, v_ref)) & 0x7f800000u);
+                            v_inv[nt][h] = power_over(v_new);
+                            v_limit = fminf(v_limit, 2.0f * v_new);
+                            const float alpha = ex2((m[nt][h] - n) * qs[nt][h]), beta = v_ref * v_inv[nt][h];
                             m[nt][h] = n;
-                            shift[nt][h] = n == -INFINITY ? 0.0f : n;
+                            limit[nt][h] = n == kNothing ? -INFINITY : n + fminf(__fdividef(kRise, qs[nt][h]), 1e38f);
                             l[nt][h] *= alpha;
                             by[h] = alpha * beta;
                         }
@@ -404,16 +416,15 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
                             for (int e = 0; e < 4; ++e) o[nt][n][e] *= by[e & 1];
                     }
                 }
-                const float w[2] = {vs[0] * v_inv, vs[1] * v_inv};
                 uint32_t b[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float x[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        x[e] = ex2(fmaf(s[nt][e] - shift[nt][e & 1], qs[nt][e & 1], kBias));
+                        x[e] = ex2(fmaf(s[nt][e] - m[nt][e & 1], qs[nt][e & 1], kBias));
                         l[nt][e & 1] += x[e];
-                        x[e] *= w[e >> 1];
+                        x[e] *= vs[e >> 1] * v_inv[nt][e & 1];
                         if (partly && s[nt][e] == -INFINITY) x[e] = 0.0f;  // whatever the scale of a position that is not seen
                     }
                     b[nt][0] = transpose(pack_f16(x[0], x[1]));
@@ -460,7 +471,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) factor[nt][h] = m[nt][h] == -INFINITY ? vref : ex2((m[nt][h] - row_top(ctl, 8 * nt + 2 * t + h)) * qs[nt][h]) * vref;
+            for (int h = 0; h < 2; ++h) factor[nt][h] = ex2((m[nt][h] - row_top(ctl, 8 * nt + 2 * t + h)) * qs[nt][h]) * power_over(v_inv[nt][h]);
         float *mine = merge + (warp % L::BUFFERS) * (L::MERGE / 4) + 2 * t * L::PITCH + g;
         if (warp >= L::BUFFERS) {
 #pragma unroll

@@ -9,7 +9,7 @@
 //   two groups of four warps turn scores into probabilities, a thread a row, alternate tiles: each group has its own S, P, O, maxima and sums, which
 //       meet at the end of the item.
 // The probabilities go back into tensor memory, in the place of their scores, as the first operand of the second product.  A thread has a whole row of 64 scores, so maximum and sum
-// need no exchange.  A row's unit is 2^u: u is its running maximum (in log2) plus the exponent of the largest value scale so far, so that the products with
+// need no exchange.  A row's unit is 2^u: u is its running maximum (in log2) plus the exponent of the largest value scale that it has seen so far, so that the products with
 // value scales fit f16 and sums of probabilities and of values are in the same unit.
 //
 // Bound by the two softmax groups.  A tile takes one 3300 clocks, 1400 for the bound on its scores and 1900 for the probabilities, so 64 positions of 128 rows
@@ -415,7 +415,16 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                         }
                     }
                     const float4 k_tops = *reinterpret_cast<const float4 *>(ctl.k_top[buf]), v_tops = *reinterpret_cast<const float4 *>(ctl.v_top[buf]);
-                    const float k_top = max3(fmaxf(k_tops.x, k_tops.y), k_tops.z, k_tops.w), v_top = max3(fmaxf(v_tops.x, v_tops.y), v_tops.z, v_tops.w);
+                    const float k_top = max3(fmaxf(k_tops.x, k_tops.y), k_tops.z, k_tops.w);
+                    float v_top = max3(fmaxf(v_tops.x, v_tops.y), v_tops.z, v_tops.w);
+                    if (partly && v_top >= v_limit) {  // only what this row sees counts: it may be smaller by any factor
+                        v_top = 0.0f;
+                        if (seen != 0) {
+#pragma unroll 1
+                            for (uint32_t j = 0; j < TILE; ++j)
+                                if (seen >> ((j & 32) + position_of32(j & 31)) & 1u) v_top = fmaxf(v_top, ctl.v_scale[buf][j]);
+                        }
+                    }
                     bool raised = false;
                     if (__any_sync(0xffffffffu, fmaxf(top, other) * k_top > m + rise)) {
                         top = other = -INFINITY;

@@ -7,7 +7,7 @@ import torch
 
 import hidet_b200
 from hidet_b200 import ffi
-from test_serving_gpu import TYPES, a_cache, check_log_probs, clean_status, normal  # noqa: F401
+from test_serving_gpu import TYPES, a_cache, check_attention, check_log_probs, clean_status, normal, slots_in  # noqa: F401
 from test_serving_paths_gpu import wide
 
 pytestmark = pytest.mark.gpu
@@ -153,3 +153,33 @@ def test_log_probs_of_rows_up_to_the_largest_number(dtype, vocab, repeat):
             # what is not at the largest number adds nothing: 16 bits hold it 16 apart from its neighbour
             assert entropy[0] == entropy[2] == entropy[5] == 0.0 and entropy[1] == pytest.approx(math.log(2.0), abs=1e-6) and entropy[3] == pytest.approx(math.log(2.0), abs=1e-6)
             assert entropy[4] == pytest.approx(math.log(vocab), abs=1e-5)
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('heads,kv_heads,dim,tokens,long', FORMS[1:] + [(8, 2, 256, (3, 2), False)])
+@pytest.mark.parametrize('size', [1e3, 1e9, 1e20])
+@pytest.mark.parametrize('masked', [False, True])
+def test_large_values_that_a_row_does_not_see_do_not_matter(dtype, heads, kv_heads, dim, tokens, long, size, masked):
+    """The last token's value is larger than the others'.  It alone sees it; its neighbours' results stay, to the bit."""
+    lengths = [700, 41]
+    cache, table = a_cache(lengths, kv_heads, dim, 16)
+    if long:
+        cache, table = wide((cache, table))
+    q, starts, n = normal(sum(tokens), heads, dim, seed=69, dtype=dtype), ints(0, tokens[0], sum(tokens)), ints(*lengths)
+    mask = torch.zeros((sum(tokens), max(tokens)), dtype=torch.bool, device='cuda')
+    for b, t in enumerate(tokens):
+        mask[sum(tokens[:b]):sum(tokens[:b + 1]), :t] = torch.tril(torch.ones((t, t), dtype=torch.bool, device='cuda'))
+    mask = mask if masked else None
+    want = hidet_b200.quantized_cache_attention(q, cache, table, n, starts=starts, mask=mask, return_lse=True)
+    for b, t in enumerate(tokens):
+        last = slots_in(table, b, lengths[b], 16)[-1:]
+        k, v = hidet_b200.quantized_cache_read(cache, last, torch.float32)
+        hidet_b200.quantized_cache_append(cache, k, v * size, last)
+    got = hidet_b200.quantized_cache_attention(q, cache, table, n, starts=starts, mask=mask, return_lse=True)
+    first = 0
+    for t in tokens:
+        rows = slice(first, first + t - 1)
+        assert torch.equal(got[0][rows], want[0][rows]) and torch.equal(got[1][rows], want[1][rows])
+        first += t
+    if size < 1e4 or dtype == torch.bfloat16:  # else the last token's results are beyond the type
+        check_attention(lengths, list(tokens), heads, kv_heads, dim, 16, dtype, mask=mask, cache=(cache, table), q=q)
