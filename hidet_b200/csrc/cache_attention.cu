@@ -543,7 +543,7 @@ B200Q_API size_t b200q_quantized_cache_attention_workspace_bytes(int64_t batch, 
     if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || !cache_dim(head_dim)) return 0;
     const int64_t few = (int64_t)2 * kMaxCtas * 16 * (head_dim + 2) * 4;
     const int64_t many = may_be_wide(tokens, heads / kv_heads, batch, head_dim) ? (int64_t)2 * kMostWideCtas * 128 * (head_dim + 2) * 4 + kMostWideCtas * 64 : 0;  // 64: an item's description
-    return (size_t)(kCounterBytes + (few > many ? few : many));
+    return kWorkspaceHead + (size_t)(few > many ? few : many);
 }
 
 B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, float *lse, const void *cache, int64_t pages, int64_t page_size, const int32_t *page_table,
@@ -602,7 +602,7 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
     p.by_group = divisor_of((uint32_t)p.group);
     p.scale_log2 = scale * kLog2e;
     p.counters = static_cast<unsigned int *>(workspace);
-    p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kCounterBytes);
+    p.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kWorkspaceHead);
     p.partial_floats = (int64_t)2 * kMostWideCtas * 128 * (head_dim + 2);  // of the kernel for many rows
     p.status = device_status_word();
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -13,7 +13,6 @@ namespace cache_attention {
 
 constexpr int kMaxCtas = 3 * 148;         // of a launch; the workspace is made for them
 constexpr int kMostWideCtas = 148;        // of the kernel for many rows
-constexpr int kCounterBytes = 65536 * 4;  // arrival counters in front of the workspace, zero between calls: kMaxCtas a round of additions
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are kept 2^6 times as large, and a row's maximum is raised when a score passes it by 2^8 (rarely, behind its first
@@ -24,6 +23,8 @@ constexpr float kLeastNormal = 1.1754943508222875e-38f;
 
 constexpr int RECORDS = 4;     // of a tile
 constexpr int FAN = 8;         // pieces of an item that are added at once
+// Three rounds of additions, each with a counter for every CTA in the workspace's head.
+static_assert(FAN * FAN * FAN >= kMaxCtas && 3 * kMaxCtas <= kWorkspaceCounters, "");
 
 struct AttentionArgs : PlanArgs {
     const void *q;

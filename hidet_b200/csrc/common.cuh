@@ -49,6 +49,11 @@ constexpr unsigned int kKernelUnaligned = 4;
 constexpr unsigned int kKernelPair = 5;
 constexpr unsigned int kKernelMid = 6;
 
+// A stream has one workspace, and kernels of different kinds take turns at it.  Its head holds the arrival counters of all that have any, zero between
+// calls; partial sums lie behind it in every kernel.
+constexpr int64_t kWorkspaceCounters = 65536;
+constexpr size_t kWorkspaceHead = (size_t)kWorkspaceCounters * 4;
+
 // Number of SMs of the current device (cached per device).
 int sm_count();
 

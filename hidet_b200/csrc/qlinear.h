@@ -84,8 +84,7 @@ int check_large_outputs(const OutTargets &out);
 
 // The one-SM tensor-memory kernel for large M ([K, N] weights), which serves the multicast delivery.
 // How it splits K (narrow problems only) and the scratch that takes: fp32 partial sums
-// [k_splits][M][N] behind an untouched head of kSplitWorkspaceHead bytes (the small-M kernel's counters live there).
-constexpr size_t kSplitWorkspaceHead = (size_t)65536 * 4;
+// [k_splits][M][N] behind an untouched kWorkspaceHead.
 struct PrefillSplit {
     int k_splits = 1;
     int kb_per_split = 0;

@@ -57,7 +57,6 @@ struct Config {
     static constexpr int SMEM_BYTES = NEED < 46 * 1024 + 512 ? 46 * 1024 + 512 : NEED;
     static_assert(CONSUMER_WARPS * ROWS * STAGING_ROW * 4 <= STAGES * W_STAGE_BYTES, "the staging blocks reuse the weight ring");
 };
-constexpr int64_t kMaxCounters = 65536;      // arrival counters at the head of the workspace
 constexpr int kPortableCluster = 8;          // what every device runs; beyond it the occupancy query has the last word
 constexpr int kMaxCluster = 16;              // largest cluster of the plan
 // Columns of a tile that each CTA of a cluster owns, and whether a rank's slices from all of them have their place in the receive buffer (not
@@ -721,11 +720,11 @@ DecodePlan plan_decode_portable(int64_t M, int64_t N, int64_t K) {
         if (splits > k_iters / 8) splits = k_iters / 8;
         if (splits > 64) splits = 64;
         groups = (int)(splits / c);
-        if (groups < 1 || tiles * c > kMaxCounters) groups = 1;
+        if (groups < 1 || tiles * c > kWorkspaceCounters) groups = 1;
     }
     // The counter region has one fixed size, so that counters never land on bytes an earlier call of
     // another shape used for partial sums: the region stays all-zero between calls.
-    pl.counter_bytes = groups > 1 ? (size_t)kMaxCounters * 4 : 0;
+    pl.counter_bytes = groups > 1 ? kWorkspaceHead : 0;
     pl.partial_bytes = groups > 1 ? (size_t)groups * M * N * 4 : 0;
     pl.cluster = c;
     pl.groups = groups;

@@ -492,7 +492,7 @@ PrefillSplit plan_prefill_split(int64_t M, int64_t N, int64_t K) {
     ps.kb_per_split = (int)ceil_div(k_blocks, splits);
     ps.k_splits = (int)ceil_div(k_blocks, ps.kb_per_split);
     if (ps.k_splits < 2) return PrefillSplit();
-    ps.workspace_bytes = kSplitWorkspaceHead + (size_t)ps.k_splits * M * N * sizeof(float);
+    ps.workspace_bytes = kWorkspaceHead + (size_t)ps.k_splits * M * N * sizeof(float);
     return ps;
 }
 
@@ -520,7 +520,7 @@ static int launch_prefill_tm(const void *a, const void *wq, const void *scale, c
     p.m_tiles = (int)ceil_div(M, TM);
     p.k_splits = split.k_splits;
     p.kb_per_split = split.k_splits > 1 ? split.kb_per_split : (int)ceil_div(K, BK);
-    p.partial = split.k_splits > 1 ? reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kSplitWorkspaceHead) : nullptr;
+    p.partial = split.k_splits > 1 ? reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kWorkspaceHead) : nullptr;
     const int64_t total = (int64_t)p.n_tiles * p.m_tiles * p.k_splits;
     if (total > 2147483647LL) return set_error(B200Q_UNSUPPORTED, "qlinear: problem too large for the tile counter");
     const unsigned grid = (unsigned)(total < sms ? total : sms);

@@ -27,10 +27,6 @@ constexpr int COLS_PER_THREAD = 8;   // one 32-bit word of packed codes
 constexpr int WORDS_X = 32;          // threads along N: a warp covers 256 columns
 constexpr int K_SLICES = 8;          // warps of a CTA, each on its own k rows
 constexpr int THREADS = WORDS_X * K_SLICES;
-// The head of a workspace is where the int8 kernels keep their arrival counters (all-zero between calls); this op
-// leaves it alone, so one workspace can serve both.
-constexpr size_t kReservedHead = (size_t)65536 * 4;
-
 struct Params {
     const __half *a;        // [M, K]
     const uint32_t *q;      // [K, N / 8] words
@@ -494,8 +490,8 @@ Plan plan(int64_t M, int64_t N, int64_t K, int64_t G) {
 // Scratch a call asks for.  The tensor-core kernel has no use for any: its group sizes are held to what the shared head
 // takes, whatever the problem, and a call without a workspace is refused for every group size alike.
 size_t workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t G) {
-    if (G % 16 == 0) return kReservedHead + 256;
-    return kReservedHead + (size_t)plan(M, N, K, G).splits * M * N * sizeof(float);
+    if (G % 16 == 0) return kWorkspaceHead + 256;
+    return kWorkspaceHead + (size_t)plan(M, N, K, G).splits * M * N * sizeof(float);
 }
 
 }  // namespace u4
@@ -559,7 +555,7 @@ B200Q_API int b200q_qlinear_f16_u4(const void *a, const void *q, const void *sca
     }
     u4::Plan pl = u4::plan(M, N, K, group_size);
     // Operands the tensor-core kernel cannot take (an unaligned a or c) with its amount of scratch: one split.
-    const bool direct = workspace_bytes < u4::kReservedHead + (size_t)pl.splits * M * N * sizeof(float);
+    const bool direct = workspace_bytes < kWorkspaceHead + (size_t)pl.splits * M * N * sizeof(float);
     if (direct) pl = {1, (int)K};
     u4::Params p;
     p.direct = direct ? static_cast<__half *>(c) : nullptr;
@@ -567,7 +563,7 @@ B200Q_API int b200q_qlinear_f16_u4(const void *a, const void *q, const void *sca
     p.q = static_cast<const uint32_t *>(q);
     p.scale = static_cast<const __half *>(scale);
     p.zeros = static_cast<const __half *>(zeros);
-    p.partial = reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + u4::kReservedHead);
+    p.partial = reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kWorkspaceHead);
     p.M = (int)M;
     p.N = (int)N;
     p.K = (int)K;

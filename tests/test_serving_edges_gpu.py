@@ -7,6 +7,7 @@ import torch
 
 import hidet_b200
 from hidet_b200 import ffi
+from hidet_b200.runtime import workspaces
 from test_serving_gpu import TYPES, a_cache, check_attention, check_log_probs, clean_status, normal, slots_in  # noqa: F401
 from test_serving_paths_gpu import wide
 
@@ -183,3 +184,40 @@ def test_large_values_that_a_row_does_not_see_do_not_matter(dtype, heads, kv_hea
         first += t
     if size < 1e4 or dtype == torch.bfloat16:  # else the last token's results are beyond the type
         check_attention(lengths, list(tokens), heads, kv_heads, dim, 16, dtype, mask=mask, cache=(cache, table), q=q)
+
+
+@pytest.mark.parametrize('heads,kv_heads,dim,tokens,long', FORMS)
+def test_the_workspace_is_shared_with_the_linears(heads, kv_heads, dim, tokens, long):
+    """Attention in many pieces and linears that meet in the workspace take turns at it, and its counters are zero in between."""
+    lengths = [30000, 9000]
+    cache, table = a_cache(lengths, kv_heads, dim, 64)
+    if long:
+        cache, table = wide((cache, table))
+    q, starts, n = normal(sum(tokens), heads, dim, seed=70), ints(0, tokens[0], sum(tokens)), ints(*lengths)
+    a, w = normal(2, 65536, seed=71), torch.randint(-128, 128, (65536, 128), dtype=torch.int8, device='cuda', generator=torch.Generator('cuda').manual_seed(72))
+    scale = torch.full((128,), 1e-4, dtype=torch.float16, device='cuda')
+    stream = torch.cuda.current_stream().cuda_stream
+    first = None
+    for _ in range(3):
+        got = [hidet_b200.quantized_cache_attention(q, cache, table, n, starts=starts)]
+        buffer = workspaces._buffers[(torch.cuda.current_device(), stream)]
+        assert not buffer[:65536 * 4].any() and buffer[65536 * 4:].any()
+        got.append(hidet_b200.symmetric_quant_matmul(a, w, scale))
+        assert not workspaces._buffers[(torch.cuda.current_device(), stream)][:65536 * 4].any()
+        first = first or got
+        assert all(torch.equal(x, y) for x, y in zip(first, got))
+    want = (a.double() @ w.double()) * scale.double()
+    assert (first[1].double() - want).abs().max() <= (2.0 ** -11 + 2.0 ** -14) * want.abs().max()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [6000, 28772])
+@pytest.mark.parametrize('repeat', [1, 30])
+def test_log_probs_when_few_of_the_threads_have_all_the_large_ones(dtype, vocab, repeat):
+    """Lists that overflow by vectors, by elements and not at all, of parts with 256 threads that take 16 bytes each in turn."""
+    each, threads = 16 // dtype.itemsize, [0, 1, 16, 20, 40, 80, 200]
+    at = torch.arange(vocab, device='cuda')
+    rows = torch.stack([normal(vocab, seed=73 + i, dtype=torch.float32) + 60.0 * ((at // each) % 256 < n) for i, n in enumerate(threads)]).to(dtype)
+    tokens = torch.arange(len(threads), device='cuda')
+    for top in (1, 32):
+        check_log_probs(rows.repeat(repeat, 1), tokens.repeat(repeat), top)
