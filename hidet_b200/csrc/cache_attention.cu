@@ -212,11 +212,10 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
         item.rows = -1;
         if (!dead) publish(item);
         write_unowned<D>(p, line.placed, lane);
-        if (dead) {  // nothing may be on its way when the CTA ends
-            for (int back = 1; back <= STAGES && back <= it; ++back) {
-                const int at = it - back;
-                mbar_wait(smem_u32(&ctl.full[at % STAGES]), (at / STAGES) & 1, 1u << 16);
-            }
+        // Nothing may be on its way when the CTA ends, whoever's wait has run out.
+        for (int back = 1; back <= STAGES && back <= it; ++back) {
+            const int at = it - back;
+            mbar_wait(smem_u32(&ctl.full[at % STAGES]), (at / STAGES) & 1, 1u << 16);
         }
         return;
     }

@@ -178,11 +178,10 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
         }
         __syncwarp();
         write_unowned<D>(p, line.placed, lane);
-        if (!ok) {  // nothing may be on its way when the CTA ends
-            for (int back = 1; back <= RAW_STAGES && back <= it; ++back) {
-                const int at = it - back;
-                mbar_wait(smem_u32(&ctl.raw_full[at % RAW_STAGES]), (at / RAW_STAGES) & 1, 1u << 16);
-            }
+        // Nothing may be on its way when the CTA ends, whoever's wait has run out.  (Where the end was told, a stage was empty for that.)
+        for (int back = 1; back <= RAW_STAGES - (ok ? 1 : 0) && back <= it; ++back) {
+            const int at = it - back;
+            mbar_wait(smem_u32(&ctl.raw_full[at % RAW_STAGES]), (at / RAW_STAGES) & 1, 1u << 16);
         }
     } else if (warp == MMA_WARP) {
         // ---------------- products ----------------
