@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
         float m[NT][2], l[NT][2], qs[NT][2], limit[NT][2];  // limit: a score beyond it is too large for m
         // A row's values are counted in a power of two: its reciprocal, and the first scale that is too large for one of this thread's rows.  Each row has its own,
         // since what one row sees may be larger by any factor than what another does.
-        float v_inv[NT][2], v_limit = 2.0f * kLeastNormal;
+        float v_inv[NT][2], v_limit = INFINITY;
         uint2 q_reg[L::Q_IN_REGISTERS ? NT * D / 16 : 1];
         {
             // the queries, as MMA fragments: for chunk c and row g lane (g, t) has elements 16 c + 4t .. + 3
@@ -371,41 +371,35 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
                     for (int h = 0; h < 2; ++h)
                         if (key0 + key_of_lane + 2 * h >= length) vs[h] = 0.0f;
                 }
-                bool up = false, v_up = fmaxf(vs[0], vs[1]) >= v_limit;
+                bool up = fmaxf(vs[0], vs[1]) >= v_limit;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) up |= fmaxf(s[nt][h], s[nt][2 + h]) > limit[nt][h];
-                // The largest scale that a row sees.
-                auto v_top = [&](int nt, int h) { return fmaxf(partly && s[nt][h] == -INFINITY ? 0.0f : vs[0], partly && s[nt][2 + h] == -INFINITY ? 0.0f : vs[1]); };
-                if (partly && v_up) {
-                    v_up = false;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) v_up |= v_top(nt, h) * v_inv[nt][h] >= 2.0f;
-                }
-                if (__any_sync(0xffffffffu, up || v_up)) {
-                    const bool higher = __any_sync(0xffffffffu, up);  // else a row's maximum stays, whoever's values are large
+                if (__any_sync(0xffffffffu, up)) {  // then each row by what it sees itself, whatever the others do
                     v_limit = INFINITY;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float by[2];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            float n = higher ? fmaxf(s[nt][h], s[nt][2 + h]) : kNothing, v = v_top(nt, h);
+                            float n = fmaxf(s[nt][h], s[nt][2 + h]), v = fmaxf(s[nt][h] == -INFINITY ? 0.0f : vs[0], s[nt][2 + h] == -INFINITY ? 0.0f : vs[1]);
 #pragma unroll
                             for (int d = 4; d < 32; d *= 2) {
                                 n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, d));
                                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
                             }
-                            n = fmaxf(n, m[nt][h]);
-                            const float v_ref = power_over(v_inv[nt][h]), v_new = __uint_as_float(__float_as_uint(fmaxf(v, v_ref)) & 0x7f800000u);
+                            float alpha = 1.0f;
+                            if (n > limit[nt][h]) {
+                                alpha = ex2((m[nt][h] - n) * qs[nt][h]);
+                                m[nt][h] = n;
+                                float rise;
+                                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rise) : "f"(qs[nt][h]));
+                                limit[nt][h] = n + fminf(kRise * rise, 1e38f);
+                            }
+                            const float v_ref = power_over(v_inv[nt][h]), v_new = __uint_as_float(__float_as_uint(fmaxf(v, v_ref)) & 0x7f800000u), beta = v_ref * power_over(v_new);
                             v_inv[nt][h] = power_over(v_new);
-                            v_limit = fminf(v_limit, 2.0f * v_new);
-                            const float alpha = ex2((m[nt][h] - n) * qs[nt][h]), beta = v_ref * v_inv[nt][h];
-                            m[nt][h] = n;
-                            limit[nt][h] = n == kNothing ? -INFINITY : n + fminf(__fdividef(kRise, qs[nt][h]), 1e38f);
+                            if (m[nt][h] > kNothing) v_limit = fminf(v_limit, 2.0f * v_new);  // else its first position will pass the other limit
                             l[nt][h] *= alpha;
                             by[h] = alpha * beta;
                         }
@@ -414,6 +408,7 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
 #pragma unroll
                             for (int e = 0; e < 4; ++e) o[nt][n][e] *= by[e & 1];
                     }
+                    __syncwarp();
                 }
                 uint32_t b[NT][2];
 #pragma unroll

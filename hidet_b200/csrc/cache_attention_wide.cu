@@ -72,6 +72,29 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // Four scales, read where this stands: ahead of their use they would take as many registers as the scores.
 __device__ __forceinline__ void scales_at(uint32_t addr, f32x2 &a, f32x2 &b) { asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr)); }
 
+// The largest value scale of what a row sees of a tile (the others may be larger by any factor), or another with its exponent: records that it sees entirely by their
+// largest, and others only if one in them would change the exponent.  Seldom called, and what it costs is the way of its instructions into the caches: a function of its
+// own adds 0 to 3 % to calls with a few tiles a CTA (inline 1 to 6, as loops that stay loops 1 to 6, with a load for each position 44).
+__device__ __noinline__ float seen_v_top(const float *scales, const float *tops, uint64_t seen, float v_limit) {
+    const float4 of = *reinterpret_cast<const float4 *>(tops);
+    auto bits = [&](int w) { return (uint32_t)(seen >> (16 * w)) & 0xffffu; };
+    float top = fmaxf(fmaxf(bits(0) == 0xffffu ? of.x : 0.0f, bits(1) == 0xffffu ? of.y : 0.0f), fmaxf(bits(2) == 0xffffu ? of.z : 0.0f, bits(3) == 0xffffu ? of.w : 0.0f));
+    const float enough = fmaxf(v_limit, __uint_as_float((__float_as_uint(top) & 0x7f800000u) + 0x00800000u));
+    if (seen == 0 || fmaxf(fmaxf(of.x, of.y), fmaxf(of.z, of.w)) < enough) return top;
+#pragma unroll 1
+    for (int w = 0; w < RECORDS; ++w) {
+        const uint32_t own = bits(w);
+        if (own == 0 || tops[w] < enough) continue;
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(scales + 16 * w + j);
+            top = fmaxf(top, fmaxf(fmaxf(own >> position_of(j) & 1u ? v.x : 0.0f, own >> position_of(j + 1) & 1u ? v.y : 0.0f),
+                                   fmaxf(own >> position_of(j + 2) & 1u ? v.z : 0.0f, own >> position_of(j + 3) & 1u ? v.w : 0.0f)));
+        }
+    }
+    return top;
+}
+
 struct Control {
     uint64_t raw_full[RAW_STAGES], raw_empty[RAW_STAGES], kv_full[KV_STAGES], kv_empty[KV_STAGES], item_full[ITEMS], item_empty[ITEMS];
     uint64_t q_full, s_full[2][2], p_full[2][2], pv_done[2], item_done, drained;  // [group][buffer]
@@ -364,7 +387,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
             }
             const float rise = fminf(kRise / qs, 1e38f);
             float m = -INFINITY, shift = 0.0f, sum = 0.0f;  // shift: m, or 0 as long as nothing was seen
-            float exponent = 0.0f, v_limit = kLeastNormal;  // of the value scales, and the first scale that is too large for it
+            // Of the value scales that the row has seen, and the first scale that is too large for it (none as long as it has seen nothing: its first score raises the maximum).
+            float exponent = 0.0f, v_limit = INFINITY;
 
             for (int i = grp; i < item.tiles; i += 2) {
                 const int buf = (kv + i) % KV_STAGES, key0 = (item.tile0 + i) * TILE;
@@ -416,14 +440,6 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                     const float4 k_tops = *reinterpret_cast<const float4 *>(ctl.k_top[buf]), v_tops = *reinterpret_cast<const float4 *>(ctl.v_top[buf]);
                     const float k_top = max3(fmaxf(k_tops.x, k_tops.y), k_tops.z, k_tops.w);
                     float v_top = max3(fmaxf(v_tops.x, v_tops.y), v_tops.z, v_tops.w);
-                    if (partly && v_top >= v_limit) {  // only what this row sees counts: it may be smaller by any factor
-                        v_top = 0.0f;
-                        if (seen != 0) {
-#pragma unroll 1
-                            for (uint32_t j = 0; j < TILE; ++j)
-                                if (seen >> ((j & 32) + position_of32(j & 31)) & 1u) v_top = fmaxf(v_top, ctl.v_scale[buf][j]);
-                        }
-                    }
                     bool raised = false;
                     if (__any_sync(0xffffffffu, fmaxf(top, other) * k_top > m + rise)) {
                         top = other = -INFINITY;
@@ -448,10 +464,13 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                     if (!__any_sync(0xffffffffu, raised)) top = m;
                     if (__any_sync(0xffffffffu, raised || v_top >= v_limit)) {
                         const float was = exponent;
+                        if (v_limit == INFINITY && seen != 0) v_limit = kLeastNormal;
+                        if (partly) v_top = seen_v_top(ctl.v_scale[buf], ctl.v_top[buf], seen, v_limit);
                         if (v_top >= v_limit) {
                             exponent = fmaxf((float)((int)(__float_as_uint(v_top) >> 23) - 127), kLeastUnit);
                             v_limit = __uint_as_float((uint32_t)((int)exponent + 128) << 23);
                         }
+                        __syncwarp();
                         const float higher = fmaxf(m, top);
                         // in two steps: with value scales of very unlike sizes the whole may leave float's range where its product with the sum does not
                         const float by = higher == -INFINITY ? 1.0f : ex2(0.5f * ((m - higher) * qs + (was - exponent)));
