@@ -122,6 +122,8 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
         if len(out) != 2 or len(results) != len(given) or any(
                 y.shape != x.shape or y.dtype != x.dtype or y.device != x.device or (y.stride(-1) != 1 and dim > 1) for x, y in zip(given, results)):
             raise ValueError('out must be a pair of tensors like q and k with neighbouring elements')
+        if any(stride == 0 and n > 1 for y in results for stride, n in zip(y.stride(), y.shape)):
+            raise ValueError('out has elements that share their memory')
     targets = [heads_of(y, 'out', lead, dim)[0] for y in results]
     if any(t.untyped_storage().data_ptr() != y.untyped_storage().data_ptr() for t, y in zip(targets, results)):
         raise ValueError('the token dimensions of out cannot be viewed as one')

@@ -221,3 +221,14 @@ def test_log_probs_when_few_of_the_threads_have_all_the_large_ones(dtype, vocab,
     tokens = torch.arange(len(threads), device='cuda')
     for top in (1, 32):
         check_log_probs(rows.repeat(repeat, 1), tokens.repeat(repeat), top)
+
+
+def test_rotary_into_elements_that_share_their_memory_is_refused():
+    table, at = hidet_b200.rotary_table(16, 64), torch.arange(3, device='cuda')
+    q = normal(3, 2, 64, seed=80)
+    for out in (torch.empty_like(q)[:1].expand(3, 2, 64), torch.empty_like(q)[:, :1].expand(3, 2, 64)):
+        with pytest.raises(ValueError, match='share'):
+            hidet_b200.rotary_embedding(q, None, at, table, out=(out, None))
+    whole = torch.empty((5, 2, 64), dtype=q.dtype, device='cuda')
+    got = hidet_b200.rotary_embedding(q[:1], None, at[:1], table, out=(whole[:1, :1].expand(1, 1, 64).expand(1, 2, 64)[:, :1].as_strided((1, 2, 64), (0, 64, 1)), None))
+    assert torch.equal(got[0], hidet_b200.rotary_embedding(q[:1], None, at[:1], table)[0])  # one token: its stride does not matter
