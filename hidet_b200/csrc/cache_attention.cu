@@ -9,6 +9,8 @@
 // that they cannot leave f16's range whatever the values' size), are rounded to f16 for the second product, an error of 2^-12 of each, at random; the sums
 // that divide are float.
 //
+// A row's maximum follows its scores only where one passes it by 2^8, an idea published with recent attention kernels: between such steps nothing is rescaled.
+//
 // The work is in tiles of positions for one (sequence, key/value head, 8 * NT query rows).  The tiles of all sequences stand in
 // one line, with a gap in front of every item for what that costs besides where pieces are long, and the line is cut into equal pieces, one a CTA, whatever the sequences' lengths are (the host does not know them: they
 // are on the device, so that a captured step can be replayed as they grow).  A CTA's piece may end one item and begin others; items in
@@ -20,8 +22,8 @@
 // (and not the rows) shared out among the warps, each code is converted once per CTA.
 //
 // Bound by the cache's bytes where sequences are long: pieces stream at 5.9 TB/s, and 8 us are the launch, the plan, the first tile and the additions.  Measured with
-// 128 elements a head, 64 heads over 8: 32 sequences of 90 to 8000 positions 58 us, one of 131071 58 us, 4.7 TB/s each.  Where they are short it is
-// latency: 5.25 us for one tile, 7.6 for two pieces and their sum, 10.6 for 577 positions of 32 heads.  (Code that the instruction caches hold already, by an
+// 128 elements a head, 64 heads over 8: 32 sequences of 90 to 8000 positions 58 us, one of 131071 57 us, 4.7 TB/s each.  Where they are short it is
+// latency: 5.0 us for one tile, 7.0 for two pieces and their sum, 10.4 for 577 positions of 32 heads.  (Code that the instruction caches hold already, by an
 // item without rows in front, and all of the queries' loads on their way at once change nothing there.)
 #include <atomic>
 
@@ -511,8 +513,8 @@ int launch_sized(AttentionArgs p, cudaStream_t stream) {
 
 // Items of 8 query rows, and of 16 where more than 8 share a key/value head and there is much work: these read the cache once for twice the rows, but a tile, an item's ends
 // and the additions take them half as long again, and fewer fit an SM.  Measured (8 / 16 rows, us; tiles as in is_wide): 1 sequence of 512 positions, 8 heads of
-// 128, 16 rows (72 tiles) 9.2 / 13.0; of 16384 (2056) 21.9 / 30.0; 16 of 4096 (8320) 50.1 / 53.5; 24 of 4000 (12192) 68.1 / 69.2, with 64 elements 48.9 / 41.9, 96: 61.8 / 55.5,
-// 192: 99.4 / 85.8, 256: 138 / 122; 1 of 131071 (16392) 92 / 86.
+// 128, 16 rows (72 tiles) 9.2 / 12.7; of 16384 (2056) 21.7 / 28.9; 16 of 4096 (8320) 49.7 / 51.5; 24 of 4000 (12288) 67.3 / 66.3, with 64 elements 49.2 / 41.4, 96: 60.9 / 55.7,
+// 192: 99.5 / 86.4, 256: 138 / 125; 1 of 131071 (16392) 92 / 83.
 template <typename T>
 int launch_typed(const AttentionArgs &p, int dim, cudaStream_t stream) {
     const bool sixteen = p.batch > 0 && p.tokens * p.group > 8 * (int64_t)p.batch && tiles_of_16(p) > 10000;

@@ -51,8 +51,9 @@ inline bool may_be_wide(int64_t tokens, int64_t group, int64_t batch, int64_t di
 // Tiles of 64 positions and 16 rows, by what the page table could hold.
 inline int64_t tiles_of_16(const AttentionArgs &p) { return p.batch * (int64_t)p.kv_heads * (p.capacity / TILE + 1) * ((p.tokens * p.group / p.batch + 15) / 16); }  // batch > 0
 // It takes the calls with more than 4200 of them; its fixed costs are 6 us higher.  Measured
-// (few / many rows, us) with 8 key/value heads of 128 elements: 1 sequence of 4096 positions, 96 rows (3120 tiles) 24.8 / 39.3; 4 of 4096, 32 rows (4160) 29.5 / 34.3;
-// 16 of 600, 48 rows (4224) 31.5 / 26.5; 16 of 300, 96 rows (4608) 35.6 / 24.6; 4 of 4096, 64 rows (8320) 48 / 35; 8 of 8000, 48 rows (24192) 128 / 78.
+// (few / many rows, us) with 8 key/value heads of 128 elements, pages of 64: 1 sequence of 4096 positions, 96 rows (3120 tiles) 24.2 / 40.1; 4 of 4096, 32 rows (4160) 28.9 / 33.3;
+// 16 of 600, 48 rows (4224) 31.0 / 27.3; 16 of 300, 96 rows (4608) 34.9 / 24.6; 4 of 4096, 64 rows (8320) 47.4 / 34.1; 8 of 8000, 48 rows (24192) 107 / 76.5.  It is wrong for
+// some calls of few rows: 8 of 4096, 24 rows (8320) 39.0 / 46.0.
 inline bool is_wide(const AttentionArgs &p, int64_t dim) { return p.batch > 0 && may_be_wide(p.tokens, p.group, p.batch, dim) && tiles_of_16(p) > 4200; }
 int launch_wide(const AttentionArgs &p, int dim, bool bf16, cudaStream_t stream);
 

@@ -12,14 +12,14 @@
 // need no exchange.  A row's unit is 2^u: u is its running maximum (in log2) plus the exponent of the largest value scale that it has seen so far, so that the products with
 // value scales fit f16 and sums of probabilities and of values are in the same unit.
 //
-// Bound by the two softmax groups.  A tile takes one 3300 clocks, 1400 for the bound on its scores and 1900 for the probabilities, so 64 positions of 128 rows
-// pass every 1650, in which the tensor cores work for 256 (15 % of the time by the counters); the groups issue in 37 % of the slots and wait for tensor
-// memory, for scales (four bytes a clock, whoever asks for them) and for instructions.  The codes' conversion, 900 clocks a tile, keeps out of the way.
-// An item has about 8000 clocks that no tile hides: its queries, its first scores, the last product and the result.
+// Bound by the two softmax groups.  A tile takes one 3400 clocks, 600 for the bound on its scores and 2800 for the probabilities (an item's first, whose maximum is
+// looked for, 1800 and 2000), so 64 positions of 128 rows pass every 1700, in which the tensor cores work for 256 (15 % of the time by the counters); the groups
+// issue in 37 % of the slots and wait for tensor memory, for scales (four bytes a clock, whoever asks for them) and for instructions.  The codes' conversion, 950
+// clocks a tile, keeps out of the way.  An item has about 8000 clocks that no tile hides: its queries, its first scores, the last product and the result.
 //
-// Measured with 128 elements a head, f16 (and in the kernel for few rows), us: 8 sequences of 4096 positions, 64 rows, 64 heads over 8: 142 (523), 483 TFLOP/s counting
-// all positions; 8 of 820 to 4096, 64 rows, 32 over 8: 59 (197); 16 of 600, 48 rows, 32 over 8: 41 (96); 50 of 90, 11 rows, 128 over 32, where it is the
-// items' cost above all: 77 (146).
+// Measured with 128 elements a head, f16 (and in the kernel for few rows), us: 8 sequences of 4096 positions, 64 tokens, 64 heads over 8: 142 (524), 484 TFLOP/s counting
+// all positions; 8 of 820 to 4096, 64 tokens, 32 over 8: 59 (190); 16 of 600, 48 tokens, 32 over 8: 41 (91); 50 of 90, 11 tokens, 128 over 32, where it is the
+// items' cost above all: 79 (109).
 // Slower: one reading of the scores with all 64 in registers (spills, and code beyond the instruction caches), two groups that convert, the
 // next item's queries loaded in front of the last product (registers spill: 88 us where it was 82 then).
 #include <stddef.h>

@@ -8,7 +8,7 @@
 // A row, or with few or long rows a part of one, is brought into a CTA's shared memory by one bulk copy (the bytes in front of its first and
 // behind its last 16-byte boundary by loads) and read from there twice: for the maximum of every thread, and for the sums.  CTAs of a row are a cluster and meet in the shared memory of the first.
 //
-// Measured: 2047 rows of 32002 bf16 logits with 20 alternatives 41 us, 3.2 TB/s (without alternatives 30); 2476 of 6842 with 5: 21.8; one row 6.1.  A copy at
+// Measured: 2047 rows of 32002 bf16 logits with 20 alternatives 41 us, 3.2 TB/s (without alternatives 30); 2476 of 6842 with 5: 21.3; one row 6.0; float32, 1000 rows of 32000: 44.6, 2.9 TB/s.  A copy at
 // memory's rate would take 20 us, and the instructions, 12 an element, 22: what is above that is that a row's steps (copy, maxima, bound, sums, alternatives) wait for one another, and with three rows an SM, all that fits its
 // shared memory, half of the issue slots stay empty.  More threads a row, parts of half the size (two CTAs a row: 83 us) and candidates sought outside
 // the sums' loop (43 to 50 us) are slower.  Five CTAs an SM, where shared memory lets them, want 48 registers, for which loops are unrolled by two and four: with three

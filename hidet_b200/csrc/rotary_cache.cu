@@ -10,10 +10,10 @@
 // Scales are float: as f16 they would add 2^-11 to an error of 2^-8 at worst, for 2 bytes of 2 D + 8.
 //
 // Each element crosses memory once: the rotation of q and k and the quantization of k and v are one launch, in which a row's lanes hold it in
-// registers from load to store.  Measured (64 + 8 heads of 128, 2048 tokens, bf16) 15.6 us for the rotation, 4.9 TB/s of what is read and written, with half of the
-// issue slots used and the rest waiting for the loads behind the position's; (32 + 8 + 8 heads of 128, 8192 tokens, bf16) 41 us for the append, 4.7 TB/s, some
-// 300 instructions a warp for its four rows; (8 heads of 128, 16384 tokens, f16) 21.1 us for the read, 4.8 TB/s with 72 % of the issue slots.  A few
-// tokens cost the launch, 4.3 us.
+// registers from load to store.  Measured (64 + 8 heads of 128, 2048 tokens, bf16) 15.8 us for the rotation, 4.9 TB/s of what is read and written, with half of the
+// issue slots used and the rest waiting for the loads behind the position's; (32 + 8 + 8 heads of 128, 8192 tokens, bf16) 43 us for the append, 4.4 TB/s, some
+// 300 instructions a warp for its four rows; (8 heads of 128, 16384 tokens, f16) 20.9 us for the read, 4.9 TB/s with 60 % of the issue slots.  In float32, where
+// bytes count for more, 24.6 us (6.2 TB/s), 59.7 (6.0) and 37.5 (4.5).  A few tokens cost the launch, 4.3 us.
 #include "serving.cuh"
 
 namespace b200q {
@@ -235,7 +235,7 @@ __device__ __forceinline__ float larger(float top, float x) {
     return r;
 }
 
-// Five blocks an SM: for six the registers spill, 50 us for the 41 above; four take 42.5.
+// Five blocks an SM: for six the registers spill, a fifth slower; four are slower by 4 %.
 // GROUP lanes (threadIdx.x, dim / 16 of them active) hold a row: a head of q (rotated and written), of k (rotated and quantized) or of v (quantized).
 template <typename T, bool VEC, int GROUP>
 __global__ void __launch_bounds__(kThreads, 5) append_kernel(const __grid_constant__ HeadRows q, const __grid_constant__ HeadRows q_out, const __grid_constant__ HeadRows k,
