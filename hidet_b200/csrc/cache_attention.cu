@@ -284,10 +284,10 @@ __global__ void __launch_bounds__(THREADS, Layout<D, NT>::PER_SM) cache_attentio
                 if (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
                     for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    const uint32_t e = min(max(__float_as_uint(top) >> 23, 64u), 253u);
+                    const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
                     if (top > 0.0f) down = __uint_as_float((254u - e) << 23), up = __uint_as_float(e << 23);
                 }
-                if (lane == 0) ctl.q_scale[r] = up * p.scale_log2;
+                if (lane == 0) ctl.q_scale[r] = fmaxf(up * p.scale_log2, kLeastNormal);  // not zero, which makes NaN of a hidden position's -inf
 #pragma unroll
                 for (int j = 0; j < (D + 127) / 128; ++j) {
                     const int d = 4 * lane + 128 * j;

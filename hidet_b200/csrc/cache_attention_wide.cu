@@ -365,8 +365,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache_attention_wide_kernel(const 
                     met = true;
                     break;
                 }
-                auto exponent_of = [&](int row) { return min(max(__float_as_uint(fmaxf(ctl.top[0][row], ctl.top[1][row])) >> 23, 64u), 253u); };
-                if (kScaled) qs *= __uint_as_float(exponent_of(r) << 23);
+                auto exponent_of = [&](int row) { return min(max(__float_as_uint(fmaxf(ctl.top[0][row], ctl.top[1][row])) >> 23, 1u), 253u); };
+                if (kScaled) qs = fmaxf(qs * __uint_as_float(exponent_of(r) << 23), kLeastNormal);  // not zero, which makes NaN of a hidden position's -inf
 #pragma unroll
                 for (int i = 0; i < LANES; ++i) {
                     const int own = 32 * quarter + STEP * i + lane / LANES;

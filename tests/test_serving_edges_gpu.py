@@ -232,3 +232,18 @@ def test_rotary_into_elements_that_share_their_memory_is_refused():
     whole = torch.empty((5, 2, 64), dtype=q.dtype, device='cuda')
     got = hidet_b200.rotary_embedding(q[:1], None, at[:1], table, out=(whole[:1, :1].expand(1, 1, 64).expand(1, 2, 64)[:, :1].as_strided((1, 2, 64), (0, 64, 1)), None))
     assert torch.equal(got[0], hidet_b200.rotary_embedding(q[:1], None, at[:1], table)[0])  # one token: its stride does not matter
+
+
+@pytest.mark.parametrize('heads,kv_heads,dim,tokens,long', FORMS)
+@pytest.mark.parametrize('q_std,k_std,scale', [(1e-28, 1.0, 1e27), (1e-36, 1.0, 1e29), (1e-37, 1e30, 1e6), (1e36, 1e-3, 1e-20), (1e-38, 1e-3, 1e-20), (1e20, 1e15, 1e-20)])
+def test_queries_and_scales_of_any_size(heads, kv_heads, dim, tokens, long, q_std, k_std, scale):
+    """A row's scores may be of ordinary size although its elements are not."""
+    lengths = [700, 90]
+    cache, table = a_cache(lengths, kv_heads, dim, 16)
+    for b, n in enumerate(lengths):
+        k, v = (normal(n, kv_heads, dim, seed=81 + i, dtype=torch.float32) for i in range(2))
+        hidet_b200.quantized_cache_append(cache, k * k_std, v, slots_in(table, b, n, 16))
+    if long:
+        cache, table = wide((cache, table))
+    q = (normal(sum(tokens), heads, dim, seed=83, dtype=torch.float32).double() * q_std).bfloat16()
+    check_attention(lengths, list(tokens), heads, kv_heads, dim, 16, torch.bfloat16, cache=(cache, table), q=q, scale=scale)
