@@ -23,7 +23,7 @@ def quantized_cache_attention(q: torch.Tensor, cache: torch.Tensor, page_table: 
     mask        None: a token sees every position up to its own.  Or bool / uint8 [tokens, w] with a row for every row of q: of the positions in front of its
                 sequence's new tokens it sees all, and the j-th of these where mask[row, j] (w at least the most of a sequence).  Trees of drafted
                 tokens are such masks.  A row that sees nothing is zeros.
-    scale       1 / sqrt(dim) by default.
+    scale       a positive number, 1 / sqrt(dim) by default.
     Returns the result in q's shape and type, and with return_lse also the natural logarithm of the softmax's denominators, float32 of q's shape without dim.
 
     Everything that changes from step to step is on the device: a captured step can be replayed while the sequences grow.  Lengths beyond the page

@@ -15,7 +15,8 @@ MOST_TOP = 32
 def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(log_probs, entropy, top_log_probs, top_indices) under softmax(logits[..., :]), all float32 but the int64 indices.
 
-    logits [..., vocab] float16, bfloat16 or float32; tokens int32 or int64, [...] or [..., n] (n tokens of every row): log_probs has their shape.
+    logits [..., vocab] float16, bfloat16 or float32, rows of up to 1638400 bytes (409600 tokens in float32); tokens int32 or int64,
+    [...] or [..., n] (n tokens of every row): log_probs has their shape.
     entropy [...] in nats; top_log_probs and top_indices [..., top] (top at most 32) the largest, descending, equal logits by index.
     -inf logits are tokens without probability; a row with a NaN or +inf, or of nothing but -inf, gives NaN.  A token outside the vocabulary has -inf and is
     reported by b200q_check_status."""

@@ -365,7 +365,7 @@ B200Q_API int b200q_quantized_cache_attention(const b200q_heads *q, void *out, f
 /*
  * Log probabilities under softmax(logits[row, :]): log_probs[row, j] of tokens[row, j] (int32 or int64 [rows, given]), the entropy of the row
  * (in nats), and the `top` (at most 32) largest log probabilities, descending, equal logits by index, with their tokens.  All float sums and
- * results; logits f16, bf16 or f32, rows row_stride elements apart.  A token outside the vocabulary has -inf and is reported.  -inf logits are
+ * results; logits f16, bf16 or f32, rows of up to 1638400 bytes, row_stride elements apart.  A token outside the vocabulary has -inf and is reported.  -inf logits are
  * tokens without probability; a row with a NaN or +inf, or of nothing but -inf, has NaN.
  */
 B200Q_API int b200q_token_log_probs(const void *logits, int64_t row_stride, const void *tokens, float *log_probs, float *entropy,

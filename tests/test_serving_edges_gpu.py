@@ -247,3 +247,12 @@ def test_queries_and_scales_of_any_size(heads, kv_heads, dim, tokens, long, q_st
         cache, table = wide((cache, table))
     q = (normal(sum(tokens), heads, dim, seed=83, dtype=torch.float32).double() * q_std).bfloat16()
     check_attention(lengths, list(tokens), heads, kv_heads, dim, 16, torch.bfloat16, cache=(cache, table), q=q, scale=scale)
+
+
+@pytest.mark.parametrize('dtype,vocab', [(torch.float32, 409600), (torch.bfloat16, 819200), (torch.float16, 819193)])
+def test_log_probs_of_the_longest_rows(dtype, vocab):
+    logits = normal(3, vocab + 1, seed=90, dtype=dtype, std=3.0)
+    check_log_probs(logits[:, :vocab], torch.tensor([0, vocab - 1, 77], device='cuda'), 20)
+    if vocab * dtype.itemsize == 1638400:
+        with pytest.raises(ffi.BackendException, match='are supported'):
+            hidet_b200.token_log_probs(logits, torch.zeros(3, dtype=torch.int64, device='cuda'))
