@@ -10,7 +10,8 @@
 //       meet at the end of the item.
 // The probabilities go back into tensor memory, in the place of their scores, as the first operand of the second product.  A thread has a whole row of 64 scores, so maximum and sum
 // need no exchange.  A row's unit is 2^u: u is its running maximum (in log2) plus the exponent of the largest value scale that it has seen so far, so that the products with
-// value scales fit f16 and sums of probabilities and of values are in the same unit.
+// value scales fit f16 and sums of probabilities and of values are in the same unit.  (So an exponential's argument has the exponent in it: where value scales are
+// near 2^-16, or 2^16, it is off by 2^-20 and the denominator's logarithm by up to 3e-6.  The result is not: its sums have the same errors above and below.)
 //
 // Bound by the two softmax groups.  A tile takes one 3400 clocks, 600 for the bound on its scores and 2800 for the probabilities (an item's first, whose maximum is
 // looked for, 1800 and 2000), so 64 positions of 128 rows pass every 1700, in which the tensor cores work for 256 (15 % of the time by the counters); the groups

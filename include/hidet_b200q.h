@@ -350,7 +350,8 @@ B200Q_API int b200q_quantized_cache_read(const void *cache, int64_t pages, int64
  * mask, NULL, the width counts as 0).
  * A row that sees nothing has zeros, and -inf in lse, and so has a row that no sequence has (in front of starts[0], from starts[batch] on).  head h reads key/value head h / (heads / kv_heads).
  *   out[row, h] = sum_j softmax_j(scale q . k_j) v_j, dense [tokens, heads, head_dim] in q's type (f16 or bf16); lse (float [tokens, heads], may be
- * NULL) the natural logarithm of the softmax's denominator.  q and out: 16-byte aligned,
+ * NULL) the natural logarithm of the softmax's denominator.  Values are taken to stay below 10^34 over the number of positions in magnitude (sums of
+ * them, times 2^14, are float).  q and out: 16-byte aligned,
  * strides multiples of 8 elements.
  * The workspace is one of b200q_qlinear_f16_i8's kind: zero-filled once, its counters are zero again after every call.
  */
