@@ -101,3 +101,21 @@ def test_starts_out_of_order_or_range(program, rows, grid, starts):
 def test_rows_without_a_sequence(program, rows, grid):
     for starts in ([0, 0, 0], [9, 9, 9]):
         assert plan(program, rows, grid, [100, 200], 9, starts) == ([], 0)
+
+
+def test_random_starts(program):
+    rng = random.Random(9)
+    for _ in range(60):
+        rows, grid = rng.choice([(8, 20), (128, 9)])
+        batch = rng.choice([1, 2, 33, 64])
+        starts = sorted(rng.randint(0, 50) for _ in range(batch + 1))
+        if rng.random() < 0.5:
+            starts[rng.randrange(batch + 1)] = rng.choice([-5, 7, 60])
+        lengths = [rng.randint(0, 500) for _ in range(batch)]
+        fine = starts == sorted(starts) and 0 <= starts[0] and starts[-1] <= 50
+        pieces, status = plan(program, rows, grid, lengths, 50, starts, 2, 3)
+        assert status == (0 if fine else 1 << 25)
+        if fine:
+            check(pieces, rows, lengths, starts, 2, 3)
+        else:
+            assert not pieces
