@@ -18,6 +18,10 @@ from .quant import (
     symmetric_quant_matmul,
     symmetric_quant_matmul_f16_i8,
     symmetric_quant_matmul_atomic_f16_i8,
+    quantize_tokens,
+    symmetric_quant_matmul_i8,
+    route_tokens,
+    mixture_of_experts,
 )
 from .serving import (
     rotary_table,

@@ -160,11 +160,12 @@ B200Q_API int b200q_check_status(void) {
     B200Q_CUDA_TRY(cudaMemcpy(word, zero, sizeof(zero), cudaMemcpyHostToDevice));
     if ((v[0] & 0x80000000u) == 0) {
         if (v[0] == 0x40000000u) return b200q::set_error(B200Q_INVALID_ARGUMENT, "an embedding lookup met an index outside its table (that row was written as zeros)");
-        return b200q::set_error(B200Q_INVALID_ARGUMENT, "kernels met indexes outside their range:%s%s%s%s%s%s", v[0] & 0x40000000u ? " a row outside an embedding table;" : "",
+        return b200q::set_error(B200Q_INVALID_ARGUMENT, "kernels met indexes outside their range:%s%s%s%s%s%s%s", v[0] & 0x40000000u ? " a row outside an embedding table;" : "",
                                 v[0] & b200q::kBadPosition ? " a position outside a rotary table;" : "", v[0] & b200q::kBadSlot ? " a slot outside a cache;" : "",
                                 v[0] & b200q::kBadPage ? " a page outside a cache or a length beyond its page table;" : "",
                                 v[0] & b200q::kBadToken ? " a token outside the vocabulary;" : "",
-                                v[0] & b200q::kBadStarts ? " sequences whose rows are out of order or outside;" : "");
+                                v[0] & b200q::kBadStarts ? " sequences whose rows are out of order or outside;" : "",
+                                v[0] & b200q::kBadExpert ? " an expert that its layer does not have;" : "");
     }
     return b200q::set_error(B200Q_KERNEL_TIMEOUT,
                             "a bounded device-side wait ran out: first in kernel id %u at wait site %u; all that ran out, or-ed: 0x%08x",

@@ -186,6 +186,11 @@ SIGNATURES = {
         c_int,
         True,
     ),
+    'b200q_quantize_tokens': ([c_void_p, c_int64, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p], c_int, True),
+    'b200q_qlinear_i8_i8': ([c_void_p] * 5 + [c_int64] * 3 + [c_int] * 3 + [c_void_p] * 2, c_int, True),
+    'b200q_route_tokens': ([c_void_p, c_int64] + [c_void_p] * 3 + [c_int64] * 4 + [c_int] * 3 + [c_void_p], c_int, True),
+    'b200q_mixture_of_experts_workspace_bytes': ([c_int64] * 5, c_size_t, False),
+    'b200q_mixture_of_experts': ([c_void_p, c_int64] + [c_void_p] * 7 + [c_int64, c_void_p] + [c_int64] * 5 + [c_int] * 2 + [c_void_p, c_size_t, c_void_p], c_int, True),
     'b200q_token_log_probs': ([c_void_p, c_int64] + [c_void_p] * 5 + [c_int64] * 4 + [c_int] * 2 + [c_void_p], c_int, True),
 }
 

@@ -291,6 +291,56 @@ B200Q_API int b200q_qlinear_f16_i8_static(const void *a, const void *wq, const v
                                           int64_t K, int w_layout, void *stream);
 
 /*
+ * ---- linears on int8 tokens ----
+ *
+ * These and the layers of experts below are launched as programmatic dependents of the kernel in front and let the kernel behind them start early.  The codes of a weight
+ * (wq, gate_up, down) may be requested before the dependency on the kernel in front is honoured, as b200q_qlinear_f16_i8 requests them for few rows:
+ * what is said of them at the top of this file holds here for every size.  None of them writes the codes of a weight.
+ */
+
+/*
+ * Tokens as int8 codes with one float scale each: row r of x (row_stride elements apart, of `type`, b200q_float_type) ->
+ *   y = x, or, with norm (of x's type, [width]), y = x * norm / sqrt(mean(x^2) + eps);   amax = max |y|
+ *   codes[r, i] = rint(y_i * (127 / amax)) (ties to even; dense rows of `width` bytes),   scales[r] = amax / 127
+ * in float; behind the norm the codes are taken from x * norm, in which the row's factor cancels.  A row whose amax (of x, or of x * norm) is below 2^-100 is
+ * zeros with a scale of zero; a row with a NaN or an infinity, or whose squares overflow in front of a norm, has a scale of NaN (codes of zero in the first case).
+ */
+B200Q_API int b200q_quantize_tokens(const void *x, int64_t row_stride, const void *norm, float eps, void *codes, float *scales, int64_t rows, int64_t width, int type,
+                                    void *stream);
+
+/*
+ * The product of int8 tokens and an int8 weight: c[M, N] (f16 or bf16 by out_type) =
+ *   float(sum_k a[m, k] wq[k, n]) * scale[n] * a_scale[m], then what `epilogue` (NULL: nothing) says, with bias and residual of c's type, in float, rounded once.
+ * The sum is exact, of 32 bits, for K up to 131071; beyond, B200Q_UNSUPPORTED.  a int8 [M, K], a_scale float [M], wq int8 [K, N] or [N, K] by w_layout, scale [N] of scale_type
+ * (b200q_float_type).  Any sizes and alignments; 16-byte aligned bases and rows (K, and N or N / 2 of the result) are fast.  c may be the residual.  No workspace.
+ */
+B200Q_API int b200q_qlinear_i8_i8(const void *a, const float *a_scale, const void *wq, const void *scale, void *c, int64_t M, int64_t N, int64_t K, int w_layout,
+                                  int scale_type, int out_type, const b200q_epilogue *epilogue, void *stream);
+
+/*
+ * ---- layers of experts ----
+ *
+ * route: logits l = x router^T (x [tokens, width], x_stride elements apart; router [count, width] dense, of x's type or f32), the `top` (at most 32) largest of a token's `count` (at most 1024), descending,
+ * equal ones by index, into experts[tokens, top], and into weights[tokens, top] exp(l_j) over the sum of the chosen ones, or (over_all != 0) of all.  In float.
+ * NaN counts as the largest; a token with a NaN or +inf among its logits, or with nothing but -inf, has weights of NaN.
+ */
+B200Q_API int b200q_route_tokens(const void *x, int64_t x_stride, const void *router, int32_t *experts, float *weights, int64_t tokens, int64_t width, int64_t count,
+                                 int64_t top, int over_all, int type, int router_type, void *stream);
+
+/*
+ * The experts' part of the layer, on int8 weights: out[t] (f16 or bf16, of x's type, dense) =
+ *   residual[t] + sum_j weights[t, j] * down_scale[e] (down[e] h),   h = silu(g) * u,   (g, u) = gate_up_scale[e] (gate_up[e] x[t]),   e = experts[t, j]
+ * gate_up int8 [count, 2 inner, hidden], its rows (gate_f, up_f) pairs at (2 f, 2 f + 1); down int8 [count, hidden, inner]; scales of scale_type, one for each row; both are what
+ * b200q_symmetric_quantize makes of the rows of all experts.  Sums are float; x and h are rounded to f16, a row at a time scaled by a power of two where
+ * their range asks for it.  The results do not depend on the run.  residual may be NULL, or out.  An assignment to a negative expert is passed over, one to an expert that is not there too, and is
+ * reported by b200q_check_status.  The workspace is one of b200q_qlinear_f16_i8's kind.
+ */
+B200Q_API size_t b200q_mixture_of_experts_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top);
+B200Q_API int b200q_mixture_of_experts(const void *x, int64_t x_stride, const int32_t *experts, const float *weights, const void *gate_up, const void *gate_up_scale,
+                                       const void *down, const void *down_scale, const void *residual, int64_t residual_stride, void *out, int64_t tokens, int64_t hidden,
+                                       int64_t inner, int64_t count, int64_t top, int type, int scale_type, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * ---- the operators around the linears of a decoder ----
  *
  * Launched as programmatic dependents of the kernel in front; they read and write nothing before the dependency on it is honoured, and
