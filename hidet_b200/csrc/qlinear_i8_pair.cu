@@ -1,0 +1,480 @@
+// The int8 x int8 product for many tokens, on pairs of SMs: tcgen05.mma kind::i8 with cta_group::2.
+//
+// Computed transposed, D[n, m] = sum_k w[k, n] a[m, k], sums of 32 bits in tensor memory: a pair owns 256 channels x tm tokens (tm a multiple of 32, at most
+// 256), of which each CTA fetches its own 128 channels and half of the tokens, 128 k a stage, straight into the form that the tensor core reads; nothing is
+// converted.  Tokens are the columns because their number is what comes in odd sizes: tm follows it in steps of 32, where lanes go by 256.  A weight [N, K] is a
+// K-major operand, one [K, N] an MN-major one.
+//
+// One persistent CTA per SM, ten warps:
+//   warps 0-7  epilogue, two groups that take the 32-token blocks of a tile in turn: tensor memory -> float, the two scales, bias, gate / up pairing, residual ->
+//              16 bits, transposed through a staging buffer (two per group, taken in turn) by matrix stores, 16-byte stores of whole output rows
+//   warp 8     TMA producer; both CTAs' copies count on the first CTA's barrier
+//   warp 9     MMA issuer (first CTA of the pair only), one thread for the whole loop
+// Two accumulators, so that a tile's epilogue runs beside the next one's products.
+//
+// Every wait is bounded: a wait that runs out records where and raises a CTA-wide flag, all roles leave, the first CTA waits for what was armed and issued, and the
+// two CTAs meet at a cluster barrier before either gives back tensor memory or retires.
+#include <atomic>
+
+#include "qlinear_i8.h"
+#include "umma.cuh"
+
+namespace b200q {
+namespace i8pair {
+
+constexpr unsigned int kKernelI8Pair = 9;
+constexpr int TN = 128;                      // channels per CTA; a pair's tile has twice as many
+constexpr int BK = 128;                      // k per stage = four MMAs of K = 32
+constexpr int W_BYTES = BK * TN;
+constexpr int MAX_STAGES = 10;
+constexpr int EPI_GROUPS = 2;
+constexpr int LOAD_WARP = 8, MMA_WARP = 9;
+constexpr int THREADS = 32 * 10;
+constexpr int TMEM_COLS = 512;
+constexpr int ROW_BYTES = TN * 2 + 16;       // one output row in the staging buffer, padded: matrix stores touch every bank once
+constexpr int STAGING_BYTES = 32 * ROW_BYTES;
+constexpr int RING_BYTES = 188 * 1024;
+constexpr int SMEM_BYTES = RING_BYTES + EPI_GROUPS * 2 * STAGING_BYTES + 1024;  // + alignment slack
+
+struct Params {
+    I8Args a;
+    int tm;                    // tokens per tile
+    int n_tiles, m_tiles;
+    int band;                  // token tiles that are walked together, channel tile by channel tile
+    int k_blocks;
+    int stages;
+};
+
+__device__ __forceinline__ void tile_of(const Params &p, int u, int &n0, int &m0) {
+    const int band_tiles = p.band * p.n_tiles;
+    const int b = u / band_tiles, r = u - b * band_tiles;
+    const int rows = min(p.band, p.m_tiles - b * p.band);
+    const int n = r / rows;
+    n0 = n * 2 * TN;
+    m0 = (b * p.band + (r - n * rows)) * p.tm;
+}
+
+// A tile into this CTA's shared memory, its bytes counted on a barrier of the pair's first CTA.
+__device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "l"(policy)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t idesc_i8(int m, int n, bool a_mn_major) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn_major << 15) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_pair_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// A tile of [k][128 channels] in rows of 128 swizzled bytes: 8-row groups 1024 bytes apart, both strides (there is one group of channels, so that one of them is not used).
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3fffu) | (64ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if (BF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+    if (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+template <bool BF16>
+__device__ __forceinline__ float value_at(const void *p, int64_t i) {
+    return BF16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]) : __half2float(static_cast<const __half *>(p)[i]);
+}
+
+// NK: the weight is [N, K].  PAIRS: channels (2j, 2j + 1) = (gate, up).
+template <bool NK, bool BF16, bool PAIRS>
+__global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(2, 1, 1)
+    i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const Params p) {
+    extern __shared__ unsigned char smem_dyn[];
+    __shared__ __align__(8) uint64_t full[MAX_STAGES];    // (first CTA) both CTAs' tiles of the stage have landed
+    __shared__ __align__(8) uint64_t empty[MAX_STAGES];   // the MMAs that read it have completed
+    __shared__ __align__(8) uint64_t acc_full[2];         // an accumulator holds a finished tile
+    __shared__ __align__(8) uint64_t acc_empty[2];        // (first CTA) both CTAs' epilogue warps have read it out
+    __shared__ __align__(8) uint64_t drain_bar;           // every MMA issued has completed (teardown)
+    __shared__ uint32_t tmem_base_slot;
+    __shared__ int abort_flag;
+
+    const uint32_t smem_base = (smem_u32(smem_dyn) + 1023u) & ~1023u;  // swizzled operands; the same in both CTAs
+    unsigned char *smem_gen = smem_dyn + (smem_base - smem_u32(smem_dyn));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int units = p.n_tiles * p.m_tiles;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const uint32_t stages = p.stages, stage_bytes = W_BYTES + (uint32_t)p.tm * (BK / 2);
+    constexpr int STAGING_OFF = RING_BYTES;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < MAX_STAGES; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(smem_u32(&acc_full[b]), 1);
+            mbar_init(smem_u32(&acc_empty[b]), 2 * 4 * EPI_GROUPS);
+        }
+        mbar_init(smem_u32(&drain_bar), 1);
+        abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == MMA_WARP) {
+        umma::alloc_pair(smem_u32(&tmem_base_slot), TMEM_COLS);
+        umma::relinquish_pair();
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    cluster_arrive_release();
+    cluster_wait_acquire();  // both CTAs' barriers are set up and both have their tensor memory
+    umma::fence_after_sync();
+    const uint32_t tmem_base = tmem_base_slot;
+    if (lane == 0 && warp == LOAD_WARP) {
+        tma_prefetch_desc(&map_w);
+        tma_prefetch_desc(&map_a);
+    }
+    pdl_wait();
+
+    auto wait = [&](uint32_t bar, uint32_t parity, unsigned int site) -> bool {
+        bool ok = mbar_wait(bar, parity, umma::kFastPolls);
+        if (__all_sync(0xffffffffu, ok)) return true;
+        if (!ok) ok = umma::wait_or_abort<kKernelI8Pair>(bar, parity, site, &abort_flag, p.a.status);
+        return __all_sync(0xffffffffu, ok);
+    };
+    auto wait_one = [&](uint32_t bar, uint32_t parity, unsigned int site) -> bool {
+        return mbar_wait(bar, parity, umma::kFastPolls) || umma::wait_or_abort<kKernelI8Pair>(bar, parity, site, &abort_flag, p.a.status);
+    };
+
+    if (warp == LOAD_WARP) {
+        // ---------------- TMA producer ----------------
+        pdl_launch_dependents();  // tensor memory is allocated: a kernel that is placed as this one's CTAs leave cannot take it away
+        if (lane == 0) {
+            const uint64_t keep = l2_policy_evict_last();  // both operands are read again by other tiles
+            const uint32_t full0 = map_to_rank(smem_u32(&full[0]), 0);
+            uint32_t i = 0;
+            umma::Ring r;
+            bool ok = true;
+            for (int u = first; u < units && ok; u += step) {
+                int n, m;
+                tile_of(p, u, n, m);
+                n += (int)rank * TN;
+                m += (int)rank * (p.tm / 2);
+                for (int kb = 0; kb < p.k_blocks; ++kb, ++i, r.advance(1, stages)) {
+                    if (i >= stages && !wait_one(smem_u32(&empty[r.slot]), r.phase ^ 1u, 1)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t at = smem_base + r.slot * stage_bytes, bar = full0 + 8 * r.slot;
+                    if (rank == 0) mbar_expect_tx(smem_u32(&full[r.slot]), 2 * stage_bytes);
+                    load_pair(at, &map_w, NK ? kb * BK : n, NK ? n : kb * BK, bar, keep);
+                    load_pair(at + W_BYTES, &map_a, kb * BK, m, bar, keep);
+                }
+            }
+            // Teardown: every copy armed must have landed before a CTA may retire; what counts them is the first CTA's barriers, and the second CTA
+            // waits for the first at the cluster barrier below.  Slot s was last used for the largest j < i with j % stages == s.
+            for (uint32_t s = 0; rank == 0 && s < stages; ++s) {
+                if (i <= s) continue;
+                const uint32_t j = i - 1 - (i - 1 - s) % stages;
+                if (!mbar_wait(smem_u32(&full[s]), (j / stages) & 1)) report_timeout(p.a.status, kKernelI8Pair, 7);
+            }
+        }
+    } else if (warp == MMA_WARP) {
+        // ---------------- MMA issuer ----------------
+        if (rank == 0 && elect_one()) {
+            const uint32_t idesc = idesc_i8(2 * TN, p.tm, !NK);
+            constexpr uint32_t W_STEP = NK ? 32 / 16 : 32 * TN / 16;  // of the weight's descriptor, 32 k on
+            uint32_t t_iter = 0;
+            umma::Ring r;
+            bool ok = true, here = false;
+            for (int u = first; u < units && ok; u += step, ++t_iter) {
+                const uint32_t buf = t_iter & 1, acc_use = t_iter >> 1;
+                if (acc_use >= 1 && !wait_one(smem_u32(&acc_empty[buf]), (acc_use - 1) & 1, 3)) break;
+                umma::fence_after_sync();
+                const uint32_t d_addr = tmem_base + buf * p.tm;
+                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                    if (!here && !wait_one(smem_u32(&full[r.slot]), r.phase, 4)) {
+                        ok = false;
+                        break;
+                    }
+                    umma::fence_after_sync();
+                    const uint32_t at = smem_base + r.slot * stage_bytes;
+                    const uint64_t w_desc = NK ? umma::smem_desc_sw128(at) : smem_desc_mn(at), a_desc = umma::smem_desc_sw128(at + W_BYTES);
+#pragma unroll
+                    for (int ks = 0; ks < BK / 32; ++ks) mma_pair_i8(d_addr, w_desc + W_STEP * ks, a_desc + 2 * ks, idesc, (kb > 0 || ks > 0) ? 1u : 0u);
+                    umma::commit_pair(smem_u32(&empty[r.slot]));
+                    r.advance(1, stages);
+                    here = mbar_test(smem_u32(&full[r.slot]), r.phase);
+                }
+                if (ok) umma::commit_pair(smem_u32(&acc_full[buf]));
+            }
+            // Teardown: no MMA may still be running when tensor memory is given back or the peer retires.
+            umma::commit_pair_self(smem_u32(&drain_bar));
+            if (!mbar_wait(smem_u32(&drain_bar), 0)) report_timeout(p.a.status, kKernelI8Pair, 8);
+        }
+    } else {
+        // ---------------- epilogue ----------------
+        const int eg = warp >> 2;               // takes blocks eg, eg + EPI_GROUPS, ...
+        const int q = warp & 3;                 // tensor-memory lanes 32 q .. 32 q + 31
+        const int et = 32 * q + lane;           // 0 .. 127
+        auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + eg) : "memory"); };
+        const int g = lane >> 2, tq = lane & 3; // fragment coordinates: channel g of 8, tokens 2 tq, 2 tq + 1 of 8
+        const int M = p.a.M, N = p.a.N;
+        const void *res = p.a.residual;
+        const bool res_vec = !PAIRS && p.a.residual_vec;
+        const int out_n = PAIRS ? N >> 1 : N;
+        constexpr int ROW_CHUNKS_LOG2 = PAIRS ? 3 : 4;         // 16-byte pieces of a tile's output row
+        const int chunk = et & ((1 << ROW_CHUNKS_LOG2) - 1);
+        const int row_in_pass = et >> ROW_CHUNKS_LOG2;
+        constexpr int PASS_ROWS = 128 >> ROW_CHUNKS_LOG2;
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(32 * q) << 16);
+        uint32_t t_iter = 0, block = 0;         // block: the group's 32-token blocks so far, staging buffers in turn
+        for (int u = first; u < units; u += step, ++t_iter) {
+            int n0, m0;
+            tile_of(p, u, n0, m0);
+            n0 += (int)rank * TN;
+            const uint32_t buf = t_iter & 1, acc_use = t_iter >> 1;
+            const int m_left = min(M - m0, p.tm);
+            const int blocks = (m_left + 31) / 32;
+            const uint32_t acc = lane_addr + buf * p.tm;
+            float sc[2][2], bias[2][2];  // [16-channel block][8-channel half]: channel 16 h + 8 e + g of this warp's 32
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int n = n0 + 32 * q + 16 * h + 8 * e + g;
+                    sc[h][e] = n < N ? i8_scale(p.a.scale, p.a.scale_type, n) : 0.0f;
+                    bias[h][e] = n < N && p.a.bias != nullptr ? value_at<BF16>(p.a.bias, n) : 0.0f;
+                }
+            if (!all_of_128(1 + eg, wait(smem_u32(&acc_full[buf]), acc_use & 1, 10))) break;  // the group stays or leaves as one
+            umma::fence_after_sync();
+            const int out_n0 = PAIRS ? n0 >> 1 : n0;
+            const bool cols_ok = out_n0 + chunk * 8 < out_n;  // widths are multiples of 8: eight channels are in or out together
+            const size_t out_off = (size_t)m0 * out_n + out_n0 + chunk * 8;
+            if (eg >= blocks) {  // a tile of a single block: nothing for this group
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&acc_empty[buf]), 0));
+            }
+#pragma unroll 1
+            for (int cb = eg; cb < blocks; cb += EPI_GROUPS, ++block) {
+                unsigned char *staging = smem_gen + STAGING_OFF + (2 * eg + (block & 1)) * STAGING_BYTES;
+                const uint32_t staging_a = smem_base + STAGING_OFF + (2 * eg + (block & 1)) * STAGING_BYTES;
+                float sa[4][2];  // token 8 j + 2 tq + i
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int m = cb * 32 + 8 * j + 2 * tq + i;
+                        sa[j][i] = m < m_left ? p.a.a_scale[m0 + m] : 0.0f;
+                    }
+                if (res_vec) {
+                    // the residual's block goes through the staging buffer into the fragments' layout
+#pragma unroll
+                    for (int pass = 0; pass < 4; ++pass) {
+                        const int r = pass * 8 + row_in_pass, m = cb * 32 + r;
+                        uint4 val = make_uint4(0, 0, 0, 0);
+                        if (m < m_left && cols_ok) val = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(res) + (size_t)(m0 + m) * p.a.ldr + out_n0 + chunk * 8));
+                        *reinterpret_cast<uint4 *>(staging + r * ROW_BYTES + chunk * 16) = val;
+                    }
+                    group_sync();
+                }
+                uint32_t v[2][16];
+                umma::ld_16x256b_x4(acc + cb * 32, v[0]);
+                umma::ld_16x256b_x4(acc + (16u << 16) + cb * 32, v[1]);
+                umma::ld_wait();
+                if (cb + EPI_GROUPS >= blocks) {  // the group's part of the accumulator is in registers
+                    umma::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&acc_empty[buf]), 0));
+                }
+                // v[h][4 j + 2 e + i]: channel 16 h + 8 e + g, token 8 j + 2 tq + i
+                auto sum_of = [&](int h, int j, int e, int i) { return fmaf((float)(int)v[h][4 * j + 2 * e + i] * sc[h][e], sa[j][i], bias[h][e]); };
+                if (PAIRS) {
+                    // Lanes with even g hold gates, the lanes with g + 1 what they multiply; of the two 8-channel halves each lane of such a pair finishes one,
+                    // for its two tokens.
+                    const bool odd = g & 1;
+#pragma unroll
+                    for (int j = 0; j < 4; j += 2) {
+                        float z[2][2][2];  // [token block j, j + 1][channel block h][token]
+#pragma unroll
+                        for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    const float y0 = sum_of(h, j + jj, 0, i), y1 = sum_of(h, j + jj, 1, i);
+                                    const float other = __shfl_xor_sync(0xffffffffu, odd ? y0 : y1, 4);
+                                    z[jj][h][i] = silu(odd ? other : y0) * (odd ? y1 : other);
+                                }
+                        if (res != nullptr) {
+#pragma unroll
+                            for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                    for (int i = 0; i < 2; ++i) {
+                                        const int oc = out_n0 + 16 * q + 8 * h + (odd ? 4 : 0) + (g >> 1), m = cb * 32 + 8 * (j + jj) + 2 * tq + i;
+                                        if (oc < out_n && m < m_left) z[jj][h][i] += value_at<BF16>(res, (int64_t)(m0 + m) * p.a.ldr + oc);
+                                    }
+                        }
+                        uint32_t pk[4];
+#pragma unroll
+                        for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) pk[2 * jj + h] = pack2<BF16>(z[jj][h][0], z[jj][h][1]);
+                        // result channel g / 2 (even g) or 4 + g / 2 (odd g) of each 8: stored in the order of g, put right on the way out
+                        const int mi = lane >> 3;
+                        umma::stmatrix_x4_trans(staging_a + (8 * (j + (mi >> 1)) + (lane & 7)) * ROW_BYTES + (16 * q + 8 * (mi & 1)) * 2, pk);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t place = staging_a + (8 * j + (lane & 7)) * ROW_BYTES + (32 * q + 8 * (lane >> 3)) * 2;
+                        uint32_t rs[4] = {0u, 0u, 0u, 0u}, pk[4];
+                        if (res_vec) umma::ldmatrix_x4_trans(rs, place);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                float y[2] = {sum_of(h, j, e, 0), sum_of(h, j, e, 1)};
+                                if (res_vec) {
+                                    const float2 r2 = unpack2<BF16>(rs[2 * h + e]);
+                                    y[0] += r2.x;
+                                    y[1] += r2.y;
+                                } else if (res != nullptr) {
+                                    const int n = n0 + 32 * q + 16 * h + 8 * e + g;
+#pragma unroll
+                                    for (int i = 0; i < 2; ++i) {
+                                        const int m = cb * 32 + 8 * j + 2 * tq + i;
+                                        if (n < N && m < m_left) y[i] += value_at<BF16>(res, (int64_t)(m0 + m) * p.a.ldr + n);
+                                    }
+                                }
+                                pk[2 * h + e] = pack2<BF16>(y[0], y[1]);
+                            }
+                        umma::stmatrix_x4_trans(place, pk);
+                    }
+                }
+                group_sync();  // the four warps: block complete; the other buffer is free
+#pragma unroll 4
+                for (int r = row_in_pass; r < 32; r += PASS_ROWS) {
+                    const int m = cb * 32 + r;
+                    if (m < m_left && cols_ok) {
+                        uint4 val = *reinterpret_cast<const uint4 *>(staging + r * ROW_BYTES + chunk * 16);
+                        if (PAIRS) {  // channels stand in the order 0 4 1 5 2 6 3 7
+                            val = make_uint4(__byte_perm(val.x, val.y, 0x5410), __byte_perm(val.z, val.w, 0x5410), __byte_perm(val.x, val.y, 0x7632),
+                                             __byte_perm(val.z, val.w, 0x7632));
+                        }
+                        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.a.c) + out_off + (size_t)m * out_n) = val;
+                    }
+                }
+            }
+        }
+    }
+
+    // ---------------- teardown: both CTAs are done with each other's shared and tensor memory ----------------
+    __syncwarp();
+    umma::fence_before_sync();
+    cluster_arrive_release();
+    cluster_wait_acquire();
+    if (warp == MMA_WARP) {
+        umma::fence_after_sync();
+        umma::dealloc_pair(tmem_base, TMEM_COLS);
+    }
+}
+
+template <bool NK, bool BF16, bool PAIRS>
+int launch_as(const CUtensorMap &map_w, const CUtensorMap &map_a, const Params &p, unsigned grid, cudaStream_t stream) {
+    static std::atomic<bool> attr_set[64];  // per device; a repeated set by a racing thread is harmless
+    int dev = 0;
+    B200Q_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
+        B200Q_CUDA_TRY(cudaFuncSetAttribute(i8_pair_kernel<NK, BF16, PAIRS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+        if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(THREADS, 1, 1);
+    cfg.dynamicSmemBytes = SMEM_BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attrs[1];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 1;
+    B200Q_CUDA_TRY(cudaLaunchKernelEx(&cfg, i8_pair_kernel<NK, BF16, PAIRS>, map_w, map_a, p));
+    return B200Q_OK;
+}
+
+}  // namespace i8pair
+
+// Tokens per tile: the number with the least rounds of tiles times clocks a stage.
+int plan_i8_pair(int64_t M, int64_t N) {
+    using namespace i8pair;
+    int sms = sm_count();
+    if (sms <= 0) sms = 148;
+    int best = 256;
+    double least = 0.0;
+    for (int tm = 256; tm >= 32; tm -= 32) {
+        const int64_t units = ceil_div(M, tm) * ceil_div(N, 2 * TN);
+        const double products = 2.0 * tm, copies = (W_BYTES + tm * (BK / 2)) / 50.0;
+        const double cost = (double)ceil_div(units, sms / 2) * (products > copies ? products : copies);
+        if (least == 0.0 || cost < least) least = cost, best = tm;
+    }
+    return best;
+}
+
+int launch_i8_pair(const I8Args &a, int tm, cudaStream_t stream) {
+    using namespace i8pair;
+    CUtensorMap map_w, map_a;
+    int rc = a.nk ? make_tensor_map_2d(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, (uint64_t)a.K, (uint64_t)a.N, (uint64_t)a.K, BK, TN, CU_TENSOR_MAP_SWIZZLE_128B,
+                                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B)
+                  : make_tensor_map_2d(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, (uint64_t)a.N, (uint64_t)a.K, (uint64_t)a.N, TN, BK, CU_TENSOR_MAP_SWIZZLE_128B,
+                                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    if (rc != B200Q_OK) return rc;
+    rc = make_tensor_map_2d(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.a, (uint64_t)a.K, (uint64_t)a.M, (uint64_t)a.K, BK, (uint32_t)(tm / 2), CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    if (rc != B200Q_OK) return rc;
+    Params p = {};
+    p.a = a;
+    p.tm = tm;
+    p.n_tiles = (int)ceil_div(a.N, 2 * TN);
+    p.m_tiles = (int)ceil_div(a.M, tm);
+    // as many token tiles in a band as leave the band's codes well inside L2
+    int64_t band = ((int64_t)48 << 20) / ((int64_t)tm * a.K);
+    if (band < 1) band = 1;
+    p.band = (int)(band < p.m_tiles ? band : p.m_tiles);
+    p.k_blocks = (int)ceil_div(a.K, BK);
+    const int stages = RING_BYTES / (W_BYTES + tm * (BK / 2));
+    p.stages = stages < MAX_STAGES ? stages : MAX_STAGES;
+    const int64_t units = (int64_t)p.n_tiles * p.m_tiles;
+    if (units * 2 > 2147483647LL) return set_error(B200Q_UNSUPPORTED, "qlinear_i8_i8: problem too large for the tile counter");
+    int sms = sm_count();
+    if (sms <= 0) sms = 148;
+    const int64_t pairs_at_once = sms / 2;
+    const unsigned grid = 2u * (unsigned)(units < pairs_at_once ? units : pairs_at_once);
+    const int form = (a.nk ? 4 : 0) + (a.out_type == B200Q_BF16 ? 2 : 0) + (a.pairs ? 1 : 0);
+    switch (form) {
+        case 0: return launch_as<false, false, false>(map_w, map_a, p, grid, stream);
+        case 1: return launch_as<false, false, true>(map_w, map_a, p, grid, stream);
+        case 2: return launch_as<false, true, false>(map_w, map_a, p, grid, stream);
+        case 3: return launch_as<false, true, true>(map_w, map_a, p, grid, stream);
+        case 4: return launch_as<true, false, false>(map_w, map_a, p, grid, stream);
+        case 5: return launch_as<true, false, true>(map_w, map_a, p, grid, stream);
+        case 6: return launch_as<true, true, false>(map_w, map_a, p, grid, stream);
+        default: return launch_as<true, true, true>(map_w, map_a, p, grid, stream);
+    }
+}
+
+}  // namespace b200q
