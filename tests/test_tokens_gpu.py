@@ -52,7 +52,8 @@ def test_quantize_tokens_is_the_formula_in_float(dtype):
     x = normal(generator(1), 64, 1536, dtype=dtype)
     amax = x.float().abs().amax(-1, keepdim=True)
     codes, scales = hidet_b200.quantize_tokens(x)
-    assert torch.equal(codes, torch.round(x.float() * (torch.full_like(amax, 127.0) / amax)).to(torch.int8))
+    by = torch.full_like(amax, 127.0) / amax  # rounded to float; the product of two floats is exact in 64 bits
+    assert torch.equal(codes, torch.round(x.double() * by.double()).to(torch.int8))
     assert torch.equal(scales, (amax / torch.full_like(amax, 127.0))[:, 0])
 
 
