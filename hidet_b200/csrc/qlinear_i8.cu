@@ -108,6 +108,10 @@ B200Q_API int b200q_qlinear_i8_i8(const void *a, const float *a_scale, const voi
     p.residual_vec = p.residual != nullptr && aligned_to(p.residual, 16) && (p.ldr % 8 == 0 || M == 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool lines = aligned_to(a, 16) && aligned_to(wq, 16) && aligned_to(c, 16) && K > 0 && K % 16 == 0 && (p.nk || N % 16 == 0) && width % 8 == 0;
+    if (lines && M <= 64) {
+        const int tm = (int)round_up(M, 16);
+        return launch_i8_split(p, tm, plan_i8_split(M, N, tm), s);
+    }
     if (lines) return launch_i8_pair(p, plan_i8_pair(M, N), s);
     return launch_i8_any(p, s);
 }

@@ -32,6 +32,9 @@ int launch_i8_any(const I8Args &p, cudaStream_t stream);
 // 16-byte aligned bases and rows of both operands and the result; tm tokens per tile, a multiple of 32 up to 256.
 int plan_i8_pair(int64_t M, int64_t N);
 int launch_i8_pair(const I8Args &p, int tm, cudaStream_t stream);
+// tm a multiple of 16 up to 256, a cluster of up to eight CTAs for a tile.
+int plan_i8_split(int64_t M, int64_t N, int tm);
+int launch_i8_split(const I8Args &p, int tm, int cluster, cudaStream_t stream);
 
 #ifdef __CUDACC__
 __device__ __forceinline__ float i8_scale(const void *p, int type, int64_t i) {
