@@ -92,7 +92,7 @@ extern "C" {
 B200Q_API size_t b200q_mixture_of_experts_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top) {
     using namespace b200q;
     if (tokens <= 0 || hidden <= 0 || inner < 0 || count < 0 || top <= 0) return 0;
-    return kWorkspaceHead + (size_t)round_up(tokens * top * inner * 4, 256);
+    return kWorkspaceHead + experts_stream_bytes(tokens, hidden, inner, count, top);
 }
 
 B200Q_API int b200q_mixture_of_experts(const void *x, int64_t x_stride, const int32_t *experts, const float *weights, const void *gate_up, const void *gate_up_scale,
@@ -116,13 +116,24 @@ B200Q_API int b200q_mixture_of_experts(const void *x, int64_t x_stride, const in
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
         return set_error(B200Q_WORKSPACE_TOO_SMALL, "%s: needs %zu bytes of workspace, got %zu", op, need, workspace == nullptr ? (size_t)0 : workspace_bytes);
     }
+    if (!aligned_to(workspace, 16)) return set_error(B200Q_INVALID_ARGUMENT, "%s: the workspace is not 16-byte aligned", op);
     ExpertsArgs p = {};
     p.x = x, p.x_stride = x_stride, p.experts = experts, p.weights = weights, p.gate_up = static_cast<const int8_t *>(gate_up), p.down = static_cast<const int8_t *>(down);
     p.gate_up_scale = gate_up_scale, p.down_scale = down_scale, p.residual = residual, p.out = out, p.residual_stride = residual_stride;
     p.tokens = (int)tokens, p.hidden = (int)hidden, p.inner = (int)inner, p.count = (int)count, p.top = (int)top, p.scale_type = scale_type, p.type = type;
     p.status = device_status_word();
-    float *h = reinterpret_cast<float *>(static_cast<char *>(workspace) + kWorkspaceHead);
-    return launch_any(p, h, static_cast<cudaStream_t>(stream));
+    float *scratch = reinterpret_cast<float *>(static_cast<char *>(workspace) + kWorkspaceHead);
+    for (int64_t t = 0; t < tokens; t += kExpertsTokens) {
+        ExpertsArgs q = p;
+        q.tokens = (int)(tokens - t < kExpertsTokens ? tokens - t : kExpertsTokens);
+        q.x = static_cast<const uint16_t *>(x) + t * x_stride, q.out = static_cast<uint16_t *>(out) + t * hidden;
+        if (top > 0) q.experts = experts + t * top, q.weights = weights + t * top;
+        if (residual != nullptr) q.residual = static_cast<const uint16_t *>(residual) + t * residual_stride;
+        const int rc = experts_stream_supported(q) ? launch_experts_stream(q, static_cast<unsigned int *>(workspace), scratch, static_cast<cudaStream_t>(stream))
+                                                   : launch_any(q, scratch, static_cast<cudaStream_t>(stream));
+        if (rc != B200Q_OK) return rc;
+    }
+    return B200Q_OK;
 }
 
 }  // extern "C"

@@ -94,6 +94,8 @@ def mixture_of_experts(x: torch.Tensor, experts: torch.Tensor, weights: torch.Te
     elif out.dtype != x.dtype or out.shape != x.shape or not out.is_contiguous():
         raise ValueError('out must be a contiguous tensor of {} {}'.format(x.dtype, list(x.shape)))
     rows = rows_of(x)
+    if rows.data_ptr() % 16 != 0 or rows.stride(0) % 8 != 0:
+        rows = rows.clone(memory_format=torch.contiguous_format)  # loads of eight elements
     others = rows_of(residual) if residual is not None else None
     experts, weights, gate_up, down = experts.contiguous(), weights.contiguous(), gate_up.contiguous(), down.contiguous()
     gate_up_scale, down_scale = gate_up_scale.contiguous(), down_scale.contiguous()
