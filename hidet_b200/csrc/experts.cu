@@ -92,7 +92,7 @@ extern "C" {
 B200Q_API size_t b200q_mixture_of_experts_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top) {
     using namespace b200q;
     if (tokens <= 0 || hidden <= 0 || inner < 0 || count < 0 || top <= 0) return 0;
-    return kWorkspaceHead + experts_stream_bytes(tokens, hidden, inner, count, top);
+    return kWorkspaceHead + experts_stream_bytes(tokens, inner, top);
 }
 
 B200Q_API int b200q_mixture_of_experts(const void *x, int64_t x_stride, const int32_t *experts, const float *weights, const void *gate_up, const void *gate_up_scale,

@@ -31,7 +31,7 @@ constexpr int64_t kExpertsTokens = 64;  // of one launch
 
 // Rows and bases in lines of 16 bytes, up to 1024 experts, 32 a token.
 bool experts_stream_supported(const ExpertsArgs &p);
-size_t experts_stream_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top);
+size_t experts_stream_bytes(int64_t tokens, int64_t inner, int64_t top);
 int launch_experts_stream(const ExpertsArgs &p, unsigned int *counters, float *scratch, cudaStream_t stream);
 
 }  // namespace b200q

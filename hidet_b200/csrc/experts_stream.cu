@@ -1,19 +1,24 @@
 // A layer of experts over a few tokens as two streams of int8 weights: gate and up, and down.  Inference at batch sizes where the weights of the experts that have
 // a token are all there is to read.
 //
-// Both kernels are the same machine.  Every CTA makes the list of entries, an expert with up to 8 G of its assignments (an expert with more has several), and takes an
-// equal, contiguous part of all their units: 32 rows of an entry's weight over all of K (gate and up), or over a part of it (down).  A copying warp streams the
-// unit's tiles, 32 rows x 512 k, through a ring; eight warps have 64 k of a tile each:
-//     weights  a lane's 16 neighbouring k of a row in one load, int8 -> exact f16, the 16-row operand of mma.sync
-//     tokens   a lane's same 16 k of its column's token from global memory (they stay in L1), -> f16, the 8-column operand
-//     sums     float, of the eight warps added in shared memory, in their order
-// With one to eight tokens an expert the product is a stream, so what tcgen05 would add is not needed and its 128 lanes would stand mostly empty; the conversions take about a
-// third of the issue slots at memory's rate.
-// Gate and up: h = silu(g) u in float to global memory, and its largest magnitude per assignment.  Down: h is scaled by a power of two from that, so that f16 holds it
-// whatever the range (as tokens in bf16 are, by their own largest), and a unit's sums, times scale and weight, are a piece of every assignment's result.  The
-// CTA that brings a column tile's last piece adds them up, token by token, assignments and parts of K in their order: the result does not depend on who came when.
+// The tensor core multiplies the weights as they are, int8 by int8: a token's row is written as whole numbers v = rint(x 2^e), |v| <= 2^22 (e by the row's largest
+// element, so that an element is off by at most 2^-22 of that), and these as three digits of 8 bits, v = 65536 d2 + 256 d1 + d0 with d in -128 .. 127.  A tile of 128 rows of the weight is the
+// first operand of tcgen05.mma, three columns for each token are the second, sums of 32 bits are exact, and float begins behind them.  So weights are only ever copied,
+// and what is computed on them costs no issue slots.  (As f16 by mma.sync, with int8 widened in registers, a tile took 260 instructions of each of eight warps, and the
+// stream stood at 3.2 TB/s.)
 //
-// Down starts while gate and up run: its CTAs fill their rings with weights and wait there for h.
+// Every CTA makes the list of entries, an expert with up to C of its assignments (an expert with more has several entries), and takes an equal, contiguous part of
+// all stages, 128 rows x 128 k each.  16 warps:
+//     warp 0      copies the weights' tiles into a ring
+//     warp 1      issues the products, into two accumulators in turn
+//     warps 4-7   finish: tensor memory -> float -> h, or results
+//     warps 8-15  digits: take the ring's stages in turn and put the tokens' digits beside the weights' tile
+// Gate and up: rows (2 f, 2 f + 1) are neighbouring lanes; h = silu(g) u in float to global memory, and its largest magnitude per assignment, which is what down's
+// digits are scaled by.  A unit (an entry's 128 rows) that two or more CTAs share has its whole-number sums added by the one that comes last.
+// Down: a column tile's entries follow one another, and what a CTA has of them it adds up in float, times scales and weights, in their order; the CTA that comes last adds the
+// CTAs' parts in theirs.  Nothing depends on who comes when.
+//
+// Down's CTAs start as those of gate and up leave, and fill their rings with weights while they wait for h.
 //
 // Waits are bounded: one that runs out is reported and raises a flag, after which nobody in the CTA waits or copies any more; everyone goes through the motions
 // to the end, so that no barrier is left alone.
@@ -25,27 +30,32 @@ namespace b200q {
 namespace {
 
 constexpr unsigned int kKernelExperts = 11;
-constexpr int ROWS = 32;                  // of a unit
-constexpr int BOX_K = 128;                // one copy: 32 rows x 128 k, rows of 128 swizzled bytes
-constexpr int BOXES = 4, STAGE_K = BOX_K * BOXES;
-constexpr int BOX_BYTES = ROWS * BOX_K, STAGE_BYTES = BOX_BYTES * BOXES;
-constexpr int MATH_WARPS = 8, MATH_THREADS = 32 * MATH_WARPS, COPY_WARP = MATH_WARPS, FINISH_WARPS = 3;
-constexpr int WARP_K = STAGE_K / MATH_WARPS;
-constexpr int UP_THREADS = MATH_THREADS + 32, DOWN_THREADS = UP_THREADS + 32 * FINISH_WARPS;
-constexpr int MOST_STAGES = 6;
+constexpr int TN = 128, BK = 128;         // rows and k of a stage
+constexpr int W_BYTES = TN * BK;
+constexpr int DIGITS = 3;
+constexpr int COPY_WARP = 0, MMA_WARP = 1, FINISH_WARP0 = 4, DIGIT_WARP0 = 8, DIGIT_WARPS = 8;
+constexpr int WARPS = 16, THREADS = 32 * WARPS;
+constexpr int MOST_STAGES = 10;
+constexpr int MOST_SMEM = 225 * 1024;
 constexpr int MOST_ASSIGNMENTS = 2048;    // of one launch
 constexpr int MOST_EXPERTS = 1024;
-// what of the workspace's counters is whose
-constexpr int COUNTER_TILES = 32768, COUNTER_DONE = COUNTER_TILES, COUNTER_MAX = COUNTER_TILES + 1;
+constexpr int kMostExact = 131071;        // products of 2^14 whose sum 32 bits hold
+constexpr uint16_t kNone = 0xffff;
+// what of the workspace's counters is whose: arrivals at what CTAs share (by the first of them), CTAs that are through, h's largest magnitudes
+constexpr int MOST_CTAS = 1024, COUNTER_UP = 0, COUNTER_DOWN = MOST_CTAS, COUNTER_DONE = 2 * MOST_CTAS, COUNTER_MAX = 4 * MOST_CTAS;
 
 struct StreamArgs {
     ExpertsArgs a;
     float *h;             // [assignments, inner]
-    float *pieces;        // [parts][assignments, hidden]
+    void *shared;         // gate and up: int32 [CTAs][2][columns][128]; down: float [CTAs][2][tokens][128]
     unsigned int *counters;
-    int tiles;            // of 32 rows, of an expert's weight
-    int parts, part_k;    // of K (down); part_k a multiple of STAGE_K unless there is one part
+    int tiles;            // of 128 rows, of an expert's weight
+    int k_blocks;
+    int per_entry;        // C: assignments of an entry
+    int columns;          // 3 C, rounded up to 16
+    uint32_t tmem_cols;
     int stages;
+    int digit_warps;      // that take stages in turn
 };
 
 struct Entry {
@@ -58,91 +68,118 @@ __device__ __forceinline__ float scale_at(const void *p, int type, int64_t i) {
     return static_cast<const float *>(p)[i];
 }
 
-// The power of two that brings a largest magnitude (as bits) to 2^14 .. 2^15, and its inverse; one for zero, infinity and NaN.
+// The power of two that brings a row's largest magnitude (as bits) to 2^21 .. 2^22, and its inverse.  Rows below 2^-98 are zeros; rows with an infinity or a NaN are NaN.
 __device__ __forceinline__ float power_for(uint32_t bits, float &inverse) {
-    int e = 141 - (int)(bits >> 23);  // 127 + 14 - exponent
-    e = bits == 0 || bits >= 0x7f800000u ? 0 : max(-120, min(120, e));
-    inverse = __uint_as_float((uint32_t)(127 - e) << 23);
-    return __uint_as_float((uint32_t)(127 + e) << 23);
+    const int e = 148 - (int)(bits >> 23);  // 127 + 21 - exponent
+    const bool zero = e > 119;
+    inverse = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : zero ? 0.0f : __uint_as_float((uint32_t)(127 - e) << 23);
+    return zero || bits >= 0x7f800000u ? 0.0f : __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-// 16 neighbouring elements of a token as eight f16 pairs.
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
+// 16 neighbouring elements of a token.
 struct FromF16 {
     typedef uint4 Raw[2];
     static __device__ __forceinline__ void load(const void *row, int64_t k, Raw &r) {
         const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const __half *>(row) + k);
         r[0] = p[0], r[1] = p[1];
     }
-    static __device__ __forceinline__ void convert(const Raw &r, float, uint32_t (&b)[8]) {
-        b[0] = r[0].x, b[1] = r[0].y, b[2] = r[0].z, b[3] = r[0].w, b[4] = r[1].x, b[5] = r[1].y, b[6] = r[1].z, b[7] = r[1].w;
+    static __device__ __forceinline__ void widen(uint32_t w, float &lo, float &hi) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        lo = f.x, hi = f.y;
+    }
+    static __device__ __forceinline__ uint32_t largest(uint32_t bits, uint32_t w) {  // as float's
+        return max(bits, max(__float_as_uint(__half2float(__ushort_as_half((uint16_t)(w & 0x7fffu)))), __float_as_uint(__half2float(__ushort_as_half((uint16_t)(w >> 16 & 0x7fffu))))));
     }
 };
 struct FromBF16 {
     typedef uint4 Raw[2];
-    static __device__ __forceinline__ void load(const void *row, int64_t k, Raw &r) {
-        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(row) + k);
-        r[0] = p[0], r[1] = p[1];
-    }
-    static __device__ __forceinline__ void convert(const Raw &r, float by, uint32_t (&b)[8]) {
-        const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
-        const f32x2 by2 = pair_of(by, by);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float lo, hi;
-            halves(mul2(pair_of(w[i] << 16, w[i] & 0xffff0000u), by2), lo, hi);
-            b[i] = pack_f16(lo, hi);
-        }
-    }
+    static __device__ __forceinline__ void load(const void *row, int64_t k, Raw &r) { FromF16::load(row, k, r); }
+    static __device__ __forceinline__ void widen(uint32_t w, float &lo, float &hi) { lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u); }
+    static __device__ __forceinline__ uint32_t largest(uint32_t bits, uint32_t w) { return max(bits, max(w << 16 & 0x7fff0000u, w & 0x7fff0000u)); }
 };
 struct FromF32 {
-    typedef float4 Raw[4];
+    typedef uint4 Raw[4];
     static __device__ __forceinline__ void load(const void *row, int64_t k, Raw &r) {
-        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(row) + k);
+        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const float *>(row) + k);
 #pragma unroll
         for (int i = 0; i < 4; ++i) r[i] = p[i];
     }
-    static __device__ __forceinline__ void convert(const Raw &r, float by, uint32_t (&b)[8]) {
-        const f32x2 by2 = pair_of(by, by);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float lo, hi;
-            halves(mul2(pair_of(r[i].x, r[i].y), by2), lo, hi);
-            b[2 * i] = pack_f16(lo, hi);
-            halves(mul2(pair_of(r[i].z, r[i].w), by2), lo, hi);
-            b[2 * i + 1] = pack_f16(lo, hi);
-        }
-    }
 };
+template <typename X>
+__device__ __forceinline__ void widen4(const typename X::Raw &r, int i, float (&f)[4]) {
+    const uint4 v = r[i >> 1];
+    X::widen(i & 1 ? v.z : v.x, f[0], f[1]);
+    X::widen(i & 1 ? v.w : v.y, f[2], f[3]);
+}
+template <>
+__device__ __forceinline__ void widen4<FromF32>(const FromF32::Raw &r, int i, float (&f)[4]) {
+    f[0] = __uint_as_float(r[i].x), f[1] = __uint_as_float(r[i].y), f[2] = __uint_as_float(r[i].z), f[3] = __uint_as_float(r[i].w);
+}
 
-template <int G>
+// The digits of four elements, a word each: adding 1.5 * 2^23 rounds to a whole number that stands in the sum's low bits, and with 128 added to each digit they are its bytes.
+__device__ __forceinline__ void digits_of(const float (&f)[4], float by, uint32_t (&d)[DIGITS]) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(fmaf(f[i], by, 12582912.0f)) + (0x808080u - 0x4b400000u);
+    const uint32_t lo = __byte_perm(u[0], u[1], 0x5140), hi = __byte_perm(u[2], u[3], 0x5140);
+    d[0] = __byte_perm(lo, hi, 0x5410) ^ 0x80808080u;
+    d[1] = __byte_perm(lo, hi, 0x7632) ^ 0x80808080u;
+    d[2] = __byte_perm(__byte_perm(u[0], u[1], 0x0062), __byte_perm(u[2], u[3], 0x0062), 0x5410) ^ 0x80808080u;
+}
+
+__device__ __forceinline__ uint32_t idesc_i8(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+__device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void ld_32x32b_x8(uint32_t taddr, int (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+
 struct Shared {
-    uint64_t full[MOST_STAGES], empty[MOST_STAGES];
-    uint64_t ready[2], freed[2];          // (down) a unit's pieces are in memory; its finishing is over
-    int abort_flag, entries, last;
-    float by[2][8 * G], back[2][8 * G];   // powers of two of the columns' tokens, of this entry and the next
-    alignas(16) float sums[MATH_WARPS][ROWS][8 * G + 2];
+    uint64_t weights[MOST_STAGES], tokens[MOST_STAGES], empty[MOST_STAGES];  // a stage's two operands are in place; its products are through
+    uint64_t acc_full[2], acc_empty[2], drain;
+    uint32_t tmem_base;
+    int abort_flag, entries, last, to_add;
+    int add[2][3];  // (down) what this CTA adds up at the end: tile, first and last CTA
     int counts[MOST_EXPERTS];
-    uint16_t chosen[MOST_ASSIGNMENTS];    // the expert of every assignment, or kNone
-    uint16_t order[MOST_ASSIGNMENTS];     // assignments, by expert
-    Entry entry[1];                       // as many as there are
+};
+// Behind it: by, back, share [n] (float, of the assignments in their order), entry [n], chosen, order [n] (uint16), (down) sums [tokens][128] (float)
+struct Lists {
+    float *by, *back, *share;
+    Entry *entry;
+    uint16_t *chosen, *order;
+    float *sums;
+    __host__ __device__ static constexpr int bytes(int n, int tokens) { return round16(12 * n) + round16(12 * n) + round16(4 * n) + tokens * TN * 4; }
+    __host__ __device__ static constexpr int round16(int b) { return (b + 15) / 16 * 16; }
+    __device__ __forceinline__ Lists(unsigned char *at, int n) {
+        by = reinterpret_cast<float *>(at), back = by + n, share = back + n;
+        at += round16(12 * n);
+        entry = reinterpret_cast<Entry *>(at);
+        at += round16(12 * n);
+        chosen = reinterpret_cast<uint16_t *>(at), order = chosen + n;
+        sums = reinterpret_cast<float *>(at + round16(4 * n));
+    }
 };
 
 // The entries of a launch: counts by expert, a scan over the experts, assignments in their places.  Every CTA makes them for itself, so an expert's assignments stand in
 // their own order: as they come they would differ from CTA to CTA, and with them who is in which entry of an expert with several.
-constexpr uint16_t kNone = 0xffff;
-template <int G>
-__device__ void make_entries(const ExpertsArgs &a, Shared<G> &s, int threads) {
+__device__ void make_entries(const ExpertsArgs &a, int columns, Shared &s, const Lists &l) {
     const int n = a.tokens * a.top;
-    for (int e = threadIdx.x; e < a.count; e += threads) s.counts[e] = 0;
+    for (int e = threadIdx.x; e < a.count; e += THREADS) s.counts[e] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += threads) {
+    for (int i = threadIdx.x; i < n; i += THREADS) {
         const int e = __ldcg(a.experts + i);
         const bool there = e >= 0 && e < a.count;
-        s.chosen[i] = there ? (uint16_t)e : kNone;
+        l.chosen[i] = there ? (uint16_t)e : kNone;
         if (there) atomicAdd(&s.counts[e], 1);
         else if (e >= 0 && blockIdx.x == 0 && a.status != nullptr) atomicOr(a.status, kBadExpert);
     }
@@ -150,14 +187,14 @@ __device__ void make_entries(const ExpertsArgs &a, Shared<G> &s, int threads) {
     if (threadIdx.x < 32) {
         int first = 0, entries = 0;  // assignments and entries of the experts so far
         for (int e0 = 0; e0 < a.count; e0 += 32) {
-            const int e = e0 + threadIdx.x, mine = e < a.count ? s.counts[e] : 0, my_entries = (mine + 8 * G - 1) / (8 * G);
+            const int e = e0 + threadIdx.x, mine = e < a.count ? s.counts[e] : 0, my_entries = (mine + columns - 1) / columns;
             int at = mine, at_entry = my_entries;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int x = __shfl_up_sync(0xffffffffu, at, o), y = __shfl_up_sync(0xffffffffu, at_entry, o);
                 if ((int)threadIdx.x >= o) at += x, at_entry += y;
             }
-            for (int i = 0; i < my_entries; ++i) s.entry[entries + at_entry - my_entries + i] = {e, first + at - mine + i * 8 * G, min(8 * G, mine - i * 8 * G)};
+            for (int i = 0; i < my_entries; ++i) l.entry[entries + at_entry - my_entries + i] = {e, first + at - mine + i * columns, min(columns, mine - i * columns)};
             if (e < a.count) s.counts[e] = first + at - mine;
             first += __shfl_sync(0xffffffffu, at, 31), entries += __shfl_sync(0xffffffffu, at_entry, 31);
         }
@@ -165,11 +202,11 @@ __device__ void make_entries(const ExpertsArgs &a, Shared<G> &s, int threads) {
         __syncwarp();
         for (int i0 = 0; i0 < n; i0 += 32) {
             const int i = i0 + threadIdx.x;
-            const uint32_t e = i < n ? s.chosen[i] : kNone, same = __match_any_sync(0xffffffffu, e);
+            const uint32_t e = i < n ? l.chosen[i] : kNone, same = __match_any_sync(0xffffffffu, e);
             const int place = e != kNone ? s.counts[e] : 0;
             __syncwarp();
             if (e != kNone) {
-                s.order[place + __popc(same & ((1u << threadIdx.x) - 1u))] = (uint16_t)i;
+                l.order[place + __popc(same & ((1u << threadIdx.x) - 1u))] = (uint16_t)i;
                 if ((same >> threadIdx.x) == 1u) s.counts[e] = place + __popc(same);  // the last of them
             }
             __syncwarp();
@@ -177,6 +214,26 @@ __device__ void make_entries(const ExpertsArgs &a, Shared<G> &s, int threads) {
     }
     __syncthreads();
 }
+
+// Where a CTA is in its part of the stages.  Gate and up: k fastest, then an entry's tiles, then entries; down: k, then a tile's entries, then tiles.
+template <bool DOWN>
+struct Place {
+    int entry, tile, k;
+    __device__ __forceinline__ Place(int64_t stage, const StreamArgs &p, int entries) {
+        const int64_t u = stage / p.k_blocks;
+        const int inner = DOWN ? max(entries, 1) : p.tiles;
+        const int outer = (int)(u / inner), in = (int)(u - (int64_t)outer * inner);
+        k = (int)(stage - u * p.k_blocks);
+        entry = DOWN ? in : outer, tile = DOWN ? outer : in;
+    }
+    __device__ __forceinline__ void next_unit(const StreamArgs &p, int entries) {
+        if (DOWN) {
+            if (++entry == entries) entry = 0, ++tile;
+        } else {
+            if (++tile == p.tiles) tile = 0, ++entry;
+        }
+    }
+};
 
 __device__ __forceinline__ float token_value(const void *p, int type, int64_t i) {
     return type == B200Q_F16 ? __half2float(static_cast<const __half *>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
@@ -189,38 +246,50 @@ __device__ __forceinline__ void store_result(const ExpertsArgs &a, int t, int n,
 }
 
 // X: what the tokens are; DOWN: h, else x.
-template <int G, bool DOWN, typename X>
-__global__ void __launch_bounds__(DOWN ? DOWN_THREADS : UP_THREADS, 1) experts_stream_kernel(const __grid_constant__ CUtensorMap map_w, const StreamArgs p) {
+template <bool DOWN, typename X>
+__global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid_constant__ CUtensorMap map_w, const StreamArgs p) {
     extern __shared__ unsigned char smem_dyn[];
     const uint32_t ring = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char *ring_gen = smem_dyn + (ring - smem_u32(smem_dyn));
-    Shared<G> &s = *reinterpret_cast<Shared<G> *>(ring_gen + p.stages * STAGE_BYTES);
+    const uint32_t stages = p.stages, stage_bytes = W_BYTES + (uint32_t)p.columns * BK;
+    Shared &s = *reinterpret_cast<Shared *>(ring_gen + stages * stage_bytes);
     const ExpertsArgs &a = p.a;
+    const Lists l(reinterpret_cast<unsigned char *>(&s + 1), a.tokens * a.top);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int THREADS = DOWN ? DOWN_THREADS : UP_THREADS;
-    constexpr int AHEAD = G < 2 ? G : 2;  // groups of columns whose tokens are on their way
-    const uint32_t stages = p.stages;
-    const int K = DOWN ? a.inner : a.hidden;
+    const int K = DOWN ? a.inner : a.hidden, rows = DOWN ? a.hidden : 2 * a.inner;
 
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < stages; ++i) {
-            mbar_init(smem_u32(&s.full[i]), 1);
-            mbar_init(smem_u32(&s.empty[i]), MATH_WARPS);
+            mbar_init(smem_u32(&s.weights[i]), 1);
+            mbar_init(smem_u32(&s.tokens[i]), 1);
+            mbar_init(smem_u32(&s.empty[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&s.ready[i]), MATH_WARPS);
-            mbar_init(smem_u32(&s.freed[i]), 1);
+            mbar_init(smem_u32(&s.acc_full[i]), 1);
+            mbar_init(smem_u32(&s.acc_empty[i]), 4);
         }
-        s.abort_flag = 0;
+        mbar_init(smem_u32(&s.drain), 1);
+        s.abort_flag = 0, s.to_add = 0;
         mbar_fence_init();
+    }
+    if (warp == MMA_WARP) {
+        umma::alloc(smem_u32(&s.tmem_base), p.tmem_cols);
+        umma::relinquish();
     }
     // The experts were chosen in front of gate and up, which waits for that before it lets down start: down may read them, and request weights, without waiting.
     if (!DOWN) pdl_wait();
-    make_entries<G>(a, s, THREADS);
+    umma::fence_before_sync();
+    make_entries(a, p.per_entry, s, l);
+    umma::fence_after_sync();
     pdl_launch_dependents();
-    const int per_entry = p.tiles * p.parts;
-    const int64_t units = (int64_t)s.entries * per_entry;
-    const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+    const uint32_t tmem_base = s.tmem_base;
+    const int entries = s.entries;
+    const int64_t total = (int64_t)entries * p.tiles * p.k_blocks;
+    const int64_t ctas = total < gridDim.x ? (total > 0 ? total : 1) : gridDim.x;  // that have a part
+    auto first_of = [&](int64_t cta) { return cta < ctas ? total * cta / ctas : total; };
+    const int64_t s0 = first_of(blockIdx.x), s1 = first_of((int64_t)blockIdx.x + 1);
+    const int mine = (int)(s1 - s0);  // stages of this CTA
+    const Place<DOWN> start(s0, p, entries);
 
     auto wait = [&](uint64_t *bar, uint32_t parity, unsigned int site) {
         const uint32_t b = smem_u32(bar);
@@ -231,241 +300,291 @@ __global__ void __launch_bounds__(DOWN ? DOWN_THREADS : UP_THREADS, 1) experts_s
         report_timeout(a.status, kKernelExperts, site);
         atomicExch(&s.abort_flag, 1);
     };
-    auto k_of = [&](int64_t u, int &k0, int &k1, int &tile, int &entry) {
-        entry = (int)(u / per_entry);
-        const int r = (int)(u - (int64_t)entry * per_entry), part = r / p.tiles;
-        tile = r - part * p.tiles;
-        k0 = part * p.part_k, k1 = min(K, k0 + p.part_k);
-    };
 
     if (warp == COPY_WARP) {
         // ---------------- the stream of weights ----------------
         if (lane == 0) {
             const uint64_t once = l2_policy_evict_first();
+            Place<DOWN> at = start;
             umma::Ring r;
-            uint32_t i = 0;
-            bool ok = true;
-            for (int64_t u = u0; u < u1 && ok; ++u) {
-                int k0, k1, tile, entry;
-                k_of(u, k0, k1, tile, entry);
-                const int row = s.entry[entry].expert * (DOWN ? a.hidden : 2 * a.inner) + tile * ROWS;
-                for (int k = k0; k < k1; k += STAGE_K, ++i, r.advance(1, stages)) {
-                    if (i >= stages) wait(&s.empty[r.slot], r.phase ^ 1u, 1);
-                    if (*reinterpret_cast<volatile int *>(&s.abort_flag) != 0) {
-                        ok = false;
-                        break;
-                    }
-                    const int boxes = min(BOXES, (k1 - k + BOX_K - 1) / BOX_K);
-                    const uint32_t bar = smem_u32(&s.full[r.slot]), at = ring + r.slot * STAGE_BYTES;
-                    mbar_expect_tx(bar, boxes * BOX_BYTES);
-                    for (int b = 0; b < boxes; ++b) tma_load_2d_hint(at + b * BOX_BYTES, &map_w, k + b * BOX_K, row, bar, once);
-                }
+            int i = 0;
+            for (; i < mine; ++i, r.advance(1, stages)) {
+                if (i >= (int)stages) wait(&s.empty[r.slot], r.phase ^ 1u, 1);
+                if (*reinterpret_cast<volatile int *>(&s.abort_flag) != 0) break;
+                const uint32_t bar = smem_u32(&s.weights[r.slot]);
+                mbar_expect_tx(bar, W_BYTES);
+                tma_load_2d_hint(ring + r.slot * stage_bytes, &map_w, at.k * BK, l.entry[at.entry].expert * rows + at.tile * TN, bar, once);
+                if (++at.k == p.k_blocks) at.k = 0, at.next_unit(p, entries);
             }
             // every copy armed has landed before the CTA may retire
-            for (uint32_t t = 0; t < stages; ++t) {
-                if (i <= t) continue;
-                const uint32_t j = i - 1 - (i - 1 - t) % stages;
-                if (!mbar_wait(smem_u32(&s.full[t]), (j / stages) & 1)) report_timeout(a.status, kKernelExperts, 7);
-            }
+            for (int t = i > (int)stages ? i - (int)stages : 0; t < i; ++t)
+                if (!mbar_wait(smem_u32(&s.weights[t % stages]), (t / stages) & 1)) report_timeout(a.status, kKernelExperts, 7);
         }
         __syncwarp();
         if (DOWN) pdl_wait();
-    } else if (warp < MATH_WARPS) {
+    } else if (warp == MMA_WARP) {
         // ---------------- products ----------------
+        if (elect_one()) {
+            const uint32_t idesc = idesc_i8(TN, p.columns);
+            umma::Ring r;
+            int k = start.k;
+            uint32_t unit = 0;
+            for (int i = 0; i < mine;) {
+                const uint32_t buf = unit & 1;
+                if (unit >= 2) wait(&s.acc_empty[buf], ((unit >> 1) - 1) & 1, 3);
+                umma::fence_after_sync();
+                const uint32_t d = tmem_base + buf * p.columns;
+                for (bool first = true; k < p.k_blocks && i < mine; ++k, ++i, first = false, r.advance(1, stages)) {
+                    wait(&s.weights[r.slot], r.phase, 4);
+                    wait(&s.tokens[r.slot], r.phase, 5);
+                    umma::fence_after_sync();
+                    const uint32_t at = ring + r.slot * stage_bytes;
+                    const uint64_t w_desc = umma::smem_desc_sw128(at), x_desc = umma::smem_desc_sw128(at + W_BYTES);
+#pragma unroll
+                    for (int ks = 0; ks < BK / 32; ++ks) mma_i8(d, w_desc + 2 * ks, x_desc + 2 * ks, idesc, !first || ks > 0 ? 1u : 0u);
+                    umma::commit(smem_u32(&s.empty[r.slot]));
+                }
+                umma::commit(smem_u32(&s.acc_full[buf]));
+                ++unit, k = 0;
+            }
+            umma::commit(smem_u32(&s.drain));
+            if (!mbar_wait(smem_u32(&s.drain), 0)) report_timeout(a.status, kKernelExperts, 8);
+        }
+        __syncwarp();
+        if (DOWN) pdl_wait();
+    } else if (warp >= 2) {
         if (DOWN) pdl_wait();  // h
-        const int g = lane >> 2, t = lane & 3;
-        // An eighth of a load's lanes reads two rows' four chunks: they lie in different banks where the rows are four apart (chunk c of row r stands at c ^ (r & 7)).
-        const int row = (g >> 1) | ((g & 1) << 2);
-        const int chunk = (warp & 1) * 4 + t;
-        const uint32_t a_off = (uint32_t)(warp >> 1) * BOX_BYTES + row * BOX_K + ((uint32_t)(chunk ^ row) << 4);
-        umma::Ring r;
-        int now = -1, which = 0;
-        Entry en = {0, 0, 0};
-        const void *rows[G];
-        float by[G];
-        for (int64_t u = u0; u < u1; ++u) {
-            int k0, k1, tile, entry;
-            k_of(u, k0, k1, tile, entry);
-            if (entry != now) {
-                // ---- another expert: its tokens' rows, and the powers of two that they are scaled by ----
-                now = entry, which ^= 1, en = s.entry[entry];
-                for (int c = warp; c < 8 * G; c += MATH_WARPS) {
-                    float inverse = 1.0f, power = 1.0f;
-                    if (c < en.count) {
-                        const int as = s.order[en.first + c];
-                        uint32_t bits = 0;
-                        if (DOWN) {
-                            bits = __ldcg(p.counters + COUNTER_MAX + as);
-                            power = power_for(bits, inverse);
-                        } else if (a.type == B200Q_BF16) {
-                            const uint4 *x = reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.x) + (int64_t)(as / a.top) * a.x_stride);
-#pragma unroll 4
-                            for (int i = lane; i < K / 8; i += 32) {
-                                const uint4 v = x[i];
-                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) bits = max(bits, max(w[j] << 16 & 0x7fff0000u, w[j] & 0x7fff0000u));
-                            }
-                            power = power_for(__reduce_max_sync(0xffffffffu, bits), inverse);
-                        }
-                    }
-                    if (lane == 0) s.by[which][c] = power, s.back[which][c] = inverse;
+        // ---------------- the powers of two of the rows that this CTA's entries have ----------------
+        if (mine > 0) {
+            if (DOWN) {
+                const Entry last = l.entry[entries - 1];
+                for (int i = threadIdx.x - 64; i < last.first + last.count; i += THREADS - 64) {
+                    const int as = l.order[i];
+                    l.by[i] = power_for(__ldcg(p.counters + COUNTER_MAX + as), l.back[i]);
+                    l.share[i] = __ldcg(a.weights + as);
                 }
-                asm volatile("bar.sync 1, %0;" ::"n"(MATH_THREADS) : "memory");
-#pragma unroll
-                for (int i = 0; i < G; ++i) {
-                    const int c = 8 * i + g, as = c < en.count ? s.order[en.first + c] : 0;
-                    by[i] = s.by[which][c];
-                    rows[i] = DOWN ? static_cast<const void *>(p.h + (int64_t)as * K) : static_cast<const void *>(static_cast<const uint16_t *>(a.x) + (int64_t)(as / a.top) * a.x_stride);
-                }
-            }
-            float acc[2][G][4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < G; ++j)
-#pragma unroll
-                    for (int l = 0; l < 4; ++l) acc[i][j][l] = 0.0f;
-            for (int k = k0; k < k1; k += STAGE_K, r.advance(1, stages)) {
-                const int64_t mine = k + warp * WARP_K + 16 * t;
-                const bool some = k + warp * WARP_K < k1, inside = mine < k1;  // K is a multiple of 16
-                auto fetch = [&](int i, typename X::Raw &x) {
-                    if (inside && 8 * i + g < en.count) X::load(rows[i], mine, x);
-                    else memset(x, 0, sizeof(x));
-                };
-                typename X::Raw raw[AHEAD];
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) fetch(i, raw[i]);
-                wait(&s.full[r.slot], r.phase, 2);
-                if (some) {
-                    const unsigned char *at = ring_gen + r.slot * STAGE_BYTES + a_off;
-                    uint4 w[4];  // rows + 0, 8, 16, 24
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4 *>(at + i * 8 * BOX_K);
-                    uint32_t f[4][8];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) umma::cvt_s8x4_to_f16_pairs(v[j], f[i][2 * j], f[i][2 * j + 1]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < G; ++i) {
-                        if (8 * i < en.count) {
-                            uint32_t b[8];
-                            X::convert(raw[i % AHEAD], by[i], b);
-                            if (i + AHEAD < G && 8 * (i + AHEAD) < en.count) fetch(i + AHEAD, raw[i % AHEAD]);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                mma_m16n8k16(acc[0][i], f[0][2 * j], f[1][2 * j], f[0][2 * j + 1], f[1][2 * j + 1], b[2 * j], b[2 * j + 1]);
-                                mma_m16n8k16(acc[1][i], f[2][2 * j], f[3][2 * j], f[2][2 * j + 1], f[3][2 * j + 1], b[2 * j], b[2 * j + 1]);
-                            }
-                        }
-                    }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&s.empty[r.slot]));
-            }
-            // ---- the eight warps' sums ----
-            const int groups = (en.count + 7) / 8;
-#pragma unroll
-            for (int i = 0; i < G; ++i) {
-                if (i < groups) {
-#pragma unroll
-                    for (int l = 0; l < 2; ++l) {
-                        *reinterpret_cast<float2 *>(&s.sums[warp][16 * l + row][8 * i + 2 * t]) = make_float2(acc[l][i][0], acc[l][i][1]);
-                        *reinterpret_cast<float2 *>(&s.sums[warp][16 * l + 8 + row][8 * i + 2 * t]) = make_float2(acc[l][i][2], acc[l][i][3]);
-                    }
-                }
-            }
-            asm volatile("bar.sync 1, %0;" ::"n"(MATH_THREADS) : "memory");
-            if (!DOWN) {
-                // thread: pair j of 16, column c
-                for (int i = threadIdx.x; i < 128 * groups; i += MATH_THREADS) {
-                    const int j = i & 15, c = i >> 4, f = tile * (ROWS / 2) + j;
-                    float gate = 0.0f, up = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < MATH_WARPS; ++w) gate += s.sums[w][2 * j][c], up += s.sums[w][2 * j + 1][c];
-                    uint32_t bits = 0;
-                    const int as = c < en.count ? s.order[en.first + c] : 0;
-                    if (c < en.count && f < a.inner) {
-                        const int64_t at = (int64_t)en.expert * 2 * a.inner + 2 * f;
-                        const float back = s.back[which][c];
-                        gate = gate * back * scale_at(a.gate_up_scale, a.scale_type, at);
-                        up = up * back * scale_at(a.gate_up_scale, a.scale_type, at + 1);
-                        const float h = silu(gate) * up;
-                        p.h[(int64_t)as * a.inner + f] = h;
-                        bits = __float_as_uint(h) & 0x7fffffffu;
-                    }
-#pragma unroll
-                    for (int o = 8; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
-                    if (j == 0 && c < en.count) atomicMax(p.counters + COUNTER_MAX + as, bits);
-                }
-                asm volatile("bar.sync 1, %0;" ::"n"(MATH_THREADS) : "memory");  // the sums have been read
             } else {
-                const uint32_t nth = (uint32_t)(u - u0);
-                const int part = k0 / p.part_k;
-                for (int i = threadIdx.x; i < 256 * groups; i += MATH_THREADS) {
-                    const int j = i & 31, c = i >> 5, n = tile * ROWS + j;
-                    float y = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < MATH_WARPS; ++w) y += s.sums[w][j][c];
-                    if (c < en.count && n < a.hidden) {
-                        const int as = s.order[en.first + c];
-                        y = y * s.back[which][c] * scale_at(a.down_scale, a.scale_type, (int64_t)en.expert * a.hidden + n) * __ldcg(a.weights + as);
-                        __stcg(p.pieces + ((int64_t)part * a.tokens * a.top + as) * a.hidden + n, y);
+                const Place<DOWN> end(s1 - 1, p, entries);
+                const Entry last = l.entry[end.entry];
+                for (int i = l.entry[start.entry].first + warp - 2; i < last.first + last.count; i += WARPS - 2) {
+                    const uint4 *x = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.x) + (int64_t)(l.order[i] / a.top) * a.x_stride);
+                    uint32_t bits = 0;
+#pragma unroll 4
+                    for (int j = lane; j < K / 8; j += 32) {
+                        const uint4 v = x[j];
+                        if constexpr (!DOWN) bits = X::largest(X::largest(X::largest(X::largest(bits, v.x), v.y), v.z), v.w);
                     }
+                    bits = __reduce_max_sync(0xffffffffu, bits);
+                    if (lane == 0) l.by[i] = power_for(bits, l.back[i]);
                 }
-                if (nth >= 2) wait(&s.freed[nth & 1], ((nth >> 1) - 1) & 1, 3);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&s.ready[nth & 1]));
-                asm volatile("bar.sync 1, %0;" ::"n"(MATH_THREADS) : "memory");
             }
         }
-    } else if (DOWN) {
-        // ---------------- finishing: who brings a column tile's last piece adds them up ----------------
-        pdl_wait();
-        const int ft = threadIdx.x - UP_THREADS;
-        for (int64_t u = u0; u < u1; ++u) {
-            const uint32_t nth = (uint32_t)(u - u0);
-            int k0, k1, tile, entry;
-            k_of(u, k0, k1, tile, entry);
-            wait(&s.ready[nth & 1], (nth >> 1) & 1, 4);
-            if (ft == 0) {
-                __threadfence();
-                const unsigned int pieces = (unsigned int)(s.entries * p.parts);
-                const bool last = atomicAdd(p.counters + tile, 1u) == pieces - 1;
-                if (last) p.counters[tile] = 0;
-                __threadfence();
-                s.last = last;
-            }
-            asm volatile("bar.sync 2, %0;" ::"n"(32 * FINISH_WARPS) : "memory");
-            if (s.last) {
-                const int n = tile * ROWS + (ft & 7) * 4;  // four columns a thread: hidden is a multiple of 16
-                for (int t = ft >> 3; t < a.tokens && n < a.hidden; t += 4 * FINISH_WARPS) {
-                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int j = 0; j < a.top; ++j) {
-                        const int as = t * a.top + j, e = __ldcg(a.experts + as);
-                        if (e < 0 || e >= a.count) continue;
-#pragma unroll 4
-                        for (int q = 0; q < p.parts; ++q) {
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(p.pieces + ((int64_t)q * a.tokens * a.top + as) * a.hidden + n));
-                            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        asm volatile("bar.sync 1, %0;" ::"n"(THREADS - 64) : "memory");
+        if (warp >= DIGIT_WARP0) {
+            // ---------------- digits ----------------
+            const int me = warp - DIGIT_WARP0;
+            Place<DOWN> at(s0 + me, p, entries);
+            // No more warps than stages: a wait tells a phase from its neighbours only, and a warp that has written its last stage knows that the one two rounds of the ring in front of its next has been read.
+            for (int i = me; i < mine && me < p.digit_warps; i += p.digit_warps) {
+                const Entry en = l.entry[at.entry];
+                const uint32_t slot = (uint32_t)i % stages, use = (uint32_t)i / stages;
+                unsigned char *tile = ring_gen + slot * stage_bytes + W_BYTES;
+                const int items = en.count * (BK / 16);  // 16 k of a column
+                bool waited = use == 0;
+                for (int j = lane; j < items || !waited; j += 32) {
+                    const int c = j / (BK / 16), chunk = j % (BK / 16), k = at.k * BK + chunk * 16;
+                    typename X::Raw raw;
+                    float by = 0.0f;
+                    if (j < items && k < K) {
+                        const int as = l.order[en.first + c];
+                        const void *row = DOWN ? static_cast<const void *>(p.h + (int64_t)as * K) : static_cast<const void *>(static_cast<const uint16_t *>(a.x) + (int64_t)(as / a.top) * a.x_stride);
+                        X::load(row, k, raw);
+                        by = l.by[en.first + c];
+                    } else {
+                        memset(raw, 0, sizeof(raw));
+                    }
+                    if (!waited) wait(&s.empty[slot], (use - 1) & 1, 2);
+                    waited = true;
+                    if (j < items) {
+                        uint32_t d[DIGITS][4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            float f[4];
+                            uint32_t w[DIGITS];
+                            widen4<X>(raw, q, f);
+                            digits_of(f, by, w);
+#pragma unroll
+                            for (int g = 0; g < DIGITS; ++g) d[g][q] = w[g];
+                        }
+#pragma unroll
+                        for (int g = 0; g < DIGITS; ++g) {
+                            const int row = g * p.per_entry + c;
+                            *reinterpret_cast<uint4 *>(tile + row * BK + ((chunk ^ (row & 7)) << 4)) = make_uint4(d[g][0], d[g][1], d[g][2], d[g][3]);
                         }
                     }
-                    store_result(a, t, n, sum.x), store_result(a, t, n + 1, sum.y), store_result(a, t, n + 2, sum.z), store_result(a, t, n + 3, sum.w);
                 }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s.tokens[slot]));
+                for (at.k += p.digit_warps; at.k >= p.k_blocks; at.k -= p.k_blocks) at.next_unit(p, entries);
             }
-            asm volatile("bar.sync 2, %0;" ::"n"(32 * FINISH_WARPS) : "memory");
-            if (ft == 0) mbar_arrive(smem_u32(&s.freed[nth & 1]));
+        } else if (warp >= FINISH_WARP0) {
+            // ---------------- results ----------------
+            const int q = warp - FINISH_WARP0, row = 32 * q + lane, C = p.per_entry;
+            const uint32_t lane_addr = tmem_base + ((uint32_t)(32 * q) << 16);
+            auto meet = [&]() { asm volatile("bar.sync 2, 128;" ::: "memory"); };
+            auto cta_of = [&](int64_t stage) { return (int)(((stage + 1) * ctas - 1) / total); };
+            // Who came to `counter` last of n: all threads' stores in front of it are seen by the last one's loads behind it.
+            auto came_last = [&](unsigned int *counter, int n) {
+                __threadfence();
+                meet();
+                if (row == 0) {
+                    const bool last = atomicAdd(counter, 1u) == (unsigned int)(n - 1);
+                    if (last) *counter = 0;
+                    s.last = last;
+                }
+                meet();
+                __threadfence();
+                return s.last != 0;
+            };
+            Place<DOWN> at = start;
+            uint32_t unit = 0;
+            for (int i = 0; i < mine; ++unit) {
+                const uint32_t buf = unit & 1;
+                const int first_k = at.k, steps = min(p.k_blocks - at.k, mine - i);
+                const Entry en = l.entry[at.entry];
+                const int n = at.tile * TN + row;
+                const bool there = n < rows;
+                const float scale = there ? scale_at(DOWN ? a.down_scale : a.gate_up_scale, a.scale_type, (int64_t)en.expert * rows + n) : 0.0f;
+                if (DOWN && (i == 0 || (at.entry == 0 && at.k == 0))) {
+                    for (int t = 0; t < a.tokens; ++t) l.sums[t * TN + row] = 0.0f;
+                }
+                wait(&s.acc_full[buf], (unit >> 1) & 1, 6);
+                umma::fence_after_sync();
+                const uint32_t acc = lane_addr + buf * p.columns;
+                int c0 = blockIdx.x, c1 = blockIdx.x;
+                bool finish = true;
+                if (!DOWN && steps < p.k_blocks) {
+                    // a unit of several CTAs: this one's sums to the others, and whoever comes last adds them
+                    const int64_t u = (s0 + i) / p.k_blocks;
+                    c0 = cta_of(u * p.k_blocks), c1 = cta_of((u + 1) * p.k_blocks - 1);
+                    int *to = static_cast<int *>(p.shared) + ((int64_t)blockIdx.x * 2 + (i > 0)) * p.columns * TN + row;
+                    for (int c = 0; c < en.count; c += 8) {
+                        int v[DIGITS][8];
+#pragma unroll
+                        for (int g = 0; g < DIGITS; ++g) ld_32x32b_x8(acc + g * C + c, v[g]);
+                        umma::ld_wait();
+#pragma unroll
+                        for (int g = 0; g < DIGITS; ++g)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if (c + j < en.count) __stcg(to + (g * C + c + j) * TN, v[g][j]);
+                    }
+                    finish = came_last(p.counters + COUNTER_UP + c0, c1 - c0 + 1);
+                }
+                for (int c = 0; finish && c < en.count; c += 8) {
+                    int v[DIGITS][8];
+#pragma unroll
+                    for (int g = 0; g < DIGITS; ++g) ld_32x32b_x8(acc + g * C + c, v[g]);
+                    umma::ld_wait();
+                    if (!DOWN) {
+                        for (int other = c0; other <= c1; ++other) {
+                            if (other == (int)blockIdx.x) continue;
+                            // the first of them has this unit last, the others first
+                            const int64_t u = (s0 + i) / p.k_blocks;
+                            const int *from = static_cast<const int *>(p.shared) + ((int64_t)other * 2 + (first_of(other) / p.k_blocks != u)) * p.columns * TN + row;
+#pragma unroll
+                            for (int g = 0; g < DIGITS; ++g)
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    if (c + j < en.count) v[g][j] += __ldcg(from + (g * C + c + j) * TN);
+                        }
+                    }
+                    float y[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        y[j] = fmaf((float)v[2][j], 65536.0f, fmaf((float)v[1][j], 256.0f, (float)v[0][j]));
+                        if (c + j < en.count) y[j] *= l.back[en.first + c + j] * scale;
+                    }
+                    if (DOWN) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            if (c + j < en.count) l.sums[l.order[en.first + c + j] / a.top * TN + row] += y[j] * l.share[en.first + c + j];
+                        }
+                    } else {
+                        // even lanes have gates, odd ones what they multiply; of two columns each lane of a pair finishes one
+                        const bool odd = lane & 1;
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2) {
+                            const float other = __shfl_xor_sync(0xffffffffu, odd ? y[j] : y[j + 1], 1);
+                            const int col = c + j + (odd ? 1 : 0);
+                            const float h = silu(odd ? other : y[j]) * (odd ? y[j + 1] : other);
+                            uint32_t bits = 0;
+                            int as = 0;
+                            if (col < en.count) {
+                                as = l.order[en.first + col];
+                                if (there) {
+                                    p.h[(int64_t)as * a.inner + (n >> 1)] = h;
+                                    bits = __float_as_uint(h) & 0x7fffffffu;
+                                }
+                            }
+                            const uint32_t even_most = __reduce_max_sync(0xffffffffu, odd ? 0u : bits), odd_most = __reduce_max_sync(0xffffffffu, odd ? bits : 0u);
+                            if (lane < 2 && col < en.count) atomicMax(p.counters + COUNTER_MAX + as, odd ? odd_most : even_most);
+                        }
+                    }
+                }
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s.acc_empty[buf]));
+                i += steps;
+                if (DOWN && (i == mine || (at.entry == entries - 1 && first_k + steps == p.k_blocks))) {
+                    // the tile's last stage, or this CTA's
+                    const int64_t t0 = (int64_t)at.tile * entries * p.k_blocks, t1 = t0 + (int64_t)entries * p.k_blocks;
+                    if (t0 >= s0 && t1 <= s1) {
+                        for (int t = 0; t < a.tokens && there; ++t) store_result(a, t, n, l.sums[t * TN + row]);
+                    } else {
+                        c0 = cta_of(t0), c1 = cta_of(t1 - 1);
+                        float *to = static_cast<float *>(p.shared) + ((int64_t)blockIdx.x * 2 + (t0 > s0)) * a.tokens * TN + row;
+                        for (int t = 0; t < a.tokens; ++t) __stcg(to + t * TN, l.sums[t * TN + row]);
+                        if (came_last(p.counters + COUNTER_DOWN + c0, c1 - c0 + 1) && row == 0) {
+                            int *add = s.add[s.to_add];
+                            add[0] = at.tile, add[1] = c0, add[2] = c1;
+                            ++s.to_add;
+                        }
+                    }
+                }
+                at.k = 0;
+                at.next_unit(p, entries);
+            }
         }
     }
+    // ---------------- the end ----------------
+    umma::fence_before_sync();
+    __syncthreads();
+    if (warp == MMA_WARP) {
+        umma::fence_after_sync();
+        umma::dealloc(tmem_base, p.tmem_cols);
+    }
     if (DOWN) {
-        if (units == 0) {  // nobody is anyone's: the residual, or zeros
+        // tiles of several CTAs whose last this one was: all warps, a token each, four columns a lane
+        for (int i = 0; i < s.to_add; ++i) {
+            const int tile = s.add[i][0], n = tile * TN + lane * 4;
+            const int64_t t0 = (int64_t)tile * entries * p.k_blocks;
+            for (int t = warp; t < a.tokens && n < a.hidden; t += WARPS) {  // hidden is a multiple of 16
+                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                for (int c = s.add[i][1]; c <= s.add[i][2]; ++c) {
+                    const bool second = t0 > first_of(c);
+                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.shared) + (((int64_t)c * 2 + second) * a.tokens + t) * TN + lane * 4));
+                    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+                }
+                store_result(a, t, n, sum.x), store_result(a, t, n + 1, sum.y), store_result(a, t, n + 2, sum.z), store_result(a, t, n + 3, sum.w);
+            }
+        }
+        if (total == 0) {  // nobody is anyone's: the residual, or zeros
             for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < (int64_t)a.tokens * a.hidden; i += (int64_t)gridDim.x * THREADS) store_result(a, (int)(i / a.hidden), (int)(i % a.hidden), 0.0f);
         }
         // the largest magnitudes are zero again when all CTAs have read them
-        __syncthreads();
         if (threadIdx.x == 0) {
             __threadfence();
             s.last = atomicAdd(p.counters + COUNTER_DONE, 1u) == gridDim.x - 1;
@@ -478,76 +597,60 @@ __global__ void __launch_bounds__(DOWN ? DOWN_THREADS : UP_THREADS, 1) experts_s
     }
 }
 
-template <int G, bool DOWN, typename X>
+int grid_of() {
+    const int sms = sm_count() > 0 ? sm_count() : 148;
+    return sms < MOST_CTAS ? sms : MOST_CTAS;
+}
+
+// Assignments of an entry: as many as there are tokens, where three digits of them fill sixteens of columns.
+int per_entry_of(int64_t tokens) { return tokens <= 5 ? 5 : tokens <= 10 ? 10 : tokens <= 16 ? 16 : tokens <= 32 ? 32 : 64; }
+int columns_of(int64_t tokens) { return (int)round_up(DIGITS * per_entry_of(tokens), 16); }
+
+template <bool DOWN, typename X>
 int launch_stream(const CUtensorMap &map, StreamArgs p, cudaStream_t stream) {
     const ExpertsArgs &a = p.a;
-    const int assignments = a.tokens * a.top;
-    const int shared = (int)sizeof(Shared<G>) + (int)sizeof(Entry) * assignments;
-    // two kernels side by side on an SM where that leaves four stages
-    const int most = 113 * 1024 - 1024 - shared >= 4 * STAGE_BYTES ? 113 * 1024 : 225 * 1024;
-    const int stages = (most - 1024 - shared) / STAGE_BYTES;
+    const int rows = DOWN ? a.hidden : 2 * a.inner, K = DOWN ? a.inner : a.hidden;
+    p.tiles = (int)ceil_div(rows, TN), p.k_blocks = (int)ceil_div(K, BK);
+    const int shared = (int)sizeof(Shared) + Lists::bytes(a.tokens * a.top, DOWN ? a.tokens : 0), stage = W_BYTES + p.columns * BK;
+    const int stages = (MOST_SMEM - 1024 - shared) / stage;
     p.stages = stages < MOST_STAGES ? stages : MOST_STAGES;
+    p.digit_warps = p.stages < DIGIT_WARPS ? p.stages : DIGIT_WARPS;
     static std::atomic<bool> attr_set[64];
-    const int rc = allow_smem(attr_set, experts_stream_kernel<G, DOWN, X>, 225 * 1024);
+    const int rc = allow_smem(attr_set, experts_stream_kernel<DOWN, X>, MOST_SMEM);
     if (rc != B200Q_OK) return rc;
-    const int grid = sm_count() > 0 ? sm_count() : 148;
-    return launch_after("experts_stream_kernel", experts_stream_kernel<G, DOWN, X>, dim3((unsigned)grid), DOWN ? DOWN_THREADS : UP_THREADS,
-                        (size_t)(1024 + p.stages * STAGE_BYTES + shared), 1, stream, map, p);
-}
-
-template <int G>
-int launch_both(const CUtensorMap &up, const CUtensorMap &down, StreamArgs p, cudaStream_t stream) {
-    StreamArgs first = p;
-    first.tiles = (int)ceil_div(2 * (int64_t)p.a.inner, ROWS), first.parts = 1, first.part_k = p.a.hidden;
-    const int rc = p.a.type == B200Q_F16 ? launch_stream<G, false, FromF16>(up, first, stream) : launch_stream<G, false, FromBF16>(up, first, stream);
-    return rc != B200Q_OK ? rc : launch_stream<G, true, FromF32>(down, p, stream);
-}
-
-// Parts of K of down: units enough for an equal share of every SM, two stages of K each at least.
-int parts_of(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top, int &part_k) {
-    const int64_t experts = count < tokens * top ? count : tokens * top, units = experts * ceil_div(hidden, ROWS);
-    int64_t parts = ceil_div(148 * 12, units > 0 ? units : 1);
-    const int64_t most = ceil_div(inner, 2 * STAGE_K);
-    if (parts > most) parts = most;
-    if (parts > 8) parts = 8;
-    if (parts < 1) parts = 1;
-    part_k = parts == 1 ? (int)inner : (int)round_up(ceil_div(inner, parts), STAGE_K);
-    return (int)ceil_div(inner, part_k);
+    return launch_after("experts_stream_kernel", experts_stream_kernel<DOWN, X>, dim3((unsigned)grid_of()), THREADS, (size_t)(1024 + p.stages * stage + shared), 1, stream, map, p);
 }
 
 }  // namespace
 
 bool experts_stream_supported(const ExpertsArgs &a) {
     return a.hidden % 16 == 0 && a.inner % 16 == 0 && a.inner > 0 && aligned_to(a.x, 16) && (a.tokens == 1 || a.x_stride % 8 == 0) && aligned_to(a.gate_up, 16) && aligned_to(a.down, 16) &&
-           a.count > 0 && a.count <= MOST_EXPERTS && a.top > 0 && a.top <= MOST_ASSIGNMENTS / 64 && a.hidden / ROWS < COUNTER_TILES && (int64_t)a.count * 2 * a.inner < 0x7fffff00LL &&
-           (int64_t)a.count * a.hidden < 0x7fffff00LL;
+           a.count > 0 && a.count <= MOST_EXPERTS && a.top > 0 && a.top <= MOST_ASSIGNMENTS / kExpertsTokens && a.hidden <= kMostExact && a.inner <= kMostExact &&
+           (int64_t)a.count * 2 * a.inner < 0x7fffff00LL && (int64_t)a.count * a.hidden < 0x7fffff00LL;
 }
 
-size_t experts_stream_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top) {
-    int64_t most = 0;
-    for (int64_t t : {tokens < kExpertsTokens ? tokens : kExpertsTokens, tokens % kExpertsTokens}) {
-        int part_k = 0;
-        const int64_t bytes = 4 * (round_up(t * top * inner, 64) + (t > 0 && inner > 0 ? parts_of(t, hidden, inner, count, top, part_k) : 0) * t * top * hidden);
-        if (bytes > most) most = bytes;
-    }
-    return (size_t)most;
+size_t experts_stream_bytes(int64_t tokens, int64_t inner, int64_t top) {
+    if (tokens > kExpertsTokens) tokens = kExpertsTokens;
+    const int64_t sums = columns_of(tokens), results = tokens;
+    return (size_t)(4 * (round_up(tokens * top * inner, 64) + (int64_t)grid_of() * 2 * TN * (sums > results ? sums : results)));
 }
 
-int launch_experts_stream(const ExpertsArgs &all, unsigned int *counters, float *scratch, cudaStream_t stream) {
+int launch_experts_stream(const ExpertsArgs &a, unsigned int *counters, float *scratch, cudaStream_t stream) {
     CUtensorMap up, down;
-    int rc = make_tensor_map_2d(&up, CU_TENSOR_MAP_DATA_TYPE_UINT8, all.gate_up, (uint64_t)all.hidden, (uint64_t)all.count * 2 * all.inner, (uint64_t)all.hidden, BOX_K, ROWS,
+    int rc = make_tensor_map_2d(&up, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.gate_up, (uint64_t)a.hidden, (uint64_t)a.count * 2 * a.inner, (uint64_t)a.hidden, BK, TN,
                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     if (rc != B200Q_OK) return rc;
-    rc = make_tensor_map_2d(&down, CU_TENSOR_MAP_DATA_TYPE_UINT8, all.down, (uint64_t)all.inner, (uint64_t)all.count * all.hidden, (uint64_t)all.inner, BOX_K, ROWS,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    rc = make_tensor_map_2d(&down, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.down, (uint64_t)a.inner, (uint64_t)a.count * a.hidden, (uint64_t)a.inner, BK, TN, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
     if (rc != B200Q_OK) return rc;
     StreamArgs p = {};
-    p.a = all;
-    const ExpertsArgs &a = p.a;
-    p.h = scratch, p.pieces = scratch + round_up((int64_t)a.tokens * a.top * a.inner, 64), p.counters = counters;
-    p.tiles = (int)ceil_div(a.hidden, ROWS);
-    p.parts = parts_of(a.tokens, a.hidden, a.inner, a.count, a.top, p.part_k);
-    return a.tokens <= 8 ? launch_both<1>(up, down, p, stream) : a.tokens <= 16 ? launch_both<2>(up, down, p, stream) : launch_both<4>(up, down, p, stream);
+    p.a = a;
+    p.h = scratch, p.shared = scratch + round_up((int64_t)a.tokens * a.top * a.inner, 64), p.counters = counters;
+    p.per_entry = per_entry_of(a.tokens), p.columns = columns_of(a.tokens);
+    p.tmem_cols = 32;
+    while ((int)p.tmem_cols < 2 * p.columns + 8) p.tmem_cols *= 2;  // eight columns are read at a time, some of them behind the last
+    rc = a.type == B200Q_F16 ? launch_stream<false, FromF16>(up, p, stream) : launch_stream<false, FromBF16>(up, p, stream);
+    return rc != B200Q_OK ? rc : launch_stream<true, FromF32>(down, p, stream);
 }
 
 }  // namespace b200q

@@ -54,13 +54,13 @@ def product(a, a_scale, weight, scale, layout, bias, residual, pairs, dtype):
 
 
 def experts(x, chosen, weights, gate_up, s1, down, s2, residual):
-    """(result, bound) of a layer of experts.  x is rounded to float16 at most 2^-39 of its row's largest element off; h by 2^-11 of itself and by 2^-39 of its row's largest; float sums of n
-    products by (n / 8 + 32) roundings of 2^-23 of their magnitudes (sums run eight or more products at a time)."""
+    """(result, bound) of a layer of experts.  x and h are at most 2^-22 of their row's largest element off (whole numbers of up to 2^22, at least 2^21 for the largest, rounded); what stands for the sum of
+    n products in float is off by no more than (n / 8 + 32) roundings of 2^-23 of their magnitudes (float sums run eight or more products at a time; whole ones are exact)."""
     rows, hidden = x.shape
     inner = down.shape[2]
     xd = x.double()
     out, bound = torch.zeros_like(xd), torch.zeros_like(xd)
-    dx = xd.abs().amax(-1, keepdim=True) * 2.0 ** -38
+    dx = xd.abs().amax(-1, keepdim=True) * 2.0 ** -22
     for e in range(down.shape[0]):
         share = torch.where(chosen == e, weights.double(), 0.0)
         token = (chosen == e).any(-1).nonzero()[:, 0]
@@ -71,7 +71,7 @@ def experts(x, chosen, weights, gate_up, s1, down, s2, residual):
         y = xd[token] @ w1.t()
         dy = xd[token].abs() @ w1.abs().t() * ((hidden / 8 + 32) * 2 * F32) + dx[token] * w1.abs().sum(1)
         h, dh = silu_mul(y[:, 0::2], y[:, 1::2], dy[:, 0::2], dy[:, 1::2])
-        dh = dh + (h.abs() + dh) * 2.0 ** -11 + (h.abs() + dh).amax(-1, keepdim=True) * 2.0 ** -38
+        dh = dh + (h.abs() + dh).amax(-1, keepdim=True) * 2.0 ** -22
         o = h @ w2.t()
         do = dh @ w2.abs().t() + (h.abs() + dh) @ w2.abs().t() * ((inner / 8 + 32) * 2 * F32)
         out[token] += share * o
