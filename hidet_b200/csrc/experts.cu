@@ -92,7 +92,7 @@ extern "C" {
 B200Q_API size_t b200q_mixture_of_experts_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top) {
     using namespace b200q;
     if (tokens <= 0 || hidden <= 0 || inner < 0 || count < 0 || top <= 0) return 0;
-    return kWorkspaceHead + experts_stream_bytes(tokens, inner, top);
+    return kWorkspaceHead + experts_stream_bytes(experts_at_once(tokens, top), inner, top);
 }
 
 B200Q_API int b200q_mixture_of_experts(const void *x, int64_t x_stride, const int32_t *experts, const float *weights, const void *gate_up, const void *gate_up_scale,
@@ -123,9 +123,10 @@ B200Q_API int b200q_mixture_of_experts(const void *x, int64_t x_stride, const in
     p.tokens = (int)tokens, p.hidden = (int)hidden, p.inner = (int)inner, p.count = (int)count, p.top = (int)top, p.scale_type = scale_type, p.type = type;
     p.status = device_status_word();
     float *scratch = reinterpret_cast<float *>(static_cast<char *>(workspace) + kWorkspaceHead);
-    for (int64_t t = 0; t < tokens; t += kExpertsTokens) {
+    const int64_t at_once = experts_at_once(tokens, top);
+    for (int64_t t = 0; t < tokens; t += at_once) {
         ExpertsArgs q = p;
-        q.tokens = (int)(tokens - t < kExpertsTokens ? tokens - t : kExpertsTokens);
+        q.tokens = (int)(tokens - t < at_once ? tokens - t : at_once);
         q.x = static_cast<const uint16_t *>(x) + t * x_stride, q.out = static_cast<uint16_t *>(out) + t * hidden;
         if (top > 0) q.experts = experts + t * top, q.weights = weights + t * top;
         if (residual != nullptr) q.residual = static_cast<const uint16_t *>(residual) + t * residual_stride;

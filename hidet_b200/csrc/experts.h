@@ -27,9 +27,15 @@ struct ExpertsArgs {
     unsigned int *status;
 };
 
-constexpr int64_t kExpertsTokens = 64;  // of one launch
+// Tokens of one launch: 64, or as many as have 1024 assignments.
+constexpr int64_t kExpertsTokens = 64, kExpertsAssignments = 1024;
+inline int64_t experts_at_once(int64_t tokens, int64_t top) {
+    int64_t most = top * kExpertsTokens > kExpertsAssignments ? kExpertsAssignments / top : kExpertsTokens;
+    if (most < 1) most = 1;
+    return tokens < most ? tokens : most;
+}
 
-// Rows and bases in lines of 16 bytes, up to 1024 experts, 32 a token.
+// Rows and bases in lines of 16 bytes, up to 1024 experts; tokens of one launch.
 bool experts_stream_supported(const ExpertsArgs &p);
 size_t experts_stream_bytes(int64_t tokens, int64_t inner, int64_t top);
 int launch_experts_stream(const ExpertsArgs &p, unsigned int *counters, float *scratch, cudaStream_t stream);

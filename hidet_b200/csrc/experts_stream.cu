@@ -12,7 +12,7 @@
 //     warp 0      copies the weights' tiles into a ring
 //     warp 1      issues the products, into two accumulators in turn
 //     warps 4-7   finish: tensor memory -> float -> h, or results
-//     warps 8-15  digits: take the ring's stages in turn and put the tokens' digits beside the weights' tile
+//     warps 8-15  digits: four teams take the ring's stages in turn and put the tokens' digits beside the weights' tile
 // Gate and up: rows (2 f, 2 f + 1) are neighbouring lanes; h = silu(g) u in float to global memory, and its largest magnitude per assignment, which is what down's
 // digits are scaled by.  A unit (an entry's 128 rows) that two or more CTAs share has its whole-number sums added by the one that comes last.
 // Down: a column tile's entries follow one another, and what a CTA has of them it adds up in float, times scales and weights, in their order; the CTA that comes last adds the
@@ -33,11 +33,11 @@ constexpr unsigned int kKernelExperts = 11;
 constexpr int TN = 128, BK = 128;         // rows and k of a stage
 constexpr int W_BYTES = TN * BK;
 constexpr int DIGITS = 3;
-constexpr int COPY_WARP = 0, MMA_WARP = 1, FINISH_WARP0 = 4, DIGIT_WARP0 = 8, DIGIT_WARPS = 8;
-constexpr int WARPS = 16, THREADS = 32 * WARPS;
+constexpr int COPY_WARP = 0, MMA_WARP = 1, FINISH_WARP0 = 4, DIGIT_WARP0 = 8, TEAM = 2, TEAMS = 4;
+constexpr int WARPS = DIGIT_WARP0 + TEAM * TEAMS, THREADS = 32 * WARPS;
 constexpr int MOST_STAGES = 10;
 constexpr int MOST_SMEM = 225 * 1024;
-constexpr int MOST_ASSIGNMENTS = 2048;    // of one launch
+constexpr int MOST_ASSIGNMENTS = kExpertsAssignments;
 constexpr int MOST_EXPERTS = 1024;
 constexpr int kMostExact = 131071;        // products of 2^14 whose sum 32 bits hold
 constexpr uint16_t kNone = 0xffff;
@@ -51,15 +51,17 @@ struct StreamArgs {
     unsigned int *counters;
     int tiles;            // of 128 rows, of an expert's weight
     int k_blocks;
-    int per_entry;        // C: assignments of an entry
-    int columns;          // 3 C, rounded up to 16
+    int most;             // assignments of an entry
     uint32_t tmem_cols;
-    int stages;
-    int digit_warps;      // that take stages in turn
+    int ring_bytes;
 };
 
+// What an entry's columns are laid out for: C assignments, whose digits of one rank stand side by side, and 3 C rounded up to 16 columns.
+__host__ __device__ __forceinline__ int columns_for(int count) { return count <= 5 ? 5 : count <= 10 ? 10 : count <= 16 ? 16 : count <= 32 ? 32 : 64; }
+__host__ __device__ __forceinline__ int sixteens(int c) { return (DIGITS * c + 15) / 16 * 16; }
+
 struct Entry {
-    int expert, first, count;  // its assignments are order[first ..]
+    uint16_t expert, first, count;  // its assignments are order[first ..]
 };
 
 __device__ __forceinline__ float scale_at(const void *p, int type, int64_t i) {
@@ -148,7 +150,7 @@ struct Shared {
     uint64_t weights[MOST_STAGES], tokens[MOST_STAGES], empty[MOST_STAGES];  // a stage's two operands are in place; its products are through
     uint64_t acc_full[2], acc_empty[2], drain;
     uint32_t tmem_base;
-    int abort_flag, entries, last, to_add;
+    int abort_flag, entries, largest, last, to_add;
     int add[2][3];  // (down) what this CTA adds up at the end: tile, first and last CTA
     int counts[MOST_EXPERTS];
 };
@@ -158,13 +160,13 @@ struct Lists {
     Entry *entry;
     uint16_t *chosen, *order;
     float *sums;
-    __host__ __device__ static constexpr int bytes(int n, int tokens) { return round16(12 * n) + round16(12 * n) + round16(4 * n) + tokens * TN * 4; }
+    __host__ __device__ static constexpr int bytes(int n, int tokens) { return round16(12 * n) + round16(6 * n) + round16(4 * n) + tokens * TN * 4; }
     __host__ __device__ static constexpr int round16(int b) { return (b + 15) / 16 * 16; }
     __device__ __forceinline__ Lists(unsigned char *at, int n) {
         by = reinterpret_cast<float *>(at), back = by + n, share = back + n;
         at += round16(12 * n);
         entry = reinterpret_cast<Entry *>(at);
-        at += round16(12 * n);
+        at += round16(6 * n);
         chosen = reinterpret_cast<uint16_t *>(at), order = chosen + n;
         sums = reinterpret_cast<float *>(at + round16(4 * n));
     }
@@ -185,7 +187,7 @@ __device__ void make_entries(const ExpertsArgs &a, int columns, Shared &s, const
     }
     __syncthreads();
     if (threadIdx.x < 32) {
-        int first = 0, entries = 0;  // assignments and entries of the experts so far
+        int first = 0, entries = 0, largest = 0;  // assignments and entries of the experts so far
         for (int e0 = 0; e0 < a.count; e0 += 32) {
             const int e = e0 + threadIdx.x, mine = e < a.count ? s.counts[e] : 0, my_entries = (mine + columns - 1) / columns;
             int at = mine, at_entry = my_entries;
@@ -194,11 +196,13 @@ __device__ void make_entries(const ExpertsArgs &a, int columns, Shared &s, const
                 const int x = __shfl_up_sync(0xffffffffu, at, o), y = __shfl_up_sync(0xffffffffu, at_entry, o);
                 if ((int)threadIdx.x >= o) at += x, at_entry += y;
             }
-            for (int i = 0; i < my_entries; ++i) l.entry[entries + at_entry - my_entries + i] = {e, first + at - mine + i * columns, min(columns, mine - i * columns)};
+            largest = max(largest, min(mine, columns));
+            for (int i = 0; i < my_entries; ++i) l.entry[entries + at_entry - my_entries + i] = {(uint16_t)e, (uint16_t)(first + at - mine + i * columns), (uint16_t)min(columns, mine - i * columns)};
             if (e < a.count) s.counts[e] = first + at - mine;
             first += __shfl_sync(0xffffffffu, at, 31), entries += __shfl_sync(0xffffffffu, at_entry, 31);
         }
-        if (threadIdx.x == 0) s.entries = entries;
+        largest = __reduce_max_sync(0xffffffffu, largest);
+        if (threadIdx.x == 0) s.entries = entries, s.largest = largest;
         __syncwarp();
         for (int i0 = 0; i0 < n; i0 += 32) {
             const int i = i0 + threadIdx.x;
@@ -251,17 +255,16 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
     extern __shared__ unsigned char smem_dyn[];
     const uint32_t ring = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char *ring_gen = smem_dyn + (ring - smem_u32(smem_dyn));
-    const uint32_t stages = p.stages, stage_bytes = W_BYTES + (uint32_t)p.columns * BK;
-    Shared &s = *reinterpret_cast<Shared *>(ring_gen + stages * stage_bytes);
+    Shared &s = *reinterpret_cast<Shared *>(ring_gen + p.ring_bytes);
     const ExpertsArgs &a = p.a;
     const Lists l(reinterpret_cast<unsigned char *>(&s + 1), a.tokens * a.top);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int K = DOWN ? a.inner : a.hidden, rows = DOWN ? a.hidden : 2 * a.inner;
 
     if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < stages; ++i) {
+        for (int i = 0; i < MOST_STAGES; ++i) {
             mbar_init(smem_u32(&s.weights[i]), 1);
-            mbar_init(smem_u32(&s.tokens[i]), 1);
+            mbar_init(smem_u32(&s.tokens[i]), TEAM);
             mbar_init(smem_u32(&s.empty[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -279,14 +282,19 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
     // The experts were chosen in front of gate and up, which waits for that before it lets down start: down may read them, and request weights, without waiting.
     if (!DOWN) pdl_wait();
     umma::fence_before_sync();
-    make_entries(a, p.per_entry, s, l);
+    make_entries(a, p.most, s, l);
     umma::fence_after_sync();
     pdl_launch_dependents();
     const uint32_t tmem_base = s.tmem_base;
     const int entries = s.entries;
-    const int64_t total = (int64_t)entries * p.tiles * p.k_blocks;
-    const int64_t ctas = total < gridDim.x ? (total > 0 ? total : 1) : gridDim.x;  // that have a part
-    auto first_of = [&](int64_t cta) { return cta < ctas ? total * cta / ctas : total; };
+    // Stages as large as the largest entry asks for, and as many as there is room for.
+    const int C = columns_for(s.largest), columns = sixteens(C);
+    const uint32_t stage_bytes = W_BYTES + (uint32_t)columns * BK, stages = min(MOST_STAGES, p.ring_bytes / stage_bytes);
+    const int64_t units = (int64_t)entries * p.tiles, total = units * p.k_blocks;
+    // Gate and up: whole units where the CTA with the most has hardly more than an equal part, whose pieces have to be brought together (which takes the time of some ten stages).
+    const bool whole = !DOWN && (units + gridDim.x - 1) / gridDim.x * p.k_blocks <= total / gridDim.x + 10;
+    const int64_t parts = whole ? units : total, ctas = parts < gridDim.x ? (parts > 0 ? parts : 1) : gridDim.x;  // CTAs that have a part
+    auto first_of = [&](int64_t cta) { return cta < ctas ? parts * cta / ctas * (whole ? p.k_blocks : 1) : total; };
     const int64_t s0 = first_of(blockIdx.x), s1 = first_of((int64_t)blockIdx.x + 1);
     const int mine = (int)(s1 - s0);  // stages of this CTA
     const Place<DOWN> start(s0, p, entries);
@@ -325,7 +333,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
     } else if (warp == MMA_WARP) {
         // ---------------- products ----------------
         if (elect_one()) {
-            const uint32_t idesc = idesc_i8(TN, p.columns);
+            const uint32_t idesc = idesc_i8(TN, columns);
             umma::Ring r;
             int k = start.k;
             uint32_t unit = 0;
@@ -333,7 +341,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                 const uint32_t buf = unit & 1;
                 if (unit >= 2) wait(&s.acc_empty[buf], ((unit >> 1) - 1) & 1, 3);
                 umma::fence_after_sync();
-                const uint32_t d = tmem_base + buf * p.columns;
+                const uint32_t d = tmem_base + buf * columns;
                 for (bool first = true; k < p.k_blocks && i < mine; ++k, ++i, first = false, r.advance(1, stages)) {
                     wait(&s.weights[r.slot], r.phase, 4);
                     wait(&s.tokens[r.slot], r.phase, 5);
@@ -382,69 +390,73 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
         asm volatile("bar.sync 1, %0;" ::"n"(THREADS - 64) : "memory");
         if (warp >= DIGIT_WARP0) {
             // ---------------- digits ----------------
-            const int me = warp - DIGIT_WARP0;
-            Place<DOWN> at(s0 + me, p, entries);
-            // No more warps than stages: a wait tells a phase from its neighbours only, and a warp that has written its last stage knows that the one two rounds of the ring in front of its next has been read.
-            for (int i = me; i < mine && me < p.digit_warps; i += p.digit_warps) {
+            // Teams of two warps take stages in turn.  No more teams than stages: a wait tells a phase from its neighbours only, and a team that has written its last stage
+            // knows that the one two rounds of the ring in front of its next has been read.
+            const int team = (warp - DIGIT_WARP0) / TEAM, me = (warp - DIGIT_WARP0) % TEAM * 32 + lane;
+            Place<DOWN> at(s0 + team, p, entries);
+            for (int i = team; i < mine; i += TEAMS) {
                 const Entry en = l.entry[at.entry];
                 const uint32_t slot = (uint32_t)i % stages, use = (uint32_t)i / stages;
                 unsigned char *tile = ring_gen + slot * stage_bytes + W_BYTES;
                 const int items = en.count * (BK / 16);  // 16 k of a column
-                bool waited = use == 0;
-                for (int j = lane; j < items || !waited; j += 32) {
-                    const int c = j / (BK / 16), chunk = j % (BK / 16), k = at.k * BK + chunk * 16;
-                    typename X::Raw raw;
-                    float by = 0.0f;
+                auto fetch = [&](int j, typename X::Raw &raw, float &by) {
+                    const int c = j / (BK / 16), k = at.k * BK + j % (BK / 16) * 16;
+                    by = 0.0f;
+                    memset(raw, 0, sizeof(raw));
                     if (j < items && k < K) {
                         const int as = l.order[en.first + c];
                         const void *row = DOWN ? static_cast<const void *>(p.h + (int64_t)as * K) : static_cast<const void *>(static_cast<const uint16_t *>(a.x) + (int64_t)(as / a.top) * a.x_stride);
                         X::load(row, k, raw);
                         by = l.by[en.first + c];
-                    } else {
-                        memset(raw, 0, sizeof(raw));
                     }
-                    if (!waited) wait(&s.empty[slot], (use - 1) & 1, 2);
-                    waited = true;
-                    if (j < items) {
-                        uint32_t d[DIGITS][4];
+                };
+                typename X::Raw raw, next;
+                float by, next_by;
+                fetch(me, raw, by);
+                if (use > 0) wait(&s.empty[slot], (use - 1) & 1, 2);
+                for (int j = me; j < items; j += 32 * TEAM) {
+                    fetch(j + 32 * TEAM, next, next_by);
+                    const int c = j / (BK / 16), chunk = j % (BK / 16);
+                    uint32_t d[DIGITS][4];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            float f[4];
-                            uint32_t w[DIGITS];
-                            widen4<X>(raw, q, f);
-                            digits_of(f, by, w);
+                    for (int q = 0; q < 4; ++q) {
+                        float f[4];
+                        uint32_t w[DIGITS];
+                        widen4<X>(raw, q, f);
+                        digits_of(f, by, w);
 #pragma unroll
-                            for (int g = 0; g < DIGITS; ++g) d[g][q] = w[g];
-                        }
-#pragma unroll
-                        for (int g = 0; g < DIGITS; ++g) {
-                            const int row = g * p.per_entry + c;
-                            *reinterpret_cast<uint4 *>(tile + row * BK + ((chunk ^ (row & 7)) << 4)) = make_uint4(d[g][0], d[g][1], d[g][2], d[g][3]);
-                        }
+                        for (int g = 0; g < DIGITS; ++g) d[g][q] = w[g];
                     }
+#pragma unroll
+                    for (int g = 0; g < DIGITS; ++g) {
+                        const int row = g * C + c;
+                        *reinterpret_cast<uint4 *>(tile + row * BK + ((chunk ^ (row & 7)) << 4)) = make_uint4(d[g][0], d[g][1], d[g][2], d[g][3]);
+                    }
+                    memcpy(raw, next, sizeof(raw));
+                    by = next_by;
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&s.tokens[slot]));
-                for (at.k += p.digit_warps; at.k >= p.k_blocks; at.k -= p.k_blocks) at.next_unit(p, entries);
+                for (at.k += TEAMS; at.k >= p.k_blocks; at.k -= p.k_blocks) at.next_unit(p, entries);
             }
         } else if (warp >= FINISH_WARP0) {
             // ---------------- results ----------------
-            const int q = warp - FINISH_WARP0, row = 32 * q + lane, C = p.per_entry;
+            const int q = warp - FINISH_WARP0, row = 32 * q + lane;
             const uint32_t lane_addr = tmem_base + ((uint32_t)(32 * q) << 16);
             auto meet = [&]() { asm volatile("bar.sync 2, 128;" ::: "memory"); };
             auto cta_of = [&](int64_t stage) { return (int)(((stage + 1) * ctas - 1) / total); };
-            // Who came to `counter` last of n: all threads' stores in front of it are seen by the last one's loads behind it.
+            // Who came to `counter` last of n: what all threads stored in front of it is seen by the last one's loads behind it.
             auto came_last = [&](unsigned int *counter, int n) {
-                __threadfence();
                 meet();
                 if (row == 0) {
-                    const bool last = atomicAdd(counter, 1u) == (unsigned int)(n - 1);
+                    unsigned int before;
+                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+                    const bool last = before == (unsigned int)(n - 1);
                     if (last) *counter = 0;
                     s.last = last;
                 }
                 meet();
-                __threadfence();
                 return s.last != 0;
             };
             Place<DOWN> at = start;
@@ -461,14 +473,14 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                 }
                 wait(&s.acc_full[buf], (unit >> 1) & 1, 6);
                 umma::fence_after_sync();
-                const uint32_t acc = lane_addr + buf * p.columns;
+                const uint32_t acc = lane_addr + buf * columns;
                 int c0 = blockIdx.x, c1 = blockIdx.x;
                 bool finish = true;
                 if (!DOWN && steps < p.k_blocks) {
                     // a unit of several CTAs: this one's sums to the others, and whoever comes last adds them
                     const int64_t u = (s0 + i) / p.k_blocks;
                     c0 = cta_of(u * p.k_blocks), c1 = cta_of((u + 1) * p.k_blocks - 1);
-                    int *to = static_cast<int *>(p.shared) + ((int64_t)blockIdx.x * 2 + (i > 0)) * p.columns * TN + row;
+                    int *to = static_cast<int *>(p.shared) + ((int64_t)blockIdx.x * 2 + (i > 0)) * columns * TN + row;
                     for (int c = 0; c < en.count; c += 8) {
                         int v[DIGITS][8];
 #pragma unroll
@@ -492,7 +504,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                             if (other == (int)blockIdx.x) continue;
                             // the first of them has this unit last, the others first
                             const int64_t u = (s0 + i) / p.k_blocks;
-                            const int *from = static_cast<const int *>(p.shared) + ((int64_t)other * 2 + (first_of(other) / p.k_blocks != u)) * p.columns * TN + row;
+                            const int *from = static_cast<const int *>(p.shared) + ((int64_t)other * 2 + (first_of(other) / p.k_blocks != u)) * columns * TN + row;
 #pragma unroll
                             for (int g = 0; g < DIGITS; ++g)
 #pragma unroll
@@ -602,36 +614,30 @@ int grid_of() {
     return sms < MOST_CTAS ? sms : MOST_CTAS;
 }
 
-// Assignments of an entry: as many as there are tokens, where three digits of them fill sixteens of columns.
-int per_entry_of(int64_t tokens) { return tokens <= 5 ? 5 : tokens <= 10 ? 10 : tokens <= 16 ? 16 : tokens <= 32 ? 32 : 64; }
-int columns_of(int64_t tokens) { return (int)round_up(DIGITS * per_entry_of(tokens), 16); }
-
 template <bool DOWN, typename X>
 int launch_stream(const CUtensorMap &map, StreamArgs p, cudaStream_t stream) {
     const ExpertsArgs &a = p.a;
     const int rows = DOWN ? a.hidden : 2 * a.inner, K = DOWN ? a.inner : a.hidden;
     p.tiles = (int)ceil_div(rows, TN), p.k_blocks = (int)ceil_div(K, BK);
-    const int shared = (int)sizeof(Shared) + Lists::bytes(a.tokens * a.top, DOWN ? a.tokens : 0), stage = W_BYTES + p.columns * BK;
-    const int stages = (MOST_SMEM - 1024 - shared) / stage;
-    p.stages = stages < MOST_STAGES ? stages : MOST_STAGES;
-    p.digit_warps = p.stages < DIGIT_WARPS ? p.stages : DIGIT_WARPS;
+    const int shared = (int)sizeof(Shared) + Lists::bytes(a.tokens * a.top, DOWN ? a.tokens : 0);
+    p.ring_bytes = (MOST_SMEM - 1024 - shared) / 1024 * 1024;
+    static_assert((MOST_SMEM - 2048 - (int)sizeof(Shared) - Lists::bytes(MOST_ASSIGNMENTS, kExpertsTokens)) / (W_BYTES + 192 * BK) >= TEAMS, "a stage for every team, whatever the sizes");
     static std::atomic<bool> attr_set[64];
     const int rc = allow_smem(attr_set, experts_stream_kernel<DOWN, X>, MOST_SMEM);
     if (rc != B200Q_OK) return rc;
-    return launch_after("experts_stream_kernel", experts_stream_kernel<DOWN, X>, dim3((unsigned)grid_of()), THREADS, (size_t)(1024 + p.stages * stage + shared), 1, stream, map, p);
+    return launch_after("experts_stream_kernel", experts_stream_kernel<DOWN, X>, dim3((unsigned)grid_of()), THREADS, (size_t)(1024 + p.ring_bytes + shared), 1, stream, map, p);
 }
 
 }  // namespace
 
 bool experts_stream_supported(const ExpertsArgs &a) {
     return a.hidden % 16 == 0 && a.inner % 16 == 0 && a.inner > 0 && aligned_to(a.x, 16) && (a.tokens == 1 || a.x_stride % 8 == 0) && aligned_to(a.gate_up, 16) && aligned_to(a.down, 16) &&
-           a.count > 0 && a.count <= MOST_EXPERTS && a.top > 0 && a.top <= MOST_ASSIGNMENTS / kExpertsTokens && a.hidden <= kMostExact && a.inner <= kMostExact &&
+           a.count > 0 && a.count <= MOST_EXPERTS && a.top > 0 && a.tokens * a.top <= MOST_ASSIGNMENTS && a.hidden <= kMostExact && a.inner <= kMostExact &&
            (int64_t)a.count * 2 * a.inner < 0x7fffff00LL && (int64_t)a.count * a.hidden < 0x7fffff00LL;
 }
 
 size_t experts_stream_bytes(int64_t tokens, int64_t inner, int64_t top) {
-    if (tokens > kExpertsTokens) tokens = kExpertsTokens;
-    const int64_t sums = columns_of(tokens), results = tokens;
+    const int64_t sums = sixteens(columns_for((int)tokens)), results = tokens;
     return (size_t)(4 * (round_up(tokens * top * inner, 64) + (int64_t)grid_of() * 2 * TN * (sums > results ? sums : results)));
 }
 
@@ -646,9 +652,9 @@ int launch_experts_stream(const ExpertsArgs &a, unsigned int *counters, float *s
     StreamArgs p = {};
     p.a = a;
     p.h = scratch, p.shared = scratch + round_up((int64_t)a.tokens * a.top * a.inner, 64), p.counters = counters;
-    p.per_entry = per_entry_of(a.tokens), p.columns = columns_of(a.tokens);
+    p.most = columns_for(a.tokens);
     p.tmem_cols = 32;
-    while ((int)p.tmem_cols < 2 * p.columns + 8) p.tmem_cols *= 2;  // eight columns are read at a time, some of them behind the last
+    while ((int)p.tmem_cols < 2 * sixteens(p.most) + 8) p.tmem_cols *= 2;  // eight columns are read at a time, some of them behind the last
     rc = a.type == B200Q_F16 ? launch_stream<false, FromF16>(up, p, stream) : launch_stream<false, FromBF16>(up, p, stream);
     return rc != B200Q_OK ? rc : launch_stream<true, FromF32>(down, p, stream);
 }
