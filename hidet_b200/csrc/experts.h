@@ -35,7 +35,7 @@ inline int64_t experts_at_once(int64_t tokens, int64_t top) {
     return tokens < most ? tokens : most;
 }
 
-// Rows and bases in lines of 16 bytes, up to 1024 experts; tokens of one launch.
+// Rows and bases in lines of 16 bytes, up to 512 experts; tokens of one launch.
 bool experts_stream_supported(const ExpertsArgs &p);
 size_t experts_stream_bytes(int64_t tokens, int64_t inner, int64_t top);
 int launch_experts_stream(const ExpertsArgs &p, unsigned int *counters, float *scratch, cudaStream_t stream);

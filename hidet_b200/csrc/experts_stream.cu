@@ -36,29 +36,31 @@ constexpr int DIGITS = 3;
 constexpr int COPY_WARP = 0, MMA_WARP = 1, FINISH_WARP0 = 4, DIGIT_WARP0 = 8, TEAM = 2, TEAMS = 4;
 constexpr int WARPS = DIGIT_WARP0 + TEAM * TEAMS, THREADS = 32 * WARPS;
 constexpr int MOST_STAGES = 10;
-constexpr int MOST_SMEM = 225 * 1024;
+constexpr int MOST_SMEM = 227 * 1024;
 constexpr int MOST_ASSIGNMENTS = kExpertsAssignments;
-constexpr int MOST_EXPERTS = 1024;
+constexpr int MOST_EXPERTS = 512;
 constexpr int kMostExact = 131071;        // products of 2^14 whose sum 32 bits hold
 constexpr uint16_t kNone = 0xffff;
 // what of the workspace's counters is whose: arrivals at what CTAs share (by the first of them), CTAs that are through, h's largest magnitudes
 constexpr int MOST_CTAS = 1024, COUNTER_UP = 0, COUNTER_DOWN = MOST_CTAS, COUNTER_DONE = 2 * MOST_CTAS, COUNTER_MAX = 4 * MOST_CTAS;
+
+constexpr int EARLY_TOKENS = 16;          // whose largest elements are sought before it is known which of them a CTA needs
 
 struct StreamArgs {
     ExpertsArgs a;
     float *h;             // [assignments, inner]
     void *shared;         // gate and up: int32 [CTAs][2][columns][128]; down: float [CTAs][2][tokens][128]
     unsigned int *counters;
-    int tiles;            // of 128 rows, of an expert's weight
-    int k_blocks;
+    uint32_t tiles;       // of 128 rows, of an expert's weight
+    uint32_t k_blocks;
     int most;             // assignments of an entry
     uint32_t tmem_cols;
     int ring_bytes;
 };
 
 // What an entry's columns are laid out for: C assignments, whose digits of one rank stand side by side, and 3 C rounded up to 16 columns.
-__host__ __device__ __forceinline__ int columns_for(int count) { return count <= 5 ? 5 : count <= 10 ? 10 : count <= 16 ? 16 : count <= 32 ? 32 : 64; }
-__host__ __device__ __forceinline__ int sixteens(int c) { return (DIGITS * c + 15) / 16 * 16; }
+__host__ __device__ constexpr int columns_for(int count) { return count <= 5 ? 5 : count <= 10 ? 10 : count <= 16 ? 16 : count <= 32 ? 32 : 64; }
+__host__ __device__ constexpr int sixteens(int c) { return (DIGITS * c + 15) / 16 * 16; }
 
 struct Entry {
     uint16_t expert, first, count;  // its assignments are order[first ..]
@@ -146,91 +148,123 @@ __device__ __forceinline__ void ld_32x32b_x8(uint32_t taddr, int (&v)[8]) {
                  : "memory");
 }
 
-struct Shared {
+struct alignas(16) Shared {
     uint64_t weights[MOST_STAGES], tokens[MOST_STAGES], empty[MOST_STAGES];  // a stage's two operands are in place; its products are through
     uint64_t acc_full[2], acc_empty[2], drain;
     uint32_t tmem_base;
     int abort_flag, entries, largest, last, to_add;
     int add[2][3];  // (down) what this CTA adds up at the end: tile, first and last CTA
-    int counts[MOST_EXPERTS];
+    int duplicates;
+    uint32_t bits[EARLY_TOKENS];
 };
-// Behind it: by, back, share [n] (float, of the assignments in their order), entry [n], chosen, order [n] (uint16), (down) sums [tokens][128] (float)
+// Behind it: counts [experts], who [experts] (the tokens of an expert, a bit each), by, back, share [n] (float, of the assignments in their order), entry [n], chosen, order, token [n] (uint16),
+// (down) sums [tokens][128] (float)
 struct Lists {
+    int *counts;
+    uint2 *who;
     float *by, *back, *share;
     Entry *entry;
-    uint16_t *chosen, *order;
+    uint16_t *chosen, *order, *token;
     float *sums;
-    __host__ __device__ static constexpr int bytes(int n, int tokens) { return round16(12 * n) + round16(6 * n) + round16(4 * n) + tokens * TN * 4; }
+    __host__ __device__ static constexpr int bytes(int n, int experts, int tokens) { return round16(12 * experts) + round16(12 * n) + round16(6 * n) + round16(6 * n) + tokens * TN * 4; }
     __host__ __device__ static constexpr int round16(int b) { return (b + 15) / 16 * 16; }
-    __device__ __forceinline__ Lists(unsigned char *at, int n) {
+    __device__ __forceinline__ Lists(unsigned char *at, int n, int experts) {
+        who = reinterpret_cast<uint2 *>(at), counts = reinterpret_cast<int *>(who + experts);
+        at += round16(12 * experts);
         by = reinterpret_cast<float *>(at), back = by + n, share = back + n;
         at += round16(12 * n);
         entry = reinterpret_cast<Entry *>(at);
         at += round16(6 * n);
-        chosen = reinterpret_cast<uint16_t *>(at), order = chosen + n;
-        sums = reinterpret_cast<float *>(at + round16(4 * n));
+        chosen = reinterpret_cast<uint16_t *>(at), order = chosen + n, token = order + n;
+        sums = reinterpret_cast<float *>(at + round16(6 * n));
     }
 };
 
-// The entries of a launch: counts by expert, a scan over the experts, assignments in their places.  Every CTA makes them for itself, so an expert's assignments stand in
-// their own order: as they come they would differ from CTA to CTA, and with them who is in which entry of an expert with several.
-__device__ void make_entries(const ExpertsArgs &a, int columns, Shared &s, const Lists &l) {
+// The entries of a launch: counts by expert and the tokens that they are of, a sum over the experts, assignments in their places.  Every CTA makes them for itself, so an
+// expert's assignments stand in their own order: as they come they would differ from CTA to CTA, and with them whose column is whose.  `meanwhile` runs while the experts are on their way.
+template <typename F>
+__device__ __forceinline__ void make_entries(const ExpertsArgs &a, int columns, Shared &s, const Lists &l, F meanwhile) {
     const int n = a.tokens * a.top;
-    for (int e = threadIdx.x; e < a.count; e += THREADS) s.counts[e] = 0;
+    for (int e = threadIdx.x; e < a.count; e += THREADS) l.counts[e] = 0, l.who[e] = make_uint2(0, 0);
+    if (threadIdx.x < EARLY_TOKENS) s.bits[threadIdx.x] = 0;
+    if (threadIdx.x == 0) s.duplicates = 0;
     __syncthreads();
+    meanwhile();
     for (int i = threadIdx.x; i < n; i += THREADS) {
-        const int e = __ldcg(a.experts + i);
+        const int e = __ldcg(a.experts + i), t = i / a.top;
         const bool there = e >= 0 && e < a.count;
         l.chosen[i] = there ? (uint16_t)e : kNone;
-        if (there) atomicAdd(&s.counts[e], 1);
-        else if (e >= 0 && blockIdx.x == 0 && a.status != nullptr) atomicOr(a.status, kBadExpert);
+        if (there) {
+            atomicAdd(&l.counts[e], 1);
+            const uint32_t bit = 1u << (t & 31);
+            if (atomicOr(t < 32 ? &l.who[e].x : &l.who[e].y, bit) & bit) s.duplicates = 1;
+        } else if (e >= 0 && blockIdx.x == 0 && a.status != nullptr) {
+            atomicOr(a.status, kBadExpert);
+        }
     }
     __syncthreads();
     if (threadIdx.x < 32) {
-        int first = 0, entries = 0, largest = 0;  // assignments and entries of the experts so far
-        for (int e0 = 0; e0 < a.count; e0 += 32) {
-            const int e = e0 + threadIdx.x, mine = e < a.count ? s.counts[e] : 0, my_entries = (mine + columns - 1) / columns;
-            int at = mine, at_entry = my_entries;
+        const int each = (a.count + 31) / 32, e0 = threadIdx.x * each, e1 = min(a.count, e0 + each);
+        int mine = 0, my_entries = 0, largest = 0;
+        for (int e = e0; e < e1; ++e) {
+            const int c = l.counts[e];
+            mine += c, my_entries += (c + columns - 1) / columns, largest = max(largest, min(c, columns));
+        }
+        int at = mine, at_entry = my_entries;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, at, o), y = __shfl_up_sync(0xffffffffu, at_entry, o);
-                if ((int)threadIdx.x >= o) at += x, at_entry += y;
-            }
-            largest = max(largest, min(mine, columns));
-            for (int i = 0; i < my_entries; ++i) l.entry[entries + at_entry - my_entries + i] = {(uint16_t)e, (uint16_t)(first + at - mine + i * columns), (uint16_t)min(columns, mine - i * columns)};
-            if (e < a.count) s.counts[e] = first + at - mine;
-            first += __shfl_sync(0xffffffffu, at, 31), entries += __shfl_sync(0xffffffffu, at_entry, 31);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, at, o), y = __shfl_up_sync(0xffffffffu, at_entry, o);
+            if ((int)threadIdx.x >= o) at += x, at_entry += y;
+        }
+        if (threadIdx.x == 31) s.entries = at_entry;
+        at -= mine, at_entry -= my_entries;
+        for (int e = e0; e < e1; ++e) {
+            const int c = l.counts[e];
+            l.counts[e] = at;
+            for (int i = 0; i < c; i += columns) l.entry[at_entry++] = {(uint16_t)e, (uint16_t)(at + i), (uint16_t)min(columns, c - i)};
+            at += c;
         }
         largest = __reduce_max_sync(0xffffffffu, largest);
-        if (threadIdx.x == 0) s.entries = entries, s.largest = largest;
+        if (threadIdx.x == 0) s.largest = largest;
         __syncwarp();
-        for (int i0 = 0; i0 < n; i0 += 32) {
-            const int i = i0 + threadIdx.x;
-            const uint32_t e = i < n ? l.chosen[i] : kNone, same = __match_any_sync(0xffffffffu, e);
-            const int place = e != kNone ? s.counts[e] : 0;
-            __syncwarp();
-            if (e != kNone) {
-                l.order[place + __popc(same & ((1u << threadIdx.x) - 1u))] = (uint16_t)i;
-                if ((same >> threadIdx.x) == 1u) s.counts[e] = place + __popc(same);  // the last of them
+        if (s.duplicates) {  // a token that has an expert twice: one assignment after the other
+            for (int i0 = 0; i0 < n; i0 += 32) {
+                const int i = i0 + threadIdx.x;
+                const uint32_t e = i < n ? l.chosen[i] : kNone, same = __match_any_sync(0xffffffffu, e);
+                const int place = e != kNone ? l.counts[e] : 0;
+                __syncwarp();
+                if (e != kNone) {
+                    const int to = place + __popc(same & ((1u << threadIdx.x) - 1u));
+                    l.order[to] = (uint16_t)i, l.token[to] = (uint16_t)(i / a.top);
+                    if ((same >> threadIdx.x) == 1u) l.counts[e] = place + __popc(same);  // the last of them
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
     }
     __syncthreads();
+    if (!s.duplicates) {
+        for (int i = threadIdx.x; i < n; i += THREADS) {
+            const uint32_t e = l.chosen[i], t = i / a.top;
+            if (e == kNone) continue;
+            const uint32_t before = (1u << (t & 31)) - 1u;
+            const int to = l.counts[e] + (t < 32 ? __popc(l.who[e].x & before) : __popc(l.who[e].x) + __popc(l.who[e].y & before));
+            l.order[to] = (uint16_t)i, l.token[to] = (uint16_t)t;
+        }
+        __syncthreads();
+    }
 }
 
 // Where a CTA is in its part of the stages.  Gate and up: k fastest, then an entry's tiles, then entries; down: k, then a tile's entries, then tiles.
 template <bool DOWN>
 struct Place {
-    int entry, tile, k;
-    __device__ __forceinline__ Place(int64_t stage, const StreamArgs &p, int entries) {
-        const int64_t u = stage / p.k_blocks;
-        const int inner = DOWN ? max(entries, 1) : p.tiles;
-        const int outer = (int)(u / inner), in = (int)(u - (int64_t)outer * inner);
-        k = (int)(stage - u * p.k_blocks);
+    uint32_t entry, tile, k;
+    __device__ __forceinline__ Place(uint32_t stage, const StreamArgs &p, uint32_t entries) {
+        const uint32_t u = stage / p.k_blocks, inner = DOWN ? max(entries, 1u) : p.tiles, outer = u / inner, in = u - outer * inner;
+        k = stage - u * p.k_blocks;
         entry = DOWN ? in : outer, tile = DOWN ? outer : in;
     }
-    __device__ __forceinline__ void next_unit(const StreamArgs &p, int entries) {
+    __device__ __forceinline__ void next_unit(const StreamArgs &p, uint32_t entries) {
         if (DOWN) {
             if (++entry == entries) entry = 0, ++tile;
         } else {
@@ -257,7 +291,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
     unsigned char *ring_gen = smem_dyn + (ring - smem_u32(smem_dyn));
     Shared &s = *reinterpret_cast<Shared *>(ring_gen + p.ring_bytes);
     const ExpertsArgs &a = p.a;
-    const Lists l(reinterpret_cast<unsigned char *>(&s + 1), a.tokens * a.top);
+    const Lists l(reinterpret_cast<unsigned char *>(&s + 1), a.tokens * a.top, a.count);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int K = DOWN ? a.inner : a.hidden, rows = DOWN ? a.hidden : 2 * a.inner;
 
@@ -282,20 +316,41 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
     // The experts were chosen in front of gate and up, which waits for that before it lets down start: down may read them, and request weights, without waiting.
     if (!DOWN) pdl_wait();
     umma::fence_before_sync();
-    make_entries(a, p.most, s, l);
+    // The largest magnitudes of a few tokens, a warp 1024 elements at a time, in front of the weights' requests, behind which they would wait.
+    make_entries(a, p.most, s, l, [&]() {
+        if constexpr (!DOWN) {
+            const int pieces = (K + 1023) / 1024;
+            for (int i = warp; a.tokens <= EARLY_TOKENS && i < a.tokens * pieces; i += WARPS) {
+                const int t = i / pieces, k = (i - t * pieces) * 1024 + lane * 8;
+                uint32_t bits = 0;
+                uint4 v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = make_uint4(0, 0, 0, 0);
+                    if (k + j * 256 < K) v[j] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.x) + t * a.x_stride + k + j * 256);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) bits = X::largest(X::largest(X::largest(X::largest(bits, v[j].x), v[j].y), v[j].z), v[j].w);
+                bits = __reduce_max_sync(0xffffffffu, bits);
+                if (lane == 0) atomicMax(&s.bits[t], bits);
+            }
+        }
+    });
     umma::fence_after_sync();
     pdl_launch_dependents();
     const uint32_t tmem_base = s.tmem_base;
-    const int entries = s.entries;
+    const uint32_t entries = s.entries;
     // Stages as large as the largest entry asks for, and as many as there is room for.
     const int C = columns_for(s.largest), columns = sixteens(C);
-    const uint32_t stage_bytes = W_BYTES + (uint32_t)columns * BK, stages = min(MOST_STAGES, p.ring_bytes / stage_bytes);
-    const int64_t units = (int64_t)entries * p.tiles, total = units * p.k_blocks;
+    const uint32_t stage_bytes = W_BYTES + (uint32_t)columns * BK, stages = min((uint32_t)MOST_STAGES, p.ring_bytes / stage_bytes);
+    const uint32_t units = entries * p.tiles, total = units * p.k_blocks;
     // Gate and up: whole units where the CTA with the most has hardly more than an equal part, whose pieces have to be brought together (which takes the time of some ten stages).
     const bool whole = !DOWN && (units + gridDim.x - 1) / gridDim.x * p.k_blocks <= total / gridDim.x + 10;
-    const int64_t parts = whole ? units : total, ctas = parts < gridDim.x ? (parts > 0 ? parts : 1) : gridDim.x;  // CTAs that have a part
-    auto first_of = [&](int64_t cta) { return cta < ctas ? parts * cta / ctas * (whole ? p.k_blocks : 1) : total; };
-    const int64_t s0 = first_of(blockIdx.x), s1 = first_of((int64_t)blockIdx.x + 1);
+    // A part of CTA c: `each` pieces, and one of the `more` that are left.  (Divisions of 64 bits took 2 us of a kernel's start, and more at its end.)
+    const uint32_t pieces = whole ? units : total, step = whole ? p.k_blocks : 1, each = pieces / gridDim.x, more = pieces - each * gridDim.x;
+    auto first_of = [&](uint32_t c) { return (c * each + min(c, more)) * step; };
+    auto cta_of = [&](uint32_t stage) { return stage < more * (each + 1) ? stage / (each + 1) : more + (stage - more * (each + 1)) / each; };  // of parts by stages
+    const uint32_t s0 = first_of(blockIdx.x), s1 = first_of(blockIdx.x + 1);
     const int mine = (int)(s1 - s0);  // stages of this CTA
     const Place<DOWN> start(s0, p, entries);
 
@@ -321,7 +376,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                 if (*reinterpret_cast<volatile int *>(&s.abort_flag) != 0) break;
                 const uint32_t bar = smem_u32(&s.weights[r.slot]);
                 mbar_expect_tx(bar, W_BYTES);
-                tma_load_2d_hint(ring + r.slot * stage_bytes, &map_w, at.k * BK, l.entry[at.entry].expert * rows + at.tile * TN, bar, once);
+                tma_load_2d_hint(ring + r.slot * stage_bytes, &map_w, at.k * BK, (int)(l.entry[at.entry].expert * (uint32_t)rows + at.tile * TN), bar, once);
                 if (++at.k == p.k_blocks) at.k = 0, at.next_unit(p, entries);
             }
             // every copy armed has landed before the CTA may retire
@@ -335,8 +390,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
         if (elect_one()) {
             const uint32_t idesc = idesc_i8(TN, columns);
             umma::Ring r;
-            int k = start.k;
-            uint32_t unit = 0;
+            uint32_t k = start.k, unit = 0;
             for (int i = 0; i < mine;) {
                 const uint32_t buf = unit & 1;
                 if (unit >= 2) wait(&s.acc_empty[buf], ((unit >> 1) - 1) & 1, 3);
@@ -374,16 +428,20 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
             } else {
                 const Place<DOWN> end(s1 - 1, p, entries);
                 const Entry last = l.entry[end.entry];
-                for (int i = l.entry[start.entry].first + warp - 2; i < last.first + last.count; i += WARPS - 2) {
-                    const uint4 *x = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.x) + (int64_t)(l.order[i] / a.top) * a.x_stride);
-                    uint32_t bits = 0;
-#pragma unroll 4
-                    for (int j = lane; j < K / 8; j += 32) {
-                        const uint4 v = x[j];
-                        if constexpr (!DOWN) bits = X::largest(X::largest(X::largest(X::largest(bits, v.x), v.y), v.z), v.w);
+                if (a.tokens <= EARLY_TOKENS) {
+                    for (int i = l.entry[start.entry].first + threadIdx.x - 64; i < last.first + last.count; i += THREADS - 64) l.by[i] = power_for(s.bits[l.token[i]], l.back[i]);
+                } else {
+                    for (int i = l.entry[start.entry].first + warp - 2; i < last.first + last.count; i += WARPS - 2) {
+                        const uint4 *x = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.x) + (int64_t)l.token[i] * a.x_stride);
+                        uint32_t bits = 0;
+#pragma unroll 8
+                        for (int j = lane; j < K / 8; j += 32) {
+                            const uint4 v = x[j];
+                            if constexpr (!DOWN) bits = X::largest(X::largest(X::largest(X::largest(bits, v.x), v.y), v.z), v.w);
+                        }
+                        bits = __reduce_max_sync(0xffffffffu, bits);
+                        if (lane == 0) l.by[i] = power_for(bits, l.back[i]);
                     }
-                    bits = __reduce_max_sync(0xffffffffu, bits);
-                    if (lane == 0) l.by[i] = power_for(bits, l.back[i]);
                 }
             }
         }
@@ -394,28 +452,36 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
             // knows that the one two rounds of the ring in front of its next has been read.
             const int team = (warp - DIGIT_WARP0) / TEAM, me = (warp - DIGIT_WARP0) % TEAM * 32 + lane;
             Place<DOWN> at(s0 + team, p, entries);
+            auto fetch = [&](const Entry &en, uint32_t k_block, int j, typename X::Raw &raw, float &by) {  // 16 k of a column
+                const int c = j / (BK / 16), k = (int)k_block * BK + j % (BK / 16) * 16;
+                by = 0.0f;
+                memset(raw, 0, sizeof(raw));
+                if (c < en.count && k < K) {
+                    const void *row = DOWN ? static_cast<const void *>(p.h + (int64_t)l.order[en.first + c] * K)
+                                           : static_cast<const void *>(static_cast<const uint16_t *>(a.x) + (int64_t)l.token[en.first + c] * a.x_stride);
+                    X::load(row, k, raw);
+                    by = l.by[en.first + c];
+                }
+            };
+            // What a stage needs first is asked for a stage of the team ahead.
+            typename X::Raw raw, next;
+            float by = 0.0f, next_by = 0.0f;
+            Entry en = {0, 0, 0};
+            if (team < mine) {
+                en = l.entry[at.entry];
+                fetch(en, at.k, me, raw, by);
+            }
             for (int i = team; i < mine; i += TEAMS) {
-                const Entry en = l.entry[at.entry];
-                const uint32_t slot = (uint32_t)i % stages, use = (uint32_t)i / stages;
+                const uint32_t slot = (uint32_t)i % stages, use = (uint32_t)i / stages, k_block = at.k;
+                const Entry here = en;
                 unsigned char *tile = ring_gen + slot * stage_bytes + W_BYTES;
-                const int items = en.count * (BK / 16);  // 16 k of a column
-                auto fetch = [&](int j, typename X::Raw &raw, float &by) {
-                    const int c = j / (BK / 16), k = at.k * BK + j % (BK / 16) * 16;
-                    by = 0.0f;
-                    memset(raw, 0, sizeof(raw));
-                    if (j < items && k < K) {
-                        const int as = l.order[en.first + c];
-                        const void *row = DOWN ? static_cast<const void *>(p.h + (int64_t)as * K) : static_cast<const void *>(static_cast<const uint16_t *>(a.x) + (int64_t)(as / a.top) * a.x_stride);
-                        X::load(row, k, raw);
-                        by = l.by[en.first + c];
-                    }
-                };
-                typename X::Raw raw, next;
-                float by, next_by;
-                fetch(me, raw, by);
+                for (at.k += TEAMS; at.k >= p.k_blocks; at.k -= p.k_blocks) at.next_unit(p, entries);
+                if (i + TEAMS < mine) en = l.entry[at.entry];
                 if (use > 0) wait(&s.empty[slot], (use - 1) & 1, 2);
-                for (int j = me; j < items; j += 32 * TEAM) {
-                    fetch(j + 32 * TEAM, next, next_by);
+                for (int j = me; j < here.count * (BK / 16); j += 32 * TEAM) {
+                    const bool more_here = j + 32 * TEAM < here.count * (BK / 16);
+                    if (more_here) fetch(here, k_block, j + 32 * TEAM, next, next_by);
+                    else if (i + TEAMS < mine) fetch(en, at.k, me, next, next_by);
                     const int c = j / (BK / 16), chunk = j % (BK / 16);
                     uint32_t d[DIGITS][4];
 #pragma unroll
@@ -435,17 +501,16 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                     memcpy(raw, next, sizeof(raw));
                     by = next_by;
                 }
+                if (me >= here.count * (BK / 16) && i + TEAMS < mine) fetch(en, at.k, me, raw, by);  // nothing here, perhaps something there
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&s.tokens[slot]));
-                for (at.k += TEAMS; at.k >= p.k_blocks; at.k -= p.k_blocks) at.next_unit(p, entries);
             }
         } else if (warp >= FINISH_WARP0) {
             // ---------------- results ----------------
             const int q = warp - FINISH_WARP0, row = 32 * q + lane;
             const uint32_t lane_addr = tmem_base + ((uint32_t)(32 * q) << 16);
             auto meet = [&]() { asm volatile("bar.sync 2, 128;" ::: "memory"); };
-            auto cta_of = [&](int64_t stage) { return (int)(((stage + 1) * ctas - 1) / total); };
             // Who came to `counter` last of n: what all threads stored in front of it is seen by the last one's loads behind it.
             auto came_last = [&](unsigned int *counter, int n) {
                 meet();
@@ -463,7 +528,8 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
             uint32_t unit = 0;
             for (int i = 0; i < mine; ++unit) {
                 const uint32_t buf = unit & 1;
-                const int first_k = at.k, steps = min(p.k_blocks - at.k, mine - i);
+                const uint32_t first_k = at.k;
+                const int steps = min((int)(p.k_blocks - at.k), mine - i);
                 const Entry en = l.entry[at.entry];
                 const int n = at.tile * TN + row;
                 const bool there = n < rows;
@@ -474,12 +540,12 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                 wait(&s.acc_full[buf], (unit >> 1) & 1, 6);
                 umma::fence_after_sync();
                 const uint32_t acc = lane_addr + buf * columns;
-                int c0 = blockIdx.x, c1 = blockIdx.x;
+                uint32_t c0 = blockIdx.x, c1 = blockIdx.x;
                 bool finish = true;
-                if (!DOWN && steps < p.k_blocks) {
+                if (!DOWN && steps < (int)p.k_blocks) {
                     // a unit of several CTAs: this one's sums to the others, and whoever comes last adds them
-                    const int64_t u = (s0 + i) / p.k_blocks;
-                    c0 = cta_of(u * p.k_blocks), c1 = cta_of((u + 1) * p.k_blocks - 1);
+                    const uint32_t u0 = s0 + i - first_k;
+                    c0 = cta_of(u0), c1 = cta_of(u0 + p.k_blocks - 1);
                     int *to = static_cast<int *>(p.shared) + ((int64_t)blockIdx.x * 2 + (i > 0)) * columns * TN + row;
                     for (int c = 0; c < en.count; c += 8) {
                         int v[DIGITS][8];
@@ -492,7 +558,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                             for (int j = 0; j < 8; ++j)
                                 if (c + j < en.count) __stcg(to + (g * C + c + j) * TN, v[g][j]);
                     }
-                    finish = came_last(p.counters + COUNTER_UP + c0, c1 - c0 + 1);
+                    finish = came_last(p.counters + COUNTER_UP + c0, (int)(c1 - c0 + 1));
                 }
                 for (int c = 0; finish && c < en.count; c += 8) {
                     int v[DIGITS][8];
@@ -500,11 +566,10 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                     for (int g = 0; g < DIGITS; ++g) ld_32x32b_x8(acc + g * C + c, v[g]);
                     umma::ld_wait();
                     if (!DOWN) {
-                        for (int other = c0; other <= c1; ++other) {
-                            if (other == (int)blockIdx.x) continue;
+                        for (uint32_t other = c0; other <= c1; ++other) {
+                            if (other == blockIdx.x) continue;
                             // the first of them has this unit last, the others first
-                            const int64_t u = (s0 + i) / p.k_blocks;
-                            const int *from = static_cast<const int *>(p.shared) + ((int64_t)other * 2 + (first_of(other) / p.k_blocks != u)) * columns * TN + row;
+                            const int *from = static_cast<const int *>(p.shared) + ((int64_t)other * 2 + (first_of(other) < s0 + i - first_k)) * columns * TN + row;
 #pragma unroll
                             for (int g = 0; g < DIGITS; ++g)
 #pragma unroll
@@ -521,7 +586,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                     if (DOWN) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            if (c + j < en.count) l.sums[l.order[en.first + c + j] / a.top * TN + row] += y[j] * l.share[en.first + c + j];
+                            if (c + j < en.count) l.sums[l.token[en.first + c + j] * TN + row] += y[j] * l.share[en.first + c + j];
                         }
                     } else {
                         // even lanes have gates, odd ones what they multiply; of two columns each lane of a pair finishes one
@@ -549,18 +614,18 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&s.acc_empty[buf]));
                 i += steps;
-                if (DOWN && (i == mine || (at.entry == entries - 1 && first_k + steps == p.k_blocks))) {
+                if (DOWN && (i == mine || (at.entry == entries - 1 && first_k + (uint32_t)steps == p.k_blocks))) {
                     // the tile's last stage, or this CTA's
-                    const int64_t t0 = (int64_t)at.tile * entries * p.k_blocks, t1 = t0 + (int64_t)entries * p.k_blocks;
+                    const uint32_t t0 = at.tile * entries * p.k_blocks, t1 = t0 + entries * p.k_blocks;
                     if (t0 >= s0 && t1 <= s1) {
                         for (int t = 0; t < a.tokens && there; ++t) store_result(a, t, n, l.sums[t * TN + row]);
                     } else {
                         c0 = cta_of(t0), c1 = cta_of(t1 - 1);
                         float *to = static_cast<float *>(p.shared) + ((int64_t)blockIdx.x * 2 + (t0 > s0)) * a.tokens * TN + row;
                         for (int t = 0; t < a.tokens; ++t) __stcg(to + t * TN, l.sums[t * TN + row]);
-                        if (came_last(p.counters + COUNTER_DOWN + c0, c1 - c0 + 1) && row == 0) {
+                        if (came_last(p.counters + COUNTER_DOWN + c0, (int)(c1 - c0 + 1)) && row == 0) {
                             int *add = s.add[s.to_add];
-                            add[0] = at.tile, add[1] = c0, add[2] = c1;
+                            add[0] = (int)at.tile, add[1] = (int)c0, add[2] = (int)c1;
                             ++s.to_add;
                         }
                     }
@@ -581,14 +646,19 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
         // tiles of several CTAs whose last this one was: all warps, a token each, four columns a lane
         for (int i = 0; i < s.to_add; ++i) {
             const int tile = s.add[i][0], n = tile * TN + lane * 4;
-            const int64_t t0 = (int64_t)tile * entries * p.k_blocks;
+            const uint32_t t0 = (uint32_t)tile * entries * p.k_blocks;
             for (int t = warp; t < a.tokens && n < a.hidden; t += WARPS) {  // hidden is a multiple of 16
                 float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                for (int c = s.add[i][1]; c <= s.add[i][2]; ++c) {
-                    const bool second = t0 > first_of(c);
-                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.shared) + (((int64_t)c * 2 + second) * a.tokens + t) * TN + lane * 4));
-                    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+                for (int c = s.add[i][1]; c <= s.add[i][2]; c += 12) {
+                    float4 v[12];
+#pragma unroll
+                    for (int j = 0; j < 12; ++j) {
+                        v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        const bool second = t0 > first_of(c + j);
+                        if (c + j <= s.add[i][2]) v[j] = __ldcg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.shared) + (((int64_t)(c + j) * 2 + second) * a.tokens + t) * TN + lane * 4));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 12; ++j) sum.x += v[j].x, sum.y += v[j].y, sum.z += v[j].z, sum.w += v[j].w;
                 }
                 store_result(a, t, n, sum.x), store_result(a, t, n + 1, sum.y), store_result(a, t, n + 2, sum.z), store_result(a, t, n + 3, sum.w);
             }
@@ -618,10 +688,11 @@ template <bool DOWN, typename X>
 int launch_stream(const CUtensorMap &map, StreamArgs p, cudaStream_t stream) {
     const ExpertsArgs &a = p.a;
     const int rows = DOWN ? a.hidden : 2 * a.inner, K = DOWN ? a.inner : a.hidden;
-    p.tiles = (int)ceil_div(rows, TN), p.k_blocks = (int)ceil_div(K, BK);
-    const int shared = (int)sizeof(Shared) + Lists::bytes(a.tokens * a.top, DOWN ? a.tokens : 0);
+    p.tiles = (uint32_t)ceil_div(rows, TN), p.k_blocks = (uint32_t)ceil_div(K, BK);
+    const int shared = (int)sizeof(Shared) + Lists::bytes(a.tokens * a.top, a.count, DOWN ? a.tokens : 0);
     p.ring_bytes = (MOST_SMEM - 1024 - shared) / 1024 * 1024;
-    static_assert((MOST_SMEM - 2048 - (int)sizeof(Shared) - Lists::bytes(MOST_ASSIGNMENTS, kExpertsTokens)) / (W_BYTES + 192 * BK) >= TEAMS, "a stage for every team, whatever the sizes");
+    static_assert((MOST_SMEM - 2048 - (int)sizeof(Shared) - Lists::bytes(MOST_ASSIGNMENTS, MOST_EXPERTS, kExpertsTokens)) / (W_BYTES + sixteens(columns_for(kExpertsTokens)) * BK) >= TEAMS,
+                  "a stage for every team, whatever the sizes");
     static std::atomic<bool> attr_set[64];
     const int rc = allow_smem(attr_set, experts_stream_kernel<DOWN, X>, MOST_SMEM);
     if (rc != B200Q_OK) return rc;

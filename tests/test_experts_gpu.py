@@ -93,7 +93,7 @@ def check_layer(x, experts, weights, *w, residual=None):
 
 @pytest.mark.parametrize('dtype,scale_dtype', [(F16, F16), (BF16, F32), (BF16, BF16)])
 @pytest.mark.parametrize('tokens,count,top,hidden,inner', [(1, 8, 2, 512, 1024), (1, 1, 1, 16, 16), (2, 4, 2, 1040, 272), (5, 16, 4, 256, 768), (8, 2, 2, 512, 528), (9, 3, 1, 144, 2064),
-                                                         (17, 8, 2, 1024, 512), (33, 64, 6, 512, 176), (64, 4, 2, 256, 512), (64, 2, 2, 1024, 256), (65, 4, 3, 256, 128), (150, 8, 2, 128, 64), (3, 200, 8, 384, 96), (40, 40, 32, 256, 64), (40, 8, 2, 4096, 1024), (6, 8, 2, 2048, 1536)])
+                                                         (17, 8, 2, 1024, 512), (33, 64, 6, 512, 176), (64, 4, 2, 256, 512), (64, 2, 2, 1024, 256), (65, 4, 3, 256, 128), (150, 8, 2, 128, 64), (3, 200, 8, 384, 96), (2, 600, 4, 64, 32), (40, 40, 32, 256, 64), (40, 8, 2, 4096, 1024), (6, 8, 2, 2048, 1536)])
 def test_layer(tokens, count, top, hidden, inner, dtype, scale_dtype):
     gen = generator(tokens, count, hidden)
     x = normal(gen, tokens, hidden, dtype=dtype)
