@@ -8,11 +8,11 @@
 // stream stood at 3.2 TB/s.)
 //
 // Every CTA makes the list of entries, an expert with up to C of its assignments (an expert with more has several entries), and takes an equal, contiguous part of
-// all stages, 128 rows x 128 k each.  16 warps:
+// all stages, 128 rows x 128 k each.  Warps:
 //     warp 0      copies the weights' tiles into a ring
 //     warp 1      issues the products, into two accumulators in turn
 //     warps 4-7   finish: tensor memory -> float -> h, or results
-//     warps 8-15  digits: four teams take the ring's stages in turn and put the tokens' digits beside the weights' tile
+//     the others  digits: four teams take the ring's stages in turn and put the tokens' digits beside the weights' tile
 // Gate and up: rows (2 f, 2 f + 1) are neighbouring lanes; h = silu(g) u in float to global memory, and its largest magnitude per assignment, which is what down's
 // digits are scaled by.  A unit (an entry's 128 rows) that two or more CTAs share has its whole-number sums added by the one that comes last.
 // Down: a column tile's entries follow one another, and what a CTA has of them it adds up in float, times scales and weights, in their order; the CTA that comes last adds the
@@ -22,6 +22,8 @@
 //
 // Waits are bounded: one that runs out is reported and raises a flag, after which nobody in the CTA waits or copies any more; everyone goes through the motions
 // to the end, so that no barrier is left alone.
+#include <type_traits>
+
 #include "experts.h"
 #include "serving.cuh"
 #include "umma.cuh"
@@ -33,8 +35,12 @@ constexpr unsigned int kKernelExperts = 11;
 constexpr int TN = 128, BK = 128;         // rows and k of a stage
 constexpr int W_BYTES = TN * BK;
 constexpr int DIGITS = 3;
-constexpr int COPY_WARP = 0, MMA_WARP = 1, FINISH_WARP0 = 4, DIGIT_WARP0 = 8, TEAM = 2, TEAMS = 4;
-constexpr int WARPS = DIGIT_WARP0 + TEAM * TEAMS, THREADS = 32 * WARPS;
+constexpr int COPY_WARP = 0, MMA_WARP = 1, FINISH_WARP0 = 4, DIGIT_WARP0 = 8, TEAMS = 4;
+constexpr int ITEMS = BK / 8;             // of a column in a stage, a thread's eight elements each
+// Warps of a team: with more than a dozen assignments an expert, whose rows come from L2, four keep enough of them on their way (64 tokens, two of eight experts: 350 us with two, 281
+// with four); with fewer they are in each other's way (32 tokens: 235 and 248).
+constexpr int MANY = 12;
+__host__ __device__ constexpr int threads_of(int team) { return 32 * (DIGIT_WARP0 + team * TEAMS); }
 constexpr int MOST_STAGES = 10;
 constexpr int MOST_SMEM = 227 * 1024;
 constexpr int MOST_ASSIGNMENTS = kExpertsAssignments;
@@ -80,13 +86,10 @@ __device__ __forceinline__ float power_for(uint32_t bits, float &inverse) {
     return zero || bits >= 0x7f800000u ? 0.0f : __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-// 16 neighbouring elements of a token.
+// Eight neighbouring elements of a token.
 struct FromF16 {
-    typedef uint4 Raw[2];
-    static __device__ __forceinline__ void load(const void *row, int64_t k, Raw &r) {
-        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const __half *>(row) + k);
-        r[0] = p[0], r[1] = p[1];
-    }
+    typedef uint4 Raw[1];
+    static __device__ __forceinline__ void load(const void *row, int k, Raw &r) { r[0] = *reinterpret_cast<const uint4 *>(static_cast<const __half *>(row) + k); }
     static __device__ __forceinline__ void widen(uint32_t w, float &lo, float &hi) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
         lo = f.x, hi = f.y;
@@ -96,24 +99,22 @@ struct FromF16 {
     }
 };
 struct FromBF16 {
-    typedef uint4 Raw[2];
-    static __device__ __forceinline__ void load(const void *row, int64_t k, Raw &r) { FromF16::load(row, k, r); }
+    typedef uint4 Raw[1];
+    static __device__ __forceinline__ void load(const void *row, int k, Raw &r) { FromF16::load(row, k, r); }
     static __device__ __forceinline__ void widen(uint32_t w, float &lo, float &hi) { lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u); }
     static __device__ __forceinline__ uint32_t largest(uint32_t bits, uint32_t w) { return max(bits, max(w << 16 & 0x7fff0000u, w & 0x7fff0000u)); }
 };
 struct FromF32 {
-    typedef uint4 Raw[4];
-    static __device__ __forceinline__ void load(const void *row, int64_t k, Raw &r) {
+    typedef uint4 Raw[2];
+    static __device__ __forceinline__ void load(const void *row, int k, Raw &r) {
         const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const float *>(row) + k);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = p[i];
+        r[0] = p[0], r[1] = p[1];
     }
 };
 template <typename X>
 __device__ __forceinline__ void widen4(const typename X::Raw &r, int i, float (&f)[4]) {
-    const uint4 v = r[i >> 1];
-    X::widen(i & 1 ? v.z : v.x, f[0], f[1]);
-    X::widen(i & 1 ? v.w : v.y, f[2], f[3]);
+    X::widen(i ? r[0].z : r[0].x, f[0], f[1]);
+    X::widen(i ? r[0].w : r[0].y, f[2], f[3]);
 }
 template <>
 __device__ __forceinline__ void widen4<FromF32>(const FromF32::Raw &r, int i, float (&f)[4]) {
@@ -141,7 +142,10 @@ __device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_
         "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void ld_32x32b_x8(uint32_t taddr, int (&v)[8]) {
+__device__ __forceinline__ void ld_columns(uint32_t taddr, int (&v)[2]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void ld_columns(uint32_t taddr, int (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                  : "r"(taddr)
@@ -182,7 +186,7 @@ struct Lists {
 
 // The entries of a launch: counts by expert and the tokens that they are of, a sum over the experts, assignments in their places.  Every CTA makes them for itself, so an
 // expert's assignments stand in their own order: as they come they would differ from CTA to CTA, and with them whose column is whose.  `meanwhile` runs while the experts are on their way.
-template <typename F>
+template <int THREADS, typename F>
 __device__ __forceinline__ void make_entries(const ExpertsArgs &a, int columns, Shared &s, const Lists &l, F meanwhile) {
     const int n = a.tokens * a.top;
     for (int e = threadIdx.x; e < a.count; e += THREADS) l.counts[e] = 0, l.who[e] = make_uint2(0, 0);
@@ -284,8 +288,9 @@ __device__ __forceinline__ void store_result(const ExpertsArgs &a, int t, int n,
 }
 
 // X: what the tokens are; DOWN: h, else x.
-template <bool DOWN, typename X>
-__global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid_constant__ CUtensorMap map_w, const StreamArgs p) {
+template <bool DOWN, int TEAM, typename X>
+__global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(const __grid_constant__ CUtensorMap map_w, const StreamArgs p) {
+    constexpr int THREADS = threads_of(TEAM), WARPS = THREADS / 32;
     extern __shared__ unsigned char smem_dyn[];
     const uint32_t ring = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char *ring_gen = smem_dyn + (ring - smem_u32(smem_dyn));
@@ -317,7 +322,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
     if (!DOWN) pdl_wait();
     umma::fence_before_sync();
     // The largest magnitudes of a few tokens, a warp 1024 elements at a time, in front of the weights' requests, behind which they would wait.
-    make_entries(a, p.most, s, l, [&]() {
+    make_entries<THREADS>(a, p.most, s, l, [&]() {
         if constexpr (!DOWN) {
             const int pieces = (K + 1023) / 1024;
             for (int i = warp; a.tokens <= EARLY_TOKENS && i < a.tokens * pieces; i += WARPS) {
@@ -452,8 +457,8 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
             // knows that the one two rounds of the ring in front of its next has been read.
             const int team = (warp - DIGIT_WARP0) / TEAM, me = (warp - DIGIT_WARP0) % TEAM * 32 + lane;
             Place<DOWN> at(s0 + team, p, entries);
-            auto fetch = [&](const Entry &en, uint32_t k_block, int j, typename X::Raw &raw, float &by) {  // 16 k of a column
-                const int c = j / (BK / 16), k = (int)k_block * BK + j % (BK / 16) * 16;
+            auto fetch = [&](const Entry &en, uint32_t k_block, int j, typename X::Raw &raw, float &by) {  // eight k of a column
+                const int c = j / ITEMS, k = (int)k_block * BK + j % ITEMS * 8;
                 by = 0.0f;
                 memset(raw, 0, sizeof(raw));
                 if (c < en.count && k < K) {
@@ -478,36 +483,34 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                 for (at.k += TEAMS; at.k >= p.k_blocks; at.k -= p.k_blocks) at.next_unit(p, entries);
                 if (i + TEAMS < mine) en = l.entry[at.entry];
                 if (use > 0) wait(&s.empty[slot], (use - 1) & 1, 2);
-                for (int j = me; j < here.count * (BK / 16); j += 32 * TEAM) {
-                    const bool more_here = j + 32 * TEAM < here.count * (BK / 16);
+                for (int j = me; j < here.count * ITEMS; j += 32 * TEAM) {
+                    const bool more_here = j + 32 * TEAM < here.count * ITEMS;
                     if (more_here) fetch(here, k_block, j + 32 * TEAM, next, next_by);
                     else if (i + TEAMS < mine) fetch(en, at.k, me, next, next_by);
-                    const int c = j / (BK / 16), chunk = j % (BK / 16);
-                    uint32_t d[DIGITS][4];
+                    const int c = j / ITEMS, place = j % ITEMS;
+                    uint32_t d[2][DIGITS];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
+                    for (int q = 0; q < 2; ++q) {
                         float f[4];
-                        uint32_t w[DIGITS];
                         widen4<X>(raw, q, f);
-                        digits_of(f, by, w);
-#pragma unroll
-                        for (int g = 0; g < DIGITS; ++g) d[g][q] = w[g];
+                        digits_of(f, by, d[q]);
                     }
 #pragma unroll
                     for (int g = 0; g < DIGITS; ++g) {
                         const int row = g * C + c;
-                        *reinterpret_cast<uint4 *>(tile + row * BK + ((chunk ^ (row & 7)) << 4)) = make_uint4(d[g][0], d[g][1], d[g][2], d[g][3]);
+                        *reinterpret_cast<uint2 *>(tile + row * BK + (((place >> 1) ^ (row & 7)) << 4) + (place & 1) * 8) = make_uint2(d[0][g], d[1][g]);
                     }
                     memcpy(raw, next, sizeof(raw));
                     by = next_by;
                 }
-                if (me >= here.count * (BK / 16) && i + TEAMS < mine) fetch(en, at.k, me, raw, by);  // nothing here, perhaps something there
+                if (me >= here.count * ITEMS && i + TEAMS < mine) fetch(en, at.k, me, raw, by);  // nothing here, perhaps something there
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&s.tokens[slot]));
             }
         } else if (warp >= FINISH_WARP0) {
             // ---------------- results ----------------
+            constexpr int WIDE = TEAM == 4 ? 8 : 2;  // columns at a time
             const int q = warp - FINISH_WARP0, row = 32 * q + lane;
             const uint32_t lane_addr = tmem_base + ((uint32_t)(32 * q) << 16);
             auto meet = [&]() { asm volatile("bar.sync 2, 128;" ::: "memory"); };
@@ -547,23 +550,26 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
                     const uint32_t u0 = s0 + i - first_k;
                     c0 = cta_of(u0), c1 = cta_of(u0 + p.k_blocks - 1);
                     int *to = static_cast<int *>(p.shared) + ((int64_t)blockIdx.x * 2 + (i > 0)) * columns * TN + row;
-                    for (int c = 0; c < en.count; c += 8) {
-                        int v[DIGITS][8];
+#pragma unroll 1
+                    for (int c = 0; c < en.count; c += WIDE) {
+                        int v[DIGITS][WIDE];
 #pragma unroll
-                        for (int g = 0; g < DIGITS; ++g) ld_32x32b_x8(acc + g * C + c, v[g]);
+                        for (int g = 0; g < DIGITS; ++g) ld_columns(acc + g * C + c, v[g]);
                         umma::ld_wait();
 #pragma unroll
                         for (int g = 0; g < DIGITS; ++g)
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
+                            for (int j = 0; j < WIDE; ++j)
                                 if (c + j < en.count) __stcg(to + (g * C + c + j) * TN, v[g][j]);
                     }
                     finish = came_last(p.counters + COUNTER_UP + c0, (int)(c1 - c0 + 1));
                 }
-                for (int c = 0; finish && c < en.count; c += 8) {
-                    int v[DIGITS][8];
+                // With few columns two at a time: the code is short, and most of its first run is waiting for it.
+#pragma unroll 1
+                for (int c = 0; finish && c < en.count; c += WIDE) {
+                    int v[DIGITS][WIDE];
 #pragma unroll
-                    for (int g = 0; g < DIGITS; ++g) ld_32x32b_x8(acc + g * C + c, v[g]);
+                    for (int g = 0; g < DIGITS; ++g) ld_columns(acc + g * C + c, v[g]);
                     umma::ld_wait();
                     if (!DOWN) {
                         for (uint32_t other = c0; other <= c1; ++other) {
@@ -573,26 +579,26 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
 #pragma unroll
                             for (int g = 0; g < DIGITS; ++g)
 #pragma unroll
-                                for (int j = 0; j < 8; ++j)
+                                for (int j = 0; j < WIDE; ++j)
                                     if (c + j < en.count) v[g][j] += __ldcg(from + (g * C + c + j) * TN);
                         }
                     }
-                    float y[8];
+                    float y[WIDE];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < WIDE; ++j) {
                         y[j] = fmaf((float)v[2][j], 65536.0f, fmaf((float)v[1][j], 256.0f, (float)v[0][j]));
                         if (c + j < en.count) y[j] *= l.back[en.first + c + j] * scale;
                     }
                     if (DOWN) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
+                        for (int j = 0; j < WIDE; ++j) {
                             if (c + j < en.count) l.sums[l.token[en.first + c + j] * TN + row] += y[j] * l.share[en.first + c + j];
                         }
                     } else {
                         // even lanes have gates, odd ones what they multiply; of two columns each lane of a pair finishes one
                         const bool odd = lane & 1;
 #pragma unroll
-                        for (int j = 0; j < 8; j += 2) {
+                        for (int j = 0; j < WIDE; j += 2) {
                             const float other = __shfl_xor_sync(0xffffffffu, odd ? y[j] : y[j + 1], 1);
                             const int col = c + j + (odd ? 1 : 0);
                             const float h = silu(odd ? other : y[j]) * (odd ? y[j + 1] : other);
@@ -647,21 +653,40 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
         for (int i = 0; i < s.to_add; ++i) {
             const int tile = s.add[i][0], n = tile * TN + lane * 4;
             const uint32_t t0 = (uint32_t)tile * entries * p.k_blocks;
-            for (int t = warp; t < a.tokens && n < a.hidden; t += WARPS) {  // hidden is a multiple of 16
-                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int c = s.add[i][1]; c <= s.add[i][2]; c += 12) {
-                    float4 v[12];
+            // ROWS tokens of a warp, and ABREAST CTAs' parts of each, are asked for at once
+            auto add_up = [&](auto rows_at_once, auto abreast) {
+                constexpr int ROWS = decltype(rows_at_once)::value, ABREAST = decltype(abreast)::value;
+                for (int t = warp; t < a.tokens && n < a.hidden; t += ROWS * WARPS) {  // hidden is a multiple of 16
+                    float4 sum[ROWS];
 #pragma unroll
-                    for (int j = 0; j < 12; ++j) {
-                        v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        const bool second = t0 > first_of(c + j);
-                        if (c + j <= s.add[i][2]) v[j] = __ldcg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.shared) + (((int64_t)(c + j) * 2 + second) * a.tokens + t) * TN + lane * 4));
+                    for (int r = 0; r < ROWS; ++r) sum[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+                    for (int c = s.add[i][1]; c <= s.add[i][2]; c += ABREAST) {
+                        float4 v[ABREAST][ROWS];
+#pragma unroll
+                        for (int j = 0; j < ABREAST; ++j) {
+                            const bool second = t0 > first_of(c + j);
+                            const float *from = static_cast<const float *>(p.shared) + ((int64_t)(c + j) * 2 + second) * a.tokens * TN + lane * 4;
+#pragma unroll
+                            for (int r = 0; r < ROWS; ++r) {
+                                v[j][r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                if (c + j <= s.add[i][2] && t + r * WARPS < a.tokens) v[j][r] = __ldcg(reinterpret_cast<const float4 *>(from + (t + r * WARPS) * TN));
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < ABREAST; ++j)
+#pragma unroll
+                            for (int r = 0; r < ROWS; ++r) sum[r].x += v[j][r].x, sum[r].y += v[j][r].y, sum[r].z += v[j][r].z, sum[r].w += v[j][r].w;
                     }
 #pragma unroll
-                    for (int j = 0; j < 12; ++j) sum.x += v[j].x, sum.y += v[j].y, sum.z += v[j].z, sum.w += v[j].w;
+                    for (int r = 0; r < ROWS; ++r) {
+                        const int row = t + r * WARPS;
+                        if (row < a.tokens) store_result(a, row, n, sum[r].x), store_result(a, row, n + 1, sum[r].y), store_result(a, row, n + 2, sum[r].z), store_result(a, row, n + 3, sum[r].w);
+                    }
                 }
-                store_result(a, t, n, sum.x), store_result(a, t, n + 1, sum.y), store_result(a, t, n + 2, sum.z), store_result(a, t, n + 3, sum.w);
-            }
+            };
+            if (a.tokens <= WARPS) add_up(std::integral_constant<int, 1>(), std::integral_constant<int, 12>());
+            else add_up(std::integral_constant<int, 3>(), std::integral_constant<int, 4>());
         }
         if (total == 0) {  // nobody is anyone's: the residual, or zeros
             for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < (int64_t)a.tokens * a.hidden; i += (int64_t)gridDim.x * THREADS) store_result(a, (int)(i / a.hidden), (int)(i % a.hidden), 0.0f);
@@ -684,7 +709,7 @@ int grid_of() {
     return sms < MOST_CTAS ? sms : MOST_CTAS;
 }
 
-template <bool DOWN, typename X>
+template <bool DOWN, int TEAM, typename X>
 int launch_stream(const CUtensorMap &map, StreamArgs p, cudaStream_t stream) {
     const ExpertsArgs &a = p.a;
     const int rows = DOWN ? a.hidden : 2 * a.inner, K = DOWN ? a.inner : a.hidden;
@@ -694,9 +719,15 @@ int launch_stream(const CUtensorMap &map, StreamArgs p, cudaStream_t stream) {
     static_assert((MOST_SMEM - 2048 - (int)sizeof(Shared) - Lists::bytes(MOST_ASSIGNMENTS, MOST_EXPERTS, kExpertsTokens)) / (W_BYTES + sixteens(columns_for(kExpertsTokens)) * BK) >= TEAMS,
                   "a stage for every team, whatever the sizes");
     static std::atomic<bool> attr_set[64];
-    const int rc = allow_smem(attr_set, experts_stream_kernel<DOWN, X>, MOST_SMEM);
+    const int rc = allow_smem(attr_set, experts_stream_kernel<DOWN, TEAM, X>, MOST_SMEM);
     if (rc != B200Q_OK) return rc;
-    return launch_after("experts_stream_kernel", experts_stream_kernel<DOWN, X>, dim3((unsigned)grid_of()), THREADS, (size_t)(1024 + p.ring_bytes + shared), 1, stream, map, p);
+    return launch_after("experts_stream_kernel", experts_stream_kernel<DOWN, TEAM, X>, dim3((unsigned)grid_of()), threads_of(TEAM), (size_t)(1024 + p.ring_bytes + shared), 1, stream, map, p);
+}
+
+template <int TEAM>
+int launch_both(const CUtensorMap &up, const CUtensorMap &down, const StreamArgs &p, cudaStream_t stream) {
+    const int rc = p.a.type == B200Q_F16 ? launch_stream<false, TEAM, FromF16>(up, p, stream) : launch_stream<false, TEAM, FromBF16>(up, p, stream);
+    return rc != B200Q_OK ? rc : launch_stream<true, TEAM, FromF32>(down, p, stream);
 }
 
 }  // namespace
@@ -725,9 +756,8 @@ int launch_experts_stream(const ExpertsArgs &a, unsigned int *counters, float *s
     p.h = scratch, p.shared = scratch + round_up((int64_t)a.tokens * a.top * a.inner, 64), p.counters = counters;
     p.most = columns_for(a.tokens);
     p.tmem_cols = 32;
-    while ((int)p.tmem_cols < 2 * sixteens(p.most) + 8) p.tmem_cols *= 2;  // eight columns are read at a time, some of them behind the last
-    rc = a.type == B200Q_F16 ? launch_stream<false, FromF16>(up, p, stream) : launch_stream<false, FromBF16>(up, p, stream);
-    return rc != B200Q_OK ? rc : launch_stream<true, FromF32>(down, p, stream);
+    while ((int)p.tmem_cols < 2 * sixteens(p.most) + 8) p.tmem_cols *= 2;  // up to eight columns are read at a time, some of them behind the last
+    return (int64_t)a.tokens * a.top > (int64_t)MANY * a.count ? launch_both<4>(up, down, p, stream) : launch_both<2>(up, down, p, stream);
 }
 
 }  // namespace b200q
