@@ -3,16 +3,16 @@
 //     l[e] = sum_h x[h] r[e, h];   the `top` largest l, equal ones by index;   weight_j = exp(l_j - m) / sum exp(l - m)
 // over the chosen ones or over all, m the largest.  In float.
 //
-// A cluster of eight CTAs has up to four tokens; each CTA has every eighth expert, and a warp an expert (or, where there are fewer experts than
-// warps, a part of one's row).  So a row of the router is read once for four tokens and all of a cluster's logits meet in the first CTA's
-// shared memory, where a warp a token puts them in order.  A decode step's router is some KB to MB in L2: what takes the time is
-// latency (launch, a row, the cluster's barrier, the choices one after the other).
+// Up to four tokens have a cluster of up to eight CTAs, a warp two experts at a time (or, of few experts, a share of their rows): a row of the router is read once for four tokens, a token's
+// element is widened once for two experts, and all logits meet in the first CTA's shared memory, where a warp a token puts them in order, every lane with its experts' keys
+// in registers.  A decode step's router is some KB to MB in L2: what takes the time is latency (launch, a row, the cluster's barrier, the choices one after the
+// other), so loads are asked for eight at a time.  One token, 8 experts, rows of 4096: 3.0 us; 7 tokens, 64 of 2048: 6.2; 48 tokens, 128 of 2048: 10.8.
 #include "serving.cuh"
 
 namespace b200q {
 namespace {
 
-constexpr int WARPS = 8, THREADS = 32 * WARPS, CLUSTER = 8;
+constexpr int WARPS = 8, THREADS = 32 * WARPS, MOST_CLUSTER = 8;
 constexpr int MOST_EXPERTS = 1024, MOST_TOKENS = 4, MOST_TOP = 32;
 
 struct RouteArgs {
@@ -20,9 +20,8 @@ struct RouteArgs {
     int64_t x_stride;
     int32_t *experts;
     float *weights;
-    int tokens, width, count, top;
+    int tokens, width, count, top, cluster;
     bool all;           // weights over all experts
-    bool vec_x, vec_r;
 };
 
 __device__ __forceinline__ uint32_t ordered(float v) {  // NaN is the largest, -0 is 0
@@ -30,9 +29,9 @@ __device__ __forceinline__ uint32_t ordered(float v) {  // NaN is the largest, -
     return v != v ? 0xffffffffu : b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-template <typename T>
-__device__ __forceinline__ void load_some(const T *p, int left, bool vec, float (&f)[8]) {
-    if (left >= 8 && vec) {
+template <bool VEC, typename T>
+__device__ __forceinline__ void load_some(const T *p, int left, float (&f)[8]) {
+    if (VEC) {
         const Pack8<T> x = load8<T, true>(p);
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = Elems<T>::one(x.v[i]);
@@ -42,118 +41,123 @@ __device__ __forceinline__ void load_some(const T *p, int left, bool vec, float 
     }
 }
 
-template <typename T, typename R>
+// The `top` largest of a token's logits, by a warp; lane l has experts l, l + 32, .. and their keys, zero for none and for the ones that are taken.
+template <int EACH>
+__device__ __forceinline__ void choose(const RouteArgs &p, const float *l, int64_t row, int lane) {
+    uint32_t key[EACH];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int e = lane + 32 * i;
+        const float v = e < p.count ? l[e] : 0.0f;
+        bad |= v != v;
+        key[i] = e < p.count ? ordered(v) : 0u;
+    }
+    int mine = -1;  // lane j: the j-th choice
+    for (int j = 0; j < p.top; ++j) {
+        uint32_t best = 0, place = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (key[i] > best) best = key[i], place = lane + 32 * i;
+        const uint32_t top = __reduce_max_sync(0xffffffffu, best), e = __reduce_min_sync(0xffffffffu, best == top ? place : 0x7fffffffu);
+        if (lane == j) mine = (int)e;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (lane + 32 * i == (int)e) key[i] = 0;
+    }
+    const float v = mine >= 0 ? l[mine] : 0.0f, m = __shfl_sync(0xffffffffu, v, 0);
+    const float share = mine >= 0 ? expf(v - m) : 0.0f;
+    float total = share;
+    if (p.all) {
+        total = 0.0f;
+        for (int e = lane; e < p.count; e += 32) total += expf(l[e] - m);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    // a logit that is no number makes its token's weights none, also where it was not chosen
+    if (__any_sync(0xffffffffu, bad)) total = __uint_as_float(0x7fc00000u);
+    if (mine >= 0) {
+        p.experts[row + lane] = mine;
+        p.weights[row + lane] = __fdiv_rn(share, total);
+    }
+}
+
+// VEC: rows of tokens and router are whole vectors of eight elements on 16-byte boundaries.
+template <typename T, typename R, bool VEC>
 __global__ void __launch_bounds__(THREADS) route_kernel(const RouteArgs p) {
-    __shared__ float parts[WARPS][MOST_TOKENS];
     __shared__ float logits[MOST_TOKENS][MOST_EXPERTS];  // of the cluster's first CTA: all experts
+    __shared__ float parts[WARPS][2][MOST_TOKENS];
     const uint32_t rank = cluster_ctarank();
-    const int first = (int)(blockIdx.x / CLUSTER) * MOST_TOKENS, tokens = min(MOST_TOKENS, p.tokens - first);
+    const int first = (int)(blockIdx.x / p.cluster) * MOST_TOKENS, tokens = min(MOST_TOKENS, p.tokens - first);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int mine = (p.count - (int)rank + CLUSTER - 1) / CLUSTER;  // experts of this CTA
-    // warps that share a row: as many as leave none idle
-    const int share = mine > 4 ? 1 : mine > 2 ? 2 : mine > 1 ? 4 : 8;
-    const uint32_t logits0 = map_to_rank(smem_u32(&logits[0][0]), 0);
+    const uint32_t logits0 = p.cluster > 1 ? map_to_rank(smem_u32(&logits[0][0]), 0) : 0u;
+    // two experts a warp, or a share of their rows where the CTA has fewer than its warps can take
+    const int pairs = (p.count + 2 * p.cluster - 1) / (2 * p.cluster), share = pairs > 4 ? 1 : pairs > 2 ? 2 : pairs > 1 ? 4 : 8, part = warp % share;
     pdl_launch_dependents();
+    cluster_arrive_release();  // this CTA is there
     pdl_wait();
-    cluster_arrive_release();
-    cluster_wait_acquire();  // the first CTA is there
-    const int at_once = WARPS / share, part = warp % share;
-    for (int i0 = 0; i0 < mine; i0 += at_once) {
-        const int i = i0 + warp / share, e = (int)rank + CLUSTER * i;
-        float sum[MOST_TOKENS] = {};
-        if (i < mine) {
-            const R *r = static_cast<const R *>(p.router) + (int64_t)e * p.width;
+    bool met = false;
+    for (int pair = 0; pair < pairs; pair += WARPS / share) {
+        const int e0 = 2 * ((pair + warp / share) * p.cluster + (int)rank);
+        const bool some = pair + warp / share < pairs && e0 < p.count, two = e0 + 1 < p.count;
+        float sum[2][MOST_TOKENS] = {};
+        if (some) {
+            const R *r = static_cast<const R *>(p.router) + (int64_t)e0 * p.width;
             const T *x = static_cast<const T *>(p.x) + first * p.x_stride;
-#pragma unroll 2
+#pragma unroll 4
             for (int at = (part * 32 + lane) * 8; at < p.width; at += share * 256) {
-                const int left = p.width - at;
-                float w[8];
-                load_some(r + at, left, p.vec_r, w);
+                float w[2][8];
+                load_some<VEC>(r + at, p.width - at, w[0]);
+                load_some<VEC>(r + (two ? p.width : 0) + at, p.width - at, w[1]);
 #pragma unroll
                 for (int t = 0; t < MOST_TOKENS; ++t) {
                     if (t < tokens) {
                         float v[8];
-                        load_some(x + t * p.x_stride + at, left, p.vec_x, v);
+                        load_some<VEC>(x + t * p.x_stride + at, p.width - at, v);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) sum[t] = fmaf(v[j], w[j], sum[t]);
+                        for (int j = 0; j < 8; ++j) sum[0][t] = fmaf(v[j], w[0][j], sum[0][t]), sum[1][t] = fmaf(v[j], w[1][j], sum[1][t]);
                     }
                 }
             }
 #pragma unroll
-            for (int t = 0; t < MOST_TOKENS; ++t)
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], o);
-        }
-        if (share > 1) {
-            if (lane == 0) {
-#pragma unroll
-                for (int t = 0; t < MOST_TOKENS; ++t) parts[warp][t] = sum[t];
-            }
-            __syncthreads();
-            if (part == 0) {
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int t = 0; t < MOST_TOKENS; ++t)
-                    for (int s = 1; s < share; ++s) sum[t] += parts[warp + s][t];
-            }
-            __syncthreads();
-        }
-        if (i < mine && part == 0 && lane == 0) {
 #pragma unroll
-            for (int t = 0; t < MOST_TOKENS; ++t)
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(logits0 + (uint32_t)(t * MOST_EXPERTS + e) * 4), "f"(sum[t]) : "memory");
+                    for (int o = 16; o > 0; o >>= 1) sum[i][t] += __shfl_xor_sync(0xffffffffu, sum[i][t], o);
         }
+        if (lane == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int t = 0; t < MOST_TOKENS; ++t) parts[warp][i][t] = sum[i][t];
+        }
+        __syncthreads();
+        if (!met) cluster_wait_acquire();  // the first CTA is there
+        met = true;
+        const int i = lane >> 2, t = lane & 3;
+        if (some && part == 0 && lane < 8 && e0 + i < p.count && t < tokens) {
+            float l = 0.0f;
+            for (int s = 0; s < share; ++s) l += parts[warp + s][i][t];
+            if (p.cluster > 1) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(logits0 + (uint32_t)(t * MOST_EXPERTS + e0 + i) * 4), "f"(l) : "memory");
+            else logits[t][e0 + i] = l;
+        }
+        __syncthreads();
     }
     cluster_arrive_release();
     cluster_wait_acquire();
     if (rank != 0 || warp >= tokens) return;
-    // ---- a warp a token; lane l has experts l, l + 32, ..: its best of those not yet taken, and the warp's ----
-    float *l = logits[warp];
     const int64_t row = (int64_t)(first + warp) * p.top;
-    auto best_of_mine = [&](uint32_t &key, int &place) {
-        key = 0, place = 0x7fffffff;
-        for (int e = lane; e < p.count; e += 32) {
-            const uint32_t k = ordered(l[e]);
-            if (k > key || place == 0x7fffffff) key = k, place = e;
-        }
-    };
-    uint32_t key, taken = 0;  // taken: bit i of lane's i-th expert
-    int place;
-    best_of_mine(key, place);
-    const bool any = place != 0x7fffffff;
-    bool left = any;
-    float m = 0.0f, total = 0.0f, chosen = 0.0f;
-    for (int j = 0; j < p.top; ++j) {
-        const uint32_t top = __reduce_max_sync(0xffffffffu, left ? key : 0u);
-        const int e = (int)__reduce_min_sync(0xffffffffu, left && key == top ? (uint32_t)place : 0x7fffffffu);
-        const float v = l[e];
-        if (j == 0) m = v;
-        const float w = expf(v - m);
-        total += w;
-        if (lane == j) chosen = w;
-        if (lane == 0) p.experts[row + j] = e;
-        if ((e & 31) == lane) {
-            taken |= 1u << (e >> 5);
-            left = false;
-            for (int i = 0, o = lane; o < p.count; ++i, o += 32) {
-                if (taken >> i & 1u) continue;
-                const uint32_t k = ordered(l[o]);
-                if (!left || k > key) key = k, place = o, left = true;
-            }
-        }
-        __syncwarp();
-    }
-    if (p.all) {
-        total = 0.0f;
-        for (int e = lane; e < p.count; e += 32) total += expf(l[e] - m);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    } else {
-        // a logit that is no number makes its token's weights none, also where it was not chosen
-        bool bad = false;
-        for (int e = lane; e < p.count; e += 32) bad |= l[e] != l[e];
-        if (__any_sync(0xffffffffu, bad)) total = __uint_as_float(0x7fc00000u);
-    }
-    if (lane < p.top) p.weights[row + lane] = __fdiv_rn(chosen, total);
+    if (p.count <= 32) choose<1>(p, logits[warp], row, lane);
+    else if (p.count <= 128) choose<4>(p, logits[warp], row, lane);
+    else choose<MOST_EXPERTS / 32>(p, logits[warp], row, lane);
+}
+
+template <typename T, typename R>
+int launch_typed(const RouteArgs &p, bool vec, cudaStream_t stream) {
+    const dim3 grid((unsigned)(ceil_div(p.tokens, MOST_TOKENS) * p.cluster));
+    return vec ? launch_after("route_kernel", route_kernel<T, R, true>, grid, THREADS, 0, p.cluster, stream, p)
+               : launch_after("route_kernel", route_kernel<T, R, false>, grid, THREADS, 0, p.cluster, stream, p);
 }
 
 }  // namespace
@@ -176,18 +180,14 @@ B200Q_API int b200q_route_tokens(const void *x, int64_t x_stride, const void *ro
     if (experts == nullptr || weights == nullptr || (width > 0 && (x == nullptr || router == nullptr))) return set_error(B200Q_INVALID_ARGUMENT, "%s: null pointer argument", op);
     if (tokens > 0x3fffffffLL || width > 0x3fffffffLL) return set_error(B200Q_UNSUPPORTED, "%s: %lld tokens of %lld elements", op, (long long)tokens, (long long)width);
     const int64_t size = type == B200Q_F32 ? 4 : 2, router_size = router_type == B200Q_F32 ? 4 : 2;
-    const RouteArgs p = {x, router, x_stride, experts, weights, (int)tokens, (int)width, (int)count, (int)top, over_all != 0,
-                         aligned_to(x, 16) && (tokens == 1 || x_stride * size % 16 == 0), aligned_to(router, 16) && (count == 1 || width * router_size % 16 == 0)};
-    const dim3 grid((unsigned)(ceil_div(tokens, MOST_TOKENS) * CLUSTER));
+    int cluster = 1;
+    while (cluster < MOST_CLUSTER && 2 * cluster < count) cluster *= 2;
+    const RouteArgs p = {x, router, x_stride, experts, weights, (int)tokens, (int)width, (int)count, (int)top, cluster, over_all != 0};
+    const bool vec = width % 8 == 0 && aligned_to(x, 16) && (tokens == 1 || x_stride * size % 16 == 0) && aligned_to(router, 16) && width * router_size % 16 == 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const char *name = "route_kernel";
-    if (type == B200Q_F32) return launch_after(name, route_kernel<float, float>, grid, THREADS, 0, CLUSTER, s, p);
-    if (type == B200Q_F16) {
-        return router_type == B200Q_F32 ? launch_after(name, route_kernel<__half, float>, grid, THREADS, 0, CLUSTER, s, p)
-                                        : launch_after(name, route_kernel<__half, __half>, grid, THREADS, 0, CLUSTER, s, p);
-    }
-    return router_type == B200Q_F32 ? launch_after(name, route_kernel<__nv_bfloat16, float>, grid, THREADS, 0, CLUSTER, s, p)
-                                    : launch_after(name, route_kernel<__nv_bfloat16, __nv_bfloat16>, grid, THREADS, 0, CLUSTER, s, p);
+    if (type == B200Q_F32) return launch_typed<float, float>(p, vec, s);
+    if (type == B200Q_F16) return router_type == B200Q_F32 ? launch_typed<__half, float>(p, vec, s) : launch_typed<__half, __half>(p, vec, s);
+    return router_type == B200Q_F32 ? launch_typed<__nv_bfloat16, float>(p, vec, s) : launch_typed<__nv_bfloat16, __nv_bfloat16>(p, vec, s);
 }
 
 }  // extern "C"
