@@ -44,6 +44,11 @@ struct Library {
     decltype(&b200q_quantized_cache_attention_workspace_bytes) attention_workspace_bytes = nullptr;
     decltype(&b200q_quantized_cache_attention) attention = nullptr;
     decltype(&b200q_token_log_probs) log_probs = nullptr;
+    decltype(&b200q_quantize_tokens) quantize_tokens = nullptr;
+    decltype(&b200q_qlinear_i8_i8) matmul_i8 = nullptr;
+    decltype(&b200q_route_tokens) route_tokens = nullptr;
+    decltype(&b200q_mixture_of_experts_workspace_bytes) experts_workspace_bytes = nullptr;
+    decltype(&b200q_mixture_of_experts) experts = nullptr;
 } lib;
 
 // Scratch buffers that the Python side owns and has told us about, by stream and device.
@@ -500,6 +505,164 @@ PyObject *log_probs(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     END_HANDLE_TH_ERRORS
 }
 
+// t has `like`'s sizes but the last, and `last` there (-1: no last at all)
+inline bool shaped_like(const at::Tensor &t, const at::Tensor &like, int64_t last) {
+    const int64_t lead = like.dim() - 1;
+    if (t.dim() != (last < 0 ? lead : lead + 1) || (last >= 0 && t.size(-1) != last)) return false;
+    for (int64_t d = 0; d < lead; ++d)
+        if (t.size(d) != like.size(d)) return false;
+    return true;
+}
+
+// quantize_tokens(x, norm or None, eps) -> (codes, scales)
+PyObject *quantize_tokens(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    PLAIN_OR_NONE(n_args == 3 && lib.quantize_tokens != nullptr && !watched() && PyFloat_CheckExact(args[2]));
+    const at::Tensor *x = plain_tensor(args[0]), *norm = nullptr;
+    PLAIN_OR_NONE(x && x->dim() >= 1 && x->numel() > 0 && float_code(x->scalar_type()) >= 0);
+    Where w;
+    PLAIN_OR_NONE(where_is(*x, w));
+    const int64_t width = x->size(-1);
+    if (args[1] != Py_None) {
+        norm = plain_tensor(args[1]);
+        PLAIN_OR_NONE(norm && norm->scalar_type() == x->scalar_type() && norm->dim() == 1 && norm->size(0) == width && norm->get_device() == w.device);
+    }
+    at::Tensor codes = empty(x->sizes(), at::kChar, w.device), scales = empty(x->sizes().slice(0, x->dim() - 1), at::kFloat, w.device);
+    const void *xp = x->const_data_ptr(), *np = norm ? norm->const_data_ptr() : nullptr;
+    void *cp = codes.data_ptr();
+    float *sp = static_cast<float *>(scales.data_ptr());
+    const float eps = (float)PyFloat_AS_DOUBLE(args[2]);
+    int status;
+    WITHOUT_GIL(status, lib.quantize_tokens(xp, width, np, eps, cp, sp, x->numel() / width, width, float_code(x->scalar_type()), w.stream));
+    PLAIN_OR_NONE(status == B200Q_OK);
+    PyObject *first = THPVariable_Wrap(std::move(codes));
+    return pair_of(first, THPVariable_Wrap(std::move(scales)));
+    END_HANDLE_TH_ERRORS
+}
+
+// matmul_i8(a, a_scale, weight, scale, weight_layout, out, bias, residual, activation, dtype)
+PyObject *matmul_i8(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    PLAIN_OR_NONE(n_args == 10 && lib.matmul_i8 != nullptr && !watched() && THPDtype_Check(args[9]));
+    const at::Tensor *a = plain_tensor(args[0]), *a_scale = plain_tensor(args[1]), *weight = plain_tensor(args[2]), *scale = plain_tensor(args[3]);
+    PLAIN_OR_NONE(a && a_scale && weight && scale && a->dim() >= 1 && a->numel() > 0 && weight->dim() == 2 && weight->numel() > 0 && scale->dim() == 1);
+    const at::ScalarType dtype = reinterpret_cast<THPDtype *>(args[9])->scalar_type;
+    const bool nk = is_text(args[4], "NK"), pairs = is_text(args[8], "silu_mul");
+    PLAIN_OR_NONE((nk || is_text(args[4], "KN")) && (pairs || args[8] == Py_None) && (dtype == at::kHalf || dtype == at::kBFloat16));
+    PLAIN_OR_NONE(a->scalar_type() == at::kChar && weight->scalar_type() == at::kChar && a_scale->scalar_type() == at::kFloat && float_code(scale->scalar_type()) >= 0);
+    const int64_t k = a->size(-1), n = weight->size(nk ? 0 : 1), m = a->numel() / k;
+    PLAIN_OR_NONE(weight->size(nk ? 1 : 0) == k && scale->size(0) == n && shaped_like(*a_scale, *a, -1) && !(pairs && n % 2 != 0));
+    Where w;
+    PLAIN_OR_NONE(where_is(*a, w) && a_scale->get_device() == w.device && weight->get_device() == w.device && scale->get_device() == w.device);
+    const int64_t n_out = pairs ? n / 2 : n;
+    auto of_result = [&](const at::Tensor *t) { return t && t->scalar_type() == dtype && t->get_device() == w.device && shaped_like(*t, *a, n_out); };
+    b200q_epilogue ep = {};
+    ep.ldr = n_out;
+    ep.activation = pairs ? B200Q_ACT_SILU_MUL : B200Q_ACT_NONE;
+    if (args[6] != Py_None) {
+        const at::Tensor *bias = plain_tensor(args[6]);
+        PLAIN_OR_NONE(bias && bias->scalar_type() == dtype && bias->get_device() == w.device && bias->dim() == 1 && bias->size(0) == n);
+        ep.bias = bias->const_data_ptr();
+    }
+    if (args[7] != Py_None) {
+        const at::Tensor *residual = plain_tensor(args[7]);
+        PLAIN_OR_NONE(of_result(residual));
+        ep.residual = residual->const_data_ptr();
+    }
+    at::Tensor made;
+    void *c;
+    if (args[5] != Py_None) {
+        const at::Tensor *out = plain_tensor(args[5]);
+        PLAIN_OR_NONE(of_result(out));
+        c = out->data_ptr();
+    } else {
+        at::DimVector shape(a->sizes());
+        shape.back() = n_out;
+        made = empty(shape, dtype, w.device);
+        c = made.data_ptr();
+    }
+    const void *ap = a->const_data_ptr(), *wp = weight->const_data_ptr(), *sp = scale->const_data_ptr();
+    const float *asp = static_cast<const float *>(a_scale->const_data_ptr());
+    int status;
+    WITHOUT_GIL(status, lib.matmul_i8(ap, asp, wp, sp, c, m, n, k, nk ? B200Q_LAYOUT_NK : B200Q_LAYOUT_KN, float_code(scale->scalar_type()), float_code(dtype), &ep, w.stream));
+    PLAIN_OR_NONE(status == B200Q_OK);
+    if (!made.defined()) return Py_NewRef(args[5]);
+    return THPVariable_Wrap(std::move(made));
+    END_HANDLE_TH_ERRORS
+}
+
+// route_tokens(x, router, top_k, normalize) -> (experts, weights)
+PyObject *route_tokens(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    PLAIN_OR_NONE(n_args == 4 && lib.route_tokens != nullptr && !watched() && PyLong_CheckExact(args[2]) && PyBool_Check(args[3]));
+    const at::Tensor *x = plain_tensor(args[0]), *router = plain_tensor(args[1]);
+    PLAIN_OR_NONE(x && router && x->dim() >= 1 && x->numel() > 0 && router->dim() == 2 && float_code(x->scalar_type()) >= 0);
+    PLAIN_OR_NONE(router->size(1) == x->size(-1) && (router->scalar_type() == x->scalar_type() || router->scalar_type() == at::kFloat));
+    const int64_t width = x->size(-1), count = router->size(0), top = PyLong_AsLongLong(args[2]);
+    Where w;
+    PLAIN_OR_NONE(top >= 1 && top <= 32 && top <= count && where_is(*x, w) && router->get_device() == w.device);
+    at::DimVector shape(x->sizes());
+    shape.back() = top;
+    at::Tensor experts = empty(shape, at::kInt, w.device), weights = empty(shape, at::kFloat, w.device);
+    const void *xp = x->const_data_ptr(), *rp = router->const_data_ptr();
+    int32_t *ep = static_cast<int32_t *>(experts.data_ptr());
+    float *wp = static_cast<float *>(weights.data_ptr());
+    int status;
+    WITHOUT_GIL(status, lib.route_tokens(xp, width, rp, ep, wp, x->numel() / width, width, count, top, args[3] == Py_False, float_code(x->scalar_type()), float_code(router->scalar_type()), w.stream));
+    PLAIN_OR_NONE(status == B200Q_OK);
+    PyObject *first = THPVariable_Wrap(std::move(experts));
+    return pair_of(first, THPVariable_Wrap(std::move(weights)));
+    END_HANDLE_TH_ERRORS
+}
+
+// experts(x, experts, weights, gate_up, gate_up_scale, down, down_scale, residual or None, out or None)
+PyObject *experts(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
+    HANDLE_TH_ERRORS
+    PLAIN_OR_NONE(n_args == 9 && lib.experts != nullptr && !watched());
+    const at::Tensor *t[7];
+    for (int i = 0; i < 7; ++i) PLAIN_OR_NONE((t[i] = plain_tensor(args[i])) != nullptr && t[i]->numel() > 0);
+    const at::Tensor &x = *t[0], &chosen = *t[1], &weights = *t[2], &gate_up = *t[3], &s1 = *t[4], &down = *t[5], &s2 = *t[6];
+    PLAIN_OR_NONE(x.dim() >= 1 && (x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16) && chosen.scalar_type() == at::kInt && weights.scalar_type() == at::kFloat);
+    PLAIN_OR_NONE(gate_up.scalar_type() == at::kChar && down.scalar_type() == at::kChar && float_code(s1.scalar_type()) >= 0 && s2.scalar_type() == s1.scalar_type());
+    PLAIN_OR_NONE(chosen.dim() == x.dim() && shaped_like(chosen, x, chosen.size(-1)) && weights.sizes() == chosen.sizes() && gate_up.dim() == 3 && down.dim() == 3 && s1.dim() == 2 && s2.dim() == 2);
+    const int64_t hidden = x.size(-1), tokens = x.numel() / hidden, count = gate_up.size(0), inner = gate_up.size(1) / 2, top = chosen.size(-1);
+    PLAIN_OR_NONE(gate_up.size(1) % 2 == 0 && gate_up.size(2) == hidden && down.size(0) == count && down.size(1) == hidden && down.size(2) == inner);
+    PLAIN_OR_NONE(s1.size(0) == count && s1.size(1) == 2 * inner && s2.size(0) == count && s2.size(1) == hidden && (reinterpret_cast<uintptr_t>(x.const_data_ptr()) & 15u) == 0 && hidden % 8 == 0);
+    Where w;
+    PLAIN_OR_NONE(where_is(x, w));
+    for (int i = 1; i < 7; ++i) PLAIN_OR_NONE(t[i]->get_device() == w.device);
+    auto of_result = [&](const at::Tensor *r) { return r && r->scalar_type() == x.scalar_type() && r->get_device() == w.device && r->sizes() == x.sizes(); };
+    const void *residual = nullptr;
+    if (args[7] != Py_None) {
+        const at::Tensor *r = plain_tensor(args[7]);
+        PLAIN_OR_NONE(of_result(r));
+        residual = r->const_data_ptr();
+    }
+    void *ws;
+    size_t ws_bytes;
+    PLAIN_OR_NONE(find_scratch(w, lib.experts_workspace_bytes(tokens, hidden, inner, count, top), ws, ws_bytes));
+    at::Tensor made;
+    void *out;
+    if (args[8] != Py_None) {
+        const at::Tensor *o = plain_tensor(args[8]);
+        PLAIN_OR_NONE(of_result(o));
+        out = o->data_ptr();
+    } else {
+        made = empty(x.sizes(), x.scalar_type(), w.device);
+        out = made.data_ptr();
+    }
+    const void *xp = x.const_data_ptr(), *gp = gate_up.const_data_ptr(), *s1p = s1.const_data_ptr(), *dp = down.const_data_ptr(), *s2p = s2.const_data_ptr();
+    const int32_t *cp = static_cast<const int32_t *>(chosen.const_data_ptr());
+    const float *wp = static_cast<const float *>(weights.const_data_ptr());
+    int status;
+    WITHOUT_GIL(status, lib.experts(xp, hidden, cp, wp, gp, s1p, dp, s2p, residual, hidden, out, tokens, hidden, inner, count, top, float_code(x.scalar_type()), float_code(s1.scalar_type()), ws,
+                                    ws_bytes, w.stream));
+    PLAIN_OR_NONE(status == B200Q_OK);
+    if (!made.defined()) return Py_NewRef(args[8]);
+    return THPVariable_Wrap(std::move(made));
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(an address for each member of Library, in their order)
 PyObject *bind(PyObject *, PyObject *args) {
     static_assert(sizeof(Library) % sizeof(void *) == 0, "");
@@ -514,6 +677,7 @@ PyObject *bind(PyObject *, PyObject *args) {
     auto set = [&](auto &member) { member = reinterpret_cast<std::remove_reference_t<decltype(member)>>(p[i++]); };
     set(lib.quantize), set(lib.dequantize), set(lib.take), set(lib.workspace_bytes), set(lib.linear), set(lib.linear_fused), set(lib.w4_workspace_bytes), set(lib.w4);
     set(lib.rotary), set(lib.append), set(lib.read), set(lib.attention_workspace_bytes), set(lib.attention), set(lib.log_probs);
+    set(lib.quantize_tokens), set(lib.matmul_i8), set(lib.route_tokens), set(lib.experts_workspace_bytes), set(lib.experts);
     Py_RETURN_NONE;
 }
 
@@ -546,6 +710,10 @@ PyMethodDef methods[] = {FAST(linear),
                          FAST(read),
                          FAST(attention),
                          FAST(log_probs),
+                         FAST(quantize_tokens),
+                         FAST(matmul_i8),
+                         FAST(route_tokens),
+                         FAST(experts),
                          {"bind", bind, METH_VARARGS, nullptr},
                          {"set_scratch", set_scratch, METH_VARARGS, nullptr},
                          {"clear_scratch", clear_scratch, METH_NOARGS, nullptr},

@@ -27,8 +27,10 @@ LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'lib')
 _BOUND = ('b200q_symmetric_quantize', 'b200q_symmetric_dequantize', 'b200q_embedding_dequantize', 'b200q_qlinear_workspace_bytes',
           'b200q_qlinear_f16_i8', 'b200q_qlinear_f16_i8_fused', 'b200q_qlinear_f16_u4_workspace_bytes', 'b200q_qlinear_f16_u4',
           'b200q_rotary_embedding', 'b200q_quantized_cache_append', 'b200q_quantized_cache_read', 'b200q_quantized_cache_attention_workspace_bytes',
-          'b200q_quantized_cache_attention', 'b200q_token_log_probs')
-_FUNCTIONS = ('linear', 'quantize', 'dequantize', 'take', 'w4', 'rotary', 'append', 'read', 'attention', 'log_probs')
+          'b200q_quantized_cache_attention', 'b200q_token_log_probs', 'b200q_quantize_tokens', 'b200q_qlinear_i8_i8', 'b200q_route_tokens',
+          'b200q_mixture_of_experts_workspace_bytes', 'b200q_mixture_of_experts')
+_FUNCTIONS = ('linear', 'quantize', 'dequantize', 'take', 'w4', 'rotary', 'append', 'read', 'attention', 'log_probs', 'quantize_tokens', 'matmul_i8', 'route_tokens',
+              'experts')
 _module = None
 
 
@@ -84,5 +86,5 @@ def _stand_in(name):
     return first_call
 
 
-quantize_tokens = matmul_i8 = route_tokens = experts = _unavailable
-linear, quantize, dequantize, take, w4, rotary, append, read, attention, log_probs = (_stand_in(name) for name in _FUNCTIONS)
+(linear, quantize, dequantize, take, w4, rotary, append, read, attention, log_probs, quantize_tokens, matmul_i8, route_tokens,
+ experts) = (_stand_in(name) for name in _FUNCTIONS)

@@ -59,7 +59,7 @@ def mixture_of_experts(x: torch.Tensor, experts: torch.Tensor, weights: torch.Te
     x [..., hidden] float16 or bfloat16; experts int32 and weights float32 [..., k] (route_tokens, or any other choice: an expert may come twice).
     gate_up int8 [count, 2 inner, hidden], rows 2 f and 2 f + 1 the gate and the up projection's f-th; down int8 [count, hidden, inner]; scales [count, 2 inner] and [count, hidden] of one type (float16,
     bfloat16 or float32).  Negative experts are passed over (padding: a token of nothing but these is its residual, or zeros); one beyond the layer's is passed over and reported by b200q_check_status.
-    Sums are float32, the result is rounded once and is the same on every run.  out: a contiguous tensor for the result, which may be the residual but not x.
+    Sums are float32, the result is rounded once and is the same on every run.  out: a contiguous tensor for the result, which may be the residual, or x.
 
     For a few tokens: time goes to reading the weights of the experts that have one, once for 64 tokens.  Not differentiable."""
     result = native.experts(x, experts, weights, gate_up, gate_up_scale, down, down_scale, residual, out)

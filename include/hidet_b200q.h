@@ -332,7 +332,7 @@ B200Q_API int b200q_route_tokens(const void *x, int64_t x_stride, const void *ro
  *   residual[t] + sum_j weights[t, j] * down_scale[e] (down[e] h),   h = silu(g) * u,   (g, u) = gate_up_scale[e] (gate_up[e] x[t]),   e = experts[t, j]
  * gate_up int8 [count, 2 inner, hidden], its rows (gate_f, up_f) pairs at (2 f, 2 f + 1); down int8 [count, hidden, inner]; scales of scale_type, one for each row; both are what
  * b200q_symmetric_quantize makes of the rows of all experts.  Sums are float; x and h are rounded to f16, a row at a time scaled by a power of two where
- * their range asks for it.  The results do not depend on the run.  residual may be NULL, or out.  An assignment to a negative expert is passed over, one to an expert that is not there too, and is
+ * their range asks for it.  The results do not depend on the run.  out may be residual, or x.  An assignment to a negative expert is passed over, one to an expert that is not there too, and is
  * reported by b200q_check_status.  The workspace is one of b200q_qlinear_f16_i8's kind.
  */
 B200Q_API size_t b200q_mixture_of_experts_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top);

@@ -176,6 +176,8 @@ def test_layer_of_strided_operands():
     out = big[..., :256].contiguous()
     want = hidet_b200.mixture_of_experts(big[..., :256], experts, weights, *w, residual=out)
     assert torch.equal(hidet_b200.mixture_of_experts(big[..., :256], experts, weights, *w, residual=out, out=out), want) and torch.equal(out, want)
+    place = big[..., :256].contiguous()  # a layer in its input's place
+    assert torch.equal(hidet_b200.mixture_of_experts(place, experts, weights, *w, residual=place, out=place), hidet_b200.mixture_of_experts(big[..., :256], experts, weights, *w, residual=big[..., :256]))
     moved = torch.empty(w[0].numel() + 1, dtype=torch.int8, device='cuda')[1:].view(w[0].shape).copy_(w[0])  # a base that is not aligned
     got = hidet_b200.mixture_of_experts(big[..., :256], experts, weights, moved, *w[1:])
     ref.check(got.view(12, 256), *ref.experts(big[..., :256].reshape(12, 256), experts.view(12, 2), weights.view(12, 2), *w, None))
