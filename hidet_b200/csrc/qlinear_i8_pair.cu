@@ -12,6 +12,9 @@
 //   warp 9     MMA issuer (first CTA of the pair only), one thread for the whole loop
 // Two accumulators, so that a tile's epilogue runs beside the next one's products.
 //
+// Where tiles are few, K is shared by the two or four pairs of a cluster, a tile each cluster and no second one.  Sums are whole numbers: when all have theirs, every pair
+// hands the others the 32-token blocks that they finish (its fragments as they come out of tensor memory, into the ring, which is no longer in use) and adds what it gets.
+//
 // Every wait is bounded: a wait that runs out records where and raises a CTA-wide flag, all roles leave, the first CTA waits for what was armed and issued, and the
 // two CTAs meet at a cluster barrier before either gives back tensor memory or retires.
 #include <atomic>
@@ -33,6 +36,7 @@ constexpr int THREADS = 32 * 10;
 constexpr int TMEM_COLS = 512;
 constexpr int ROW_BYTES = TN * 2 + 16;       // one output row in the staging buffer, padded: matrix stores touch every bank once
 constexpr int STAGING_BYTES = 32 * ROW_BYTES;
+constexpr int FRAGMENT_BYTES = 32 * 32 * 4;  // a warp's part of a block's sums
 constexpr int RING_BYTES = 188 * 1024;
 constexpr int SMEM_BYTES = RING_BYTES + EPI_GROUPS * 2 * STAGING_BYTES + 1024;  // + alignment slack
 
@@ -43,6 +47,7 @@ struct Params {
     int band;                  // token tiles that are walked together, channel tile by channel tile
     int k_blocks;
     int stages;
+    int split;                 // pairs of a cluster, which share K
 };
 
 __device__ __forceinline__ void tile_of(const Params &p, int u, int &n0, int &m0) {
@@ -73,6 +78,10 @@ __device__ __forceinline__ void mma_pair_i8(uint32_t tmem_d, uint64_t desc_a, ui
         "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// One arrival at this place of the CTAs of a mask, when every MMA issued so far has completed.
+__device__ __forceinline__ void commit_to(uint32_t bar, uint16_t mask) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(mask) : "memory");
+}
 // A tile of [k][128 channels] in rows of 128 swizzled bytes: 8-row groups 1024 bytes apart, both strides (there is one group of channels, so that one of them is not used).
 __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
     return (uint64_t)((addr >> 4) & 0x3fffu) | (64ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
@@ -99,7 +108,7 @@ __device__ __forceinline__ float value_at(const void *p, int64_t i) {
 
 // NK: the weight is [N, K].  PAIRS: channels (2j, 2j + 1) = (gate, up).
 template <bool NK, bool BF16, bool PAIRS>
-__global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(2, 1, 1)
+__global__ void __launch_bounds__(THREADS, 1)
     i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const Params p) {
     extern __shared__ unsigned char smem_dyn[];
     __shared__ __align__(8) uint64_t full[MAX_STAGES];    // (first CTA) both CTAs' tiles of the stage have landed
@@ -113,9 +122,10 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(2, 1, 1)
     const uint32_t smem_base = (smem_u32(smem_dyn) + 1023u) & ~1023u;  // swizzled operands; the same in both CTAs
     unsigned char *smem_gen = smem_dyn + (smem_base - smem_u32(smem_dyn));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_ctarank();
-    const int units = p.n_tiles * p.m_tiles;
-    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const uint32_t cluster_rank = cluster_ctarank(), rank = cluster_rank & 1u, lead = cluster_rank & ~1u;  // in the pair; the pair's first CTA
+    const int units = p.n_tiles * p.m_tiles, share = (int)(cluster_rank >> 1);
+    const int first = blockIdx.x / (2 * p.split), step = gridDim.x / (2 * p.split);
+    const int kb0 = p.k_blocks * share / p.split, kb1 = p.k_blocks * (share + 1) / p.split;
     const uint32_t stages = p.stages, stage_bytes = W_BYTES + (uint32_t)p.tm * (BK / 2);
     constexpr int STAGING_OFF = RING_BYTES;
 
@@ -146,7 +156,7 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(2, 1, 1)
         tma_prefetch_desc(&map_w);
         tma_prefetch_desc(&map_a);
     }
-    pdl_wait();
+    if (warp != LOAD_WARP) pdl_wait();  // every other role: none of their bounded waits runs against the kernel in front
 
     auto wait = [&](uint32_t bar, uint32_t parity, unsigned int site) -> bool {
         bool ok = mbar_wait(bar, parity, umma::kFastPolls);
@@ -158,29 +168,49 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(2, 1, 1)
         return mbar_wait(bar, parity, umma::kFastPolls) || umma::wait_or_abort<kKernelI8Pair>(bar, parity, site, &abort_flag, p.a.status);
     };
 
+    // Where pairs share K, all threads of their cluster meet twice: when the sums are complete, and when they have been handed over.
+    auto meet = [&]() {
+        if (p.split == 1) return;
+        __syncwarp();
+        cluster_arrive_release();
+        cluster_wait_acquire();
+    };
+
     if (warp == LOAD_WARP) {
         // ---------------- TMA producer ----------------
         pdl_launch_dependents();  // tensor memory is allocated: a kernel that is placed as this one's CTAs leave cannot take it away
         if (lane == 0) {
             const uint64_t keep = l2_policy_evict_last();  // both operands are read again by other tiles
-            const uint32_t full0 = map_to_rank(smem_u32(&full[0]), 0);
+            const uint32_t full0 = map_to_rank(smem_u32(&full[0]), lead);
+            auto load_w = [&](uint32_t slot, int n, int kb) {
+                if (rank == 0) mbar_expect_tx(smem_u32(&full[slot]), 2 * stage_bytes);
+                load_pair(smem_base + slot * stage_bytes, &map_w, NK ? kb * BK : n, NK ? n : kb * BK, full0 + 8 * slot, keep);
+            };
+            auto load_a = [&](uint32_t slot, int m, int kb) { load_pair(smem_base + slot * stage_bytes + W_BYTES, &map_a, kb * BK, m, full0 + 8 * slot, keep); };
+            // The first tile's weights are requested before the kernel in front has finished, its tokens behind it.
+            int n, m;
+            tile_of(p, first, n, m);
+            n += (int)rank * TN;
+            m += (int)rank * (p.tm / 2);
+            const int ahead = min(kb1 - kb0, (int)stages);
+            for (int j = 0; j < ahead; ++j) load_w(j, n, kb0 + j);
+            pdl_wait();
+            for (int j = 0; j < ahead; ++j) load_a(j, m, kb0 + j);
             uint32_t i = 0;
             umma::Ring r;
             bool ok = true;
             for (int u = first; u < units && ok; u += step) {
-                int n, m;
                 tile_of(p, u, n, m);
                 n += (int)rank * TN;
                 m += (int)rank * (p.tm / 2);
-                for (int kb = 0; kb < p.k_blocks; ++kb, ++i, r.advance(1, stages)) {
+                for (int kb = kb0; kb < kb1; ++kb, ++i, r.advance(1, stages)) {
+                    if (i < (uint32_t)ahead) continue;
                     if (i >= stages && !wait_one(smem_u32(&empty[r.slot]), r.phase ^ 1u, 1)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t at = smem_base + r.slot * stage_bytes, bar = full0 + 8 * r.slot;
-                    if (rank == 0) mbar_expect_tx(smem_u32(&full[r.slot]), 2 * stage_bytes);
-                    load_pair(at, &map_w, NK ? kb * BK : n, NK ? n : kb * BK, bar, keep);
-                    load_pair(at + W_BYTES, &map_a, kb * BK, m, bar, keep);
+                    load_w(r.slot, n, kb);
+                    load_a(r.slot, m, kb);
                 }
             }
             // Teardown: every copy armed must have landed before a CTA may retire; what counts them is the first CTA's barriers, and the second CTA
@@ -191,10 +221,13 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(2, 1, 1)
                 if (!mbar_wait(smem_u32(&full[s]), (j / stages) & 1)) report_timeout(p.a.status, kKernelI8Pair, 7);
             }
         }
+        meet();
+        meet();
     } else if (warp == MMA_WARP) {
         // ---------------- MMA issuer ----------------
         if (rank == 0 && elect_one()) {
             const uint32_t idesc = idesc_i8(2 * TN, p.tm, !NK);
+            const uint16_t both = (uint16_t)(3u << lead);
             constexpr uint32_t W_STEP = NK ? 32 / 16 : 32 * TN / 16;  // of the weight's descriptor, 32 k on
             uint32_t t_iter = 0;
             umma::Ring r;
@@ -204,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(2, 1, 1)
                 if (acc_use >= 1 && !wait_one(smem_u32(&acc_empty[buf]), (acc_use - 1) & 1, 3)) break;
                 umma::fence_after_sync();
                 const uint32_t d_addr = tmem_base + buf * p.tm;
-                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!here && !wait_one(smem_u32(&full[r.slot]), r.phase, 4)) {
                         ok = false;
                         break;
@@ -213,17 +246,19 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(2, 1, 1)
                     const uint32_t at = smem_base + r.slot * stage_bytes;
                     const uint64_t w_desc = NK ? umma::smem_desc_sw128(at) : smem_desc_mn(at), a_desc = umma::smem_desc_sw128(at + W_BYTES);
 #pragma unroll
-                    for (int ks = 0; ks < BK / 32; ++ks) mma_pair_i8(d_addr, w_desc + W_STEP * ks, a_desc + 2 * ks, idesc, (kb > 0 || ks > 0) ? 1u : 0u);
-                    umma::commit_pair(smem_u32(&empty[r.slot]));
+                    for (int ks = 0; ks < BK / 32; ++ks) mma_pair_i8(d_addr, w_desc + W_STEP * ks, a_desc + 2 * ks, idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
+                    commit_to(smem_u32(&empty[r.slot]), both);
                     r.advance(1, stages);
                     here = mbar_test(smem_u32(&full[r.slot]), r.phase);
                 }
-                if (ok) umma::commit_pair(smem_u32(&acc_full[buf]));
+                if (ok) commit_to(smem_u32(&acc_full[buf]), both);
             }
             // Teardown: no MMA may still be running when tensor memory is given back or the peer retires.
             umma::commit_pair_self(smem_u32(&drain_bar));
             if (!mbar_wait(smem_u32(&drain_bar), 0)) report_timeout(p.a.status, kKernelI8Pair, 8);
         }
+        meet();
+        meet();
     } else {
         // ---------------- epilogue ----------------
         const int eg = warp >> 2;               // takes blocks eg, eg + EPI_GROUPS, ...
@@ -258,17 +293,39 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(2, 1, 1)
                     sc[h][e] = n < N ? i8_scale(p.a.scale, p.a.scale_type, n) : 0.0f;
                     bias[h][e] = n < N && p.a.bias != nullptr ? value_at<BF16>(p.a.bias, n) : 0.0f;
                 }
-            if (!all_of_128(1 + eg, wait(smem_u32(&acc_full[buf]), acc_use & 1, 10))) break;  // the group stays or leaves as one
+            const bool ok = all_of_128(1 + eg, wait(smem_u32(&acc_full[buf]), acc_use & 1, 10));  // the group stays or leaves as one
+            if (!ok && p.split == 1) break;
             umma::fence_after_sync();
+            if (p.split > 1) {
+                // Block cb is finished by pair cb % split, as the (cb / split)-th of its blocks.
+                meet();
+                const int of_each = (blocks + p.split - 1) / p.split;
+                for (int cb = 0; ok && cb < blocks; ++cb) {
+                    const int owner = cb % p.split, nth = cb / p.split;
+                    if (owner == share || nth % EPI_GROUPS != eg) continue;
+                    uint32_t v[2][16];
+                    umma::ld_16x256b_x4(acc + cb * 32, v[0]);
+                    umma::ld_16x256b_x4(acc + (16u << 16) + cb * 32, v[1]);
+                    umma::ld_wait();
+                    const uint32_t to = map_to_rank(smem_base + (uint32_t)((share * of_each + nth) * 4 + q) * FRAGMENT_BYTES + lane * 16, 2 * owner + rank);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + i * 512), "r"(v[i >> 2][4 * (i & 3)]), "r"(v[i >> 2][4 * (i & 3) + 1]),
+                                     "r"(v[i >> 2][4 * (i & 3) + 2]), "r"(v[i >> 2][4 * (i & 3) + 3])
+                                     : "memory");
+                }
+                meet();
+                if (!ok) break;
+            }
             const int out_n0 = PAIRS ? n0 >> 1 : n0;
             const bool cols_ok = out_n0 + chunk * 8 < out_n;  // widths are multiples of 8: eight channels are in or out together
             const size_t out_off = (size_t)m0 * out_n + out_n0 + chunk * 8;
-            if (eg >= blocks) {  // a tile of a single block: nothing for this group
+            if (p.split == 1 && eg >= blocks) {  // a tile of a single block: nothing for this group
                 __syncwarp();
-                if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&acc_empty[buf]), 0));
+                if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&acc_empty[buf]), lead));
             }
 #pragma unroll 1
-            for (int cb = eg; cb < blocks; cb += EPI_GROUPS, ++block) {
+            for (int cb = share + p.split * eg; cb < blocks; cb += p.split * EPI_GROUPS, ++block) {
                 unsigned char *staging = smem_gen + STAGING_OFF + (2 * eg + (block & 1)) * STAGING_BYTES;
                 const uint32_t staging_a = smem_base + STAGING_OFF + (2 * eg + (block & 1)) * STAGING_BYTES;
                 float sa[4][2];  // token 8 j + 2 tq + i
@@ -294,10 +351,21 @@ __global__ void __launch_bounds__(THREADS, 1) __cluster_dims__(2, 1, 1)
                 umma::ld_16x256b_x4(acc + cb * 32, v[0]);
                 umma::ld_16x256b_x4(acc + (16u << 16) + cb * 32, v[1]);
                 umma::ld_wait();
-                if (cb + EPI_GROUPS >= blocks) {  // the group's part of the accumulator is in registers
+                if (p.split > 1) {
+                    const int of_each = (blocks + p.split - 1) / p.split;
+                    for (int from = 0; from < p.split; ++from) {
+                        if (from == share) continue;
+                        const unsigned char *at = smem_gen + ((from * of_each + cb / p.split) * 4 + q) * FRAGMENT_BYTES + lane * 16;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint4 w = *reinterpret_cast<const uint4 *>(at + i * 512);
+                            v[i >> 2][4 * (i & 3)] += w.x, v[i >> 2][4 * (i & 3) + 1] += w.y, v[i >> 2][4 * (i & 3) + 2] += w.z, v[i >> 2][4 * (i & 3) + 3] += w.w;
+                        }
+                    }
+                } else if (cb + EPI_GROUPS >= blocks) {  // the group's part of the accumulator is in registers
                     umma::fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&acc_empty[buf]), 0));
+                    if (lane == 0) mbar_arrive_remote(map_to_rank(smem_u32(&acc_empty[buf]), lead));
                 }
                 // v[h][4 j + 2 e + i]: channel 16 h + 8 e + g, token 8 j + 2 tq + i
                 auto sum_of = [&](int h, int j, int e, int i) { return fmaf((float)(int)v[h][4 * j + 2 * e + i] * sc[h][e], sa[j][i], bias[h][e]); };
@@ -408,34 +476,21 @@ int launch_as(const CUtensorMap &map_w, const CUtensorMap &map_a, const Params &
     cfg.blockDim = dim3(THREADS, 1, 1);
     cfg.dynamicSmemBytes = SMEM_BYTES;
     cfg.stream = stream;
-    cudaLaunchAttribute attrs[1];
+    cudaLaunchAttribute attrs[2];
     attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = 2 * (unsigned)p.split;
+    attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
     cfg.attrs = attrs;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     B200Q_CUDA_TRY(cudaLaunchKernelEx(&cfg, i8_pair_kernel<NK, BF16, PAIRS>, map_w, map_a, p));
     return B200Q_OK;
 }
 
 }  // namespace i8pair
 
-// Tokens per tile: the number with the least rounds of tiles times clocks a stage.
-int plan_i8_pair(int64_t M, int64_t N) {
-    using namespace i8pair;
-    int sms = sm_count();
-    if (sms <= 0) sms = 148;
-    int best = 256;
-    double least = 0.0;
-    for (int tm = 256; tm >= 32; tm -= 32) {
-        const int64_t units = ceil_div(M, tm) * ceil_div(N, 2 * TN);
-        const double products = 2.0 * tm, copies = (W_BYTES + tm * (BK / 2)) / 50.0;
-        const double cost = (double)ceil_div(units, sms / 2) * (products > copies ? products : copies);
-        if (least == 0.0 || cost < least) least = cost, best = tm;
-    }
-    return best;
-}
-
-int launch_i8_pair(const I8Args &a, int tm, cudaStream_t stream) {
+int launch_i8_pair(const I8Args &a, int tm, int split, cudaStream_t stream) {
     using namespace i8pair;
     CUtensorMap map_w, map_a;
     int rc = a.nk ? make_tensor_map_2d(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, (uint64_t)a.K, (uint64_t)a.N, (uint64_t)a.K, BK, TN, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -462,8 +517,10 @@ int launch_i8_pair(const I8Args &a, int tm, cudaStream_t stream) {
     if (units * 2 > 2147483647LL) return set_error(B200Q_UNSUPPORTED, "qlinear_i8_i8: problem too large for the tile counter");
     int sms = sm_count();
     if (sms <= 0) sms = 148;
+    if (split > p.k_blocks) split = 1;  // each has a part
+    p.split = split;
     const int64_t pairs_at_once = sms / 2;
-    const unsigned grid = 2u * (unsigned)(units < pairs_at_once ? units : pairs_at_once);
+    const unsigned grid = split > 1 ? 2u * (unsigned)(units * split) : 2u * (unsigned)(units < pairs_at_once ? units : pairs_at_once);
     const int form = (a.nk ? 4 : 0) + (a.out_type == B200Q_BF16 ? 2 : 0) + (a.pairs ? 1 : 0);
     switch (form) {
         case 0: return launch_as<false, false, false>(map_w, map_a, p, grid, stream);

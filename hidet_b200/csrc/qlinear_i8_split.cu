@@ -227,16 +227,6 @@ int launch_as(const CUtensorMap &map_w, const CUtensorMap &map_a, const Params &
 
 }  // namespace i8split
 
-// As many CTAs a tile as all have a place at once, two an SM: with more, the last ones' start and end stand alone (one token through 4096 x 22016, 172 tiles: 16.9 us
-// with one CTA a tile, 22.9 with two; through 4096 x 4096, 32 tiles: 6.1 with four or eight, 7.4 with two).
-int plan_i8_split(int64_t M, int64_t N, int tm) {
-    using namespace i8split;
-    const int64_t tiles = ceil_div(N, TN) * ceil_div(M, tm), places = 2 * (sm_count() > 0 ? sm_count() : 148);
-    int cluster = 1;
-    while (cluster < 8 && tiles * (cluster + 1) <= places) ++cluster;
-    return cluster;
-}
-
 int launch_i8_split(const I8Args &a, int tm, int cluster, cudaStream_t stream) {
     using namespace i8split;
     CUtensorMap map_w, map_a;

@@ -126,6 +126,14 @@ def test_product_by_sizes(k, n, layout):
 
 
 @pytest.mark.parametrize('layout', ['KN', 'NK'])
+@pytest.mark.parametrize('m,k,n', [(606, 2720, 16), (700, 8192, 512), (685, 4016, 16), (500, 8208, 784), (990, 16384, 272), (1, 656, 4880), (1, 992, 16), (121, 8208, 2064), (40, 4096, 6160), (2500, 512, 1040)])
+def test_product_whose_inner_dimension_is_shared(m, k, n, layout):
+    """Sizes for which CTAs or pairs of them share K by one, two, four and eight."""
+    check_product(m, k, n, layout, bias=True, residual=True)
+    check_product(m, k, n, layout, BF16, pairs=True)
+
+
+@pytest.mark.parametrize('layout', ['KN', 'NK'])
 @pytest.mark.parametrize('m,k,n', [(1, 1, 1), (3, 5, 7), (2, 130, 66), (70, 513, 131), (65, 64, 100), (9, 1000, 24), (130, 24, 40), (5, 4100, 18)])
 def test_product_of_any_alignment(m, k, n, layout):
     check_product(m, k, n, layout, bias=True, residual=True)
