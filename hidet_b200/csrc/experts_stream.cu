@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "experts.h"
+#include "experts_parts.cuh"
 #include "serving.cuh"
 #include "umma.cuh"
 
@@ -348,14 +349,8 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
     // Stages as large as the largest entry asks for, and as many as there is room for.
     const int C = columns_for(s.largest), columns = sixteens(C);
     const uint32_t stage_bytes = W_BYTES + (uint32_t)columns * BK, stages = min((uint32_t)MOST_STAGES, p.ring_bytes / stage_bytes);
-    const uint32_t units = entries * p.tiles, total = units * p.k_blocks;
-    // Gate and up: whole units where the CTA with the most has hardly more than an equal part, whose pieces have to be brought together (which takes the time of some ten stages).
-    const bool whole = !DOWN && (units + gridDim.x - 1) / gridDim.x * p.k_blocks <= total / gridDim.x + 10;
-    // A part of CTA c: `each` pieces, and one of the `more` that are left.  (Divisions of 64 bits took 2 us of a kernel's start, and more at its end.)
-    const uint32_t pieces = whole ? units : total, step = whole ? p.k_blocks : 1, each = pieces / gridDim.x, more = pieces - each * gridDim.x;
-    auto first_of = [&](uint32_t c) { return (c * each + min(c, more)) * step; };
-    auto cta_of = [&](uint32_t stage) { return stage < more * (each + 1) ? stage / (each + 1) : more + (stage - more * (each + 1)) / each; };  // of parts by stages
-    const uint32_t s0 = first_of(blockIdx.x), s1 = first_of(blockIdx.x + 1);
+    const Parts parts(entries * p.tiles, p.k_blocks, gridDim.x, !DOWN);
+    const uint32_t s0 = parts.first_of(blockIdx.x), s1 = parts.first_of(blockIdx.x + 1);
     const int mine = (int)(s1 - s0);  // stages of this CTA
     const Place<DOWN> start(s0, p, entries);
 
@@ -548,8 +543,8 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
                 if (!DOWN && steps < (int)p.k_blocks) {
                     // a unit of several CTAs: this one's sums to the others, and whoever comes last adds them
                     const uint32_t u0 = s0 + i - first_k;
-                    c0 = cta_of(u0), c1 = cta_of(u0 + p.k_blocks - 1);
-                    int *to = static_cast<int *>(p.shared) + ((int64_t)blockIdx.x * 2 + (i > 0)) * columns * TN + row;
+                    c0 = parts.cta_of(u0), c1 = parts.cta_of(u0 + p.k_blocks - 1);
+                    int *to = static_cast<int *>(p.shared) + ((int64_t)blockIdx.x * 2 + parts.second_place(blockIdx.x, u0)) * columns * TN + row;
 #pragma unroll 1
                     for (int c = 0; c < en.count; c += WIDE) {
                         int v[DIGITS][WIDE];
@@ -575,7 +570,7 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
                         for (uint32_t other = c0; other <= c1; ++other) {
                             if (other == blockIdx.x) continue;
                             // the first of them has this unit last, the others first
-                            const int *from = static_cast<const int *>(p.shared) + ((int64_t)other * 2 + (first_of(other) < s0 + i - first_k)) * columns * TN + row;
+                            const int *from = static_cast<const int *>(p.shared) + ((int64_t)other * 2 + parts.second_place(other, s0 + i - first_k)) * columns * TN + row;
 #pragma unroll
                             for (int g = 0; g < DIGITS; ++g)
 #pragma unroll
@@ -626,8 +621,8 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
                     if (t0 >= s0 && t1 <= s1) {
                         for (int t = 0; t < a.tokens && there; ++t) store_result(a, t, n, l.sums[t * TN + row]);
                     } else {
-                        c0 = cta_of(t0), c1 = cta_of(t1 - 1);
-                        float *to = static_cast<float *>(p.shared) + ((int64_t)blockIdx.x * 2 + (t0 > s0)) * a.tokens * TN + row;
+                        c0 = parts.cta_of(t0), c1 = parts.cta_of(t1 - 1);
+                        float *to = static_cast<float *>(p.shared) + ((int64_t)blockIdx.x * 2 + parts.second_place(blockIdx.x, t0)) * a.tokens * TN + row;
                         for (int t = 0; t < a.tokens; ++t) __stcg(to + t * TN, l.sums[t * TN + row]);
                         if (came_last(p.counters + COUNTER_DOWN + c0, (int)(c1 - c0 + 1)) && row == 0) {
                             int *add = s.add[s.to_add];
@@ -665,7 +660,7 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
                         float4 v[ABREAST][ROWS];
 #pragma unroll
                         for (int j = 0; j < ABREAST; ++j) {
-                            const bool second = t0 > first_of(c + j);
+                            const bool second = parts.second_place(c + j, t0);
                             const float *from = static_cast<const float *>(p.shared) + ((int64_t)(c + j) * 2 + second) * a.tokens * TN + lane * 4;
 #pragma unroll
                             for (int r = 0; r < ROWS; ++r) {
@@ -688,7 +683,7 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
             if (a.tokens <= WARPS) add_up(std::integral_constant<int, 1>(), std::integral_constant<int, 12>());
             else add_up(std::integral_constant<int, 3>(), std::integral_constant<int, 4>());
         }
-        if (total == 0) {  // nobody is anyone's: the residual, or zeros
+        if (parts.total == 0) {  // nobody is anyone's: the residual, or zeros
             for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < (int64_t)a.tokens * a.hidden; i += (int64_t)gridDim.x * THREADS) store_result(a, (int)(i / a.hidden), (int)(i % a.hidden), 0.0f);
         }
         // the largest magnitudes are zero again when all CTAs have read them

@@ -27,13 +27,6 @@ struct I8Args {
     unsigned int *status;
 };
 
-// Which kernel takes a product whose operands and result lie in lines of 16 bytes, in tiles of how many tokens, and how many CTAs (pairs of them) share a tile's K.
-struct I8Plan {
-    bool pair = false;
-    int tm = 0, split = 1;
-};
-I8Plan plan_i8(int64_t M, int64_t N, int64_t K, int sms);
-
 // Every alignment and size.
 int launch_i8_any(const I8Args &p, cudaStream_t stream);
 // 16-byte aligned bases and rows of both operands and the result; tm tokens per tile, a multiple of 32 up to 256; split (1, 2 or 4) pairs that
