@@ -1,11 +1,11 @@
 // Tokens -> int8 codes with one float scale each, as they are or behind an RMS norm.
 //
 //     y = x,  or  y = x * w / sqrt(mean(x^2) + eps);   amax = max |y|,  code = rint(y * (127 / amax)),  scale = amax / 127
-// in float, but for the product inside rint, which is not rounded.  The factor 1 / sqrt(..) is the same for a whole row, so it cancels out of the codes: they are taken
+// in float, each operation rounded: where amax is 127 times a small number, products lie in the middle between whole numbers by the dozen, and only the rounded product says so.  The factor 1 / sqrt(..) is the same for a whole row, so it cancels out of the codes: they are taken
 // from x * w, and the factor stands in the scale alone.  So one round of sums and maxima over the row is enough, and the order of the sum never moves a code.
 //
 // A row is read once into registers, of a CTA or (up to 1024 elements) of a warp, as the bytes it has in memory, and widened twice.  Its floor is memory, 3 bytes an element
-// of 16 bits; close behind stand the instructions, some 4 an element: maxima are taken of 16-bit pairs, and one addition of 1.5 * 2^23, fused with the product,
+// of 16 bits; close behind stand the instructions, some 4 an element: maxima are taken of 16-bit pairs, and an addition of 1.5 * 2^23
 // rounds to a whole number that then stands in the sum's lowest byte.  Rows beyond 16384 elements are read a second time, from L2.
 #include "serving.cuh"
 
@@ -178,14 +178,14 @@ __global__ void __launch_bounds__(VECS == 0 ? MOST_THREADS : VECS == 4 ? 512 : 2
         if (bad) scale = __uint_as_float(0x7fc00000u);
         p.scales[row] = scale;
     }
-    const f32x2 by2 = pair_of(by, by), whole = pair_of(12582912.0f, 12582912.0f);
+    const f32x2 by2 = pair_of(by, by);
     auto put = [&](const f32x2 (&y)[4], int at) {
         uint32_t c[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float lo, hi;
-            halves(fma2(y[i], by2, whole), lo, hi);
-            c[2 * i] = __float_as_uint(lo), c[2 * i + 1] = __float_as_uint(hi);
+            halves(mul2(y[i], by2), lo, hi);
+            c[2 * i] = __float_as_uint(__fadd_rn(lo, 12582912.0f)), c[2 * i + 1] = __float_as_uint(__fadd_rn(hi, 12582912.0f));
         }
         uint2 q;
         q.x = keep & __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);

@@ -302,7 +302,7 @@ B200Q_API int b200q_qlinear_f16_i8_static(const void *a, const void *wq, const v
  * Tokens as int8 codes with one float scale each: row r of x (row_stride elements apart, of `type`, b200q_float_type) ->
  *   y = x, or, with norm (of x's type, [width]), y = x * norm / sqrt(mean(x^2) + eps);   amax = max |y|
  *   codes[r, i] = rint(y_i * (127 / amax)) (ties to even; dense rows of `width` bytes),   scales[r] = amax / 127
- * in float; behind the norm the codes are taken from x * norm, in which the row's factor cancels.  A row whose amax (of x, or of x * norm) is below 2^-100 is
+ * in float, each operation rounded; behind the norm the codes are taken from x * norm, in which the row's factor cancels.  A row whose amax (of x, or of x * norm) is below 2^-100 is
  * zeros with a scale of zero; a row with a NaN or an infinity, or whose squares overflow in front of a norm, has a scale of NaN (codes of zero in the first case).
  */
 B200Q_API int b200q_quantize_tokens(const void *x, int64_t row_stride, const void *norm, float eps, void *codes, float *scales, int64_t rows, int64_t width, int type,

@@ -48,13 +48,25 @@ def test_quantize_tokens(rows, width, dtype):
 
 
 @pytest.mark.parametrize('dtype', [F16, BF16, F32])
-def test_quantize_tokens_is_the_formula_in_float(dtype):
-    x = normal(generator(1), 64, 1536, dtype=dtype)
+@pytest.mark.parametrize('width', [200, 1536, 5000, 20000])
+def test_quantize_tokens_is_the_formula_in_float(width, dtype):
+    """Bit for bit, also where products lie in the middle between whole numbers: rows whose largest element is 127 times a small number, of multiples of half of that."""
+    gen = generator(1, width)
+    x = normal(gen, 64, width, dtype=F32)
+    small = torch.arange(1, 33, device='cuda').float()[:, None] * 2.0 ** -12
+    x[:32] = (torch.randint(-127, 127, (32, width), generator=gen, device='cuda') + 0.5) * small
+    x[:32, 7] = 127 * small[:, 0]
+    x = x.to(dtype)
     amax = x.float().abs().amax(-1, keepdim=True)
     codes, scales = hidet_b200.quantize_tokens(x)
-    by = torch.full_like(amax, 127.0) / amax  # rounded to float; the product of two floats is exact in 64 bits
-    assert torch.equal(codes, torch.round(x.double() * by.double()).to(torch.int8))
+    assert torch.equal(codes, torch.round(x.float() * (torch.full_like(amax, 127.0) / amax)).to(torch.int8))
     assert torch.equal(scales, (amax / torch.full_like(amax, 127.0))[:, 0])
+    norm = (1 + normal(gen, width, std=0.2)).to(dtype)
+    y = x.float() * norm.float()
+    amax = y.abs().amax(-1, keepdim=True)
+    assert torch.equal(hidet_b200.quantize_tokens(x, norm)[0], torch.round(y * (torch.full_like(amax, 127.0) / amax)).to(torch.int8))
+    ones = torch.ones_like(norm)
+    assert torch.equal(hidet_b200.quantize_tokens(x, ones)[0], codes)
 
 
 def test_quantize_tokens_of_any_strides_and_shapes():
