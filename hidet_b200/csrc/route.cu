@@ -3,10 +3,11 @@
 //     l[e] = sum_h x[h] r[e, h];   the `top` largest l, equal ones by index;   weight_j = exp(l_j - m) / sum exp(l - m)
 // over the chosen ones or over all, m the largest.  In float.
 //
-// Up to four tokens have a cluster of up to eight CTAs, a warp two experts at a time (or, of few experts, a share of their rows): a row of the router is read once for four tokens, a token's
-// element is widened once for two experts, and all logits meet in the first CTA's shared memory, where a warp a token puts them in order, every lane with its experts' keys
-// in registers.  A decode step's router is some KB to MB in L2: what takes the time is latency (launch, a row, the cluster's barrier, the choices one after the
-// other), so loads are asked for eight at a time.  One token, 8 experts, rows of 4096: 3.0 us; 7 tokens, 64 of 2048: 6.2; 48 tokens, 128 of 2048: 10.8.
+// A cluster of up to eight CTAs has eight tokens (four, in float or where rows are no whole vectors) and shares the experts; a row of the router is read once for them.  Tokens and router of one
+// 16-bit type are multiplied by tensor instructions, whose products are exact and whose sums are float; others by float ones.  All logits meet in the first CTA's shared
+// memory, where a warp a token puts them in order, every lane with its experts' keys in registers.  A decode step's router is some KB to MB in L2: what takes the time is
+// latency (launch, a row, the cluster's barrier, the choices one after the other), so loads are asked for eight at a time.  One token, 8 experts, rows of 4096:
+// 3.3 us; 7 tokens, 64 of 2048: 3.5; 48 tokens, 128 of 2048: 4.0 (float instructions: 2.9, 6.0 and 10.4); 512 tokens, 64 of 2048: 8.0.
 #include "serving.cuh"
 
 namespace b200q {
@@ -14,6 +15,7 @@ namespace {
 
 constexpr int WARPS = 8, THREADS = 32 * WARPS, MOST_CLUSTER = 8;
 constexpr int MOST_EXPERTS = 1024, MOST_TOKENS = 4, MOST_TOP = 32;
+constexpr int TOKENS_AT_ONCE = WARPS, STEPS = 8;  // of the kernel on tensor instructions: tokens of a cluster, 32 k each
 
 struct RouteArgs {
     const void *x, *router;
@@ -153,11 +155,95 @@ __global__ void __launch_bounds__(THREADS) route_kernel(const RouteArgs p) {
     else choose<MOST_EXPERTS / 32>(p, logits[warp], row, lane);
 }
 
+// D[16 x 8] += A[16 x 16] * B[16 x 8], experts by tokens.
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    mma_m16n8k16(d, a0, a1, a2, a3, b0, b1);
+}
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Tokens and router of one 16-bit type, in whole vectors.  A warp has 16 experts and a share of their rows; a lane's eight neighbouring k of a row, which one load brings, are the same eight of its
+// token's, so two instructions take 32 k of 16 experts and eight tokens from three loads, eight steps of which are under way.
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 1) route_mma_kernel(const RouteArgs p) {
+    __shared__ float logits[TOKENS_AT_ONCE][MOST_EXPERTS];  // of the cluster's first CTA
+    __shared__ float parts[WARPS][16][TOKENS_AT_ONCE];
+    const uint32_t rank = cluster_ctarank();
+    const int first = (int)(blockIdx.x / p.cluster) * TOKENS_AT_ONCE, tokens = min(TOKENS_AT_ONCE, p.tokens - first);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t logits0 = p.cluster > 1 ? map_to_rank(smem_u32(&logits[0][0]), 0) : 0u;
+    const int groups = (p.count + 16 * p.cluster - 1) / (16 * p.cluster), share = groups > 4 ? 1 : groups > 2 ? 2 : groups > 1 ? 4 : 8, part = warp % share;
+    pdl_launch_dependents();
+    cluster_arrive_release();  // this CTA is there
+    pdl_wait();
+    bool met = false;
+    const T *x = static_cast<const T *>(p.x) + (int64_t)(first + min(g, tokens - 1)) * p.x_stride;
+    for (int group = 0; group < groups; group += WARPS / share) {
+        const int e0 = 16 * ((group + warp / share) * p.cluster + (int)rank);
+        const bool some = group + warp / share < groups && e0 < p.count;
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (some) {
+            const T *r0 = static_cast<const T *>(p.router) + (int64_t)min(e0 + g, p.count - 1) * p.width, *r1 = static_cast<const T *>(p.router) + (int64_t)min(e0 + 8 + g, p.count - 1) * p.width;
+            for (int k0 = part * 32 * STEPS; k0 < p.width; k0 += share * 32 * STEPS) {
+                uint4 a0[STEPS], a1[STEPS], b[STEPS];
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const int k = k0 + 32 * i + 8 * t;
+                    a0[i] = a1[i] = b[i] = make_uint4(0, 0, 0, 0);
+                    if (k < p.width) {
+                        a0[i] = *reinterpret_cast<const uint4 *>(r0 + k), a1[i] = *reinterpret_cast<const uint4 *>(r1 + k);
+                        b[i] = *reinterpret_cast<const uint4 *>(x + k);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    mma<T>(d, a0[i].x, a1[i].x, a0[i].y, a1[i].y, b[i].x, b[i].y);
+                    mma<T>(d, a0[i].z, a1[i].z, a0[i].w, a1[i].w, b[i].z, b[i].w);
+                }
+            }
+        }
+        // d: experts g and g + 8, tokens 2 t and 2 t + 1
+        parts[warp][g][2 * t] = d[0], parts[warp][g][2 * t + 1] = d[1], parts[warp][g + 8][2 * t] = d[2], parts[warp][g + 8][2 * t + 1] = d[3];
+        __syncthreads();
+        if (!met) cluster_wait_acquire();  // the first CTA is there
+        met = true;
+        for (int i = threadIdx.x; i < WARPS / share * 16 * TOKENS_AT_ONCE; i += THREADS) {
+            const int of = i / (16 * TOKENS_AT_ONCE), e = i / TOKENS_AT_ONCE % 16, token = i % TOKENS_AT_ONCE, expert = 16 * ((group + of) * p.cluster + (int)rank) + e;
+            if (group + of >= groups || expert >= p.count || token >= tokens) continue;
+            float l = 0.0f;
+            for (int s = 0; s < share; ++s) l += parts[of * share + s][e][token];
+            if (p.cluster > 1) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(logits0 + (uint32_t)(token * MOST_EXPERTS + expert) * 4), "f"(l) : "memory");
+            else logits[token][expert] = l;
+        }
+        __syncthreads();
+    }
+    cluster_arrive_release();
+    cluster_wait_acquire();
+    if (rank != 0 || warp >= tokens) return;
+    const int64_t row = (int64_t)(first + warp) * p.top;
+    if (p.count <= 32) choose<1>(p, logits[warp], row, lane);
+    else if (p.count <= 128) choose<4>(p, logits[warp], row, lane);
+    else choose<MOST_EXPERTS / 32>(p, logits[warp], row, lane);
+}
+
 template <typename T, typename R>
 int launch_typed(const RouteArgs &p, bool vec, cudaStream_t stream) {
     const dim3 grid((unsigned)(ceil_div(p.tokens, MOST_TOKENS) * p.cluster));
     return vec ? launch_after("route_kernel", route_kernel<T, R, true>, grid, THREADS, 0, p.cluster, stream, p)
                : launch_after("route_kernel", route_kernel<T, R, false>, grid, THREADS, 0, p.cluster, stream, p);
+}
+template <typename T>
+int launch_mma(RouteArgs p, cudaStream_t stream) {
+    p.cluster = 1;
+    while (p.cluster < MOST_CLUSTER && 16 * p.cluster < p.count) p.cluster *= 2;
+    return launch_after("route_mma_kernel", route_mma_kernel<T>, dim3((unsigned)(ceil_div(p.tokens, TOKENS_AT_ONCE) * p.cluster)), THREADS, 0, p.cluster, stream, p);
 }
 
 }  // namespace
@@ -185,6 +271,8 @@ B200Q_API int b200q_route_tokens(const void *x, int64_t x_stride, const void *ro
     const RouteArgs p = {x, router, x_stride, experts, weights, (int)tokens, (int)width, (int)count, (int)top, cluster, over_all != 0};
     const bool vec = width % 8 == 0 && aligned_to(x, 16) && (tokens == 1 || x_stride * size % 16 == 0) && aligned_to(router, 16) && width * router_size % 16 == 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (vec && type == router_type && type == B200Q_F16) return launch_mma<__half>(p, s);
+    if (vec && type == router_type && type == B200Q_BF16) return launch_mma<__nv_bfloat16>(p, s);
     if (type == B200Q_F32) return launch_typed<float, float>(p, vec, s);
     if (type == B200Q_F16) return router_type == B200Q_F32 ? launch_typed<__half, float>(p, vec, s) : launch_typed<__half, __half>(p, vec, s);
     return router_type == B200Q_F32 ? launch_typed<__nv_bfloat16, float>(p, vec, s) : launch_typed<__nv_bfloat16, __nv_bfloat16>(p, vec, s);

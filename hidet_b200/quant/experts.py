@@ -23,6 +23,13 @@ from .tokens import rows_of
 MOST_EXPERTS, MOST_TOP = 1024, 32
 
 
+def lines_of(rows: torch.Tensor) -> torch.Tensor:
+    """Rows that begin on boundaries of 16 bytes, for loads of eight elements: a copy where they do not."""
+    if rows.data_ptr() % 16 != 0 or (rows.stride(0) % 8 != 0 and rows.shape[0] > 1):
+        return rows.clone(memory_format=torch.contiguous_format)
+    return rows
+
+
 def route_tokens(x: torch.Tensor, router: torch.Tensor, top_k: int, normalize: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
     """(experts, weights) [..., top_k], int32 and float32: the experts whose logits x @ router.T are the largest, descending, equal ones by index, and their shares of the
     softmax, over the chosen ones (normalize) or over all.
@@ -43,7 +50,7 @@ def route_tokens(x: torch.Tensor, router: torch.Tensor, top_k: int, normalize: b
         raise ValueError('{} experts: up to {} are supported'.format(count, MOST_EXPERTS))
     if not isinstance(top_k, int) or isinstance(top_k, bool) or not 1 <= top_k <= min(MOST_TOP, count):
         raise ValueError('top_k must be a whole number of 1 to {}, got {!r}'.format(min(MOST_TOP, count), top_k))
-    rows, router = rows_of(x), router.contiguous()
+    rows, router = lines_of(rows_of(x)), router.contiguous()
     experts = torch.empty(list(x.shape[:-1]) + [top_k], dtype=torch.int32, device=x.device)
     weights = torch.empty(list(x.shape[:-1]) + [top_k], dtype=torch.float32, device=x.device)
     with torch.cuda.device(x.device):
@@ -93,9 +100,7 @@ def mixture_of_experts(x: torch.Tensor, experts: torch.Tensor, weights: torch.Te
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     elif out.dtype != x.dtype or out.shape != x.shape or not out.is_contiguous():
         raise ValueError('out must be a contiguous tensor of {} {}'.format(x.dtype, list(x.shape)))
-    rows = rows_of(x)
-    if rows.data_ptr() % 16 != 0 or rows.stride(0) % 8 != 0:
-        rows = rows.clone(memory_format=torch.contiguous_format)  # loads of eight elements
+    rows = lines_of(rows_of(x))
     others = rows_of(residual) if residual is not None else None
     experts, weights, gate_up, down = experts.contiguous(), weights.contiguous(), gate_up.contiguous(), down.contiguous()
     gate_up_scale, down_scale = gate_up_scale.contiguous(), down_scale.contiguous()
