@@ -372,6 +372,7 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
             umma::Ring r;
             int i = 0;
             for (; i < mine; ++i, r.advance(1, stages)) {
+                if (DOWN && i == (int)stages) pdl_wait();  // the bounded waits do not run against the kernel in front
                 if (i >= (int)stages) wait(&s.empty[r.slot], r.phase ^ 1u, 1);
                 if (*reinterpret_cast<volatile int *>(&s.abort_flag) != 0) break;
                 const uint32_t bar = smem_u32(&s.weights[r.slot]);
@@ -387,6 +388,7 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
         if (DOWN) pdl_wait();
     } else if (warp == MMA_WARP) {
         // ---------------- products ----------------
+        if (DOWN) pdl_wait();
         if (elect_one()) {
             const uint32_t idesc = idesc_i8(TN, columns);
             umma::Ring r;
@@ -412,8 +414,6 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
             umma::commit(smem_u32(&s.drain));
             if (!mbar_wait(smem_u32(&s.drain), 0)) report_timeout(a.status, kKernelExperts, 8);
         }
-        __syncwarp();
-        if (DOWN) pdl_wait();
     } else if (warp >= 2) {
         if (DOWN) pdl_wait();  // h
         // ---------------- the powers of two of the rows that this CTA's entries have ----------------

@@ -601,6 +601,7 @@ PyObject *route_tokens(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     const int64_t width = x->size(-1), count = router->size(0), top = PyLong_AsLongLong(args[2]);
     Where w;
     PLAIN_OR_NONE(top >= 1 && top <= 32 && top <= count && where_is(*x, w) && router->get_device() == w.device);
+    PLAIN_OR_NONE(width % 8 != 0 || (reinterpret_cast<uintptr_t>(x->const_data_ptr()) & 15u) == 0);
     at::DimVector shape(x->sizes());
     shape.back() = top;
     at::Tensor experts = empty(shape, at::kInt, w.device), weights = empty(shape, at::kFloat, w.device);

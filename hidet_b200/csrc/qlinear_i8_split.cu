@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(THREADS) i8_split_kernel(const __grid_constant
         for (int j = max(0, i - (int)stages); j < i; ++j)
             if (!mbar_wait(smem_u32(&full[(uint32_t)j % stages]), ((uint32_t)j / stages) & 1)) report_timeout(p.a.status, kKernelI8Split, 7);
     } else if (warp == MMA_WARP && elect_one()) {
+        pdl_wait();  // the bounded waits do not run against the kernel in front
         const uint32_t idesc = idesc_i8(TN, p.tm, !NK);
         constexpr uint32_t W_STEP = NK ? 32 / 16 : 32 * TN / 16;
         for (int i = 0; i < blocks; ++i) {

@@ -1,8 +1,9 @@
 // Tokens -> int8 codes with one float scale each, as they are or behind an RMS norm.
 //
 //     y = x,  or  y = x * w / sqrt(mean(x^2) + eps);   amax = max |y|,  code = rint(y * (127 / amax)),  scale = amax / 127
-// in float, each operation rounded: where amax is 127 times a small number, products lie in the middle between whole numbers by the dozen, and only the rounded product says so.  The factor 1 / sqrt(..) is the same for a whole row, so it cancels out of the codes: they are taken
-// from x * w, and the factor stands in the scale alone.  So one round of sums and maxima over the row is enough, and the order of the sum never moves a code.
+// in float, each operation rounded: where amax is 127 times a small number, products lie in the middle between whole numbers by the dozen, and only the rounded
+// product says so.  The factor 1 / sqrt(..) is the same for a whole row, so it cancels out of the codes: they are taken from x * w, and the factor stands in the scale
+// alone.  So one round of sums and maxima over the row is enough, and the order of the sum never moves a code.
 //
 // A row is read once into registers, of a CTA or (up to 1024 elements) of a warp, as the bytes it has in memory, and widened twice.  Its floor is memory, 3 bytes an element
 // of 16 bits; close behind stand the instructions, some 4 an element: maxima are taken of 16-bit pairs, and an addition of 1.5 * 2^23

@@ -24,7 +24,9 @@ MOST_EXPERTS, MOST_TOP = 1024, 32
 
 
 def lines_of(rows: torch.Tensor) -> torch.Tensor:
-    """Rows that begin on boundaries of 16 bytes, for loads of eight elements: a copy where they do not."""
+    """Rows that begin on boundaries of 16 bytes, for loads of eight elements: a copy where they do not and a copy's would."""
+    if rows.shape[1] % 8 != 0:
+        return rows
     if rows.data_ptr() % 16 != 0 or (rows.stride(0) % 8 != 0 and rows.shape[0] > 1):
         return rows.clone(memory_format=torch.contiguous_format)
     return rows

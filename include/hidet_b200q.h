@@ -331,9 +331,12 @@ B200Q_API int b200q_route_tokens(const void *x, int64_t x_stride, const void *ro
  * The experts' part of the layer, on int8 weights: out[t] (f16 or bf16, of x's type, dense) =
  *   residual[t] + sum_j weights[t, j] * down_scale[e] (down[e] h),   h = silu(g) * u,   (g, u) = gate_up_scale[e] (gate_up[e] x[t]),   e = experts[t, j]
  * gate_up int8 [count, 2 inner, hidden], its rows (gate_f, up_f) pairs at (2 f, 2 f + 1); down int8 [count, hidden, inner]; scales of scale_type, one for each row; both are what
- * b200q_symmetric_quantize makes of the rows of all experts.  Sums are float; x and h are rounded to f16, a row at a time scaled by a power of two where
- * their range asks for it.  The results do not depend on the run.  out may be residual, or x.  An assignment to a negative expert is passed over, one to an expert that is not there too, and is
- * reported by b200q_check_status.  The workspace is one of b200q_qlinear_f16_i8's kind.
+ * b200q_symmetric_quantize makes of the rows of all experts.  Products with a row of x or h are taken of whole numbers of 23 bits: an element is held to 2^-22 of the largest in its row
+ * (a row whose largest is below 2^-98 is zeros), and the sums over 128 of them or more are exact; all that follows is float.  A row with a NaN or an infinity gives NaN.  Where hidden, inner,
+ * x_stride and the bases are not all multiples of 16 bytes' worth, or there are more than 512 experts, slower kernels take the call, with products and sums in float.
+ * The results do not depend on the run.  out may be residual, or x.  An assignment to a negative expert is passed over, one to an expert that is not there too, and the latter is
+ * reported by b200q_check_status.  The weights are read once for 64 tokens (for fewer, where these have more than 1024 assignments).
+ * The workspace is one of b200q_qlinear_f16_i8's kind.
  */
 B200Q_API size_t b200q_mixture_of_experts_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top);
 B200Q_API int b200q_mixture_of_experts(const void *x, int64_t x_stride, const int32_t *experts, const float *weights, const void *gate_up, const void *gate_up_scale,

@@ -5,7 +5,7 @@ import torch
 import hidet_b200
 import token_reference as ref
 from hidet_b200 import ffi
-from test_tokens_gpu import BF16, F16, F32, codes_of, generator, normal
+from test_tokens_gpu import BF16, F16, F32, codes_of, far_rows, generator, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -226,3 +226,47 @@ def test_refusals():
                        (lambda: f(x, e, p, *w, out=x.float()), 'out')):
         with pytest.raises(ValueError, match=text):
             call()
+
+
+def test_tokens_far_apart_and_weights_beyond_32_bits():
+    gen = generator(19)
+    x, router = far_rows(gen, 3, 512, (1 << 30) + 8, BF16), normal(gen, 24, 512, dtype=BF16)
+    got, want = hidet_b200.route_tokens(x, router, 4), hidet_b200.route_tokens(x.contiguous(), router, 4)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    w = layer(gen, 24, 512, 272)
+    assert torch.equal(hidet_b200.mixture_of_experts(x, *got, *w, residual=x), hidet_b200.mixture_of_experts(x.contiguous(), *got, *w, residual=x.contiguous()))
+    del x
+    count, hidden, inner = 40, 8192, 7008  # 4.6 and 2.3 GB
+    last = layer(gen, 1, hidden, inner)
+    gate_up, down = torch.empty(count, 2 * inner, hidden, dtype=torch.int8, device='cuda'), torch.empty(count, hidden, inner, dtype=torch.int8, device='cuda')
+    gate_up[-1:], down[-1:] = last[0], last[2]
+    x, weights = normal(gen, 2, hidden, dtype=F16), torch.ones(2, 1, device='cuda')
+    chosen = torch.full((2, 1), count - 1, dtype=torch.int32, device='cuda')
+    got = hidet_b200.mixture_of_experts(x, chosen, weights, gate_up, last[1].expand(count, -1), down, last[3].expand(count, -1))
+    assert torch.equal(got, hidet_b200.mixture_of_experts(x, torch.zeros_like(chosen), weights, *last))
+
+
+@pytest.mark.parametrize('hidden,inner', [(512, 256), (100, 36)])
+def test_two_layers_at_once(hidden, inner):
+    """Two streams with layers of their own, a hundred calls under way, beside linears on int8 tokens."""
+    gen = generator(20, hidden)
+    layers = [layer(gen, 8, hidden, inner) for _ in range(2)]
+    xs = [normal(gen, n, hidden, dtype=F16) for n in (3, 40)]
+    picks = [choices(gen, n, 8, 2) for n in (3, 40)]
+    wq, scale = codes_of(gen, hidden, hidden), torch.full((hidden,), 1e-3, device='cuda')
+
+    def step(i):
+        y = hidet_b200.mixture_of_experts(xs[i], *picks[i], *layers[i])
+        return hidet_b200.symmetric_quant_matmul_i8(*hidet_b200.quantize_tokens(y), wq, scale)
+
+    want = [step(0), step(1)]
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(50):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+    assert ffi.func('b200q_check_status')() == ffi.OK

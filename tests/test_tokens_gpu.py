@@ -261,3 +261,43 @@ def test_refusals():
             call()
     with pytest.raises(ffi.BackendException, match='eps'):
         hidet_b200.quantize_tokens(x, eps=-1.0)
+
+
+# ---- beyond 32 bits ----
+
+def far_rows(gen, rows, width, stride, dtype):
+    """Rows that lie `stride` elements apart, in memory of which nothing else is written."""
+    x = torch.empty((rows - 1) * stride + width, dtype=dtype, device='cuda').as_strided((rows, width), (stride, 1))
+    x.copy_(normal(gen, rows, width, dtype=dtype))
+    return x
+
+
+def test_tokens_far_apart_and_many():
+    gen = generator(30)
+    x = far_rows(gen, 3, 520, (1 << 30) + 8, BF16)
+    codes, scales = hidet_b200.quantize_tokens(x)
+    want = hidet_b200.quantize_tokens(x.contiguous())
+    assert torch.equal(codes, want[0]) and torch.equal(scales, want[1])
+    del x
+    x = torch.zeros((1 << 18) + 40, 8192, dtype=BF16, device='cuda')  # more than 2^31 elements
+    x[-40:] = normal(gen, 40, 8192, dtype=BF16)
+    codes, scales = hidet_b200.quantize_tokens(x)
+    want = hidet_b200.quantize_tokens(x[-40:].clone())
+    assert torch.equal(codes[-40:], want[0]) and torch.equal(scales[-40:], want[1]) and not scales[:-40].any()
+
+
+@pytest.mark.parametrize('m,k,n', [((1 << 18) + 40, 8192, 16), ((1 << 17) + 40, 64, 16400), ((1 << 17) + 41, 62, 16402)])
+def test_products_of_more_than_32_bits_of_elements(m, k, n):
+    gen = generator(31, n)
+    a, scales = torch.zeros(m, k, dtype=torch.int8, device='cuda'), torch.ones(m, device='cuda')
+    a[-40:] = codes_of(gen, 40, k)
+    w, scale = codes_of(gen, k, n), torch.full((n,), 1e-3, device='cuda')
+    r = torch.zeros(m, n, dtype=F16, device='cuda')
+    r[-40:] = normal(gen, 40, n, dtype=F16)
+    added = r[-40:].clone()
+    got = hidet_b200.symmetric_quant_matmul_i8(a, scales, w, scale, residual=r, out=r)
+    assert not got[:-40].any()
+    # the sum is exact; its product with the scale is one rounding, the addition another, the result the last
+    want = (a[-40:].double() @ w.double()) * scale.double()
+    both = want + added.double()
+    assert torch.all((got[-40:].double() - both).abs() <= both.abs() * 2.0 ** -11 + (want.abs() + both.abs()) * 2.0 ** -23 + 2.0 ** -24)
