@@ -1,5 +1,6 @@
-// A layer of experts over a few tokens, on int8 weights: the entry point, and the kernels that take every alignment.
+// A layer of experts on int8 weights: the entry point, and the kernels that take every alignment.
 #include "experts.h"
+#include "experts_digits.cuh"
 #include "serving.cuh"
 
 namespace b200q {
@@ -7,14 +8,6 @@ namespace {
 
 constexpr int ANY_WARPS = 8;
 
-__device__ __forceinline__ float scale_at(const void *p, int type, int64_t i) {
-    if (type == B200Q_F16) return __half2float(static_cast<const __half *>(p)[i]);
-    if (type == B200Q_BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-    return static_cast<const float *>(p)[i];
-}
-__device__ __forceinline__ float value_at(const void *p, int type, int64_t i) {
-    return type == B200Q_F16 ? __half2float(static_cast<const __half *>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -38,7 +31,7 @@ __global__ void __launch_bounds__(32 * ANY_WARPS) experts_any_up_kernel(const Ex
         const int8_t *w = p.gate_up + row * p.hidden;
         float g = 0.0f, u = 0.0f;
         for (int i = lane; i < p.hidden; i += 32) {
-            const float x = value_at(p.x, p.type, a / p.top * p.x_stride + i);
+            const float x = token_value(p.x, p.type, a / p.top * p.x_stride + i);
             g = fmaf(x, (float)w[i], g);
             u = fmaf(x, (float)w[p.hidden + i], u);
         }
@@ -64,7 +57,7 @@ __global__ void __launch_bounds__(32 * ANY_WARPS) experts_any_down_kernel(const 
             sum = fmaf(warp_sum(y) * scale_at(p.down_scale, p.scale_type, row), p.weights[a], sum);
         }
         if (lane == 0) {
-            if (p.residual != nullptr) sum += value_at(p.residual, p.type, t * p.residual_stride + n);
+            if (p.residual != nullptr) sum += token_value(p.residual, p.type, t * p.residual_stride + n);
             const int64_t at = (int64_t)t * p.hidden + n;
             if (p.type == B200Q_F16) static_cast<__half *>(p.out)[at] = __float2half_rn(sum);
             else static_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(sum);
@@ -84,6 +77,18 @@ int launch_any(const ExpertsArgs &p, float *h, cudaStream_t stream) {
                         32 * ANY_WARPS, 0, 1, stream, p, h);
 }
 
+// Whether the tokens are many: made digits of once, for all tiles of the weights (experts_many.cu), or by every tile for itself (experts_stream.cu).  The latter pays by the assignment and tile,
+// and at its shared parts by an expert's assignments; the former some 7 us for the kernels in front, between and behind.  us, the latter and the former:
+//     8 and 16 tokens, 2 of 8 experts of 4096 x 14336       210 216    250 242       32 and 64: 276 249    330 261
+//     24 and 64 tokens, 6 of 64 of 2048 x 1408               95 99     112 107       48 tokens, 8 of 128 of 2048 x 768: 111 113
+//     16 and 32 tokens, 2 of 4 of 1024 x 4096                28 34      37 37        32 tokens, 8 of 8 of 512 x 1024: 36 27
+//     32 and 64 tokens, 2 of 16 of 2048 x 8192              139 147    156 152
+// More than 64 tokens would have the weights read again by the latter (128 tokens, 2 of 8 of 4096 x 14336: 655 300).
+bool are_many(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top) {
+    const double assignments = (double)tokens * (double)top;
+    return tokens > kExpertsTokens || assignments / (double)(count > 0 ? count : 1) + 1.5e-8 * assignments * (double)hidden * (double)inner > 21.0;
+}
+
 }  // namespace
 }  // namespace b200q
 
@@ -92,7 +97,9 @@ extern "C" {
 B200Q_API size_t b200q_mixture_of_experts_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top) {
     using namespace b200q;
     if (tokens <= 0 || hidden <= 0 || inner < 0 || count < 0 || top <= 0) return 0;
-    return kWorkspaceHead + experts_stream_bytes(experts_at_once(tokens, top), inner, top);
+    const size_t few = experts_stream_bytes(experts_at_once(tokens, top), inner, top);
+    const size_t many = are_many(tokens, hidden, inner, count, top) ? experts_many_bytes(experts_many_at_once(tokens, hidden, inner, count, top), hidden, inner, count, top) : 0;
+    return kWorkspaceHead + (few > many ? few : many);
 }
 
 B200Q_API int b200q_mixture_of_experts(const void *x, int64_t x_stride, const int32_t *experts, const float *weights, const void *gate_up, const void *gate_up_scale,
@@ -123,15 +130,19 @@ B200Q_API int b200q_mixture_of_experts(const void *x, int64_t x_stride, const in
     p.tokens = (int)tokens, p.hidden = (int)hidden, p.inner = (int)inner, p.count = (int)count, p.top = (int)top, p.scale_type = scale_type, p.type = type;
     p.status = device_status_word();
     float *scratch = reinterpret_cast<float *>(static_cast<char *>(workspace) + kWorkspaceHead);
-    const int64_t at_once = experts_at_once(tokens, top);
+    const bool fast = experts_fast(p), many = fast && are_many(tokens, hidden, inner, count, top);
+    const int64_t at_once = many ? experts_many_at_once(tokens, hidden, inner, count, top) : experts_at_once(tokens, top);
     for (int64_t t = 0; t < tokens; t += at_once) {
         ExpertsArgs q = p;
         q.tokens = (int)(tokens - t < at_once ? tokens - t : at_once);
         q.x = static_cast<const uint16_t *>(x) + t * x_stride, q.out = static_cast<uint16_t *>(out) + t * hidden;
         if (top > 0) q.experts = experts + t * top, q.weights = weights + t * top;
         if (residual != nullptr) q.residual = static_cast<const uint16_t *>(residual) + t * residual_stride;
-        const int rc = experts_stream_supported(q) ? launch_experts_stream(q, static_cast<unsigned int *>(workspace), scratch, static_cast<cudaStream_t>(stream))
-                                                   : launch_any(q, scratch, static_cast<cudaStream_t>(stream));
+        unsigned int *counters = static_cast<unsigned int *>(workspace);
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const int rc = many                                            ? launch_experts_many(q, counters, scratch, s)
+                       : fast && at_once * top <= kExpertsAssignments ? launch_experts_stream(q, counters, scratch, s)
+                                                                       : launch_any(q, scratch, s);
         if (rc != B200Q_OK) return rc;
     }
     return B200Q_OK;

@@ -27,7 +27,7 @@ struct ExpertsArgs {
     unsigned int *status;
 };
 
-// Tokens of one launch: 64, or as many as have 1024 assignments.
+// Few tokens of one launch: 64, or as many as have 1024 assignments.
 constexpr int64_t kExpertsTokens = 64, kExpertsAssignments = 1024;
 inline int64_t experts_at_once(int64_t tokens, int64_t top) {
     int64_t most = top * kExpertsTokens > kExpertsAssignments ? kExpertsAssignments / top : kExpertsTokens;
@@ -35,9 +35,14 @@ inline int64_t experts_at_once(int64_t tokens, int64_t top) {
     return tokens < most ? tokens : most;
 }
 
-// Rows and bases in lines of 16 bytes, up to 512 experts; tokens of one launch.
-bool experts_stream_supported(const ExpertsArgs &p);
+// Rows and bases in lines of 16 bytes, up to 512 experts.
+bool experts_fast(const ExpertsArgs &p);
+// Few tokens, those of one launch.
 size_t experts_stream_bytes(int64_t tokens, int64_t inner, int64_t top);
 int launch_experts_stream(const ExpertsArgs &p, unsigned int *counters, float *scratch, cudaStream_t stream);
+// Many, as many as one launch takes.
+int64_t experts_many_at_once(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top);
+size_t experts_many_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top);
+int launch_experts_many(const ExpertsArgs &p, unsigned int *counters, void *scratch, cudaStream_t stream);
 
 }  // namespace b200q

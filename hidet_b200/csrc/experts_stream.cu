@@ -5,7 +5,8 @@
 // element, so that an element is off by at most 2^-22 of that), and these as three digits of 8 bits, v = 65536 d2 + 256 d1 + d0 with d in -128 .. 127.  A tile of 128 rows of the weight is the
 // first operand of tcgen05.mma, three columns for each token are the second, sums of 32 bits are exact, and float begins behind them.  So weights are only ever copied,
 // and what is computed on them costs no issue slots.  (As f16 by mma.sync, with int8 widened in registers, a tile took 260 instructions of each of eight warps, and the
-// stream stood at 3.2 TB/s.)
+// stream stood at 3.2 TB/s.)  One token, two of eight experts of 4096 x 14336: 65 us, 5.4 TB/s; 8 tokens 210 us, 6.0 TB/s; 7 tokens, six of 64 of 2048 x 1408: 56 us.  What is not the stream
+// is some 5 us at the start of either kernel (launch, entries, first loads) and the meeting of parts at its end.
 //
 // Every CTA makes the list of entries, an expert with up to C of its assignments (an expert with more has several entries), and takes an equal, contiguous part of
 // all stages, 128 rows x 128 k each.  Warps:
@@ -25,6 +26,7 @@
 #include <type_traits>
 
 #include "experts.h"
+#include "experts_digits.cuh"
 #include "experts_parts.cuh"
 #include "serving.cuh"
 #include "umma.cuh"
@@ -35,18 +37,15 @@ namespace {
 constexpr unsigned int kKernelExperts = 11;
 constexpr int TN = 128, BK = 128;         // rows and k of a stage
 constexpr int W_BYTES = TN * BK;
-constexpr int DIGITS = 3;
 constexpr int COPY_WARP = 0, MMA_WARP = 1, FINISH_WARP0 = 4, DIGIT_WARP0 = 8, TEAMS = 4;
 constexpr int ITEMS = BK / 8;             // of a column in a stage, a thread's eight elements each
-// Warps of a team: with more than a dozen assignments an expert, whose rows come from L2, four keep enough of them on their way (64 tokens, two of eight experts: 350 us with two, 281
-// with four); with fewer they are in each other's way (32 tokens: 235 and 248).
-constexpr int MANY = 12;
-__host__ __device__ constexpr int threads_of(int team) { return 32 * (DIGIT_WARP0 + team * TEAMS); }
+constexpr int TEAM = 2;                   // warps
+constexpr int THREADS = 32 * (DIGIT_WARP0 + TEAM * TEAMS), WARPS = THREADS / 32;
+constexpr int WIDE = 2;                   // columns at a time that results are made of: the code is short, and most of its first run is waiting for it
 constexpr int MOST_STAGES = 10;
 constexpr int MOST_SMEM = 227 * 1024;
 constexpr int MOST_ASSIGNMENTS = kExpertsAssignments;
 constexpr int MOST_EXPERTS = 512;
-constexpr int kMostExact = 131071;        // products of 2^14 whose sum 32 bits hold
 constexpr uint16_t kNone = 0xffff;
 // what of the workspace's counters is whose: arrivals at what CTAs share (by the first of them), CTAs that are through, h's largest magnitudes
 constexpr int MOST_CTAS = 1024, COUNTER_UP = 0, COUNTER_DOWN = MOST_CTAS, COUNTER_DONE = 2 * MOST_CTAS, COUNTER_MAX = 4 * MOST_CTAS;
@@ -73,66 +72,6 @@ struct Entry {
     uint16_t expert, first, count;  // its assignments are order[first ..]
 };
 
-__device__ __forceinline__ float scale_at(const void *p, int type, int64_t i) {
-    if (type == B200Q_F16) return __half2float(static_cast<const __half *>(p)[i]);
-    if (type == B200Q_BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-    return static_cast<const float *>(p)[i];
-}
-
-// The power of two that brings a row's largest magnitude (as bits) to 2^21 .. 2^22, and its inverse.  Rows below 2^-98 are zeros; rows with an infinity or a NaN are NaN.
-__device__ __forceinline__ float power_for(uint32_t bits, float &inverse) {
-    const int e = 148 - (int)(bits >> 23);  // 127 + 21 - exponent
-    const bool zero = e > 119;
-    inverse = bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : zero ? 0.0f : __uint_as_float((uint32_t)(127 - e) << 23);
-    return zero || bits >= 0x7f800000u ? 0.0f : __uint_as_float((uint32_t)(127 + e) << 23);
-}
-
-// Eight neighbouring elements of a token.
-struct FromF16 {
-    typedef uint4 Raw[1];
-    static __device__ __forceinline__ void load(const void *row, int k, Raw &r) { r[0] = *reinterpret_cast<const uint4 *>(static_cast<const __half *>(row) + k); }
-    static __device__ __forceinline__ void widen(uint32_t w, float &lo, float &hi) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-        lo = f.x, hi = f.y;
-    }
-    static __device__ __forceinline__ uint32_t largest(uint32_t bits, uint32_t w) {  // as float's
-        return max(bits, max(__float_as_uint(__half2float(__ushort_as_half((uint16_t)(w & 0x7fffu)))), __float_as_uint(__half2float(__ushort_as_half((uint16_t)(w >> 16 & 0x7fffu))))));
-    }
-};
-struct FromBF16 {
-    typedef uint4 Raw[1];
-    static __device__ __forceinline__ void load(const void *row, int k, Raw &r) { FromF16::load(row, k, r); }
-    static __device__ __forceinline__ void widen(uint32_t w, float &lo, float &hi) { lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u); }
-    static __device__ __forceinline__ uint32_t largest(uint32_t bits, uint32_t w) { return max(bits, max(w << 16 & 0x7fff0000u, w & 0x7fff0000u)); }
-};
-struct FromF32 {
-    typedef uint4 Raw[2];
-    static __device__ __forceinline__ void load(const void *row, int k, Raw &r) {
-        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const float *>(row) + k);
-        r[0] = p[0], r[1] = p[1];
-    }
-};
-template <typename X>
-__device__ __forceinline__ void widen4(const typename X::Raw &r, int i, float (&f)[4]) {
-    X::widen(i ? r[0].z : r[0].x, f[0], f[1]);
-    X::widen(i ? r[0].w : r[0].y, f[2], f[3]);
-}
-template <>
-__device__ __forceinline__ void widen4<FromF32>(const FromF32::Raw &r, int i, float (&f)[4]) {
-    f[0] = __uint_as_float(r[i].x), f[1] = __uint_as_float(r[i].y), f[2] = __uint_as_float(r[i].z), f[3] = __uint_as_float(r[i].w);
-}
-
-// The digits of four elements, a word each: adding 1.5 * 2^23 rounds to a whole number that stands in the sum's low bits, and with 128 added to each digit they are its bytes.
-__device__ __forceinline__ void digits_of(const float (&f)[4], float by, uint32_t (&d)[DIGITS]) {
-    uint32_t u[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(fmaf(f[i], by, 12582912.0f)) + (0x808080u - 0x4b400000u);
-    const uint32_t lo = __byte_perm(u[0], u[1], 0x5140), hi = __byte_perm(u[2], u[3], 0x5140);
-    d[0] = __byte_perm(lo, hi, 0x5410) ^ 0x80808080u;
-    d[1] = __byte_perm(lo, hi, 0x7632) ^ 0x80808080u;
-    d[2] = __byte_perm(__byte_perm(u[0], u[1], 0x0062), __byte_perm(u[2], u[3], 0x0062), 0x5410) ^ 0x80808080u;
-}
-
 __device__ __forceinline__ uint32_t idesc_i8(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 __device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -145,12 +84,6 @@ __device__ __forceinline__ void mma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_
 }
 __device__ __forceinline__ void ld_columns(uint32_t taddr, int (&v)[2]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void ld_columns(uint32_t taddr, int (&v)[8]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                 : "r"(taddr)
-                 : "memory");
 }
 
 struct alignas(16) Shared {
@@ -187,7 +120,7 @@ struct Lists {
 
 // The entries of a launch: counts by expert and the tokens that they are of, a sum over the experts, assignments in their places.  Every CTA makes them for itself, so an
 // expert's assignments stand in their own order: as they come they would differ from CTA to CTA, and with them whose column is whose.  `meanwhile` runs while the experts are on their way.
-template <int THREADS, typename F>
+template <typename F>
 __device__ __forceinline__ void make_entries(const ExpertsArgs &a, int columns, Shared &s, const Lists &l, F meanwhile) {
     const int n = a.tokens * a.top;
     for (int e = threadIdx.x; e < a.count; e += THREADS) l.counts[e] = 0, l.who[e] = make_uint2(0, 0);
@@ -278,9 +211,6 @@ struct Place {
     }
 };
 
-__device__ __forceinline__ float token_value(const void *p, int type, int64_t i) {
-    return type == B200Q_F16 ? __half2float(static_cast<const __half *>(p)[i]) : __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-}
 __device__ __forceinline__ void store_result(const ExpertsArgs &a, int t, int n, float v) {
     if (a.residual != nullptr) v += token_value(a.residual, a.type, t * a.residual_stride + n);
     const int64_t at = (int64_t)t * a.hidden + n;
@@ -289,9 +219,8 @@ __device__ __forceinline__ void store_result(const ExpertsArgs &a, int t, int n,
 }
 
 // X: what the tokens are; DOWN: h, else x.
-template <bool DOWN, int TEAM, typename X>
-__global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(const __grid_constant__ CUtensorMap map_w, const StreamArgs p) {
-    constexpr int THREADS = threads_of(TEAM), WARPS = THREADS / 32;
+template <bool DOWN, typename X>
+__global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid_constant__ CUtensorMap map_w, const StreamArgs p) {
     extern __shared__ unsigned char smem_dyn[];
     const uint32_t ring = (smem_u32(smem_dyn) + 1023u) & ~1023u;
     unsigned char *ring_gen = smem_dyn + (ring - smem_u32(smem_dyn));
@@ -323,7 +252,7 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
     if (!DOWN) pdl_wait();
     umma::fence_before_sync();
     // The largest magnitudes of a few tokens, a warp 1024 elements at a time, in front of the weights' requests, behind which they would wait.
-    make_entries<THREADS>(a, p.most, s, l, [&]() {
+    make_entries(a, p.most, s, l, [&]() {
         if constexpr (!DOWN) {
             const int pieces = (K + 1023) / 1024;
             for (int i = warp; a.tokens <= EARLY_TOKENS && i < a.tokens * pieces; i += WARPS) {
@@ -505,7 +434,6 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
             }
         } else if (warp >= FINISH_WARP0) {
             // ---------------- results ----------------
-            constexpr int WIDE = TEAM == 4 ? 8 : 2;  // columns at a time
             const int q = warp - FINISH_WARP0, row = 32 * q + lane;
             const uint32_t lane_addr = tmem_base + ((uint32_t)(32 * q) << 16);
             auto meet = [&]() { asm volatile("bar.sync 2, 128;" ::: "memory"); };
@@ -559,7 +487,6 @@ __global__ void __launch_bounds__(threads_of(TEAM), 1) experts_stream_kernel(con
                     }
                     finish = came_last(p.counters + COUNTER_UP + c0, (int)(c1 - c0 + 1));
                 }
-                // With few columns two at a time: the code is short, and most of its first run is waiting for it.
 #pragma unroll 1
                 for (int c = 0; finish && c < en.count; c += WIDE) {
                     int v[DIGITS][WIDE];
@@ -704,7 +631,7 @@ int grid_of() {
     return sms < MOST_CTAS ? sms : MOST_CTAS;
 }
 
-template <bool DOWN, int TEAM, typename X>
+template <bool DOWN, typename X>
 int launch_stream(const CUtensorMap &map, StreamArgs p, cudaStream_t stream) {
     const ExpertsArgs &a = p.a;
     const int rows = DOWN ? a.hidden : 2 * a.inner, K = DOWN ? a.inner : a.hidden;
@@ -714,23 +641,17 @@ int launch_stream(const CUtensorMap &map, StreamArgs p, cudaStream_t stream) {
     static_assert((MOST_SMEM - 2048 - (int)sizeof(Shared) - Lists::bytes(MOST_ASSIGNMENTS, MOST_EXPERTS, kExpertsTokens)) / (W_BYTES + sixteens(columns_for(kExpertsTokens)) * BK) >= TEAMS,
                   "a stage for every team, whatever the sizes");
     static std::atomic<bool> attr_set[64];
-    const int rc = allow_smem(attr_set, experts_stream_kernel<DOWN, TEAM, X>, MOST_SMEM);
+    const int rc = allow_smem(attr_set, experts_stream_kernel<DOWN, X>, MOST_SMEM);
     if (rc != B200Q_OK) return rc;
-    return launch_after("experts_stream_kernel", experts_stream_kernel<DOWN, TEAM, X>, dim3((unsigned)grid_of()), threads_of(TEAM), (size_t)(1024 + p.ring_bytes + shared), 1, stream, map, p);
-}
-
-template <int TEAM>
-int launch_both(const CUtensorMap &up, const CUtensorMap &down, const StreamArgs &p, cudaStream_t stream) {
-    const int rc = p.a.type == B200Q_F16 ? launch_stream<false, TEAM, FromF16>(up, p, stream) : launch_stream<false, TEAM, FromBF16>(up, p, stream);
-    return rc != B200Q_OK ? rc : launch_stream<true, TEAM, FromF32>(down, p, stream);
+    return launch_after("experts_stream_kernel", experts_stream_kernel<DOWN, X>, dim3((unsigned)grid_of()), THREADS, (size_t)(1024 + p.ring_bytes + shared), 1, stream, map, p);
 }
 
 }  // namespace
 
-bool experts_stream_supported(const ExpertsArgs &a) {
+bool experts_fast(const ExpertsArgs &a) {
     return a.hidden % 16 == 0 && a.inner % 16 == 0 && a.inner > 0 && aligned_to(a.x, 16) && (a.tokens == 1 || a.x_stride % 8 == 0) && aligned_to(a.gate_up, 16) && aligned_to(a.down, 16) &&
-           a.count > 0 && a.count <= MOST_EXPERTS && a.top > 0 && a.tokens * a.top <= MOST_ASSIGNMENTS && a.hidden <= kMostExact && a.inner <= kMostExact &&
-           (int64_t)a.count * 2 * a.inner < 0x7fffff00LL && (int64_t)a.count * a.hidden < 0x7fffff00LL;
+           a.count > 0 && a.count <= MOST_EXPERTS && a.top > 0 && a.hidden <= kMostExact && a.inner <= kMostExact && (int64_t)a.count * 2 * a.inner < 0x7fffff00LL &&
+           (int64_t)a.count * a.hidden < 0x7fffff00LL;
 }
 
 size_t experts_stream_bytes(int64_t tokens, int64_t inner, int64_t top) {
@@ -751,8 +672,9 @@ int launch_experts_stream(const ExpertsArgs &a, unsigned int *counters, float *s
     p.h = scratch, p.shared = scratch + round_up((int64_t)a.tokens * a.top * a.inner, 64), p.counters = counters;
     p.most = columns_for(a.tokens);
     p.tmem_cols = 32;
-    while ((int)p.tmem_cols < 2 * sixteens(p.most) + 8) p.tmem_cols *= 2;  // up to eight columns are read at a time, some of them behind the last
-    return (int64_t)a.tokens * a.top > (int64_t)MANY * a.count ? launch_both<4>(up, down, p, stream) : launch_both<2>(up, down, p, stream);
+    while ((int)p.tmem_cols < 2 * sixteens(p.most) + WIDE) p.tmem_cols *= 2;  // some columns are read behind the last
+    rc = a.type == B200Q_F16 ? launch_stream<false, FromF16>(up, p, stream) : launch_stream<false, FromBF16>(up, p, stream);
+    return rc != B200Q_OK ? rc : launch_stream<true, FromF32>(down, p, stream);
 }
 
 }  // namespace b200q

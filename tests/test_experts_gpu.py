@@ -100,6 +100,19 @@ def test_layer(tokens, count, top, hidden, inner, dtype, scale_dtype):
     check_layer(x, *choices(gen, tokens, count, top), *layer(gen, count, hidden, inner, scale_dtype), residual=normal(gen, tokens, hidden, dtype=dtype) if tokens % 2 else None)
 
 
+@pytest.mark.parametrize('dtype,scale_dtype', [(F16, F16), (BF16, F32)])
+@pytest.mark.parametrize('tokens,count,top,hidden,inner', [(65, 8, 1, 512, 272), (81, 1, 1, 16, 16), (200, 512, 8, 128, 64), (300, 1, 1, 256, 528), (321, 3, 2, 1040, 144), (640, 64, 6, 272, 176), (1000, 8, 2, 2064, 400),
+                                                         (100, 40, 32, 144, 256), (4500, 4, 2, 64, 48), (66, 4, 4, 128, 4096), (2000, 2, 1, 256, 128), (70, 600, 2, 64, 32)])
+def test_layer_of_many_tokens(tokens, count, top, hidden, inner, dtype, scale_dtype):
+    gen = generator(tokens, count, hidden, 1)
+    x = normal(gen, tokens, hidden, dtype=dtype)
+    experts, weights = choices(gen, tokens, count, top)
+    experts[5], experts[-1, 0], experts[7] = -1, -3, experts[7, 0].item()  # nobody's, in part nobody's, one expert for all
+    residual = normal(gen, tokens, hidden, dtype=dtype) if tokens % 2 else None
+    got = check_layer(x, experts, weights, *layer(gen, count, hidden, inner, scale_dtype), residual=residual)
+    assert torch.equal(got[5], residual[5]) if residual is not None else not got[5].any()
+
+
 @pytest.mark.parametrize('tokens,count,top,hidden,inner', [(1, 3, 2, 50, 30), (7, 4, 2, 129, 65), (70, 2, 1, 24, 8), (2, 2, 2, 1, 1)])
 def test_layer_of_any_alignment(tokens, count, top, hidden, inner):
     gen = generator(tokens, hidden)
@@ -183,9 +196,10 @@ def test_layer_of_strided_operands():
     ref.check(got.view(12, 256), *ref.experts(big[..., :256].reshape(12, 256), experts.view(12, 2), weights.view(12, 2), *w, None))
 
 
-def test_layer_captured_on_other_streams_and_beside_itself():
+@pytest.mark.parametrize('tokens', [6, 300])
+def test_layer_captured_on_other_streams_and_beside_itself(tokens):
     gen = generator(17)
-    x, router, w = normal(gen, 6, 512, dtype=F16), normal(gen, 16, 512, dtype=F16, std=0.05), layer(gen, 16, 512, 256)
+    x, router, w = normal(gen, tokens, 512, dtype=F16), normal(gen, 16, 512, dtype=F16, std=0.05), layer(gen, 16, 512, 256)
 
     def step():
         experts, weights = hidet_b200.route_tokens(x, router, 4)
@@ -203,7 +217,7 @@ def test_layer_captured_on_other_streams_and_beside_itself():
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
     graphs = [hidet_b200.CudaGraph(lambda: [x], lambda inputs: [step()]) for _ in range(2)]
-    other = normal(gen, 6, 512, dtype=F16)
+    other = normal(gen, tokens, 512, dtype=F16)
     for values in (other, x.clone()):
         x.copy_(values)
         want = step()
