@@ -175,13 +175,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) experts_plan_kernel(const ManyAr
 // ---------------- image ----------------
 constexpr int IMAGE_THREADS = 256;
 
+// A slot's row is shared by the CTAs of a column of the grid, each of which looks for the largest of all of it.
 template <typename X, bool OF_H>
 __global__ void __launch_bounds__(IMAGE_THREADS) experts_image_kernel(const ManyArgs p) {
     __shared__ uint32_t largest;
     const int s = blockIdx.x, K = OF_H ? p.a.inner : p.a.hidden;
-    pdl_launch_dependents();
     if (threadIdx.x == 0) largest = 0;
     pdl_wait();
+    pdl_launch_dependents();  // behind the wait: the product reads the plan without waiting for more
     if (s >= p.plan->slots) return;
     const Slot slot = p.slot[s];
     if (slot.assignment < 0) return;
@@ -204,11 +205,11 @@ __global__ void __launch_bounds__(IMAGE_THREADS) experts_image_kernel(const Many
     bits = largest;
     float back;
     const float by = power_for(bits, back);
-    if (threadIdx.x == 0) p.back[s] = back;
+    if (threadIdx.x == 0 && blockIdx.y == 0) p.back[s] = back;
     int8_t *to = p.image + (int64_t)slot.row * K;
     const int64_t apart = (int64_t)slot.stride * K;
 #pragma unroll 2
-    for (int k = threadIdx.x * 8; k < K; k += IMAGE_THREADS * 8) {
+    for (int k = (blockIdx.y * IMAGE_THREADS + threadIdx.x) * 8; k < K; k += gridDim.y * IMAGE_THREADS * 8) {
         typename X::Raw raw;
         X::load(row, k, raw);
         uint32_t d[2][DIGITS];
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_product_kernel(const __gri
         umma::alloc_pair(smem_u32(&tmem_base_slot), TMEM_COLS);
         umma::relinquish_pair();
     }
-    pdl_wait();
+    // The plan is complete: the kernel in front waited for it, or for one that did, before it let this one start.
     const int groups = p.plan->groups, entries = p.plan->entries;
     const Rounds mine(tiles * entries, k_blocks, (int)gridDim.x / 2, pair, p.plan->largest);
     for (int i = threadIdx.x; i < groups; i += THREADS) group[i] = p.plan->group[i];
@@ -330,13 +331,14 @@ __global__ void __launch_bounds__(THREADS, 1) experts_product_kernel(const __gri
         return mbar_wait(bar, parity, umma::kFastPolls) || umma::wait_or_abort<kKernelExpertsMany>(bar, parity, site, &abort_flag, a.status);
     };
     Units at(group, tiles);
+    if (warp != LOAD_WARP) pdl_wait();  // no bounded wait runs against the kernel in front
 
     if (warp == LOAD_WARP) {
         // ---------------- TMA producer ----------------
         if (lane == 0) {
             const uint64_t keep = l2_policy_evict_last(), once = l2_policy_evict_first();
             const uint32_t full0 = map_to_rank(smem_u32(&full[0]), 0);
-            uint32_t i = 0;
+            uint32_t i = 0, ahead = 0;
             umma::Ring r;
             bool ok = true;
             for (int t = 0; t < mine.count() && ok; ++t) {
@@ -344,17 +346,28 @@ __global__ void __launch_bounds__(THREADS, 1) experts_product_kernel(const __gri
                 int expert, tile, which;
                 at.find(mine.unit(t), expert, tile, which);
                 const Entry en = entry[which];
+                const CUtensorMap *image = &map_x.of[en.slots / SLOTS - 1];
                 const int half = columns_of(en.slots) / 2, row = expert * rows + tile * 2 * TN + (int)rank * TN, x_row = DIGITS * en.slot + (int)rank * half;
                 const uint64_t policy = group[at.g].entries > 1 ? keep : once;
+                auto load_w = [&](uint32_t slot, int kb) {
+                    if (rank == 0) mbar_expect_tx(smem_u32(&full[slot]), 2 * (W_BYTES + half * BK));
+                    load_pair(smem_base + slot * STAGE_BYTES, &map_w, kb * BK, row, full0 + 8 * slot, policy);
+                };
+                auto load_x = [&](uint32_t slot, int kb) { load_pair(smem_base + slot * STAGE_BYTES + W_BYTES, image, kb * BK, x_row, full0 + 8 * slot, keep); };
+                if (t == 0) {  // the first weights are requested before the image is complete
+                    ahead = (uint32_t)min(kb1 - kb0, STAGES);
+                    for (uint32_t j = 0; j < ahead; ++j) load_w(j, kb0 + (int)j);
+                    pdl_wait();
+                    for (uint32_t j = 0; j < ahead; ++j) load_x(j, kb0 + (int)j);
+                }
                 for (int kb = kb0; kb < kb1; ++kb, ++i, r.advance(1, STAGES)) {
+                    if (i < ahead) continue;
                     if (i >= STAGES && !wait_one(smem_u32(&empty[r.slot]), r.phase ^ 1u, 1)) {
                         ok = false;
                         break;
                     }
-                    if (rank == 0) mbar_expect_tx(smem_u32(&full[r.slot]), 2 * (W_BYTES + half * BK));
-                    const uint32_t to = smem_base + r.slot * STAGE_BYTES;
-                    load_pair(to, &map_w, kb * BK, row, full0 + 8 * r.slot, policy);
-                    load_pair(to + W_BYTES, &map_x.of[en.slots / SLOTS - 1], kb * BK, x_row, full0 + 8 * r.slot, keep);
+                    load_w(r.slot, kb);
+                    load_x(r.slot, kb);
                 }
             }
             // Every copy armed must have landed before a CTA may retire; what counts them is the first CTA's barriers, and the second CTA waits for the first at the
@@ -611,7 +624,10 @@ int launch_product(const ManyArgs &p, cudaStream_t stream) {
 
 template <typename X, bool OF_H>
 int launch_image(const ManyArgs &p, cudaStream_t stream) {
-    return launch_after("experts_image_kernel", experts_image_kernel<X, OF_H>, dim3((unsigned)p.most_slots), IMAGE_THREADS, 0, 1, stream, p);
+    // few slots: a CTA 2048 elements, as long as all CTAs run at once (64 rows of 14336: 6.5 us for 10)
+    const int64_t pieces = ceil_div(OF_H ? p.a.inner : p.a.hidden, IMAGE_THREADS * 8), room = 8 * 148 / p.most_slots;
+    const int64_t share = room < 1 ? 1 : room < pieces ? room : pieces;
+    return launch_after("experts_image_kernel", experts_image_kernel<X, OF_H>, dim3((unsigned)p.most_slots, (unsigned)share), IMAGE_THREADS, 0, 1, stream, p);
 }
 
 }  // namespace
