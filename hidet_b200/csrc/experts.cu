@@ -78,15 +78,17 @@ int launch_any(const ExpertsArgs &p, float *h, cudaStream_t stream) {
 }
 
 // Whether the tokens are many: made digits of once, for all tiles of the weights (experts_many.cu), or by every tile for itself (experts_stream.cu).  The latter pays by the assignment and tile,
-// and at its shared parts by an expert's assignments; the former some 7 us for the kernels in front, between and behind.  us, the latter and the former:
-//     8 and 16 tokens, 2 of 8 experts of 4096 x 14336       210 216    250 242       32 and 64: 276 249    330 261
-//     24 and 64 tokens, 6 of 64 of 2048 x 1408               95 99     112 107       48 tokens, 8 of 128 of 2048 x 768: 111 113
-//     16 and 32 tokens, 2 of 4 of 1024 x 4096                28 34      37 37        32 tokens, 8 of 8 of 512 x 1024: 36 27
-//     32 and 64 tokens, 2 of 16 of 2048 x 8192              139 147    156 152
-// More than 64 tokens would have the weights read again by the latter (128 tokens, 2 of 8 of 4096 x 14336: 655 300).
+// and at its shared parts by an expert's assignments; the former some microseconds for the kernels in front, between and behind.  us, the latter and the former:
+//     8, 16, 32, 64 tokens, 2 of 8 experts of 4096 x 14336   207 206    242 234    276 237    330 248
+//     24, 48, 64 tokens, 6 of 64 of 2048 x 1408               95 99     107 104    113 105
+//     48, 64 tokens, 8 of 128 of 2048 x 768                  111 113    120 119
+//     16, 32 tokens, 2 of 4 of 1024 x 4096                    28 30      37 32
+//     16, 32, 64 tokens, 2 of 16 of 2048 x 8192              123 128    140 142    157 143
+//     16 tokens, 4 and 8 of 8 of 512 x 1024                   23 23      24 22        8, 16 tokens, 4 of 4 of 2048 x 4096   35.5 36.7    42.5 39
+// More than 64 tokens would have the weights read again by the latter (128 tokens, 2 of 8 of 4096 x 14336: 655 270).
 bool are_many(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top) {
     const double assignments = (double)tokens * (double)top;
-    return tokens > kExpertsTokens || assignments / (double)(count > 0 ? count : 1) + 1.5e-8 * assignments * (double)hidden * (double)inner > 21.0;
+    return tokens > kExpertsTokens || assignments / (double)(count > 0 ? count : 1) + 1.5e-8 * assignments * (double)hidden * (double)inner > 16.0;
 }
 
 }  // namespace

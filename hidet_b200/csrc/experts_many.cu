@@ -15,7 +15,7 @@
 // are neighbours in a round of all pairs, so that a tile of its weight comes from memory once (a contiguous part of the tiles for every pair instead: down of 512 tokens 230 us for 142).
 // Bounded waits and their ends are as there.
 //
-// What bounds it, two of eight experts of 4096 x 14336: with 64 tokens (257 us) the weights' way from memory, 215 us; with 512 (570 us: 270 + 145 us by themselves, the rest small kernels and
+// What bounds it, two of eight experts of 4096 x 14336: with 64 tokens (248 us) the weights' way from memory, 215 us; with 512 (570 us: 270 + 145 us by themselves, the rest small kernels and
 // the clock under the power cap) and 2048 (2.3 ms, 1.9 POP/s) an SM's copies, some 40 bytes a clock of which 16 KB a stage are weights, whatever the entry's columns.  A copy of the
 // image is one box: in boxes of 16 rows 512 tokens took 733 us for 863.  Rows' largest magnitudes are stored by warp and not gathered with atomics: gate and up 332 us with them, 274 without.
 #include <type_traits>
