@@ -16,7 +16,7 @@
 // Bounded waits and their ends are as there.
 //
 // What bounds it, two of eight experts of 4096 x 14336: with 64 tokens (248 us) the weights' way from memory, 215 us; with 512 (570 us: 270 + 145 us by themselves, the rest small kernels and
-// the clock under the power cap) and 2048 (2.3 ms, 1.9 POP/s) an SM's copies, some 40 bytes a clock of which 16 KB a stage are weights, whatever the entry's columns.  A copy of the
+// the clock under the power cap) and 2048 (2.0 ms, 2.1 POP/s) an SM's copies, some 40 bytes a clock of which 16 KB a stage are weights, whatever the entry's columns.  A copy of the
 // image is one box: in boxes of 16 rows 512 tokens took 733 us for 863.  Rows' largest magnitudes are stored by warp and not gathered with atomics: gate and up 332 us with them, 274 without.
 #include <type_traits>
 
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_product_kernel(const __gri
                 const float back[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
                 float y[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = fmaf((float)v[2][j], 65536.0f, fmaf((float)v[1][j], 256.0f, (float)v[0][j])) * (back[j] * scale);
+                for (int j = 0; j < 8; ++j) y[j] = fmaf((float)v[2][j], 65536.0f, fmaf((float)v[1][j], 256.0f, (float)v[0][j])) * scale * back[j];  // the scale first: it and the power of two may be small together
                 if (DOWN) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
@@ -600,7 +600,7 @@ Places places_for(int64_t assignments, int64_t hidden, int64_t inner, int64_t co
     p.bytes = at;
     return p;
 }
-constexpr size_t kMostBytes = (size_t)256 << 20;
+constexpr size_t kMostBytes = (size_t)512 << 20;  // half of it: 2048 tokens, two of eight experts of 4096 x 14336, in four parts, 2.3 ms for 2.0
 
 template <bool DOWN>
 int launch_product(const ManyArgs &p, cudaStream_t stream) {
@@ -634,7 +634,7 @@ int launch_image(const ManyArgs &p, cudaStream_t stream) {
 
 int64_t experts_many_at_once(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top) {
     int64_t most = MOST_ASSIGNMENTS;
-    while (most > 256 && places_for(most, hidden, inner, count).bytes > kMostBytes) most /= 2;
+    while (most > SLOTS && places_for(most, hidden, inner, count).bytes > kMostBytes) most /= 2;
     most = most / top > 1 ? most / top : 1;
     return tokens < most ? tokens : most;
 }

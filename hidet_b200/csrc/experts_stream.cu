@@ -509,7 +509,8 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
 #pragma unroll
                     for (int j = 0; j < WIDE; ++j) {
                         y[j] = fmaf((float)v[2][j], 65536.0f, fmaf((float)v[1][j], 256.0f, (float)v[0][j]));
-                        if (c + j < en.count) y[j] *= l.back[en.first + c + j] * scale;
+                        y[j] *= scale;  // first: it and the power of two may be small together
+                        if (c + j < en.count) y[j] *= l.back[en.first + c + j];
                     }
                     if (DOWN) {
 #pragma unroll

@@ -70,7 +70,7 @@ def mixture_of_experts(x: torch.Tensor, experts: torch.Tensor, weights: torch.Te
     bfloat16 or float32).  Negative experts are passed over (padding: a token of nothing but these is its residual, or zeros); one beyond the layer's is passed over and reported by b200q_check_status.
     Sums are float32, the result is rounded once and is the same on every run.  out: a contiguous tensor for the result, which may be the residual, or x.
 
-    A few tokens are a stream of the weights of the experts that have one; many (more than 64, or dozens an expert) are matrix products over the tokens sorted by expert, with up to 256 MB of
+    A few tokens are a stream of the weights of the experts that have one; many (more than 64, or dozens an expert) are matrix products over the tokens sorted by expert, with up to half a gigabyte of
     scratch.  Not differentiable."""
     result = native.experts(x, experts, weights, gate_up, gate_up_scale, down, down_scale, residual, out)
     if result is not None:

@@ -335,7 +335,7 @@ B200Q_API int b200q_route_tokens(const void *x, int64_t x_stride, const void *ro
  * (a row whose largest is below 2^-98 is zeros), and the sums over 128 of them or more are exact; all that follows is float.  A row with a NaN or an infinity gives NaN.  Where hidden, inner,
  * x_stride and the bases are not all multiples of 16 bytes' worth, or there are more than 512 experts, slower kernels take the call, with products and sums in float.
  * The results do not depend on the run.  out may be residual, or x.  An assignment to a negative expert is passed over, one to an expert that is not there too, and the latter is
- * reported by b200q_check_status.  The weights of an expert that has a token are read once, for up to thousands of tokens (as many as have 8192 assignments, or scratch of 256 MB).
+ * reported by b200q_check_status.  The weights of an expert that has a token are read once, for up to thousands of tokens (as many as have 8192 assignments, or half a gigabyte of workspace).
  * The workspace is one of b200q_qlinear_f16_i8's kind.
  */
 B200Q_API size_t b200q_mixture_of_experts_workspace_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top);

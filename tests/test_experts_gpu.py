@@ -166,6 +166,15 @@ def test_values_of_any_size(dtype):
     assert h > 1e3
 
 
+@pytest.mark.parametrize('tokens', [8, 80])
+def test_small_tokens_with_small_scales(tokens):
+    """Sums whose power of two and scale are small together, below float's range, but not what they stand for."""
+    gen = generator(24)
+    x = (normal(gen, tokens, 512) * torch.logspace(-15, -12, tokens, device='cuda')[:, None]).to(BF16)
+    w = layer(gen, 4, 512, 384)
+    check_layer(x, *choices(gen, tokens, 4, 2), w[0], w[1].float() * 20, w[2], w[3].float() * 1e-6)
+
+
 def test_tokens_that_are_no_numbers_stay_among_themselves():
     gen = generator(15)
     x, w = normal(gen, 9, 256, dtype=BF16), layer(gen, 3, 256, 128)
@@ -283,4 +292,57 @@ def test_two_layers_at_once(hidden, inner):
                 got[i].append(step(i))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+    assert ffi.func('b200q_check_status')() == ffi.OK
+
+
+def test_many_tokens_in_place_and_of_every_kind():
+    """Results in the tokens' place, tokens that are no numbers, of any size and of large hidden values, assignments to nobody, beyond the layer and many times to one expert."""
+    gen = generator(21)
+    x, w = normal(gen, 300, 512, dtype=BF16), layer(gen, 6, 512, 272)
+    experts, weights = choices(gen, 300, 6, 2)
+    clean = check_layer(x, experts, weights, *w, residual=x)
+    place = x.clone()
+    assert torch.equal(hidet_b200.mixture_of_experts(place, experts, weights, *w, residual=place, out=place), clean) and torch.equal(place, clean)
+    odd = x.clone()
+    odd[4, 7], odd[100], odd[299, 0] = float('nan'), float('inf'), float('-inf')
+    broken = weights.clone()
+    broken[6, 1] = float('nan')
+    got = hidet_b200.mixture_of_experts(odd, experts, broken, *w, residual=x)
+    bad = torch.zeros(300, dtype=torch.bool, device='cuda')
+    bad[[4, 6, 100, 299]] = True
+    assert got[bad].isnan().all() and torch.equal(got[~bad], clean[~bad])
+    sizes = (x.float() * torch.logspace(-30, 3, 300, device='cuda')[:, None]).to(BF16)
+    sizes[17] = 0
+    check_layer(sizes, experts, weights, w[0], w[1].float() * 20, w[2], w[3].float() * 1e-6)
+    nobody = torch.full_like(experts, -1)
+    assert torch.equal(hidet_b200.mixture_of_experts(x, nobody, weights, *w, residual=x), x) and not hidet_b200.mixture_of_experts(x, nobody, weights, *w).any()
+    assert ffi.func('b200q_check_status')() == ffi.OK
+    beyond, passed = experts.clone(), experts.clone()
+    beyond[8, 0], beyond[200, 1], passed[8, 0], passed[200, 1] = 6, 2 ** 31 - 1, -1, -2
+    assert torch.equal(hidet_b200.mixture_of_experts(x, beyond, weights, *w), hidet_b200.mixture_of_experts(x, passed, weights, *w))
+    with pytest.raises(ffi.BackendException, match='expert'):
+        ffi.func('b200q_check_status')()
+
+
+@pytest.mark.parametrize('tokens,top', [(1, 1500), (3, 700), (2, 4096), (70, 150)])
+def test_tokens_of_many_assignments(tokens, top):
+    gen = generator(22, tokens, top)
+    x, w = normal(gen, tokens, 128, dtype=F16), layer(gen, 5, 128, 64)
+    experts = torch.randint(-1, 5, (tokens, top), generator=gen, device='cuda', dtype=torch.int32)
+    check_layer(x, experts, torch.rand((tokens, top), generator=gen, device='cuda') / top, *w)
+
+
+def test_layers_share_a_workspace_in_turn():
+    """Few tokens, many and unaligned ones, and linears, in every order on one stream."""
+    gen = generator(23)
+    calls = []
+    for tokens, count, top, hidden, inner in ((2, 8, 2, 512, 768), (200, 8, 2, 512, 768), (64, 4, 4, 256, 512), (5, 3, 2, 50, 30), (1000, 16, 4, 128, 64)):
+        x, w, picks = normal(gen, tokens, hidden, dtype=F16), layer(gen, count, hidden, inner), choices(gen, tokens, count, top)
+        calls.append(lambda x=x, w=w, picks=picks: hidet_b200.mixture_of_experts(x, *picks, *w))
+    for m in (3, 40):
+        a, wq, scale = normal(gen, m, 4096, dtype=F16), codes_of(gen, 4096, 512), torch.full((512,), 1e-3, dtype=F16, device='cuda')
+        calls.append(lambda a=a, wq=wq, scale=scale: hidet_b200.symmetric_quant_matmul(a, wq, scale))
+    want = [call() for call in calls]
+    for i in torch.randint(0, len(calls), (200,), generator=torch.Generator().manual_seed(3)).tolist():
+        assert torch.equal(calls[i](), want[i])
     assert ffi.func('b200q_check_status')() == ffi.OK

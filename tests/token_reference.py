@@ -55,12 +55,18 @@ def product(a, a_scale, weight, scale, layout, bias, residual, pairs, dtype):
 
 def experts(x, chosen, weights, gate_up, s1, down, s2, residual):
     """(result, bound) of a layer of experts.  x and h are at most 2^-22 of their row's largest element off (whole numbers of up to 2^22, at least 2^21 for the largest, rounded); what stands for the sum of
-    n products in float is off by no more than (n / 8 + 32) roundings of 2^-23 of their magnitudes (float sums run eight or more products at a time; whole ones are exact)."""
+    n products in float is off by no more than (n / 8 + 32) roundings of 2^-23 of their magnitudes (float sums run eight or more products at a time; whole ones are exact).
+    A row of x or h whose largest element is below 2^-98 may be zeros, as the layer's documentation says: an element is then off by itself, by the largest at most."""
     rows, hidden = x.shape
     inner = down.shape[2]
     xd = x.double()
     out, bound = torch.zeros_like(xd), torch.zeros_like(xd)
-    dx = xd.abs().amax(-1, keepdim=True) * 2.0 ** -22
+
+    def held(least, most):  # how far elements of a row are held, whose largest lies between these
+        return torch.where(least < 2.0 ** -98, most, most * 2.0 ** -22)
+
+    largest = xd.abs().amax(-1, keepdim=True)
+    dx = held(largest, largest)
     for e in range(down.shape[0]):
         share = torch.where(chosen == e, weights.double(), 0.0)
         token = (chosen == e).any(-1).nonzero()[:, 0]
@@ -71,7 +77,7 @@ def experts(x, chosen, weights, gate_up, s1, down, s2, residual):
         y = xd[token] @ w1.t()
         dy = xd[token].abs() @ w1.abs().t() * ((hidden / 8 + 32) * 2 * F32) + dx[token] * w1.abs().sum(1)
         h, dh = silu_mul(y[:, 0::2], y[:, 1::2], dy[:, 0::2], dy[:, 1::2])
-        dh = dh + (h.abs() + dh).amax(-1, keepdim=True) * 2.0 ** -22
+        dh = dh + held((h.abs() - dh).amax(-1, keepdim=True), (h.abs() + dh).amax(-1, keepdim=True))
         o = h @ w2.t()
         do = dh @ w2.abs().t() + (h.abs() + dh) @ w2.abs().t() * ((inner / 8 + 32) * 2 * F32)
         out[token] += share * o
