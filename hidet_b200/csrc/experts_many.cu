@@ -600,7 +600,7 @@ Places places_for(int64_t assignments, int64_t hidden, int64_t inner, int64_t co
     p.bytes = at;
     return p;
 }
-constexpr size_t kMostBytes = (size_t)512 << 20;  // half of it: 2048 tokens, two of eight experts of 4096 x 14336, in four parts, 2.3 ms for 2.0
+constexpr size_t kMostBytes = (size_t)511 << 20;  // with the workspace's head half a gigabyte.  Half of it: 2048 tokens, two of eight experts of 4096 x 14336, in four parts, 2.3 ms for 2.0
 
 template <bool DOWN>
 int launch_product(const ManyArgs &p, cudaStream_t stream) {
@@ -633,10 +633,11 @@ int launch_image(const ManyArgs &p, cudaStream_t stream) {
 }  // namespace
 
 int64_t experts_many_at_once(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top) {
-    int64_t most = MOST_ASSIGNMENTS;
-    while (most > SLOTS && places_for(most, hidden, inner, count).bytes > kMostBytes) most /= 2;
+    int64_t most = (int64_t)kMostBytes / ((4 + DIGITS) * (hidden > inner ? hidden : inner));  // assignments
+    if (most > MOST_ASSIGNMENTS) most = MOST_ASSIGNMENTS;
+    while (most > SLOTS && places_for(most, hidden, inner, count).bytes > kMostBytes) most -= most / 16 > 0 ? most / 16 : 1;
     most = most / top > 1 ? most / top : 1;
-    return tokens < most ? tokens : most;
+    return ceil_div(tokens, ceil_div(tokens, most));  // parts of one size
 }
 
 size_t experts_many_bytes(int64_t tokens, int64_t hidden, int64_t inner, int64_t count, int64_t top) { return places_for(tokens * top, hidden, inner, count).bytes; }

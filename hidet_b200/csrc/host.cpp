@@ -599,6 +599,7 @@ PyObject *route_tokens(PyObject *, PyObject *const *args, Py_ssize_t n_args) {
     PLAIN_OR_NONE(x && router && x->dim() >= 1 && x->numel() > 0 && router->dim() == 2 && float_code(x->scalar_type()) >= 0);
     PLAIN_OR_NONE(router->size(1) == x->size(-1) && (router->scalar_type() == x->scalar_type() || router->scalar_type() == at::kFloat));
     const int64_t width = x->size(-1), count = router->size(0), top = PyLong_AsLongLong(args[2]);
+    if (top == -1) PyErr_Clear();  // of more than 64 bits
     Where w;
     PLAIN_OR_NONE(top >= 1 && top <= 32 && top <= count && where_is(*x, w) && router->get_device() == w.device);
     PLAIN_OR_NONE(width % 8 != 0 || (reinterpret_cast<uintptr_t>(x->const_data_ptr()) & 15u) == 0);

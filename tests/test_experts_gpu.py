@@ -242,7 +242,7 @@ def test_refusals():
     e, p = choices(gen, 2, 4, 2)
     r, f = hidet_b200.route_tokens, hidet_b200.mixture_of_experts
     for call, text in ((lambda: r(x.int(), router, 2), 'float16'), (lambda: r(x, router[:, :31], 2), 'router'), (lambda: r(x, router.to(BF16), 2), 'router'), (lambda: r(x, router, 0), 'top_k'),
-                       (lambda: r(x, router, 5), 'top_k'), (lambda: r(x, router, True), 'top_k'), (lambda: r(x, torch.zeros(1025, 32, dtype=F16, device='cuda'), 2), '1024'),
+                       (lambda: r(x, router, 5), 'top_k'), (lambda: r(x, router, True), 'top_k'), (lambda: r(x, router, 2 ** 70), 'top_k'), (lambda: r(x, router, -1), 'top_k'), (lambda: r(x, torch.zeros(1025, 32, dtype=F16, device='cuda'), 2), '1024'),
                        (lambda: f(x.float(), e, p, *w), 'float16'), (lambda: f(x, e.long(), p, *w), 'experts'), (lambda: f(x, e[:1], p, *w), 'experts'), (lambda: f(x, e, p.half(), *w), 'weights'),
                        (lambda: f(x, e, p[:, :1], *w), 'weights'), (lambda: f(x, e, p, w[0][:, 1:], *w[1:]), 'gate_up'), (lambda: f(x, e, p, w[0], w[1], w[2][:, :, :47], w[3]), 'down'),
                        (lambda: f(x, e, p, w[0], w[1].float(), *w[2:]), 'scales'), (lambda: f(x, e, p, w[0], w[1][:, :95], *w[2:]), 'scales'), (lambda: f(x, e, p, *w, residual=x.float()), 'residual'),

@@ -74,3 +74,9 @@ def test_workspace_of_experts():
     need = ffi.func('b200q_mixture_of_experts_workspace_bytes')
     assert need(0, 64, 64, 8, 2) == 0
     assert 0 < need(1, 4096, 14336, 8, 2) <= need(64, 4096, 14336, 8, 2)
+
+
+@pytest.mark.parametrize('tokens,hidden,inner,count,top', [(2048, 4096, 14336, 8, 2), (10 ** 6, 4096, 14336, 8, 2), (1000, 131056, 16, 512, 1), (4096, 2048, 768, 128, 8), (300, 16, 16, 1, 1), (10 ** 7, 8192, 28672, 512, 8)])
+def test_scratch_of_many_tokens_is_bounded(tokens, hidden, inner, count, top):
+    need = ffi.func('b200q_mixture_of_experts_workspace_bytes')
+    assert 0 < need(65, hidden, inner, count, top) and need(tokens, hidden, inner, count, top) <= 1 << 29
