@@ -5,7 +5,7 @@
 // element, so that an element is off by at most 2^-22 of that), and these as three digits of 8 bits, v = 65536 d2 + 256 d1 + d0 with d in -128 .. 127.  A tile of 128 rows of the weight is the
 // first operand of tcgen05.mma, three columns for each token are the second, sums of 32 bits are exact, and float begins behind them.  So weights are only ever copied,
 // and what is computed on them costs no issue slots.  (As f16 by mma.sync, with int8 widened in registers, a tile took 260 instructions of each of eight warps, and the
-// stream stood at 3.2 TB/s.)  One token, two of eight experts of 4096 x 14336: 65 us, 5.4 TB/s; 8 tokens 210 us, 6.0 TB/s; 7 tokens, six of 64 of 2048 x 1408: 56 us.  What is not the stream
+// stream stood at 3.2 TB/s.)  One token, two of eight experts of 4096 x 14336: 62 us, 5.7 TB/s; 8 tokens 210 us, 6.0 TB/s; 7 tokens, six of 64 of 2048 x 1408: 55 us; one, six of 64 of 608 x 288: 14.  What is not the stream
 // is some 5 us at the start of either kernel (launch, entries, first loads) and the meeting of parts at its end.
 //
 // Every CTA makes the list of entries, an expert with up to C of its assignments (an expert with more has several entries), and takes an equal, contiguous part of
@@ -46,6 +46,8 @@ constexpr int MOST_STAGES = 10;
 constexpr int MOST_SMEM = 227 * 1024;
 constexpr int MOST_ASSIGNMENTS = kExpertsAssignments;
 constexpr int MOST_EXPERTS = 512;
+constexpr int FEW_ASSIGNMENTS = 128;
+static_assert(FEW_ASSIGNMENTS <= THREADS, "one a thread");
 constexpr uint16_t kNone = 0xffff;
 // what of the workspace's counters is whose: arrivals at what CTAs share (by the first of them), CTAs that are through, h's largest magnitudes
 constexpr int MOST_CTAS = 1024, COUNTER_UP = 0, COUNTER_DOWN = MOST_CTAS, COUNTER_DONE = 2 * MOST_CTAS, COUNTER_MAX = 4 * MOST_CTAS;
@@ -118,15 +120,59 @@ struct Lists {
     }
 };
 
-// The entries of a launch: counts by expert and the tokens that they are of, a sum over the experts, assignments in their places.  Every CTA makes them for itself, so an
-// expert's assignments stand in their own order: as they come they would differ from CTA to CTA, and with them whose column is whose.  `meanwhile` runs while the experts are on their way.
-template <typename F>
-__device__ __forceinline__ void make_entries(const ExpertsArgs &a, int columns, Shared &s, const Lists &l, F meanwhile) {
-    const int n = a.tokens * a.top;
-    for (int e = threadIdx.x; e < a.count; e += THREADS) l.counts[e] = 0, l.who[e] = make_uint2(0, 0);
+// What make_entries begins with, in front of the wait for the experts.
+__device__ __forceinline__ void clear_lists(const ExpertsArgs &a, Shared &s, const Lists &l) {
+    if (a.tokens * a.top > FEW_ASSIGNMENTS)
+        for (int e = threadIdx.x; e < a.count; e += THREADS) l.counts[e] = 0, l.who[e] = make_uint2(0, 0);
     if (threadIdx.x < EARLY_TOKENS) s.bits[threadIdx.x] = 0;
     if (threadIdx.x == 0) s.duplicates = 0;
     __syncthreads();
+}
+
+// The entries of a launch: counts by expert and the tokens that they are of, a sum over the experts, assignments in their places.  Every CTA makes them for itself, so an
+// expert's assignments stand in their own order: as they come they would differ from CTA to CTA, and with them whose column is whose.  `meanwhile` runs while the experts are on their way.
+// Few assignments have their places by comparing each with all: 1.2 us instead of 2.1.
+template <typename F>
+__device__ __forceinline__ void make_entries(const ExpertsArgs &a, int columns, Shared &s, const Lists &l, F meanwhile) {
+    const int n = a.tokens * a.top;
+    if (n <= FEW_ASSIGNMENTS) {
+        const int i = threadIdx.x;
+        uint16_t mine = kNone;
+        const int e = i < n ? __ldcg(a.experts + i) : -1;
+        meanwhile();
+        if (i < n) {
+            if (e >= 0 && e < a.count) mine = (uint16_t)e;
+            else if (e >= 0 && blockIdx.x == 0 && a.status != nullptr) atomicOr(a.status, kBadExpert);
+            l.chosen[i] = mine;
+        }
+        __syncthreads();
+        int *sizes = reinterpret_cast<int *>(l.by);  // by place: assignments of the entry that begins there
+        if (mine != kNone) {
+            int less = 0, before = 0, all = 0;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) {
+                const uint16_t e = l.chosen[j];
+                less += e < mine, all += e == mine, before += e == mine && j < i;
+            }
+            const int to = less + before;
+            l.order[to] = (uint16_t)i, l.token[to] = (uint16_t)(i / a.top);
+            sizes[to] = before % columns == 0 ? min(columns, all - before) : 0;
+        }
+        const int there = __syncthreads_count(mine != kNone);
+        if (threadIdx.x < 32) {
+            int entries = 0, largest = 0;
+            for (int at = (int)threadIdx.x; at - (int)threadIdx.x < there; at += 32) {
+                const int size = at < there ? sizes[at] : 0;
+                const uint32_t begins = __ballot_sync(0xffffffffu, size > 0);
+                if (size > 0) l.entry[entries + __popc(begins & ((1u << threadIdx.x) - 1u))] = {l.chosen[l.order[at]], (uint16_t)at, (uint16_t)size};
+                entries += __popc(begins), largest = max(largest, size);
+            }
+            largest = __reduce_max_sync(0xffffffffu, largest);
+            if (threadIdx.x == 0) s.entries = entries, s.largest = largest;
+        }
+        __syncthreads();
+        return;
+    }
     meanwhile();
     for (int i = threadIdx.x; i < n; i += THREADS) {
         const int e = __ldcg(a.experts + i), t = i / a.top;
@@ -248,6 +294,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
         umma::alloc(smem_u32(&s.tmem_base), p.tmem_cols);
         umma::relinquish();
     }
+    clear_lists(a, s, l);
     // The experts were chosen in front of gate and up, which waits for that before it lets down start: down may read them, and request weights, without waiting.
     if (!DOWN) pdl_wait();
     umma::fence_before_sync();
@@ -375,6 +422,17 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
             }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(THREADS - 64) : "memory");
+        if (DOWN && warp == 2) {  // the largest magnitudes are zero again when all CTAs have read them
+            int last = 0;
+            if (lane == 0) {
+                __threadfence();
+                last = atomicAdd(p.counters + COUNTER_DONE, 1u) == gridDim.x - 1;
+            }
+            if (__shfl_sync(0xffffffffu, last, 0)) {
+                for (int i = lane; i < a.tokens * a.top; i += 32) p.counters[COUNTER_MAX + i] = 0;
+                if (lane == 0) p.counters[COUNTER_DONE] = 0;
+            }
+        }
         if (warp >= DIGIT_WARP0) {
             // ---------------- digits ----------------
             // Teams of two warps take stages in turn.  No more teams than stages: a wait tells a phase from its neighbours only, and a team that has written its last stage
@@ -613,16 +671,6 @@ __global__ void __launch_bounds__(THREADS, 1) experts_stream_kernel(const __grid
         }
         if (parts.total == 0) {  // nobody is anyone's: the residual, or zeros
             for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < (int64_t)a.tokens * a.hidden; i += (int64_t)gridDim.x * THREADS) store_result(a, (int)(i / a.hidden), (int)(i % a.hidden), 0.0f);
-        }
-        // the largest magnitudes are zero again when all CTAs have read them
-        if (threadIdx.x == 0) {
-            __threadfence();
-            s.last = atomicAdd(p.counters + COUNTER_DONE, 1u) == gridDim.x - 1;
-        }
-        __syncthreads();
-        if (s.last) {
-            for (int i = threadIdx.x; i < a.tokens * a.top; i += THREADS) p.counters[COUNTER_MAX + i] = 0;
-            if (threadIdx.x == 0) p.counters[COUNTER_DONE] = 0;
         }
     }
 }
