@@ -271,6 +271,27 @@ __global__ void __launch_bounds__(THREADS, 1)
                     sc[h][e] = n < N ? i8_scale(p.a.scale, p.a.scale_type, n) : 0.0f;
                     bias[h][e] = n < N && p.a.bias != nullptr ? value_at<BF16>(p.a.bias, n) : 0.0f;
                 }
+            const int out_n0 = PAIRS ? n0 >> 1 : n0;
+            const bool cols_ok = out_n0 + chunk * 8 < out_n;  // widths are multiples of 8: eight channels are in or out together
+            // What a block needs from memory is asked for a block ahead: with few k it is what takes the time.
+            uint4 next_res[4];
+            float next_sa[4][2];  // token 8 j + 2 tq + i
+            auto ask = [&](int cb) {
+#pragma unroll
+                for (int pass = 0; res_vec && pass < 4; ++pass) {
+                    const int m = cb * 32 + pass * 8 + row_in_pass;
+                    next_res[pass] = make_uint4(0, 0, 0, 0);
+                    if (m < m_left && cols_ok) next_res[pass] = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(res) + (size_t)(m0 + m) * p.a.ldr + out_n0 + chunk * 8));
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int m = cb * 32 + 8 * j + 2 * tq + i;
+                        next_sa[j][i] = m < m_left ? p.a.a_scale[m0 + m] : 0.0f;
+                    }
+            };
+            ask(share + p.split * eg);
             const bool ok = all_of_128(1 + eg, wait(smem_u32(&acc_full[buf]), acc_use & 1, 10));  // the group stays or leaves as one
             if (!ok && p.split == 1) break;
             umma::fence_after_sync();
@@ -295,8 +316,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                 meet();
                 if (!ok) break;
             }
-            const int out_n0 = PAIRS ? n0 >> 1 : n0;
-            const bool cols_ok = out_n0 + chunk * 8 < out_n;  // widths are multiples of 8: eight channels are in or out together
             const size_t out_off = (size_t)m0 * out_n + out_n0 + chunk * 8;
             if (p.split == 1 && eg >= blocks) {  // a tile of a single block: nothing for this group
                 __syncwarp();
@@ -306,25 +325,15 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int cb = share + p.split * eg; cb < blocks; cb += p.split * EPI_GROUPS, ++block) {
                 unsigned char *staging = smem_gen + STAGING_OFF + (2 * eg + (block & 1)) * STAGING_BYTES;
                 const uint32_t staging_a = smem_base + STAGING_OFF + (2 * eg + (block & 1)) * STAGING_BYTES;
-                float sa[4][2];  // token 8 j + 2 tq + i
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int m = cb * 32 + 8 * j + 2 * tq + i;
-                        sa[j][i] = m < m_left ? p.a.a_scale[m0 + m] : 0.0f;
-                    }
+                float sa[4][2];
+                memcpy(sa, next_sa, sizeof(sa));
                 if (res_vec) {
                     // the residual's block goes through the staging buffer into the fragments' layout
 #pragma unroll
-                    for (int pass = 0; pass < 4; ++pass) {
-                        const int r = pass * 8 + row_in_pass, m = cb * 32 + r;
-                        uint4 val = make_uint4(0, 0, 0, 0);
-                        if (m < m_left && cols_ok) val = __ldcg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(res) + (size_t)(m0 + m) * p.a.ldr + out_n0 + chunk * 8));
-                        *reinterpret_cast<uint4 *>(staging + r * ROW_BYTES + chunk * 16) = val;
-                    }
+                    for (int pass = 0; pass < 4; ++pass) *reinterpret_cast<uint4 *>(staging + (pass * 8 + row_in_pass) * ROW_BYTES + chunk * 16) = next_res[pass];
                     group_sync();
                 }
+                ask(cb + p.split * EPI_GROUPS);
                 uint32_t v[2][16];
                 umma::ld_16x256b_x4(acc + cb * 32, v[0]);
                 umma::ld_16x256b_x4(acc + (16u << 16) + cb * 32, v[1]);
