@@ -10,7 +10,9 @@
 //              16 bits, transposed through a staging buffer (two per group, taken in turn) by matrix stores, 16-byte stores of whole output rows
 //   warp 8     TMA producer; both CTAs' copies count on the first CTA's barrier
 //   warp 9     MMA issuer (first CTA of the pair only), one thread for the whole loop
-// Two accumulators, so that a tile's epilogue runs beside the next one's products.
+// Two accumulators, so that a tile's epilogue runs beside the next one's products.  With few k the epilogue is what takes the time (4096 x 1024 x 4096: 20 us, 11 without it), and what it reads
+// is asked for ahead: scales a tile, the residual a tile (into L2) and a block, tokens' scales a block (2048 x 512 x 8192 with a residual: 34 us without, 29 with).  Four groups instead of two
+// help there by 3 to 10 %, and cost 1 to 5 % elsewhere.
 //
 // Where tiles are few, K is shared by the two or four pairs of a cluster, a tile each cluster and no second one.  Sums are whole numbers: when all have theirs, every pair
 // hands the others the 32-token blocks that they finish (its fragments as they come out of tensor memory, into the ring, which is no longer in use) and adds what it gets.
@@ -18,6 +20,7 @@
 // Every wait is bounded: a wait that runs out records where and raises a CTA-wide flag, all roles leave, the first CTA waits for what was armed and issued, and the
 // two CTAs meet at a cluster barrier before either gives back tensor memory or retires.
 #include <atomic>
+#include <type_traits>
 
 #include "qlinear_i8.h"
 #include "umma.cuh"
@@ -32,8 +35,8 @@ constexpr int BK = 128;                      // k per stage = four MMAs of K = 3
 constexpr int W_BYTES = BK * TN;
 constexpr int MAX_STAGES = 10;
 constexpr int EPI_GROUPS = 2;
-constexpr int LOAD_WARP = 8, MMA_WARP = 9;
-constexpr int THREADS = 32 * 10;
+constexpr int LOAD_WARP = 4 * EPI_GROUPS, MMA_WARP = LOAD_WARP + 1;
+constexpr int THREADS = 32 * (MMA_WARP + 1);
 constexpr int TMEM_COLS = 512;
 constexpr int ROW_BYTES = TN * 2 + 16;       // one output row in the staging buffer, padded: matrix stores touch every bank once
 constexpr int STAGING_BYTES = 32 * ROW_BYTES;
@@ -254,23 +257,46 @@ __global__ void __launch_bounds__(THREADS, 1)
         constexpr int PASS_ROWS = 128 >> ROW_CHUNKS_LOG2;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(32 * q) << 16);
         uint32_t t_iter = 0, block = 0;         // block: the group's 32-token blocks so far, staging buffers in turn
-        for (int u = first; u < units; u += step, ++t_iter) {
+        // A tile's residual comes to L2 a tile ahead, a row a thread: a block of it on its way is not enough for its way from memory.
+        auto prefetch_residual = [&](int u) {
+            if (PAIRS || res == nullptr || u >= units) return;
+            int n, m;
+            tile_of(p, u, n, m);
+            n += (int)rank * TN;
+            const int width = min(TN, N - n);
+            for (int r = 128 * eg + et; r < min(M - m, p.tm); r += 128 * EPI_GROUPS) {
+                const char *row = static_cast<const char *>(res) + ((int64_t)(m + r) * p.a.ldr + n) * 2;
+                for (int i = 0; i < width; i += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + 2 * i));
+            }
+        };
+        float next_sc[2][2], next_bias[2][2];  // [16-channel block][8-channel half]: channel 16 h + 8 e + g of this warp's 32
+        auto ask_scales = [&](int u) {
+            if (u >= units) return;
             int n0, m0;
             tile_of(p, u, n0, m0);
-            n0 += (int)rank * TN;
-            const uint32_t buf = t_iter & 1, acc_use = t_iter >> 1;
-            const int m_left = min(M - m0, p.tm);
-            const int blocks = (m_left + 31) / 32;
-            const uint32_t acc = lane_addr + buf * p.tm;
-            float sc[2][2], bias[2][2];  // [16-channel block][8-channel half]: channel 16 h + 8 e + g of this warp's 32
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int n = n0 + 32 * q + 16 * h + 8 * e + g;
-                    sc[h][e] = n < N ? i8_scale(p.a.scale, p.a.scale_type, n) : 0.0f;
-                    bias[h][e] = n < N && p.a.bias != nullptr ? value_at<BF16>(p.a.bias, n) : 0.0f;
+                    const int n = n0 + (int)rank * TN + 32 * q + 16 * h + 8 * e + g;
+                    next_sc[h][e] = n < N ? i8_scale(p.a.scale, p.a.scale_type, n) : 0.0f;
+                    next_bias[h][e] = n < N && p.a.bias != nullptr ? value_at<BF16>(p.a.bias, n) : 0.0f;
                 }
+        };
+        ask_scales(first);
+        prefetch_residual(first);
+        for (int u = first; u < units; u += step, ++t_iter) {
+            int n0, m0;
+            tile_of(p, u, n0, m0);
+            n0 += (int)rank * TN;
+            prefetch_residual(u + step);
+            const uint32_t buf = t_iter & 1, acc_use = t_iter >> 1;
+            const int m_left = min(M - m0, p.tm);
+            const int blocks = (m_left + 31) / 32;
+            const uint32_t acc = lane_addr + buf * p.tm;
+            float sc[2][2], bias[2][2];
+            memcpy(sc, next_sc, sizeof(sc)), memcpy(bias, next_bias, sizeof(bias));
+            ask_scales(u + step);
             const int out_n0 = PAIRS ? n0 >> 1 : n0;
             const bool cols_ok = out_n0 + chunk * 8 < out_n;  // widths are multiples of 8: eight channels are in or out together
             // What a block needs from memory is asked for a block ahead: with few k it is what takes the time.
@@ -394,32 +420,39 @@ __global__ void __launch_bounds__(THREADS, 1)
                         umma::stmatrix_x4_trans(staging_a + (8 * (j + (mi >> 1)) + (lane & 7)) * ROW_BYTES + (16 * q + 8 * (mi & 1)) * 2, pk);
                     }
                 } else {
+                    // RESIDUAL: none, vectors in the staging buffer, elements.  Apart, since a branch inside would keep one value's instructions from another's.
+                    auto finish = [&](auto residual) {
+                        constexpr int RESIDUAL = decltype(residual)::value;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t place = staging_a + (8 * j + (lane & 7)) * ROW_BYTES + (32 * q + 8 * (lane >> 3)) * 2;
-                        uint32_t rs[4] = {0u, 0u, 0u, 0u}, pk[4];
-                        if (res_vec) umma::ldmatrix_x4_trans(rs, place);
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t place = staging_a + (8 * j + (lane & 7)) * ROW_BYTES + (32 * q + 8 * (lane >> 3)) * 2;
+                            uint32_t rs[4], pk[4];
+                            if (RESIDUAL == 1) umma::ldmatrix_x4_trans(rs, place);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
+                            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                float y[2] = {sum_of(h, j, e, 0), sum_of(h, j, e, 1)};
-                                if (res_vec) {
-                                    const float2 r2 = unpack2<BF16>(rs[2 * h + e]);
-                                    y[0] += r2.x;
-                                    y[1] += r2.y;
-                                } else if (res != nullptr) {
-                                    const int n = n0 + 32 * q + 16 * h + 8 * e + g;
+                                for (int e = 0; e < 2; ++e) {
+                                    float y[2] = {sum_of(h, j, e, 0), sum_of(h, j, e, 1)};
+                                    if (RESIDUAL == 1) {
+                                        const float2 r2 = unpack2<BF16>(rs[2 * h + e]);
+                                        y[0] += r2.x;
+                                        y[1] += r2.y;
+                                    } else if (RESIDUAL == 2) {
+                                        const int n = n0 + 32 * q + 16 * h + 8 * e + g;
 #pragma unroll
-                                    for (int i = 0; i < 2; ++i) {
-                                        const int m = cb * 32 + 8 * j + 2 * tq + i;
-                                        if (n < N && m < m_left) y[i] += value_at<BF16>(res, (int64_t)(m0 + m) * p.a.ldr + n);
+                                        for (int i = 0; i < 2; ++i) {
+                                            const int m = cb * 32 + 8 * j + 2 * tq + i;
+                                            if (n < N && m < m_left) y[i] += value_at<BF16>(res, (int64_t)(m0 + m) * p.a.ldr + n);
+                                        }
                                     }
+                                    pk[2 * h + e] = pack2<BF16>(y[0], y[1]);
                                 }
-                                pk[2 * h + e] = pack2<BF16>(y[0], y[1]);
-                            }
-                        umma::stmatrix_x4_trans(place, pk);
-                    }
+                            umma::stmatrix_x4_trans(place, pk);
+                        }
+                    };
+                    if (res == nullptr) finish(std::integral_constant<int, 0>());
+                    else if (res_vec) finish(std::integral_constant<int, 1>());
+                    else finish(std::integral_constant<int, 2>());
                 }
                 group_sync();  // the four warps: block complete; the other buffer is free
 #pragma unroll 4
