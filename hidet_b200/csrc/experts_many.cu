@@ -417,13 +417,30 @@ __global__ void __launch_bounds__(THREADS, 1) experts_product_kernel(const __gri
         const int eg = warp >> 2, q = warp & 3;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(32 * q) << 16);
         auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + eg) : "memory"); };
+        // A unit's scale is asked for a unit ahead, the powers of two eight slots ahead: with few k, results take longer than products.
+        int next_tile = 0, next_which = 0;
+        float next_scale = 0.0f;
+        auto ask = [&](int t) {
+            if (t >= mine.count()) return;
+            int expert;
+            at.find(mine.unit(t), expert, next_tile, next_which);
+            const int n = next_tile * 2 * TN + (int)rank * TN + 32 * q + lane;
+            next_scale = n < rows ? scale_at(DOWN ? a.down_scale : a.gate_up_scale, a.scale_type, (int64_t)expert * rows + n) : 0.0f;
+        };
+        ask(0);
         for (int t = 0; t < mine.count(); ++t) {
-            int expert, tile, which;
-            at.find(mine.unit(t), expert, tile, which);
-            const Entry en = entry[which];
+            const int tile = next_tile;
+            const Entry en = entry[next_which];
+            const float scale = next_scale;
+            ask(t + 1);
             const int n = tile * 2 * TN + (int)rank * TN + 32 * q + lane;
             const bool there = n < rows;
-            const float scale = there ? scale_at(DOWN ? a.down_scale : a.gate_up_scale, a.scale_type, (int64_t)expert * rows + n) : 0.0f;
+            float4 b0, b1;
+            auto ask_back = [&](int c) {
+                if (c >= en.slots) return;
+                b0 = __ldcg(reinterpret_cast<const float4 *>(p.back + en.slot + c)), b1 = __ldcg(reinterpret_cast<const float4 *>(p.back + en.slot + c) + 1);
+            };
+            ask_back(8 * eg);
             const uint32_t buf = t & 1, acc = lane_addr + buf * MOST_COLUMNS;
             if (!all_of_128(1 + eg, wait(smem_u32(&acc_full[buf]), ((uint32_t)t >> 1) & 1, 10))) break;  // the group stays or leaves as one
             umma::fence_after_sync();
@@ -484,8 +501,8 @@ __global__ void __launch_bounds__(THREADS, 1) experts_product_kernel(const __gri
                             if (c + j < en.count) v[g][j] += __ldcg(from + (g * en.count + c + j) * TN);
                 }
                 const int slot = en.slot + c;
-                const float4 b0 = __ldcg(reinterpret_cast<const float4 *>(p.back + slot)), b1 = __ldcg(reinterpret_cast<const float4 *>(p.back + slot) + 1);
                 const float back[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+                ask_back(c + 8 * EPI_GROUPS);
                 float y[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[j] = fmaf((float)v[2][j], 65536.0f, fmaf((float)v[1][j], 256.0f, (float)v[0][j])) * scale * back[j];  // the scale first: it and the power of two may be small together
