@@ -22,6 +22,7 @@
 
 #include "experts.h"
 #include "experts_digits.cuh"
+#include "experts_parts.cuh"
 #include "serving.cuh"
 #include "umma.cuh"
 #include "umma_i8_pair.cuh"
@@ -35,8 +36,7 @@ using i8pair::load_pair;
 using i8pair::mma_pair_i8;
 
 constexpr unsigned int kKernelExpertsMany = 13;
-constexpr int MOST = 80;                      // assignments of an entry: 240 columns
-constexpr int SLOTS = 16;                     // an entry's slots are a multiple of this
+constexpr int MOST = kEntryMost, SLOTS = kEntrySlots;
 constexpr int MOST_EXPERTS = 512, MOST_ASSIGNMENTS = 8192, MOST_ENTRIES = MOST_EXPERTS + MOST_ASSIGNMENTS / MOST + 1;
 constexpr int MOST_SLOTS = MOST_ASSIGNMENTS + (SLOTS - 1) * MOST_ENTRIES;
 constexpr int MOST_PAIRS = 512;               // which have four of the workspace's counters each: arrivals at a unit that pairs share, at the first of them, by CTA and group
@@ -50,7 +50,6 @@ constexpr int STAGES = 6;
 constexpr int STAGE_BYTES = W_BYTES + MOST_COLUMNS / 2 * BK;
 constexpr int EPI_GROUPS = 2, LOAD_WARP = 8, MMA_WARP = 9, THREADS = 32 * 10;
 constexpr int TMEM_COLS = 512;
-constexpr int MOST_SPLIT = 8;
 
 struct Group {  // an expert that has a token
     uint16_t expert, first, entries, none;
@@ -113,12 +112,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) experts_plan_kernel(const ManyAr
         const int of_lane = (a.count + 31) / 32, e0 = min(a.count, (int)threadIdx.x * of_lane), e1 = min(a.count, e0 + of_lane);
         int my[3] = {0, 0, 0}, largest = 0;  // groups, entries, slots
         for (int e = e0; e < e1; ++e) {
-            const int c = counts[e], entries = (c + MOST - 1) / MOST, size = c > 0 ? (c + entries - 1) / entries : 1;
-            each[e] = size;
-            if (c == 0) continue;
-            const int last = c - (entries - 1) * size;  // at least one
-            largest = max(largest, (size + SLOTS - 1) / SLOTS * SLOTS);
-            my[0] += 1, my[1] += entries, my[2] += (entries - 1) * ((size + SLOTS - 1) / SLOTS * SLOTS) + (last + SLOTS - 1) / SLOTS * SLOTS;
+            const EntrySizes its(counts[e]);
+            each[e] = its.size;
+            if (counts[e] == 0) continue;
+            largest = max(largest, its.room(0));
+            my[0] += 1, my[1] += its.entries, my[2] += its.slots();
         }
         int at[3] = {my[0], my[1], my[2]};
 #pragma unroll
@@ -138,14 +136,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) experts_plan_kernel(const ManyAr
 #pragma unroll
         for (int i = 0; i < 3; ++i) at[i] -= my[i];
         for (int e = e0; e < e1; ++e) {
-            const int c = counts[e], size = each[e], entries = (c + MOST - 1) / MOST;
+            const EntrySizes its(counts[e]);
             first_slot[e] = at[2];
-            if (c == 0) continue;
-            p.plan->group[at[0]++] = {(uint16_t)e, (uint16_t)at[1], (uint16_t)entries, 0};
-            for (int i = 0; i < c; i += size) {
-                const int here = min(size, c - i), room = (here + SLOTS - 1) / SLOTS * SLOTS;
-                p.plan->entry[at[1]++] = {(uint16_t)at[2], (uint16_t)here, (uint16_t)room, 0};
-                at[2] += room;
+            if (counts[e] == 0) continue;
+            p.plan->group[at[0]++] = {(uint16_t)e, (uint16_t)at[1], (uint16_t)its.entries, 0};
+            for (int i = 0; i < its.entries; ++i) {
+                p.plan->entry[at[1]++] = {(uint16_t)at[2], (uint16_t)its.assignments(i), (uint16_t)its.room(i), 0};
+                at[2] += its.room(i);
             }
             counts[e] = 0;
         }
@@ -158,7 +155,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) experts_plan_kernel(const ManyAr
         int slot = -1;
         if (e >= 0 && e < a.count) {
             const int place = atomicAdd(&counts[e], 1), size = each[e], entry = place / size, in = place - entry * size;
-            const int start = first_slot[e] + entry * ((size + SLOTS - 1) / SLOTS * SLOTS);
+            const int start = first_slot[e] + entry * EntrySizes::rounded(size);
             slot = start + in;
             p.slot[slot] = {i, DIGITS * start + in, 0};
         }
@@ -248,25 +245,6 @@ struct Units {
 // A map of the image for each number of slots, by the columns that a CTA copies.
 struct ImageMaps {
     CUtensorMap of[MOST / SLOTS];
-};
-
-// The units of a pair: whole rounds of all pairs, neighbours at a time, and of the units that are left each is shared by `split` pairs, a part of K each.  Bringing a unit together costs the
-// time of some stages, and of some more for each pair and ten slots.
-struct Rounds {
-    int rounds, split, rest, pairs, pair, k_blocks;
-    __device__ __forceinline__ Rounds(int units, int k_blocks_, int pairs_, int pair_, int slots) : pairs(pairs_), pair(pair_), k_blocks(k_blocks_) {
-        rounds = units / pairs, rest = units - rounds * pairs, split = 1;
-        int least = k_blocks;
-        for (int s = 2; s <= MOST_SPLIT && rest * s <= pairs && s <= k_blocks; ++s) {
-            const int cost = (k_blocks + s - 1) / s + 4 + (s - 1) * slots / 10;
-            if (cost < least) least = cost, split = s;
-        }
-    }
-    __device__ __forceinline__ int count() const { return rounds + (pair < rest * split ? 1 : 0); }
-    __device__ __forceinline__ bool shared(int i) const { return i == rounds && split > 1; }
-    __device__ __forceinline__ int unit(int i) const { return i < rounds ? i * pairs + pair : rounds * pairs + pair / split; }
-    __device__ __forceinline__ int first_k(int i) const { return i < rounds ? 0 : k_blocks * (pair % split) / split; }
-    __device__ __forceinline__ int last_k(int i) const { return i < rounds ? k_blocks : k_blocks * (pair % split + 1) / split; }
 };
 
 template <bool DOWN>

@@ -1,4 +1,5 @@
-// What a CTA of the kernels of experts_stream.cu takes of a line of stages, and where its pieces lie when a unit has several CTAs.
+// What a CTA of the kernels of experts_stream.cu takes of a line of stages, and where its pieces lie when a unit has several CTAs; how experts_many.cu cuts an expert's assignments into entries, and
+// which units, and which part of their k, a pair has.
 //
 // No header of CUDA's is included, so that it runs on the host as well (tests/host/experts_parts.cpp).
 #pragma once
@@ -26,6 +27,41 @@ struct Parts {
     }
     // A CTA has at most two places for what it holds of something shared: the first for what its part begins with, the second for what it ends with.
     __host__ __device__ __forceinline__ bool second_place(uint32_t cta, uint32_t first_stage) const { return first_of(cta) < first_stage; }
+};
+
+// An expert's assignments in entries of one size but the last, each with slots for a multiple of kEntrySlots.
+constexpr int kEntryMost = 80;   // 240 columns
+constexpr int kEntrySlots = 16;
+struct EntrySizes {
+    int count, entries, size;
+    __host__ __device__ __forceinline__ EntrySizes(int count_) : count(count_) {
+        entries = (count + kEntryMost - 1) / kEntryMost;
+        size = count > 0 ? (count + entries - 1) / entries : 1;
+    }
+    __host__ __device__ static __forceinline__ int rounded(int n) { return (n + kEntrySlots - 1) / kEntrySlots * kEntrySlots; }
+    __host__ __device__ __forceinline__ int assignments(int entry) const { return entry + 1 < entries ? size : count - entry * size; }  // of the last: at least one, up to 8192 in all
+    __host__ __device__ __forceinline__ int room(int entry) const { return rounded(assignments(entry)); }
+    __host__ __device__ __forceinline__ int slots() const { return (entries - 1) * rounded(size) + room(entries - 1); }
+};
+
+constexpr int kMostSplit = 8;
+// The units of a pair: whole rounds of all pairs, neighbours at a time, and of the units that are left each is shared by `split` pairs, a part of K each.  Bringing a unit together costs the
+// time of some stages, and of some more for each pair and ten slots.
+struct Rounds {
+    int rounds, split, rest, pairs, pair, k_blocks;
+    __host__ __device__ __forceinline__ Rounds(int units, int k_blocks_, int pairs_, int pair_, int slots) : pairs(pairs_), pair(pair_), k_blocks(k_blocks_) {
+        rounds = units / pairs, rest = units - rounds * pairs, split = 1;
+        int least = k_blocks;
+        for (int s = 2; s <= kMostSplit && rest * s <= pairs && s <= k_blocks; ++s) {
+            const int cost = (k_blocks + s - 1) / s + 4 + (s - 1) * slots / 10;
+            if (cost < least) least = cost, split = s;
+        }
+    }
+    __host__ __device__ __forceinline__ int count() const { return rounds + (pair < rest * split ? 1 : 0); }
+    __host__ __device__ __forceinline__ bool shared(int i) const { return i == rounds && split > 1; }
+    __host__ __device__ __forceinline__ int unit(int i) const { return i < rounds ? i * pairs + pair : rounds * pairs + pair / split; }
+    __host__ __device__ __forceinline__ int first_k(int i) const { return i < rounds ? 0 : k_blocks * (pair % split) / split; }
+    __host__ __device__ __forceinline__ int last_k(int i) const { return i < rounds ? k_blocks : k_blocks * (pair % split + 1) / split; }
 };
 
 }  // namespace b200q

@@ -79,3 +79,38 @@ def test_plan_of_a_product(ask, sms):
             assert tm % 16 == 0 and split in (1, 2, 4, 8)
     if sms == 148:  # where the forms were timed, none is without a size
         assert seen == {(p, s) for p, most in ((0, 8), (1, 4)) for s in (1, 2, 4, 8) if s <= most}
+
+
+def test_rounds_of_units(ask):
+    """Every unit's k has every block once, in parts that are not empty, by pairs whose number in a row says who shares it; a pair's units ascend, and the shared one is its last."""
+    rng = random.Random(4)
+    cases = [(896, 32, 74, 16), (128, 112, 74, 16), (256, 112, 74, 64), (64, 4, 74, 64), (8, 16, 74, 64), (1, 1, 74, 16), (0, 7, 74, 16), (1, 1024, 74, 80), (74, 3, 74, 80), (75, 200, 74, 16)]
+    cases += [(rng.randint(0, 400), rng.randint(1, 130), rng.choice([1, 3, 10, 66, 74]), 16 * rng.randint(1, 5)) for _ in range(1500)]
+    shared_somewhere = False
+    for (units, k_blocks, pairs, slots), numbers in zip(cases, ask([('rounds',) + c for c in cases])):
+        parts, at = {}, 1
+        for pair in range(pairs):
+            count, mine = numbers[at], numbers[at + 1:at + 1 + 4 * numbers[at]]
+            at += 1 + 4 * count
+            own = [mine[i:i + 4] for i in range(0, len(mine), 4)]
+            assert all(a[0] < b[0] for a, b in zip(own, own[1:])) and all(split == 1 for _, _, _, split in own[:-1])
+            for unit, first, last, split in own:
+                assert 0 <= first < last <= k_blocks
+                parts.setdefault(unit, []).append((first, last, pair, split))
+        assert at == len(numbers) and sorted(parts) == list(range(units))
+        for unit, own in parts.items():
+            split = own[0][3]
+            shared_somewhere |= split > 1
+            assert len(own) == split and all(s == split for _, _, _, s in own) and own[0][0] == 0 and own[-1][1] == k_blocks
+            assert all(a[1] == b[0] for a, b in zip(own, own[1:]))
+            first = own[0][2]
+            assert split == 1 or (first % split == 0 and [pair for _, _, pair, _ in own] == list(range(first, first + split)))
+    assert shared_somewhere
+
+
+def test_entries_of_an_expert(ask):
+    counts = list(range(1, 8193))
+    for count, numbers in zip(counts, ask([('entries', c, 0, 0, 0) for c in counts])):
+        slots, size, sizes, rooms = numbers[0], numbers[1], numbers[2::2], numbers[3::2]
+        assert sum(sizes) == count and sum(rooms) == slots and len(sizes) == -(-count // 80)
+        assert all(s == size for s in sizes[:-1]) and 1 <= sizes[-1] <= size <= 80 and all(r == -(-s // 16) * 16 for s, r in zip(sizes, rooms))
