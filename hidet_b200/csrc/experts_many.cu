@@ -18,6 +18,7 @@
 // What bounds it, two of eight experts of 4096 x 14336: with 64 tokens (248 us) the weights' way from memory, 215 us; with 512 (570 us: 270 + 145 us by themselves, the rest small kernels and
 // the clock under the power cap) and 2048 (2.0 ms, 2.1 POP/s) an SM's copies, some 40 bytes a clock of which 16 KB a stage are weights, whatever the entry's columns.  A copy of the
 // image is one box: in boxes of 16 rows 512 tokens took 733 us for 863.  Rows' largest magnitudes are stored by warp and not gathered with atomics: gate and up 332 us with them, 274 without.
+// With few k (1000 tokens, four of 32 of 1024 x 512: 72 us, 50 of them the products) results take the time: four groups of warps make them, two take 88 us.
 #include <type_traits>
 
 #include "experts.h"
@@ -39,8 +40,8 @@ constexpr unsigned int kKernelExpertsMany = 13;
 constexpr int MOST = kEntryMost, SLOTS = kEntrySlots;
 constexpr int MOST_EXPERTS = 512, MOST_ASSIGNMENTS = 8192, MOST_ENTRIES = MOST_EXPERTS + MOST_ASSIGNMENTS / MOST + 1;
 constexpr int MOST_SLOTS = MOST_ASSIGNMENTS + (SLOTS - 1) * MOST_ENTRIES;
-constexpr int MOST_PAIRS = 512;               // which have four of the workspace's counters each: arrivals at a unit that pairs share, at the first of them, by CTA and group
-static_assert(MOST_SLOTS < 65536 && 4 * MOST_PAIRS <= kWorkspaceCounters, "slots' numbers have 16 bits");
+constexpr int MOST_PAIRS = 512;               // which have some of the workspace's counters each: arrivals at a unit that pairs share, at the first of them, by CTA and group
+static_assert(MOST_SLOTS < 65536 && 8 * MOST_PAIRS <= kWorkspaceCounters, "slots' numbers have 16 bits");
 
 constexpr int TN = 128;                       // rows of the weight per CTA; a pair's tile has twice as many
 constexpr int BK = 128;
@@ -48,7 +49,7 @@ constexpr int W_BYTES = BK * TN;
 constexpr int MOST_COLUMNS = 256;
 constexpr int STAGES = 6;
 constexpr int STAGE_BYTES = W_BYTES + MOST_COLUMNS / 2 * BK;
-constexpr int EPI_GROUPS = 2, LOAD_WARP = 8, MMA_WARP = 9, THREADS = 32 * 10;
+constexpr int EPI_GROUPS = 4, LOAD_WARP = 4 * EPI_GROUPS, MMA_WARP = LOAD_WARP + 1, THREADS = 32 * (MMA_WARP + 1);
 constexpr int TMEM_COLS = 512;
 
 struct Group {  // an expert that has a token
@@ -94,18 +95,24 @@ struct ManyArgs {
 constexpr int PLAN_THREADS = 1024;
 
 __global__ void __launch_bounds__(PLAN_THREADS) experts_plan_kernel(const ManyArgs p) {
-    __shared__ int counts[MOST_EXPERTS], first_slot[MOST_EXPERTS], each[MOST_EXPERTS];
-    __shared__ int slots;
+    __shared__ int counts[MOST_EXPERTS], taken[MOST_EXPERTS], first_slot[MOST_EXPERTS];
     const ExpertsArgs &a = p.a;
     const int n = a.tokens * a.top;
     pdl_launch_dependents();
-    for (int e = threadIdx.x; e < a.count; e += PLAN_THREADS) counts[e] = 0;
+    for (int e = threadIdx.x; e < a.count; e += PLAN_THREADS) counts[e] = 0, taken[e] = 0;
     __syncthreads();
     pdl_wait();
-    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
-        const int e = a.experts[i];
-        if (e >= 0 && e < a.count) atomicAdd(&counts[e], 1);
-        else if (e >= 0 && a.status != nullptr) atomicOr(a.status, kBadExpert);
+    constexpr int MINE = MOST_ASSIGNMENTS / PLAN_THREADS;
+    int mine[MINE];
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        const int i = j * PLAN_THREADS + (int)threadIdx.x;
+        mine[j] = i < n ? a.experts[i] : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        if (mine[j] >= 0 && mine[j] < a.count) atomicAdd(&counts[mine[j]], 1);
+        else if (mine[j] >= 0 && a.status != nullptr) atomicOr(a.status, kBadExpert);
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -113,7 +120,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) experts_plan_kernel(const ManyAr
         int my[3] = {0, 0, 0}, largest = 0;  // groups, entries, slots
         for (int e = e0; e < e1; ++e) {
             const EntrySizes its(counts[e]);
-            each[e] = its.size;
             if (counts[e] == 0) continue;
             largest = max(largest, its.room(0));
             my[0] += 1, my[1] += its.entries, my[2] += its.slots();
@@ -131,7 +137,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) experts_plan_kernel(const ManyAr
         if (threadIdx.x == 31) {
             p.plan->largest = largest;
             p.plan->groups = at[0], p.plan->entries = at[1], p.plan->slots = at[2];
-            slots = at[2];
         }
 #pragma unroll
         for (int i = 0; i < 3; ++i) at[i] -= my[i];
@@ -144,28 +149,24 @@ __global__ void __launch_bounds__(PLAN_THREADS) experts_plan_kernel(const ManyAr
                 p.plan->entry[at[1]++] = {(uint16_t)at[2], (uint16_t)its.assignments(i), (uint16_t)its.room(i), 0};
                 at[2] += its.room(i);
             }
-            counts[e] = 0;
         }
+    } else {
+        for (int s = threadIdx.x - 32; s < p.most_slots; s += PLAN_THREADS - 32) p.slot[s] = {-1, 0, 0};  // nobody's, until the others have theirs
     }
     __syncthreads();
-    for (int s = threadIdx.x; s < slots; s += PLAN_THREADS) p.slot[s] = {-1, 0, 0};
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
-        const int e = a.experts[i];
+#pragma unroll
+    for (int j = 0; j < MINE; ++j) {
+        const int i = j * PLAN_THREADS + (int)threadIdx.x, e = mine[j];
+        if (i >= n) break;
         int slot = -1;
         if (e >= 0 && e < a.count) {
-            const int place = atomicAdd(&counts[e], 1), size = each[e], entry = place / size, in = place - entry * size;
-            const int start = first_slot[e] + entry * EntrySizes::rounded(size);
+            const EntrySizes its(counts[e]);
+            const int place = atomicAdd(&taken[e], 1), entry = place / its.size, in = place - entry * its.size;
+            const int start = first_slot[e] + entry * EntrySizes::rounded(its.size);
             slot = start + in;
-            p.slot[slot] = {i, DIGITS * start + in, 0};
+            p.slot[slot] = {i, DIGITS * start + in, its.room(entry)};
         }
         p.slot_of[i] = slot;
-    }
-    __syncthreads();
-    // how far a slot's digits are apart: its entry's slots
-    for (int k = threadIdx.x >> 5; k < p.plan->entries; k += PLAN_THREADS / 32) {
-        const Entry en = p.plan->entry[k];
-        for (int i = threadIdx.x & 31; i < en.count; i += 32) p.slot[en.slot + i].stride = en.slots;
     }
 }
 
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_product_kernel(const __gri
             if (!mbar_wait(smem_u32(&drain_bar), 0)) report_timeout(a.status, kKernelExpertsMany, 8);
         }
     } else {
-        // ---------------- results: a lane a row of the weight, eight assignments at a time, the two groups in turn ----------------
+        // ---------------- results: a lane a row of the weight, eight assignments at a time, the groups in turn ----------------
         const int eg = warp >> 2, q = warp & 3;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(32 * q) << 16);
         auto group_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + eg) : "memory"); };
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(THREADS, 1) experts_product_kernel(const __gri
                 }
                 group_sync();
                 if ((threadIdx.x & 127) == 0) {
-                    unsigned int *counter = p.counters + 4 * p0 + 2 * rank + eg, before;
+                    unsigned int *counter = p.counters + (2 * p0 + (int)rank) * EPI_GROUPS + eg, before;
                     asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
                     const bool last = before == (unsigned int)(p1 - p0);
                     if (last) *counter = 0;
