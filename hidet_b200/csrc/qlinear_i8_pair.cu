@@ -11,8 +11,8 @@
 //   warp 8     TMA producer; both CTAs' copies count on the first CTA's barrier
 //   warp 9     MMA issuer (first CTA of the pair only), one thread for the whole loop
 // Two accumulators, so that a tile's epilogue runs beside the next one's products.  With few k the epilogue is what takes the time (4096 x 1024 x 4096: 20 us, 11 without it), and what it reads
-// is asked for ahead: scales a tile, the residual a tile (into L2) and a block, tokens' scales a block (2048 x 512 x 8192 with a residual: 34 us without, 29 with).  Four groups instead of two
-// help there by 3 to 10 %, and cost 1 to 5 % elsewhere.
+// is asked for ahead: scales a tile, the residual a tile (into L2) and a block, tokens' scales a block (2048 x 512 x 8192 with a residual: 34 us without, 29 with).  Four groups
+// instead of two have registers for too little of that (26 us for 20).
 //
 // Where tiles are few, K is shared by the two or four pairs of a cluster, a tile each cluster and no second one.  Sums are whole numbers: when all have theirs, every pair
 // hands the others the 32-token blocks that they finish (its fragments as they come out of tensor memory, into the ring, which is no longer in use) and adds what it gets.
