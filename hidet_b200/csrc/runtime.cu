@@ -149,6 +149,16 @@ B200Q_API const char *b200q_get_last_error(void) {
     return b200q::g_returned_error;
 }
 
+B200Q_API unsigned long long b200q_capture_id(void *stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 B200Q_API int b200q_check_status(void) {
     unsigned int *word = b200q::device_status_word();
     if (word == nullptr) return b200q::set_error(B200Q_CUDA_ERROR, "no usable CUDA device for the calling thread");

@@ -39,6 +39,7 @@ F16, BF16, F32 = 0, 1, 2
 I8, I16 = 0, 1
 LAYOUT_KN, LAYOUT_NK = 0, 1
 ACT_NONE, ACT_SILU_MUL = 0, 1
+WORKSPACE_HEAD = 65536 * 4  # bytes at a workspace's beginning that hold counters
 ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 
 
@@ -131,6 +132,7 @@ SIGNATURES = {
     'b200q_version': ([], c_int, False),
     'b200q_get_last_error': ([], c_char_p, False),
     'b200q_check_status': ([], c_int, True),
+    'b200q_capture_id': ([c_void_p], ctypes.c_ulonglong, False),
     'b200q_symmetric_quantize': ([c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p], c_int, True),
     'b200q_symmetric_dequantize': ([c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_void_p], c_int, True),
     'b200q_embedding_dequantize': (

@@ -5,7 +5,7 @@ libhidet_b200q.so.
 """
 from __future__ import annotations
 
-from typing import Dict, Optional, Tuple
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
@@ -35,26 +35,49 @@ class _Workspaces:
     """Grow-only, zero-initialised scratch per (device, stream), the role request_cuda_workspace
     plays in the reference (src/hidet/runtime/cuda/context.cpp:31-49,90-104).  The library keeps the
     part that must be zero (its tile counters) zero between calls, so a buffer is cleared only when it
-    is created."""
+    is created.
+
+    A buffer that is made while a graph is captured is cleared by a node of that graph, so it is nobody else's: not
+    another graph's, which may be replayed first, nor that of calls outside.  One that is replaced by a larger one is kept,
+    since a graph may have been captured with it; sizes double, so that all of them are no more than the last."""
 
     def __init__(self):
         self._buffers: Dict[Tuple[int, int], torch.Tensor] = {}
+        self._captures: Dict[Tuple[int, int], int] = {}  # of buffers that a graph made: which
+        self._replaced: List[torch.Tensor] = []
 
     def get(self, device: torch.device, nbytes: int) -> Tuple[int, int]:
         if nbytes == 0:
             return 0, 0
         index = device.index if device.index is not None else torch.cuda.current_device()
         key = (index, current_stream_ptr(device))
-        buf = self._buffers.get(key)
-        if buf is None or buf.numel() < nbytes:
+        buf, made_by = self._buffers.get(key), self._captures.get(key, 0)
+        capture = ffi.func('b200q_capture_id')(key[1]) if torch.cuda.is_current_stream_capturing() else 0
+        if buf is None or buf.numel() < nbytes or made_by not in (0, capture):
             size = 1 << max(20, (nbytes - 1).bit_length())
-            buf = torch.zeros(size, dtype=torch.uint8, device=torch.device('cuda', index))
+            if buf is not None and made_by == 0:
+                self._replaced.append(buf)
+            device = torch.device('cuda', index)
+            if capture:
+                buf = torch.empty(size, dtype=torch.uint8, device=device)
+                buf[:ffi.WORKSPACE_HEAD].zero_()  # with every replay
+            else:
+                buf = torch.zeros(size, dtype=torch.uint8, device=device)
             self._buffers[key] = buf
-        native.set_scratch(*key, buf.data_ptr(), buf.numel())  # for the native host path, which may be younger than the buffer
+            self._captures.pop(key, None)
+            if capture:
+                self._captures[key] = capture
+            made_by = capture
+        if made_by:
+            native.set_scratch(*key, 0, 0)  # the native host path does not know of captures
+        else:
+            native.set_scratch(*key, buf.data_ptr(), buf.numel())  # for that path, which may be younger than the buffer
         return buf.data_ptr(), buf.numel()
 
     def clear(self) -> None:
         self._buffers.clear()
+        self._captures.clear()
+        self._replaced.clear()
         native.clear_scratch()
 
     def swap(self, device: torch.device, stream: int, buffer: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -64,6 +87,7 @@ class _Workspaces:
         share the buffer nor replace it by a larger one while the graph still writes to it."""
         index = device.index if device.index is not None else torch.cuda.current_device()
         before = self._buffers.pop((index, stream), None)
+        self._captures.pop((index, stream), None)
         if buffer is not None:
             self._buffers[(index, stream)] = buffer
         native.set_scratch(index, stream, buffer.data_ptr() if buffer is not None else 0, buffer.numel() if buffer is not None else 0)

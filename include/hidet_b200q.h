@@ -73,6 +73,9 @@ typedef enum b200q_weight_layout { B200Q_LAYOUT_KN = 0, B200Q_LAYOUT_NK = 1 } b2
 /* Library version as major*10000 + minor*100 + patch. */
 B200Q_API int b200q_version(void);
 
+/* The number of the capture that `stream` records, which no other has; 0 where it records none.  A workspace that was cleared by a node of one graph is no workspace for another. */
+B200Q_API unsigned long long b200q_capture_id(void *stream);
+
 /* Message of the last failed call on this thread, or "" if none; clears it.
  * Counterpart of hidet_get_last_error (src/hidet/runtime/logging.cpp:29-36). */
 B200Q_API const char *b200q_get_last_error(void);
