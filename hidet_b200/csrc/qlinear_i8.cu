@@ -2,8 +2,6 @@
 #include "qlinear_i8.h"
 #include "qlinear_i8_plan.h"
 #include "serving.cuh"
-#include <cstdio>
-#include <cstdlib>
 
 namespace b200q {
 namespace {
@@ -111,12 +109,6 @@ B200Q_API int b200q_qlinear_i8_i8(const void *a, const float *a_scale, const voi
     p.residual_vec = p.residual != nullptr && aligned_to(p.residual, 16) && (p.ldr % 8 == 0 || M == 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool lines = aligned_to(a, 16) && aligned_to(wq, 16) && aligned_to(c, 16) && K > 0 && K % 16 == 0 && (p.nk || N % 16 == 0) && width % 8 == 0;
-    if (const char *e = getenv("I8_PLAN")) {
-        int kind = 0, tm = 0, cl = 1;
-        sscanf(e, "%d,%d,%d", &kind, &tm, &cl);
-        if (lines && kind == 1) return launch_i8_split(p, tm, cl, s);
-        if (lines && kind == 2) return launch_i8_pair(p, tm, cl, s);
-    }
     if (lines) {
         const I8Plan plan = plan_i8(M, N, K, sm_count() > 0 ? sm_count() : 148);
         return plan.pair ? launch_i8_pair(p, plan.tm, plan.split, s) : launch_i8_split(p, plan.tm, plan.split, s);
