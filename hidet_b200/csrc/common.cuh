@@ -63,6 +63,11 @@ int resident_clusters(const void *kernel, int threads, int smem, int cluster);
 // True where the stream has only some of the device's SMs (a green context's): launches there may not hold what the device holds.
 bool part_of_device(cudaStream_t stream);
 
+// quantize_tokens lets the kernel behind it start before its codes are there, and the kernel of f16 rows on int8 weights for few rows reads a weight's first codes before the kernel in front has
+// finished.  The former notes its stream, and the latter, where it finds that noted, is launched behind the end of all in front of it and takes the note away.
+void note_unfinished_codes(cudaStream_t stream);
+bool take_unfinished_codes(cudaStream_t stream);
+
 // Encodes a 2-D tiled tensor map.  `inner`/`outer` are the tensor extents in elements, `row_bytes`
 // the stride between consecutive outer indices, box_* the tile extents.  swizzle is a
 // CUtensorMapSwizzle value.  Returns a b200q_status.

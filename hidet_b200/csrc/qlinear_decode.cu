@@ -873,7 +873,7 @@ int launch_decode_kn(const void *a, const void *wq, const void *scale, void *c, 
     attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attrs[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attrs;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = take_unfinished_codes(stream) ? 1 : 2;  // the codes may be those of a kernel in front that lets others start before they are there
     void *args[2] = {&map_w, &p};
     B200Q_CUDA_TRY(cudaLaunchKernelExC(&cfg, kernel, args));
     return B200Q_OK;

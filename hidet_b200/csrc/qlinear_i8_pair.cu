@@ -168,15 +168,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                 load_pair(smem_base + slot * stage_bytes, &map_w, NK ? kb * BK : n, NK ? n : kb * BK, full0 + 8 * slot, keep);
             };
             auto load_a = [&](uint32_t slot, int m, int kb) { load_pair(smem_base + slot * stage_bytes + W_BYTES, &map_a, kb * BK, m, full0 + 8 * slot, keep); };
-            // The first tile's weights are requested before the kernel in front has finished, its tokens behind it.
+            // The first tile's weights are asked for into L2 before the kernel in front has finished, which may be the one that writes them; they come from there behind it, with the tokens.
             int n, m;
             tile_of(p, first, n, m);
             n += (int)rank * TN;
             m += (int)rank * (p.tm / 2);
             const int ahead = min(kb1 - kb0, (int)stages);
-            for (int j = 0; j < ahead; ++j) load_w(j, n, kb0 + j);
+            for (int j = 0; j < ahead; ++j) tma_prefetch_2d(&map_w, NK ? (kb0 + j) * BK : n, NK ? n : (kb0 + j) * BK);
             pdl_wait();
-            for (int j = 0; j < ahead; ++j) load_a(j, m, kb0 + j);
+            for (int j = 0; j < ahead; ++j) load_w(j, n, kb0 + j), load_a(j, m, kb0 + j);
             uint32_t i = 0;
             umma::Ring r;
             bool ok = true;

@@ -101,6 +101,51 @@ int resident_clusters(const void *kernel, int threads, int smem, int cluster) {
     return n;
 }
 
+namespace {
+struct Noted {
+    int device;
+    cudaStream_t stream;
+};
+constexpr int kMostNoted = 256;  // with more, every stream counts as noted from then on
+std::mutex g_noted_mutex;
+Noted g_noted[kMostNoted];
+std::atomic<int> g_noted_count{0};
+}  // namespace
+
+void note_unfinished_codes(cudaStream_t stream) {
+    int device = -1;
+    (void)cudaGetDevice(&device);
+    const std::lock_guard<std::mutex> lock(g_noted_mutex);
+    const int n = g_noted_count.load(std::memory_order_relaxed);
+    for (int i = 0; i < n && i < kMostNoted; ++i)
+        if (g_noted[i].device == device && g_noted[i].stream == stream) return;
+    if (n < kMostNoted) g_noted[n] = {device, stream};
+    if (n <= kMostNoted) g_noted_count.store(n + 1, std::memory_order_release);
+}
+
+bool take_unfinished_codes(cudaStream_t stream) {
+    if (g_noted_count.load(std::memory_order_acquire) == 0) return false;
+    int device = -1;
+    (void)cudaGetDevice(&device);
+    const std::lock_guard<std::mutex> lock(g_noted_mutex);
+    const int n = g_noted_count.load(std::memory_order_relaxed);
+    if (n > kMostNoted) return true;
+    int at = 0;
+    while (at < n && !(g_noted[at].device == device && g_noted[at].stream == stream)) ++at;
+    if (at == n) return false;
+    // A launch that is only captured orders nothing outside its graph, and a thread's own default stream has the same name in every thread: their notes stay.
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusActive;
+    if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) {
+        (void)cudaGetLastError();
+        status = cudaStreamCaptureStatusActive;
+    }
+    if (status == cudaStreamCaptureStatusNone && stream != cudaStreamPerThread) {
+        g_noted[at] = g_noted[n - 1];
+        g_noted_count.store(n - 1, std::memory_order_release);
+    }
+    return true;
+}
+
 bool part_of_device(cudaStream_t stream) {
     typedef CUresult (*GetGreenCtxFn)(CUstream, CUgreenCtx *);
     static GetGreenCtxFn fn = nullptr;

@@ -250,6 +250,7 @@ B200Q_API int b200q_quantize_tokens(const void *x, int64_t x_stride, const void 
     const int64_t size = type == B200Q_F32 ? 4 : 2;
     TokensArgs p = {x, x_stride, width > 0 ? norm : nullptr, eps, static_cast<int8_t *>(codes), scales, rows, (int)width,
                     aligned_to(x, 16) && (rows == 1 || x_stride * size % 16 == 0), aligned_to(norm, 16), aligned_to(codes, 8) && (rows == 1 || width % 8 == 0)};
+    note_unfinished_codes(s);
     switch (type) {
         case B200Q_F16: return p.norm ? launch_typed<__half, true>(p, s) : launch_typed<__half, false>(p, s);
         case B200Q_BF16: return p.norm ? launch_typed<__nv_bfloat16, true>(p, s) : launch_typed<__nv_bfloat16, false>(p, s);

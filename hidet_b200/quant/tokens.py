@@ -32,7 +32,9 @@ def quantize_tokens(x: torch.Tensor, norm: Optional[torch.Tensor] = None, eps: f
 
     A token's code is rint(y * (127 / amax)), its scale amax / 127, amax the largest magnitude of its y: x itself or, with norm [width] (of x's type),
     the RMS norm x / sqrt(mean(x^2) + eps) * norm, which is not rounded in between.  Tokens of zeros (below 2^-100) have a scale of zero; a token with a NaN or an infinity
-    has a scale of NaN, and so whatever is computed from it is NaN."""
+    has a scale of NaN, and so whatever is computed from it is NaN.
+
+    What it returns for rows [N, K] may also be a weight, at once: symmetric_quant_matmul_i8(*quantize_tokens(x), *quantize_tokens(w), weight_layout='NK')."""
     pair = native.quantize_tokens(x, norm, eps)
     if pair is not None:
         return pair
@@ -59,7 +61,7 @@ def symmetric_quant_matmul_i8(a: torch.Tensor, a_scale: torch.Tensor, weight: to
     """c[..., M, N] = (a[..., M, K] @ weight) * scale * a_scale[..., M, None] in `dtype` (float16 or bfloat16).
 
     a int8 with a_scale float32 (quantize_tokens), weight int8 [K, N] (weight_layout 'KN') or [N, K] ('NK') with scale [N] (float16, bfloat16 or float32).
-    The sum over k is exact (K up to 131071); scales, bias [N], activation and residual (both of `dtype`, in symmetric_quant_matmul's order and meaning, for either layout)
+    Every operand may be the result of the call in front.  The sum over k is exact (K up to 131071); scales, bias [N], activation and residual (both of `dtype`, in symmetric_quant_matmul's order and meaning, for either layout)
     are float and the result is rounded once.  out: a contiguous tensor for the result, which may be the residual."""
     c = native.matmul_i8(a, a_scale, weight, scale, weight_layout, out, bias, residual, activation, dtype)
     if c is not None:

@@ -28,12 +28,13 @@
  *     24 rows on weights of 6 Mi codes and more.)
  *     Kernels that do not themselves execute griddepcontrol.launch_dependents (b200q_symmetric_quantize, the packing
  *     kernels and every other kernel of this library but the quantized linears and the operators around them (rotary, cache,
- *     attention, log probabilities), memcpy / memset nodes, ordinary kernels) let dependents start only when they have finished, so producing a weight with
+ *     attention, log probabilities, linears on int8 tokens, layers of experts), memcpy / memset nodes, ordinary kernels) let dependents start only when they have finished, so producing a weight with
  *     b200q_symmetric_quantize and using it in the next call on the same stream is safe.  Not safe: writing the codes of
  *     an int8 weight from a kernel that triggers its dependents early when nothing but kernels of that kind lie between
  *     it and the quantized linear that reads them on the same stream (the quantized linears are themselves of that
  *     kind: the f16 result of one of them may be the next one's scales, but its bytes may not be the next one's codes);
- *     put an event or any ordinary kernel between the two.
+ *     put an event or any ordinary kernel between the two.  b200q_quantize_tokens is the exception: it lets the kernel behind it start before its codes are there, notes that of its
+ *     stream, and the small-M kernel's next launch there waits for the end of all in front of it.  So its codes may be any linear's weight in the next call.
  *   - matrices are dense row-major.  "KN" weight layout = [K, N] with N contiguous, the layout of
  *     the reference operator (python/hidet/graph/ops/quant/matmul.py:30-32); "NK" = [N, K] with K
  *     contiguous, the layout torch.nn.Linear stores.
@@ -296,9 +297,9 @@ B200Q_API int b200q_qlinear_f16_i8_static(const void *a, const void *wq, const v
 /*
  * ---- linears on int8 tokens ----
  *
- * These and the layers of experts below are launched as programmatic dependents of the kernel in front and let the kernel behind them start early.  The codes of a weight
- * (wq, gate_up, down) may be requested before the dependency on the kernel in front is honoured, as b200q_qlinear_f16_i8 requests them for few rows:
- * what is said of them at the top of this file holds here for every size.  None of them writes the codes of a weight.
+ * These and the layers of experts below are launched as programmatic dependents of the kernel in front and let the kernel behind them start early.  Ahead of the dependency on the kernel in
+ * front the products ask for a weight's first codes into L2 only, which is where all writes meet; every operand (a, wq, gate_up, down, scales, experts and the others) is read behind it, at every size,
+ * so any of them may be the result of the kernel in front, whatever that is.  b200q_quantize_tokens writes codes that may be a weight [N, K] (see the top of this file).
  */
 
 /*
