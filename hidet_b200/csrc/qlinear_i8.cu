@@ -99,7 +99,7 @@ B200Q_API int b200q_qlinear_i8_i8(const void *a, const float *a_scale, const voi
     }
     if (M == 0 || N == 0) return B200Q_OK;
     if (K > kMostInner) return set_error(B200Q_UNSUPPORTED, "%s: K=%lld: sums of up to %lld products fit 32 bits", op, (long long)K, (long long)kMostInner);
-    if (M > 2147483647LL || N > 2147483647LL) return set_error(B200Q_UNSUPPORTED, "%s: sizes beyond 2^31-1 are not supported", op);
+    if (M > kMostOuter || N > kMostOuter) return set_error(B200Q_UNSUPPORTED, "%s: M=%lld N=%lld: sizes of 2^31-255 and more are not supported", op, (long long)M, (long long)N);
     if (c == nullptr || scale == nullptr || a_scale == nullptr || (K > 0 && (a == nullptr || wq == nullptr))) return set_error(B200Q_INVALID_ARGUMENT, "%s: null pointer argument", op);
     I8Args p = {};
     p.a = static_cast<const int8_t *>(a), p.w = static_cast<const int8_t *>(wq), p.a_scale = a_scale, p.scale = scale, p.bias = e.bias, p.residual = e.residual;

@@ -9,6 +9,7 @@
 namespace b200q {
 
 constexpr int64_t kMostInner = 131071;
+constexpr int64_t kMostOuter = 0x7fffffffLL - 255;  // of M and N: tiles of up to 256, whose ends are ints too
 
 struct I8Args {
     const int8_t *a, *w;

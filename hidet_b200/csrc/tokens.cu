@@ -14,6 +14,7 @@ namespace b200q {
 namespace {
 
 constexpr int MOST_THREADS = 1024;
+constexpr int64_t kMostWidth = 0x7fffffffLL - 8 * MOST_THREADS;  // the step behind a row's last element is an int too
 constexpr uint32_t kLeastAmax = 0x0d800000u;  // 2^-100: 127 / amax is finite from here on
 constexpr uint32_t kInfinity = 0x7f800000u;
 constexpr int ROWS_OF_WARPS = 8;              // rows of a CTA whose warps have one each
@@ -243,7 +244,7 @@ B200Q_API int b200q_quantize_tokens(const void *x, int64_t x_stride, const void 
     if (type < B200Q_F16 || type > B200Q_F32) return set_error(B200Q_INVALID_ARGUMENT, "%s: unknown float type %d", op, type);
     if (!(eps >= 0.0f && eps < INFINITY)) return set_error(B200Q_INVALID_ARGUMENT, "%s: eps must be a number of at least 0, got %g", op, (double)eps);
     if (rows == 0) return B200Q_OK;
-    if (width > 0x7fffff00LL || rows > 2147483647LL) return set_error(B200Q_UNSUPPORTED, "%s: %lld rows of %lld elements", op, (long long)rows, (long long)width);
+    if (width > kMostWidth || rows > 2147483647LL) return set_error(B200Q_UNSUPPORTED, "%s: %lld rows of %lld elements", op, (long long)rows, (long long)width);
     if (scales == nullptr || (width > 0 && (x == nullptr || codes == nullptr))) return set_error(B200Q_INVALID_ARGUMENT, "%s: null pointer argument", op);
     if (x_stride < 0) return set_error(B200Q_INVALID_ARGUMENT, "%s: negative stride", op);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -307,7 +307,7 @@ B200Q_API int b200q_qlinear_f16_i8_static(const void *a, const void *wq, const v
  *   y = x, or, with norm (of x's type, [width]), y = x * norm / sqrt(mean(x^2) + eps);   amax = max |y|
  *   codes[r, i] = rint(y_i * (127 / amax)) (ties to even; dense rows of `width` bytes),   scales[r] = amax / 127
  * in float, each operation rounded; behind the norm the codes are taken from x * norm, in which the row's factor cancels.  A row whose amax (of x, or of x * norm) is below 2^-100 is
- * zeros with a scale of zero; a row with a NaN or an infinity, or whose squares overflow in front of a norm, has a scale of NaN (codes of zero in the first case).
+ * zeros with a scale of zero; a row with a NaN or an infinity, or whose squares overflow in front of a norm, has a scale of NaN (codes of zero in the first case).  Rows of 2^31 - 8192 elements and more: B200Q_UNSUPPORTED.
  */
 B200Q_API int b200q_quantize_tokens(const void *x, int64_t row_stride, const void *norm, float eps, void *codes, float *scales, int64_t rows, int64_t width, int type,
                                     void *stream);
@@ -316,7 +316,7 @@ B200Q_API int b200q_quantize_tokens(const void *x, int64_t row_stride, const voi
  * The product of int8 tokens and an int8 weight: c[M, N] (f16 or bf16 by out_type) =
  *   float(sum_k a[m, k] wq[k, n]) * scale[n] * a_scale[m], then what `epilogue` (NULL: nothing) says, with bias and residual of c's type, in float, rounded once.
  * The sum is exact, of 32 bits, for K up to 131071; beyond, B200Q_UNSUPPORTED.  a int8 [M, K], a_scale float [M], wq int8 [K, N] or [N, K] by w_layout, scale [N] of scale_type
- * (b200q_float_type).  Any sizes and alignments; 16-byte aligned bases and rows (K, and N or N / 2 of the result) are fast.  c may be the residual.  No workspace.
+ * (b200q_float_type).  M and N below 2^31 - 255, any alignments; 16-byte aligned bases and rows (K, and N or N / 2 of the result) are fast.  c may be the residual.  No workspace.
  */
 B200Q_API int b200q_qlinear_i8_i8(const void *a, const float *a_scale, const void *wq, const void *scale, void *c, int64_t M, int64_t N, int64_t K, int w_layout,
                                   int scale_type, int out_type, const b200q_epilogue *epilogue, void *stream);
