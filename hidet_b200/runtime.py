@@ -43,7 +43,6 @@ class _Workspaces:
 
     def __init__(self):
         self._buffers: Dict[Tuple[int, int], torch.Tensor] = {}
-        self._captures: Dict[Tuple[int, int], int] = {}  # of buffers that a graph made: which
         self._replaced: List[torch.Tensor] = []
 
     def get(self, device: torch.device, nbytes: int) -> Tuple[int, int]:
@@ -51,32 +50,45 @@ class _Workspaces:
             return 0, 0
         index = device.index if device.index is not None else torch.cuda.current_device()
         key = (index, current_stream_ptr(device))
-        buf, made_by = self._buffers.get(key), self._captures.get(key, 0)
-        capture = ffi.func('b200q_capture_id')(key[1]) if torch.cuda.is_current_stream_capturing() else 0
+        buf, capture = self._buffers.get(key), self._capture(key[1])
+        made_by = self._made_by(buf)
         if buf is None or buf.numel() < nbytes or made_by not in (0, capture):
             size = 1 << max(20, (nbytes - 1).bit_length())
             if buf is not None and made_by == 0:
                 self._replaced.append(buf)
-            device = torch.device('cuda', index)
             if capture:
-                buf = torch.empty(size, dtype=torch.uint8, device=device)
+                buf = self._allocate(torch.empty, index, size)
                 buf[:ffi.WORKSPACE_HEAD].zero_()  # with every replay
+                buf.made_by = capture
             else:
-                buf = torch.zeros(size, dtype=torch.uint8, device=device)
+                buf = self._allocate(torch.zeros, index, size)
             self._buffers[key] = buf
-            self._captures.pop(key, None)
-            if capture:
-                self._captures[key] = capture
-            made_by = capture
-        if made_by:
+        self._tell(key)  # the native host path, which may be younger than the buffer
+        return buf.data_ptr(), buf.numel()
+
+    @staticmethod
+    def _capture(stream: int) -> int:
+        """The capture that the current stream is in, or 0."""
+        return ffi.func('b200q_capture_id')(stream) if torch.cuda.is_current_stream_capturing() else 0
+
+    @staticmethod
+    def _allocate(how, index: int, size: int) -> torch.Tensor:
+        return how(size, dtype=torch.uint8, device=torch.device('cuda', index))
+
+    @staticmethod
+    def _made_by(buffer: Optional[torch.Tensor]) -> int:
+        """The capture that made a buffer, or 0.  It stands with the buffer, which may leave its place and come back (swap)."""
+        return getattr(buffer, 'made_by', 0)
+
+    def _tell(self, key: Tuple[int, int]) -> None:
+        buf = self._buffers.get(key)
+        if buf is None or self._made_by(buf):
             native.set_scratch(*key, 0, 0)  # the native host path does not know of captures
         else:
-            native.set_scratch(*key, buf.data_ptr(), buf.numel())  # for that path, which may be younger than the buffer
-        return buf.data_ptr(), buf.numel()
+            native.set_scratch(*key, buf.data_ptr(), buf.numel())
 
     def clear(self) -> None:
         self._buffers.clear()
-        self._captures.clear()
         self._replaced.clear()
         native.clear_scratch()
 
@@ -87,10 +99,9 @@ class _Workspaces:
         share the buffer nor replace it by a larger one while the graph still writes to it."""
         index = device.index if device.index is not None else torch.cuda.current_device()
         before = self._buffers.pop((index, stream), None)
-        self._captures.pop((index, stream), None)
         if buffer is not None:
             self._buffers[(index, stream)] = buffer
-        native.set_scratch(index, stream, buffer.data_ptr() if buffer is not None else 0, buffer.numel() if buffer is not None else 0)
+        self._tell((index, stream))
         return before
 
 
