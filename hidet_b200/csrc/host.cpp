@@ -49,6 +49,7 @@ struct Library {
     decltype(&b200q_route_tokens) route_tokens = nullptr;
     decltype(&b200q_mixture_of_experts_workspace_bytes) experts_workspace_bytes = nullptr;
     decltype(&b200q_mixture_of_experts) experts = nullptr;
+    decltype(&b200q_capture_id) capture_id = nullptr;
 } lib;
 
 // Scratch buffers that the Python side owns and has told us about, by stream and device.
@@ -96,7 +97,7 @@ inline bool find_scratch(const Where &w, size_t need, void *&ptr, size_t &bytes)
     bytes = 0;
     if (need == 0) return true;
     const auto it = scratch.find({reinterpret_cast<uintptr_t>(w.stream), w.device});
-    if (it == scratch.end() || it->second.bytes < need) return false;
+    if (it == scratch.end() || it->second.bytes < need || lib.capture_id(w.stream) != 0) return false;  // a graph has scratch of its own
     ptr = it->second.ptr;
     bytes = it->second.bytes;
     return true;
@@ -679,7 +680,7 @@ PyObject *bind(PyObject *, PyObject *args) {
     auto set = [&](auto &member) { member = reinterpret_cast<std::remove_reference_t<decltype(member)>>(p[i++]); };
     set(lib.quantize), set(lib.dequantize), set(lib.take), set(lib.workspace_bytes), set(lib.linear), set(lib.linear_fused), set(lib.w4_workspace_bytes), set(lib.w4);
     set(lib.rotary), set(lib.append), set(lib.read), set(lib.attention_workspace_bytes), set(lib.attention), set(lib.log_probs);
-    set(lib.quantize_tokens), set(lib.matmul_i8), set(lib.route_tokens), set(lib.experts_workspace_bytes), set(lib.experts);
+    set(lib.quantize_tokens), set(lib.matmul_i8), set(lib.route_tokens), set(lib.experts_workspace_bytes), set(lib.experts), set(lib.capture_id);
     Py_RETURN_NONE;
 }
 

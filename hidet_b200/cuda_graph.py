@@ -29,7 +29,7 @@ class CudaGraph:
         device = self._inputs[0].device
         self._stream = torch.cuda.Stream(device)
         self._stream.wait_stream(torch.cuda.current_stream(device))
-        around = workspaces.swap(device, self._stream.cuda_stream, None)
+        around = workspaces.swap(device, self._stream.cuda_stream, None, exclusive=True)
         try:
             with torch.cuda.stream(self._stream):
                 for _ in range(max(num_warmup, 1)):  # allocates the graph's scratch before the capture
@@ -69,7 +69,9 @@ class CudaGraph:
         # The scratch belongs to the capture stream.  Once this object is gone its block must not be handed out there before
         # the replays on other streams are over.
         if self._scratch is not None and stream.cuda_stream not in self._replayed_on:
-            self._scratch.record_stream(stream)
+            for buffer in (self._scratch, workspaces.outside(self._scratch)):  # the second where the capture needed more than the warm-up
+                if buffer is not None:
+                    buffer.record_stream(stream)
             self._replayed_on.add(stream.cuda_stream)
         with torch.cuda.stream(stream):
             self._graph.replay()

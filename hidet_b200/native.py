@@ -28,7 +28,7 @@ _BOUND = ('b200q_symmetric_quantize', 'b200q_symmetric_dequantize', 'b200q_embed
           'b200q_qlinear_f16_i8', 'b200q_qlinear_f16_i8_fused', 'b200q_qlinear_f16_u4_workspace_bytes', 'b200q_qlinear_f16_u4',
           'b200q_rotary_embedding', 'b200q_quantized_cache_append', 'b200q_quantized_cache_read', 'b200q_quantized_cache_attention_workspace_bytes',
           'b200q_quantized_cache_attention', 'b200q_token_log_probs', 'b200q_quantize_tokens', 'b200q_qlinear_i8_i8', 'b200q_route_tokens',
-          'b200q_mixture_of_experts_workspace_bytes', 'b200q_mixture_of_experts')
+          'b200q_mixture_of_experts_workspace_bytes', 'b200q_mixture_of_experts', 'b200q_capture_id')
 _FUNCTIONS = ('linear', 'quantize', 'dequantize', 'take', 'w4', 'rotary', 'append', 'read', 'attention', 'log_probs', 'quantize_tokens', 'matmul_i8', 'route_tokens',
               'experts')
 _module = None

@@ -5,7 +5,7 @@ libhidet_b200q.so.
 """
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, Optional, Set, Tuple
 
 import torch
 
@@ -37,32 +37,35 @@ class _Workspaces:
     part that must be zero (its tile counters) zero between calls, so a buffer is cleared only when it
     is created.
 
-    A buffer that is made while a graph is captured is cleared by a node of that graph, so it is nobody else's: not
-    another graph's, which may be replayed first, nor that of calls outside.  One that is replaced by a larger one is kept,
-    since a graph may have been captured with it; sizes double, so that all of them are no more than the last."""
+    A graph has scratch of its own: what its capture makes is cleared by a node of the graph and is nobody else's, neither another graph's, which
+    may be replayed first or at the same time, nor that of calls outside, which have theirs again when the capture is over.  So no graph holds what calls
+    outside outgrow.  CudaGraph instead captures with the buffer that its own warm-up made and takes that away (swap, exclusive)."""
 
     def __init__(self):
+        # A buffer that a capture made stands in front of the one of calls outside, which it keeps as `outside`.
         self._buffers: Dict[Tuple[int, int], torch.Tensor] = {}
-        self._replaced: List[torch.Tensor] = []
+        self._exclusive: Set[Tuple[int, int]] = set()
 
     def get(self, device: torch.device, nbytes: int) -> Tuple[int, int]:
         if nbytes == 0:
             return 0, 0
         index = device.index if device.index is not None else torch.cuda.current_device()
         key = (index, current_stream_ptr(device))
-        buf, capture = self._buffers.get(key), self._capture(key[1])
-        made_by = self._made_by(buf)
-        if buf is None or buf.numel() < nbytes or made_by not in (0, capture):
+        last, capture = self._buffers.get(key), self._capture(key[1])
+        outside = self.outside(last)
+        if capture and self._made_by(last) == capture:
+            buf = last
+        else:
+            buf = outside if not capture or key in self._exclusive else None
+        if buf is None or buf.numel() < nbytes:
             size = 1 << max(20, (nbytes - 1).bit_length())
-            if buf is not None and made_by == 0:
-                self._replaced.append(buf)
             if capture:
                 buf = self._allocate(torch.empty, index, size)
                 buf[:ffi.WORKSPACE_HEAD].zero_()  # with every replay
-                buf.made_by = capture
+                buf.made_by, buf.outside = capture, outside
             else:
                 buf = self._allocate(torch.zeros, index, size)
-            self._buffers[key] = buf
+        self._buffers[key] = buf
         self._tell(key)  # the native host path, which may be younger than the buffer
         return buf.data_ptr(), buf.numel()
 
@@ -80,28 +83,32 @@ class _Workspaces:
         """The capture that made a buffer, or 0.  It stands with the buffer, which may leave its place and come back (swap)."""
         return getattr(buffer, 'made_by', 0)
 
+    def outside(self, buffer: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        """What calls outside captures have of a stream's scratch: the buffer, or the one behind it."""
+        return buffer.outside if self._made_by(buffer) else buffer
+
     def _tell(self, key: Tuple[int, int]) -> None:
-        buf = self._buffers.get(key)
-        if buf is None or self._made_by(buf):
-            native.set_scratch(*key, 0, 0)  # the native host path does not know of captures
-        else:
-            native.set_scratch(*key, buf.data_ptr(), buf.numel())
+        """The native host path takes what calls outside have; it leaves a capture's calls to this one."""
+        buf = self.outside(self._buffers.get(key))
+        native.set_scratch(*key, *((buf.data_ptr(), buf.numel()) if buf is not None else (0, 0)))
 
     def clear(self) -> None:
         self._buffers.clear()
-        self._replaced.clear()
         native.clear_scratch()
 
-    def swap(self, device: torch.device, stream: int, buffer: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    def swap(self, device: torch.device, stream: int, buffer: Optional[torch.Tensor], exclusive: bool = False) -> Optional[torch.Tensor]:
         """Puts `buffer` (None: nothing, a new one is made when it is needed) in the place of a stream's scratch and
         returns what was there.  A captured graph takes the buffer its launches were recorded with into its own keeping
         this way: streams come from a small pool, so a later graph or eager call may run on the same one, and must neither
-        share the buffer nor replace it by a larger one while the graph still writes to it."""
+        share the buffer nor replace it by a larger one while the graph still writes to it.  exclusive: until the next swap a capture
+        may use what calls outside made, since its owner takes it away."""
         index = device.index if device.index is not None else torch.cuda.current_device()
-        before = self._buffers.pop((index, stream), None)
+        key = (index, stream)
+        before = self._buffers.pop(key, None)
+        (self._exclusive.add if exclusive else self._exclusive.discard)(key)
         if buffer is not None:
-            self._buffers[(index, stream)] = buffer
-        self._tell((index, stream))
+            self._buffers[key] = buffer
+        self._tell(key)
         return before
 
 

@@ -50,3 +50,33 @@ def test_plain_captures_around_a_cuda_graph_on_the_same_stream():
     finally:
         torch.cuda.synchronize()
         workspaces.swap(torch.device('cuda', torch.cuda.current_device()), stream.cuda_stream, before)
+
+
+def test_plain_captures_on_a_stream_that_is_warm_are_replayed_at_the_same_time():
+    """Each has scratch of its own, also where calls outside have left some on the stream."""
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+    calls = [operands(40, 1024, 768, 1), operands(33, 1024, 512, 2)]
+    want = [call() for call in calls]
+    graphs, results = [], []
+    stream.wait_stream(torch.cuda.current_stream())
+    for call in calls:
+        with torch.cuda.stream(stream):
+            call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            results.append(call())
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for i in range(40):
+        for s, graph, result in zip((stream, other), graphs, results):
+            with torch.cuda.stream(s):
+                graph.replay()
+                if i % 4 == 0:
+                    calls[0]()     # and calls outside beside them
+        if i % 8 == 7:
+            torch.cuda.synchronize()
+            for result, w in zip(results, want):
+                assert torch.equal(result, w)
+                result.zero_()
+            torch.cuda.synchronize()
+    assert ffi.func('b200q_check_status')() == ffi.OK
