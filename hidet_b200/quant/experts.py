@@ -68,7 +68,9 @@ def mixture_of_experts(x: torch.Tensor, experts: torch.Tensor, weights: torch.Te
     x [..., hidden] float16 or bfloat16; experts int32 and weights float32 [..., k] (route_tokens, or any other choice: an expert may come twice).
     gate_up int8 [count, 2 inner, hidden], rows 2 f and 2 f + 1 the gate and the up projection's f-th; down int8 [count, hidden, inner]; scales [count, 2 inner] and [count, hidden] of one type (float16,
     bfloat16 or float32).  Negative experts are passed over (padding: a token of nothing but these is its residual, or zeros); one beyond the layer's is passed over and reported by b200q_check_status.
-    Sums are float32, the result is rounded once and is the same on every run.  out: a contiguous tensor for the result, which may be the residual, or x.
+    Rows of x and h are multiplied as whole numbers against their largest element, an element held to 2^-22 of it (float32 elsewhere, and where sizes or bases are no multiples of 16 bytes'
+    worth or there are more than 512 experts); the sums of these products are exact, what follows is float32, the result is rounded once and is the same on every run.  That shows only in an output
+    that takes next to nothing from an element over 2^10 (f16; 2^12 bf16) times the others'.  out: a contiguous tensor for the result, which may be the residual, or x.
 
     A few tokens are a stream of the weights of the experts that have one; many (more than 64, or dozens an expert) are matrix products over the tokens sorted by expert, with up to half a gigabyte of
     scratch.  Not differentiable."""
