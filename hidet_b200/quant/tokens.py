@@ -32,7 +32,7 @@ def quantize_tokens(x: torch.Tensor, norm: Optional[torch.Tensor] = None, eps: f
 
     A token's code is rint(y * (127 / amax)), its scale amax / 127, amax the largest magnitude of its y: x itself or, with norm [width] (of x's type),
     the RMS norm x / sqrt(mean(x^2) + eps) * norm, which is not rounded in between.  Tokens of zeros (below 2^-100) have a scale of zero; a token with a NaN or an infinity
-    has a scale of NaN, and so whatever is computed from it is NaN.
+    (or whose squares are beyond float32 in front of a norm) has a scale of NaN, and so whatever is computed from it is NaN.
 
     What it returns for rows [N, K] may also be a weight, at once: symmetric_quant_matmul_i8(*quantize_tokens(x), *quantize_tokens(w), weight_layout='NK')."""
     pair = native.quantize_tokens(x, norm, eps)
