@@ -170,7 +170,9 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], uint32_t a0, u
 }
 
 // Tokens and router of one 16-bit type, in whole vectors.  A warp has 16 experts and a share of their rows; a lane's eight neighbouring k of a row, which one load brings, are the same eight of its
-// token's, so two instructions take 32 k of 16 experts and eight tokens from three loads, eight steps of which are under way.
+// token's, so two instructions take 32 k of 16 experts and eight tokens from three loads, eight steps of which are under way.  The instructions cut their sums where float would round them, always
+// towards zero: eight of them in a row, and
+// their sums are added as floats (with all of a warp's in a row weights of 1024 tokens, 256 experts of 7168, were 2.0e-6 off, root mean square, 2.5e-7 now).
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 1) route_mma_kernel(const RouteArgs p) {
     __shared__ float logits[TOKENS_AT_ONCE][MOST_EXPERTS];  // of the cluster's first CTA
@@ -202,11 +204,14 @@ __global__ void __launch_bounds__(THREADS, 1) route_mma_kernel(const RouteArgs p
                         b[i] = *reinterpret_cast<const uint4 *>(x + k);
                     }
                 }
+                float s[2][4] = {};
 #pragma unroll
                 for (int i = 0; i < STEPS; ++i) {
-                    mma<T>(d, a0[i].x, a1[i].x, a0[i].y, a1[i].y, b[i].x, b[i].y);
-                    mma<T>(d, a0[i].z, a1[i].z, a0[i].w, a1[i].w, b[i].z, b[i].w);
+                    mma<T>(s[0], a0[i].x, a1[i].x, a0[i].y, a1[i].y, b[i].x, b[i].y);
+                    mma<T>(s[1], a0[i].z, a1[i].z, a0[i].w, a1[i].w, b[i].z, b[i].w);
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[i] += s[0][i] + s[1][i];
             }
         }
         // d: experts g and g + 8, tokens 2 t and 2 t + 1
