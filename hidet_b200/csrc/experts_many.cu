@@ -15,9 +15,9 @@
 // are neighbours in a round of all pairs, so that a tile of its weight comes from memory once (a contiguous part of the tiles for every pair instead: down of 512 tokens 230 us for 142).
 // Bounded waits and their ends are as there.
 //
-// What bounds it, two of eight experts of 4096 x 14336: with 64 tokens (248 us) the weights' way from memory, 215 us; with 512 (570 us: 270 + 145 us by themselves, the rest small kernels and
-// the clock under the power cap) and 2048 (2.0 ms, 2.1 POP/s) an SM's copies, some 40 bytes a clock of which 16 KB a stage are weights, whatever the entry's columns.  A copy of the
-// image is one box: in boxes of 16 rows 512 tokens took 733 us for 863.  Rows' largest magnitudes are stored by warp and not gathered with atomics: gate and up 332 us with them, 274 without.
+// What bounds it, two of eight experts of 4096 x 14336: with 64 tokens (235 to 247 us) the weights' way from memory, 215 us; with 512 (487 to 530 us: 270 + 145 us by themselves, the rest small kernels and
+// the clock under the power cap) and 2048 (1.93 to 2.1 ms, up to 2.2 POP/s) an SM's copies, some 40 bytes a clock of which 16 KB a stage are weights, whatever the entry's columns.  A copy of the
+// image is one box: in boxes of 16 rows 512 tokens took 733 us, 576 in one then.  Rows' largest magnitudes are stored by warp and not gathered with atomics: gate and up 332 us with them, 274 without.
 // With few k (1000 tokens, four of 32 of 1024 x 512: 72 us, 50 of them the products) results take the time: four groups of warps make them, two take 88 us.
 #include <type_traits>
 

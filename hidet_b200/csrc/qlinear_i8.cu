@@ -7,7 +7,7 @@ namespace b200q {
 namespace {
 
 // A tile of 64 x 64 by 256 threads, four rows and four columns each, four products an instruction; operands pass through shared memory byte by byte, which is
-// what takes the time.  For rows that are not multiples of 16 bytes and bases that are not aligned.
+// what takes the time (333 x 4096 x 4096 334 us, 13 where the weight is aligned; one token 128, 5.6).  For rows that are not multiples of 16 bytes and bases that are not aligned.
 constexpr int TILE = 64, STEP = 64, PITCH = STEP / 4 + 1;
 
 __global__ void __launch_bounds__(256) i8_any_kernel(const I8Args p) {

@@ -7,7 +7,8 @@
 // 16-bit type are multiplied by tensor instructions, whose products are exact and whose sums are float; others by float ones.  All logits meet in the first CTA's shared
 // memory, where a warp a token puts them in order, every lane with its experts' keys in registers.  A decode step's router is some KB to MB in L2: what takes the time is
 // latency (launch, a row, the cluster's barrier, the choices one after the other), so loads are asked for eight at a time.  One token, 8 experts, rows of 4096:
-// 3.3 us; 7 tokens, 64 of 2048: 3.5; 48 tokens, 128 of 2048: 4.0 (float instructions: 2.9, 6.0 and 10.4); 512 tokens, 64 of 2048: 8.0.
+// 3.3 us; 7 tokens, 64 of 2048: 3.4; 48 tokens, 128 of 2048: 4.0; 64 tokens, 256 of 7168: 12.5; 512 tokens, 64 of 2048: 7.1.  With a float router, or float tokens, on float instructions: 2.7, 5.9, 10.3,
+// 61 and 20 to 22.  With more tokens than a cluster has the router is read again by every cluster, which is what the last two are.
 #include "serving.cuh"
 
 namespace b200q {
