@@ -19,6 +19,7 @@
 // the clock under the power cap) and 2048 (1.93 to 2.1 ms, up to 2.2 POP/s) an SM's copies, some 40 bytes a clock of which 16 KB a stage are weights, whatever the entry's columns.  A copy of the
 // image is one box: in boxes of 16 rows 512 tokens took 733 us, 576 in one then.  Rows' largest magnitudes are stored by warp and not gathered with atomics: gate and up 332 us with them, 274 without.
 // With few k (1000 tokens, four of 32 of 1024 x 512: 72 us, 50 of them the products) results take the time: four groups of warps make them, two take 88 us.
+#include <cstddef>
 #include <type_traits>
 
 #include "experts.h"
@@ -62,11 +63,12 @@ struct Slot {
     int assignment;       // or -1
     int row, stride;      // its digit g is row + g * stride of the image
 };
-struct Plan {
+struct alignas(16) Plan {
     int groups, entries, slots, largest;  // largest: slots of an entry
     Group group[MOST_EXPERTS];
     Entry entry[MOST_ENTRIES];
 };
+static_assert(sizeof(Group) == 8 && sizeof(Entry) == 8 && offsetof(Plan, group) == 16 && offsetof(Plan, entry) % 8 == 0, "read as vectors");
 constexpr int LISTS_BYTES = (int)(sizeof(Group) * MOST_EXPERTS + sizeof(Entry) * MOST_ENTRIES);
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + (LISTS_BYTES + 15) / 16 * 16 + 1024;
 static_assert(SMEM_BYTES <= 226 * 1024, "beside what is declared in the kernel");
@@ -287,11 +289,13 @@ __global__ void __launch_bounds__(THREADS, 1) experts_product_kernel(const __gri
         umma::alloc_pair(smem_u32(&tmem_base_slot), TMEM_COLS);
         umma::relinquish_pair();
     }
-    // The plan is complete: the kernel in front waited for it, or for one that did, before it let this one start.
-    const int groups = p.plan->groups, entries = p.plan->entries;
-    const Rounds mine(tiles * entries, k_blocks, (int)gridDim.x / 2, pair, p.plan->largest);
-    for (int i = threadIdx.x; i < groups; i += THREADS) group[i] = p.plan->group[i];
-    for (int i = threadIdx.x; i < entries; i += THREADS) entry[i] = p.plan->entry[i];
+    // The plan is complete: the kernel in front waited for it, or for one that did, before it let this one start.  It comes from L2: ahead of its own wait this kernel has no promise that the SM's
+    // first-level cache does not hold the plan of an earlier layer, which stood in the same place.
+    const int4 sizes = __ldcg(reinterpret_cast<const int4 *>(p.plan));  // groups, entries, slots, largest
+    const int groups = sizes.x, entries = sizes.y;
+    const Rounds mine(tiles * entries, k_blocks, (int)gridDim.x / 2, pair, sizes.w);
+    for (int i = threadIdx.x; i < groups; i += THREADS) *reinterpret_cast<uint2 *>(&group[i]) = __ldcg(reinterpret_cast<const uint2 *>(&p.plan->group[i]));
+    for (int i = threadIdx.x; i < entries; i += THREADS) *reinterpret_cast<uint2 *>(&entry[i]) = __ldcg(reinterpret_cast<const uint2 *>(&p.plan->entry[i]));
     umma::fence_before_sync();
     __syncthreads();
     cluster_arrive_release();
